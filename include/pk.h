@@ -312,6 +312,150 @@ int pk_get_dump(pk_engine *eng, const char *name, float *out, int cap, int *n_ou
 void pk_request_stop(void);
 void pk_clear_stop(void);
 
+/* ------------------------------------- drafted decoding over a quantised cache
+ * No reference counterpart: the reference's cache is f32 and its decode step
+ * takes one token.  Device pointers and a stream, as the op level above; every
+ * call may be captured into a graph and none allocates or waits.  Element
+ * types are PK_TYPE_F32, PK_TYPE_F16 and PK_TYPE_BF16.  All calls run on the
+ * current device, which must be the one that holds the memory and the stream.
+ *
+ * A paged cache of one layer.  A row is one (position, kv head) of K or V:
+ *   PK_KV_Q8  code byte = c + 128, c = round(x / D) to even, |c| <= 127,
+ *             D = amax / 127; the row stands for D * c
+ *   PK_KV_Q4  nibble j (low first) = c + 8, c = round(x / (D * s_b)) to even,
+ *             -8 <= c <= 7, D = amax / 105, s_b = ceil(amax_b / (7 * D)) in
+ *             1..15 for dimensions 32 b .. 32 b + 31, nibble b of the word
+ *             behind D; the row stands for D * (c * s_b)
+ * (f32 arithmetic, every operation rounded once; c * s_b is exact; the
+ * quotient is not rounded before the rounding to c.)  NaN is stored as 0 and
+ * magnitudes above 2^127, infinities among them, as 2^127.
+ *   k, v    codes [n_pages][n_kv][page_size][head_dim | head_dim / 2 bytes],
+ *           16-byte aligned
+ *   ks, vs  scales [n_pages][n_kv][page_size][1 | 2 words], 16-byte aligned
+ * page_size is a power of two, 16 .. 65536; head_dim is 64 or 128. */
+#define PK_KV_Q8 2
+#define PK_KV_Q4 3
+typedef struct {
+  void *k, *v;
+  float *ks, *vs;
+  int type, n_pages, page_size, n_kv, head_dim;
+} pk_kv_cache;
+
+/* The sequences of a call (device arrays).  Sequence s has ctx[s] committed
+ * positions and the new tokens start[s] .. start[s + 1] - 1 of the call's
+ * token arrays, token i of them at position ctx[s] + i.  pages[s][j] is the
+ * page of its positions j * page_size ..; an entry outside 0 .. n_pages - 1
+ * is no page: what would be written there is dropped, what would be read is
+ * masked (attention) or zero (pk_kv_load).  start ascends within 0 .. n_tok,
+ * the token arrays' rows; rows that no sequence has are neither read nor
+ * written.  max_new and max_len are bounds the host knows: of the new tokens
+ * of one sequence, and of its committed positions and new tokens together;
+ * what is beyond them is left out.  A page that a call writes belongs to one
+ * sequence of it. */
+typedef struct {
+  const int *start, *ctx, *pages;
+  int n_seq, max_pages, n_tok, max_new, max_len;
+} pk_kv_seqs;
+
+/* K and V rows of the new tokens, [n_tok][n_kv][head_dim] with strides in
+ * elements (head_dim contiguous), quantised into the cache; and positions
+ * ctx[s] .. read back from it into rows start[s] .. of k and v. */
+int pk_kv_store(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const void *k, const void *v, int type,
+                int64_t tok_stride, int64_t head_stride, void *stream);
+int pk_kv_load(const pk_kv_cache *cache, const pk_kv_seqs *seqs, void *k, void *v, int type, int64_t tok_stride,
+               int64_t head_stride, void *stream);
+/* Accepts drafts: position ctx[s] + j becomes what position ctx[s] + keep[s][j]
+ * holds, for j < n_keep[s] (device arrays, keep [n_seq][keep_stride]).  The path
+ * of a tree numbered parents first has keep[s][j] >= j; entries below that, or
+ * not below the sequence's new tokens, are skipped. */
+int pk_kv_keep(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const int *keep, int keep_stride, const int *n_keep,
+               void *stream);
+
+/* Attention of the new tokens over the cache, which already holds their K and
+ * V (pk_kv_store).  Query head h reads kv head h / (n_head / n_kv).  Token i of
+ * a sequence sees every committed position, and of the new ones those j whose
+ * bit j & 63 of word j >> 6 of its mask is set (a drafted tree: its ancestors
+ * and itself), or j <= i where mask is null.  New tokens past 64 * mask_words
+ * are seen by none.  A row that sees nothing gets 0.
+ *   q, out  [n_tok][n_head][head_dim] of one type, strides in elements
+ *   mask    device, [n_tok][mask_words], or null
+ * Scores and sums are f32; a softmax weight times its V scale is rounded to
+ * f16 as a fraction of the row's largest (to two f16 terms for f32 queries).
+ * scratch: pk_kv_attn_scratch_bytes bytes of device memory, 16-byte aligned
+ * (may be null when that is 0), which calls that overlap in time, replays of
+ * captured graphs among them, must not share. */
+typedef struct {
+  const void *q;
+  void *out;
+  const uint64_t *mask;
+  int64_t q_tok_stride, q_head_stride, out_tok_stride, out_head_stride;
+  int type, n_head, mask_words;
+  float scale;  /* of q . k, > 0; usually 1 / sqrt(head_dim) */
+} pk_kv_query;
+size_t pk_kv_attn_scratch_bytes(const pk_kv_cache *cache, const pk_kv_seqs *seqs, int n_head, int type);
+int pk_kv_attn(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const pk_kv_query *query, void *scratch,
+               size_t scratch_bytes, void *stream);
+
+/* Rotary positions.  pk_rope_turns (host code) writes the n_rot / 2 pairs'
+ * turns a position, theta^(-2 i / n_rot) / (2 pi) in double, and the gain of
+ * the rotated values; the caller keeps the table in device memory.  Scaling
+ * for contexts longer than the trained one:
+ *   PK_ROPE_LINEAR  every turn divided by factor
+ *   PK_ROPE_NTK     theta * factor^(n_rot / (n_rot - 2)): the slowest pair is
+ *                   divided by factor, the fastest not at all
+ *   PK_ROPE_YARN    pairs that turn at most `low` times in n_ctx_train
+ *                   positions divided by factor, those that turn at least
+ *                   `high` times kept, linear in between; gain
+ *                   0.1 ln(factor) + 1 (or the one given)
+ * factors (host, n_rot / 2 values or null) divides each pair's turns first. */
+#define PK_ROPE_NONE 0
+#define PK_ROPE_LINEAR 1
+#define PK_ROPE_NTK 2
+#define PK_ROPE_YARN 3
+typedef struct {
+  int n_rot, scaling;
+  double theta, factor, n_ctx_train, low, high, gain; /* gain 0: the scaling's own */
+  const float *factors;
+} pk_rope_spec;
+int pk_rope_turns(const pk_rope_spec *spec, double *turns, float *gain);
+/* Rotates the first n_rot dimensions of every head by pos[t] times the turns:
+ * pairs (2 i, 2 i + 1) for PK_ROPE_INTERLEAVED, (i, i + n_rot / 2) for
+ * PK_ROPE_HALF; the other dimensions are copied.  q or k may be null (no heads
+ * of it); an output may be its own input.  Angles are reduced in double. */
+#define PK_ROPE_INTERLEAVED 0
+#define PK_ROPE_HALF 1
+typedef struct {
+  const void *q, *k;
+  void *q_out, *k_out;
+  const int *pos;       /* device, [n_tok] */
+  const double *turns;  /* device, [n_rot / 2] */
+  int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride; /* of the inputs, in elements */
+  int64_t qo_tok_stride, qo_head_stride, ko_tok_stride, ko_head_stride;
+  int type, layout, n_tok, n_head, n_kv, head_dim, n_rot;
+  float gain;
+} pk_rope_args;
+int pk_rope(const pk_rope_args *args, void *stream);
+
+/* Rules applied to logits [rows][n] before a token is drawn (pk_sample,
+ * argmax); out may be the logits.  For token t seen c times among the row's
+ * first n_hist ids:  x = x > 0 ? x / repeat : x * repeat, then
+ * x - (c * freq + presence), where c > 0;  then + the sum of the row's biases
+ * of t, added in the list's order;  then -inf where bit t & 31 of word t >> 5
+ * of allow is 0.  Device arrays; a null one is a rule not used; a stride of 0
+ * gives every row the same list.  Ids outside 0 .. n - 1 are ignored. */
+typedef struct {
+  const float *repeat, *freq, *presence; /* [rows] */
+  const uint32_t *hist;                  /* [rows][hist_stride] */
+  const int *n_hist;                     /* [rows], or null: n_hist_max ids in every row */
+  const uint32_t *bias_id;               /* [rows][bias_stride], n_bias of them */
+  const float *bias;
+  const uint32_t *allow;                 /* [rows][allow_stride] */
+  int64_t hist_stride, bias_stride, allow_stride;
+  int n_hist_max, n_bias;
+} pk_logit_rules;
+int pk_apply_logit_rules(const void *logits, void *out, int type, int rows, int n, int64_t in_stride,
+                         int64_t out_stride, const pk_logit_rules *rules, void *stream);
+
 /* ------------------------------------------------- tensor-parallel decode
  * No reference counterpart: the reference runs one engine per process on the
  * CPU.  This splits a llama stack over T GPUs, one process per GPU (the

@@ -18,6 +18,9 @@ import ctypes as C
 import os
 import subprocess
 
+from . import drafts
+from .drafts import KvCache, KvSeqs, RopeTable, logit_rules, rope
+
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG_DIR = os.path.dirname(HERE)
 LIB_PATH = os.path.join(PKG_DIR, "lib", "libpocketinfer_b200.so")
@@ -46,6 +49,7 @@ SYMBOLS = [
     "pk_streams_begin", "pk_stream_prefill", "pk_streams_decode", "pk_streams_set_position",
     "pk_tokenizer_load", "pk_tokenizer_free", "pk_tokenizer_info_get", "pk_tokenize", "pk_token_bytes",
     "pk_token_is_eog", "pk_utf8_flush", "pk_text_find", "pk_chat_apply", "pk_chat_prompt", "pk_chat_is_minicpm5", "pk_chat_direct_suffix", "pk_chat_thinking_suffix",
+    "pk_kv_store", "pk_kv_load", "pk_kv_keep", "pk_kv_attn_scratch_bytes", "pk_kv_attn", "pk_rope_turns", "pk_rope", "pk_apply_logit_rules",
 ]
 
 
@@ -152,6 +156,7 @@ def lib():
         "pk_chat_prompt": ([P, P, I, I, I, SZ, P, SZ, C.POINTER(SZ), C.POINTER(I), C.POINTER(I)], I),
         "pk_chat_direct_suffix": ([], C.c_char_p), "pk_chat_thinking_suffix": ([], C.c_char_p),
     }
+    sig.update(drafts.SIGNATURES)
     for name, (args, res) in sig.items():
         fn = getattr(L, name)
         fn.argtypes = args

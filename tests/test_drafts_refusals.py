@@ -1,0 +1,150 @@
+"""The drafted-decoding entry points refuse bad arguments before they touch the device (no GPU needed)."""
+import ctypes as C
+import math
+
+import pytest
+
+from pocketinfer import drafts as D
+
+INVALID, UNSUPPORTED = 1, 2
+A = 1 << 20  # an aligned address that is never followed: every call here returns before a launch
+
+
+def cache(**kw):
+    c = D.KvCacheC(A, A, A, A, D.KV_Q8, 4, 64, 2, 128)
+    for k, v in kw.items():
+        setattr(c, k, v)
+    return c
+
+
+def seqs(**kw):
+    s = D.KvSeqsC(A, A, A, 2, 4, 8, 4, 200)
+    for k, v in kw.items():
+        setattr(s, k, v)
+    return s
+
+
+def query(**kw):
+    q = D.KvQueryC(A, A, None, 512, 128, 512, 128, 0, 4, 0, 0.1)
+    for k, v in kw.items():
+        setattr(q, k, v)
+    return q
+
+
+BAD_CACHE = [({"type": 1}, UNSUPPORTED), ({"type": 9}, UNSUPPORTED), ({"head_dim": 96}, UNSUPPORTED), ({"head_dim": 0}, UNSUPPORTED),
+             ({"n_pages": 0}, INVALID), ({"n_kv": 0}, INVALID), ({"page_size": 8}, INVALID), ({"page_size": 48}, INVALID),
+             ({"page_size": 131072}, INVALID), ({"k": None}, INVALID), ({"vs": None}, INVALID), ({"v": A + 8}, INVALID), ({"ks": A + 4}, INVALID)]
+BAD_SEQS = [{"n_seq": -1}, {"n_tok": -1}, {"max_new": -3}, {"max_len": -1}, {"max_pages": 0}, {"start": None}, {"ctx": None},
+            {"pages": None}, {"ctx": A + 2}, {"max_len": (1 << 30) + 1}]
+
+
+@pytest.mark.parametrize("what", ["store", "load", "keep", "attn"])
+def test_bad_cache_and_sequences(pk, what):
+    lib = pk.lib()
+
+    def call(c, s):
+        c, s = C.byref(c), C.byref(s)
+        if what == "keep":
+            return lib.pk_kv_keep(c, s, A, 4, A, None)
+        if what == "attn":
+            return lib.pk_kv_attn(c, s, C.byref(query()), A, 1 << 30, None)
+        return getattr(lib, "pk_kv_" + what)(c, s, A, A, 0, 512, 128, None)
+
+    for kw, code in BAD_CACHE:
+        assert call(cache(**kw), seqs()) == code, kw
+        assert pk.last_error()
+    for kw in BAD_SEQS:
+        assert call(cache(), seqs(**kw)) == INVALID, kw
+    for kw in ({"n_seq": 0}, {"n_tok": 0}, {"max_new": 0}, {"max_len": 0}):  # nothing to do
+        assert call(cache(), seqs(**kw, start=None, ctx=None, pages=None)) == 0, kw
+
+
+def test_rows_and_keep(pk):
+    lib, c, s = pk.lib(), cache(), seqs()
+    for fn in (lib.pk_kv_store, lib.pk_kv_load):
+        for args, code in (((None, A, 0, 512, 128), INVALID), ((A, None, 0, 512, 128), INVALID), ((A + 2, A, 0, 512, 128), INVALID),
+                           ((A, A + 1, 1, 512, 128), INVALID), ((A, A, 12, 512, 128), UNSUPPORTED), ((A, A, 0, 512, 127), INVALID),
+                           ((A, A, 0, -1, 128), INVALID), ((A, A, 0, 1 << 41, 128), INVALID)):
+            assert fn(C.byref(c), C.byref(s), *args, None) == code, args
+    assert lib.pk_kv_load(C.byref(c), C.byref(s), A, A, 0, 64, 128, None) == INVALID  # rows would overlap
+    for args in ((None, 4, A), (A, 4, None), (A + 1, 4, A), (A, -1, A)):
+        assert lib.pk_kv_keep(C.byref(c), C.byref(s), *args, None) == INVALID, args
+    assert lib.pk_kv_keep(C.byref(c), C.byref(s), A, 0, A, None) == 0
+
+
+def test_attention(pk):
+    lib, c, s = pk.lib(), cache(), seqs()
+    need = lib.pk_kv_attn_scratch_bytes(C.byref(c), C.byref(seqs(max_len=100000, max_pages=4096)), 4, 0)
+    assert need > 0 and need % 4 == 0
+    assert lib.pk_kv_attn_scratch_bytes(C.byref(c), C.byref(s), 3, 0) == 0
+    for kw, code in (({"type": 12}, UNSUPPORTED), ({"n_head": 0}, INVALID), ({"n_head": 3}, INVALID), ({"scale": 0.0}, INVALID),
+                     ({"scale": -1.0}, INVALID), ({"scale": math.inf}, INVALID), ({"scale": math.nan}, INVALID), ({"q": None}, INVALID),
+                     ({"out": None}, INVALID), ({"q": A + 2}, INVALID), ({"mask": A, "mask_words": 0}, INVALID),
+                     ({"mask": A + 4, "mask_words": 1}, INVALID), ({"mask": A, "mask_words": 5000}, INVALID),
+                     ({"q_tok_stride": -1}, INVALID), ({"out_head_stride": 64}, INVALID), ({"out_tok_stride": 100}, INVALID)):
+        assert lib.pk_kv_attn(C.byref(c), C.byref(s), C.byref(query(**kw)), A, 1 << 30, None) == code, kw
+    big = seqs(max_len=100000, max_pages=4096)
+    for scratch, size in ((None, need), (A, need - 1), (A + 8, need), (A, 0)):
+        assert lib.pk_kv_attn(C.byref(c), C.byref(big), C.byref(query()), scratch, size, None) == INVALID
+    assert str(need) in pk.last_error()
+
+
+def test_rope(pk):
+    lib = pk.lib()
+    out, g = (C.c_double * 64)(), C.c_float()
+
+    def spec(**kw):
+        p = D.RopeSpecC(128, 0, 10000.0, 1.0, 4096.0, 1.0, 32.0, 0.0, None)
+        for k, v in kw.items():
+            setattr(p, k, v)
+        return C.byref(p)
+
+    assert lib.pk_rope_turns(spec(), out, C.byref(g)) == 0 and g.value == 1.0 and abs(out[0] * 2 * math.pi - 1) < 1e-15
+    for kw in ({"n_rot": 0}, {"n_rot": 7}, {"n_rot": 5000}, {"theta": 0.0}, {"theta": math.nan}, {"scaling": 4}, {"scaling": -1},
+               {"scaling": 1, "factor": 0.0}, {"scaling": 3, "factor": 2.0, "n_ctx_train": 0.0}, {"scaling": 3, "factor": 2.0, "low": 40.0},
+               {"gain": -1.0}, {"factors": C.cast((C.c_float * 64)(*([1.0] * 63 + [0.0])), C.c_void_p)}):
+        assert lib.pk_rope_turns(spec(**kw), out, C.byref(g)) == INVALID, kw
+    assert lib.pk_rope_turns(None, out, C.byref(g)) == INVALID
+
+    def args(**kw):
+        a = D.RopeArgsC(A, A, A, A, A, A, 512, 128, 256, 128, 512, 128, 256, 128, 0, 0, 3, 4, 2, 128, 128, 1.0)
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return C.byref(a)
+
+    for kw, code in (({"type": 8}, UNSUPPORTED), ({"layout": 2}, INVALID), ({"n_rot": 130}, INVALID), ({"n_rot": 3}, INVALID),
+                     ({"n_tok": -1}, INVALID), ({"q": None, "k": None}, INVALID), ({"pos": None}, INVALID), ({"turns": A + 4}, INVALID),
+                     ({"q_out": None}, INVALID), ({"k_out": None}, INVALID), ({"q": A + 2}, INVALID), ({"ko_head_stride": 64}, INVALID),
+                     ({"q_tok_stride": -4}, INVALID)):
+        assert lib.pk_rope(args(**kw), None) == code, kw
+    assert lib.pk_rope(args(n_tok=0), None) == 0
+    assert lib.pk_rope(args(n_head=0, k=None), None) == 0
+
+
+def test_logit_rules(pk):
+    lib = pk.lib()
+
+    def call(ptr=(A, A), ty=0, rows=2, n=100, st=(100, 100), **kw):
+        r = D.LogitRulesC()
+        for k, v in kw.items():
+            setattr(r, k, v)
+        return lib.pk_apply_logit_rules(ptr[0], ptr[1], ty, rows, n, st[0], st[1], C.byref(r), None)
+
+    assert call(ty=12) == UNSUPPORTED
+    for kw in ({"ptr": (None, A)}, {"ptr": (A, None)}, {"ptr": (A + 1, A)}, {"rows": -1}, {"n": -1}, {"st": (-1, 100)}, {"st": (100, 99)},
+               {"st": (200, 100)}, {"hist": A, "n_hist_max": -1}, {"bias_id": A, "n_bias": 3}, {"bias": A}, {"hist": A, "hist_stride": -1},
+               {"allow": A + 2}, {"n_bias": -1}):
+        assert call(**kw) == INVALID, kw
+    assert lib.pk_apply_logit_rules(A, A, 0, 2, 100, 100, 100, None, None) == INVALID
+    assert call(rows=0) == 0 and call(n=0) == 0
+
+
+def test_binding_refuses_host_tensors(pk):
+    torch = pytest.importorskip("torch")
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    for bad in (lambda: pk.KvSeqs(i(3), i(2), i(2, 4), 8, 4, 100), lambda: pk.KvSeqs(i(3).long(), i(2), i(2, 4), 8, 4, 100),
+                lambda: pk.KvCache.empty(4, 16, 2, 128, "q6", device="cpu"), lambda: pk.KvCache.empty(4, 16, 2, 128, "q8", device="cpu"),
+                lambda: pk.logit_rules(torch.zeros(2, 8)), lambda: pk.RopeTable(127, device="cpu"),
+                lambda: pk.rope(pk.RopeTable(64, device="cpu"), i(2), torch.zeros(2, 1, 64), layout="quarter")):
+        with pytest.raises(pk.PkError):
+            bad()
