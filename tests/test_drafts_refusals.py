@@ -148,3 +148,35 @@ def test_binding_refuses_host_tensors(pk):
                 lambda: pk.rope(pk.RopeTable(64, device="cpu"), i(2), torch.zeros(2, 1, 64), layout="quarter")):
         with pytest.raises(pk.PkError):
             bad()
+
+
+def test_packed_structures_match_the_header():
+    """The packed bytes have the fields where the ctypes structures (the C layouts) have them."""
+    q = D.PACK_QUERY(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 0.5)
+    r = D.PACK_ROPE(*range(1, 22), 0.5)
+    u = D.PACK_RULES(*range(1, 14))
+    for cls, data, last in ((D.KvQueryC, q, 0.5), (D.RopeArgsC, r, 0.5), (D.LogitRulesC, u, 13)):
+        s = cls.from_buffer_copy(data + bytes(C.sizeof(cls) - len(data)))
+        got = [getattr(s, n) for n, _ in cls._fields_]
+        assert got == list(range(1, len(got))) + [last], cls
+
+
+def test_binding_structures_match_the_compiler(tmp_path):
+    """sizeof and offsetof of the header's structures, as a C compiler has them."""
+    import os
+    import subprocess
+
+    from conftest import ROOT
+
+    names = {"pk_kv_cache": D.KvCacheC, "pk_kv_seqs": D.KvSeqsC, "pk_kv_query": D.KvQueryC, "pk_rope_spec": D.RopeSpecC,
+             "pk_rope_args": D.RopeArgsC, "pk_logit_rules": D.LogitRulesC}
+    lines = [f'printf("{n} %zu", sizeof({n}));' + "".join(f'printf(" %zu", offsetof({n}, {f}));' for f, _ in c._fields_) + 'puts("");'
+             for n, c in names.items()]
+    src = tmp_path / "layout.c"
+    src.write_text('#include <stdio.h>\n#include "pk.h"\nint main(void) {\n' + "\n".join(lines) + "\nreturn 0;\n}\n")
+    exe = str(tmp_path / "layout")
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", exe], check=True)
+    for line in subprocess.run([exe], capture_output=True, text=True, check=True).stdout.splitlines():
+        name, size, *offs = line.split()
+        c = names[name]
+        assert int(size) == C.sizeof(c) and [int(o) for o in offs] == [getattr(c, f).offset for f, _ in c._fields_], name
