@@ -22,12 +22,7 @@ cudaError_t launch_kv_load(const pk_kv_cache &c, const pk_kv_seqs &s, void *k, v
 cudaError_t launch_kv_keep(const pk_kv_cache &c, const pk_kv_seqs &s, const int *keep, int keep_stride,
                            const int *n_keep, cudaStream_t st);
 
-// How a call of the attention is split: chunk positions per unit of work and
-// the most units a sequence has (one: no partial results).
-struct KvSplit {
-  int chunk = 0, n_chunk = 1, variant = 0, row_tiles = 1;
-};
-KvSplit kv_attn_split(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type);
+// (0: no partial results)
 size_t kv_attn_scratch_bytes(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type);
 cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_query &q, void *scratch,
                            cudaStream_t st);

@@ -16,10 +16,16 @@
 // sums of w and the outputs are f32; M follows the running maximum only when
 // that has grown by 2^6, so most tiles leave the outputs as they are.
 //
-// The contraction's order is free, so fragments are loaded straight from the
-// cache rows: of 4 lanes that share a key each takes a quarter of its row's
-// bytes as its k values, and of 8 lanes that share a position pair each takes
-// an eighth of the V rows as its output dimensions.
+// The products are formed transposed, S^T = K Q^T and O^T = V^T P^T, with keys
+// and dimensions as the instruction's 16 rows and query rows as its 8 columns:
+// a kv head's query rows (one for a plain token of an ungrouped head, 8 for a
+// group of 8) then cost matrix work in steps of 8, not 16, and each code that
+// was made f16 serves every column.  The weights, made with a key a lane row,
+// become the second product's operand by 8 x 8 register transposes.  The
+// contraction's order is free, so fragments are loaded as the cache's rows
+// lie: of 4 lanes that share a key each takes a quarter of its row's bytes as
+// its k values, and of 8 lanes that share two keys each takes an eighth of
+// the V rows as its output dimensions.
 #include <math_constants.h>
 
 #include <algorithm>
@@ -32,6 +38,7 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int MIN_CHUNK = 256;
+constexpr int NSTAGE = 4;  // tiles of 16 positions in flight per key group
 // M moves when the maximum passes it by 2^GROW; a row's factor inv is set so
 // that its largest weight times scale is SET and set again past TOP (f16 ends
 // at 65504), so what rounds to a subnormal is below 2^-23 of the largest.
@@ -48,6 +55,20 @@ __device__ __forceinline__ float ex2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// The transpose of an 8 x 8 f16 matrix held two columns a lane.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// A barrier of n threads (whole warps).
+__device__ __forceinline__ void bar_n(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
 __device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 // (a, b) as two f16 and, for the second term, what the rounding left.
@@ -57,10 +78,11 @@ __device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t hi) {
   return pack2(a - f.x, b - f.y);
 }
 
-// Over the four lanes that share a row.
-__device__ __forceinline__ float quad_max(float v) {
-  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 1));
-  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
+// Over the eight lanes that share two query rows.
+__device__ __forceinline__ float key_max(float v) {
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+  v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+  return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
 }
 
 // Bytes x_i = c_i + 128 in the low and high halves of (1024 + x) f16 words:
@@ -80,18 +102,36 @@ struct AttnKArgs {
   pk_kv_query q;
   float *part_o;   // [n_tok][n_head][n_chunk][DH]
   float2 *part_ml; // [n_tok][n_head][n_chunk]
-  int chunk, n_chunk, row_tiles, group, vec_q, vec_o;
+  int chunk, n_chunk, row_tiles, group, page_shift, vec_q, vec_o;
 };
 
-// Positions of a row tile's chunk, and whether the sequence's rows come from
-// more than one chunk (then this one's go to the scratch).
+// A CTA's work: one chunk of positions [lo, hi) for one tile of the rows (token
+// i, query head of kv head h) of one sequence.  Sequences of more than one
+// chunk (nch) leave theirs in the scratch.
 struct Unit {
   SeqView sv;
   int s, h, rt, ch, lo, hi, nch, rows;
 };
+__device__ __forceinline__ Unit unit_of(const AttnKArgs &a) {
+  Unit u;
+  unsigned id = blockIdx.x;
+  u.rt = (int)(id % (unsigned)a.row_tiles);
+  id /= (unsigned)a.row_tiles;
+  u.h = (int)(id % (unsigned)a.c.n_kv);
+  id /= (unsigned)a.c.n_kv;
+  u.ch = (int)(id % (unsigned)a.n_chunk);
+  u.s = (int)(id / (unsigned)a.n_chunk);
+  u.sv = seq_view(a.s, a.c.page_size, u.s);
+  u.rows = u.sv.n * a.group;
+  u.nch = (u.sv.total + a.chunk - 1) / a.chunk;
+  u.lo = u.ch * a.chunk;
+  u.hi = min(u.sv.total, u.lo + a.chunk);
+  return u;
+}
 
 // DH / 4 query elements of a row from lane t's quarter, scaled to |q'| < 2;
-// rs is the row's r.  All lanes of the warp call it.
+// rs is the row's r.  All lanes of the warp call it; the four lanes of a quad
+// hold one row.
 template <int DH, class E>
 __device__ __forceinline__ void load_q(const AttnKArgs &a, const Unit &u, int row, int t, float (&x)[DH / 4], float &rs) {
   const bool on = row < u.rows;
@@ -116,7 +156,6 @@ __device__ __forceinline__ void load_q(const AttnKArgs &a, const Unit &u, int ro
   for (int j = 0; j < DH / 4; j++) x[j] *= down;
   rs = a.q.scale * kLog2e * up;
 }
-
 template <int DH>
 __device__ __forceinline__ void load_q_any(const AttnKArgs &a, const Unit &u, int row, int t, float (&x)[DH / 4], float &rs) {
   if (a.q.type == T_F32) load_q<DH, float>(a, u, row, t, x, rs);
@@ -140,255 +179,338 @@ __device__ __forceinline__ bool sees(const AttnKArgs &a, const Unit &u, int i, i
   return (__ldg(a.q.mask + (size_t)(u.sv.first + i) * a.q.mask_words + (j >> 6)) >> (j & 63)) & 1;
 }
 
-// One warp's state: 16 rows (lane's rows g and g + 8) over some positions.
-template <int TYPE, int DH, int NT>
-struct Warp {
-  static constexpr int KS = DH / 16, NV = DH / 8;
+// A tile in shared memory: 16 rows of K codes, 16 of V codes, their scales.
+// Rows lie in lines of 128 bytes whose 16-byte slots are exchanged by line, so
+// that both the K reads (8 rows x 4 quarters) and the V reads (every second
+// row x 8 eighths) of a warp touch every bank once.
+template <int TYPE, int DH>
+struct Tile {
   static constexpr int RB = TYPE == PK_KV_Q8 ? DH : DH / 2, SW = TYPE == PK_KV_Q8 ? 1 : 2;
-  uint32_t q[NT][KS][4];
-  float o[NV][4];
-  float rs[2], m[2], l[2], inv[2];
-
-  __device__ __forceinline__ void init(const AttnKArgs &a, const Unit &u, int row0, int lane) {
-    const int g = lane >> 2, t = lane & 3;
+  static constexpr int CODES = 16 * RB, SCALES = 16 * SW * 4;
+  static constexpr int BYTES = 2 * (CODES + SCALES);
+  static constexpr int KS = DH / 16;
+  __device__ static __forceinline__ uint32_t at(int row, int byte) {  // of a K or V block
+    constexpr int RPL = 128 / RB, CPR = RB / 16;
+    const int line = row / RPL, x = RB == 128 ? line & 7 : (line & 3) * 2;
+    return line * 128 + ((((row % RPL) * CPR + (byte >> 4)) ^ x) << 4) + (byte & 15);
+  }
+  // Copies of a key group's n threads (thread i) into the tile at dst.
+  __device__ static __forceinline__ void copy(const pk_kv_cache &c, long long row, uint32_t dst, int i, int n) {
+    const uint8_t *k = reinterpret_cast<const uint8_t *>(c.k) + row * RB, *v = reinterpret_cast<const uint8_t *>(c.v) + row * RB;
+    constexpr int CH = CODES / 16, SC = SCALES / 16;
 #pragma unroll
-    for (int r = 0; r < 2; r++) {
-      float x[DH / 4];
-      load_q_any<DH>(a, u, row0 + g + 8 * r, t, x, rs[r]);
+    for (int j = 0; j < CH; j += 32) {
+      const int x = j + i;
+      if (x < CH) {
+        const uint32_t o = at(x / (RB / 16), (x % (RB / 16)) * 16);
+        cp16(dst + o, k + 16 * x);
+        cp16(dst + CODES + o, v + 16 * x);
+      }
+      if (n > 32) break;  // (more than one warp: the loop below)
+    }
+    if (n > 32) {
+      for (int x = i + n; x < CH; x += n) {
+        const uint32_t o = at(x / (RB / 16), (x % (RB / 16)) * 16);
+        cp16(dst + o, k + 16 * x);
+        cp16(dst + CODES + o, v + 16 * x);
+      }
+    }
+    if (i < 2 * SC) {
+      const float *s = (i < SC ? c.ks : c.vs) + row * SW + (i % SC) * 4;
+      cp16(dst + 2 * CODES + 16 * i, s);
+    }
+  }
+};
+
+// One warp's state: 8 NB query rows (this lane's are 8 b + 2 t + {0, 1}) over
+// some of the positions.  QS: the query fragments stay in shared memory, where
+// registers would not hold them beside the outputs.
+template <int TYPE, int DH, int NT, int NB>
+struct Warp {
+  using T = Tile<TYPE, DH>;
+  static constexpr int KS = DH / 16, MV = DH / 16, RB = T::RB, SW = T::SW;
+  static constexpr bool QS = NT * NB * KS * 2 > 64;
+  static constexpr int QBYTES = QS ? NT * NB * KS * 32 * 8 : 0;
+  uint32_t q[QS ? 1 : NT][QS ? 1 : NB][QS ? 1 : KS][2];
+  uint32_t qs;  // shared address of this lane's fragments
+  float o[NB][MV][4];
+  float rs[NB][2], m[NB][2], l[NB][2], inv[NB][2];
+
+  // store_q: this warp writes the fragments to shared memory at qsmem (its key
+  // group's warps of the same rows write the same values).
+  __device__ __forceinline__ void init(const AttnKArgs &a, const Unit &u, int row0, int lane, uint32_t qsmem) {
+    const int g = lane >> 2, t = lane & 3;
+    qs = qsmem + lane * 8;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      float x[DH / 4], r;
+      load_q_any<DH>(a, u, row0 + 8 * b + g, t, x, r);  // lanes of quad g: row g
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        rs[b][e] = __shfl_sync(0xffffffffu, r, 4 * (2 * t + e));
+        m[b][e] = -CUDART_INF_F;
+        l[b][e] = 0.0f;
+        inv[b][e] = 0x1p100f;
+      }
 #pragma unroll
       for (int j = 0; j < KS; j++) {
+        uint32_t f[NT][2];
 #pragma unroll
         for (int e = 0; e < 2; e++) {
           const float x0 = x[dim_of<TYPE>(j, 2 * e)], x1 = x[dim_of<TYPE>(j, 2 * e + 1)];
-          q[0][j][r + 2 * e] = pack2(x0, x1);
-          if (NT == 2) q[NT - 1][j][r + 2 * e] = rest2(x0, x1, q[0][j][r + 2 * e]);
+          f[0][e] = pack2(x0, x1);
+          if (NT == 2) f[NT - 1][e] = rest2(x0, x1, f[0][e]);
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+          if (QS) {
+            asm volatile("st.shared.v2.u32 [%0], {%1,%2};" ::"r"(qs + (uint32_t)(((n * NB + b) * KS + j) * 256)), "r"(f[n][0]), "r"(f[n][1]) : "memory");
+          } else {
+            q[n][b][j][0] = f[n][0];
+            q[n][b][j][1] = f[n][1];
+          }
         }
       }
-      m[r] = -CUDART_INF_F;
-      l[r] = 0.0f;
-      inv[r] = 0x1p100f;
-    }
 #pragma unroll
-    for (int i = 0; i < NV; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  }
-
-  __device__ __forceinline__ void scale_row(int r, float f) {
-#pragma unroll
-    for (int i = 0; i < NV; i++) {
-      o[i][2 * r] *= f;
-      o[i][2 * r + 1] *= f;
+      for (int i = 0; i < MV; i++) o[b][i][0] = o[b][i][1] = o[b][i][2] = o[b][i][3] = 0.0f;
     }
   }
+  __device__ __forceinline__ uint2 frag(int n, int b, int j) const {
+    if (QS) return sld_v2(qs + (uint32_t)(((n * NB + b) * KS + j) * 256));
+    return make_uint2(q[QS ? 0 : n][QS ? 0 : b][QS ? 0 : j][0], q[QS ? 0 : n][QS ? 0 : b][QS ? 0 : j][1]);
+  }
 
-  // Sixteen positions p0 .. p0 + 15 (one page's rows from `row`, or row < 0).
-  // masked: some of them may be out of reach of some row.
-  __device__ __forceinline__ void tile(const AttnKArgs &a, const Unit &u, int row0, int p0, long long row, bool masked,
-                                       int lane) {
+  __device__ __forceinline__ void scale_row(int b, int e, float f) {
+#pragma unroll
+    for (int i = 0; i < MV; i++) {
+      o[b][i][e] *= f;
+      o[b][i][2 + e] *= f;
+    }
+  }
+
+  // Sixteen positions p0 .. p0 + 15, in shared memory at sm.  MASKED: some of
+  // them may be out of reach of some row.
+  template <bool MASKED>
+  __device__ __forceinline__ void tile(const AttnKArgs &a, const Unit &u, int row0, int p0, uint32_t sm, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    const uint8_t *kc = reinterpret_cast<const uint8_t *>(a.c.k) + (size_t)row * RB;
-    const uint8_t *vc = reinterpret_cast<const uint8_t *>(a.c.v) + (size_t)row * RB;
-    const float *ks = a.c.ks + (size_t)row * SW, *vs = a.c.vs + (size_t)row * SW;
-    float s[2][4];
+    const uint32_t ksc = sm + 2 * T::CODES, vsc = ksc + T::SCALES;
+    float s[NB][4];
+    float dk[2], dv[2];
+    {
+      uint32_t w[2][RB / 16], sd[2] = {0, 0}, md[2] = {0, 0};
 #pragma unroll
-    for (int n = 0; n < 2; n++) {
-      s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-      const uint8_t *kp = kc + (size_t)(8 * n + g) * RB + t * (RB / 4);
-      uint32_t w[RB / 16];
-      if (RB / 4 >= 16) {
+      for (int n = 0; n < 2; n++) {  // keys g and g + 8
+        const int row = 8 * n + g;
+        if (RB / 4 >= 16) {
 #pragma unroll
-        for (int i = 0; i < RB / 64; i++) *reinterpret_cast<uint4 *>(w + 4 * i) = reinterpret_cast<const uint4 *>(kp)[i];
-      } else {
-        *reinterpret_cast<uint2 *>(w) = *reinterpret_cast<const uint2 *>(kp);
+          for (int i = 0; i < RB / 64; i++) {
+            const uint4 v = sld_v4(sm + T::at(row, t * (RB / 4) + 16 * i));
+            w[n][4 * i] = v.x; w[n][4 * i + 1] = v.y; w[n][4 * i + 2] = v.z; w[n][4 * i + 3] = v.w;
+          }
+        } else {
+          const uint2 v = sld_v2(sm + T::at(row, t * (RB / 4)));
+          w[n][0] = v.x; w[n][1] = v.y;
+        }
+        if (TYPE == PK_KV_Q4) {
+          const uint2 v = sld_v2(ksc + row * 8);
+          dk[n] = __uint_as_float(v.x);
+          const int sb = (int)((v.y >> (4 * (t * (DH / 4) / 32))) & 15u);
+          sd[n] = dup_h(sb);
+          md[n] = dup_h(-1032 * sb);
+        } else {
+          dk[n] = sld_f(ksc + row * 4);
+        }
+        dv[n] = sld_f(vsc + row * 4 * SW);
       }
-      uint32_t sub = 0, sd = 0, md = 0;
-      if (TYPE == PK_KV_Q4) {
-        sub = __float_as_uint(ks[2 * (8 * n + g) + 1]);
-        const int sb = (int)((sub >> (4 * (t * (DH / 4) / 32))) & 15u);
-        sd = dup_h(sb);
-        md = dup_h(-1032 * sb);
+      float lo[NT == 2 ? NB : 1][4];
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.0f;
+        if (NT == 2) lo[NT == 2 ? b : 0][0] = lo[NT == 2 ? b : 0][1] = lo[NT == 2 ? b : 0][2] = lo[NT == 2 ? b : 0][3] = 0.0f;
       }
 #pragma unroll
       for (int j = 0; j < KS; j++) {
-        uint32_t b0, b1;
-        if (TYPE == PK_KV_Q8) {
-          b0 = codes_of(w[j], 0x4140);
-          b1 = codes_of(w[j], 0x4342);
-        } else {
-          b0 = nibbles_of(w[j / 2] >> (8 * (j % 2)), sd, md);
-          b1 = nibbles_of(w[j / 2] >> (8 * (j % 2) + 4), sd, md);
+        uint32_t f[4];
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          if (TYPE == PK_KV_Q8) {
+            f[n] = codes_of(w[n][j], 0x4140);
+            f[2 + n] = codes_of(w[n][j], 0x4342);
+          } else {
+            f[n] = nibbles_of(w[n][j / 2] >> (8 * (j % 2)), sd[n], md[n]);
+            f[2 + n] = nibbles_of(w[n][j / 2] >> (8 * (j % 2) + 4), sd[n], md[n]);
+          }
         }
-        mma16816(s[n], q[0][j], b0, b1);
-        if (NT == 2) mma16816(s[n], q[NT - 1][j], b0, b1);
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+          const uint2 x = frag(0, b, j);
+          mma16816(s[b], f, x.x, x.y);
+          if (NT == 2) {  // small terms in sums of their own
+            const uint2 y = frag(NT - 1, b, j);
+            mma16816(lo[NT == 2 ? b : 0], f, y.x, y.y);
+          }
+        }
+      }
+      if (NT == 2) {
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) s[b][i] += lo[NT == 2 ? b : 0][i];
       }
     }
-    // this lane's columns: positions p0 + 8 n + 2 t + {0, 1}
-    float dk[2][2], dv[2][2];
-    uint32_t vsub[2][2];
+    // s[b][2 n + e]: key g + 8 n, row 8 b + 2 t + e
+    uint32_t seen = 0xffffffffu;  // bit 4 b + 2 n + e
+    if (MASKED) {
+      seen = 0;
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          const int row = row0 + 8 * b + 2 * t + e, i = row / a.group;
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+            const int p = p0 + g + 8 * n;
+            if (p < u.hi && row < u.rows && (p < u.sv.ctx || sees(a, u, i, p - u.sv.ctx))) seen |= 1u << (4 * b + 2 * n + e);
+          }
+        }
+    }
+    auto off = [&](int b, int i) { return MASKED && !((seen >> (4 * b + i)) & 1u); };
+    float mx[NB][2];
+    bool grow = false;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        s[b][i] *= dk[i >> 1];
+        if (off(b, i)) s[b][i] = -CUDART_INF_F;
+      }
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        mx[b][e] = key_max(fmaxf(s[b][e], s[b][2 + e])) * rs[b][e];
+        grow |= mx[b][e] > m[b][e] + GROW;  // m starts at -inf: a row's first position is always more
+      }
+    }
+    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          if (!(mx[b][e] > m[b][e] + GROW)) continue;
+          l[b][e] *= ex2(m[b][e] - mx[b][e]);
+          // what o holds shrinks by the same factor, which goes into inv; past
+          // 2^100 (at the first position, from infinity) into o
+          const float f = inv[b][e] * ex2(mx[b][e] - m[b][e]);
+          m[b][e] = mx[b][e];
+          inv[b][e] = fminf(f, 0x1p100f);
+          if (f > 0x1p100f) scale_row(b, e, 0x1p100f / f);
+        }
+    }
+    float xm[NB][2];
+    bool big = false;
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) {
+        const float mu = m[b][e] == -CUDART_INF_F ? 0.0f : m[b][e];
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          const float p = ex2(fmaf(s[b][2 * n + e], rs[b][e], -mu));
+          l[b][e] += p;
+          s[b][2 * n + e] = off(b, 2 * n + e) ? 0.0f : p * dv[n];
+        }
+        xm[b][e] = key_max(fmaxf(s[b][e], s[b][2 + e]));
+        big |= xm[b][e] * inv[b][e] > TOP;
+      }
+    if (__any_sync(0xffffffffu, big)) {
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+          if (!(xm[b][e] * inv[b][e] > TOP)) continue;
+          const float now = SET / fmaxf(xm[b][e], 0x1p-100f);
+          scale_row(b, e, now / inv[b][e]);
+          inv[b][e] = now;
+        }
+    }
+    uint32_t p[NT][NB][2];  // keys 2 t, 2 t + 1 (+ 8) of row 8 b + g
+#pragma unroll
+    for (int b = 0; b < NB; b++)
+#pragma unroll
+      for (int n = 0; n < 2; n++) {
+        const float x0 = s[b][2 * n] * inv[b][0], x1 = s[b][2 * n + 1] * inv[b][1];
+        const uint32_t hi = pack2(x0, x1);
+        p[0][b][n] = transpose8(hi);
+        if (NT == 2) p[NT - 1][b][n] = transpose8(rest2(x0, x1, hi));
+      }
+    // V: this lane's DH / 8 dimensions of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+    constexpr int VB = RB / 8, VW = VB / 4;
+    const uint32_t vb = sm + T::CODES;
+    uint32_t v[2][2][VW];
+    uint32_t sd[2] = {0, 0}, md[2] = {0, 0};
 #pragma unroll
     for (int n = 0; n < 2; n++) {
 #pragma unroll
       for (int e = 0; e < 2; e++) {
-        const int k = 8 * n + 2 * t + e;
-        dk[n][e] = ks[k * SW];
-        dv[n][e] = vs[k * SW];
-        if (TYPE == PK_KV_Q4) vsub[n][e] = __float_as_uint(vs[k * SW + SW - 1]);
-      }
-    }
-    bool vis[2][2][2];  // by n-tile, column, row
-    if (masked) {
-#pragma unroll
-      for (int n = 0; n < 2; n++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const int p = p0 + 8 * n + 2 * t + e;
-#pragma unroll
-          for (int r = 0; r < 2; r++) {
-            const int rr = row0 + g + 8 * r;
-            vis[n][e][r] = p < u.hi && rr < u.rows && (p < u.sv.ctx || sees(a, u, rr / a.group, p - u.sv.ctx));
-          }
+        const uint32_t at = vb + T::at(8 * n + 2 * t + e, g * VB);
+        if (VB == 16) {
+          const uint4 x = sld_v4(at);
+          v[n][e][0] = x.x; v[n][e][1 % VW] = x.y; v[n][e][2 % VW] = x.z; v[n][e][3 % VW] = x.w;
+        } else if (VB == 8) {
+          const uint2 x = sld_v2(at);
+          v[n][e][0] = x.x; v[n][e][1 % VW] = x.y;
+        } else {
+          v[n][e][0] = __float_as_uint(sld_f(at));
         }
-    }
-    float mx[2];
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-#pragma unroll
-      for (int n = 0; n < 2; n++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const float v = s[n][2 * r + e] * dk[n][e] * rs[r];
-          s[n][2 * r + e] = masked && !vis[n][e][r] ? -CUDART_INF_F : v;
-        }
-      mx[r] = quad_max(fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])));
-    }
-    // m starts at -inf: a row's first position is always more
-    const bool grow0 = mx[0] > m[0] + GROW, grow1 = mx[1] > m[1] + GROW;
-    if (__any_sync(0xffffffffu, grow0 || grow1)) {
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        if (!(r ? grow1 : grow0)) continue;
-        l[r] *= ex2(m[r] - mx[r]);
-        // what o holds shrinks by the same factor, which goes into inv; past
-        // 2^100 (at the first position, from infinity) into o
-        const float f = inv[r] * ex2(mx[r] - m[r]);
-        m[r] = mx[r];
-        inv[r] = fminf(f, 0x1p100f);
-        if (f > 0x1p100f) scale_row(r, 0x1p100f / f);
       }
-    }
-    float xm[2];
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-      const float mu = m[r] == -CUDART_INF_F ? 0.0f : m[r];
-      xm[r] = 0.0f;
-#pragma unroll
-      for (int n = 0; n < 2; n++)
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const float p = ex2(s[n][2 * r + e] - mu);
-          l[r] += p;
-          const float x = masked && !vis[n][e][r] ? 0.0f : p * dv[n][e];
-          s[n][2 * r + e] = x;
-          xm[r] = fmaxf(xm[r], x);
-        }
-      xm[r] = quad_max(xm[r]);
-    }
-    const bool big0 = xm[0] * inv[0] > TOP, big1 = xm[1] * inv[1] > TOP;
-    if (__any_sync(0xffffffffu, big0 || big1)) {
-#pragma unroll
-      for (int r = 0; r < 2; r++) {
-        if (!(r ? big1 : big0)) continue;
-        const float now = SET / fmaxf(xm[r], 0x1p-100f);
-        scale_row(r, now / inv[r]);
-        inv[r] = now;
-      }
-    }
-    uint32_t ph[NT][4];
-#pragma unroll
-    for (int r = 0; r < 2; r++) {
-#pragma unroll
-      for (int n = 0; n < 2; n++) {
-        const float x0 = s[n][2 * r] * inv[r], x1 = s[n][2 * r + 1] * inv[r];
-        ph[0][r + 2 * n] = pack2(x0, x1);
-        if (NT == 2) ph[NT - 1][r + 2 * n] = rest2(x0, x1, ph[0][r + 2 * n]);
-      }
-    }
-    // V: this lane's DH / 8 dimensions of the four positions of its columns
-    constexpr int VB = RB / 8, VW = VB / 4;
-    uint32_t v[2][2][VW];
-#pragma unroll
-    for (int n = 0; n < 2; n++)
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const uint8_t *vp = vc + (size_t)(8 * n + 2 * t + e) * RB + g * VB;
-        if (VB == 16) *reinterpret_cast<uint4 *>(v[n][e]) = *reinterpret_cast<const uint4 *>(vp);
-        else if (VB == 8) *reinterpret_cast<uint2 *>(v[n][e]) = *reinterpret_cast<const uint2 *>(vp);
-        else v[n][e][0] = *reinterpret_cast<const uint32_t *>(vp);
-      }
-    uint32_t sd[2] = {0, 0}, md[2] = {0, 0};
-    if (TYPE == PK_KV_Q4) {
-      const int sh = 4 * (g * (DH / 8) / 32);
-#pragma unroll
-      for (int n = 0; n < 2; n++) {
-        const int s0 = (int)((vsub[n][0] >> sh) & 15u), s1 = (int)((vsub[n][1] >> sh) & 15u);
+      if (TYPE == PK_KV_Q4) {
+        const int sh = 4 * (g * (DH / 8) / 32);
+        const uint4 x = sld_v4(vsc + (8 * n + 2 * t) * 8);  // D, sub, D, sub
+        const int s0 = (int)((x.y >> sh) & 15u), s1 = (int)((x.w >> sh) & 15u);
         sd[n] = h2u(__halves2half2(__int2half_rn(s0), __int2half_rn(s1)));
         md[n] = h2u(__halves2half2(__int2half_rn(-1032 * s0), __int2half_rn(-1032 * s1)));
       }
     }
+    // of a word's values two a product: dimensions d (rows 0-7), d + 1 (rows 8-15)
 #pragma unroll
     for (int w = 0; w < VW; w++) {
-      if (TYPE == PK_KV_Q8) {
-        uint32_t x[2][2];
+      uint32_t x[2][2];
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-          x[n][0] = __byte_perm(v[n][0][w], v[n][1][w], 0x5140);
-          x[n][1] = __byte_perm(v[n][0][w], v[n][1][w], 0x7362);
-        }
+      for (int n = 0; n < 2; n++) {
+        x[n][0] = __byte_perm(v[n][0][w], v[n][1][w], TYPE == PK_KV_Q8 ? 0x5140 : 0x5410);
+        x[n][1] = __byte_perm(v[n][0][w], v[n][1][w], TYPE == PK_KV_Q8 ? 0x7362 : 0x7632);
+      }
+      constexpr int PW = TYPE == PK_KV_Q8 ? 2 : 4;  // products a word
 #pragma unroll
-        for (int d = 0; d < 4; d++) {
-          const uint32_t sel = d & 1 ? 0x4342 : 0x4140;
-          const uint32_t b0 = codes_of(x[0][d / 2], sel), b1 = codes_of(x[1][d / 2], sel);
-          mma16816(o[4 * w + d], ph[0], b0, b1);
-          if (NT == 2) mma16816(o[4 * w + d], ph[NT - 1], b0, b1);
-        }
-      } else {
-        uint32_t x[2][2];
+      for (int d = 0; d < PW; d++) {
+        uint32_t f[4];
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-          x[n][0] = __byte_perm(v[n][0][w], v[n][1][w], 0x5410);
-          x[n][1] = __byte_perm(v[n][0][w], v[n][1][w], 0x7632);
-        }
+        for (int n = 0; n < 2; n++)
 #pragma unroll
-        for (int d = 0; d < 8; d++) {
-          const uint32_t b0 = nibbles_of(x[0][d / 4] >> (4 * (d % 4)), sd[0], md[0]);
-          const uint32_t b1 = nibbles_of(x[1][d / 4] >> (4 * (d % 4)), sd[1], md[1]);
-          mma16816(o[8 * w + d], ph[0], b0, b1);
-          if (NT == 2) mma16816(o[8 * w + d], ph[NT - 1], b0, b1);
+          for (int e = 0; e < 2; e++) {
+            if (TYPE == PK_KV_Q8) f[2 * n + e] = codes_of(x[n][d], e ? 0x4342 : 0x4140);
+            else f[2 * n + e] = nibbles_of(x[n][d / 2] >> (4 * (2 * (d % 2) + e)), sd[n], md[n]);
+          }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+          float(&acc)[4] = o[b][w * PW + d];
+          if (NT == 2) {  // the tensor core's own sums drop bits below the running one's last; f32 adds round
+            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma16816(c, f, p[NT - 1][b][0], p[NT - 1][b][1]);
+            mma16816(c, f, p[0][b][0], p[0][b][1]);
+#pragma unroll
+            for (int i = 0; i < 4; i++) acc[i] += c[i];
+          } else {
+            mma16816(acc, f, p[0][b][0], p[0][b][1]);
+          }
         }
       }
     }
   }
 };
 
-__device__ __forceinline__ Unit unit_of(const AttnKArgs &a, int rows_tile) {
-  Unit u;
-  long long id = blockIdx.x;
-  u.rt = (int)(id % a.row_tiles);
-  id /= a.row_tiles;
-  u.h = (int)(id % a.c.n_kv);
-  id /= a.c.n_kv;
-  u.ch = (int)(id % a.n_chunk);
-  u.s = (int)(id / a.n_chunk);
-  u.sv = seq_view(a.s, a.c.page_size, u.s);
-  u.rows = u.sv.n * a.group;
-  u.nch = (u.sv.total + a.chunk - 1) / a.chunk;
-  u.lo = u.ch * a.chunk;
-  u.hi = min(u.sv.total, u.lo + a.chunk);
-  return u;
-}
-
-// Writes element pairs of lane's rows: the final row, or the chunk's part.
+// Writes DH / 8 elements of a row: final, or the chunk's part.
 template <int DH>
-__device__ __forceinline__ void write_row(const AttnKArgs &a, const Unit &u, int row, int d0, const float *x) {
+__device__ __forceinline__ void write_row(const AttnKArgs &a, const Unit &u, int row, int d0, const float (&x)[DH / 8]) {
   const int i = row / a.group, h = u.h * a.group + row - i * a.group;
   const long long tok = u.sv.first + i;
   if (u.nch > 1) {
@@ -398,66 +520,121 @@ __device__ __forceinline__ void write_row(const AttnKArgs &a, const Unit &u, int
     return;
   }
   const long long off = tok * a.q.out_tok_stride + (long long)h * a.q.out_head_stride + d0;
-  float v[DH / 8];
-#pragma unroll
-  for (int j = 0; j < DH / 8; j++) v[j] = x[j];
-  if (a.q.type == T_F32) store_n<float, DH / 8>(reinterpret_cast<float *>(a.q.out) + off, a.vec_o, v);
-  else if (a.q.type == T_F16) store_n<__half, DH / 8>(reinterpret_cast<__half *>(a.q.out) + off, a.vec_o, v);
-  else store_n<__nv_bfloat16, DH / 8>(reinterpret_cast<__nv_bfloat16 *>(a.q.out) + off, a.vec_o, v);
+  if (a.q.type == T_F32) store_n<float, DH / 8>(reinterpret_cast<float *>(a.q.out) + off, a.vec_o, x);
+  else if (a.q.type == T_F16) store_n<__half, DH / 8>(reinterpret_cast<__half *>(a.q.out) + off, a.vec_o, x);
+  else store_n<__nv_bfloat16, DH / 8>(reinterpret_cast<__nv_bfloat16 *>(a.q.out) + off, a.vec_o, x);
 }
 
-// A CTA: 16 rows of one kv head of one sequence over one chunk of positions;
-// its warps take tiles of 16 positions in turn and add up at the end.
+// A CTA of 4 warps: RG groups of 8 NB rows times KG = 4 / RG groups of
+// positions.  The warps of a key group share its ring of tiles; key group k
+// takes every KG-th tile from k, and the groups are added up at the end.
 constexpr int AW = 4;
-template <int TYPE, int DH, int NT>
+template <int TYPE, int DH, int NT, int NB, int RG>
+struct Geo {
+  using T = Tile<TYPE, DH>;
+  using W = Warp<TYPE, DH, NT, NB>;
+  static constexpr int KG = AW / RG, ROWS = 8 * NB * RG;
+  static constexpr int RING = KG * NSTAGE * T::BYTES;
+  static constexpr int SUM = KG * ROWS * (DH + 4) * 4;  // outputs (rows padded by 16 bytes), then m, l
+  static constexpr int SMEM = (RING + RG * W::QBYTES) > SUM + KG * ROWS * 8 ? (RING + RG * W::QBYTES) : SUM + KG * ROWS * 8;
+};
+
+template <int TYPE, int DH, int NT, int NB, int RG>
 __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
-  __shared__ float so[AW][16][DH];
-  __shared__ float sm[AW][16], sl[AW][16];
+  using G = Geo<TYPE, DH, NT, NB, RG>;
+  using T = typename G::T;
+  extern __shared__ __align__(128) uint8_t smem[];
   pdl_trigger();
   pdl_wait();
-  const Unit u = unit_of(a, 16);
-  const int row0 = u.rt * 16;
-  if (u.ch >= max(u.nch, 1) || row0 >= u.rows) return;
+  const Unit u = unit_of(a);
+  const int tile0 = u.rt * G::ROWS;
+  if (u.ch >= max(u.nch, 1) || tile0 >= u.rows) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  Warp<TYPE, DH, NT> W;
-  W.init(a, u, row0, lane);
-  for (int p0 = u.lo + 16 * warp; p0 < u.hi; p0 += 16 * AW) {
-    const long long row = row_at(a.c, a.s, u.s, p0, u.h);
-    if (row < 0) continue;
-    W.tile(a, u, row0, p0, row, p0 + 16 > min(u.sv.ctx, u.hi), lane);
-  }
-#pragma unroll
-  for (int r = 0; r < 2; r++) {
-    W.l[r] += __shfl_xor_sync(0xffffffffu, W.l[r], 1);
-    W.l[r] += __shfl_xor_sync(0xffffffffu, W.l[r], 2);
-    if (t == 0) {
-      sm[warp][g + 8 * r] = W.m[r];
-      sl[warp][g + 8 * r] = W.l[r];
+  const int rg = warp % RG, kg = warp / RG, row0 = tile0 + rg * 8 * NB;
+  // without a mask nobody sees past the tile's last token
+  const int last = (min(tile0 + G::ROWS, u.rows) - 1) / a.group;
+  const int hi = a.q.mask ? u.hi : min(u.hi, u.sv.ctx + last + 1);
+  const int span = hi - u.lo - 16 * kg, nt = span > 0 ? (span + 16 * G::KG - 1) / (16 * G::KG) : 0;
+  const uint32_t ring = shaddr(smem) + kg * NSTAGE * T::BYTES;
+  const int ti = rg * 32 + lane, tn = 32 * RG;
+  // lane i holds the page of tile i of the block of 32 tiles being copied, and
+  // of the one being used; -1: none
+  auto pages_of = [&](int i0) {
+    const int i = i0 + lane, p = u.lo + 16 * (kg + G::KG * i);
+    if (i >= nt) return -1;
+    const int j = p >> a.page_shift;
+    const int pg = j < a.s.max_pages ? __ldg(a.s.pages + (size_t)u.s * a.s.max_pages + j) : -1;
+    return pg >= 0 && pg < a.c.n_pages ? pg : -1;
+  };
+  int ahead = pages_of(0), now = ahead;
+  auto issue = [&](int i) {
+    if (i > 0 && (i & 31) == 0) ahead = pages_of(i);
+    const int pg = __shfl_sync(0xffffffffu, ahead, i & 31);
+    if (i < nt && pg >= 0) {
+      const int p = u.lo + 16 * (kg + G::KG * i);
+      const long long row = ((long long)pg * a.c.n_kv + u.h) * a.c.page_size + (p & (a.c.page_size - 1));
+      T::copy(a.c, row, ring + (i % NSTAGE) * T::BYTES, ti, tn);
     }
+    cp_commit();
+  };
 #pragma unroll
-    for (int e = 0; e < 2; e++)
-#pragma unroll
-      for (int i = 0; i < DH / 8; i++) so[warp][g + 8 * r][(2 * t + e) * (DH / 8) + i] = W.o[i][2 * r + e] / W.inv[r];
+  for (int i = 0; i < NSTAGE - 1; i++) issue(i);
+  typename G::W W;
+  W.init(a, u, row0, lane, shaddr(smem) + G::RING + rg * G::W::QBYTES);
+  __syncwarp();
+  for (int i = 0; i < nt; i++) {
+    cp_wait<NSTAGE - 2>();
+    if (RG > 1) bar_n(1 + kg, tn);
+    else __syncwarp();
+    if (i > 0 && (i & 31) == 0) now = ahead;  // (the copies are less than 32 tiles ahead)
+    const int pg = __shfl_sync(0xffffffffu, now, i & 31);
+    issue(i + NSTAGE - 1);
+    if (pg < 0) continue;
+    const int p0 = u.lo + 16 * (kg + G::KG * i);
+    const uint32_t sm = ring + (i % NSTAGE) * T::BYTES;
+    if (p0 + 16 > min(u.sv.ctx, hi)) W.template tile<true>(a, u, row0, p0, sm, lane);
+    else W.template tile<false>(a, u, row0, p0, sm, lane);
   }
+  cp_wait<0>();
+  __syncthreads();  // the ring's memory is free
+  float *so = reinterpret_cast<float *>(smem);
+  float2 *sml = reinterpret_cast<float2 *>(smem + G::SUM);
+#pragma unroll
+  for (int b = 0; b < NB; b++)
+#pragma unroll
+    for (int e = 0; e < 2; e++) {
+      float l = W.l[b][e];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      const int r = kg * G::ROWS + rg * 8 * NB + 8 * b + 2 * t + e;
+      if (g == 0) sml[r] = make_float2(W.m[b][e], l);
+      const float f = 1.0f / W.inv[b][e];
+#pragma unroll
+      for (int i = 0; i < DH / 16; i += 2)
+        *reinterpret_cast<float4 *>(so + r * (DH + 4) + g * (DH / 8) + 2 * i) =
+            make_float4(W.o[b][i][e] * f, W.o[b][i][2 + e] * f, W.o[b][i + 1][e] * f, W.o[b][i + 1][2 + e] * f);
+    }
   __syncthreads();
-  for (int x = threadIdx.x; x < 16 * 8; x += 32 * AW) {
+  for (int x = threadIdx.x; x < G::ROWS * 8; x += 32 * AW) {
     const int r = x >> 3, d0 = (x & 7) * (DH / 8);
-    if (row0 + r >= u.rows) continue;
+    if (tile0 + r >= u.rows) continue;
     float M = -CUDART_INF_F, L = 0.0f, acc[DH / 8];
 #pragma unroll
-    for (int w = 0; w < AW; w++) M = fmaxf(M, sm[w][r]);
+    for (int k = 0; k < G::KG; k++) M = fmaxf(M, sml[k * G::ROWS + r].x);
 #pragma unroll
     for (int j = 0; j < DH / 8; j++) acc[j] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < AW; w++) {
-      const float f = sl[w][r] == 0.0f ? 0.0f : ex2(sm[w][r] - M);  // a NaN sum stays one
-      L = fmaf(f, sl[w][r], L);
+    for (int k = 0; k < G::KG; k++) {
+      const float2 ml = sml[k * G::ROWS + r];
+      const float f = ml.y == 0.0f ? 0.0f : ex2(ml.x - M);  // a NaN sum stays one
+      L = fmaf(f, ml.y, L);
 #pragma unroll
-      for (int j = 0; j < DH / 8; j++) acc[j] = fmaf(f, so[w][r][d0 + j], acc[j]);
+      for (int j = 0; j < DH / 8; j++) acc[j] = fmaf(f, so[(k * G::ROWS + r) * (DH + 4) + d0 + j], acc[j]);
     }
     if (u.nch > 1) {
       if ((x & 7) == 0) {
-        const int i = (row0 + r) / a.group, h = u.h * a.group + (row0 + r) - i * a.group;
+        const int i = (tile0 + r) / a.group, h = u.h * a.group + (tile0 + r) - i * a.group;
         a.part_ml[((long long)(u.sv.first + i) * a.q.n_head + h) * a.n_chunk + u.ch] = make_float2(M, L);
       }
     } else {
@@ -465,7 +642,7 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
 #pragma unroll
       for (int j = 0; j < DH / 8; j++) acc[j] *= inv;
     }
-    write_row<DH>(a, u, row0 + r, d0, acc);
+    write_row<DH>(a, u, tile0 + r, d0, acc);
   }
 }
 
@@ -528,38 +705,69 @@ cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
+// The kernel's variant by the rows that a kv head's tile may have: columns in
+// steps of 8 up to 32 a warp (16 where f32's two terms double the query
+// fragments of 128 dimensions), then two or four warps side by side.
+struct Variant {
+  void (*k)(AttnKArgs) = nullptr;
+  int smem = 0, rows = 0;
+};
+template <int TYPE, int DH, int NT, int NB, int RG>
+Variant variant_as() {
+  using G = Geo<TYPE, DH, NT, NB, RG>;
+  return {k_kv_attn<TYPE, DH, NT, NB, RG>, G::SMEM, G::ROWS};
+}
+template <int TYPE, int DH, int NT>
+Variant variant_rows(long long rows) {
+  constexpr int NBM = NT == 2 && DH == 128 ? 2 : 4;
+  if (rows <= 8) return variant_as<TYPE, DH, NT, 1, 1>();
+  if (rows <= 16) return variant_as<TYPE, DH, NT, 2, 1>();
+  if (rows <= 8 * NBM) return variant_as<TYPE, DH, NT, NBM, 1>();
+  if (rows <= 16 * NBM) return variant_as<TYPE, DH, NT, NBM, 2>();
+  return variant_as<TYPE, DH, NT, NBM, 4>();
+}
 template <int TYPE, int DH>
-void (*attn_kernel(int type))(AttnKArgs) {
-  return type == T_F32 ? k_kv_attn<TYPE, DH, 2> : k_kv_attn<TYPE, DH, 1>;
+Variant variant_type(int type, long long rows) {
+  return type == T_F32 ? variant_rows<TYPE, DH, 2>(rows) : variant_rows<TYPE, DH, 1>(rows);
+}
+Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type) {
+  const long long rows = (long long)s.max_new * (n_head / c.n_kv);
+  if (c.type == PK_KV_Q8) return c.head_dim == 64 ? variant_type<PK_KV_Q8, 64>(type, rows) : variant_type<PK_KV_Q8, 128>(type, rows);
+  return c.head_dim == 64 ? variant_type<PK_KV_Q4, 64>(type, rows) : variant_type<PK_KV_Q4, 128>(type, rows);
 }
 
-}  // namespace
-
-KvSplit kv_attn_split(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type) {
-  KvSplit p;
-  const int group = n_head / c.n_kv;
-  p.row_tiles = (int)(((long long)s.max_new * group + 15) / 16);
+struct Split {
+  int chunk, n_chunk, row_tiles;
+};
+Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, const Variant &v) {
+  Split p;
+  const long long rows = (long long)s.max_new * (n_head / c.n_kv);
+  p.row_tiles = (int)((rows + v.rows - 1) / v.rows);
   const long long units = (long long)s.n_seq * c.n_kv * p.row_tiles, want = 148 * 8;
   const long long most = (s.max_len + MIN_CHUNK - 1) / MIN_CHUNK;
-  long long n = std::max<long long>(1, std::min(most, units ? want / units : 1));
-  p.chunk = (int)std::min<long long>(((s.max_len + n - 1) / n + 63) / 64 * 64, 1 << 30);
+  const long long n = std::max<long long>(1, std::min(most, want / units));
+  p.chunk = (int)(((s.max_len + n - 1) / n + 63) / 64 * 64);
   p.n_chunk = (int)((s.max_len + (long long)p.chunk - 1) / p.chunk);
   return p;
 }
 
+}  // namespace
+
 size_t kv_attn_scratch_bytes(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type) {
-  const KvSplit p = kv_attn_split(c, s, n_head, type);
+  const Split p = split_of(c, s, n_head, variant_of(c, s, n_head, type));
   if (p.n_chunk <= 1) return 0;
   return (size_t)s.n_tok * n_head * p.n_chunk * (c.head_dim + 2) * sizeof(float);
 }
 
 cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_query &q, void *scratch,
                            cudaStream_t st) {
-  const KvSplit p = kv_attn_split(c, s, q.n_head, q.type);
+  const Variant v = variant_of(c, s, q.n_head, q.type);
+  const Split p = split_of(c, s, q.n_head, v);
   AttnKArgs a{};
   a.c = c; a.s = s; a.q = q;
   a.chunk = p.chunk; a.n_chunk = p.n_chunk; a.row_tiles = p.row_tiles;
   a.group = q.n_head / c.n_kv;
+  while ((1 << a.page_shift) < c.page_size) a.page_shift++;
   const uintptr_t es = q.type == T_F32 ? 4 : 2;
   a.vec_q = (((uintptr_t)q.q | (uintptr_t)q.q_tok_stride * es | (uintptr_t)q.q_head_stride * es) & 15) == 0;
   a.vec_o = (((uintptr_t)q.out | (uintptr_t)q.out_tok_stride * es | (uintptr_t)q.out_head_stride * es) & 15) == 0;
@@ -568,10 +776,8 @@ cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_k
   a.part_ml = p.n_chunk > 1 ? reinterpret_cast<float2 *>(a.part_o + rows * p.n_chunk * c.head_dim) : nullptr;
   const long long blocks = (long long)s.n_seq * c.n_kv * p.row_tiles * p.n_chunk, jb = ((long long)rows + 3) / 4;
   if (blocks > 0x7fffffffLL || jb > 0x7fffffffLL) return cudaErrorInvalidValue;
-  void (*k)(AttnKArgs) = c.type == PK_KV_Q8
-                             ? (c.head_dim == 64 ? attn_kernel<PK_KV_Q8, 64>(q.type) : attn_kernel<PK_KV_Q8, 128>(q.type))
-                             : (c.head_dim == 64 ? attn_kernel<PK_KV_Q4, 64>(q.type) : attn_kernel<PK_KV_Q4, 128>(q.type));
-  cudaError_t e = launch(k, dim3((unsigned)blocks), dim3(32 * AW), 0, st, a);
+  cudaError_t e = cudaFuncSetAttribute(v.k, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem);
+  if (e == cudaSuccess) e = launch(v.k, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
   if (e != cudaSuccess || p.n_chunk <= 1) return e;
   return launch(c.head_dim == 64 ? k_kv_attn_join<64> : k_kv_attn_join<128>, dim3((unsigned)jb), dim3(128), 0, st, a);
 }
