@@ -15,16 +15,15 @@ namespace {
 
 constexpr int CT = 128;  // threads of a CTA
 
-// round(x / d) to even for |x / d| < 2^20, exactly: the f32 quotient's
-// rounding error can only move a value across the middle between two codes,
-// and the remainder x - d * c, exact in f32 (both terms are multiples of the
-// smaller one's last place and the difference is below 2 d), tells on which
-// side of it x lies.
-__device__ __forceinline__ float code_of(float x, float d) {
-  float c = rintf(fdiv(x, d));
+// round(x / d) to even for |x / d| < 2^20, exactly, with inv = 1 / d: the
+// product x inv is within 3 f32 roundings of the quotient, which can only move
+// a value across the middle between two codes; the remainder x - d c, exact in
+// f32 (both terms are multiples of the smaller one's last place and the
+// difference is below 2 d), tells on which side of it x lies.
+__device__ __forceinline__ float code_of(float x, float d, float inv) {
+  float c = rintf(isinf(inv) ? fdiv(x, d) : fmul(x, inv));  // (1 / d overflows for d < 2^-128)
   const float r = __fmaf_rn(-d, c, x), h = 0.5f * d, a = fabsf(r);
-  if (a > h) c += r > 0.0f ? 1.0f : -1.0f;
-  else if (a == h && (((int)c) & 1)) c += r > 0.0f ? 1.0f : -1.0f;
+  if (a > h || (a == h && (((int)c) & 1))) c += r > 0.0f ? 1.0f : -1.0f;
   return c;
 }
 
@@ -37,77 +36,113 @@ struct RowsArgs {
   int vec, parts;
 };
 
-// A warp's place: token t and its pass-th set of rows.  Row r < 2 n_kv of a
-// token is K (r < n_kv) or V of kv head r mod n_kv.
+// A warp has one token and U sets of its rows (row r < 2 n_kv of a token is K,
+// r < n_kv, or V of kv head r mod n_kv): the rows' values are asked for
+// before the token's sequence, position and page are looked up, a chain of
+// four dependent reads that is the same for all of them.
+constexpr int U = 4;
+struct Place {
+  int t, set0, lane, l;
+};
+__device__ __forceinline__ Place place_of(int parts, int L) {
+  const long long w = (long long)blockIdx.x * (CT / 32) + (threadIdx.x >> 5);
+  Place p;
+  p.t = (int)(w / parts);
+  p.set0 = (int)(w - (long long)p.t * parts) * U;
+  p.lane = threadIdx.x & 31;
+  p.l = p.lane % L;
+  return p;
+}
+// The cache row of kv head 0 at token t's position, or -1 (no sequence, past
+// the bounds, no page); *mine: the token is some sequence's.
+__device__ __forceinline__ long long head0_row(const RowsArgs &a, int t, int lane, bool *mine) {
+  *mine = false;
+  const int s = seq_of(a.s, t, lane);
+  if (s < 0) return -1;
+  const SeqView sv = seq_view(a.s, a.c.page_size, s);
+  const int i = t - sv.first, p = sv.ctx + i;
+  *mine = i < sv.n;
+  if (i >= sv.n || sv.ctx < 0 || p >= sv.total) return -1;
+  return row_at(a.c, a.s, s, p, 0);
+}
+
 template <int TYPE, int DH, int T>
 __global__ void __launch_bounds__(CT) k_kv_store(const RowsArgs a) {
   using E = elem_t<T>;
   constexpr int L = DH / 8, RW = 32 / L;
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, l = lane % L;
-  const long long w = (long long)blockIdx.x * (CT / 32) + (threadIdx.x >> 5);
-  const int t = (int)(w / a.parts), part = (int)(w - (long long)t * a.parts);
-  if (t >= a.s.n_tok) return;
-  const int s = seq_of(a.s, t, lane);
-  if (s < 0) return;
-  const SeqView sv = seq_view(a.s, a.c.page_size, s);
-  const int p = sv.ctx + (t - sv.first);
-  if (t - sv.first >= sv.n || sv.ctx < 0 || p >= sv.total) return;
-  const int r = part * RW + lane / L;
-  const bool on = r < 2 * a.c.n_kv;
-  const int which = r >= a.c.n_kv ? 1 : 0, h = on ? r - which * a.c.n_kv : 0;
-  const E *src = reinterpret_cast<const E *>(which ? a.src[1] : a.src[0]) + (long long)t * a.tok_stride +
-                 (long long)h * a.head_stride + 8 * l;
-  float x[8];
-  if (on) load_n<E, 8>(src, a.vec, x);
-  float m = 0.0f;
+  const Place pl = place_of(a.parts, L);
+  if (pl.t >= a.s.n_tok) return;
+  const int l = pl.l, lane = pl.lane;
+  float x[U][8];
 #pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float v = on ? x[i] : 0.0f;
-    x[i] = isnan(v) ? 0.0f : fminf(fmaxf(v, -0x1p127f), 0x1p127f);
-    m = fmaxf(m, fabsf(x[i]));
+  for (int k = 0; k < U; k++) {
+    const int r = (pl.set0 + k) * RW + lane / L, which = r >= a.c.n_kv ? 1 : 0;
+    if (r < 2 * a.c.n_kv) {
+      load_n<E, 8>(reinterpret_cast<const E *>(which ? a.src[1] : a.src[0]) + (long long)pl.t * a.tok_stride +
+                       (long long)(r - which * a.c.n_kv) * a.head_stride + 8 * l,
+                   a.vec, x[k]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[k][i] = 0.0f;
+    }
   }
-  const long long row = on ? row_at(a.c, a.s, s, p, h) : -1;
-  uint8_t *codes = reinterpret_cast<uint8_t *>(which ? a.c.v : a.c.k);
-  float *scales = which ? a.c.vs : a.c.ks;
-  if (TYPE == PK_KV_Q8) {
+  bool mine;
+  const long long row0 = head0_row(a, pl.t, lane, &mine);
+  if (row0 < 0) return;
 #pragma unroll
-    for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float d = fdiv(m, 127.0f);
-    uint32_t u[2] = {0, 0};
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-      const float c = d > 0.0f ? fminf(fmaxf(code_of(x[i], d), -127.0f), 127.0f) : 0.0f;
-      u[i / 4] |= (uint32_t)((int)c + 128) << (8 * (i % 4));
-    }
-    if (row < 0) return;
-    *reinterpret_cast<uint2 *>(codes + (size_t)row * DH + 8 * l) = make_uint2(u[0], u[1]);
-    if (l == 0) scales[row] = d;
-  } else {
-    float mb = m;  // of the 32 dimensions
-#pragma unroll
-    for (int o = 2; o > 0; o >>= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
-    m = mb;
-#pragma unroll
-    for (int o = L / 2; o > 2; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float d = fdiv(m, 105.0f);
-    // d == 0: the quotient is NaN (0 / 0) or infinite, and the row stands for 0 either way
-    const float sb = d > 0.0f ? fminf(fmaxf(ceilf(fdiv(mb, fmul(7.0f, d))), 1.0f), 15.0f) : 1.0f;
-    const float step = fmul(d, sb);
-    uint32_t u = 0;
+  for (int k = 0; k < U; k++) {
+    const int r = (pl.set0 + k) * RW + lane / L, which = r >= a.c.n_kv ? 1 : 0;
+    const bool on = r < 2 * a.c.n_kv;
+    if ((pl.set0 + k) * RW >= 2 * a.c.n_kv) break;  // (the whole warp)
+    const size_t row = (size_t)row0 + (size_t)(r - which * a.c.n_kv) * a.c.page_size;
+    float m = 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const float c = step > 0.0f ? fminf(fmaxf(code_of(x[i], step), -8.0f), 7.0f) : 0.0f;
-      u |= (uint32_t)((int)c + 8) << (4 * i);
+      x[k][i] = isnan(x[k][i]) ? 0.0f : fminf(fmaxf(x[k][i], -0x1p127f), 0x1p127f);
+      m = fmaxf(m, fabsf(x[k][i]));
     }
-    uint32_t word = 0;
-    const int base = lane - l;
+    uint8_t *codes = reinterpret_cast<uint8_t *>(which ? a.c.v : a.c.k);
+    float *scales = which ? a.c.vs : a.c.ks;
+    if (TYPE == PK_KV_Q8) {
 #pragma unroll
-    for (int b = 0; b < DH / 32; b++) word |= (uint32_t)__shfl_sync(0xffffffffu, sb, base + 4 * b) << (4 * b);
-    if (row < 0) return;
-    *reinterpret_cast<uint32_t *>(codes + (size_t)row * (DH / 2) + 4 * l) = u;
-    if (l == 0) *reinterpret_cast<float2 *>(scales + 2 * row) = make_float2(d, __uint_as_float(word));
+      for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float d = fdiv(m, 127.0f), inv = fdiv(1.0f, d);
+      uint32_t u[2] = {0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float c = d > 0.0f ? fminf(fmaxf(code_of(x[k][i], d, inv), -127.0f), 127.0f) : 0.0f;
+        u[i / 4] |= (uint32_t)((int)c + 128) << (8 * (i % 4));
+      }
+      if (on) {
+        *reinterpret_cast<uint2 *>(codes + row * DH + 8 * l) = make_uint2(u[0], u[1]);
+        if (l == 0) scales[row] = d;
+      }
+    } else {
+#pragma unroll
+      for (int o = 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float mb = m;  // of the 32 dimensions
+#pragma unroll
+      for (int o = L / 2; o > 2; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const float d = fdiv(m, 105.0f);
+      // d == 0: the quotient is NaN (0 / 0) or infinite, and the row stands for 0 either way
+      const float sb = d > 0.0f ? fminf(fmaxf(ceilf(fdiv(mb, fmul(7.0f, d))), 1.0f), 15.0f) : 1.0f;
+      const float step = fmul(d, sb), inv = fdiv(1.0f, step);
+      uint32_t u = 0;
+#pragma unroll
+      for (int i = 0; i < 8; i++) {
+        const float c = step > 0.0f ? fminf(fmaxf(code_of(x[k][i], step, inv), -8.0f), 7.0f) : 0.0f;
+        u |= (uint32_t)((int)c + 8) << (4 * i);
+      }
+      uint32_t word = 0;
+#pragma unroll
+      for (int b = 0; b < DH / 32; b++) word |= (uint32_t)__shfl_sync(0xffffffffu, sb, lane - l + 4 * b) << (4 * b);
+      if (on) {
+        *reinterpret_cast<uint32_t *>(codes + row * (DH / 2) + 4 * l) = u;
+        if (l == 0) *reinterpret_cast<float2 *>(scales + 2 * row) = make_float2(d, __uint_as_float(word));
+      }
+    }
   }
 }
 
@@ -117,40 +152,52 @@ __global__ void __launch_bounds__(CT) k_kv_load(const RowsArgs a) {
   constexpr int L = DH / 8, RW = 32 / L;
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, l = lane % L;
-  const long long w = (long long)blockIdx.x * (CT / 32) + (threadIdx.x >> 5);
-  const int t = (int)(w / a.parts), part = (int)(w - (long long)t * a.parts);
-  if (t >= a.s.n_tok) return;
-  const int s = seq_of(a.s, t, lane);
-  if (s < 0) return;
-  const SeqView sv = seq_view(a.s, a.c.page_size, s);
-  if (t - sv.first >= sv.n) return;
-  const int p = sv.ctx + (t - sv.first);
-  const int r = part * RW + lane / L;
-  if (r >= 2 * a.c.n_kv) return;
-  const int which = r >= a.c.n_kv ? 1 : 0, h = r - which * a.c.n_kv;
-  const long long row = sv.ctx >= 0 && p < sv.total ? row_at(a.c, a.s, s, p, h) : -1;
-  const uint8_t *codes = reinterpret_cast<const uint8_t *>(which ? a.c.v : a.c.k);
-  const float *scales = which ? a.c.vs : a.c.ks;
-  float x[8];
-  if (row < 0) {
+  const Place pl = place_of(a.parts, L);
+  if (pl.t >= a.s.n_tok) return;
+  const int l = pl.l;
+  bool mine;
+  const long long row0 = head0_row(a, pl.t, pl.lane, &mine);
+  if (!mine) return;
+  uint2 u[U];
+  float2 d[U];
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = 0.0f;
-  } else if (TYPE == PK_KV_Q8) {
-    const uint2 u = *reinterpret_cast<const uint2 *>(codes + (size_t)row * DH + 8 * l);
-    const float d = scales[row];
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = fmul(d, (float)((int)(((i < 4 ? u.x : u.y) >> (8 * (i % 4))) & 255u) - 128));
-  } else {
-    const uint32_t u = *reinterpret_cast<const uint32_t *>(codes + (size_t)row * (DH / 2) + 4 * l);
-    const float2 d = *reinterpret_cast<const float2 *>(scales + 2 * row);
-    const int sb = (int)((__float_as_uint(d.y) >> (4 * (l / 4))) & 15u);
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = fmul(d.x, (float)(((int)((u >> (4 * i)) & 15u) - 8) * sb));
+  for (int k = 0; k < U; k++) {
+    const int r = (pl.set0 + k) * RW + pl.lane / L, which = r >= a.c.n_kv ? 1 : 0;
+    u[k] = make_uint2(0, 0);
+    d[k] = make_float2(0.0f, 0.0f);  // no page: D = 0
+    if (row0 < 0 || r >= 2 * a.c.n_kv) continue;
+    const size_t row = (size_t)row0 + (size_t)(r - which * a.c.n_kv) * a.c.page_size;
+    const uint8_t *codes = reinterpret_cast<const uint8_t *>(which ? a.c.v : a.c.k);
+    const float *scales = which ? a.c.vs : a.c.ks;
+    if (TYPE == PK_KV_Q8) {
+      u[k] = *reinterpret_cast<const uint2 *>(codes + row * DH + 8 * l);
+      d[k].x = scales[row];
+    } else {
+      u[k].x = *reinterpret_cast<const uint32_t *>(codes + row * (DH / 2) + 4 * l);
+      d[k] = *reinterpret_cast<const float2 *>(scales + 2 * row);
+    }
   }
-  E *dst = reinterpret_cast<E *>(which ? a.dst[1] : a.dst[0]) + (long long)t * a.tok_stride +
-           (long long)h * a.head_stride + 8 * l;
-  store_n<E, 8>(dst, a.vec, x);
+#pragma unroll
+  for (int k = 0; k < U; k++) {
+    const int r = (pl.set0 + k) * RW + pl.lane / L, which = r >= a.c.n_kv ? 1 : 0;
+    if (r >= 2 * a.c.n_kv) continue;
+    float x[8];
+    if (TYPE == PK_KV_Q8) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = fmul(d[k].x, (float)((int)(((i < 4 ? u[k].x : u[k].y) >> (8 * (i % 4))) & 255u) - 128));
+    } else {
+      const int sb = (int)((__float_as_uint(d[k].y) >> (4 * (l / 4))) & 15u);
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = fmul(d[k].x, (float)(((int)((u[k].x >> (4 * i)) & 15u) - 8) * sb));
+    }
+    if (row0 < 0) {
+#pragma unroll
+      for (int i = 0; i < 8; i++) x[i] = 0.0f;
+    }
+    store_n<E, 8>(reinterpret_cast<E *>(which ? a.dst[1] : a.dst[0]) + (long long)pl.t * a.tok_stride +
+                      (long long)(r - which * a.c.n_kv) * a.head_stride + 8 * l,
+                  a.vec, x);
+  }
 }
 
 // Accepted drafts: a warp owns (sequence, kv head, K or V) and moves its rows
@@ -236,7 +283,7 @@ cudaError_t rows(bool store, RowsArgs a, int type, cudaStream_t st) {
   const uintptr_t p0 = (uintptr_t)(store ? a.src[0] : a.dst[0]), p1 = (uintptr_t)(store ? a.src[1] : a.dst[1]);
   a.vec = ((p0 | p1 | (uintptr_t)(a.tok_stride * (long)es) | (uintptr_t)(a.head_stride * (long)es)) & 15) == 0;
   const int rw = 32 / (a.c.head_dim / 8);
-  a.parts = (2 * a.c.n_kv + rw - 1) / rw;
+  a.parts = (2 * a.c.n_kv + rw * U - 1) / (rw * U);
   const long long warps = (long long)a.s.n_tok * a.parts, blocks = (warps + CT / 32 - 1) / (CT / 32);
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)blocks);

@@ -3,6 +3,8 @@
 // f32 tables of every position; these are the op level's, for any position.
 #include <math_constants.h>
 
+#include <algorithm>
+
 #include "pk_cache.cuh"
 #include "pk_cache.h"
 
@@ -25,125 +27,286 @@ cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
 }
 
 // ------------------------------------------------------------------- rotary
-// A CTA takes one token: the angles once for all heads (double: position
-// times turns, less its whole turns, is exact to 2^-53 of the angle; the
-// remainder's cosine and sine in f32), then every head's elements.
+// A CTA takes one token and some of its heads: the angles once for them all
+// (double: position times turns, less its whole turns, is exact to 2^-53 of
+// the angle; the remainder's cosine and sine in f32), while the first values
+// are on their way.  An item is V elements (16 bytes where everything is
+// aligned for it): for interleaved pairs a run of a head's dimensions, for
+// the half layout V pairs' two runs, or a run that is copied.
 constexpr int RT = 256;
-template <int T>
-__global__ void __launch_bounds__(RT) k_rope(const pk_rope_args a) {
+// AL: whole runs, aligned to their size; otherwise moved by elements, the last
+// run of an odd head_dim one short.
+template <int T, int V, bool HALF, bool AL>
+struct alignas(16) RopeItem {
   using E = elem_t<T>;
+  E a[V], b[HALF ? V : 1];
+  E *out;
+  int i;    // first pair; HALF: -1 for a copied run
+  int len;  // elements
+  template <class X>
+  __device__ __forceinline__ void move(X *dst, const X *src) const {
+    constexpr int B = V * (int)sizeof(X);
+    if (AL && B == 16) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
+    else if (AL && B == 8) *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(src);
+    else if (AL && B == 4) *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(src);
+    else
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (AL || e < len) dst[e] = src[e];
+  }
+  __device__ __forceinline__ void load(const pk_rope_args &p, long long t, int x, int per, int nq) {
+    const int hh = x / per, k = x - hh * per, half = p.n_rot / 2;
+    const bool isk = hh >= nq;
+    const int h = isk ? hh - nq : hh;
+    const E *in = reinterpret_cast<const E *>(isk ? p.k : p.q) + t * (isk ? p.k_tok_stride : p.q_tok_stride) +
+                  h * (isk ? p.k_head_stride : p.q_head_stride);
+    out = reinterpret_cast<E *>(isk ? p.k_out : p.q_out) + t * (isk ? p.ko_tok_stride : p.qo_tok_stride) +
+          h * (isk ? p.ko_head_stride : p.qo_head_stride);
+    len = min(V, p.head_dim - k * V);
+    if (HALF) {
+      len = V;
+      const bool rot = k * V < half;
+      i = rot ? k * V : -1;
+      const int d = rot ? k * V : k * V + half;  // items past the pairs: dimensions n_rot ..
+      out += d;
+      move(a, in + d);
+      if (rot) move(b, in + d + half);
+    } else {
+      i = k * V / 2;
+      out += k * V;
+      move(a, in + k * V);
+    }
+  }
+  __device__ __forceinline__ void finish(const float2 *cs, int half) {
+    if (HALF) {
+      if (i >= 0) {
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          const float2 c = cs[i + e];
+          const float u = to_f(a[e]), v = to_f(b[e]);
+          a[e] = from_f<E>(u * c.x - v * c.y);
+          b[e] = from_f<E>(u * c.y + v * c.x);
+        }
+        move(out + half, b);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e + 1 < V; e += 2) {
+        if (i + e / 2 >= half) break;
+        const float2 c = cs[i + e / 2];
+        const float u = to_f(a[e]), v = to_f(a[e + 1]);
+        a[e] = from_f<E>(u * c.x - v * c.y);
+        a[e + 1] = from_f<E>(u * c.y + v * c.x);
+      }
+    }
+    move(out, a);
+  }
+};
+
+template <int T, int V, bool HALF, bool AL>
+__global__ void __launch_bounds__(RT) k_rope(const pk_rope_args p, int heads_cta) {
+  constexpr int N = 4;  // items in flight a thread
   extern __shared__ float2 cs[];  // [n_rot / 2]
   pdl_trigger();
   pdl_wait();
   const long long t = blockIdx.x;
-  const int half = a.n_rot / 2;
-  const double pos = (double)__ldg(a.pos + t);
-  for (int i = threadIdx.x; i < half; i += RT) {
-    double x = pos * __ldg(a.turns + i);
-    x -= rint(x);
-    float s, c;
-    sincospif(2.0f * (float)x, &s, &c);
-    cs[i] = make_float2(c * a.gain, s * a.gain);
-  }
-  __syncthreads();
-  const int per = a.head_dim - half, nq = a.q ? a.n_head : 0, heads = nq + (a.k ? a.n_kv : 0);  // work items a head
-  for (int x = threadIdx.x; x < heads * per; x += RT) {
-    const int hh = x / per, i = x - hh * per;
-    const bool k = hh >= nq;
-    const int h = k ? hh - nq : hh;
-    const E *in = reinterpret_cast<const E *>(k ? a.k : a.q) + t * (k ? a.k_tok_stride : a.q_tok_stride) +
-                  h * (k ? a.k_head_stride : a.q_head_stride);
-    E *out = reinterpret_cast<E *>(k ? a.k_out : a.q_out) + t * (k ? a.ko_tok_stride : a.qo_tok_stride) +
-             h * (k ? a.ko_head_stride : a.qo_head_stride);
-    if (i >= half) {
-      out[i + half] = in[i + half];
-      continue;
+  const int half = p.n_rot / 2, nq = p.q ? p.n_head : 0, heads = nq + (p.k ? p.n_kv : 0);
+  // items a head: dimensions (interleaved), or pairs and the dimensions past them
+  const int per = HALF ? (p.head_dim - half) / V : (p.head_dim + V - 1) / V;
+  const int x0 = (int)blockIdx.y * heads_cta * per, x1 = min(heads, ((int)blockIdx.y + 1) * heads_cta) * per;
+  for (int x = x0; x < x1; x += RT * N) {
+    RopeItem<T, V, HALF, AL> it[N];
+#pragma unroll
+    for (int n = 0; n < N; n++)
+      if (x + n * RT + (int)threadIdx.x < x1) it[n].load(p, t, x + n * RT + threadIdx.x, per, nq);
+    if (x == x0) {
+      const double pos = (double)__ldg(p.pos + t);
+      for (int i = threadIdx.x; i < half; i += RT) {
+        double r = pos * __ldg(p.turns + i);
+        r -= rint(r);
+        float s, c;
+        sincospif(2.0f * (float)r, &s, &c);
+        cs[i] = make_float2(c * p.gain, s * p.gain);
+      }
+      __syncthreads();
     }
-    const int d0 = a.layout == PK_ROPE_HALF ? i : 2 * i, d1 = a.layout == PK_ROPE_HALF ? i + half : 2 * i + 1;
-    const float u = to_f(in[d0]), v = to_f(in[d1]);
-    const float2 c = cs[i];
-    out[d0] = from_f<E>(u * c.x - v * c.y);
-    out[d1] = from_f<E>(u * c.y + v * c.x);
+#pragma unroll
+    for (int n = 0; n < N; n++)
+      if (x + n * RT + (int)threadIdx.x < x1) it[n].finish(cs, half);
   }
 }
 
-// -------------------------------------------------------------- logit rules
-// A CTA takes SEG logits of a row.  It counts the row's history ids that fall
-// into its segment in shared memory (whole counts: their order does not
-// matter), adds up the biases there in the list's order, and then goes over
-// the segment once.
-constexpr int LT = 256, SEG = 2048;
+template <int T, int V, bool HALF, bool AL>
+cudaError_t rope_as(const pk_rope_args &a, cudaStream_t st) {
+  // few tokens: a token's heads over several CTAs, so that all SMs take part
+  const int heads = (a.q ? a.n_head : 0) + (a.k ? a.n_kv : 0);
+  const int want = std::max(1, std::min(heads, 592 / std::max(a.n_tok, 1)));
+  const int per = (heads + want - 1) / want;
+  return launch(k_rope<T, V, HALF, AL>, dim3((unsigned)a.n_tok, (unsigned)((heads + per - 1) / per)), dim3(RT),
+                (size_t)(a.n_rot / 2) * sizeof(float2), st, a, per);
+}
 template <int T>
-__global__ void __launch_bounds__(LT) k_logit_rules(const void *in, void *out, int n, long in_stride, long out_stride,
-                                                    const pk_logit_rules r, int segs) {
+cudaError_t rope_type(const pk_rope_args &a, cudaStream_t st) {
+  constexpr int W = 16 / (int)sizeof(elem_t<T>);
+  const bool half = a.layout == PK_ROPE_HALF;
+  // whether items of V elements are whole and aligned
+  auto fits = [&](int v) {
+    uintptr_t bits = 0;
+    if (a.q) bits |= (uintptr_t)a.q | (uintptr_t)a.q_out | ((uintptr_t)(a.q_tok_stride | a.q_head_stride | a.qo_tok_stride | a.qo_head_stride) * sizeof(elem_t<T>));
+    if (a.k) bits |= (uintptr_t)a.k | (uintptr_t)a.k_out | ((uintptr_t)(a.k_tok_stride | a.k_head_stride | a.ko_tok_stride | a.ko_head_stride) * sizeof(elem_t<T>));
+    return bits % (v * sizeof(elem_t<T>)) == 0 && a.head_dim % v == 0 && (!half || (a.n_rot / 2) % v == 0);
+  };
+  if (half) return fits(W) ? rope_as<T, W, true, true>(a, st) : fits(2) ? rope_as<T, 2, true, true>(a, st) : rope_as<T, 1, true, false>(a, st);
+  return fits(W) ? rope_as<T, W, false, true>(a, st) : rope_as<T, 2, false, false>(a, st);
+}
+
+// -------------------------------------------------------------- logit rules
+// A CTA takes SEG logits of a row, NT threads.  Its logits are asked for
+// first; then it counts the row's history ids that fall into its segment in
+// shared memory (whole counts: their order does not matter) and collects the
+// biases of the segment there, in the list's order, which one warp adds up;
+// then the segment is finished and written.
+template <int T, int SEG, int NT>
+__global__ void __launch_bounds__(NT) k_logit_rules(const void *in, void *out, int n, long in_stride, long out_stride,
+                                                    const pk_logit_rules r, int segs, int vec) {
   using E = elem_t<T>;
-  __shared__ int cnt[SEG];
-  __shared__ float bias[SEG];
+  constexpr int V = 16 / (int)sizeof(E), RUNS = SEG / (NT * V);  // a thread has runs of V elements
+  static_assert(RUNS * NT * V == SEG, "whole runs");
+  extern __shared__ __align__(16) uint8_t smem[];
+  int *cnt = reinterpret_cast<int *>(smem);                             // [SEG], where there is a history
+  float *bias = reinterpret_cast<float *>(smem) + (r.hist ? SEG : 0);   // [SEG], where there are biases
+  __shared__ uint32_t bid[NT];
+  __shared__ float bval[NT];
+  __shared__ int bcount[NT / 32];
   pdl_trigger();
   pdl_wait();
   const long long row = blockIdx.x / segs;
-  const int lo = (int)(blockIdx.x - row * segs) * SEG, m = min(SEG, n - lo);
-  for (int i = threadIdx.x; i < SEG; i += LT) {
-    cnt[i] = 0;
-    bias[i] = 0.0f;
+  const int lo = (int)(blockIdx.x - row * segs) * SEG, m = min(SEG, n - lo), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const E *x = reinterpret_cast<const E *>(in) + row * in_stride + lo;
+  E *y = reinterpret_cast<E *>(out) + row * out_stride + lo;
+  alignas(16) E v[RUNS][V];
+#pragma unroll
+  for (int k = 0; k < RUNS; k++) {
+    const int i = (k * NT + tid) * V;
+    if (vec && i + V <= m) {
+      *reinterpret_cast<uint4 *>(v[k]) = *reinterpret_cast<const uint4 *>(x + i);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (i + e < m) v[k][e] = x[i + e];
+    }
   }
+  const int words = (r.hist ? SEG : 0) + (r.bias_id ? SEG : 0);
+  for (int i = tid; i < words / 4; i += NT) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   if (r.hist) {
     const uint32_t *ids = r.hist + row * r.hist_stride;
     const int nh = min(max(r.n_hist ? __ldg(r.n_hist + row) : r.n_hist_max, 0), r.n_hist_max);
-    for (int i = threadIdx.x; i < nh; i += LT) {
+#pragma unroll 4
+    for (int i = tid; i < nh; i += NT) {
       const uint32_t d = __ldg(ids + i) - (uint32_t)lo;
       if (d < (uint32_t)m) atomicAdd(&cnt[d], 1);
     }
   }
-  if (r.bias_id && threadIdx.x < 32) {  // one warp, so that equal ids add up in order
-    for (int i0 = 0; i0 < r.n_bias; i0 += 32) {
-      const int i = i0 + threadIdx.x;
+  if (r.bias_id) {
+    for (int i0 = 0; i0 < r.n_bias; i0 += NT) {  // (uniform)
+      const int i = i0 + tid;
       const uint32_t d = i < r.n_bias ? __ldg(r.bias_id + row * r.bias_stride + i) - (uint32_t)lo : 0xffffffffu;
       const float b = i < r.n_bias ? __ldg(r.bias + row * r.bias_stride + i) : 0.0f;
-      const unsigned same = __match_any_sync(0xffffffffu, d < (uint32_t)m ? d : 0xffffffffu);
+      const unsigned here = __ballot_sync(0xffffffffu, d < (uint32_t)m);
+      if (lane == 0) bcount[warp] = __popc(here);
+      __syncthreads();
+      int at = __popc(here & ((1u << lane) - 1)), all = 0;
+#pragma unroll
+      for (int w = 0; w < NT / 32; w++) {
+        at += w < warp ? bcount[w] : 0;
+        all += bcount[w];
+      }
       if (d < (uint32_t)m) {
-        for (unsigned left = same; left; left &= left - 1) {  // the group's lanes in order
-          if ((int)threadIdx.x == __ffs(left) - 1) bias[d] += b;
-          __syncwarp(same);
+        bid[at] = d;
+        bval[at] = b;
+      }
+      __syncthreads();
+      if (warp == 0) {
+        for (int j0 = 0; j0 < all; j0 += 32) {
+          const uint32_t id = j0 + lane < all ? bid[j0 + lane] : 0xffffffffu;
+          const unsigned same = __match_any_sync(0xffffffffu, id);
+          if (id != 0xffffffffu) {
+            for (unsigned left = same; left; left &= left - 1) {  // lanes with the same id, in order
+              if (lane == __ffs(left) - 1) bias[id] += bval[j0 + lane];
+              __syncwarp(same);
+            }
+          }
+          __syncwarp();
         }
       }
-      __syncwarp();
+      __syncthreads();
     }
   }
   __syncthreads();
   const float rep = r.repeat ? __ldg(r.repeat + row) : 1.0f, fr = r.freq ? __ldg(r.freq + row) : 0.0f,
               pr = r.presence ? __ldg(r.presence + row) : 0.0f;
-  const E *x = reinterpret_cast<const E *>(in) + row * in_stride + lo;
-  E *y = reinterpret_cast<E *>(out) + row * out_stride + lo;
-  for (int i = threadIdx.x; i < m; i += LT) {
-    float v = to_f(x[i]);
-    const int c = cnt[i];
-    if (c > 0) {
-      v = v > 0.0f ? fdiv(v, rep) : fmul(v, rep);
-      v = fsub(v, fadd(fmul((float)c, fr), pr));
+  const uint32_t *allow = r.allow ? r.allow + row * r.allow_stride + (lo >> 5) : nullptr;
+#pragma unroll
+  for (int k = 0; k < RUNS; k++) {
+    const int i = (k * NT + tid) * V;
+    if (i >= m) break;
+    const uint32_t ok = allow ? __ldg(allow + (i >> 5)) >> (i & 31) : 0xffffffffu;  // V divides 32
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+      if (i + e >= m) break;
+      float f = to_f(v[k][e]);
+      if (r.hist) {
+        const int c = cnt[i + e];
+        if (c > 0) {
+          f = f > 0.0f ? fdiv(f, rep) : fmul(f, rep);
+          f = fsub(f, fadd(fmul((float)c, fr), pr));
+        }
+      }
+      if (r.bias_id) f = fadd(f, bias[i + e]);
+      v[k][e] = from_f<E>((ok >> e) & 1 ? f : -CUDART_INF_F);
     }
-    v = fadd(v, bias[i]);
-    if (r.allow && !((__ldg(r.allow + row * r.allow_stride + ((lo + i) >> 5)) >> (i & 31)) & 1)) v = -CUDART_INF_F;
-    y[i] = from_f<E>(v);
+    if (vec && i + V <= m) {
+      *reinterpret_cast<uint4 *>(y + i) = *reinterpret_cast<const uint4 *>(v[k]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (i + e < m) y[i + e] = v[k][e];
+    }
   }
+}
+
+template <int T, int SEG, int NT>
+cudaError_t rules_as(const void *in, void *out, int rows, int n, long is, long os, const pk_logit_rules &r, cudaStream_t st) {
+  constexpr int es = (int)sizeof(elem_t<T>);
+  const int segs = (n + SEG - 1) / SEG;
+  const long long blocks = (long long)rows * segs;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const int vec = (((uintptr_t)in | (uintptr_t)out | (rows > 1 ? (uintptr_t)(is | os) * es : 0)) & 15) == 0;
+  const int smem = ((r.hist ? SEG : 0) + (r.bias_id ? SEG : 0)) * 4;
+  const cudaError_t e = cudaFuncSetAttribute(k_logit_rules<T, SEG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * SEG * 4);
+  if (e != cudaSuccess) return e;
+  return launch(k_logit_rules<T, SEG, NT>, dim3((unsigned)blocks), dim3(NT), (size_t)smem, st, in, out, n, is, os, r, segs, vec);
+}
+// Every CTA goes over the whole history, so segments are large (8192: 64 KB of
+// counts and biases, three CTAs an SM) unless that leaves SMs idle.
+template <int T>
+cudaError_t rules_type(const void *in, void *out, int rows, int n, long is, long os, const pk_logit_rules &r, cudaStream_t st) {
+  if ((long long)rows * ((n + 8191) / 8192) < 296) return rules_as<T, 2048, 256>(in, out, rows, n, is, os, r, st);
+  return rules_as<T, 8192, 512>(in, out, rows, n, is, os, r, st);
 }
 
 }  // namespace
 
 cudaError_t launch_rope(const pk_rope_args &a, cudaStream_t st) {
-  void (*k)(pk_rope_args) = a.type == T_F32 ? k_rope<T_F32> : a.type == T_F16 ? k_rope<T_F16> : k_rope<T_BF16>;
-  return launch(k, dim3((unsigned)a.n_tok), dim3(RT), (size_t)(a.n_rot / 2) * sizeof(float2), st, a);
+  return a.type == T_F32 ? rope_type<T_F32>(a, st) : a.type == T_F16 ? rope_type<T_F16>(a, st) : rope_type<T_BF16>(a, st);
 }
 
 cudaError_t launch_logit_rules(const void *logits, void *out, int type, int rows, int n, long in_stride,
                                long out_stride, const pk_logit_rules &r, cudaStream_t st) {
-  const int segs = (n + SEG - 1) / SEG;
-  const long long blocks = (long long)rows * segs;
-  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  void (*k)(const void *, void *, int, long, long, pk_logit_rules, int) =
-      type == T_F32 ? k_logit_rules<T_F32> : type == T_F16 ? k_logit_rules<T_F16> : k_logit_rules<T_BF16>;
-  return launch(k, dim3((unsigned)blocks), dim3(LT), 0, st, logits, out, n, in_stride, out_stride, r, segs);
+  return type == T_F32   ? rules_type<T_F32>(logits, out, rows, n, in_stride, out_stride, r, st)
+         : type == T_F16 ? rules_type<T_F16>(logits, out, rows, n, in_stride, out_stride, r, st)
+                         : rules_type<T_BF16>(logits, out, rows, n, in_stride, out_stride, r, st);
 }
 
 }  // namespace pk
