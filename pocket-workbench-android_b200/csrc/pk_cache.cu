@@ -15,16 +15,60 @@ namespace {
 
 constexpr int CT = 128;  // threads of a CTA
 
-// round(x / d) to even for |x / d| < 2^20, exactly, with inv = 1 / d: the
-// product x inv is within 3 f32 roundings of the quotient, which can only move
-// a value across the middle between two codes; the remainder x - d c, exact in
-// f32 (both terms are multiples of the smaller one's last place and the
-// difference is below 2 d), tells on which side of it x lies.
-__device__ __forceinline__ float code_of(float x, float d, float inv) {
-  float c = rintf(isinf(inv) ? fdiv(x, d) : fmul(x, inv));  // (1 / d overflows for d < 2^-128)
-  const float r = __fmaf_rn(-d, c, x), h = 0.5f * d, a = fabsf(r);
-  if (a > h || (a == h && (((int)c) & 1))) c += r > 0.0f ? 1.0f : -1.0f;
-  return c;
+// (a0 b0 + c0, a1 b1 + c1), rounded once each, in one instruction.
+__device__ __forceinline__ void fma_x2(float a0, float a1, float b0, float b1, float c0, float c1, float &d0, float &d1) {
+  asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 a, a, b, c;\n mov.b64 {%0, %1}, a;\n}"
+      : "=f"(d0), "=f"(d1)
+      : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+
+// The codes of a lane's eight values, round(x / d) to even, as the bits of
+// 1.5 2^23 + c (whose last bits are c's); most: the largest code.  The product
+// with an approximate reciprocal lies within 2^-15 of the quotient (below 128;
+// the reciprocal's error and the rounding), so c is off by at most one, and
+// only where x lies within 2^-14 of a step of the middle between two codes.
+// There the remainder x - d c, exact in f32 (both terms are multiples of the
+// smaller one's last place and the difference is below 2 d), tells on which
+// side.  Scales near f32's lower end are moved up with their values first;
+// below its normal range D itself is coarse and quotients may pass `most`.
+__device__ __forceinline__ void codes8(float (&x)[8], float d, float most, uint32_t (&u)[8]) {
+  const bool tiny = !(d >= 0x1p-60f);
+  if (tiny) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = d > 0.0f ? x[i] * 0x1p64f : 0.0f;
+    d = d > 0.0f ? d * 0x1p64f : 1.0f;
+  }
+  float inv, far = 0.0f;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d));
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    float t0, t1, c0, c1, r0, r1;
+    fma_x2(x[i], x[i + 1], inv, inv, 12582912.0f, 12582912.0f, t0, t1);
+    fma_x2(t0, t1, -1.0f, -1.0f, 12582912.0f, 12582912.0f, c0, c1);  // -c
+    fma_x2(c0, c1, d, d, x[i], x[i + 1], r0, r1);
+    u[i] = __float_as_uint(t0);
+    u[i + 1] = __float_as_uint(t1);
+    far = fmaxf(far, fmaxf(fabsf(r0), fabsf(r1)));
+  }
+  if (tiny || far >= d * (0.5f - 0x1p-14f)) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+      float c = fsub(__uint_as_float(u[i]), 12582912.0f);
+      const float r = __fmaf_rn(-d, c, x[i]), h = 0.5f * d, a = fabsf(r);
+      if (a > h || (a == h && (u[i] & 1u))) c += r > 0.0f ? 1.0f : -1.0f;
+      c = fminf(fmaxf(c, most < 127.0f ? -8.0f : -127.0f), most);
+      u[i] = __float_as_uint(fadd(c, 12582912.0f));
+    }
+  }
+}
+// m / c for c = 127, 105 as the division rounds it (Markstein: one correction
+// of the product with the rounded reciprocal by the exact remainder; equal to
+// the division for every 24-bit significand), or by it near the ends.
+__device__ __forceinline__ float over(float m, float c, float rc) {
+  if (!(m >= 0x1p-90f)) return fdiv(m, c);
+  const float q = fmul(m, rc);
+  return __fmaf_rn(__fmaf_rn(-c, q, m), rc, q);
 }
 
 struct RowsArgs {
@@ -33,22 +77,22 @@ struct RowsArgs {
   const void *src[2];
   void *dst[2];
   long tok_stride, head_stride;
-  int vec, parts;
+  int vec, parts, sets;  // parts: warps a token; sets: row sets a warp (a multiple of U)
 };
 
-// A warp has one token and U sets of its rows (row r < 2 n_kv of a token is K,
-// r < n_kv, or V of kv head r mod n_kv): the rows' values are asked for
-// before the token's sequence, position and page are looked up, a chain of
-// four dependent reads that is the same for all of them.
-constexpr int U = 4;
+// A warp has one token and some sets of RW heads, K and V of each, U sets at a
+// time: the rows' values are asked for before the token's sequence, position
+// and page are looked up, a chain of four dependent reads that is the same for
+// all of them, and from set to set only additions lead.
+constexpr int U = 2;
 struct Place {
   int t, set0, lane, l;
 };
-__device__ __forceinline__ Place place_of(int parts, int L) {
+__device__ __forceinline__ Place place_of(const RowsArgs &a, int L) {
   const long long w = (long long)blockIdx.x * (CT / 32) + (threadIdx.x >> 5);
   Place p;
-  p.t = (int)(w / parts);
-  p.set0 = (int)(w - (long long)p.t * parts) * U;
+  p.t = (int)(w / a.parts);
+  p.set0 = (int)(w - (long long)p.t * a.parts) * a.sets;
   p.lane = threadIdx.x & 31;
   p.l = p.lane % L;
   return p;
@@ -66,82 +110,128 @@ __device__ __forceinline__ long long head0_row(const RowsArgs &a, int t, int lan
   return row_at(a.c, a.s, s, p, 0);
 }
 
-template <int TYPE, int DH, int T>
-__global__ void __launch_bounds__(CT) k_kv_store(const RowsArgs a) {
-  using E = elem_t<T>;
-  constexpr int L = DH / 8, RW = 32 / L;
-  pdl_trigger();
-  pdl_wait();
-  const Place pl = place_of(a.parts, L);
-  if (pl.t >= a.s.n_tok) return;
-  const int l = pl.l, lane = pl.lane;
-  float x[U][8];
+// Quantises a row held eight values a lane and writes it: codes at `codes`
+// (this lane's), scale at `scale` (the row's).  All lanes of the warp call it.
+template <int TYPE, int DH, class E>
+__device__ __forceinline__ void store_row(const uint4 (&raw)[sizeof(E) / 2], bool on, int lane, int l, uint8_t *codes, float *scale) {
+  constexpr int L = DH / 8;
+  float x[8];
+  uint32_t mb = 0;  // bits of the largest magnitude: NaN's are above infinity's
 #pragma unroll
-  for (int k = 0; k < U; k++) {
-    const int r = (pl.set0 + k) * RW + lane / L, which = r >= a.c.n_kv ? 1 : 0;
-    if (r < 2 * a.c.n_kv) {
-      load_n<E, 8>(reinterpret_cast<const E *>(which ? a.src[1] : a.src[0]) + (long long)pl.t * a.tok_stride +
-                       (long long)(r - which * a.c.n_kv) * a.head_stride + 8 * l,
-                   a.vec, x[k]);
-    } else {
+  for (int i = 0; i < 8; i++) x[i] = to_f(reinterpret_cast<const E *>(raw)[i]);
+  if (sizeof(E) == 2) {  // two at a time
+    const uint32_t m2 = __vmaxu2(__vmaxu2(raw[0].x & 0x7fff7fffu, raw[0].y & 0x7fff7fffu),
+                                 __vmaxu2(raw[0].z & 0x7fff7fffu, raw[0].w & 0x7fff7fffu));
+    const uint16_t m1 = (uint16_t)max(m2 >> 16, m2 & 0xffffu);
+    mb = __float_as_uint(to_f(*reinterpret_cast<const E *>(&m1))) & 0x7fffffffu;
+  } else {
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[k][i] = 0.0f;
-    }
+    for (int i = 0; i < 8; i++) mb = max(mb, __float_as_uint(x[i]) & 0x7fffffffu);
   }
-  bool mine;
-  const long long row0 = head0_row(a, pl.t, lane, &mine);
-  if (row0 < 0) return;
-#pragma unroll
-  for (int k = 0; k < U; k++) {
-    const int r = (pl.set0 + k) * RW + lane / L, which = r >= a.c.n_kv ? 1 : 0;
-    const bool on = r < 2 * a.c.n_kv;
-    if ((pl.set0 + k) * RW >= 2 * a.c.n_kv) break;  // (the whole warp)
-    const size_t row = (size_t)row0 + (size_t)(r - which * a.c.n_kv) * a.c.page_size;
-    float m = 0.0f;
+  if (mb > 0x7f000000u) {  // 2^127
+    mb = 0;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      x[k][i] = isnan(x[k][i]) ? 0.0f : fminf(fmaxf(x[k][i], -0x1p127f), 0x1p127f);
-      m = fmaxf(m, fabsf(x[k][i]));
+      x[i] = isnan(x[i]) ? 0.0f : fminf(fmaxf(x[i], -0x1p127f), 0x1p127f);
+      mb = max(mb, __float_as_uint(x[i]) & 0x7fffffffu);
     }
-    uint8_t *codes = reinterpret_cast<uint8_t *>(which ? a.c.v : a.c.k);
-    float *scales = which ? a.c.vs : a.c.ks;
-    if (TYPE == PK_KV_Q8) {
+  }
+  uint32_t u[8];
+  if (TYPE == PK_KV_Q8) {
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float d = fdiv(m, 127.0f), inv = fdiv(1.0f, d);
-      uint32_t u[2] = {0, 0};
+    for (int o = L / 2; o > 0; o >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+    const float d = over(__uint_as_float(mb), 127.0f, 1.0f / 127.0f);
+    codes8(x, d, 127.0f, u);
+    uint32_t w[2];
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float c = d > 0.0f ? fminf(fmaxf(code_of(x[k][i], d, inv), -127.0f), 127.0f) : 0.0f;
-        u[i / 4] |= (uint32_t)((int)c + 128) << (8 * (i % 4));
-      }
-      if (on) {
-        *reinterpret_cast<uint2 *>(codes + row * DH + 8 * l) = make_uint2(u[0], u[1]);
-        if (l == 0) scales[row] = d;
-      }
+    for (int i = 0; i < 2; i++)
+      w[i] = __byte_perm(__byte_perm(u[4 * i], u[4 * i + 1], 0x0040), __byte_perm(u[4 * i + 2], u[4 * i + 3], 0x0040), 0x5410) ^ 0x80808080u;
+    if (on) {
+      *reinterpret_cast<uint2 *>(codes) = make_uint2(w[0], w[1]);
+      if (l == 0) *scale = d;
+    }
+  } else {
+#pragma unroll
+    for (int o = 2; o > 0; o >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+    const float block = __uint_as_float(mb);  // of the 32 dimensions
+#pragma unroll
+    for (int o = L / 2; o > 2; o >>= 1) mb = max(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+    const float d = over(__uint_as_float(mb), 105.0f, 1.0f / 105.0f);
+    // ceil of the rounded quotient block / (7 d), 1 .. 15 (1 for d = 0): the
+    // division itself only where a quotient 2^-20 off could change it
+    const float d7 = fmul(7.0f, d);
+    float inv, sb = 15.0f;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(d7));
+    const float q = fmul(block, inv), near = rintf(q);
+    if (!(d >= 0x1p-100f) || (fabsf(q - near) < 0x1p-16f && near < 15.0f))
+      sb = d > 0.0f ? fminf(fmaxf(ceilf(fdiv(block, d7)), 1.0f), 15.0f) : 1.0f;
+    else if (q < 14.5f)
+      sb = fmaxf(ceilf(q), 1.0f);
+    codes8(x, fmul(d, sb), 7.0f, u);
+    uint32_t w = 0x88888888u - 0x4b400000u * 0x11111111u;  // sum of (c + 8) 16^i, by the words' last bits
+#pragma unroll
+    for (int i = 0; i < 8; i++) w += u[i] << (4 * i);
+    uint32_t word = (uint32_t)sb << (4 * (l / 4));
+    word |= __shfl_xor_sync(0xffffffffu, word, 4);
+    if (DH == 128) word |= __shfl_xor_sync(0xffffffffu, word, 8);
+    if (on) {
+      *reinterpret_cast<uint32_t *>(codes) = w;
+      if (l == 0) *reinterpret_cast<float2 *>(scale) = make_float2(d, __uint_as_float(word));
+    }
+  }
+}
+
+template <int TYPE, int DH, int T>
+__global__ void __launch_bounds__(CT, 8) k_kv_store(const RowsArgs a) {
+  using E = elem_t<T>;
+  constexpr int L = DH / 8, RW = 32 / L, RB = TYPE == PK_KV_Q8 ? DH : DH / 2, SW = TYPE == PK_KV_Q8 ? 1 : 2, W = sizeof(E) / 2;
+  pdl_trigger();
+  pdl_wait();
+  const Place pl = place_of(a, L);
+  if (pl.t >= a.s.n_tok) return;
+  const int set1 = min(pl.set0 + a.sets, (a.c.n_kv + RW - 1) / RW);
+  int h = pl.set0 * RW + pl.lane / L;
+  const long long off = (long long)pl.t * a.tok_stride + (long long)h * a.head_stride + 8 * pl.l, step = RW * a.head_stride;
+  const E *k = reinterpret_cast<const E *>(a.src[0]) + off, *v = reinterpret_cast<const E *>(a.src[1]) + off;
+  uint4 rk[U][W], rv[U][W];
+  auto ask1 = [&](uint4(&raw)[W], const E *p) {
+    if (a.vec) {
+#pragma unroll
+      for (int w = 0; w < W; w++) raw[w] = __ldg(reinterpret_cast<const uint4 *>(p) + w);
     } else {
 #pragma unroll
-      for (int o = 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float mb = m;  // of the 32 dimensions
+      for (int i = 0; i < 8; i++) reinterpret_cast<E *>(raw)[i] = p[i];
+    }
+  };
+  auto ask = [&](int h) {  // the next U sets
 #pragma unroll
-      for (int o = L / 2; o > 2; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-      const float d = fdiv(m, 105.0f);
-      // d == 0: the quotient is NaN (0 / 0) or infinite, and the row stands for 0 either way
-      const float sb = d > 0.0f ? fminf(fmaxf(ceilf(fdiv(mb, fmul(7.0f, d))), 1.0f), 15.0f) : 1.0f;
-      const float step = fmul(d, sb), inv = fdiv(1.0f, step);
-      uint32_t u = 0;
+    for (int i = 0; i < U; i++) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float c = step > 0.0f ? fminf(fmaxf(code_of(x[k][i], step, inv), -8.0f), 7.0f) : 0.0f;
-        u |= (uint32_t)((int)c + 8) << (4 * i);
-      }
-      uint32_t word = 0;
+      for (int w = 0; w < W; w++) rk[i][w] = rv[i][w] = make_uint4(0, 0, 0, 0);
+      if (h + i * RW >= a.c.n_kv) continue;
+      ask1(rk[i], k);
+      ask1(rv[i], v);
+      k += step;
+      v += step;
+    }
+  };
+  ask(h);
+  bool mine;
+  const long long row0 = head0_row(a, pl.t, pl.lane, &mine);
+  if (row0 < 0) return;
+  const size_t row = (size_t)row0 + (size_t)h * a.c.page_size, rows = (size_t)RW * a.c.page_size;
+  size_t co = row * RB + pl.l * (RB / L), so = row * SW;
+  for (int set = pl.set0; set < set1; set += U) {
+    if (set > pl.set0) ask(h);
 #pragma unroll
-      for (int b = 0; b < DH / 32; b++) word |= (uint32_t)__shfl_sync(0xffffffffu, sb, lane - l + 4 * b) << (4 * b);
-      if (on) {
-        *reinterpret_cast<uint32_t *>(codes + row * (DH / 2) + 4 * l) = u;
-        if (l == 0) *reinterpret_cast<float2 *>(scales + 2 * row) = make_float2(d, __uint_as_float(word));
-      }
+    for (int i = 0; i < U; i++) {
+      if (set + i >= set1) break;  // (the whole warp)
+      const bool on = h < a.c.n_kv;
+      store_row<TYPE, DH, E>(rk[i], on, pl.lane, pl.l, reinterpret_cast<uint8_t *>(a.c.k) + co, a.c.ks + so);
+      store_row<TYPE, DH, E>(rv[i], on, pl.lane, pl.l, reinterpret_cast<uint8_t *>(a.c.v) + co, a.c.vs + so);
+      co += rows * RB;
+      so += rows * SW;
+      h += RW;
     }
   }
 }
@@ -149,54 +239,69 @@ __global__ void __launch_bounds__(CT) k_kv_store(const RowsArgs a) {
 template <int TYPE, int DH, int T>
 __global__ void __launch_bounds__(CT) k_kv_load(const RowsArgs a) {
   using E = elem_t<T>;
-  constexpr int L = DH / 8, RW = 32 / L;
+  constexpr int L = DH / 8, RW = 32 / L, RB = TYPE == PK_KV_Q8 ? DH : DH / 2, SW = TYPE == PK_KV_Q8 ? 1 : 2;
   pdl_trigger();
   pdl_wait();
-  const Place pl = place_of(a.parts, L);
+  const Place pl = place_of(a, L);
   if (pl.t >= a.s.n_tok) return;
-  const int l = pl.l;
   bool mine;
   const long long row0 = head0_row(a, pl.t, pl.lane, &mine);
   if (!mine) return;
-  uint2 u[U];
-  float2 d[U];
+  const int h0 = pl.set0 * RW + pl.lane / L, h1 = min(a.c.n_kv, (pl.set0 + a.sets) * RW);
+  const size_t row = (size_t)max(row0, 0LL) + (size_t)h0 * a.c.page_size, rows = (size_t)RW * a.c.page_size;
+  size_t co = row * RB + pl.l * (RB / L), so = row * SW;
+  long long off = (long long)pl.t * a.tok_stride + (long long)h0 * a.head_stride + 8 * pl.l;
+  for (int h = h0; h < h1; h += U * RW) {
+    uint2 u[U][2];
+    float2 d[U][2];
 #pragma unroll
-  for (int k = 0; k < U; k++) {
-    const int r = (pl.set0 + k) * RW + pl.lane / L, which = r >= a.c.n_kv ? 1 : 0;
-    u[k] = make_uint2(0, 0);
-    d[k] = make_float2(0.0f, 0.0f);  // no page: D = 0
-    if (row0 < 0 || r >= 2 * a.c.n_kv) continue;
-    const size_t row = (size_t)row0 + (size_t)(r - which * a.c.n_kv) * a.c.page_size;
-    const uint8_t *codes = reinterpret_cast<const uint8_t *>(which ? a.c.v : a.c.k);
-    const float *scales = which ? a.c.vs : a.c.ks;
-    if (TYPE == PK_KV_Q8) {
-      u[k] = *reinterpret_cast<const uint2 *>(codes + row * DH + 8 * l);
-      d[k].x = scales[row];
-    } else {
-      u[k].x = *reinterpret_cast<const uint32_t *>(codes + row * (DH / 2) + 4 * l);
-      d[k] = *reinterpret_cast<const float2 *>(scales + 2 * row);
+    for (int i = 0; i < U; i++) {
+#pragma unroll
+      for (int w = 0; w < 2; w++) {
+        u[i][w] = make_uint2(0x80808080u, 0x80808080u);
+        d[i][w] = make_float2(0.0f, 0.0f);  // no page: D = 0
+        if (row0 < 0 || h + i * RW >= h1) continue;
+        const uint8_t *codes = reinterpret_cast<const uint8_t *>(w ? a.c.v : a.c.k) + co;
+        const float *scales = (w ? a.c.vs : a.c.ks) + so;
+        if (TYPE == PK_KV_Q8) {
+          u[i][w] = *reinterpret_cast<const uint2 *>(codes);
+          d[i][w].x = *scales;
+        } else {
+          u[i][w].x = *reinterpret_cast<const uint32_t *>(codes);
+          d[i][w] = *reinterpret_cast<const float2 *>(scales);
+        }
+      }
+      co += rows * RB;
+      so += rows * SW;
     }
-  }
 #pragma unroll
-  for (int k = 0; k < U; k++) {
-    const int r = (pl.set0 + k) * RW + pl.lane / L, which = r >= a.c.n_kv ? 1 : 0;
-    if (r >= 2 * a.c.n_kv) continue;
-    float x[8];
-    if (TYPE == PK_KV_Q8) {
+    for (int i = 0; i < U; i++) {
+      if (h + i * RW >= h1) break;
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = fmul(d[k].x, (float)((int)(((i < 4 ? u[k].x : u[k].y) >> (8 * (i % 4))) & 255u) - 128));
-    } else {
-      const int sb = (int)((__float_as_uint(d[k].y) >> (4 * (l / 4))) & 15u);
+      for (int w = 0; w < 2; w++) {
+        float x[8];
+        const float dd = d[i][w].x;
+        if (TYPE == PK_KV_Q8) {
 #pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = fmul(d[k].x, (float)(((int)((u[k].x >> (4 * i)) & 15u) - 8) * sb));
+          for (int e = 0; e < 4; e++) {
+            const float2 f = __half22float2(u2h(codes_of(e < 2 ? u[i][w].x : u[i][w].y, e % 2 ? 0x4342 : 0x4140)));
+            x[2 * e] = fmul(dd, f.x);
+            x[2 * e + 1] = fmul(dd, f.y);
+          }
+        } else {
+          const int sb = (int)((__float_as_uint(d[i][w].y) >> (4 * (pl.l / 4))) & 15u);
+          const uint32_t s2 = dup_h(sb), m2 = dup_h(-1032 * sb);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {  // nibbles e and e + 4
+            const float2 f = __half22float2(u2h(nibbles_of(u[i][w].x >> (4 * e), s2, m2)));
+            x[e] = fmul(dd, f.x);
+            x[e + 4] = fmul(dd, f.y);
+          }
+        }
+        store_n<E, 8>(reinterpret_cast<E *>(a.dst[w]) + off, a.vec, x);
+      }
+      off += RW * a.head_stride;
     }
-    if (row0 < 0) {
-#pragma unroll
-      for (int i = 0; i < 8; i++) x[i] = 0.0f;
-    }
-    store_n<E, 8>(reinterpret_cast<E *>(which ? a.dst[1] : a.dst[0]) + (long long)pl.t * a.tok_stride +
-                      (long long)(r - which * a.c.n_kv) * a.head_stride + 8 * l,
-                  a.vec, x);
   }
 }
 
@@ -283,7 +388,12 @@ cudaError_t rows(bool store, RowsArgs a, int type, cudaStream_t st) {
   const uintptr_t p0 = (uintptr_t)(store ? a.src[0] : a.dst[0]), p1 = (uintptr_t)(store ? a.src[1] : a.dst[1]);
   a.vec = ((p0 | p1 | (uintptr_t)(a.tok_stride * (long)es) | (uintptr_t)(a.head_stride * (long)es)) & 15) == 0;
   const int rw = 32 / (a.c.head_dim / 8);
-  a.parts = (2 * a.c.n_kv + rw * U - 1) / (rw * U);
+  // U sets a warp, or all where that still gives every SM 48 warps: the
+  // look-ups are then shared by more rows
+  const int all = (a.c.n_kv + rw - 1) / rw;
+  a.sets = U;
+  while (a.sets < all && (long long)a.s.n_tok * ((all + 2 * a.sets - 1) / (2 * a.sets)) >= 148 * 48) a.sets *= 2;
+  a.parts = (all + a.sets - 1) / a.sets;
   const long long warps = (long long)a.s.n_tok * a.parts, blocks = (warps + CT / 32 - 1) / (CT / 32);
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   const dim3 grid((unsigned)blocks);

@@ -57,6 +57,20 @@ __device__ __forceinline__ void store_n(E *p, bool vec, const float (&v)[N]) {
   }
 }
 
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
+
+// Bytes x_i = c_i + 128 in the low and high halves of (1024 + x) f16 words:
+// 0x6400 | x is 1024 + x, and 1152 taken off leaves c exactly.
+__device__ __forceinline__ uint32_t codes_of(uint32_t bytes, uint32_t sel) {
+  return h2u(__hsub2(u2h(__byte_perm(bytes, 0x64646464u, sel)), u2h(0x64806480u)));
+}
+// Nibbles x = c + 8 at bits 0-3 and 16-19: (1024 + x) s - 1032 s = c s, exact.
+__device__ __forceinline__ uint32_t nibbles_of(uint32_t w, uint32_t s, uint32_t m1032s) {
+  return h2u(__hfma2(u2h((w & 0x000f000fu) | 0x64006400u), u2h(s), u2h(m1032s)));
+}
+__device__ __forceinline__ uint32_t dup_h(int s) { return h2u(__half2half2(__int2half_rn(s))); }
+
 // One sequence's bounds, made safe whatever the device arrays hold: rows
 // [first, first + n) of the token arrays, n <= max_new, and committed
 // positions ctx >= 0; total = positions in reach, at most max_len and what

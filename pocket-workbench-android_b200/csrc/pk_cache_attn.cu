@@ -69,8 +69,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // A barrier of n threads (whole warps).
 __device__ __forceinline__ void bar_n(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
-__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2 *>(&u); }
 // (a, b) as two f16 and, for the second term, what the rounding left.
 __device__ __forceinline__ uint32_t pack2(float a, float b) { return h2u(__floats2half2_rn(a, b)); }
 __device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t hi) {
@@ -84,17 +82,6 @@ __device__ __forceinline__ float key_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
 }
-
-// Bytes x_i = c_i + 128 in the low and high halves of (1024 + x) f16 words:
-// 0x6400 | x is 1024 + x, and 1152 taken off leaves c exactly.
-__device__ __forceinline__ uint32_t codes_of(uint32_t bytes, uint32_t sel) {
-  return h2u(__hsub2(u2h(__byte_perm(bytes, 0x64646464u, sel)), u2h(0x64806480u)));
-}
-// Nibbles x = c + 8 at bits 0-3 and 16-19: (1024 + x) s - 1032 s = c s, exact.
-__device__ __forceinline__ uint32_t nibbles_of(uint32_t w, uint32_t s, uint32_t m1032s) {
-  return h2u(__hfma2(u2h((w & 0x000f000fu) | 0x64006400u), u2h(s), u2h(m1032s)));
-}
-__device__ __forceinline__ uint32_t dup_h(int s) { return h2u(__half2half2(__int2half_rn(s))); }
 
 struct AttnKArgs {
   pk_kv_cache c;

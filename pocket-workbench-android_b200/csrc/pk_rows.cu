@@ -32,80 +32,30 @@ cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem,
 // the angle; the remainder's cosine and sine in f32), while the first values
 // are on their way.  An item is V elements (16 bytes where everything is
 // aligned for it): for interleaved pairs a run of a head's dimensions, for
-// the half layout V pairs' two runs, or a run that is copied.
+// the half layout V pairs' two runs, or a run that is copied.  A thread keeps
+// its place in the head and goes from head to head, so its cosines and sines
+// stay in registers and its addresses are additions (with an item's place
+// divided out anew, index arithmetic was half the kernel's instructions).
 constexpr int RT = 256;
 // AL: whole runs, aligned to their size; otherwise moved by elements, the last
-// run of an odd head_dim one short.
-template <int T, int V, bool HALF, bool AL>
-struct alignas(16) RopeItem {
-  using E = elem_t<T>;
-  E a[V], b[HALF ? V : 1];
-  E *out;
-  int i;    // first pair; HALF: -1 for a copied run
-  int len;  // elements
-  template <class X>
-  __device__ __forceinline__ void move(X *dst, const X *src) const {
-    constexpr int B = V * (int)sizeof(X);
-    if (AL && B == 16) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
-    else if (AL && B == 8) *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(src);
-    else if (AL && B == 4) *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(src);
-    else
+// run of an odd head_dim one short (n < V).
+template <int V, bool AL, class X>
+__device__ __forceinline__ void move_run(X *dst, const X *src, int n) {
+  constexpr int B = V * (int)sizeof(X);
+  if (AL && B == 16) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(src);
+  else if (AL && B == 8) *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<const uint2 *>(src);
+  else if (AL && B == 4) *reinterpret_cast<uint32_t *>(dst) = *reinterpret_cast<const uint32_t *>(src);
+  else
 #pragma unroll
-      for (int e = 0; e < V; e++)
-        if (AL || e < len) dst[e] = src[e];
-  }
-  __device__ __forceinline__ void load(const pk_rope_args &p, long long t, int x, int per, int nq) {
-    const int hh = x / per, k = x - hh * per, half = p.n_rot / 2;
-    const bool isk = hh >= nq;
-    const int h = isk ? hh - nq : hh;
-    const E *in = reinterpret_cast<const E *>(isk ? p.k : p.q) + t * (isk ? p.k_tok_stride : p.q_tok_stride) +
-                  h * (isk ? p.k_head_stride : p.q_head_stride);
-    out = reinterpret_cast<E *>(isk ? p.k_out : p.q_out) + t * (isk ? p.ko_tok_stride : p.qo_tok_stride) +
-          h * (isk ? p.ko_head_stride : p.qo_head_stride);
-    len = min(V, p.head_dim - k * V);
-    if (HALF) {
-      len = V;
-      const bool rot = k * V < half;
-      i = rot ? k * V : -1;
-      const int d = rot ? k * V : k * V + half;  // items past the pairs: dimensions n_rot ..
-      out += d;
-      move(a, in + d);
-      if (rot) move(b, in + d + half);
-    } else {
-      i = k * V / 2;
-      out += k * V;
-      move(a, in + k * V);
-    }
-  }
-  __device__ __forceinline__ void finish(const float2 *cs, int half) {
-    if (HALF) {
-      if (i >= 0) {
-#pragma unroll
-        for (int e = 0; e < V; e++) {
-          const float2 c = cs[i + e];
-          const float u = to_f(a[e]), v = to_f(b[e]);
-          a[e] = from_f<E>(u * c.x - v * c.y);
-          b[e] = from_f<E>(u * c.y + v * c.x);
-        }
-        move(out + half, b);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e + 1 < V; e += 2) {
-        if (i + e / 2 >= half) break;
-        const float2 c = cs[i + e / 2];
-        const float u = to_f(a[e]), v = to_f(a[e + 1]);
-        a[e] = from_f<E>(u * c.x - v * c.y);
-        a[e + 1] = from_f<E>(u * c.y + v * c.x);
-      }
-    }
-    move(out, a);
-  }
-};
+    for (int e = 0; e < V; e++)
+      if (AL || e < n) dst[e] = src[e];
+}
 
 template <int T, int V, bool HALF, bool AL>
 __global__ void __launch_bounds__(RT) k_rope(const pk_rope_args p, int heads_cta) {
-  constexpr int N = 4;  // items in flight a thread
+  using E = elem_t<T>;
+  constexpr int N = HALF ? 2 : 3;  // items in flight a thread
+  constexpr int NP = HALF ? V : V / 2;  // pairs of an item
   extern __shared__ float2 cs[];  // [n_rot / 2]
   pdl_trigger();
   pdl_wait();
@@ -113,26 +63,77 @@ __global__ void __launch_bounds__(RT) k_rope(const pk_rope_args p, int heads_cta
   const int half = p.n_rot / 2, nq = p.q ? p.n_head : 0, heads = nq + (p.k ? p.n_kv : 0);
   // items a head: dimensions (interleaved), or pairs and the dimensions past them
   const int per = HALF ? (p.head_dim - half) / V : (p.head_dim + V - 1) / V;
-  const int x0 = (int)blockIdx.y * heads_cta * per, x1 = min(heads, ((int)blockIdx.y + 1) * heads_cta) * per;
-  for (int x = x0; x < x1; x += RT * N) {
-    RopeItem<T, V, HALF, AL> it[N];
+  const int h1 = min(heads, ((int)blockIdx.y + 1) * heads_cta);
+  const int wide = min(per, RT), step = RT / wide;  // threads a head, heads at a time
+  const int row = (int)threadIdx.x / wide;
+  const E *in[2] = {reinterpret_cast<const E *>(p.q) + t * p.q_tok_stride,
+                    reinterpret_cast<const E *>(p.k) + t * p.k_tok_stride - nq * p.k_head_stride};
+  E *out[2] = {reinterpret_cast<E *>(p.q_out) + t * p.qo_tok_stride,
+               reinterpret_cast<E *>(p.k_out) + t * p.ko_tok_stride - nq * p.ko_head_stride};
+  bool first = true;
+  for (int k = (int)threadIdx.x - row * wide; first || k < per; k += wide) {
+    const bool mine = row < step && k < per;
+    const bool rot = HALF ? k * V < half : true;
+    const int d = HALF && !rot ? k * V + half : k * V;  // past the pairs: dimensions n_rot ..
+    const int len = HALF ? V : min(V, p.head_dim - d);
+    float2 c[NP];
+    for (int h = (int)blockIdx.y * heads_cta + row; first || h < h1; h += step * N) {
+      alignas(16) E a[N][V], b[N][HALF ? V : 1];
 #pragma unroll
-    for (int n = 0; n < N; n++)
-      if (x + n * RT + (int)threadIdx.x < x1) it[n].load(p, t, x + n * RT + threadIdx.x, per, nq);
-    if (x == x0) {
-      const double pos = (double)__ldg(p.pos + t);
-      for (int i = threadIdx.x; i < half; i += RT) {
-        double r = pos * __ldg(p.turns + i);
-        r -= rint(r);
-        float s, c;
-        sincospif(2.0f * (float)r, &s, &c);
-        cs[i] = make_float2(c * p.gain, s * p.gain);
+      for (int n = 0; n < N; n++) {
+        const int hh = h + n * step;
+        if (!mine || hh >= h1) continue;
+        const E *x = (hh >= nq ? in[1] + hh * p.k_head_stride : in[0] + hh * p.q_head_stride) + d;
+        move_run<V, AL>(a[n], x, len);
+        if (HALF && rot) move_run<V, AL>(b[n], x + half, len);
       }
-      __syncthreads();
-    }
+      if (first) {
+        first = false;
+        const double pos = (double)__ldg(p.pos + t);
+        for (int i = threadIdx.x; i < half; i += RT) {
+          double r = pos * __ldg(p.turns + i);
+          r -= rint(r);
+          float sn, co;
+          sincospif(2.0f * (float)r, &sn, &co);
+          cs[i] = make_float2(co * p.gain, sn * p.gain);
+        }
+        __syncthreads();
+      }
+      if (!mine) break;
+      if (h < (int)blockIdx.y * heads_cta + step) {
 #pragma unroll
-    for (int n = 0; n < N; n++)
-      if (x + n * RT + (int)threadIdx.x < x1) it[n].finish(cs, half);
+        for (int e = 0; e < NP; e++) {
+          const int i = HALF ? k * V + e : k * V / 2 + e;
+          c[e] = i < half ? cs[i] : make_float2(1.0f, 0.0f);
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < N; n++) {
+        const int hh = h + n * step;
+        if (hh >= h1) continue;
+        E *y = (hh >= nq ? out[1] + hh * p.ko_head_stride : out[0] + hh * p.qo_head_stride) + d;
+        if (HALF) {
+          if (rot) {
+#pragma unroll
+            for (int e = 0; e < V; e++) {
+              const float u = to_f(a[n][e]), v = to_f(b[n][e]);
+              a[n][e] = from_f<E>(u * c[e].x - v * c[e].y);
+              b[n][e] = from_f<E>(u * c[e].y + v * c[e].x);
+            }
+            move_run<V, AL>(y + half, b[n], len);
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e + 1 < V; e += 2) {
+            if (k * V / 2 + e / 2 >= half) break;  // past the pairs: copied as they are
+            const float u = to_f(a[n][e]), v = to_f(a[n][e + 1]);
+            a[n][e] = from_f<E>(u * c[e / 2].x - v * c[e / 2].y);
+            a[n][e + 1] = from_f<E>(u * c[e / 2].y + v * c[e / 2].x);
+          }
+        }
+        move_run<V, AL>(y, a[n], len);
+      }
+    }
   }
 }
 
@@ -161,16 +162,20 @@ cudaError_t rope_type(const pk_rope_args &a, cudaStream_t st) {
 }
 
 // -------------------------------------------------------------- logit rules
-// A CTA takes SEG logits of a row, NT threads.  Its logits are asked for
-// first; then it counts the row's history ids that fall into its segment in
-// shared memory (whole counts: their order does not matter) and collects the
-// biases of the segment there, in the list's order, which one warp adds up;
-// then the segment is finished and written.
+// A CTA takes SEG logits of a row, NT threads.  All that it reads (logits,
+// masks, the first HB NT history ids, the first NT biases, the row's numbers)
+// is asked for at the start, while its counts are cleared, so that it waits
+// for memory once; asked for where it is used, that was five times in a row
+// and 97 us for 250 rows of 128256.  It counts the row's ids that fall into
+// its segment in shared memory (whole counts: their order does not matter)
+// and collects the biases of the segment there, in the list's order, which
+// one warp adds up; then the segment is finished and written.
 template <int T, int SEG, int NT>
 __global__ void __launch_bounds__(NT) k_logit_rules(const void *in, void *out, int n, long in_stride, long out_stride,
                                                     const pk_logit_rules r, int segs, int vec) {
   using E = elem_t<T>;
   constexpr int V = 16 / (int)sizeof(E), RUNS = SEG / (NT * V);  // a thread has runs of V elements
+  constexpr int HB = 6;
   static_assert(RUNS * NT * V == SEG, "whole runs");
   extern __shared__ __align__(16) uint8_t smem[];
   int *cnt = reinterpret_cast<int *>(smem);                             // [SEG], where there is a history
@@ -180,14 +185,19 @@ __global__ void __launch_bounds__(NT) k_logit_rules(const void *in, void *out, i
   __shared__ int bcount[NT / 32];
   pdl_trigger();
   pdl_wait();
-  const long long row = blockIdx.x / segs;
+  const int row = blockIdx.x / segs;
   const int lo = (int)(blockIdx.x - row * segs) * SEG, m = min(SEG, n - lo), tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const E *x = reinterpret_cast<const E *>(in) + row * in_stride + lo;
   E *y = reinterpret_cast<E *>(out) + row * out_stride + lo;
+  const uint32_t *ids = r.hist + row * r.hist_stride;
+  const uint32_t *allow = r.allow ? r.allow + row * r.allow_stride + (lo >> 5) : nullptr;
   alignas(16) E v[RUNS][V];
+  uint32_t ok[RUNS], hid[HB];
 #pragma unroll
   for (int k = 0; k < RUNS; k++) {
     const int i = (k * NT + tid) * V;
+    ok[k] = 0xffffffffu;
+    if (i >= m) continue;
     if (vec && i + V <= m) {
       *reinterpret_cast<uint4 *>(v[k]) = *reinterpret_cast<const uint4 *>(x + i);
     } else {
@@ -195,24 +205,48 @@ __global__ void __launch_bounds__(NT) k_logit_rules(const void *in, void *out, i
       for (int e = 0; e < V; e++)
         if (i + e < m) v[k][e] = x[i + e];
     }
+    if (allow) ok[k] = __ldg(allow + (i >> 5)) >> (i & 31);  // V divides 32
   }
+  int nh = 0;
+  if (r.hist) {
+    nh = r.n_hist ? __ldg(r.n_hist + row) : r.n_hist_max;
+#pragma unroll
+    for (int h = 0; h < HB; h++) {
+      hid[h] = 0xffffffffu;
+      if (h * NT + tid < r.n_hist_max) hid[h] = __ldg(ids + h * NT + tid);
+    }
+  }
+  uint32_t b_id = 0xffffffffu;
+  float b_val = 0.0f;
+  if (r.bias_id && tid < r.n_bias) {
+    b_id = __ldg(r.bias_id + row * r.bias_stride + tid);
+    b_val = __ldg(r.bias + row * r.bias_stride + tid);
+  }
+  const float rep = r.repeat ? __ldg(r.repeat + row) : 1.0f, fr = r.freq ? __ldg(r.freq + row) : 0.0f,
+              pr = r.presence ? __ldg(r.presence + row) : 0.0f;
   const int words = (r.hist ? SEG : 0) + (r.bias_id ? SEG : 0);
   for (int i = tid; i < words / 4; i += NT) reinterpret_cast<uint4 *>(smem)[i] = make_uint4(0, 0, 0, 0);
   __syncthreads();
   if (r.hist) {
-    const uint32_t *ids = r.hist + row * r.hist_stride;
-    const int nh = min(max(r.n_hist ? __ldg(r.n_hist + row) : r.n_hist_max, 0), r.n_hist_max);
-#pragma unroll 4
-    for (int i = tid; i < nh; i += NT) {
+    nh = min(max(nh, 0), r.n_hist_max);
+#pragma unroll
+    for (int h = 0; h < HB; h++) {
+      const uint32_t d = hid[h] - (uint32_t)lo;
+      if (h * NT + tid < nh && d < (uint32_t)m) atomicAdd(&cnt[d], 1);
+    }
+    for (int i = HB * NT + tid; i < nh; i += NT) {
       const uint32_t d = __ldg(ids + i) - (uint32_t)lo;
       if (d < (uint32_t)m) atomicAdd(&cnt[d], 1);
     }
   }
   if (r.bias_id) {
     for (int i0 = 0; i0 < r.n_bias; i0 += NT) {  // (uniform)
-      const int i = i0 + tid;
-      const uint32_t d = i < r.n_bias ? __ldg(r.bias_id + row * r.bias_stride + i) - (uint32_t)lo : 0xffffffffu;
-      const float b = i < r.n_bias ? __ldg(r.bias + row * r.bias_stride + i) : 0.0f;
+      if (i0 > 0) {
+        const int i = i0 + tid;
+        b_id = i < r.n_bias ? __ldg(r.bias_id + row * r.bias_stride + i) : 0xffffffffu;
+        b_val = i < r.n_bias ? __ldg(r.bias + row * r.bias_stride + i) : 0.0f;
+      }
+      const uint32_t d = i0 + tid < r.n_bias ? b_id - (uint32_t)lo : 0xffffffffu;
       const unsigned here = __ballot_sync(0xffffffffu, d < (uint32_t)m);
       if (lane == 0) bcount[warp] = __popc(here);
       __syncthreads();
@@ -224,7 +258,7 @@ __global__ void __launch_bounds__(NT) k_logit_rules(const void *in, void *out, i
       }
       if (d < (uint32_t)m) {
         bid[at] = d;
-        bval[at] = b;
+        bval[at] = b_val;
       }
       __syncthreads();
       if (warp == 0) {
@@ -244,27 +278,35 @@ __global__ void __launch_bounds__(NT) k_logit_rules(const void *in, void *out, i
     }
   }
   __syncthreads();
-  const float rep = r.repeat ? __ldg(r.repeat + row) : 1.0f, fr = r.freq ? __ldg(r.freq + row) : 0.0f,
-              pr = r.presence ? __ldg(r.presence + row) : 0.0f;
-  const uint32_t *allow = r.allow ? r.allow + row * r.allow_stride + (lo >> 5) : nullptr;
 #pragma unroll
   for (int k = 0; k < RUNS; k++) {
     const int i = (k * NT + tid) * V;
     if (i >= m) break;
-    const uint32_t ok = allow ? __ldg(allow + (i >> 5)) >> (i & 31) : 0xffffffffu;  // V divides 32
+    // most runs have no token that was seen or biased
 #pragma unroll
-    for (int e = 0; e < V; e++) {
-      if (i + e >= m) break;
-      float f = to_f(v[k][e]);
-      if (r.hist) {
-        const int c = cnt[i + e];
-        if (c > 0) {
-          f = f > 0.0f ? fdiv(f, rep) : fmul(f, rep);
-          f = fsub(f, fadd(fmul((float)c, fr), pr));
+    for (int q = 0; q < V; q += 4) {
+      int4 c = make_int4(0, 0, 0, 0);
+      float4 b = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (r.hist) c = *reinterpret_cast<const int4 *>(cnt + i + q);
+      if (r.bias_id) b = *reinterpret_cast<const float4 *>(bias + i + q);
+      const int cc[4] = {c.x, c.y, c.z, c.w};
+      const float bb[4] = {b.x, b.y, b.z, b.w};
+      if (c.x | c.y | c.z | c.w | __float_as_int(b.x) | __float_as_int(b.y) | __float_as_int(b.z) | __float_as_int(b.w)) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float f = to_f(v[k][q + e]);
+          if (cc[e] > 0) {
+            f = f > 0.0f ? fdiv(f, rep) : fmul(f, rep);
+            f = fsub(f, fadd(fmul((float)cc[e], fr), pr));
+          }
+          v[k][q + e] = from_f<E>(fadd(f, bb[e]));
         }
       }
-      if (r.bias_id) f = fadd(f, bias[i + e]);
-      v[k][e] = from_f<E>((ok >> e) & 1 ? f : -CUDART_INF_F);
+    }
+    if (allow) {
+#pragma unroll
+      for (int e = 0; e < V; e++)
+        if (!((ok[k] >> e) & 1)) v[k][e] = from_f<E>(-CUDART_INF_F);
     }
     if (vec && i + V <= m) {
       *reinterpret_cast<uint4 *>(y + i) = *reinterpret_cast<const uint4 *>(v[k]);
