@@ -197,7 +197,7 @@ int pk_apply_logit_rules(const void *logits, void *out, int type, int rows, int 
                          int64_t out_stride, const pk_logit_rules *r, void *stream) {
   if (!is_float_type(type)) return set_error(PK_ERR_UNSUPPORTED, "pk_apply_logit_rules: element type " + std::to_string(type) + " is not f32, f16 or bf16");
   if (!r) return bad("pk_apply_logit_rules: null rules");
-  if (rows < 0 || n < 0) return bad("pk_apply_logit_rules: negative size");
+  if (rows < 0 || n < 0 || n > (1 << 30)) return bad("pk_apply_logit_rules: rows is negative or n not within 0 .. 2^30");
   if (rows == 0 || n == 0) return PK_OK;
   if (!logits || !out || (((uintptr_t)logits | (uintptr_t)out) & elem_mask(type))) return bad("pk_apply_logit_rules: null or misaligned logits");
   if (in_stride < 0 || in_stride > (1LL << 40) || out_stride > (1LL << 40) || (rows > 1 && out_stride < n) || out_stride < 0)

@@ -536,7 +536,8 @@ def rules64(x, row, repeat=None, freq=None, presence=None, hist=None, n_hist=Non
 
 
 @pytest.mark.parametrize("ty", list(DT))
-@pytest.mark.parametrize("rows,n,nh,nb", [(1, 1, 1, 1), (3, 31, 5, 2), (2, 2047, 700, 40), (5, 2049, 33, 100), (4, 73448, 3000, 300), (1, 128256, 1, 0)])
+@pytest.mark.parametrize("rows,n,nh,nb", [(1, 1, 1, 1), (3, 31, 5, 2), (2, 2047, 700, 40), (5, 2049, 33, 100), (4, 73448, 3000, 300), (1, 128256, 1, 0),
+                                          (3, 30000, 6000, 900), (2, 9001, 3413, 0), (2, 9001, 3400, 13), (700, 300, 40, 5)])
 def test_logit_rules(pk, ty, rows, n, nh, nb):
     g = gen(rows * n)
     x = randn((rows, n), n, DT[ty], std=4.0)
@@ -563,6 +564,24 @@ def test_logit_rules(pk, ty, rows, n, nh, nb):
             assert ((got[r].double() - want).abs()[~inf] <= lim[~inf]).all()
     same = x.clone()
     assert pk.logit_rules(same, **kw, out=same) is same and torch.equal(same, pk.logit_rules(x, **kw))
+
+
+@pytest.mark.parametrize("n", [61440, 61441, 65536, 128256])
+def test_logit_rules_many_rows(pk, n):
+    """Enough rows that a row is few, long parts: the tokens at the parts' ends and the row's, in place too."""
+    rows = 600
+    x = randn((rows, n), 3)
+    ends = [0, 2047, 2048, 4095, 43007, 43008, 45055, 45056, 61439, 61440, 63487, 63488, 65534, 65535, 65536, n - 2, n - 1]
+    hist = i32([[t for t in ends if t < n] + [n, 2 ** 31 - 1]])
+    pr = torch.rand(rows, generator=gen(1), device="cuda")
+    bias = randn((1, hist.shape[1]), 4)
+    want, total = x.clone(), {}
+    for t, b in zip(hist[0, :-2].tolist(), bias[0]):  # (an id may be twice among the ends)
+        total[t] = total[t] + b if t in total else b
+    for t, b in total.items():
+        want[:, t] = (x[:, t] - pr) + b
+    assert torch.equal(pk.logit_rules(x, presence=pr, hist=hist, bias_id=hist, bias=bias), want)
+    assert torch.equal(pk.logit_rules(x, presence=pr, hist=hist, bias_id=hist, bias=bias, out=x), want)
 
 
 def test_logit_rules_edges(pk):
