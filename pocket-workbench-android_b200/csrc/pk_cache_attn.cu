@@ -30,30 +30,18 @@
 
 #include <algorithm>
 
-#include "pk_cache.cuh"
-#include "pk_cache.h"
+#include "pk_cache_attn.cuh"
 
 namespace pk {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
 constexpr int MIN_CHUNK = 256;
 constexpr int NSTAGE = 4;  // tiles of 16 positions in flight per key group
-// M moves when the maximum passes it by 2^GROW; a row's factor inv is set so
-// that its largest weight times scale is SET and set again past TOP (f16 ends
-// at 65504), so what rounds to a subnormal is below 2^-23 of the largest.
-constexpr float GROW = 6.0f, SET = 512.0f, TOP = 32768.0f;
-
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 // The transpose of an 8 x 8 f16 matrix held two columns a lane.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
@@ -69,51 +57,11 @@ template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // A barrier of n threads (whole warps).
 __device__ __forceinline__ void bar_n(int id, int n) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(n) : "memory"); }
-// (a, b) as two f16 and, for the second term, what the rounding left.
-__device__ __forceinline__ uint32_t pack2(float a, float b) { return h2u(__floats2half2_rn(a, b)); }
-__device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t hi) {
-  const float2 f = __half22float2(u2h(hi));
-  return pack2(a - f.x, b - f.y);
-}
-
 // Over the eight lanes that share two query rows.
 __device__ __forceinline__ float key_max(float v) {
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
   v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-}
-
-struct AttnKArgs {
-  pk_kv_cache c;
-  pk_kv_seqs s;
-  pk_kv_query q;
-  float *part_o;   // [n_tok][n_head][n_chunk][DH]
-  float2 *part_ml; // [n_tok][n_head][n_chunk]
-  int chunk, n_chunk, row_tiles, group, page_shift, vec_q, vec_o;
-};
-
-// A CTA's work: one chunk of positions [lo, hi) for one tile of the rows (token
-// i, query head of kv head h) of one sequence.  Sequences of more than one
-// chunk (nch) leave theirs in the scratch.
-struct Unit {
-  SeqView sv;
-  int s, h, rt, ch, lo, hi, nch, rows;
-};
-__device__ __forceinline__ Unit unit_of(const AttnKArgs &a) {
-  Unit u;
-  unsigned id = blockIdx.x;
-  u.rt = (int)(id % (unsigned)a.row_tiles);
-  id /= (unsigned)a.row_tiles;
-  u.h = (int)(id % (unsigned)a.c.n_kv);
-  id /= (unsigned)a.c.n_kv;
-  u.ch = (int)(id % (unsigned)a.n_chunk);
-  u.s = (int)(id / (unsigned)a.n_chunk);
-  u.sv = seq_view(a.s, a.c.page_size, u.s);
-  u.rows = u.sv.n * a.group;
-  u.nch = (u.sv.total + a.chunk - 1) / a.chunk;
-  u.lo = u.ch * a.chunk;
-  u.hi = min(u.sv.total, u.lo + a.chunk);
-  return u;
 }
 
 // DH / 4 query elements of a row from lane t's quarter, scaled to |q'| < 2;
@@ -156,14 +104,6 @@ __device__ __forceinline__ void load_q_any(const AttnKArgs &a, const Unit &u, in
 template <int TYPE>
 __host__ __device__ constexpr int dim_of(int j, int e) {
   return TYPE == PK_KV_Q8 ? 4 * j + e : 8 * (j / 2) + 2 * (j % 2) + (e / 2) + 4 * (e % 2);
-}
-
-// Does row (token i) see draft j?
-__device__ __forceinline__ bool sees(const AttnKArgs &a, const Unit &u, int i, int j) {
-  if (j >= u.sv.n) return false;
-  if (!a.q.mask) return j <= i;
-  if ((j >> 6) >= a.q.mask_words) return false;
-  return (__ldg(a.q.mask + (size_t)(u.sv.first + i) * a.q.mask_words + (j >> 6)) >> (j & 63)) & 1;
 }
 
 // A tile in shared memory: 16 rows of K codes, 16 of V codes, their scales.
@@ -704,9 +644,12 @@ Variant variant_as() {
   using G = Geo<TYPE, DH, NT, NB, RG>;
   return {k_kv_attn<TYPE, DH, NT, NB, RG>, G::SMEM, G::ROWS};
 }
+// From TC_FROM rows on half-precision queries take the tcgen05 kernel.
+constexpr long long TC_FROM = PK_TCFROM;
 template <int TYPE, int DH, int NT>
 Variant variant_rows(long long rows) {
   constexpr int NBM = NT == 2 && DH == 128 ? 2 : 4;
+  if (NT == 1 && rows >= TC_FROM) return {nullptr, 0, TC_ATTN_ROWS};
   if (rows <= 8) return variant_as<TYPE, DH, NT, 1, 1>();
   if (rows <= 16) return variant_as<TYPE, DH, NT, 2, 1>();
   if (rows <= 8 * NBM) return variant_as<TYPE, DH, NT, NBM, 1>();
@@ -763,8 +706,9 @@ cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_k
   a.part_ml = p.n_chunk > 1 ? reinterpret_cast<float2 *>(a.part_o + rows * p.n_chunk * c.head_dim) : nullptr;
   const long long blocks = (long long)s.n_seq * c.n_kv * p.row_tiles * p.n_chunk, jb = ((long long)rows + 3) / 4;
   if (blocks > 0x7fffffffLL || jb > 0x7fffffffLL) return cudaErrorInvalidValue;
-  cudaError_t e = cudaFuncSetAttribute(v.k, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem);
-  if (e == cudaSuccess) e = launch(v.k, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
+  cudaError_t e;
+  if (!v.k) e = launch_kv_attn_tc(a, (unsigned)blocks, st);
+  else if ((e = cudaFuncSetAttribute(v.k, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem)) == cudaSuccess) e = launch(v.k, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
   if (e != cudaSuccess || p.n_chunk <= 1) return e;
   return launch(c.head_dim == 64 ? k_kv_attn_join<64> : k_kv_attn_join<128>, dim3((unsigned)jb), dim3(128), 0, st, a);
 }

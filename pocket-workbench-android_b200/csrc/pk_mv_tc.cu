@@ -42,6 +42,7 @@
 #include "pk.h"
 #include "pk_device.cuh"
 #include "pk_kernels.h"
+#include "pk_tcgen05.cuh"
 
 namespace pk {
 namespace {
@@ -119,30 +120,6 @@ __host__ __device__ inline TcLayout tc_layout(int nch) {
 
 __device__ int g_tc_err;  // 0 or PK_ERR_TIMEOUT (a bounded wait ran out in some CTA)
 
-__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ unsigned long long gtime_ns() {
-  unsigned long long t;
-  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-  return t;
-}
-__device__ __forceinline__ void mbar_init(uint32_t b, uint32_t n) {
-  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(b), "r"(n) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t b) {
-  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(b) : "memory");
-}
-__device__ __forceinline__ void mbar_expect(uint32_t b, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(b), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ bool mbar_test(uint32_t b, uint32_t parity) {
-  uint32_t ok;
-  asm volatile(
-      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-      : "=r"(ok)
-      : "r"(b), "r"(parity)
-      : "memory");
-  return ok != 0;
-}
 // Bounded wait for phase `parity` of mbarrier b; false on timeout or when
 // another thread of the CTA (*abort) or another CTA (the error word) has
 // given up.
@@ -165,9 +142,6 @@ __device__ __forceinline__ void tma_3d(uint32_t dst, const CUtensorMap *map, int
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void sts128(uint32_t a, uint32_t x, uint32_t y, uint32_t z, uint32_t w) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(x), "r"(y), "r"(z), "r"(w) : "memory");
-}
 __device__ __forceinline__ void sts32(uint32_t a, uint32_t x) {
   asm volatile("st.shared.u32 [%0], %1;" ::"r"(a), "r"(x) : "memory");
 }
@@ -184,13 +158,6 @@ __device__ __forceinline__ bool bar_or_compute(bool v) {
 }
 
 // tcgen05 ------------------------------------------------------------------
-// Shared-memory matrix descriptor, K-major without swizzle: core matrices of
-// 8 rows x 16 bytes (128 contiguous bytes); lbo = bytes between the two
-// 16-byte halves of K, sbo = bytes between groups of 8 rows.
-__device__ __forceinline__ uint64_t tc_desc(uint32_t addr, uint32_t lbo, uint32_t sbo) {
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | ((uint64_t)((lbo >> 4) & 0x3FFFu) << 16) |
-         ((uint64_t)((sbo >> 4) & 0x3FFFu) << 32) | (1ull << 46);  // version 1 (sm_100), no swizzle
-}
 // Issued by the whole of one warp with converged lanes: the descriptors are
 // warp-uniform, and the lane that elect.sync picks (lane 0, the same one each
 // time) issues the MMA and, later, its commit.
@@ -201,15 +168,6 @@ __device__ __forceinline__ void tc_mma(uint32_t d_tmem, uint64_t a, uint64_t b) 
       "l"(a), "l"(b), "r"(TC_IDESC), "r"(0), "r"(0), "r"(0), "r"(0), "r"(0)
       : "memory");
 }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-  asm volatile(
-      "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
-      " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 // 4 consecutive 32-bit TMEM columns of this thread's lane.
 __device__ __forceinline__ void tc_ld4(uint32_t taddr, int (&v)[4]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0,%1,%2,%3}, [%4];"
