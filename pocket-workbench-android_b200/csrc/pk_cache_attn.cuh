@@ -11,8 +11,8 @@ namespace pk {
 constexpr float kLog2e = 1.4426950408889634f;
 // M moves when the maximum passes it by 2^GROW; a row's factor inv is set so
 // that its largest weight times scale is SET and set again past TOP (f16 ends
-// at 65504), so what rounds to a subnormal is below 2^-23 of the largest.
-constexpr float GROW = 6.0f, SET = 512.0f, TOP = 32768.0f;
+// at 65504), so what rounds to a subnormal is below 2^-20 of the largest.
+constexpr float GROW = 6.0f, SET = 64.0f, TOP = 32768.0f;
 
 __device__ __forceinline__ float ex2(float x) {
   float y;

@@ -4,23 +4,27 @@
 //
 // A CTA takes 128 rows (token, query head) of one kv head over one chunk of
 // positions, 64 at a time: S = Q K^T (M 128 x N 64 x K head_dim) into one of
-// two TMEM buffers, weights P, O += P V (M 128 x N head_dim x K 64) in TMEM.
-// 256 threads:
+// two TMEM buffers, weights P in their place, O += P V (M 128 x N head_dim x
+// K 64) in TMEM.  288 threads:
 //   warps 0-3  softmax: thread = row = TMEM lane.  Scores from TMEM, the
 //              scales D^K and D^V applied in f32 (two at a time), weights as
-//              f16 into shared memory.  O stays in TMEM; a row's is scaled
-//              there only when its factor has to change (M grew past 2^100,
-//              or weights would leave f16), which is rare after the first
-//              tiles, and M itself moves by 2^6 at least.
-//   warps 4-7  codes: the next tiles' K and V rows on their way in registers,
-//              made f16 (exact) and put into the operands' layout; warp 4
-//              issues the products.
-// Two CTAs share an SM (96 KB and 256 TMEM columns each), so that one's
+//              f16 into the scores' columns.
+//   warps 4-7  codes: a tile's K and V rows are asked for a tile ahead, made
+//              f16 (exact) and put into the operands' layout.
+//   warp 8     issues the products.
+// Two CTAs share an SM (100 KB and 256 TMEM columns each), so that one's
 // products run beside the other's softmax.  Operands are in the canonical
-// layout without swizzle, core matrices of 8 rows x 16 bytes: 16-byte chunks of
-// consecutive rows are consecutive, and a warp's stores (a lane a row) touch
-// every bank once.  V's rows are stored as K's, which makes it an N-major
-// operand.
+// layout without swizzle, core matrices of 8 rows x 16 bytes.  V's rows are
+// stored as K's, which makes it an N-major operand.
+//
+// A row keeps one reference m for its weights 2^(s - m): they are summed as
+// they are and multiplied by D^V into f16.  It is set so that the row's
+// largest product is 2^6 (f16 ends at 2^16) and stays until a tile's weights
+// could pass f16, which their sum tells, being at least the largest: most
+// tiles need no maximum and leave O as it is.  A tile that does, the first
+// one, and those with masked positions take the long way: the largest score,
+// the largest product, a new reference if needed, the sums and O scaled by
+// 2^(old - new).
 //
 // Every wait is bounded: one that runs out sets the CTA's abort flag, after
 // which no wait waits, and its rows are written as NaN.
@@ -34,28 +38,30 @@ namespace {
 
 constexpr int NK = 64;                      // positions a tile
 constexpr int ROWS = TC_ATTN_ROWS;
-constexpr int SOFT = 128, CONV = 128;       // threads
+constexpr int SOFT = 128, CONV = 128, THREADS = SOFT + CONV + 32;
 constexpr unsigned long long WAIT_NS = 2000000000ull;
 
 template <int DH>
 struct Lay {
-  static constexpr int Q = 0, K = Q + ROWS * DH * 2, V = K + 2 * NK * DH * 2, P = V + NK * DH * 2, SC = P + ROWS * NK * 2;
-  // of two tiles: D^K [NK], D^V [NK]; positions that hold something (2 words), largest and smallest D^V of 32 (2 x 2)
-  static constexpr int SCB = 2 * NK * 4 + 16 + 16, BAR = SC + 2 * SCB, BYTES = BAR + 64;
+  // chunks of 16 bytes (8 dimensions) of consecutive positions; one chunk's
+  // stride is 16 bytes more than its 64 positions, so that the 16 lanes that
+  // store a position's chunks touch every bank once
+  static constexpr int CH = NK * 16 + 16, TILE = DH / 8 * CH;
+  static constexpr int Q = 0, K = Q + ROWS * DH * 2, V = K + 2 * TILE, SC = V + 2 * TILE;
+  // of two tiles: D^K [NK], D^V [NK]; positions that hold something (2 words), largest D^V of 32 (2)
+  static constexpr int SCB = 2 * NK * 4 + 16, BAR = SC + 2 * SCB, BYTES = BAR + 64;
   static constexpr int S_COL = 0, O_COL = 2 * NK, COLS = 256;
 };
 
-__device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity, volatile int *abort) {
-  if (mbar_test(bar, parity)) return true;
-  const unsigned long long t0 = gtime_ns();
-  while (!mbar_test(bar, parity)) {
-    if (*abort) return false;
-    if (gtime_ns() - t0 > WAIT_NS) {
-      *abort = 1;
-      return false;
-    }
+// Waits for phase `parity` of mbarrier bar; called by whole warps, whose lanes
+// leave it together (tcgen05 loads and stores are the whole warp's).
+__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int *abort) {
+  if (!mbar_test(bar, parity)) {
+    const unsigned long long t0 = gtime_ns();
+    while (!mbar_test(bar, parity) && !*abort)
+      if (gtime_ns() - t0 > WAIT_NS) *abort = 1;
   }
-  return true;
+  __syncwarp();
 }
 
 // A descriptor of an operand without swizzle (pk_tcgen05.cuh): K-major a =
@@ -71,7 +77,23 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, bool
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0), "r"(0), "r"(0), "r"(0)
       : "memory");
 }
-// 32 consecutive TMEM columns of this thread's lane.
+// The same with A in TMEM (f16, two a column).
+template <int N, bool BMN>
+__device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, bool acc) {
+  constexpr uint32_t idesc = (1u << 4) | ((BMN ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+  asm volatile(
+      "{\n .reg .pred p, e;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0), "r"(0), "r"(0), "r"(0)
+      : "memory");
+}
+// 16 and 32 consecutive TMEM columns of this thread's lane.
+__device__ __forceinline__ void ld16(uint32_t t, float (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n tcgen05.wait::ld.sync.aligned;"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+               : "r"(t)
+               : "memory");
+}
 __device__ __forceinline__ void ld32(uint32_t t, float (&v)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
@@ -83,14 +105,10 @@ __device__ __forceinline__ void ld32(uint32_t t, float (&v)[32]) {
       : "r"(t)
       : "memory");
 }
-__device__ __forceinline__ void st32(uint32_t t, const float (&v)[32]) {
+__device__ __forceinline__ void st16(uint32_t t, const uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
-      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};\n tcgen05.wait::st.sync.aligned;" ::"r"(t),
-      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]), "f"(v[10]),
-      "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]), "f"(v[19]), "f"(v[20]),
-      "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]), "f"(v[28]), "f"(v[29]), "f"(v[30]),
-      "f"(v[31])
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -121,23 +139,6 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 template <int TYPE>
 __host__ __device__ constexpr int dim8(int i) {
   return TYPE == PK_KV_Q8 ? i : (i / 2) + 4 * (i % 2);
-}
-
-// 16 bytes of a row's codes into 16-byte chunks of f16 at dst, `stride` apart.
-template <int TYPE>
-__device__ __forceinline__ void put_codes(uint32_t dst, uint32_t stride, const uint4 &raw, uint32_t s2, uint32_t m2) {
-  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-  if (TYPE == PK_KV_Q8) {
-#pragma unroll
-    for (int c = 0; c < 2; c++)
-      sts128(dst + c * stride, codes_of(w[2 * c], 0x4140), codes_of(w[2 * c], 0x4342), codes_of(w[2 * c + 1], 0x4140),
-             codes_of(w[2 * c + 1], 0x4342));
-  } else {
-#pragma unroll
-    for (int c = 0; c < 4; c++)
-      sts128(dst + c * stride, nibbles_of(w[c], s2, m2), nibbles_of(w[c] >> 4, s2, m2), nibbles_of(w[c] >> 8, s2, m2),
-             nibbles_of(w[c] >> 12, s2, m2));
-  }
 }
 
 // This thread's query row, scaled to |q'| < 2 and rounded to f16 (exact for
@@ -197,7 +198,7 @@ __device__ __forceinline__ uint64_t seen_by(const AttnKArgs &a, const Unit &u, i
 }
 
 template <int TYPE, int DH>
-__global__ void __launch_bounds__(SOFT + CONV, 2) k_kv_attn_tc(const AttnKArgs a) {
+__global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
   using L = Lay<DH>;
   constexpr int RB = TYPE == PK_KV_Q8 ? DH : DH / 2, SW = TYPE == PK_KV_Q8 ? 1 : 2;
   constexpr int W = RB / 32;  // 16-byte words of half a row
@@ -211,21 +212,22 @@ __global__ void __launch_bounds__(SOFT + CONV, 2) k_kv_attn_tc(const AttnKArgs a
   }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sb = shaddr(smem);
-  // barriers: S full x 2, scales ready x 2, P ready, PV done; the TMEM address; the abort flag
-  const uint32_t bar = sb + L::BAR, sfull = bar, scready = bar + 16, pready = bar + 32, pvdone = bar + 40;
-  volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 52);
+  // barriers: S full x 2, codes and scales ready x 2, P ready, PV done x 2; the TMEM address; the abort flag
+  const uint32_t bar = sb + L::BAR, sfull = bar, kvready = bar + 16, pready = bar + 32, pvdone = bar + 40;
+  volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 60);
   if (tid == 0) {
     mbar_init(sfull, 1);
     mbar_init(sfull + 8, 1);
-    mbar_init(scready, CONV);
-    mbar_init(scready + 8, CONV);
+    mbar_init(kvready, CONV);
+    mbar_init(kvready + 8, CONV);
     mbar_init(pready, SOFT);
     mbar_init(pvdone, 1);
+    mbar_init(pvdone + 8, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 4) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 48), "r"(L::COLS) : "memory");
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 56), "r"(L::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   const int row = tile0 + tid;
@@ -239,253 +241,267 @@ __global__ void __launch_bounds__(SOFT + CONV, 2) k_kv_attn_tc(const AttnKArgs a
   __syncthreads();
   tc_fence_after();
   pdl_trigger();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::BAR + 48);
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::BAR + 56);
   // without a mask nobody sees past the tile's last token
   const int last = (min(tile0 + ROWS, u.rows) - 1) / a.group;
   const int hi = a.q.mask ? u.hi : min(u.hi, u.sv.ctx + last + 1);
   const int nt = hi > u.lo ? (hi - u.lo + NK - 1) / NK : 0;
 
-  if (tid >= SOFT) {  // -------------------------------------------------- codes
-    const int ct = tid - SOFT, key = ct & (NK - 1), half = ct >> 6;
-    uint4 rk[W], rv[W];
-    float2 dk, dv;  // (D, sub-scales)
+  if (warp == 8) {  // ----------------------------------------------- products
+    auto scores = [&](int i) {
+      wait(kvready + 8 * (i & 1), (i >> 1) & 1, abort);
+      tc_fence_after();
+      // (addresses made anew each time: kept across the loop, the descriptors
+      // alone would take most of the registers)
+      uint32_t q = sb + L::Q, k = sb + L::K + (i & 1) * L::TILE, dt = tmem + L::S_COL + (i & 1) * NK;
+      asm volatile("" : "+r"(q), "+r"(k), "+r"(dt));
+#pragma unroll
+      for (int s = 0; s < DH / 16; s++)
+        mma_f16<NK, false>(dt, tc_desc(q + s * 2 * (ROWS * 16), ROWS * 16, 128), tc_desc(k + s * 2 * L::CH, L::CH, 128), s > 0);
+      tc_commit(sfull + 8 * (i & 1));
+    };
+    if (nt > 0) scores(0);
+    for (int i = 0; i < nt; i++) {
+      if (i + 1 < nt) scores(i + 1);  // (into the columns of tile i - 1's weights: products are done in order)
+      wait(pready, i & 1, abort);
+      tc_fence_after();
+      uint32_t w = tmem + L::S_COL + (i & 1) * NK, v = sb + L::V + (i & 1) * L::TILE;
+      asm volatile("" : "+r"(w), "+r"(v));
+#pragma unroll
+      for (int s = 0; s < NK / 16; s++)
+        mma_f16_ts<DH, true>(tmem + L::O_COL, w + s * 8, tc_desc(v + s * 16 * 16, 128, L::CH), i > 0 || s > 0);
+      tc_commit(pvdone + 8 * (i & 1));
+    }
+  } else if (tid >= SOFT) {  // ---------------------------------------- codes
+    // 8 bytes of a row a lane (RL lanes a row), NP passes of 128 / RL rows; a
+    // thread's row of pass w is w * (CONV / RL) + ct / RL
+    constexpr int RL = RB / 8, RP = CONV / RL, NP = NK / RP, CL = TYPE == PK_KV_Q8 ? 1 : 2;  // CL: chunks of 8 bytes
+    const int ct = tid - SOFT, sub = ct % RL, key0 = ct / RL;
+    const int key = ct & (NK - 1), half = ct >> 6;  // whose scale this thread passes on (half 0: K's, 1: V's)
+    uint2 rk[NP], rv[NP];
+    static_assert(TYPE == PK_KV_Q8 || RP >= 16, "a pass of 4-bit rows has whole groups");
+    uint32_t sk[TYPE == PK_KV_Q4 ? NP : 1], sv[TYPE == PK_KV_Q4 ? NP : 1];  // the rows' sub-scales
+    float d = 0.0f;
     bool on = false;
-    auto page_of = [&](int i) {
-      const int p = u.lo + NK * i + key, j = p >> a.page_shift;
-      const int pg = i < nt && p < hi && j < a.s.max_pages ? __ldg(a.s.pages + (size_t)u.s * a.s.max_pages + j) : -1;
-      return pg >= 0 && pg < a.c.n_pages ? pg : -1;
-    };
-    auto row_of = [&](int i, int pg) {
-      const int p = u.lo + NK * i + key;
-      return ((size_t)pg * a.c.n_kv + u.h) * a.c.page_size + (p & (a.c.page_size - 1));
-    };
-    auto ask = [&](uint4(&raw)[W], float2 &d, const void *codes, const float *scales, int i, int pg) {
+    // Lane x of every warp holds, for the next 8 tiles, the cache rows of
+    // positions 16 (x & 3) .. of tile x >> 2, in units of 16 rows (a page is 16
+    // positions or more): -1 where there is no page.  Such rows are read from
+    // the cache's first, whose codes are as good as any (their scales are 0).
+    int rows16 = -1;
+    const uint8_t *kp = reinterpret_cast<const uint8_t *>(a.c.k) + (key0 & 15) * RB + 8 * sub;
+    const uint8_t *vp = reinterpret_cast<const uint8_t *>(a.c.v) + (key0 & 15) * RB + 8 * sub;
+    const uint8_t *ksp = reinterpret_cast<const uint8_t *>(a.c.ks) + ((key0 & 15) * SW + 1) * 4;
+    const uint8_t *vsp = reinterpret_cast<const uint8_t *>(a.c.vs) + ((key0 & 15) * SW + 1) * 4;
+    const uint8_t *dp = reinterpret_cast<const uint8_t *>(half ? a.c.vs : a.c.ks) + (key & 15) * SW * 4;
+    auto ask = [&](int i) {
+      if ((i & 7) == 0) {
+        const int p = u.lo + NK * (i + (lane >> 2)) + 16 * (lane & 3), j = p >> a.page_shift;
+        const int pg = p < hi && j < a.s.max_pages ? __ldg(a.s.pages + (size_t)u.s * a.s.max_pages + j) : -1;
+        rows16 = pg >= 0 && pg < a.c.n_pages
+                     ? (int)((((long long)pg * a.c.n_kv + u.h) * a.c.page_size + (p & (a.c.page_size - 1))) >> 4)
+                     : -1;
+      }
+      constexpr int PG = RP < 16 ? 16 / RP : 1, GP = RP > 16 ? RP / 16 : 1;  // passes a group of 16 rows, groups a pass
 #pragma unroll
-      for (int w = 0; w < W; w++) raw[w] = TYPE == PK_KV_Q8 ? make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u)
-                                                           : make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-      d = make_float2(0.0f, 0.0f);
-      if (pg < 0) return;
-      const size_t r = row_of(i, pg);
-      const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const uint8_t *>(codes) + r * RB) + half * W;
+      for (int w = 0; w < NP; w += PG) {
+        const uint32_t r = max(__shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + w * RP / 16 + (GP > 1 ? key0 / 16 : 0)), 0);
+        const uint8_t *kr = kp + (size_t)r * (16 * RB), *vr = vp + (size_t)r * (16 * RB);
 #pragma unroll
-      for (int w = 0; w < W; w++) raw[w] = __ldg(src + w);
-      if (TYPE == PK_KV_Q8) d.x = __ldg(scales + r);
-      else d = __ldg(reinterpret_cast<const float2 *>(scales) + r);
-    };
-    auto put = [&](uint32_t dst, const uint4(&raw)[W], float2 d) {
-#pragma unroll
-      for (int w = 0; w < W; w++) {
-        constexpr int CW = TYPE == PK_KV_Q8 ? 2 : 4;  // chunks of 16 bytes of codes
-        const int chunk = (half * W + w) * CW;
-        uint32_t s2 = 0, m2 = 0;
-        if (TYPE == PK_KV_Q4) {  // 16 bytes are 32 dimensions: one sub-scale
-          const int s = (int)((__float_as_uint(d.y) >> (4 * (half * W + w))) & 15u);
-          s2 = dup_h(s);
-          m2 = dup_h(-1032 * s);
+        for (int x = 0; x < PG; x++) {
+          rk[w + x] = __ldg(reinterpret_cast<const uint2 *>(kr + x * RP * RB));
+          rv[w + x] = __ldg(reinterpret_cast<const uint2 *>(vr + x * RP * RB));
         }
-        put_codes<TYPE>(dst + chunk * (NK * 16) + key * 16, NK * 16, raw[w], s2, m2);
+        if (TYPE == PK_KV_Q4) {  // (PG is 1)
+          sk[TYPE == PK_KV_Q4 ? w : 0] = __ldg(reinterpret_cast<const uint32_t *>(ksp + (size_t)r * (16 * SW * 4)));
+          sv[TYPE == PK_KV_Q4 ? w : 0] = __ldg(reinterpret_cast<const uint32_t *>(vsp + (size_t)r * (16 * SW * 4)));
+        }
+      }
+      const int r = __shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + key / 16);
+      on = r >= 0 && u.lo + NK * i + key < hi;
+      d = __ldg(reinterpret_cast<const float *>(dp + (size_t)max(r, 0) * (16 * SW * 4)));
+    };
+    auto put = [&](uint32_t dst, const uint2(&raw)[NP], const uint32_t *subs) {
+#pragma unroll
+      for (int w = 0; w < NP; w++) {
+        const uint32_t at = dst + sub * CL * L::CH + (w * RP + key0) * 16;
+        if (TYPE == PK_KV_Q8) {
+          sts128(at, codes_of(raw[w].x, 0x4140), codes_of(raw[w].x, 0x4342), codes_of(raw[w].y, 0x4140), codes_of(raw[w].y, 0x4342));
+        } else {
+          const int s = (int)((subs[w] >> (4 * (sub / 2))) & 15u);
+          const uint32_t s2 = dup_h(s), m2 = dup_h(-1032 * s);
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            const uint32_t x = c ? raw[w].y : raw[w].x;
+            sts128(at + c * L::CH, nibbles_of(x, s2, m2), nibbles_of(x >> 4, s2, m2), nibbles_of(x >> 8, s2, m2), nibbles_of(x >> 12, s2, m2));
+          }
+        }
       }
     };
-    // K's codes and both scales of tile i, and the tile's summary
-    auto put_k = [&](int i) {
-      const int b = i & 1;
-      put(sb + L::K + b * (NK * DH * 2), rk, dk);
-      uint8_t *sc = smem + L::SC + b * L::SCB;
+    // both scales of tile i and the tile's summary
+    auto put_scales = [&](int i) {
+      uint8_t *sc = smem + L::SC + (i & 1) * L::SCB;
+      reinterpret_cast<float *>(sc)[half * NK + key] = on ? d : 0.0f;
       if (half == 0) {
-        reinterpret_cast<float *>(sc)[key] = dk.x;
         const unsigned m = __ballot_sync(0xffffffffu, on);
         if (lane == 0) reinterpret_cast<uint32_t *>(sc + 2 * NK * 4)[key >> 5] = m;
       } else {
-        reinterpret_cast<float *>(sc)[NK + key] = dv.x;
-        const uint32_t hi_v = __reduce_max_sync(0xffffffffu, __float_as_uint(dv.x) & 0x7fffffffu);
-        const uint32_t lo_v = __reduce_min_sync(0xffffffffu, dv.x > 0.0f ? __float_as_uint(dv.x) : 0x7f800000u);
-        if (lane == 0) {
-          reinterpret_cast<uint32_t *>(sc + 2 * NK * 4 + 16)[key >> 5] = hi_v;
-          reinterpret_cast<uint32_t *>(sc + 2 * NK * 4 + 24)[key >> 5] = lo_v;
-        }
+        const uint32_t x = __reduce_max_sync(0xffffffffu, on ? __float_as_uint(d) & 0x7fffffffu : 0);
+        if (lane == 0) reinterpret_cast<uint32_t *>(sc + 2 * NK * 4 + 8)[key >> 5] = x;
       }
-      mbar_arrive(scready + 8 * b);
     };
-    int pg = page_of(0), next = page_of(1);
-    ask(rk, dk, a.c.k, a.c.ks, 0, pg);
-    ask(rv, dv, a.c.v, a.c.vs, 0, pg);
-    on = pg >= 0;
-    if (nt > 0) {
-      put_k(0);
-      put(sb + L::V, rv, dv);
-      // from here rk, dk hold tile i + 1's K during iteration i, rv, dv its V
-      pg = next;
-      next = page_of(2);
-      ask(rk, dk, a.c.k, a.c.ks, 1, pg);
-      ask(rv, dv, a.c.v, a.c.vs, 1, pg);
-      on = pg >= 0;
-    }
-    auto scores = [&](int i) {  // warp 4
-      const uint32_t k = sb + L::K + (i & 1) * (NK * DH * 2), d = tmem + L::S_COL + (i & 1) * NK;
-#pragma unroll
-      for (int s = 0; s < DH / 16; s++)
-        mma_f16<NK, false>(d, tc_desc(sb + L::Q + s * 2 * (ROWS * 16), ROWS * 16, 128), tc_desc(k + s * 2 * (NK * 16), NK * 16, 128), s > 0);
-      tc_commit(sfull + 8 * (i & 1));
-    };
-    if (nt > 0) {
-      fence_async_smem();
-      asm volatile("bar.sync 1, %0;" ::"n"(CONV) : "memory");
-      if (warp == 4) {
-        tc_fence_after();
-        scores(0);
-      }
-    }
+    if (nt > 0) ask(0);
     for (int i = 0; i < nt; i++) {
-      if (i + 1 < nt) put_k(i + 1);
+      if (i >= 2) wait(sfull + 8 * (i & 1), ((i - 2) >> 1) & 1, abort);  // K of tile i - 2 has been used
+      put(sb + L::K + (i & 1) * L::TILE, rk, sk);
+      if (i >= 2) wait(pvdone + 8 * (i & 1), ((i - 2) >> 1) & 1, abort);  // and its V and scales
+      put_scales(i);
+      put(sb + L::V + (i & 1) * L::TILE, rv, sv);
       fence_async_smem();
-      asm volatile("bar.sync 1, %0;" ::"n"(CONV) : "memory");
-      if (warp == 4) {
-        if (i + 1 < nt) scores(i + 1);
-        wait(pready, i & 1, abort);
-        tc_fence_after();
-#pragma unroll
-        for (int s = 0; s < NK / 16; s++)
-          mma_f16<DH, true>(tmem + L::O_COL, tc_desc(sb + L::P + s * 2 * (ROWS * 16), ROWS * 16, 128),
-                            tc_desc(sb + L::V + s * 16 * 16, 128, NK * 16), i > 0 || s > 0);
-        tc_commit(pvdone);
-      }
-      if (i + 1 < nt) {
-        // tile i + 2's K may be asked for; V's registers are free once tile i + 1's is stored
-        const int pg2 = next;
-        next = page_of(i + 3);
-        ask(rk, dk, a.c.k, a.c.ks, i + 2, pg2);
-        wait(pvdone, i & 1, abort);
-        put(sb + L::V, rv, dv);
-        ask(rv, dv, a.c.v, a.c.vs, i + 2, pg2);
-        on = pg2 >= 0;
-      }
+      mbar_arrive(kvready + 8 * (i & 1));
+      if (i + 1 < nt) ask(i + 1);
     }
   } else {  // ------------------------------------------------------------ softmax
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const bool work = tile0 + warp * 32 < u.rows;  // (the whole warp)
     const int tok = min(row, u.rows - 1) / a.group;
-    float m = -CUDART_INF_F, l = 0.0f, inv = 0x1p100f;
+    float m = -CUDART_INF_F, l = 0.0f;
+    const float2 rs2 = make_float2(rs, rs);
+    auto pv_wait = [&](int i) { wait(pvdone + 8 * (i & 1), (i >> 1) & 1, abort); };
     // O's row times f, once the products before are done (i > 0)
     auto scale_o = [&](int i, float f) {
       if (i == 0) return;
-      wait(pvdone, (i - 1) & 1, abort);
+      pv_wait(i - 1);
       tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < DH / 16; c++) {
+        float v[16];
+        __syncwarp();
+        ld16(tmem + lanes + L::O_COL + 16 * c, v);
 #pragma unroll
-      for (int c = 0; c < DH / 32; c++) {
-        float v[32];
-        ld32(tmem + lanes + L::O_COL + 32 * c, v);
-#pragma unroll
-        for (int j = 0; j < 32; j++) v[j] *= f;
-        st32(tmem + lanes + L::O_COL + 32 * c, v);
+        for (int j = 0; j < 16; j++) v[j] *= f;
+        st16(tmem + lanes + L::O_COL + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(v));
       }
     };
     for (int i = 0; i < nt; i++) {
       const int b = i & 1, p0 = u.lo + NK * i;
-      wait(scready + 8 * b, (i >> 1) & 1, abort);
+      wait(kvready + 8 * b, (i >> 1) & 1, abort);
       wait(sfull + 8 * b, (i >> 1) & 1, abort);
       tc_fence_after();
       if (work) {
         const uint8_t *sc = smem + L::SC + b * L::SCB;
         const float4 *dk4 = reinterpret_cast<const float4 *>(sc), *dv4 = reinterpret_cast<const float4 *>(sc + NK * 4);
-        const uint64_t held = *reinterpret_cast<const uint64_t *>(sc + 2 * NK * 4);
-        const uint4 r4 = *reinterpret_cast<const uint4 *>(sc + 2 * NK * 4 + 16);
-        const float vmax = fmaxf(__uint_as_float(r4.x), __uint_as_float(r4.y)), vmin = fminf(__uint_as_float(r4.z), __uint_as_float(r4.w));
+        const uint4 r4 = *reinterpret_cast<const uint4 *>(sc + 2 * NK * 4);
+        const uint64_t held = (uint64_t)r4.y << 32 | r4.x;
+        const float vmax = fmaxf(__uint_as_float(r4.z), __uint_as_float(r4.w));
         const bool masked = p0 + NK > min(u.sv.ctx, hi) || held != ~0ull;
-        // per weight where scales differ so much that the largest says little about the others
-        const bool each = masked || !(vmax <= 65536.0f * vmin);
-        float t[NK];
-        ld32(tmem + lanes + L::S_COL + NK * b, reinterpret_cast<float(&)[32]>(t[0]));
-        ld32(tmem + lanes + L::S_COL + NK * b + 32, reinterpret_cast<float(&)[32]>(t[32]));
+        const uint32_t cols = tmem + lanes + L::S_COL + NK * b;
+        float t[32];
         float2 *t2 = reinterpret_cast<float2 *>(t);
+        auto scores = [&](int c) {  // D^K q'.c of positions 32 c ..
+          __syncwarp();
+          ld32(cols + 32 * c, t);
 #pragma unroll
-        for (int j = 0; j < NK / 4; j++) {
-          const float4 d = dk4[j];
-          t2[2 * j] = mul2(t2[2 * j], make_float2(d.x, d.y));
-          t2[2 * j + 1] = mul2(t2[2 * j + 1], make_float2(d.z, d.w));
-        }
-        uint64_t vis = ~0ull;
-        if (masked) {
-          vis = held & (row < u.rows ? seen_by(a, u, tok, p0, hi) : 0);
+          for (int j = 0; j < 8; j++) {
+            const float4 d = dk4[8 * c + j];
+            t2[2 * j] = mul2(t2[2 * j], make_float2(d.x, d.y));
+            t2[2 * j + 1] = mul2(t2[2 * j + 1], make_float2(d.z, d.w));
+          }
+        };
+        uint32_t w[2][16];
+        float2 sum[2];
+        auto weights = [&](int c, uint32_t seen) {  // of the scores in t
+          const float2 mu2 = make_float2(-m, -m);
 #pragma unroll
-          for (int j = 0; j < NK; j++)
-            if (!((vis >> j) & 1)) t[j] = -CUDART_INF_F;
-        }
-        float mx = t[0];
+          for (int j = 0; j < 8; j++) {
+            const float4 d = dv4[8 * c + j];
 #pragma unroll
-        for (int j = 1; j < NK; j++) mx = fmaxf(mx, t[j]);
-        mx *= rs;
-        float f = 1.0f;  // O's factor
-        if (mx > m + GROW) {
-          l *= ex2(m - mx);
-          const float g = inv * ex2(mx - m);
-          m = mx;
-          inv = fminf(g, 0x1p100f);
-          if (g > 0x1p100f) f = 0x1p100f / g;
-        }
-        const float mu = m == -CUDART_INF_F ? 0.0f : m;
-        const float2 rs2 = make_float2(rs, rs), mu2 = make_float2(-mu, -mu);
-        float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int j = 0; j < NK / 2; j++) {
-          t2[j] = fma2(t2[j], rs2, mu2);
-          t2[j].x = ex2(t2[j].x);
-          t2[j].y = ex2(t2[j].y);
-          sum = add2(sum, t2[j]);
-        }
-        l += sum.x + sum.y;
-        float top = ex2(mx - mu) * vmax;  // at least the largest weight times scale
-        if (each) {
-          top = 0.0f;
-#pragma unroll
-          for (int j = 0; j < NK / 4; j++) {
-            const float4 d = dv4[j];
-            const float dd[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-              t[4 * j + e] = (vis >> (4 * j + e)) & 1 ? t[4 * j + e] * dd[e] : 0.0f;
-              top = fmaxf(top, t[4 * j + e]);
+            for (int e = 0; e < 2; e++) {
+              float2 x = fma2(t2[2 * j + e], rs2, mu2);
+              x.x = ex2(x.x);
+              x.y = ex2(x.y);
+              if (seen != 0xffffffffu) {
+                if (!((seen >> (4 * j + 2 * e)) & 1)) x.x = 0.0f;
+                if (!((seen >> (4 * j + 2 * e + 1)) & 1)) x.y = 0.0f;
+              }
+              sum[e] = add2(sum[e], x);
+              x = mul2(x, e ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
+              if (seen != 0xffffffffu) {  // (a scale that is not seen may be anything)
+                if (!((seen >> (4 * j + 2 * e)) & 1)) x.x = 0.0f;
+                if (!((seen >> (4 * j + 2 * e + 1)) & 1)) x.y = 0.0f;
+              }
+              w[c][2 * j + e] = pack2(x.x, x.y);
             }
           }
-        }
-        if (top * inv > TOP) {
-          const float now = SET / fmaxf(top, 0x1p-100f);
-          f *= now / inv;
-          inv = now;
-        }
-        if (__any_sync(0xffffffffu, f != 1.0f)) scale_o(i, f);
-        const float2 inv2 = make_float2(inv, inv);
-        if (i > 0) wait(pvdone, (i - 1) & 1, abort);  // P's memory is free
+        };
+        bool longer = masked;
+        if (!masked) {
+          sum[0] = sum[1] = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int c = 0; c < NK / 8; c++) {
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 2; j++) {
-            float2 x0 = mul2(t2[4 * c + 2 * j], inv2), x1 = mul2(t2[4 * c + 2 * j + 1], inv2);
-            if (!each) {
-              const float4 d = dv4[2 * c + j];
-              x0 = mul2(x0, make_float2(d.x, d.y));
-              x1 = mul2(x1, make_float2(d.z, d.w));
-            }
-            w[2 * j] = pack2(x0.x, x0.y);
-            w[2 * j + 1] = pack2(x1.x, x1.y);
+          for (int c = 0; c < 2; c++) {
+            scores(c);
+            weights(c, 0xffffffffu);
           }
-          sts128(sb + L::P + c * (ROWS * 16) + tid * 16, w[0], w[1], w[2], w[3]);
+          const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          longer = __any_sync(0xffffffffu, !(all * vmax <= TOP && all <= 0x1p100f));  // (m is -inf at first: infinite)
+          if (!longer) l += all;
         }
-        fence_async_smem();
-      } else if (i > 0) {
-        wait(pvdone, (i - 1) & 1, abort);  // else a warp without rows could arrive twice in one phase
+        if (longer) {
+          const uint64_t vis = !masked ? ~0ull : row < u.rows ? held & seen_by(a, u, tok, p0, hi) : 0;
+          float mx = -CUDART_INF_F, top = 0.0f;
+#pragma unroll 1
+          for (int c = 0; c < 2; c++) {
+            scores(c);
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+              if ((vis >> (32 * c + j)) & 1) mx = fmaxf(mx, t[j]);
+          }
+          mx *= rs;
+          // (every lane goes through the loads from TMEM, rows that see nothing too)
+          const float *dv = reinterpret_cast<const float *>(dv4);
+#pragma unroll 1
+          for (int c = 0; c < 2; c++) {
+            scores(c);
+#pragma unroll
+            for (int j = 0; j < 32; j++)
+              if ((vis >> (32 * c + j)) & 1) top = fmaxf(top, ex2(fmaf(t[j], rs, -mx)) * dv[32 * c + j]);
+          }
+          float f = 1.0f;
+          const float most = mx + log2f(fmaxf(top, 0x1p-100f));  // the largest product's exponent
+          if (mx != -CUDART_INF_F && (m == -CUDART_INF_F || most > m + 8.0f || mx > m + 90.0f)) {
+            const float now = fmaxf(most - 6.0f, mx - 90.0f);
+            f = ex2(m - now);
+            l *= f;
+            m = now;
+          }
+          if (__any_sync(0xffffffffu, f != 1.0f)) scale_o(i, f);
+          sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+          const float keep = m;
+          if (m == -CUDART_INF_F) m = 0.0f;  // (nothing seen yet: every weight is masked)
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            scores(c);
+            weights(c, (uint32_t)(vis >> (32 * c)));
+          }
+          m = keep;
+          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+        }
+        __syncwarp();
+        st16(cols, w[0]);  // the weights take their scores' columns, two a column
+        st16(cols + 16, w[1]);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       }
+      if (i > 0) pv_wait(i - 1);  // else a warp that is ahead could arrive twice in one phase
       tc_fence_before();
       mbar_arrive(pready);
     }
     // ---- the rows
-    if (nt > 0) wait(pvdone, (nt - 1) & 1, abort);
+    if (nt > 0) pv_wait(nt - 1);
     tc_fence_after();
     if (work) {
       const int i = tok, h = u.h * a.group + (min(row, u.rows - 1) - i * a.group);
       const long long at = u.sv.first + i;
       const bool on = row < u.rows, part = u.nch > 1;
-      float f = 1.0f / inv;
+      float f = 1.0f;
       if (*abort) f = l = CUDART_NAN_F;
       if (part) {
         if (on) a.part_ml[(at * a.q.n_head + h) * a.n_chunk + u.ch] = make_float2(m, l);
@@ -498,15 +514,15 @@ __global__ void __launch_bounds__(SOFT + CONV, 2) k_kv_attn_tc(const AttnKArgs a
 #pragma unroll
       for (int c = 0; c < DH / 32; c++) {
         float v[32];
+        __syncwarp();
         if (nt > 0) {
           ld32(tmem + lanes + L::O_COL + 32 * c, v);
         } else {
 #pragma unroll
           for (int j = 0; j < 32; j++) v[j] = 0.0f;
         }
-        if (!on) continue;
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
+        for (int k = 0; k < 4 && on; k++) {
           float x[8];
 #pragma unroll
           for (int j = 0; j < 8; j++) x[dim8<TYPE>(j)] = f == 0.0f ? 0.0f : v[8 * k + j] * f;
@@ -520,7 +536,7 @@ __global__ void __launch_bounds__(SOFT + CONV, 2) k_kv_attn_tc(const AttnKArgs a
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::COLS) : "memory");
   }
@@ -536,7 +552,7 @@ cudaError_t launch_kv_attn_tc(const AttnKArgs &a, unsigned blocks, cudaStream_t 
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(SOFT + CONV);
+  cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at{};
