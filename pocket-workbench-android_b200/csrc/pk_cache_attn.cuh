@@ -26,6 +26,13 @@ __device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t hi) {
   return pack2(a - f.x, b - f.y);
 }
 
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 struct AttnKArgs {
   pk_kv_cache c;
   pk_kv_seqs s;

@@ -47,9 +47,11 @@ struct Lay {
   // stride is 16 bytes more than its 64 positions, so that the 16 lanes that
   // store a position's chunks touch every bank once
   static constexpr int CH = NK * 16 + 16, TILE = DH / 8 * CH;
-  static constexpr int Q = 0, K = Q + ROWS * DH * 2, V = K + 2 * TILE, SC = V + 2 * TILE;
-  // of two tiles: D^K [NK], D^V [NK]; positions that hold something (2 words), largest D^V of 32 (2)
-  static constexpr int SCB = 2 * NK * 4 + 16, BAR = SC + 2 * SCB, BYTES = BAR + 64;
+  static constexpr int Q = 0, K = Q + ROWS * DH * 2, V = K + 2 * TILE, RAW = V + TILE;
+  // codes in flight, K's and V's, 16 bytes a thread and pass
+  static constexpr int RAWB = NK * DH, SC = RAW + 2 * RAWB;
+  // of three tiles: D^K [NK], D^V [NK]; positions that hold something (2 words), largest D^V of 32 (2)
+  static constexpr int SCB = 2 * NK * 4 + 16, BAR = SC + 3 * SCB, BYTES = BAR + 96;
   static constexpr int S_COL = 0, O_COL = 2 * NK, COLS = 256;
 };
 
@@ -212,22 +214,22 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
   }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sb = shaddr(smem);
-  // barriers: S full x 2, codes and scales ready x 2, P ready, PV done x 2; the TMEM address; the abort flag
-  const uint32_t bar = sb + L::BAR, sfull = bar, kvready = bar + 16, pready = bar + 32, pvdone = bar + 40;
-  volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 60);
+  // barriers: S full x 2, K and scales ready x 4, P ready, PV done x 2, V ready; the TMEM address; the abort flag
+  const uint32_t bar = sb + L::BAR, sfull = bar, kready = bar + 16, pready = bar + 48, pvdone = bar + 56, vready = bar + 72;
+  volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 84);
   if (tid == 0) {
     mbar_init(sfull, 1);
     mbar_init(sfull + 8, 1);
-    mbar_init(kvready, CONV);
-    mbar_init(kvready + 8, CONV);
+    for (int i = 0; i < 4; i++) mbar_init(kready + 8 * i, CONV);
     mbar_init(pready, SOFT);
+    mbar_init(vready, CONV);
     mbar_init(pvdone, 1);
     mbar_init(pvdone + 8, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 56), "r"(L::COLS) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 80), "r"(L::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   const int row = tile0 + tid;
@@ -241,7 +243,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
   __syncthreads();
   tc_fence_after();
   pdl_trigger();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::BAR + 56);
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::BAR + 80);
   // without a mask nobody sees past the tile's last token
   const int last = (min(tile0 + ROWS, u.rows) - 1) / a.group;
   const int hi = a.q.mask ? u.hi : min(u.hi, u.sv.ctx + last + 1);
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
 
   if (warp == 8) {  // ----------------------------------------------- products
     auto scores = [&](int i) {
-      wait(kvready + 8 * (i & 1), (i >> 1) & 1, abort);
+      wait(kready + 8 * (i & 3), (i >> 2) & 1, abort);
       tc_fence_after();
       // (addresses made anew each time: kept across the loop, the descriptors
       // alone would take most of the registers)
@@ -263,9 +265,10 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     if (nt > 0) scores(0);
     for (int i = 0; i < nt; i++) {
       if (i + 1 < nt) scores(i + 1);  // (into the columns of tile i - 1's weights: products are done in order)
+      wait(vready, i & 1, abort);
       wait(pready, i & 1, abort);
       tc_fence_after();
-      uint32_t w = tmem + L::S_COL + (i & 1) * NK, v = sb + L::V + (i & 1) * L::TILE;
+      uint32_t w = tmem + L::S_COL + (i & 1) * NK, v = sb + L::V;
       asm volatile("" : "+r"(w), "+r"(v));
 #pragma unroll
       for (int s = 0; s < NK / 16; s++)
@@ -273,14 +276,17 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
       tc_commit(pvdone + 8 * (i & 1));
     }
   } else if (tid >= SOFT) {  // ---------------------------------------- codes
-    // 8 bytes of a row a lane (RL lanes a row), NP passes of 128 / RL rows; a
-    // thread's row of pass w is w * (CONV / RL) + ct / RL
-    constexpr int RL = RB / 8, RP = CONV / RL, NP = NK / RP, CL = TYPE == PK_KV_Q8 ? 1 : 2;  // CL: chunks of 8 bytes
+    // 16 bytes of a row a lane (RL lanes a row), NP passes of RP rows; a
+    // thread's row of pass w is w * RP + ct / RL.  The codes come by
+    // asynchronous copies into a place of the thread's own, from which it
+    // reads them back (left in registers, they tied up the loop: the loads of
+    // K and V wait for one another there).
+    constexpr int RL = RB / 16, RP = CONV / RL, NP = NK / RP;
     const int ct = tid - SOFT, sub = ct % RL, key0 = ct / RL;
     const int key = ct & (NK - 1), half = ct >> 6;  // whose scale this thread passes on (half 0: K's, 1: V's)
-    uint2 rk[NP], rv[NP];
-    static_assert(TYPE == PK_KV_Q8 || RP >= 16, "a pass of 4-bit rows has whole groups");
+    static_assert(RP % 16 == 0, "a pass has whole groups of 16 rows");
     uint32_t sk[TYPE == PK_KV_Q4 ? NP : 1], sv[TYPE == PK_KV_Q4 ? NP : 1];  // the rows' sub-scales
+    const uint32_t rawk = sb + L::RAW + ct * 16, rawv = rawk + L::RAWB;
     float d = 0.0f;
     bool on = false;
     // Lane x of every warp holds, for the next 8 tiles, the cache rows of
@@ -288,58 +294,60 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     // positions or more): -1 where there is no page.  Such rows are read from
     // the cache's first, whose codes are as good as any (their scales are 0).
     int rows16 = -1;
-    const uint8_t *kp = reinterpret_cast<const uint8_t *>(a.c.k) + (key0 & 15) * RB + 8 * sub;
-    const uint8_t *vp = reinterpret_cast<const uint8_t *>(a.c.v) + (key0 & 15) * RB + 8 * sub;
+    const uint8_t *kp = reinterpret_cast<const uint8_t *>(a.c.k) + (key0 & 15) * RB + 16 * sub;
+    const uint8_t *vp = reinterpret_cast<const uint8_t *>(a.c.v) + (key0 & 15) * RB + 16 * sub;
     const uint8_t *ksp = reinterpret_cast<const uint8_t *>(a.c.ks) + ((key0 & 15) * SW + 1) * 4;
     const uint8_t *vsp = reinterpret_cast<const uint8_t *>(a.c.vs) + ((key0 & 15) * SW + 1) * 4;
     const uint8_t *dp = reinterpret_cast<const uint8_t *>(half ? a.c.vs : a.c.ks) + (key & 15) * SW * 4;
-    auto ask = [&](int i) {
-      if ((i & 7) == 0) {
-        const int p = u.lo + NK * (i + (lane >> 2)) + 16 * (lane & 3), j = p >> a.page_shift;
-        const int pg = p < hi && j < a.s.max_pages ? __ldg(a.s.pages + (size_t)u.s * a.s.max_pages + j) : -1;
-        rows16 = pg >= 0 && pg < a.c.n_pages
-                     ? (int)((((long long)pg * a.c.n_kv + u.h) * a.c.page_size + (p & (a.c.page_size - 1))) >> 4)
-                     : -1;
-      }
-      constexpr int PG = RP < 16 ? 16 / RP : 1, GP = RP > 16 ? RP / 16 : 1;  // passes a group of 16 rows, groups a pass
+    auto look = [&](int i) {  // before tile i is asked for
+      if (i & 7) return;
+      const int p = u.lo + NK * (i + (lane >> 2)) + 16 * (lane & 3), j = p >> a.page_shift;
+      const int pg = p < hi && j < a.s.max_pages ? __ldg(a.s.pages + (size_t)u.s * a.s.max_pages + j) : -1;
+      rows16 = pg >= 0 && pg < a.c.n_pages
+                   ? (int)((((long long)pg * a.c.n_kv + u.h) * a.c.page_size + (p & (a.c.page_size - 1))) >> 4)
+                   : -1;
+    };
+    auto ask = [&](int i, uint32_t raw, uint32_t *subs, const uint8_t *codes, const uint8_t *scales) {
 #pragma unroll
-      for (int w = 0; w < NP; w += PG) {
-        const uint32_t r = max(__shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + w * RP / 16 + (GP > 1 ? key0 / 16 : 0)), 0);
-        const uint8_t *kr = kp + (size_t)r * (16 * RB), *vr = vp + (size_t)r * (16 * RB);
-#pragma unroll
-        for (int x = 0; x < PG; x++) {
-          rk[w + x] = __ldg(reinterpret_cast<const uint2 *>(kr + x * RP * RB));
-          rv[w + x] = __ldg(reinterpret_cast<const uint2 *>(vr + x * RP * RB));
-        }
-        if (TYPE == PK_KV_Q4) {  // (PG is 1)
-          sk[TYPE == PK_KV_Q4 ? w : 0] = __ldg(reinterpret_cast<const uint32_t *>(ksp + (size_t)r * (16 * SW * 4)));
-          sv[TYPE == PK_KV_Q4 ? w : 0] = __ldg(reinterpret_cast<const uint32_t *>(vsp + (size_t)r * (16 * SW * 4)));
-        }
+      for (int w = 0; w < NP; w++) {
+        const uint32_t r = max(__shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + w * (RP / 16) + key0 / 16), 0);
+        cp16(raw + w * (CONV * 16), codes + (size_t)r * (16 * RB));
+        if (TYPE == PK_KV_Q4) subs[w] = __ldg(reinterpret_cast<const uint32_t *>(scales + (size_t)r * (16 * SW * 4)));
       }
+      cp_commit();
+    };
+    auto ask_scale = [&](int i) {
       const int r = __shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + key / 16);
       on = r >= 0 && u.lo + NK * i + key < hi;
       d = __ldg(reinterpret_cast<const float *>(dp + (size_t)max(r, 0) * (16 * SW * 4)));
     };
-    auto put = [&](uint32_t dst, const uint2(&raw)[NP], const uint32_t *subs) {
+    auto put = [&](uint32_t dst, uint32_t raw, const uint32_t *subs) {
+      cp_wait<1>();  // (K's and V's copies take turns: all but the latest have landed)
 #pragma unroll
       for (int w = 0; w < NP; w++) {
-        const uint32_t at = dst + sub * CL * L::CH + (w * RP + key0) * 16;
+        const uint4 x = sld_v4(raw + w * (CONV * 16));
+        const uint32_t at = dst + (w * RP + key0) * 16;
         if (TYPE == PK_KV_Q8) {
-          sts128(at, codes_of(raw[w].x, 0x4140), codes_of(raw[w].x, 0x4342), codes_of(raw[w].y, 0x4140), codes_of(raw[w].y, 0x4342));
-        } else {
-          const int s = (int)((subs[w] >> (4 * (sub / 2))) & 15u);
-          const uint32_t s2 = dup_h(s), m2 = dup_h(-1032 * s);
+          // two chunks of 8 dimensions; half the lanes of a row begin with the
+          // second, so that eight lanes' stores touch every bank once
+          const bool swap = sub >= RL / 2;
+          const uint32_t a0 = swap ? x.z : x.x, a1 = swap ? x.w : x.y, b0 = swap ? x.x : x.z, b1 = swap ? x.y : x.w;
+          const uint32_t ca = at + (2 * sub + swap) * L::CH, cb = at + (2 * sub + !swap) * L::CH;
+          sts128(ca, codes_of(a0, 0x4140), codes_of(a0, 0x4342), codes_of(a1, 0x4140), codes_of(a1, 0x4342));
+          sts128(cb, codes_of(b0, 0x4140), codes_of(b0, 0x4342), codes_of(b1, 0x4140), codes_of(b1, 0x4342));
+        } else {  // four chunks, one sub-scale
+          const int s = (int)((subs[w] >> (4 * sub)) & 15u);
+          const uint32_t s2 = dup_h(s), m2 = dup_h(-1032 * s), y[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
-            const uint32_t x = c ? raw[w].y : raw[w].x;
-            sts128(at + c * L::CH, nibbles_of(x, s2, m2), nibbles_of(x >> 4, s2, m2), nibbles_of(x >> 8, s2, m2), nibbles_of(x >> 12, s2, m2));
-          }
+          for (int c = 0; c < 4; c++)
+            sts128(at + (4 * sub + c) * L::CH, nibbles_of(y[c], s2, m2), nibbles_of(y[c] >> 4, s2, m2), nibbles_of(y[c] >> 8, s2, m2),
+                   nibbles_of(y[c] >> 12, s2, m2));
         }
       }
     };
     // both scales of tile i and the tile's summary
     auto put_scales = [&](int i) {
-      uint8_t *sc = smem + L::SC + (i & 1) * L::SCB;
+      uint8_t *sc = smem + L::SC + (i % 3) * L::SCB;
       reinterpret_cast<float *>(sc)[half * NK + key] = on ? d : 0.0f;
       if (half == 0) {
         const unsigned m = __ballot_sync(0xffffffffu, on);
@@ -349,17 +357,47 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
         if (lane == 0) reinterpret_cast<uint32_t *>(sc + 2 * NK * 4 + 8)[key >> 5] = x;
       }
     };
-    if (nt > 0) ask(0);
-    for (int i = 0; i < nt; i++) {
+    // K is a tile ahead of V: tile i + 1's scores do not wait for tile i - 1's
+    // products with V, which tile i's V must (V has one buffer).  Tiles past
+    // the last are asked for as the last again, rather than under a condition
+    // that would keep the loads from being left in flight.
+    auto put_k = [&](int i) {
       if (i >= 2) wait(sfull + 8 * (i & 1), ((i - 2) >> 1) & 1, abort);  // K of tile i - 2 has been used
-      put(sb + L::K + (i & 1) * L::TILE, rk, sk);
-      if (i >= 2) wait(pvdone + 8 * (i & 1), ((i - 2) >> 1) & 1, abort);  // and its V and scales
-      put_scales(i);
-      put(sb + L::V + (i & 1) * L::TILE, rv, sv);
+      put(sb + L::K + (i & 1) * L::TILE, rawk, sk);
+      put_scales(i);  // (those of tile i - 3 have: its products with V are done)
       fence_async_smem();
-      mbar_arrive(kvready + 8 * (i & 1));
-      if (i + 1 < nt) ask(i + 1);
+      mbar_arrive(kready + 8 * (i & 3));
+      const int n = min(i + 1, nt - 1);
+      if (n > i) look(n);
+      ask(n, rawk, sk, kp, ksp);
+      ask_scale(n);
+    };
+    if (nt > 0) {
+      look(0);
+      ask(0, rawk, sk, kp, ksp);
+      ask_scale(0);
+      const int rows_v = rows16;
+      cp_commit();  // (in V's turn)
+      put_k(0);
+      const int ahead = rows16;
+      rows16 = rows_v;
+      ask(0, rawv, sv, vp, vsp);
+      rows16 = ahead;
     }
+    for (int i = 0; i < nt; i++) {
+      const int rows_v = rows16;  // (K may go on to the next 8 tiles)
+      if (i + 1 < nt) put_k(i + 1);
+      else cp_commit();  // (in K's turn)
+      if (i >= 1) wait(pvdone + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1, abort);  // V of tile i - 1 has been used
+      put(sb + L::V, rawv, sv);
+      fence_async_smem();
+      mbar_arrive(vready);
+      const int ahead = rows16;
+      rows16 = rows_v;
+      ask(min(i + 1, nt - 1), rawv, sv, vp, vsp);
+      rows16 = ahead;
+    }
+    cp_wait<0>();
   } else {  // ------------------------------------------------------------ softmax
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const bool work = tile0 + warp * 32 < u.rows;  // (the whole warp)
@@ -384,11 +422,11 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     };
     for (int i = 0; i < nt; i++) {
       const int b = i & 1, p0 = u.lo + NK * i;
-      wait(kvready + 8 * b, (i >> 1) & 1, abort);
+      wait(kready + 8 * (i & 3), (i >> 2) & 1, abort);
       wait(sfull + 8 * b, (i >> 1) & 1, abort);
       tc_fence_after();
       if (work) {
-        const uint8_t *sc = smem + L::SC + b * L::SCB;
+        const uint8_t *sc = smem + L::SC + (i % 3) * L::SCB;
         const float4 *dk4 = reinterpret_cast<const float4 *>(sc), *dv4 = reinterpret_cast<const float4 *>(sc + NK * 4);
         const uint4 r4 = *reinterpret_cast<const uint4 *>(sc + 2 * NK * 4);
         const uint64_t held = (uint64_t)r4.y << 32 | r4.x;
