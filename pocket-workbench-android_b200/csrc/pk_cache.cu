@@ -9,6 +9,7 @@
 // (Q4: over the four lanes of each 32 dimensions first).
 #include "pk_cache.cuh"
 #include "pk_cache.h"
+#include "pk_launch.h"
 
 namespace pk {
 namespace {
@@ -358,21 +359,6 @@ __global__ void __launch_bounds__(CT) k_kv_keep(const pk_kv_cache c, const pk_kv
     }
     __syncwarp();
   }
-}
-
-template <class... KArgs, class... Args>
-cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
 }
 
 template <int TYPE, int DH>

@@ -31,12 +31,13 @@
 #include <algorithm>
 
 #include "pk_cache_attn.cuh"
+#include "pk_launch.h"
 
 namespace pk {
 namespace {
 
 constexpr int MIN_CHUNK = 256;
-constexpr int NSTAGE = 4;  // tiles of 16 positions in flight per key group
+constexpr int NSTAGE = 4;  // tiles of 16 positions in a key group's ring
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
@@ -146,11 +147,14 @@ struct Tile {
 // One warp's state: 8 NB query rows (this lane's are 8 b + 2 t + {0, 1}) over
 // some of the positions.  QS: the query fragments stay in shared memory, where
 // registers would not hold them beside the outputs.
+// It goes TS tiles at a time: a step's maxima over the lanes, its tests and
+// its loop are as much work as a tile's products where there are few rows.
 template <int TYPE, int DH, int NT, int NB>
 struct Warp {
   using T = Tile<TYPE, DH>;
   static constexpr int KS = DH / 16, MV = DH / 16, RB = T::RB, SW = T::SW;
   static constexpr bool QS = NT * NB * KS * 2 > 64;
+  static constexpr int TS = NB <= 2 ? 2 : 1;  // (the scores of two would not fit the registers beside 32 rows' outputs)
   static constexpr int QBYTES = QS ? NT * NB * KS * 32 * 8 : 0;
   uint32_t q[QS ? 1 : NT][QS ? 1 : NB][QS ? 1 : KS][2];
   uint32_t qs;  // shared address of this lane's fragments
@@ -209,27 +213,29 @@ struct Warp {
     }
   }
 
-  // Sixteen positions p0 .. p0 + 15, in shared memory at sm.  MASKED: some of
-  // them may be out of reach of some row.
+  // Positions p0 .. p0 + 16 TS - 1, in shared memory from sm on.  MASKED: some
+  // of them may be out of reach of some row; bit n of `held`: tile n has a page.
   template <bool MASKED>
-  __device__ __forceinline__ void tile(const AttnKArgs &a, const Unit &u, int row0, int p0, uint32_t sm, int lane) {
+  __device__ __forceinline__ void tile(const AttnKArgs &a, const Unit &u, int row0, int p0, uint32_t sm, uint32_t held, int lane) {
     const int g = lane >> 2, t = lane & 3;
-    const uint32_t ksc = sm + 2 * T::CODES, vsc = ksc + T::SCALES;
-    float s[NB][4];
-    float dk[2], dv[2];
-    {
+    float s[NB][TS][4];  // [2 n + e]: key g + 8 n of the tile, row 8 b + 2 t + e
+    float dv[TS][2];
+#pragma unroll
+    for (int y = 0; y < TS; y++) {
+      const uint32_t sy = sm + y * T::BYTES, ksc = sy + 2 * T::CODES, vsc = ksc + T::SCALES;
       uint32_t w[2][RB / 16], sd[2] = {0, 0}, md[2] = {0, 0};
+      float dk[2];
 #pragma unroll
       for (int n = 0; n < 2; n++) {  // keys g and g + 8
         const int row = 8 * n + g;
         if (RB / 4 >= 16) {
 #pragma unroll
           for (int i = 0; i < RB / 64; i++) {
-            const uint4 v = sld_v4(sm + T::at(row, t * (RB / 4) + 16 * i));
+            const uint4 v = sld_v4(sy + T::at(row, t * (RB / 4) + 16 * i));
             w[n][4 * i] = v.x; w[n][4 * i + 1] = v.y; w[n][4 * i + 2] = v.z; w[n][4 * i + 3] = v.w;
           }
         } else {
-          const uint2 v = sld_v2(sm + T::at(row, t * (RB / 4)));
+          const uint2 v = sld_v2(sy + T::at(row, t * (RB / 4)));
           w[n][0] = v.x; w[n][1] = v.y;
         }
         if (TYPE == PK_KV_Q4) {
@@ -241,13 +247,16 @@ struct Warp {
         } else {
           dk[n] = sld_f(ksc + row * 4);
         }
-        dv[n] = sld_f(vsc + row * 4 * SW);
+        dv[y][n] = sld_f(vsc + row * 4 * SW);
       }
       float lo[NT == 2 ? NB : 1][4];
 #pragma unroll
       for (int b = 0; b < NB; b++) {
-        s[b][0] = s[b][1] = s[b][2] = s[b][3] = 0.0f;
-        if (NT == 2) lo[NT == 2 ? b : 0][0] = lo[NT == 2 ? b : 0][1] = lo[NT == 2 ? b : 0][2] = lo[NT == 2 ? b : 0][3] = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          s[b][y][i] = 0.0f;
+          if (NT == 2) lo[NT == 2 ? b : 0][i] = 0.0f;
+        }
       }
 #pragma unroll
       for (int j = 0; j < KS; j++) {
@@ -265,49 +274,52 @@ struct Warp {
 #pragma unroll
         for (int b = 0; b < NB; b++) {
           const uint2 x = frag(0, b, j);
-          mma16816(s[b], f, x.x, x.y);
+          mma16816(s[b][y], f, x.x, x.y);
           if (NT == 2) {  // small terms in sums of their own
-            const uint2 y = frag(NT - 1, b, j);
-            mma16816(lo[NT == 2 ? b : 0], f, y.x, y.y);
+            const uint2 v = frag(NT - 1, b, j);
+            mma16816(lo[NT == 2 ? b : 0], f, v.x, v.y);
           }
         }
       }
-      if (NT == 2) {
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-          for (int i = 0; i < 4; i++) s[b][i] += lo[NT == 2 ? b : 0][i];
-      }
-    }
-    // s[b][2 n + e]: key g + 8 n, row 8 b + 2 t + e
-    uint32_t seen = 0xffffffffu;  // bit 4 b + 2 n + e
-    if (MASKED) {
-      seen = 0;
 #pragma unroll
       for (int b = 0; b < NB; b++)
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-          const int row = row0 + 8 * b + 2 * t + e, i = row / a.group;
-#pragma unroll
-          for (int n = 0; n < 2; n++) {
-            const int p = p0 + g + 8 * n;
-            if (p < u.hi && row < u.rows && (p < u.sv.ctx || sees(a, u, i, p - u.sv.ctx))) seen |= 1u << (4 * b + 2 * n + e);
-          }
-        }
+        for (int i = 0; i < 4; i++) s[b][y][i] = (NT == 2 ? s[b][y][i] + lo[NT == 2 ? b : 0][i] : s[b][y][i]) * dk[i >> 1];
     }
-    auto off = [&](int b, int i) { return MASKED && !((seen >> (4 * b + i)) & 1u); };
+    uint32_t seen[TS];  // bit 4 b + 2 n + e
+    if (MASKED) {
+#pragma unroll
+      for (int y = 0; y < TS; y++) {
+        seen[y] = 0;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const int row = row0 + 8 * b + 2 * t + e, i = row / a.group;
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+              const int p = p0 + 16 * y + g + 8 * n;
+              if (((held >> y) & 1u) && p < u.hi && row < u.rows && (p < u.sv.ctx || sees(a, u, i, p - u.sv.ctx)))
+                seen[y] |= 1u << (4 * b + 2 * n + e);
+            }
+          }
+      }
+    }
+    auto off = [&](int b, int y, int i) { return MASKED && !((seen[y] >> (4 * b + i)) & 1u); };
     float mx[NB][2];
     bool grow = false;
 #pragma unroll
     for (int b = 0; b < NB; b++) {
 #pragma unroll
-      for (int i = 0; i < 4; i++) {
-        s[b][i] *= dk[i >> 1];
-        if (off(b, i)) s[b][i] = -CUDART_INF_F;
-      }
-#pragma unroll
       for (int e = 0; e < 2; e++) {
-        mx[b][e] = key_max(fmaxf(s[b][e], s[b][2 + e])) * rs[b][e];
+        float x = -CUDART_INF_F;
+#pragma unroll
+        for (int y = 0; y < TS; y++) {
+          if (off(b, y, e)) s[b][y][e] = -CUDART_INF_F;
+          if (off(b, y, 2 + e)) s[b][y][2 + e] = -CUDART_INF_F;
+          x = fmaxf(x, fmaxf(s[b][y][e], s[b][y][2 + e]));
+        }
+        mx[b][e] = key_max(x) * rs[b][e];
         grow |= mx[b][e] > m[b][e] + GROW;  // m starts at -inf: a row's first position is always more
       }
     }
@@ -333,118 +345,109 @@ struct Warp {
 #pragma unroll
       for (int e = 0; e < 2; e++) {
         const float mu = m[b][e] == -CUDART_INF_F ? 0.0f : m[b][e];
+        float x = 0.0f;
 #pragma unroll
-        for (int n = 0; n < 2; n++) {
-          const float p = ex2(fmaf(s[b][2 * n + e], rs[b][e], -mu));
-          l[b][e] += p;
-          s[b][2 * n + e] = off(b, 2 * n + e) ? 0.0f : p * dv[n];
-        }
-        xm[b][e] = key_max(fmaxf(s[b][e], s[b][2 + e]));
-        big |= xm[b][e] * inv[b][e] > TOP;
+        for (int y = 0; y < TS; y++)
+#pragma unroll
+          for (int n = 0; n < 2; n++) {
+            const float p = ex2(fmaf(s[b][y][2 * n + e], rs[b][e], -mu));
+            l[b][e] += p;
+            s[b][y][2 * n + e] = off(b, y, 2 * n + e) ? 0.0f : p * dv[y][n];
+            x = fmaxf(x, s[b][y][2 * n + e]);
+          }
+        xm[b][e] = x;
+        big |= x * inv[b][e] > TOP;
       }
     if (__any_sync(0xffffffffu, big)) {
 #pragma unroll
       for (int b = 0; b < NB; b++)
 #pragma unroll
         for (int e = 0; e < 2; e++) {
-          if (!(xm[b][e] * inv[b][e] > TOP)) continue;
-          const float now = SET / fmaxf(xm[b][e], 0x1p-100f);
+          const float top = key_max(xm[b][e]);
+          if (!(top * inv[b][e] > TOP)) continue;
+          const float now = SET / fmaxf(top, 0x1p-100f);
           scale_row(b, e, now / inv[b][e]);
           inv[b][e] = now;
         }
     }
-    uint32_t p[NT][NB][2];  // keys 2 t, 2 t + 1 (+ 8) of row 8 b + g
 #pragma unroll
-    for (int b = 0; b < NB; b++)
+    for (int y = 0; y < TS; y++) {
+      const uint32_t vb = sm + y * T::BYTES + T::CODES, vsc = vb + T::CODES + T::SCALES;
+      uint32_t p[NT][NB][2];  // keys 2 t, 2 t + 1 (+ 8) of row 8 b + g
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int n = 0; n < 2; n++) {
+          const float x0 = s[b][y][2 * n] * inv[b][0], x1 = s[b][y][2 * n + 1] * inv[b][1];
+          const uint32_t hi = pack2(x0, x1);
+          p[0][b][n] = transpose8(hi);
+          if (NT == 2) p[NT - 1][b][n] = transpose8(rest2(x0, x1, hi));
+        }
+      // V: this lane's DH / 8 dimensions of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
+      constexpr int VB = RB / 8, VW = VB / 4;
+      uint32_t v[2][2][VW];
+      uint32_t sd[2] = {0, 0}, md[2] = {0, 0};
 #pragma unroll
       for (int n = 0; n < 2; n++) {
-        const float x0 = s[b][2 * n] * inv[b][0], x1 = s[b][2 * n + 1] * inv[b][1];
-        const uint32_t hi = pack2(x0, x1);
-        p[0][b][n] = transpose8(hi);
-        if (NT == 2) p[NT - 1][b][n] = transpose8(rest2(x0, x1, hi));
-      }
-    // V: this lane's DH / 8 dimensions of keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9
-    constexpr int VB = RB / 8, VW = VB / 4;
-    const uint32_t vb = sm + T::CODES;
-    uint32_t v[2][2][VW];
-    uint32_t sd[2] = {0, 0}, md[2] = {0, 0};
 #pragma unroll
-    for (int n = 0; n < 2; n++) {
-#pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const uint32_t at = vb + T::at(8 * n + 2 * t + e, g * VB);
-        if (VB == 16) {
-          const uint4 x = sld_v4(at);
-          v[n][e][0] = x.x; v[n][e][1 % VW] = x.y; v[n][e][2 % VW] = x.z; v[n][e][3 % VW] = x.w;
-        } else if (VB == 8) {
-          const uint2 x = sld_v2(at);
-          v[n][e][0] = x.x; v[n][e][1 % VW] = x.y;
-        } else {
-          v[n][e][0] = __float_as_uint(sld_f(at));
+        for (int e = 0; e < 2; e++) {
+          const uint32_t at = vb + T::at(8 * n + 2 * t + e, g * VB);
+          if (VB == 16) {
+            const uint4 x = sld_v4(at);
+            v[n][e][0] = x.x; v[n][e][1 % VW] = x.y; v[n][e][2 % VW] = x.z; v[n][e][3 % VW] = x.w;
+          } else if (VB == 8) {
+            const uint2 x = sld_v2(at);
+            v[n][e][0] = x.x; v[n][e][1 % VW] = x.y;
+          } else {
+            v[n][e][0] = __float_as_uint(sld_f(at));
+          }
+        }
+        if (TYPE == PK_KV_Q4) {
+          const int sh = 4 * (g * (DH / 8) / 32);
+          const uint4 x = sld_v4(vsc + (8 * n + 2 * t) * 8);  // D, sub, D, sub
+          const int s0 = (int)((x.y >> sh) & 15u), s1 = (int)((x.w >> sh) & 15u);
+          sd[n] = h2u(__halves2half2(__int2half_rn(s0), __int2half_rn(s1)));
+          md[n] = h2u(__halves2half2(__int2half_rn(-1032 * s0), __int2half_rn(-1032 * s1)));
         }
       }
-      if (TYPE == PK_KV_Q4) {
-        const int sh = 4 * (g * (DH / 8) / 32);
-        const uint4 x = sld_v4(vsc + (8 * n + 2 * t) * 8);  // D, sub, D, sub
-        const int s0 = (int)((x.y >> sh) & 15u), s1 = (int)((x.w >> sh) & 15u);
-        sd[n] = h2u(__halves2half2(__int2half_rn(s0), __int2half_rn(s1)));
-        md[n] = h2u(__halves2half2(__int2half_rn(-1032 * s0), __int2half_rn(-1032 * s1)));
-      }
-    }
-    // of a word's values two a product: dimensions d (rows 0-7), d + 1 (rows 8-15)
+      // of a word's values two a product: dimensions d (rows 0-7), d + 1 (rows 8-15)
 #pragma unroll
-    for (int w = 0; w < VW; w++) {
-      uint32_t x[2][2];
+      for (int w = 0; w < VW; w++) {
+        uint32_t x[2][2];
 #pragma unroll
-      for (int n = 0; n < 2; n++) {
-        x[n][0] = __byte_perm(v[n][0][w], v[n][1][w], TYPE == PK_KV_Q8 ? 0x5140 : 0x5410);
-        x[n][1] = __byte_perm(v[n][0][w], v[n][1][w], TYPE == PK_KV_Q8 ? 0x7362 : 0x7632);
-      }
-      constexpr int PW = TYPE == PK_KV_Q8 ? 2 : 4;  // products a word
+        for (int n = 0; n < 2; n++) {
+          x[n][0] = __byte_perm(v[n][0][w], v[n][1][w], TYPE == PK_KV_Q8 ? 0x5140 : 0x5410);
+          x[n][1] = __byte_perm(v[n][0][w], v[n][1][w], TYPE == PK_KV_Q8 ? 0x7362 : 0x7632);
+        }
+        constexpr int PW = TYPE == PK_KV_Q8 ? 2 : 4;  // products a word
 #pragma unroll
-      for (int d = 0; d < PW; d++) {
-        uint32_t f[4];
+        for (int d = 0; d < PW; d++) {
+          uint32_t f[4];
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+          for (int n = 0; n < 2; n++)
 #pragma unroll
-          for (int e = 0; e < 2; e++) {
-            if (TYPE == PK_KV_Q8) f[2 * n + e] = codes_of(x[n][d], e ? 0x4342 : 0x4140);
-            else f[2 * n + e] = nibbles_of(x[n][d / 2] >> (4 * (2 * (d % 2) + e)), sd[n], md[n]);
-          }
+            for (int e = 0; e < 2; e++) {
+              if (TYPE == PK_KV_Q8) f[2 * n + e] = codes_of(x[n][d], e ? 0x4342 : 0x4140);
+              else f[2 * n + e] = nibbles_of(x[n][d / 2] >> (4 * (2 * (d % 2) + e)), sd[n], md[n]);
+            }
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-          float(&acc)[4] = o[b][w * PW + d];
-          if (NT == 2) {  // the tensor core's own sums drop bits below the running one's last; f32 adds round
-            float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            mma16816(c, f, p[NT - 1][b][0], p[NT - 1][b][1]);
-            mma16816(c, f, p[0][b][0], p[0][b][1]);
+          for (int b = 0; b < NB; b++) {
+            float(&acc)[4] = o[b][w * PW + d];
+            if (NT == 2) {  // the tensor core's own sums drop bits below the running one's last; f32 adds round
+              float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+              mma16816(c, f, p[NT - 1][b][0], p[NT - 1][b][1]);
+              mma16816(c, f, p[0][b][0], p[0][b][1]);
 #pragma unroll
-            for (int i = 0; i < 4; i++) acc[i] += c[i];
-          } else {
-            mma16816(acc, f, p[0][b][0], p[0][b][1]);
+              for (int i = 0; i < 4; i++) acc[i] += c[i];
+            } else {
+              mma16816(acc, f, p[0][b][0], p[0][b][1]);
+            }
           }
         }
       }
     }
   }
 };
-
-// Writes DH / 8 elements of a row: final, or the chunk's part.
-template <int DH>
-__device__ __forceinline__ void write_row(const AttnKArgs &a, const Unit &u, int row, int d0, const float (&x)[DH / 8]) {
-  const int i = row / a.group, h = u.h * a.group + row - i * a.group;
-  const long long tok = u.sv.first + i;
-  if (u.nch > 1) {
-    float *p = a.part_o + ((tok * a.q.n_head + h) * a.n_chunk + u.ch) * DH + d0;
-#pragma unroll
-    for (int j = 0; j < DH / 8; j += 4) *reinterpret_cast<float4 *>(p + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-    return;
-  }
-  const long long off = tok * a.q.out_tok_stride + (long long)h * a.q.out_head_stride + d0;
-  if (a.q.type == T_F32) store_n<float, DH / 8>(reinterpret_cast<float *>(a.q.out) + off, a.vec_o, x);
-  else if (a.q.type == T_F16) store_n<__half, DH / 8>(reinterpret_cast<__half *>(a.q.out) + off, a.vec_o, x);
-  else store_n<__nv_bfloat16, DH / 8>(reinterpret_cast<__nv_bfloat16 *>(a.q.out) + off, a.vec_o, x);
-}
 
 // A CTA of 4 warps: RG groups of 8 NB rows times KG = 4 / RG groups of
 // positions.  The warps of a key group share its ring of tiles; key group k
@@ -456,8 +459,9 @@ struct Geo {
   using W = Warp<TYPE, DH, NT, NB>;
   static constexpr int KG = AW / RG, ROWS = 8 * NB * RG;
   static constexpr int RING = KG * NSTAGE * T::BYTES;
-  static constexpr int SUM = KG * ROWS * (DH + 4) * 4;  // outputs (rows padded by 16 bytes), then m, l
-  static constexpr int SMEM = (RING + RG * W::QBYTES) > SUM + KG * ROWS * 8 ? (RING + RG * W::QBYTES) : SUM + KG * ROWS * 8;
+  static constexpr int SUM = KG * ROWS * (DH + 4) * 4;  // outputs (rows padded by 16 bytes), then m, l, and theirs added up
+  static constexpr int END = SUM + (KG + 1) * ROWS * 8;
+  static constexpr int SMEM = RING + RG * W::QBYTES > END ? RING + RG * W::QBYTES : END;
 };
 
 template <int TYPE, int DH, int NT, int NB, int RG>
@@ -469,57 +473,64 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
   pdl_wait();
   const Unit u = unit_of(a);
   const int tile0 = u.rt * G::ROWS;
-  if (u.ch >= max(u.nch, 1) || tile0 >= u.rows) return;
+  if (tile0 >= u.rows || (u.ch >= max(u.nch, 1) && !(a.cluster && u.nch > 1))) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int rg = warp % RG, kg = warp / RG, row0 = tile0 + rg * 8 * NB;
   // without a mask nobody sees past the tile's last token
   const int last = (min(tile0 + G::ROWS, u.rows) - 1) / a.group;
   const int hi = a.q.mask ? u.hi : min(u.hi, u.sv.ctx + last + 1);
-  const int span = hi - u.lo - 16 * kg, nt = span > 0 ? (span + 16 * G::KG - 1) / (16 * G::KG) : 0;
+  // steps of TS tiles; key group k takes every KG-th step from k
+  constexpr int TS = G::W::TS, PAIRS = NSTAGE / TS;
+  const int span = hi - u.lo - 16 * TS * kg, nt = span > 0 ? (span + 16 * TS * G::KG - 1) / (16 * TS * G::KG) : 0;
   const uint32_t ring = shaddr(smem) + kg * NSTAGE * T::BYTES;
   const int ti = rg * 32 + lane, tn = 32 * RG;
-  // lane i holds the page of tile i of the block of 32 tiles being copied, and
+  auto pos = [&](int i) { return u.lo + 16 * TS * (kg + G::KG * i); };
+  // lane x holds the page of tile x of the block of 32 tiles being copied, and
   // of the one being used; -1: none
   auto pages_of = [&](int i0) {
-    const int i = i0 + lane, p = u.lo + 16 * (kg + G::KG * i);
-    if (i >= nt) return -1;
+    const int i = i0 + lane / TS, p = pos(i) + 16 * (lane % TS);
+    if (i >= nt || p >= hi) return -1;
     const int j = p >> a.page_shift;
     const int pg = j < a.s.max_pages ? __ldg(a.s.pages + (size_t)u.s * a.s.max_pages + j) : -1;
     return pg >= 0 && pg < a.c.n_pages ? pg : -1;
   };
+  constexpr int BLOCK = 32 / TS;  // steps
   int ahead = pages_of(0), now = ahead;
   auto issue = [&](int i) {
-    if (i > 0 && (i & 31) == 0) ahead = pages_of(i);
-    const int pg = __shfl_sync(0xffffffffu, ahead, i & 31);
-    if (i < nt && pg >= 0) {
-      const int p = u.lo + 16 * (kg + G::KG * i);
-      const long long row = ((long long)pg * a.c.n_kv + u.h) * a.c.page_size + (p & (a.c.page_size - 1));
-      T::copy(a.c, row, ring + (i % NSTAGE) * T::BYTES, ti, tn);
+    if (i > 0 && i % BLOCK == 0) ahead = pages_of(i);
+#pragma unroll
+    for (int y = 0; y < TS; y++) {
+      const int pg = __shfl_sync(0xffffffffu, ahead, (i % BLOCK) * TS + y);
+      if (i < nt && pg >= 0) {
+        const long long row = ((long long)pg * a.c.n_kv + u.h) * a.c.page_size + ((pos(i) + 16 * y) & (a.c.page_size - 1));
+        T::copy(a.c, row, ring + ((i % PAIRS) * TS + y) * T::BYTES, ti, tn);
+      }
     }
     cp_commit();
   };
 #pragma unroll
-  for (int i = 0; i < NSTAGE - 1; i++) issue(i);
+  for (int i = 0; i < PAIRS - 1; i++) issue(i);
   typename G::W W;
   W.init(a, u, row0, lane, shaddr(smem) + G::RING + rg * G::W::QBYTES);
   __syncwarp();
   for (int i = 0; i < nt; i++) {
-    cp_wait<NSTAGE - 2>();
+    cp_wait<PAIRS - 2>();
     if (RG > 1) bar_n(1 + kg, tn);
     else __syncwarp();
-    if (i > 0 && (i & 31) == 0) now = ahead;  // (the copies are less than 32 tiles ahead)
-    const int pg = __shfl_sync(0xffffffffu, now, i & 31);
-    issue(i + NSTAGE - 1);
-    if (pg < 0) continue;
-    const int p0 = u.lo + 16 * (kg + G::KG * i);
-    const uint32_t sm = ring + (i % NSTAGE) * T::BYTES;
-    if (p0 + 16 > min(u.sv.ctx, hi)) W.template tile<true>(a, u, row0, p0, sm, lane);
-    else W.template tile<false>(a, u, row0, p0, sm, lane);
+    if (i > 0 && i % BLOCK == 0) now = ahead;  // (the copies are less than a block ahead)
+    uint32_t held = 0;
+#pragma unroll
+    for (int y = 0; y < TS; y++) held |= __shfl_sync(0xffffffffu, now, (i % BLOCK) * TS + y) >= 0 ? 1u << y : 0u;
+    issue(i + PAIRS - 1);
+    if (!held) continue;
+    const uint32_t sm = ring + (i % PAIRS) * TS * T::BYTES;
+    if (pos(i) + 16 * TS > min(u.sv.ctx, hi) || held != (1u << TS) - 1) W.template tile<true>(a, u, row0, pos(i), sm, held, lane);
+    else W.template tile<false>(a, u, row0, pos(i), sm, held, lane);
   }
   cp_wait<0>();
   __syncthreads();  // the ring's memory is free
   float *so = reinterpret_cast<float *>(smem);
-  float2 *sml = reinterpret_cast<float2 *>(smem + G::SUM);
+  float2 *sml = reinterpret_cast<float2 *>(smem + G::SUM), *sfin = sml + G::KG * G::ROWS;
 #pragma unroll
   for (int b = 0; b < NB; b++)
 #pragma unroll
@@ -537,6 +548,7 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
             make_float4(W.o[b][i][e] * f, W.o[b][i][2 + e] * f, W.o[b][i + 1][e] * f, W.o[b][i + 1][2 + e] * f);
     }
   __syncthreads();
+  const bool cluster = a.cluster && u.nch > 1;
   for (int x = threadIdx.x; x < G::ROWS * 8; x += 32 * AW) {
     const int r = x >> 3, d0 = (x & 7) * (DH / 8);
     if (tile0 + r >= u.rows) continue;
@@ -553,8 +565,14 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
 #pragma unroll
       for (int j = 0; j < DH / 8; j++) acc[j] = fmaf(f, so[(k * G::ROWS + r) * (DH + 4) + d0 + j], acc[j]);
     }
+    if (cluster) {  // in the place of the first group's
+#pragma unroll
+      for (int j = 0; j < DH / 8; j++) so[r * (DH + 4) + d0 + j] = acc[j];
+      if (d0 == 0) sfin[r] = make_float2(M, L);
+      continue;
+    }
     if (u.nch > 1) {
-      if ((x & 7) == 0) {
+      if (d0 == 0) {
         const int i = (tile0 + r) / a.group, h = u.h * a.group + (tile0 + r) - i * a.group;
         a.part_ml[((long long)(u.sv.first + i) * a.q.n_head + h) * a.n_chunk + u.ch] = make_float2(M, L);
       }
@@ -563,8 +581,9 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
 #pragma unroll
       for (int j = 0; j < DH / 8; j++) acc[j] *= inv;
     }
-    write_row<DH>(a, u, tile0 + r, d0, acc);
+    write_row<DH>(a, u, tile0 + r, d0, acc, u.nch > 1);
   }
+  if (cluster) join_cluster<DH>(a, u, tile0, G::ROWS, shaddr(so), shaddr(sfin), 32 * AW);
 }
 
 // Adds up the chunks of rows that have more than one: a warp a row.
@@ -611,21 +630,6 @@ __global__ void __launch_bounds__(128) k_kv_attn_join(const AttnKArgs a) {
   }
 }
 
-template <class... KArgs, class... Args>
-cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-}
-
 // The kernel's variant by the rows that a kv head's tile may have: columns in
 // steps of 8 up to 32 a warp (16 where f32's two terms double the query
 // fragments of 128 dimensions), then two or four warps side by side.
@@ -660,8 +664,16 @@ Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int ty
   return c.head_dim == 64 ? variant_type<PK_KV_Q4, 64>(type, rows) : variant_type<PK_KV_Q4, 128>(type, rows);
 }
 
+// Chunks of a sequence's positions: so many that 148 SMs have about eight CTAs
+// each, none under MIN_CHUNK positions.  Where all CTAs run at once (two an SM)
+// up to eight chunks are a cluster, whose CTAs add up through one another's
+// shared memory (up to 16 are made 8): that saves the scratch and a second
+// launch, 13 us to 11 for one token at 1500 positions.  Elsewhere a cluster's
+// CTAs would hold their SMs until its longest is done (eight 16K streams 171 us
+// against 150), so their parts go through the scratch.
 struct Split {
   int chunk, n_chunk, row_tiles;
+  bool cluster;
 };
 Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, const Variant &v) {
   Split p;
@@ -669,9 +681,11 @@ Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, const Vari
   p.row_tiles = (int)((rows + v.rows - 1) / v.rows);
   const long long units = (long long)s.n_seq * c.n_kv * p.row_tiles, want = 148 * 8;
   const long long most = (s.max_len + MIN_CHUNK - 1) / MIN_CHUNK;
-  const long long n = std::max<long long>(1, std::min(most, want / units));
+  long long n = std::max<long long>(1, std::min(most, want / units));
+  if (n > 8 && n <= 16 && units * 8 <= 296) n = 8;
   p.chunk = (int)(((s.max_len + n - 1) / n + 63) / 64 * 64);
   p.n_chunk = (int)((s.max_len + (long long)p.chunk - 1) / p.chunk);
+  p.cluster = p.n_chunk > 1 && p.n_chunk <= 8 && units * p.n_chunk <= 296;
   return p;
 }
 
@@ -679,7 +693,7 @@ Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, const Vari
 
 size_t kv_attn_scratch_bytes(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type) {
   const Split p = split_of(c, s, n_head, variant_of(c, s, n_head, type));
-  if (p.n_chunk <= 1) return 0;
+  if (p.n_chunk <= 1 || p.cluster) return 0;
   return (size_t)s.n_tok * n_head * p.n_chunk * (c.head_dim + 2) * sizeof(float);
 }
 
@@ -697,13 +711,15 @@ cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_k
   a.vec_o = (((uintptr_t)q.out | (uintptr_t)q.out_tok_stride * es | (uintptr_t)q.out_head_stride * es) & 15) == 0;
   const size_t rows = (size_t)s.n_tok * q.n_head;
   a.part_o = reinterpret_cast<float *>(scratch);
-  a.part_ml = p.n_chunk > 1 ? reinterpret_cast<float2 *>(a.part_o + rows * p.n_chunk * c.head_dim) : nullptr;
+  a.cluster = p.cluster;
+  a.part_ml = p.n_chunk > 1 && !a.cluster ? reinterpret_cast<float2 *>(a.part_o + rows * p.n_chunk * c.head_dim) : nullptr;
   const long long blocks = (long long)s.n_seq * c.n_kv * p.row_tiles * p.n_chunk, jb = ((long long)rows + 3) / 4;
   if (blocks > 0x7fffffffLL || jb > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const int cluster = a.cluster ? p.n_chunk : 1;
   cudaError_t e;
-  if (!v.k) e = launch_kv_attn_tc(a, (unsigned)blocks, st);
-  else if ((e = cudaFuncSetAttribute(v.k, cudaFuncAttributeMaxDynamicSharedMemorySize, v.smem)) == cudaSuccess) e = launch(v.k, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
-  if (e != cudaSuccess || p.n_chunk <= 1) return e;
+  if (!v.k) e = launch_kv_attn_tc(a, cluster, (unsigned)blocks, st);
+  else e = launch_cluster(v.k, cluster, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
+  if (e != cudaSuccess || p.n_chunk <= 1 || a.cluster) return e;
   return launch(c.head_dim == 64 ? k_kv_attn_join<64> : k_kv_attn_join<128>, dim3((unsigned)jb), dim3(128), 0, st, a);
 }
 

@@ -40,11 +40,12 @@ struct AttnKArgs {
   float *part_o;   // [n_tok][n_head][n_chunk][DH]
   float2 *part_ml; // [n_tok][n_head][n_chunk]
   int chunk, n_chunk, row_tiles, group, page_shift, vec_q, vec_o;
+  int cluster;  // 1: a sequence's chunks are a cluster's CTAs, which add up among themselves
 };
 
 // A CTA's work: one chunk of positions [lo, hi) for one tile of the rows (token
 // i, query head of kv head h) of one sequence.  Sequences of more than one
-// chunk (nch) leave theirs in the scratch.
+// chunk (nch) leave theirs in the scratch, or to the cluster.
 struct Unit {
   SeqView sv;
   int s, h, rt, ch, lo, hi, nch, rows;
@@ -52,12 +53,13 @@ struct Unit {
 __device__ __forceinline__ Unit unit_of(const AttnKArgs &a) {
   Unit u;
   unsigned id = blockIdx.x;
+  // a sequence's chunks side by side (a cluster's have to be)
+  u.ch = (int)(id % (unsigned)a.n_chunk);
+  id /= (unsigned)a.n_chunk;
   u.rt = (int)(id % (unsigned)a.row_tiles);
   id /= (unsigned)a.row_tiles;
   u.h = (int)(id % (unsigned)a.c.n_kv);
-  id /= (unsigned)a.c.n_kv;
-  u.ch = (int)(id % (unsigned)a.n_chunk);
-  u.s = (int)(id / (unsigned)a.n_chunk);
+  u.s = (int)(id / (unsigned)a.c.n_kv);
   u.sv = seq_view(a.s, a.c.page_size, u.s);
   u.rows = u.sv.n * a.group;
   u.nch = (u.sv.total + a.chunk - 1) / a.chunk;
@@ -75,9 +77,91 @@ __device__ __forceinline__ bool sees(const AttnKArgs &a, const Unit &u, int i, i
 }
 
 
+// Every thread of the cluster arrives, and sees what the others wrote before.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t at_rank(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float4 ld_cluster4(uint32_t a) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 ld_cluster2(uint32_t a) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
+// Writes DH / 8 elements of a row: final (out), or the chunk's part.
+template <int DH>
+__device__ __forceinline__ void write_row(const AttnKArgs &a, const Unit &u, int row, int d0, const float (&x)[DH / 8], bool part) {
+  const int i = row / a.group, h = u.h * a.group + row - i * a.group;
+  const long long tok = u.sv.first + i;
+  if (part) {
+    float *p = a.part_o + ((tok * a.q.n_head + h) * a.n_chunk + u.ch) * DH + d0;
+#pragma unroll
+    for (int j = 0; j < DH / 8; j += 4) *reinterpret_cast<float4 *>(p + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
+    return;
+  }
+  const long long off = tok * a.q.out_tok_stride + (long long)h * a.q.out_head_stride + d0;
+  if (a.q.type == T_F32) store_n<float, DH / 8>(reinterpret_cast<float *>(a.q.out) + off, a.vec_o, x);
+  else if (a.q.type == T_F16) store_n<__half, DH / 8>(reinterpret_cast<__half *>(a.q.out) + off, a.vec_o, x);
+  else store_n<__nv_bfloat16, DH / 8>(reinterpret_cast<__nv_bfloat16 *>(a.q.out) + off, a.vec_o, x);
+}
+
+// The rows of a cluster's chunks added up: each CTA has its rows' sums at
+// shared address so ([row][DH + 4] f32) and their (M, L) at sml, and takes
+// every nch-th group of DH / 8 elements.  All threads of all CTAs call it
+// after the sums are written; a CTA without a chunk only keeps step.
+template <int DH>
+__device__ __forceinline__ void join_cluster(const AttnKArgs &a, const Unit &u, int tile0, int rows, uint32_t so, uint32_t sml, int threads) {
+  cluster_sync();
+  if (u.ch < u.nch) {
+    for (int x = u.ch * threads + (int)threadIdx.x; x < rows * 8; x += u.nch * threads) {
+      const int r = x >> 3, d0 = (x & 7) * (DH / 8);
+      if (tile0 + r >= u.rows) continue;
+      float2 ml[8];
+      float M = -CUDART_INF_F, L = 0.0f, acc[DH / 8];
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        ml[c] = make_float2(-CUDART_INF_F, 0.0f);
+        if (c < u.nch) ml[c] = ld_cluster2(at_rank(sml + r * 8, c));
+        M = fmaxf(M, ml[c].x);
+      }
+#pragma unroll
+      for (int j = 0; j < DH / 8; j++) acc[j] = 0.0f;
+#pragma unroll
+      for (int c = 0; c < 8; c++) {
+        if (c >= u.nch) continue;
+        const float f = ml[c].y == 0.0f ? 0.0f : ex2(ml[c].x - M);  // a NaN sum stays one
+        L = fmaf(f, ml[c].y, L);
+        const uint32_t p = at_rank(so + (r * (DH + 4) + d0) * 4, c);
+#pragma unroll
+        for (int j = 0; j < DH / 8; j += 4) {
+          const float4 v = ld_cluster4(p + 4 * j);
+          acc[j] = fmaf(f, v.x, acc[j]);
+          acc[j + 1] = fmaf(f, v.y, acc[j + 1]);
+          acc[j + 2] = fmaf(f, v.z, acc[j + 2]);
+          acc[j + 3] = fmaf(f, v.w, acc[j + 3]);
+        }
+      }
+      const float inv = L > 0.0f || isnan(L) ? 1.0f / L : 0.0f;
+#pragma unroll
+      for (int j = 0; j < DH / 8; j++) acc[j] *= inv;
+      write_row<DH>(a, u, tile0 + r, d0, acc, false);
+    }
+  }
+  cluster_sync();  // (until then the others may be reading)
+}
+
 // The tcgen05 kernel's launch (pk_cache_attn_tc.cu): 128 rows of a kv head's
 // tile, half-precision queries.
 constexpr int TC_ATTN_ROWS = 128;
-cudaError_t launch_kv_attn_tc(const AttnKArgs &a, unsigned blocks, cudaStream_t st);
+cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int cluster, unsigned blocks, cudaStream_t st);
 
 }  // namespace pk

@@ -31,6 +31,7 @@
 #include <algorithm>
 
 #include "pk_cache_attn.cuh"
+#include "pk_launch.h"
 #include "pk_tcgen05.cuh"
 
 namespace pk {
@@ -51,7 +52,8 @@ struct Lay {
   // codes in flight, K's and V's, 16 bytes a thread and pass
   static constexpr int RAWB = NK * DH, SC = RAW + 2 * RAWB;
   // of three tiles: D^K [NK], D^V [NK]; positions that hold something (2 words), largest D^V of 32 (2)
-  static constexpr int SCB = 2 * NK * 4 + 16, BAR = SC + 3 * SCB, BYTES = BAR + 96;
+  static constexpr int SCB = 2 * NK * 4 + 16, BAR = SC + 3 * SCB, ML = BAR + 112, BYTES = ML + ROWS * 8;
+  static_assert(ROWS * (DH + 4) * 4 <= RAW, "a cluster's sums take the operands' place, not that of copies in flight");
   static constexpr int S_COL = 0, O_COL = 2 * NK, COLS = 256;
 };
 
@@ -208,20 +210,22 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
   pdl_wait();
   const Unit u = unit_of(a);
   const int tile0 = u.rt * ROWS;
-  if (u.ch >= max(u.nch, 1) || tile0 >= u.rows) {
+  const bool cluster = a.cluster && u.nch > 1;
+  if (tile0 >= u.rows || (u.ch >= max(u.nch, 1) && !cluster)) {
     pdl_trigger();
     return;
   }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sb = shaddr(smem);
-  // barriers: S full x 2, K and scales ready x 4, P ready, PV done x 2, V ready; the TMEM address; the abort flag
-  const uint32_t bar = sb + L::BAR, sfull = bar, kready = bar + 16, pready = bar + 48, pvdone = bar + 56, vready = bar + 72;
-  volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 84);
+  // barriers: S full x 2, K and scales ready x 4, P ready x 2, PV done x 2, V ready; the TMEM address; the abort flag
+  const uint32_t bar = sb + L::BAR, sfull = bar, kready = bar + 16, pready = bar + 48, pvdone = bar + 64, vready = bar + 80;
+  volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 92);
   if (tid == 0) {
-    mbar_init(sfull, 1);
-    mbar_init(sfull + 8, 1);
+    mbar_init(sfull, 2);  // the products, and the warp that issues them (which has seen the scales)
+    mbar_init(sfull + 8, 2);
     for (int i = 0; i < 4; i++) mbar_init(kready + 8 * i, CONV);
     mbar_init(pready, SOFT);
+    mbar_init(pready + 8, SOFT);
     mbar_init(vready, CONV);
     mbar_init(pvdone, 1);
     mbar_init(pvdone + 8, 1);
@@ -229,7 +233,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 80), "r"(L::COLS) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 88), "r"(L::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   const int row = tile0 + tid;
@@ -243,7 +247,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
   __syncthreads();
   tc_fence_after();
   pdl_trigger();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::BAR + 80);
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::BAR + 88);
   // without a mask nobody sees past the tile's last token
   const int last = (min(tile0 + ROWS, u.rows) - 1) / a.group;
   const int hi = a.q.mask ? u.hi : min(u.hi, u.sv.ctx + last + 1);
@@ -260,13 +264,15 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
 #pragma unroll
       for (int s = 0; s < DH / 16; s++)
         mma_f16<NK, false>(dt, tc_desc(q + s * 2 * (ROWS * 16), ROWS * 16, 128), tc_desc(k + s * 2 * L::CH, L::CH, 128), s > 0);
+      if (lane == 0) mbar_arrive(sfull + 8 * (i & 1));
+      __syncwarp();
       tc_commit(sfull + 8 * (i & 1));
     };
     if (nt > 0) scores(0);
     for (int i = 0; i < nt; i++) {
       if (i + 1 < nt) scores(i + 1);  // (into the columns of tile i - 1's weights: products are done in order)
       wait(vready, i & 1, abort);
-      wait(pready, i & 1, abort);
+      wait(pready + 8 * (i & 1), (i >> 1) & 1, abort);
       tc_fence_after();
       uint32_t w = tmem + L::S_COL + (i & 1) * NK, v = sb + L::V;
       asm volatile("" : "+r"(w), "+r"(v));
@@ -422,7 +428,6 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     };
     for (int i = 0; i < nt; i++) {
       const int b = i & 1, p0 = u.lo + NK * i;
-      wait(kready + 8 * (i & 3), (i >> 2) & 1, abort);
       wait(sfull + 8 * b, (i >> 1) & 1, abort);
       tc_fence_after();
       if (work) {
@@ -528,9 +533,8 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
         st16(cols + 16, w[1]);
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       }
-      if (i > 0) pv_wait(i - 1);  // else a warp that is ahead could arrive twice in one phase
       tc_fence_before();
-      mbar_arrive(pready);
+      mbar_arrive(pready + 8 * b);
     }
     // ---- the rows
     if (nt > 0) pv_wait(nt - 1);
@@ -542,12 +546,14 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
       float f = 1.0f;
       if (*abort) f = l = CUDART_NAN_F;
       if (part) {
-        if (on) a.part_ml[(at * a.q.n_head + h) * a.n_chunk + u.ch] = make_float2(m, l);
+        if (on && cluster) *reinterpret_cast<float2 *>(smem + L::ML + tid * 8) = make_float2(m, l);
+        else if (on) a.part_ml[((at * a.q.n_head + h) * a.n_chunk) + u.ch] = make_float2(m, l);
       } else {
         f *= l > 0.0f || isnan(l) ? 1.0f / l : 0.0f;
       }
       if (l == 0.0f) f = 0.0f;
-      float *po = part ? a.part_o + ((at * a.q.n_head + h) * a.n_chunk + u.ch) * DH : nullptr;
+      // (in a cluster: into shared memory, where the operands were)
+      float *po = !part ? nullptr : cluster ? reinterpret_cast<float *>(smem) + tid * (DH + 4) : a.part_o + ((at * a.q.n_head + h) * a.n_chunk + u.ch) * DH;
       const long long off = at * a.q.out_tok_stride + (long long)h * a.q.out_head_stride;
 #pragma unroll
       for (int c = 0; c < DH / 32; c++) {
@@ -574,6 +580,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
   }
   tc_fence_before();
   __syncthreads();
+  if (cluster) join_cluster<DH>(a, u, tile0, ROWS, sb, sb + L::ML, THREADS);
   if (warp == 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::COLS) : "memory");
@@ -582,23 +589,11 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
 
 }  // namespace
 
-cudaError_t launch_kv_attn_tc(const AttnKArgs &a, unsigned blocks, cudaStream_t st) {
+cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int cluster, unsigned blocks, cudaStream_t st) {
   void (*k)(AttnKArgs) = a.c.type == PK_KV_Q8 ? (a.c.head_dim == 64 ? k_kv_attn_tc<PK_KV_Q8, 64> : k_kv_attn_tc<PK_KV_Q8, 128>)
                                               : (a.c.head_dim == 64 ? k_kv_attn_tc<PK_KV_Q4, 64> : k_kv_attn_tc<PK_KV_Q4, 128>);
   const int smem = a.c.head_dim == 64 ? Lay<64>::BYTES : Lay<128>::BYTES;
-  const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, k, a);
+  return launch_cluster(k, cluster, dim3(blocks), dim3(THREADS), smem, st, a);
 }
 
 }  // namespace pk

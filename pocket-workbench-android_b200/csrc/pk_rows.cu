@@ -7,24 +7,10 @@
 
 #include "pk_cache.cuh"
 #include "pk_cache.h"
+#include "pk_launch.h"
 
 namespace pk {
 namespace {
-
-template <class... KArgs, class... Args>
-cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
-}
 
 // ------------------------------------------------------------------- rotary
 // A CTA takes one token and some of its heads: the angles once for them all
@@ -144,7 +130,7 @@ cudaError_t rope_as(const pk_rope_args &a, cudaStream_t st) {
   const int want = std::max(1, std::min(heads, 592 / std::max(a.n_tok, 1)));
   const int per = (heads + want - 1) / want;
   return launch(k_rope<T, V, HALF, AL>, dim3((unsigned)a.n_tok, (unsigned)((heads + per - 1) / per)), dim3(RT),
-                (size_t)(a.n_rot / 2) * sizeof(float2), st, a, per);
+                (int)(a.n_rot / 2 * sizeof(float2)), st, a, per);
 }
 template <int T>
 cudaError_t rope_type(const pk_rope_args &a, cudaStream_t st) {
@@ -562,16 +548,12 @@ cudaError_t rules_type(const void *in, void *out, int rows, int n, long is, long
     parts = (n + len - 1) / len;
     if (rows * parts > 0x7fffffffLL) return cudaErrorInvalidValue;
     const int smem = entries || r.hist || r.bias_id ? 8 << bits : 0;
-    const cudaError_t e = cudaFuncSetAttribute(k_logit_rules_hash<T, NT, 3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 8 << HASH_MOST);
-    if (e != cudaSuccess) return e;
     return launch(k_logit_rules_hash<T, NT, 3>, dim3((unsigned)(rows * parts)), dim3(NT), smem, st, in, out, n, is, os, r, (int)parts, len,
                   bits, vec);
   }
   const int segs = (n + SEG - 1) / SEG;
   const long long blocks = (long long)rows * segs;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const cudaError_t e = cudaFuncSetAttribute(k_logit_rules<T, SEG, 512, 3>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * SEG * 4);
-  if (e != cudaSuccess) return e;
   return launch(k_logit_rules<T, SEG, 512, 3>, dim3((unsigned)blocks), dim3(512), 2 * SEG * 4, st, in, out, n, is, os, r, segs, vec);
 }
 

@@ -68,12 +68,12 @@ SIGNATURES = {
 }
 
 torch = None  # set by _init, with the library and the error type
-_L = PkError = last_error = raw_stream = None
+_L = PkError = last_error = raw_stream = current_device = None
 _type_of = {}
 
 
 def _init():
-    global torch, _L, PkError, last_error, raw_stream
+    global torch, _L, PkError, last_error, raw_stream, current_device
     if _L is not None:
         return
     import torch as t
@@ -84,6 +84,7 @@ def _init():
     _type_of.update({t.float32: 0, t.float16: 1, t.bfloat16: 30})
     # the current stream's handle without building a Stream object for it (2 us a call)
     raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None) or (lambda i: t.cuda.current_stream(i).cuda_stream)
+    current_device = t.cuda.current_device
     _L = lib()
 
 
@@ -101,7 +102,7 @@ def _dtype(t, who):
 def _call(fn, device, stream, used, *args):
     """fn(*args, stream) on device number `device`; `used`: tensors made by this call, which a stream that is not the
     current one must be known to use."""
-    if stream is None and torch.cuda.current_device() == device:
+    if stream is None and current_device() == device:
         rc = fn(*args, raw_stream(device))
     else:
         with torch.cuda.device(device):
@@ -138,6 +139,7 @@ class KvSeqs:
         self.device, self.n_seq, self.n_tok, self.max_new, self.max_len = device, n, n_tok, max_new, max_len
         self.c = KvSeqsC(start.data_ptr(), ctx.data_ptr(), pages.data_ptr(), n, pages.shape[1], n_tok, max_new, max_len)
         self.ref = C.byref(self.c)
+        self.scratch = {}  # bytes that attend() needs, by what they depend on besides
 
 
 class KvCache:
@@ -191,8 +193,9 @@ class KvCache:
         """(k, v) [n_tok, n_kv, head_dim] of positions ctx .. read back; rows that no sequence has keep what they held."""
         made = ()
         if out is None:
-            kv = torch.empty((2, seqs.n_tok, self.n_kv, self.head_dim), dtype=dtype or torch.float32, device=self.k.device)
-            made, out = (kv,), kv.unbind(0)
+            dh, dt, dev = self.head_dim, dtype or torch.float32, self.k.device
+            shape, st = (seqs.n_tok, self.n_kv, dh), (self.n_kv * dh, dh, 1)
+            made = out = torch.empty_strided(shape, st, dtype=dt, device=dev), torch.empty_strided(shape, st, dtype=dt, device=dev)
         k, v = out
         _call(_L.pk_kv_load, self.device, stream, made, self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "load"))
         return k, v
@@ -224,13 +227,15 @@ class KvCache:
             made = (out,)
         elif out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or out.stride(2) != 1:
             _bad("attend: out must be as q")
-        ptr, size = None, _L.pk_kv_attn_scratch_bytes(self.ref, seqs.ref, shape[1], code)
+        ptr, size = None, seqs.scratch.get((shape[1], code, self.kind, self.n_kv, self.head_dim))
+        if size is None:
+            size = self.attend_scratch_bytes(seqs, shape[1], q.dtype)
         if scratch is not None:
             if scratch.get_device() != dev or not scratch.is_contiguous():
                 _bad("attend: scratch must be contiguous and on the cache's device")
             ptr, size = scratch.data_ptr(), scratch.numel() * scratch.element_size()
         elif size:
-            scratch = torch.empty(size, dtype=torch.uint8, device=q.device)
+            scratch = self.ks.new_empty((size + 3) // 4)
             made += (scratch,)
             ptr = scratch.data_ptr()
         o = out.stride()
@@ -240,7 +245,11 @@ class KvCache:
         return out
 
     def attend_scratch_bytes(self, seqs: KvSeqs, n_head: int, dtype) -> int:
-        return _L.pk_kv_attn_scratch_bytes(self.ref, seqs.ref, n_head, _type_of[dtype])
+        """Bytes of scratch that attend() needs (0: none); kept with the sequences, whose bounds do not change."""
+        code = _type_of[dtype]
+        n = _L.pk_kv_attn_scratch_bytes(self.ref, seqs.ref, n_head, code)
+        seqs.scratch[n_head, code, self.kind, self.n_kv, self.head_dim] = n
+        return n
 
 
 class RopeTable:
@@ -284,22 +293,25 @@ def rope(table: RopeTable, pos, q, k=None, layout: str = "interleaved", out_q=No
     _i32(pos, dev, "pos", 1)
     code, shape, made = _dtype(q, "rope"), q.shape, []
     n, dh = pos.shape[0], shape[-1]
-    for x, out in ((q, out_q), (k, out_k)):
-        if x is None:
-            continue
-        if x.dim() != 3 or x.shape[0] != n or x.shape[2] != dh or x.stride(2) != 1 or x.dtype != q.dtype or x.get_device() != dev:
-            _bad("rope: q and k must be [n_tok, heads, head_dim] of one type on the table's device, with contiguous heads")
-        if out is not None and (out.shape != x.shape or out.dtype != x.dtype or out.get_device() != dev or out.stride(2) != 1):
-            _bad("rope: an output is not as its input")
+    qs = q.stride()
+    if len(shape) != 3 or shape[0] != n or qs[2] != 1 or q.get_device() != dev:
+        _bad("rope: q must be [n_tok, heads, head_dim] on the table's device, with contiguous heads")
     if out_q is None:
         out_q = _like(q)
         made.append(out_q)
-    qs, qt, ks, kt, kp, kq, nk = q.stride(), out_q.stride(), _NO_ROWS, _NO_ROWS, 0, 0, 0
+    elif out_q.shape != shape or out_q.dtype != q.dtype or out_q.get_device() != dev or out_q.stride(2) != 1:
+        _bad("rope: an output is not as its input")
+    qt, ks, kt, kp, kq, nk = out_q.stride(), _NO_ROWS, _NO_ROWS, 0, 0, 0
     if k is not None:
+        kshape, ks = k.shape, k.stride()
+        if len(kshape) != 3 or kshape[0] != n or kshape[2] != dh or ks[2] != 1 or k.dtype != q.dtype or k.get_device() != dev:
+            _bad("rope: k must be [n_tok, heads, head_dim] of q's type on the table's device, with contiguous heads")
         if out_k is None:
             out_k = _like(k)
             made.append(out_k)
-        ks, kt, kp, kq, nk = k.stride(), out_k.stride(), k.data_ptr(), out_k.data_ptr(), k.shape[1]
+        elif out_k.shape != kshape or out_k.dtype != q.dtype or out_k.get_device() != dev or out_k.stride(2) != 1:
+            _bad("rope: an output is not as its input")
+        kt, kp, kq, nk = out_k.stride(), k.data_ptr(), out_k.data_ptr(), kshape[1]
     args = PACK_ROPE(q.data_ptr(), kp, out_q.data_ptr(), kq, pos.data_ptr(), table.turns.data_ptr(), qs[0], qs[1], ks[0], ks[1], qt[0],
                      qt[1], kt[0], kt[1], code, pairs, n, shape[1], nk, dh, table.n_rot, table.gain)
     _call(_L.pk_rope, dev, stream, made, args)
