@@ -586,38 +586,74 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
   if (cluster) join_cluster<DH>(a, u, tile0, G::ROWS, shaddr(so), shaddr(sfin), 32 * AW);
 }
 
-// Adds up the chunks of rows that have more than one: a warp a row.
-template <int DH>
-__global__ void __launch_bounds__(128) k_kv_attn_join(const AttnKArgs a) {
+// Adds up the chunks of rows that have more than one.  W warps a row, each with
+// every W-th chunk, four chunks' loads at a time: 1 (four rows a CTA) where
+// there are up to 8 chunks, 8 where there are more (one sequence of 30000
+// positions has 118, which one warp took longer over than the attention).
+template <int DH, int W>
+__global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) k_kv_attn_join(const AttnKArgs a) {
+  constexpr int V = DH / 32;
+  __shared__ float so[W][DH];
+  __shared__ float2 sml[W];
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31;
-  const long long w = (long long)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const long long tok = w / a.q.n_head;
-  const int h = (int)(w - tok * a.q.n_head);
-  if (tok >= a.s.n_tok) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long row = W == 1 ? (long long)blockIdx.x * 4 + warp : (long long)blockIdx.x;
+  const long long tok = row / a.q.n_head;
+  const int h = (int)(row - tok * a.q.n_head), w = W == 1 ? 0 : warp;
+  if (tok >= a.s.n_tok) return;  // (whole warps; with W > 1 the whole CTA, as all returns here)
   const int s = seq_of(a.s, (int)tok, lane);
   if (s < 0) return;
   const SeqView sv = seq_view(a.s, a.c.page_size, s);
   const int nch = (sv.total + a.chunk - 1) / a.chunk;
   if (tok - sv.first >= sv.n || nch <= 1) return;
-  const float2 *ml = a.part_ml + w * a.n_chunk;
-  const float *po = a.part_o + w * a.n_chunk * DH;
+  const float2 *ml = a.part_ml + row * a.n_chunk;
+  const float *po = a.part_o + row * a.n_chunk * DH + V * lane;
   float M = -CUDART_INF_F;
-  for (int c = lane; c < nch; c += 32) M = fmaxf(M, ml[c].x);
+  for (int c = w + W * lane; c < nch; c += 32 * W) M = fmaxf(M, ml[c].x);
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
-  constexpr int V = DH / 32;
   float L = 0.0f, acc[V];
 #pragma unroll
   for (int j = 0; j < V; j++) acc[j] = 0.0f;
-  for (int c = 0; c < nch; c++) {
-    const float2 x = ml[c];
-    const float f = x.y == 0.0f ? 0.0f : ex2(x.x - M);
-    L = fmaf(f, x.y, L);
-    if (f == 0.0f) continue;
+  for (int c0 = w; c0 < nch; c0 += 4 * W) {
+    float2 x[4];
+    float v[4][V];
 #pragma unroll
-    for (int j = 0; j < V; j++) acc[j] = fmaf(f, po[(size_t)c * DH + V * lane + j], acc[j]);
+    for (int k = 0; k < 4; k++) {
+      const int c = min(c0 + k * W, nch - 1);
+      x[k] = ml[c];
+      if (V == 4) *reinterpret_cast<float4 *>(v[k]) = *reinterpret_cast<const float4 *>(po + (size_t)c * DH);
+      else *reinterpret_cast<float2 *>(v[k]) = *reinterpret_cast<const float2 *>(po + (size_t)c * DH);
+    }
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const float f = c0 + k * W >= nch || x[k].y == 0.0f ? 0.0f : ex2(x[k].x - M);  // a NaN sum stays one
+      L = fmaf(f, x[k].y, L);
+#pragma unroll
+      for (int j = 0; j < V; j++)
+        if (f != 0.0f) acc[j] = fmaf(f, v[k][j], acc[j]);
+    }
+  }
+  if (W > 1) {
+    if (lane == 0) sml[w] = make_float2(M, L);
+#pragma unroll
+    for (int j = 0; j < V; j++) so[w][V * lane + j] = acc[j];
+    __syncthreads();
+    if (w > 0) return;
+    M = -CUDART_INF_F;
+#pragma unroll
+    for (int k = 0; k < W; k++) M = fmaxf(M, sml[k].x);
+    L = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; j++) acc[j] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < W; k++) {
+      const float f = sml[k].y == 0.0f ? 0.0f : ex2(sml[k].x - M);
+      L = fmaf(f, sml[k].y, L);
+#pragma unroll
+      for (int j = 0; j < V; j++) acc[j] = fmaf(f, so[k][V * lane + j], acc[j]);
+    }
   }
   const float inv = L > 0.0f || isnan(L) ? 1.0f / L : 0.0f;
   const long long off = tok * a.q.out_tok_stride + (long long)h * a.q.out_head_stride + V * lane;
@@ -643,16 +679,21 @@ Variant variant_as() {
   return {k_kv_attn<TYPE, DH, NT, NB, RG>, G::SMEM, G::ROWS};
 }
 // From TC_FROM rows on half-precision queries take the tcgen05 kernel.
-constexpr long long TC_FROM = PK_TCFROM;
+// (16 rows: 281 us here and 513 there for 40 sequences of 15000 positions; 24: 513 and 517.)
+constexpr long long TC_FROM = 17;
 template <int TYPE, int DH, int NT>
 Variant variant_rows(long long rows) {
-  constexpr int NBM = NT == 2 && DH == 128 ? 2 : 4;
-  if (NT == 1 && rows >= TC_FROM) return {nullptr, 0, TC_ATTN_ROWS};
   if (rows <= 8) return variant_as<TYPE, DH, NT, 1, 1>();
   if (rows <= 16) return variant_as<TYPE, DH, NT, 2, 1>();
-  if (rows <= 8 * NBM) return variant_as<TYPE, DH, NT, NBM, 1>();
-  if (rows <= 16 * NBM) return variant_as<TYPE, DH, NT, NBM, 2>();
-  return variant_as<TYPE, DH, NT, NBM, 4>();
+  if constexpr (NT == 1) {
+    static_assert(TC_FROM == 17, "half-precision rows past 16");
+    return {nullptr, 0, TC_ATTN_ROWS};
+  } else {
+    constexpr int NBM = DH == 128 ? 2 : 4;
+    if (rows <= 8 * NBM) return variant_as<TYPE, DH, NT, NBM, 1>();
+    if (rows <= 16 * NBM) return variant_as<TYPE, DH, NT, NBM, 2>();
+    return variant_as<TYPE, DH, NT, NBM, 4>();
+  }
 }
 template <int TYPE, int DH>
 Variant variant_type(int type, long long rows) {
@@ -714,13 +755,14 @@ cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_k
   a.cluster = p.cluster;
   a.part_ml = p.n_chunk > 1 && !a.cluster ? reinterpret_cast<float2 *>(a.part_o + rows * p.n_chunk * c.head_dim) : nullptr;
   const long long blocks = (long long)s.n_seq * c.n_kv * p.row_tiles * p.n_chunk, jb = ((long long)rows + 3) / 4;
-  if (blocks > 0x7fffffffLL || jb > 0x7fffffffLL) return cudaErrorInvalidValue;
+  if (blocks > 0x7fffffffLL || (long long)rows > 0x7fffffffLL) return cudaErrorInvalidValue;
   const int cluster = a.cluster ? p.n_chunk : 1;
   cudaError_t e;
   if (!v.k) e = launch_kv_attn_tc(a, cluster, (unsigned)blocks, st);
   else e = launch_cluster(v.k, cluster, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
   if (e != cudaSuccess || p.n_chunk <= 1 || a.cluster) return e;
-  return launch(c.head_dim == 64 ? k_kv_attn_join<64> : k_kv_attn_join<128>, dim3((unsigned)jb), dim3(128), 0, st, a);
+  if (p.n_chunk <= 8) return launch(c.head_dim == 64 ? k_kv_attn_join<64, 1> : k_kv_attn_join<128, 1>, dim3((unsigned)jb), dim3(128), 0, st, a);
+  return launch(c.head_dim == 64 ? k_kv_attn_join<64, 8> : k_kv_attn_join<128, 8>, dim3((unsigned)rows), dim3(256), 0, st, a);
 }
 
 }  // namespace pk
