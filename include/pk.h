@@ -230,7 +230,13 @@ int pk_set_order(pk_engine *eng, int order);
  * each K and V value rounded to nearest even, halving the cache (M26: 368,640
  * instead of 737,280 bytes a position); every later read converts it back
  * exactly, and all other arithmetic is unchanged.  With f16 entries decode
- * runs the per-op kernels and attention the per-(token, head) kernel. */
+ * runs the per-op kernels and attention the per-(token, head) kernel.
+ * PK_KV_Q8 and PK_KV_Q4 (below) keep the engine's and its streams' K and V in
+ * quantised pages: rotary, store and attention are then pk_rope's,
+ * pk_kv_store's and pk_kv_attn's kernels, so the sums are no longer in the
+ * reference's order; everything else of a pass is unchanged.  head_dim must be
+ * 64 or 128 (else pk_load_gguf returns PK_ERR_UNSUPPORTED), and pk_forward
+ * takes consecutive positions only (else PK_ERR_UNSUPPORTED). */
 #define PK_KV_F32 0
 #define PK_KV_F16 1
 int pk_set_kv_type(pk_engine *eng, int type);

@@ -43,6 +43,9 @@ Engine::~Engine() {
   cudaFree(d_sample_scratch_);
   cudaFree(d_sk_);
   cudaFree(d_sv_);
+  cudaFree(d_qcache_);
+  cudaFree(d_qstreams_);
+  cudaFree(d_qaux_);
   cudaFree(d_slogits_);
   cudaFreeHost(h_ids_);
   cudaFreeHost(h_pos_);
@@ -274,11 +277,15 @@ int Engine::load(const char *path) {
   // ---- KV cache (model.rs:352-387), f32: V as the reference lays it out,
   // [layer][kv_head][n_ctx][dh]; K d-major, [layer][kv_head][dh][n_ctx], so a
   // run of positions of one dimension is contiguous for the score pass.
-  kv_bytes_ = 2 * (size_t)c.n_layer * c.n_head_kv * n_ctx_ * c.head_dim * (kv_f16_ ? 2 : 4);
-  PK_CK(cudaMalloc((void **)&d_kcache_, kv_bytes_ / 2));
-  PK_CK(cudaMalloc((void **)&d_vcache_, kv_bytes_ / 2));
-  PK_CK(cudaMemsetAsync(d_kcache_, 0, kv_bytes_ / 2, st_));
-  PK_CK(cudaMemsetAsync(d_vcache_, 0, kv_bytes_ / 2, st_));
+  if (kv_q_) {
+    if ((rc = setup_qcache())) return rc;
+  } else {
+    kv_bytes_ = 2 * (size_t)c.n_layer * c.n_head_kv * n_ctx_ * c.head_dim * (kv_f16_ ? 2 : 4);
+    PK_CK(cudaMalloc((void **)&d_kcache_, kv_bytes_ / 2));
+    PK_CK(cudaMalloc((void **)&d_vcache_, kv_bytes_ / 2));
+    PK_CK(cudaMemsetAsync(d_kcache_, 0, kv_bytes_ / 2, st_));
+    PK_CK(cudaMemsetAsync(d_vcache_, 0, kv_bytes_ / 2, st_));
+  }
 
   // ---- RoPE tables, computed exactly like Scratch::new / ensure_rope
   // (model.rs:414-417, 452-457) with the C library's powf/cosf/sinf.
@@ -378,6 +385,101 @@ int Engine::load(const char *path) {
   return setup_decode();
 }
 
+#define PROF(name, bytes, launch)                 \
+  do {                                            \
+    int _rc = prof_begin(name, (double)(bytes));  \
+    if (_rc) return _rc;                          \
+    PK_CK(launch);                                \
+    if ((_rc = prof_end())) return _rc;           \
+  } while (0)
+
+// ---- quantised K/V caches (no reference counterpart): the op-level cache,
+// rotary and attention kernels in place of the exact-order ones.
+size_t Engine::qpool_half(int n_pages) const {
+  return (size_t)cfg_.n_layer * n_pages * cfg_.n_head_kv * QPAGE * (kv_row_bytes(kv_q_, cfg_.head_dim) + 4 * kv_scale_words(kv_q_));
+}
+
+int Engine::setup_qcache() {
+  const Config &c = cfg_;
+  if (c.head_dim != 64 && c.head_dim != 128)
+    return set_error(PK_ERR_UNSUPPORTED, "a quantised KV cache needs head_dim 64 or 128, the model has " + std::to_string(c.head_dim));
+  const int np = (n_ctx_ + QPAGE - 1) / QPAGE;
+  kv_bytes_ = 2 * qpool_half(np);
+  PK_CK(cudaMalloc((void **)&d_qcache_, kv_bytes_));
+  PK_CK(cudaMemsetAsync(d_qcache_, 0, kv_bytes_, st_));
+  // the most scratch a batch of this engine's needs, tokens of one sequence or one of each stream
+  pk_kv_cache kc{};
+  kc.type = kv_q_; kc.page_size = QPAGE; kc.n_kv = c.n_head_kv; kc.head_dim = c.head_dim; kc.n_pages = np;
+  for (int b = 1; b <= max_batch_; b++) {
+    pk_kv_seqs s{};
+    s.max_pages = np; s.n_tok = b; s.max_len = n_ctx_;
+    s.n_seq = 1; s.max_new = b;
+    q_scratch_bytes_ = std::max(q_scratch_bytes_, kv_attn_scratch_bytes(kc, s, c.n_head, PK_TYPE_F32));
+    s.n_seq = b; s.max_new = 1;
+    q_scratch_bytes_ = std::max(q_scratch_bytes_, kv_attn_scratch_bytes(kc, s, c.n_head, PK_TYPE_F32));
+  }
+  std::vector<int> ids((size_t)std::max(np * max_batch_, 65)), start;
+  for (size_t i = 0; i < ids.size(); i++) ids[i] = (int)i;
+  for (int b = 0; b <= max_batch_; b++) {
+    start.push_back(0);
+    start.push_back(b);
+  }
+  std::vector<double> turns((size_t)std::max(c.n_rot / 2, 1));
+  pk_rope_spec spec{};
+  spec.n_rot = c.n_rot; spec.scaling = PK_ROPE_NONE; spec.theta = c.rope_theta;
+  if (const int rc = pk_rope_turns(&spec, turns.data(), &qgain_)) return rc;
+  const size_t n0 = a256(ids.size() * 4), n1 = a256(start.size() * 4), n2 = a256(turns.size() * 8), n3 = a256(q_scratch_bytes_);
+  PK_CK(cudaMalloc((void **)&d_qaux_, n0 + n1 + n2 + NLANES * n3));
+  PK_CK(cudaMemcpyAsync(d_qaux_, ids.data(), ids.size() * 4, cudaMemcpyHostToDevice, st_));
+  PK_CK(cudaMemcpyAsync(d_qaux_ + n0, start.data(), start.size() * 4, cudaMemcpyHostToDevice, st_));
+  PK_CK(cudaMemcpyAsync(d_qaux_ + n0 + n1, turns.data(), turns.size() * 8, cudaMemcpyHostToDevice, st_));
+  PK_CK(cudaStreamSynchronize(st_));
+  d_qiota_ = (const int *)d_qaux_;
+  d_qstart_ = (const int *)(d_qaux_ + n0);
+  d_qturns_ = (const double *)(d_qaux_ + n0 + n1);
+  for (int i = 0; i < NLANES; i++) q_scratch_[i] = d_qaux_ + n0 + n1 + n2 + i * n3;
+  qcur_ = {d_qcache_, d_qcache_ + kv_bytes_ / 2, np, d_qiota_};
+  return PK_OK;
+}
+
+pk_kv_cache Engine::qlayer(const QPool &p, int l) const {
+  const size_t rows = (size_t)p.n_pages * cfg_.n_head_kv * QPAGE, rb = kv_row_bytes(kv_q_, cfg_.head_dim), sb = 4 * kv_scale_words(kv_q_);
+  pk_kv_cache c{};
+  c.type = kv_q_; c.n_pages = p.n_pages; c.page_size = QPAGE; c.n_kv = cfg_.n_head_kv; c.head_dim = cfg_.head_dim;
+  c.k = p.k + l * rows * rb;
+  c.v = p.v + l * rows * rb;
+  c.ks = (float *)(p.k + cfg_.n_layer * rows * rb + l * rows * sb);
+  c.vs = (float *)(p.v + cfg_.n_layer * rows * rb + l * rows * sb);
+  return c;
+}
+
+// The attention block of layer l: q and k rotated in place, k and v quantised
+// into the cache, the attention's f32 output into out.  The arguments are the
+// engine's own, so the kernels are launched without the C boundary's checks.
+int Engine::q_attend(const QPool &p, const pk_kv_seqs &s, int l, float *q, float *k, float *v, const int *pos, float *out, int li,
+                     int kv, cudaStream_t st) {
+  const Config &c = cfg_;
+  const int dh = c.head_dim, qdim = c.n_head * dh, kdim = c.n_head_kv * dh, n = s.n_tok;
+  const double kv_pos = (double)next_pos_ + 1.0, row = kv_row_bytes(kv_q_, dh) + 4.0 * kv_scale_words(kv_q_);
+  const pk_kv_cache cache = qlayer(p, l);
+  pk_rope_args ra{};
+  ra.q = ra.q_out = q; ra.k = ra.k_out = k; ra.pos = pos; ra.turns = d_qturns_;
+  ra.q_tok_stride = ra.qo_tok_stride = qdim; ra.k_tok_stride = ra.ko_tok_stride = kdim;
+  ra.q_head_stride = ra.qo_head_stride = ra.k_head_stride = ra.ko_head_stride = dh;
+  ra.type = PK_TYPE_F32; ra.layout = PK_ROPE_INTERLEAVED; ra.n_tok = n; ra.n_head = c.n_head; ra.n_kv = c.n_head_kv;
+  ra.head_dim = dh; ra.n_rot = c.n_rot; ra.gain = qgain_;
+  PROF("k_rope", 8.0 * n * (qdim + kdim), launch_rope(ra, st));
+  PROF("k_kv_store", 8.0 * n * kdim + 2.0 * n * c.n_head_kv * row, launch_kv_store(cache, s, k, v, PK_TYPE_F32, kdim, dh, st));
+  // the wait comes first: a chunk's event then stands for all chunks before it
+  if (kv & KV_WAIT) PK_CK(cudaStreamWaitEvent(st, kv_ev_[(li + NLANES - 1) % NLANES][l], 0));
+  if (kv & KV_RECORD) PK_CK(cudaEventRecord(kv_ev_[li][l], st));
+  pk_kv_query qa{};
+  qa.q = q; qa.out = out; qa.q_tok_stride = qa.out_tok_stride = qdim; qa.q_head_stride = qa.out_head_stride = dh;
+  qa.type = PK_TYPE_F32; qa.n_head = c.n_head; qa.scale = 1.0f / sqrtf((float)dh);
+  PROF("k_kv_attn", 2.0 * c.n_head_kv * kv_pos * row + 8.0 * n * qdim, launch_kv_attn(cache, s, qa, q_scratch_[li], st));
+  return PK_OK;
+}
+
 // Plan and device tables of the persistent decode kernel.  A model it cannot
 // run (shared memory, shapes) keeps the per-op kernel sequence; the
 // environment variable PK_DECODE=ops selects that sequence as well.
@@ -388,8 +490,8 @@ int Engine::setup_decode() {
     decode_why_ = "PK_DECODE=ops";
     return PK_OK;
   }
-  if (kv_f16_) {
-    decode_why_ = "f16 KV cache: decode runs the per-op kernels";
+  if (kv_f16_ || kv_q_) {
+    decode_why_ = "f16 or quantised KV cache: decode runs the per-op kernels";
     return PK_OK;
   }
   const Config &c = cfg_;
@@ -569,14 +671,6 @@ static double mat_stream_bytes(const DevTensor &w) {
   return (double)w.rows * (double)(w.k / be) * (double)bb;
 }
 
-#define PROF(name, bytes, launch)                 \
-  do {                                            \
-    int _rc = prof_begin(name, (double)(bytes));  \
-    if (_rc) return _rc;                          \
-    PK_CK(launch);                                \
-    if ((_rc = prof_end())) return _rc;           \
-  } while (0)
-
 // The per-token kernel sequence (model.rs:857-1170) on prefill lane li.
 // Reads ids/positions from the lane's device buffers, so a b == 1 pass
 // (lane 0) can be captured once as a CUDA graph.  kv & KV_RECORD: record
@@ -595,25 +689,41 @@ int Engine::enqueue_forward(int b, bool want_logits, bool cancellable, int li, i
   at.q = S.q; at.pos = S.pos; at.out = S.attn; at.b = b; at.n_head = c.n_head; at.n_kv = c.n_head_kv; at.dh = dh;
   at.n_ctx = n_ctx_; at.scale = 1.0f / sqrtf((float)dh);
   at.scores = S.scores;
+  pk_kv_seqs qs{};  // the batch as the quantised cache's one sequence: tokens at pos[0] ..
+  if (kv_q_) {
+    qs.start = d_qstart_ + 2 * b; qs.ctx = S.pos; qs.pages = qcur_.pages;
+    qs.n_seq = 1; qs.max_pages = (n_ctx_ + QPAGE - 1) / QPAGE; qs.n_tok = qs.max_new = b; qs.max_len = n_ctx_;
+  }
   for (int l = 0; l < c.n_layer; l++) {
     if (cancellable && g_stop.load()) return set_error(PK_ERR_STOPPED, "generation stopped");
     const LayerDev &L = layers_[l];
     float *kc = kv_at(d_kcache_, l * layer_kv), *vc = kv_at(d_vcache_, l * layer_kv);
     at.kcache = kc; at.vcache = vc; at.kv16 = kv_f16_ ? 1 : 0;
     if (b == 1) {
-      QkvArgs qa;
-      qa.wq = L.q; qa.wk = L.k; qa.wv = L.v;
-      qa.src.x = S.x; qa.src.nw = L.attn_norm; qa.src.eps = c.rms_eps;
-      qa.pos = S.pos; qa.rope_cos = d_rope_cos_; qa.rope_sin = d_rope_sin_;
-      qa.half = c.n_rot / 2; qa.dh = dh; qa.n_ctx = n_ctx_;
-      qa.qout = S.q; qa.kcache = kc; qa.vcache = vc; qa.kv16 = kv_f16_ ? 1 : 0;
-      PROF("k_qkv_b1", mat_stream_bytes(L.q) + mat_stream_bytes(L.k) + mat_stream_bytes(L.v) + 2 * ne * f4 +
-                           (qdim + 2 * kdim) * f4,
-           launch_qkv_b1(qa, S.st));
-      if (l == 0) dump("Qrope-0", S.q, (size_t)qdim);
-      if (kv & KV_RECORD) PK_CK(cudaEventRecord(kv_ev_[li][l], S.st));
-      if (kv & KV_WAIT) PK_CK(cudaStreamWaitEvent(S.st, kv_ev_[(li + NLANES - 1) % NLANES][l], 0));
-      PROF("k_attn", 2.0 * c.n_head_kv * kv_pos * dh * f4 + 2 * qdim * f4, launch_attention(at, S.st));
+      if (kv_q_) {
+        B1Src sa;
+        sa.x = S.x; sa.nw = L.attn_norm; sa.eps = c.rms_eps;
+        PROF("k_mv_b1", mat_stream_bytes(L.q) + 2 * ne * f4 + qdim * f4, launch_mv_b1(L.q, sa, S.q, false, S.st));
+        PROF("k_mv_b1", mat_stream_bytes(L.k) + 2 * ne * f4 + kdim * f4, launch_mv_b1(L.k, sa, S.k, false, S.st));
+        PROF("k_mv_b1", mat_stream_bytes(L.v) + 2 * ne * f4 + kdim * f4, launch_mv_b1(L.v, sa, S.v, false, S.st));
+        if (l == 0) { dump("Qcur-0", S.q, qdim); dump("Kcur-0", S.k, kdim); dump("Vcur-0", S.v, kdim); }
+        if (const int rc = q_attend(qcur_, qs, l, S.q, S.k, S.v, S.pos, S.attn, li, kv, S.st)) return rc;
+        if (l == 0) { dump("Qrope-0", S.q, qdim); dump("kqv_out-0", S.attn, qdim); }
+      } else {
+        QkvArgs qa;
+        qa.wq = L.q; qa.wk = L.k; qa.wv = L.v;
+        qa.src.x = S.x; qa.src.nw = L.attn_norm; qa.src.eps = c.rms_eps;
+        qa.pos = S.pos; qa.rope_cos = d_rope_cos_; qa.rope_sin = d_rope_sin_;
+        qa.half = c.n_rot / 2; qa.dh = dh; qa.n_ctx = n_ctx_;
+        qa.qout = S.q; qa.kcache = kc; qa.vcache = vc; qa.kv16 = kv_f16_ ? 1 : 0;
+        PROF("k_qkv_b1", mat_stream_bytes(L.q) + mat_stream_bytes(L.k) + mat_stream_bytes(L.v) + 2 * ne * f4 +
+                             (qdim + 2 * kdim) * f4,
+             launch_qkv_b1(qa, S.st));
+        if (l == 0) dump("Qrope-0", S.q, (size_t)qdim);
+        if (kv & KV_RECORD) PK_CK(cudaEventRecord(kv_ev_[li][l], S.st));
+        if (kv & KV_WAIT) PK_CK(cudaStreamWaitEvent(S.st, kv_ev_[(li + NLANES - 1) % NLANES][l], 0));
+        PROF("k_attn", 2.0 * c.n_head_kv * kv_pos * dh * f4 + 2 * qdim * f4, launch_attention(at, S.st));
+      }
       B1Src so;
       so.x = S.attn;
       PROF("k_mv_b1", mat_stream_bytes(L.o) + qdim * f4 + 2 * ne * f4, launch_mv_b1(L.o, so, S.x, true, S.st));
@@ -633,15 +743,21 @@ int Engine::enqueue_forward(int b, bool want_logits, bool cancellable, int li, i
       const MvOut qkv[3] = {{L.q, S.q, 1, qdim, false}, {L.k, S.k, 1, kdim, false}, {L.v, S.v, 1, kdim, false}};
       PK_CK(launch_mv_multi(3, qkv, a, st));
       if (l == 0) { dump("Qcur-0", S.q, (size_t)b * qdim); dump("Kcur-0", S.k, (size_t)b * kdim); dump("Vcur-0", S.v, (size_t)b * kdim); }
-      PK_CK(launch_rope_kv(S.q, S.k, S.v, b, S.pos, d_rope_cos_, d_rope_sin_, c.n_rot / 2, dh, c.n_head, c.n_head_kv,
-                           n_ctx_, kc, vc, st, 0, kv_f16_));
-      if (kv & KV_RECORD) PK_CK(cudaEventRecord(kv_ev_[li][l], st));
-      if (l == 0) dump("Qrope-0", S.q, (size_t)b * qdim);
-      if (kv & KV_WAIT) PK_CK(cudaStreamWaitEvent(st, kv_ev_[(li + NLANES - 1) % NLANES][l], 0));
       a.k = qdim;
-      AttnArgs atq = at;
-      atq.q8 = a;  // the attention kernel also writes Q8 of its output
-      PK_CK(launch_attention(atq, st));
+      if (kv_q_) {
+        if (const int rc = q_attend(qcur_, qs, l, S.q, S.k, S.v, S.pos, S.attn, li, kv, st)) return rc;
+        if (l == 0) { dump("Qrope-0", S.q, (size_t)b * qdim); dump("kqv_out-0", S.attn, (size_t)b * qdim); }
+        PK_CK(launch_q8(S.attn, 1, qdim, qdim, b, a, st));
+      } else {
+        PK_CK(launch_rope_kv(S.q, S.k, S.v, b, S.pos, d_rope_cos_, d_rope_sin_, c.n_rot / 2, dh, c.n_head, c.n_head_kv,
+                             n_ctx_, kc, vc, st, 0, kv_f16_));
+        if (kv & KV_RECORD) PK_CK(cudaEventRecord(kv_ev_[li][l], st));
+        if (l == 0) dump("Qrope-0", S.q, (size_t)b * qdim);
+        if (kv & KV_WAIT) PK_CK(cudaStreamWaitEvent(st, kv_ev_[(li + NLANES - 1) % NLANES][l], 0));
+        AttnArgs atq = at;
+        atq.q8 = a;  // the attention kernel also writes Q8 of its output
+        PK_CK(launch_attention(atq, st));
+      }
       PK_CK(launch_mv_lanes(L.o, a, S.x, 1, ne, true, st));
       if (l == 0) dump("ffn_inp-0", S.x, (size_t)b * ne);
       a.k = ne;
@@ -714,6 +830,8 @@ int Engine::forward_inner(const uint32_t *ids, const int *pos, int b, bool want_
   for (int i = 0; i < b; i++) {
     if (pos[i] < 0 || pos[i] >= n_ctx_) return set_error(PK_ERR_CONTEXT_FULL, "context full");
     if (ids[i] >= (uint32_t)vocab_) return set_error(PK_ERR_INVALID, "token " + std::to_string(ids[i]) + " out of vocab");
+    if (kv_q_ && pos[i] != pos[0] + i)
+      return set_error(PK_ERR_UNSUPPORTED, "a quantised KV cache takes tokens at consecutive positions");
   }
   PK_CK(cudaSetDevice(device_));
   std::memcpy(h_ids_, ids, b * sizeof(uint32_t));
@@ -990,9 +1108,10 @@ int Engine::decode_steps_device(int n_steps, uint32_t *out_ids, float *device_ms
 // then).  f16 entries are each value rounded to nearest even; attention then
 // runs on the per-(token, head) kernel and decode on the per-op kernels.
 int Engine::set_kv_type(int type) {
-  if (type != PK_KV_F32 && type != PK_KV_F16) return set_error(PK_ERR_INVALID, "unknown KV cache type");
+  if (type < PK_KV_F32 || type > PK_KV_Q4) return set_error(PK_ERR_INVALID, "unknown KV cache type");
   if (loaded_) return set_error(PK_ERR_INVALID, "the KV cache type is set before the model loads");
   kv_f16_ = type == PK_KV_F16;
+  kv_q_ = type == PK_KV_Q8 || type == PK_KV_Q4 ? type : 0;
   return PK_OK;
 }
 
@@ -1027,11 +1146,16 @@ int Engine::streams_begin(int n) {
   if (n < 1 || n > max_batch_ || n > 64) return set_error(PK_ERR_INVALID, "streams: 1..max_batch streams");
   if (n_streams_) return set_error(PK_ERR_INVALID, "streams already begun");
   PK_CK(cudaSetDevice(device_));
-  const size_t half = kv_bytes_ / 2;
-  PK_CK(cudaMalloc((void **)&d_sk_, half * n));
-  PK_CK(cudaMalloc((void **)&d_sv_, half * n));
-  PK_CK(cudaMemsetAsync(d_sk_, 0, half * n, st_));
-  PK_CK(cudaMemsetAsync(d_sv_, 0, half * n, st_));
+  if (kv_q_) {
+    PK_CK(cudaMalloc((void **)&d_qstreams_, kv_bytes_ * n));
+    PK_CK(cudaMemsetAsync(d_qstreams_, 0, kv_bytes_ * n, st_));
+  } else {
+    const size_t half = kv_bytes_ / 2;
+    PK_CK(cudaMalloc((void **)&d_sk_, half * n));
+    PK_CK(cudaMalloc((void **)&d_sv_, half * n));
+    PK_CK(cudaMemsetAsync(d_sk_, 0, half * n, st_));
+    PK_CK(cudaMemsetAsync(d_sv_, 0, half * n, st_));
+  }
   // histories above 1024 positions: the attention's scores are split over
   // chunks of 512 (1024 above 8192) positions, whose maxima need scratch
   spchunk_ = n_ctx_ > 1024 ? (n_ctx_ > 8192 ? 1024 : 512) : 0;
@@ -1065,8 +1189,13 @@ int Engine::stream_prefill(int s, const uint32_t *prompt, int n) {
   PK_CK(cudaSetDevice(device_));
   const size_t per = (size_t)cfg_.n_layer * cfg_.n_head_kv * n_ctx_ * cfg_.head_dim;  // entries of one cache
   float *k0 = d_kcache_, *v0 = d_vcache_;
-  d_kcache_ = kv_at(d_sk_, (size_t)s * per);
-  d_vcache_ = kv_at(d_sv_, (size_t)s * per);
+  const QPool q0 = qcur_;
+  if (kv_q_) {
+    qcur_ = qstream(s);
+  } else {
+    d_kcache_ = kv_at(d_sk_, (size_t)s * per);
+    d_vcache_ = kv_at(d_sv_, (size_t)s * per);
+  }
   kv_tokens_.clear();
   cached_prefill_len_ = 0;
   int rc = PK_OK;
@@ -1090,6 +1219,7 @@ int Engine::stream_prefill(int s, const uint32_t *prompt, int n) {
   if (!rc) rc = argmax(&tok);
   d_kcache_ = k0;
   d_vcache_ = v0;
+  qcur_ = q0;
   have_logits_ = false;  // the engine's own sequence is not what the logits belong to
   next_pos_ = 0;
   if (rc) return rc;
@@ -1097,6 +1227,13 @@ int Engine::stream_prefill(int s, const uint32_t *prompt, int n) {
   stok_[s] = tok;
   sready_[s] = 1;
   return PK_OK;
+}
+
+// Stream s's pages of the streams' pool (stream s's page j is s * pages + j).
+Engine::QPool Engine::qstream(int s) const {
+  const int np = (n_ctx_ + QPAGE - 1) / QPAGE;
+  const size_t half = kv_bytes_ / 2 * n_streams_;
+  return {d_qstreams_, d_qstreams_ + half, np * n_streams_, d_qiota_ + (size_t)s * np};
 }
 
 int Engine::enqueue_streams_step() {
@@ -1112,17 +1249,25 @@ int Engine::enqueue_streams_step() {
     PK_CK(launch_rmsnorm_q8(x_, L.attn_norm, c.rms_eps, ne, S, a, nullptr, st_, true));
     const MvOut qkv[3] = {{L.q, q_, 1, qdim, false}, {L.k, k_, 1, kdim, false}, {L.v, v_, 1, kdim, false}};
     PK_CK(launch_mv_multi(3, qkv, a, st_));
-    PK_CK(launch_rope_kv(q_, k_, v_, S, d_spos_, d_rope_cos_, d_rope_sin_, c.n_rot / 2, dh, c.n_head, c.n_head_kv,
-                         n_ctx_, kc, vc, st_, stride, kv_f16_));
-    AttnArgs at{};
-    at.q = q_; at.kcache = kc; at.vcache = vc; at.pos = d_spos_; at.out = attn_; at.b = S;
-    at.n_head = c.n_head; at.n_kv = c.n_head_kv; at.dh = dh; at.n_ctx = n_ctx_;
-    at.scale = 1.0f / sqrtf((float)dh); at.scores = att_scores_;
-    at.lane_stride = stride; at.b1_order = 1; at.kv16 = kv_f16_ ? 1 : 0;
-    at.pmax = d_spmax_; at.pchunk = spchunk_;
     a.k = qdim;
-    at.q8 = a;
-    PK_CK(launch_attention(at, st_));
+    if (kv_q_) {  // one token of each stream
+      pk_kv_seqs qs{};
+      qs.start = d_qiota_; qs.ctx = d_spos_; qs.pages = d_qiota_;
+      qs.n_seq = qs.n_tok = S; qs.max_pages = (n_ctx_ + QPAGE - 1) / QPAGE; qs.max_new = 1; qs.max_len = n_ctx_;
+      if (const int rc = q_attend(qstream(0), qs, l, q_, k_, v_, d_spos_, attn_, 0, 0, st_)) return rc;
+      PK_CK(launch_q8(attn_, 1, qdim, qdim, S, a, st_));
+    } else {
+      PK_CK(launch_rope_kv(q_, k_, v_, S, d_spos_, d_rope_cos_, d_rope_sin_, c.n_rot / 2, dh, c.n_head, c.n_head_kv,
+                           n_ctx_, kc, vc, st_, stride, kv_f16_));
+      AttnArgs at{};
+      at.q = q_; at.kcache = kc; at.vcache = vc; at.pos = d_spos_; at.out = attn_; at.b = S;
+      at.n_head = c.n_head; at.n_kv = c.n_head_kv; at.dh = dh; at.n_ctx = n_ctx_;
+      at.scale = 1.0f / sqrtf((float)dh); at.scores = att_scores_;
+      at.lane_stride = stride; at.b1_order = 1; at.kv16 = kv_f16_ ? 1 : 0;
+      at.pmax = d_spmax_; at.pchunk = spchunk_;
+      at.q8 = a;
+      PK_CK(launch_attention(at, st_));
+    }
     PK_CK(launch_mv_lanes(L.o, a, x_, 1, ne, true, st_));
     a.k = ne;
     PK_CK(launch_rmsnorm_q8(x_, L.ffn_norm, c.rms_eps, ne, S, a, nullptr, st_, true));

@@ -9,6 +9,7 @@
 #include "pk.h"
 #include "pk_gguf.h"
 #include "pk_decode.h"
+#include "pk_cache.h"
 #include "pk_kernels.h"
 
 namespace pk {
@@ -147,6 +148,31 @@ class Engine {
   bool use_decode_ = false;
   int order_ = PK_ORDER_EXACT;  // float order of the b = 1 decode step (pk_set_order)
   bool kv_f16_ = false;         // f16 K/V cache entries (pk_set_kv_type, before the model loads)
+  // Quantised caches (PK_KV_Q8, PK_KV_Q4; 0: not quantised): the paged cache of
+  // pk_cache.h, pages of QPAGE positions in order.  A pool holds all layers of
+  // one sequence (the engine's own) or of every stream, layer after layer;
+  // qcur_ is the sequence that a forward pass works on.
+  static constexpr int QPAGE = 64;
+  int kv_q_ = 0;
+  struct QPool {
+    uint8_t *k = nullptr, *v = nullptr;  // codes of all layers, then their scales
+    int n_pages = 0;
+    const int *pages = nullptr;          // device: this sequence's page table
+  };
+  QPool qcur_;
+  uint8_t *d_qcache_ = nullptr, *d_qstreams_ = nullptr;  // K's and V's halves
+  uint8_t *d_qaux_ = nullptr;  // page ids 0 .., {0, b} of every batch b, turns; each lane's attention scratch
+  const int *d_qiota_ = nullptr, *d_qstart_ = nullptr;
+  const double *d_qturns_ = nullptr;
+  float qgain_ = 1.0f;
+  uint8_t *q_scratch_[6] = {};
+  size_t q_scratch_bytes_ = 0;
+  size_t qpool_half(int n_pages) const;
+  int setup_qcache();
+  QPool qstream(int s) const;
+  pk_kv_cache qlayer(const QPool &p, int l) const;
+  int q_attend(const QPool &p, const pk_kv_seqs &s, int l, float *q, float *k, float *v, const int *pos, float *out, int li, int kv,
+               cudaStream_t st);
   // base + elems cache entries (f32 or f16), as the caches' float pointer type
   float *kv_at(float *base, size_t elems) const {
     return reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(base) + elems * (kv_f16_ ? 2 : 4));

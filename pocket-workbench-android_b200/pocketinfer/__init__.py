@@ -32,7 +32,7 @@ PK_ERR = {1: "PK_ERR_INVALID", 2: "PK_ERR_UNSUPPORTED", 3: "PK_ERR_CUDA", 4: "PK
 F32, F16, Q4_0, Q8_0, Q4_K, Q6_K, BF16 = 0, 1, 2, 8, 12, 14, 30
 ORDER_EXACT, ORDER_FAST = 0, 1  # pk_set_order
 MATMUL_MMA_SYNC, MATMUL_TCGEN05 = 0, 1  # pk_set_matmul_path
-KV_F32, KV_F16 = 0, 1  # pk_set_kv_type
+KV_F32, KV_F16, KV_Q8, KV_Q4 = 0, 1, 2, 3  # pk_set_kv_type
 BLOCK = {F32: (1, 4), F16: (1, 2), BF16: (1, 2), Q4_0: (32, 18), Q8_0: (32, 34), Q4_K: (256, 144), Q6_K: (256, 210)}
 
 # Every function include/pk.h declares (checked by tests/test_capi_symbols.py).
@@ -336,8 +336,8 @@ class Engine:
         self.n_ctx = n_ctx
         if order is not None:
             self.set_order(order)
-        if kv != "f32":  # "f16": f16 K/V cache entries (pk_set_kv_type), before the load
-            _check(lib().pk_set_kv_type(self.h, {"f32": KV_F32, "f16": KV_F16}[kv]))
+        if kv != "f32":  # "f16", "q8" or "q4" K/V caches (pk_set_kv_type), before the load
+            _check(lib().pk_set_kv_type(self.h, {"f32": KV_F32, "f16": KV_F16, "q8": KV_Q8, "q4": KV_Q4}[kv]))
         if path is not None:
             self.load(path)
 
