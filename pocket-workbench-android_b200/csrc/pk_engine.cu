@@ -675,7 +675,8 @@ static double mat_stream_bytes(const DevTensor &w) {
 // Reads ids/positions from the lane's device buffers, so a b == 1 pass
 // (lane 0) can be captured once as a CUDA graph.  kv & KV_RECORD: record
 // kv_ev_[li][l] once layer l's K/V are written; kv & KV_WAIT: layer l's
-// attention first waits for the previous lane's kv_ev_ of layer l.
+// attention first waits for the previous lane's kv_ev_ of layer l.  The wait
+// comes before the record, so that an event stands for all chunks before it.
 int Engine::enqueue_forward(int b, bool want_logits, bool cancellable, int li, int kv) {
   const Lane &S = lane_[li];
   const Config &c = cfg_;
@@ -720,8 +721,8 @@ int Engine::enqueue_forward(int b, bool want_logits, bool cancellable, int li, i
                              (qdim + 2 * kdim) * f4,
              launch_qkv_b1(qa, S.st));
         if (l == 0) dump("Qrope-0", S.q, (size_t)qdim);
-        if (kv & KV_RECORD) PK_CK(cudaEventRecord(kv_ev_[li][l], S.st));
         if (kv & KV_WAIT) PK_CK(cudaStreamWaitEvent(S.st, kv_ev_[(li + NLANES - 1) % NLANES][l], 0));
+        if (kv & KV_RECORD) PK_CK(cudaEventRecord(kv_ev_[li][l], S.st));
         PROF("k_attn", 2.0 * c.n_head_kv * kv_pos * dh * f4 + 2 * qdim * f4, launch_attention(at, S.st));
       }
       B1Src so;
@@ -751,9 +752,9 @@ int Engine::enqueue_forward(int b, bool want_logits, bool cancellable, int li, i
       } else {
         PK_CK(launch_rope_kv(S.q, S.k, S.v, b, S.pos, d_rope_cos_, d_rope_sin_, c.n_rot / 2, dh, c.n_head, c.n_head_kv,
                              n_ctx_, kc, vc, st, 0, kv_f16_));
-        if (kv & KV_RECORD) PK_CK(cudaEventRecord(kv_ev_[li][l], st));
         if (l == 0) dump("Qrope-0", S.q, (size_t)b * qdim);
         if (kv & KV_WAIT) PK_CK(cudaStreamWaitEvent(st, kv_ev_[(li + NLANES - 1) % NLANES][l], 0));
+        if (kv & KV_RECORD) PK_CK(cudaEventRecord(kv_ev_[li][l], st));
         AttnArgs atq = at;
         atq.q8 = a;  // the attention kernel also writes Q8 of its output
         PK_CK(launch_attention(atq, st));
