@@ -5,13 +5,14 @@
 // A CTA takes 128 rows (token, query head) of one kv head over one chunk of
 // positions, 64 at a time: S = Q K^T (M 128 x N 64 x K head_dim) into one of
 // two TMEM buffers, weights P in their place, O += P V (M 128 x N head_dim x
-// K 64) in TMEM.  288 threads:
-//   warps 0-3  softmax: thread = row = TMEM lane.  Scores from TMEM, the
-//              scales D^K and D^V applied in f32 (two at a time), weights as
-//              f16 into the scores' columns.
-//   warps 4-7  codes: a tile's K and V rows are asked for a tile ahead, made
-//              f16 (exact) and put into the operands' layout.
-//   warp 8     issues the products.
+// K 64) in TMEM.  416 threads:
+//   warps 0-3   softmax: thread = row = TMEM lane.  Scores from TMEM, the
+//               scales D^K and D^V applied in f32 (two at a time), weights as
+//               f16 into the scores' columns.
+//   warps 4-7   K's codes, and the scales of both: a tile's are asked for a
+//               tile ahead, made f16 (exact) and put into the operand's layout.
+//   warps 8-11  V's codes.
+//   warp 12     issues the products.
 // Two CTAs share an SM (100 KB and 256 TMEM columns each), so that one's
 // products run beside the other's softmax.  Operands are in the canonical
 // layout without swizzle, core matrices of 8 rows x 16 bytes.  V's rows are
@@ -39,7 +40,12 @@ namespace {
 
 constexpr int NK = 64;                      // positions a tile
 constexpr int ROWS = TC_ATTN_ROWS;
-constexpr int SOFT = 128, CONV = 128, THREADS = SOFT + CONV + 32;
+constexpr int SOFT = 128, CONV = 128, THREADS = SOFT + 2 * CONV + 32;
+// Registers: two CTAs an SM leave 72 a thread; the code warps' share of them
+// goes to the softmax's.
+constexpr int REGS = 72, REGS_SOFT = 112, REGS_CONV = 48;
+static_assert(SOFT * REGS_SOFT + 2 * CONV * REGS_CONV + 32 * REGS <= THREADS * REGS, "no more than the launch's");
+static_assert(2 * THREADS * REGS <= 65536, "two CTAs an SM");
 constexpr unsigned long long WAIT_NS = 2000000000ull;
 
 template <int DH>
@@ -48,12 +54,10 @@ struct Lay {
   // stride is 16 bytes more than its 64 positions, so that the 16 lanes that
   // store a position's chunks touch every bank once
   static constexpr int CH = NK * 16 + 16, TILE = DH / 8 * CH;
-  static constexpr int Q = 0, K = Q + ROWS * DH * 2, V = K + 2 * TILE, RAW = V + TILE;
-  // codes in flight, K's and V's, 16 bytes a thread and pass
-  static constexpr int RAWB = NK * DH, SC = RAW + 2 * RAWB;
-  // of three tiles: D^K [NK], D^V [NK]; positions that hold something (2 words), largest D^V of 32 (2)
-  static constexpr int SCB = 2 * NK * 4 + 16, BAR = SC + 3 * SCB, ML = BAR + 112, BYTES = ML + ROWS * 8;
-  static_assert(ROWS * (DH + 4) * 4 <= RAW, "a cluster's sums take the operands' place, not that of copies in flight");
+  static constexpr int Q = 0, K = Q + ROWS * DH * 2, V = K + 2 * TILE, SC = V + 2 * TILE;
+  // of four tiles: D^K [NK], D^V [NK]; positions that hold something (2 words), largest D^V of 32 (2)
+  static constexpr int SCB = 2 * NK * 4 + 16, BAR = SC + 4 * SCB, ML = BAR + 112, BYTES = ML + ROWS * 8;
+  static_assert(ROWS * (DH + 4) * 4 <= SC, "a cluster's sums take the operands' place");
   static constexpr int S_COL = 0, O_COL = 2 * NK, COLS = 256;
 };
 
@@ -66,6 +70,13 @@ __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int
       if (gtime_ns() - t0 > WAIT_NS) *abort = 1;
   }
   __syncwarp();
+}
+
+// This warpgroup's registers a thread from here on.
+template <bool MORE, int N>
+__device__ __forceinline__ void set_regs() {
+  if (MORE) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+  else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
 // A descriptor of an operand without swizzle (pk_tcgen05.cuh): K-major a =
@@ -205,7 +216,6 @@ template <int TYPE, int DH>
 __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
   using L = Lay<DH>;
   constexpr int RB = TYPE == PK_KV_Q8 ? DH : DH / 2, SW = TYPE == PK_KV_Q8 ? 1 : 2;
-  constexpr int W = RB / 32;  // 16-byte words of half a row
   extern __shared__ __align__(1024) uint8_t smem[];
   pdl_wait();
   const Unit u = unit_of(a);
@@ -217,9 +227,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
   }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sb = shaddr(smem);
-  // barriers: S full x 2, K and scales ready x 4, P ready x 2, PV done x 2, V ready; the TMEM address; the abort flag
+  // barriers: S full x 2, K and scales ready x 4, P ready x 2, PV done x 2, V ready x 2; the TMEM address; the abort flag
   const uint32_t bar = sb + L::BAR, sfull = bar, kready = bar + 16, pready = bar + 48, pvdone = bar + 64, vready = bar + 80;
-  volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 92);
+  volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 100);
   if (tid == 0) {
     mbar_init(sfull, 2);  // the products, and the warp that issues them (which has seen the scales)
     mbar_init(sfull + 8, 2);
@@ -227,13 +237,14 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     mbar_init(pready, SOFT);
     mbar_init(pready + 8, SOFT);
     mbar_init(vready, CONV);
+    mbar_init(vready + 8, CONV);
     mbar_init(pvdone, 1);
     mbar_init(pvdone + 8, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 8) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 88), "r"(L::COLS) : "memory");
+  if (warp == 12) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 96), "r"(L::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   const int row = tile0 + tid;
@@ -247,13 +258,13 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
   __syncthreads();
   tc_fence_after();
   pdl_trigger();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::BAR + 88);
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::BAR + 96);
   // without a mask nobody sees past the tile's last token
   const int last = (min(tile0 + ROWS, u.rows) - 1) / a.group;
   const int hi = a.q.mask ? u.hi : min(u.hi, u.sv.ctx + last + 1);
   const int nt = hi > u.lo ? (hi - u.lo + NK - 1) / NK : 0;
 
-  if (warp == 8) {  // ----------------------------------------------- products
+  if (warp == 12) {  // ---------------------------------------------- products
     auto scores = [&](int i) {
       wait(kready + 8 * (i & 3), (i >> 2) & 1, abort);
       tc_fence_after();
@@ -271,10 +282,10 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     if (nt > 0) scores(0);
     for (int i = 0; i < nt; i++) {
       if (i + 1 < nt) scores(i + 1);  // (into the columns of tile i - 1's weights: products are done in order)
-      wait(vready, i & 1, abort);
+      wait(vready + 8 * (i & 1), (i >> 1) & 1, abort);
       wait(pready + 8 * (i & 1), (i >> 1) & 1, abort);
       tc_fence_after();
-      uint32_t w = tmem + L::S_COL + (i & 1) * NK, v = sb + L::V;
+      uint32_t w = tmem + L::S_COL + (i & 1) * NK, v = sb + L::V + (i & 1) * L::TILE;
       asm volatile("" : "+r"(w), "+r"(v));
 #pragma unroll
       for (int s = 0; s < NK / 16; s++)
@@ -283,16 +294,15 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     }
   } else if (tid >= SOFT) {  // ---------------------------------------- codes
     // 16 bytes of a row a lane (RL lanes a row), NP passes of RP rows; a
-    // thread's row of pass w is w * RP + ct / RL.  The codes come by
-    // asynchronous copies into a place of the thread's own, from which it
-    // reads them back (left in registers, they tied up the loop: the loads of
-    // K and V wait for one another there).
+    // thread's row of pass w is w * RP + ct / RL.
+    set_regs<false, REGS_CONV>();
     constexpr int RL = RB / 16, RP = CONV / RL, NP = NK / RP;
-    const int ct = tid - SOFT, sub = ct % RL, key0 = ct / RL;
+    const bool is_v = warp >= 8;
+    const int ct = (tid - SOFT) & (CONV - 1), sub = ct % RL, key0 = ct / RL;
     const int key = ct & (NK - 1), half = ct >> 6;  // whose scale this thread passes on (half 0: K's, 1: V's)
     static_assert(RP % 16 == 0, "a pass has whole groups of 16 rows");
-    uint32_t sk[TYPE == PK_KV_Q4 ? NP : 1], sv[TYPE == PK_KV_Q4 ? NP : 1];  // the rows' sub-scales
-    const uint32_t rawk = sb + L::RAW + ct * 16, rawv = rawk + L::RAWB;
+    uint4 raw[NP];  // the next tile's codes and sub-scales
+    uint32_t subs[TYPE == PK_KV_Q4 ? NP : 1];
     float d = 0.0f;
     bool on = false;
     // Lane x of every warp holds, for the next 8 tiles, the cache rows of
@@ -300,38 +310,33 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     // positions or more): -1 where there is no page.  Such rows are read from
     // the cache's first, whose codes are as good as any (their scales are 0).
     int rows16 = -1;
-    const uint8_t *kp = reinterpret_cast<const uint8_t *>(a.c.k) + (key0 & 15) * RB + 16 * sub;
-    const uint8_t *vp = reinterpret_cast<const uint8_t *>(a.c.v) + (key0 & 15) * RB + 16 * sub;
-    const uint8_t *ksp = reinterpret_cast<const uint8_t *>(a.c.ks) + ((key0 & 15) * SW + 1) * 4;
-    const uint8_t *vsp = reinterpret_cast<const uint8_t *>(a.c.vs) + ((key0 & 15) * SW + 1) * 4;
+    const uint8_t *codes = reinterpret_cast<const uint8_t *>(is_v ? a.c.v : a.c.k) + (key0 & 15) * RB + 16 * sub;
+    const uint8_t *scales = reinterpret_cast<const uint8_t *>(is_v ? a.c.vs : a.c.ks) + ((key0 & 15) * SW + 1) * 4;
     const uint8_t *dp = reinterpret_cast<const uint8_t *>(half ? a.c.vs : a.c.ks) + (key & 15) * SW * 4;
-    auto look = [&](int i) {  // before tile i is asked for
-      if (i & 7) return;
-      const int p = u.lo + NK * (i + (lane >> 2)) + 16 * (lane & 3), j = p >> a.page_shift;
-      const int pg = p < hi && j < a.s.max_pages ? __ldg(a.s.pages + (size_t)u.s * a.s.max_pages + j) : -1;
-      rows16 = pg >= 0 && pg < a.c.n_pages
-                   ? (int)((((long long)pg * a.c.n_kv + u.h) * a.c.page_size + (p & (a.c.page_size - 1))) >> 4)
-                   : -1;
-    };
-    auto ask = [&](int i, uint32_t raw, uint32_t *subs, const uint8_t *codes, const uint8_t *scales) {
+    auto ask = [&](int i) {
+      if (!(i & 7)) {
+        const int p = u.lo + NK * (i + (lane >> 2)) + 16 * (lane & 3), j = p >> a.page_shift;
+        const int pg = p < hi && j < a.s.max_pages ? __ldg(a.s.pages + (size_t)u.s * a.s.max_pages + j) : -1;
+        rows16 = pg >= 0 && pg < a.c.n_pages
+                     ? (int)((((long long)pg * a.c.n_kv + u.h) * a.c.page_size + (p & (a.c.page_size - 1))) >> 4)
+                     : -1;
+      }
 #pragma unroll
       for (int w = 0; w < NP; w++) {
         const uint32_t r = max(__shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + w * (RP / 16) + key0 / 16), 0);
-        cp16(raw + w * (CONV * 16), codes + (size_t)r * (16 * RB));
+        raw[w] = __ldg(reinterpret_cast<const uint4 *>(codes + (size_t)r * (16 * RB)));
         if (TYPE == PK_KV_Q4) subs[w] = __ldg(reinterpret_cast<const uint32_t *>(scales + (size_t)r * (16 * SW * 4)));
       }
-      cp_commit();
+      if (!is_v) {
+        const int r = __shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + key / 16);
+        on = r >= 0 && u.lo + NK * i + key < hi;
+        d = __ldg(reinterpret_cast<const float *>(dp + (size_t)max(r, 0) * (16 * SW * 4)));
+      }
     };
-    auto ask_scale = [&](int i) {
-      const int r = __shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + key / 16);
-      on = r >= 0 && u.lo + NK * i + key < hi;
-      d = __ldg(reinterpret_cast<const float *>(dp + (size_t)max(r, 0) * (16 * SW * 4)));
-    };
-    auto put = [&](uint32_t dst, uint32_t raw, const uint32_t *subs) {
-      cp_wait<1>();  // (K's and V's copies take turns: all but the latest have landed)
+    auto put = [&](uint32_t dst) {
 #pragma unroll
       for (int w = 0; w < NP; w++) {
-        const uint4 x = sld_v4(raw + w * (CONV * 16));
+        const uint4 x = raw[w];
         const uint32_t at = dst + (w * RP + key0) * 16;
         if (TYPE == PK_KV_Q8) {
           // two chunks of 8 dimensions; half the lanes of a row begin with the
@@ -351,9 +356,10 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
         }
       }
     };
-    // both scales of tile i and the tile's summary
+    // both scales of tile i and the tile's summary, in place of tile i - 4's:
+    // tile i - 2's scores are full, so tile i - 4's weights have been used
     auto put_scales = [&](int i) {
-      uint8_t *sc = smem + L::SC + (i % 3) * L::SCB;
+      uint8_t *sc = smem + L::SC + (i & 3) * L::SCB;
       reinterpret_cast<float *>(sc)[half * NK + key] = on ? d : 0.0f;
       if (half == 0) {
         const unsigned m = __ballot_sync(0xffffffffu, on);
@@ -363,48 +369,20 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
         if (lane == 0) reinterpret_cast<uint32_t *>(sc + 2 * NK * 4 + 8)[key >> 5] = x;
       }
     };
-    // K is a tile ahead of V: tile i + 1's scores do not wait for tile i - 1's
-    // products with V, which tile i's V must (V has one buffer).  Tiles past
-    // the last are asked for as the last again, rather than under a condition
-    // that would keep the loads from being left in flight.
-    auto put_k = [&](int i) {
-      if (i >= 2) wait(sfull + 8 * (i & 1), ((i - 2) >> 1) & 1, abort);  // K of tile i - 2 has been used
-      put(sb + L::K + (i & 1) * L::TILE, rawk, sk);
-      put_scales(i);  // (those of tile i - 3 have: its products with V are done)
-      fence_async_smem();
-      mbar_arrive(kready + 8 * (i & 3));
-      const int n = min(i + 1, nt - 1);
-      if (n > i) look(n);
-      ask(n, rawk, sk, kp, ksp);
-      ask_scale(n);
-    };
-    if (nt > 0) {
-      look(0);
-      ask(0, rawk, sk, kp, ksp);
-      ask_scale(0);
-      const int rows_v = rows16;
-      cp_commit();  // (in V's turn)
-      put_k(0);
-      const int ahead = rows16;
-      rows16 = rows_v;
-      ask(0, rawv, sv, vp, vsp);
-      rows16 = ahead;
-    }
+    if (nt > 0) ask(0);
     for (int i = 0; i < nt; i++) {
-      const int rows_v = rows16;  // (K may go on to the next 8 tiles)
-      if (i + 1 < nt) put_k(i + 1);
-      else cp_commit();  // (in K's turn)
-      if (i >= 1) wait(pvdone + 8 * ((i - 1) & 1), ((i - 1) >> 1) & 1, abort);  // V of tile i - 1 has been used
-      put(sb + L::V, rawv, sv);
+      // K's buffer is free once tile i - 2's scores are there, V's once its
+      // products with V are
+      if (i >= 2) wait((is_v ? pvdone : sfull) + 8 * (i & 1), ((i - 2) >> 1) & 1, abort);
+      put(sb + (is_v ? L::V : L::K) + (i & 1) * L::TILE);
+      if (!is_v) put_scales(i);
       fence_async_smem();
-      mbar_arrive(vready);
-      const int ahead = rows16;
-      rows16 = rows_v;
-      ask(min(i + 1, nt - 1), rawv, sv, vp, vsp);
-      rows16 = ahead;
+      mbar_arrive(is_v ? vready + 8 * (i & 1) : kready + 8 * (i & 3));
+      if (i + 1 < nt) ask(i + 1);
     }
-    cp_wait<0>();
+    set_regs<true, REGS>();
   } else {  // ------------------------------------------------------------ softmax
+    set_regs<true, REGS_SOFT>();
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     const bool work = tile0 + warp * 32 < u.rows;  // (the whole warp)
     const int tok = min(row, u.rows - 1) / a.group;
@@ -431,7 +409,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
       wait(sfull + 8 * b, (i >> 1) & 1, abort);
       tc_fence_after();
       if (work) {
-        const uint8_t *sc = smem + L::SC + (i % 3) * L::SCB;
+        const uint8_t *sc = smem + L::SC + (i & 3) * L::SCB;
         const float4 *dk4 = reinterpret_cast<const float4 *>(sc), *dv4 = reinterpret_cast<const float4 *>(sc + NK * 4);
         const uint4 r4 = *reinterpret_cast<const uint4 *>(sc + 2 * NK * 4);
         const uint64_t held = (uint64_t)r4.y << 32 | r4.x;
@@ -577,11 +555,13 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
         }
       }
     }
+    __syncwarp();
+    set_regs<false, REGS>();
   }
   tc_fence_before();
   __syncthreads();
   if (cluster) join_cluster<DH>(a, u, tile0, ROWS, sb, sb + L::ML, THREADS);
-  if (warp == 8) {
+  if (warp == 12) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::COLS) : "memory");
   }
@@ -593,6 +573,16 @@ cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int cluster, unsigned blocks, 
   void (*k)(AttnKArgs) = a.c.type == PK_KV_Q8 ? (a.c.head_dim == 64 ? k_kv_attn_tc<PK_KV_Q8, 64> : k_kv_attn_tc<PK_KV_Q8, 128>)
                                               : (a.c.head_dim == 64 ? k_kv_attn_tc<PK_KV_Q4, 64> : k_kv_attn_tc<PK_KV_Q4, 128>);
   const int smem = a.c.head_dim == 64 ? Lay<64>::BYTES : Lay<128>::BYTES;
+  // the split of the registers would wait forever for what a launch does not have
+  static std::atomic<unsigned> checked{0};
+  const unsigned bit = 1u << (2 * (a.c.type == PK_KV_Q4) + (a.c.head_dim == 128));
+  if (!(checked.load(std::memory_order_relaxed) & bit)) {
+    cudaFuncAttributes f;
+    const cudaError_t e = cudaFuncGetAttributes(&f, reinterpret_cast<const void *>(k));
+    if (e != cudaSuccess) return e;
+    if (f.numRegs != REGS) return cudaErrorInvalidConfiguration;
+    checked.fetch_or(bit, std::memory_order_relaxed);
+  }
   return launch_cluster(k, cluster, dim3(blocks), dim3(THREADS), smem, st, a);
 }
 
