@@ -681,14 +681,16 @@ Variant variant_as() {
 // From TC_FROM rows on half-precision queries take the tcgen05 kernel.
 // (16 rows: 281 us here and 513 there for 40 sequences of 15000 positions; 24: 513 and 517.)
 constexpr long long TC_FROM = 17;
+constexpr long long TC32_FROM = 33;
 template <int TYPE, int DH, int NT>
 Variant variant_rows(long long rows) {
   if (rows <= 8) return variant_as<TYPE, DH, NT, 1, 1>();
   if (rows <= 16) return variant_as<TYPE, DH, NT, 2, 1>();
   if constexpr (NT == 1) {
     static_assert(TC_FROM == 17, "half-precision rows past 16");
-    return {nullptr, 0, TC_ATTN_ROWS};
+    return {nullptr, 0, 128};
   } else {
+    if (DH == 64 && rows >= TC32_FROM) return {nullptr, 0, 256};
     constexpr int NBM = DH == 128 ? 2 : 4;
     if (rows <= 8 * NBM) return variant_as<TYPE, DH, NT, NBM, 1>();
     if (rows <= 16 * NBM) return variant_as<TYPE, DH, NT, NBM, 2>();
@@ -723,10 +725,19 @@ Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, const Vari
   const long long units = (long long)s.n_seq * c.n_kv * p.row_tiles, want = 148 * 8;
   const long long most = (s.max_len + MIN_CHUNK - 1) / MIN_CHUNK;
   long long n = std::max<long long>(1, std::min(most, want / units));
-  if (n > 8 && n <= 16 && units * 8 <= 296) n = 8;
+  if (!v.k && v.rows == 256) {  // one CTA an SM: the number of chunks that takes the least rounds of tiles and beginnings
+    const long long top = std::min(most, std::max<long long>(1, want / units));
+    long long best = 0;
+    for (long long c = 1; c <= top; c++) {
+      const long long t = (units * c + 147) / 148 * ((s.max_len / c + 63) / 64 + 8);
+      if (c == 1 || t < best) best = t, n = c;
+    }
+  }
+  const long long slots = v.k || v.rows == 128 ? 296 : 128;  // CTAs that are sure to run at once, in clusters too
+  if (n > 8 && n <= 16 && units * 8 <= slots) n = 8;
   p.chunk = (int)(((s.max_len + n - 1) / n + 63) / 64 * 64);
   p.n_chunk = (int)((s.max_len + (long long)p.chunk - 1) / p.chunk);
-  p.cluster = p.n_chunk > 1 && p.n_chunk <= 8 && units * p.n_chunk <= 296;
+  p.cluster = p.n_chunk > 1 && p.n_chunk <= 8 && units * p.n_chunk <= slots;
   return p;
 }
 

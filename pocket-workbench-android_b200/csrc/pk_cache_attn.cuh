@@ -159,9 +159,8 @@ __device__ __forceinline__ void join_cluster(const AttnKArgs &a, const Unit &u, 
   cluster_sync();  // (until then the others may be reading)
 }
 
-// The tcgen05 kernel's launch (pk_cache_attn_tc.cu): 128 rows of a kv head's
-// tile, half-precision queries.
-constexpr int TC_ATTN_ROWS = 128;
+// The tcgen05 kernel's launch (pk_cache_attn_tc.cu): one or two blocks of 128
+// rows of a kv head a CTA (two CTAs an SM, or one).
 cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int cluster, unsigned blocks, cudaStream_t st);
 
 }  // namespace pk

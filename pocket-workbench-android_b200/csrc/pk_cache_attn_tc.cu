@@ -30,6 +30,8 @@
 // Every wait is bounded: one that runs out sets the CTA's abort flag, after
 // which no wait waits, and its rows are written as NaN.
 #include <algorithm>
+#include <atomic>
+#include <type_traits>
 
 #include "pk_cache_attn.cuh"
 #include "pk_launch.h"
@@ -39,34 +41,53 @@ namespace pk {
 namespace {
 
 constexpr int NK = 64;                      // positions a tile
-constexpr int ROWS = TC_ATTN_ROWS;
-constexpr int SOFT = 128, CONV = 128, THREADS = SOFT + 2 * CONV + 32;
-// Registers: two CTAs an SM leave 72 a thread; the code warps' share of them
-// goes to the softmax's.
-constexpr int REGS = 72, REGS_SOFT = 112, REGS_CONV = 48;
-static_assert(SOFT * REGS_SOFT + 2 * CONV * REGS_CONV + 32 * REGS <= THREADS * REGS, "no more than the launch's");
-static_assert(2 * THREADS * REGS <= 65536, "two CTAs an SM");
 constexpr unsigned long long WAIT_NS = 2000000000ull;
 
-template <int DH>
+// Terms of a query or weight: one f16 for half precision, two for f32.
+template <class E>
+constexpr int terms_of = std::is_same_v<E, float> ? 2 : 1;
+
+template <int DH, int NT, int BLK>
 struct Lay {
+  // (two blocks: whole warpgroups, as the last one gives registers away too)
+  static constexpr int ROWS = 128 * BLK, SOFT = 128 * BLK, CONV = 128, MMA = BLK == 1 ? 32 : 128, THREADS = SOFT + 2 * CONV + MMA;
+  // Registers a thread: at launch, and after the others have given the softmax
+  // warps theirs.
+  static constexpr int CTAS = BLK == 1 ? 2 : 1, REGS = BLK == 1 ? 72 : 96, REGS_SOFT = BLK == 1 ? 104 : NT == 2 ? 168 : 152;
+  static constexpr int REGS_CONV = BLK == 1 ? 56 : NT == 2 ? 48 : 64, REGS_MMA = BLK == 1 ? REGS : 48;
+  static_assert(SOFT * REGS_SOFT + 2 * CONV * REGS_CONV + MMA * REGS_MMA <= THREADS * REGS, "no more than the launch's");
+  static_assert(CTAS * THREADS * REGS <= 65536, "all of an SM's CTAs");
   // chunks of 16 bytes (8 dimensions) of consecutive positions; one chunk's
-  // stride is 16 bytes more than its 64 positions, so that the 16 lanes that
-  // store a position's chunks touch every bank once
+  // stride is 16 bytes more than its 64 positions, so that the lanes that
+  // store together touch every bank once
   static constexpr int CH = NK * 16 + 16, TILE = DH / 8 * CH;
-  static constexpr int Q = 0, K = Q + ROWS * DH * 2, V = K + 2 * TILE, SC = V + 2 * TILE;
+  static constexpr int QT = ROWS * DH * 2;  // a term of the queries
+  static constexpr int Q = 0, K = Q + NT * QT, V = K + 2 * TILE, OPS = V + 2 * TILE, SUMS = ROWS * (DH + 4) * 4;
+  static constexpr int SC = OPS > SUMS ? OPS : SUMS;  // (a cluster's sums take the operands' place)
   // of four tiles: D^K [NK], D^V [NK]; positions that hold something (2 words), largest D^V of 32 (2)
-  static constexpr int SCB = 2 * NK * 4 + 16, BAR = SC + 4 * SCB, ML = BAR + 112, BYTES = ML + ROWS * 8;
-  static_assert(ROWS * (DH + 4) * 4 <= SC, "a cluster's sums take the operands' place");
+  static constexpr int SCB = 2 * NK * 4 + 16, BAR = SC + 4 * SCB, ML = BAR + 64 + 48 * BLK, BYTES = ML + ROWS * 8;
+  // TMEM columns of a block of 128 rows: two buffers of scores, the output (f32: two buffers)
   static constexpr int S_COL = 0, O_COL = 2 * NK, COLS = 256;
+  static_assert(NT * DH <= 128 && CTAS * BLK * COLS <= 512, "the columns there are");
 };
 
+// mbar_test that may sleep for up to 20 us: 13 warps that ask again and again
+// take a third of an SM's issue slots.
+__device__ __forceinline__ bool mbar_sleep(uint32_t b, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+      : "=r"(ok)
+      : "r"(b), "r"(parity), "r"(20000)
+      : "memory");
+  return ok != 0;
+}
 // Waits for phase `parity` of mbarrier bar; called by whole warps, whose lanes
 // leave it together (tcgen05 loads and stores are the whole warp's).
 __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int *abort) {
-  if (!mbar_test(bar, parity)) {
+  if (!mbar_sleep(bar, parity)) {
     const unsigned long long t0 = gtime_ns();
-    while (!mbar_test(bar, parity) && !*abort)
+    while (!mbar_sleep(bar, parity) && !*abort)
       if (gtime_ns() - t0 > WAIT_NS) *abort = 1;
   }
   __syncwarp();
@@ -103,28 +124,24 @@ __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, b
       : "memory");
 }
 // 16 and 32 consecutive TMEM columns of this thread's lane.
-__device__ __forceinline__ void ld16(uint32_t t, float (&v)[16]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n tcgen05.wait::ld.sync.aligned;"
+// 16 columns are asked for, and usable after wait16 (which waits for all that
+// were asked for: one set at a time is in flight).
+__device__ __forceinline__ void ask16(uint32_t t, float (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
-               : "r"(t)
+               : "r"(t));
+}
+__device__ __forceinline__ void wait16(float (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]), "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]));
+}
+__device__ __forceinline__ void ld16(uint32_t t, float (&v)[16]) {
+  ask16(t, v);
+  wait16(v);
+}
+__device__ __forceinline__ void st16(uint32_t t, const uint32_t *v) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
                : "memory");
-}
-__device__ __forceinline__ void ld32(uint32_t t, float (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
-      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]), "=f"(v[9]),
-        "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]), "=f"(v[17]), "=f"(v[18]),
-        "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]), "=f"(v[25]), "=f"(v[26]), "=f"(v[27]),
-        "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-      : "r"(t)
-      : "memory");
-}
-__device__ __forceinline__ void st16(uint32_t t, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
 }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   float2 d;
@@ -156,15 +173,17 @@ __host__ __device__ constexpr int dim8(int i) {
   return TYPE == PK_KV_Q8 ? i : (i / 2) + 4 * (i % 2);
 }
 
-// This thread's query row, scaled to |q'| < 2 and rounded to f16 (exact for
-// f16 and bf16 down to 2^-24 of the row's largest), into the operand; its r.
+// This thread's query row into the operand, f16 as it is, bf16 scaled to
+// |q'| < 2 and rounded to f16 (exact down to 2^-24 of the row's largest); its
+// scale (the D^K that the row meets have log2(e) * scale in them).
 template <int TYPE, int DH, class E>
-__device__ __forceinline__ float put_q(const AttnKArgs &a, const Unit &u, int row, uint32_t dst) {
+__device__ __forceinline__ float put_q(const AttnKArgs &a, const Unit &u, int row, uint32_t dst, int stride, int term) {
+  constexpr bool F16 = std::is_same_v<E, __half>;
   const bool on = row < u.rows;
   const int i = row / a.group, h = u.h * a.group + row - i * a.group;
   const E *p = reinterpret_cast<const E *>(a.q.q) + (on ? (long long)(u.sv.first + i) * a.q.q_tok_stride + (long long)h * a.q.q_head_stride : 0);
   float m = 0.0f;
-  if (on) {
+  if (!F16 && on) {
 #pragma unroll
     for (int c = 0; c < DH / 8; c++) {
       float x[8];
@@ -178,16 +197,21 @@ __device__ __forceinline__ float put_q(const AttnKArgs &a, const Unit &u, int ro
   const float up = __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
 #pragma unroll
   for (int c = 0; c < DH / 8; c++) {
-    uint32_t w[4] = {0, 0, 0, 0};
+    uint32_t w[4] = {0, 0, 0, 0}, rest[4] = {0, 0, 0, 0};
     if (on) {
       float x[8];
       load_n<E, 8>(p + 8 * c, a.vec_q, x);
 #pragma unroll
-      for (int j = 0; j < 4; j++) w[j] = pack2(x[dim8<TYPE>(2 * j)] * down, x[dim8<TYPE>(2 * j + 1)] * down);
+      for (int j = 0; j < 4; j++) {
+        const float x0 = x[dim8<TYPE>(2 * j)] * down, x1 = x[dim8<TYPE>(2 * j + 1)] * down;
+        w[j] = pack2(x0, x1);
+        if (terms_of<E> == 2) rest[j] = rest2(x0, x1, w[j]);
+      }
     }
-    sts128(dst + c * (ROWS * 16), w[0], w[1], w[2], w[3]);
+    sts128(dst + c * stride, w[0], w[1], w[2], w[3]);
+    if (terms_of<E> == 2) sts128(dst + term + c * stride, rest[0], rest[1], rest[2], rest[3]);
   }
-  return a.q.scale * kLog2e * up;
+  return up;
 }
 
 // Which of positions p0 .. p0 + 63 token i sees (bit by position).
@@ -212,9 +236,12 @@ __device__ __forceinline__ uint64_t seen_by(const AttnKArgs &a, const Unit &u, i
   return v & ones(hi - p0) & ones(u.sv.ctx + u.sv.n - p0);
 }
 
-template <int TYPE, int DH>
-__global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
-  using L = Lay<DH>;
+template <int TYPE, int DH, class E, int BLK>
+__global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, terms_of<E>, BLK>::CTAS) k_kv_attn_tc(const AttnKArgs a) {
+  constexpr int NT = terms_of<E>;
+  using L = Lay<DH, NT, BLK>;
+  constexpr int ROWS = L::ROWS, SOFT = L::SOFT, CONV = L::CONV, THREADS = L::THREADS, WS = SOFT / 32;
+  constexpr bool F16 = std::is_same_v<E, __half>;
   constexpr int RB = TYPE == PK_KV_Q8 ? DH : DH / 2, SW = TYPE == PK_KV_Q8 ? 1 : 2;
   extern __shared__ __align__(1024) uint8_t smem[];
   pdl_wait();
@@ -227,78 +254,100 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
   }
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sb = shaddr(smem);
-  // barriers: S full x 2, K and scales ready x 4, P ready x 2, PV done x 2, V ready x 2; the TMEM address; the abort flag
-  const uint32_t bar = sb + L::BAR, sfull = bar, kready = bar + 16, pready = bar + 48, pvdone = bar + 64, vready = bar + 80;
-  volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 100);
+  // barriers: K and scales ready x 4, V ready x 2; the TMEM address, the abort
+  // flag; for each block of 128 rows: S full x 2, P ready x 2, PV done x 2
+  const uint32_t bar = sb + L::BAR, kready = bar, vready = bar + 32, blocks = bar + 64;
+  volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 52);
+  const int nblk = BLK == 1 ? 1 : min(BLK, (u.rows - tile0 + 127) / 128);  // that have rows
+  auto sfull_of = [&](int blk, int i) { return blocks + 48 * blk + 8 * (i & 1); };
+  auto pready_of = [&](int blk, int i) { return blocks + 48 * blk + 16 + 8 * (i & 1); };
+  auto pvdone_of = [&](int blk, int i) { return blocks + 48 * blk + 32 + 8 * (i & 1); };
   if (tid == 0) {
-    mbar_init(sfull, 2);  // the products, and the warp that issues them (which has seen the scales)
-    mbar_init(sfull + 8, 2);
     for (int i = 0; i < 4; i++) mbar_init(kready + 8 * i, CONV);
-    mbar_init(pready, SOFT);
-    mbar_init(pready + 8, SOFT);
-    mbar_init(vready, CONV);
-    mbar_init(vready + 8, CONV);
-    mbar_init(pvdone, 1);
-    mbar_init(pvdone + 8, 1);
+    for (int i = 0; i < 2; i++) {
+      mbar_init(vready + 8 * i, CONV);
+      for (int m = 0; m < BLK; m++) {
+        mbar_init(sfull_of(m, i), 2);  // the products, and the warp that issues them (which has seen the scales)
+        mbar_init(pready_of(m, i), 128);
+        mbar_init(pvdone_of(m, i), 1);
+      }
+    }
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 96), "r"(L::COLS) : "memory");
+  if (warp == WS + 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 48), "r"(BLK * L::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   const int row = tile0 + tid;
   float rs = 0.0f;
   if (tid < SOFT) {
-    const uint32_t dst = sb + L::Q + tid * 16;
-    rs = a.q.type == T_F16 ? put_q<TYPE, DH, __half>(a, u, row, dst) : put_q<TYPE, DH, __nv_bfloat16>(a, u, row, dst);
+    rs = put_q<TYPE, DH, E>(a, u, row, sb + L::Q + tid * 16, ROWS * 16, L::QT);
     fence_async_smem();
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   pdl_trigger();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::BAR + 96);
+  const uint32_t tmem = *reinterpret_cast<volatile uint32_t *>(smem + L::BAR + 48);
   // without a mask nobody sees past the tile's last token
   const int last = (min(tile0 + ROWS, u.rows) - 1) / a.group;
   const int hi = a.q.mask ? u.hi : min(u.hi, u.sv.ctx + last + 1);
   const int nt = hi > u.lo ? (hi - u.lo + NK - 1) / NK : 0;
 
-  if (warp == 12) {  // ---------------------------------------------- products
+  if (warp >= WS + 8) {  // ------------------------------------------- products
+    if (BLK > 1) set_regs<false, L::REGS_MMA>();
+    // (addresses made anew each time: kept across the loop, the descriptors
+    // alone would take most of the registers)
     auto scores = [&](int i) {
       wait(kready + 8 * (i & 3), (i >> 2) & 1, abort);
       tc_fence_after();
-      // (addresses made anew each time: kept across the loop, the descriptors
-      // alone would take most of the registers)
-      uint32_t q = sb + L::Q, k = sb + L::K + (i & 1) * L::TILE, dt = tmem + L::S_COL + (i & 1) * NK;
-      asm volatile("" : "+r"(q), "+r"(k), "+r"(dt));
+      for (int m = 0; m < nblk; m++) {
+        uint32_t q = sb + L::Q + m * (128 * 16), k = sb + L::K + (i & 1) * L::TILE, dt = tmem + m * L::COLS + L::S_COL + (i & 1) * NK;
+        asm volatile("" : "+r"(q), "+r"(k), "+r"(dt));
 #pragma unroll
-      for (int s = 0; s < DH / 16; s++)
-        mma_f16<NK, false>(dt, tc_desc(q + s * 2 * (ROWS * 16), ROWS * 16, 128), tc_desc(k + s * 2 * L::CH, L::CH, 128), s > 0);
-      if (lane == 0) mbar_arrive(sfull + 8 * (i & 1));
-      __syncwarp();
-      tc_commit(sfull + 8 * (i & 1));
+        for (int n = NT - 1; n >= 0; n--)  // (the smaller term first)
+#pragma unroll
+          for (int s = 0; s < DH / 16; s++)
+            mma_f16<NK, false>(dt, tc_desc(q + n * L::QT + s * 2 * (ROWS * 16), ROWS * 16, 128), tc_desc(k + s * 2 * L::CH, L::CH, 128),
+                               s > 0 || n < NT - 1);
+        if (lane == 0) mbar_arrive(sfull_of(m, i));
+        __syncwarp();
+        tc_commit(sfull_of(m, i));
+      }
     };
-    if (nt > 0) scores(0);
-    for (int i = 0; i < nt; i++) {
+    const int tiles = warp == WS + 8 ? nt : 0;
+    if (tiles > 0) scores(0);
+    for (int i = 0; i < tiles; i++) {
       if (i + 1 < nt) scores(i + 1);  // (into the columns of tile i - 1's weights: products are done in order)
       wait(vready + 8 * (i & 1), (i >> 1) & 1, abort);
-      wait(pready + 8 * (i & 1), (i >> 1) & 1, abort);
-      tc_fence_after();
-      uint32_t w = tmem + L::S_COL + (i & 1) * NK, v = sb + L::V + (i & 1) * L::TILE;
-      asm volatile("" : "+r"(w), "+r"(v));
+      for (int m = 0; m < nblk; m++) {
+        wait(pready_of(m, i), (i >> 1) & 1, abort);
+        tc_fence_after();
+        uint32_t w = tmem + m * L::COLS + L::S_COL + (i & 1) * NK, v = sb + L::V + (i & 1) * L::TILE;
+        uint32_t o = tmem + m * L::COLS + L::O_COL + (NT == 2 ? (i & 1) * DH : 0);
+        asm volatile("" : "+r"(w), "+r"(v), "+r"(o));
 #pragma unroll
-      for (int s = 0; s < NK / 16; s++)
-        mma_f16_ts<DH, true>(tmem + L::O_COL, w + s * 8, tc_desc(v + s * 16 * 16, 128, L::CH), i > 0 || s > 0);
-      tc_commit(pvdone + 8 * (i & 1));
+        for (int n = NT - 1; n >= 0; n--)
+#pragma unroll
+          for (int s = 0; s < NK / 16; s++)
+            mma_f16_ts<DH, true>(o, w + n * (NK / 2) + s * 8, tc_desc(v + s * 16 * 16, 128, L::CH), (NT == 1 && i > 0) || s > 0 || n < NT - 1);
+        tc_commit(pvdone_of(m, i));
+      }
     }
   } else if (tid >= SOFT) {  // ---------------------------------------- codes
     // 16 bytes of a row a lane (RL lanes a row), NP passes of RP rows; a
-    // thread's row of pass w is w * RP + ct / RL.
-    set_regs<false, REGS_CONV>();
+    // thread's row of pass w is w * RP + key0.  Eight lanes that store together
+    // have RS parts of a row and 8 / RS rows, so that they touch every bank
+    // once (a part's chunks are 2 or 4 strides from the next part's).
+    set_regs<false, L::REGS_CONV>();
+    auto role = [&](auto v_role) {
+    constexpr bool is_v = decltype(v_role)::value;
     constexpr int RL = RB / 16, RP = CONV / RL, NP = NK / RP;
-    const bool is_v = warp >= 8;
-    const int ct = (tid - SOFT) & (CONV - 1), sub = ct % RL, key0 = ct / RL;
+    constexpr int RS = TYPE == PK_KV_Q8 ? 4 : 2;
+    const int ct = (tid - SOFT) & (CONV - 1);
+    const int sub = RL <= RS ? ct % RL : ct % RS + (ct / 8 % (RL / RS)) * RS;
+    const int key0 = RL <= RS ? ct / RL : ct / RS % (8 / RS) + ct / (8 * RL / RS) * (8 / RS);
     const int key = ct & (NK - 1), half = ct >> 6;  // whose scale this thread passes on (half 0: K's, 1: V's)
     static_assert(RP % 16 == 0, "a pass has whole groups of 16 rows");
     uint4 raw[NP];  // the next tile's codes and sub-scales
@@ -310,9 +359,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     // positions or more): -1 where there is no page.  Such rows are read from
     // the cache's first, whose codes are as good as any (their scales are 0).
     int rows16 = -1;
-    const uint8_t *codes = reinterpret_cast<const uint8_t *>(is_v ? a.c.v : a.c.k) + (key0 & 15) * RB + 16 * sub;
-    const uint8_t *scales = reinterpret_cast<const uint8_t *>(is_v ? a.c.vs : a.c.ks) + ((key0 & 15) * SW + 1) * 4;
-    const uint8_t *dp = reinterpret_cast<const uint8_t *>(half ? a.c.vs : a.c.ks) + (key & 15) * SW * 4;
+    const uint8_t *codes = reinterpret_cast<const uint8_t *>(is_v ? a.c.v : a.c.k);
+    const uint32_t *subs_of = reinterpret_cast<const uint32_t *>(is_v ? a.c.vs : a.c.ks);
+    const float *d_of = half ? a.c.vs : a.c.ks;
     auto ask = [&](int i) {
       if (!(i & 7)) {
         const int p = u.lo + NK * (i + (lane >> 2)) + 16 * (lane & 3), j = p >> a.page_shift;
@@ -324,13 +373,13 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
 #pragma unroll
       for (int w = 0; w < NP; w++) {
         const uint32_t r = max(__shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + w * (RP / 16) + key0 / 16), 0);
-        raw[w] = __ldg(reinterpret_cast<const uint4 *>(codes + (size_t)r * (16 * RB)));
-        if (TYPE == PK_KV_Q4) subs[w] = __ldg(reinterpret_cast<const uint32_t *>(scales + (size_t)r * (16 * SW * 4)));
+        raw[w] = __ldg(reinterpret_cast<const uint4 *>(codes + ((size_t)r * (16 * RB) + ((key0 & 15) * RB + 16 * sub))));
+        if (TYPE == PK_KV_Q4) subs[w] = __ldg(subs_of + ((size_t)r * (16 * SW) + ((key0 & 15) * SW + 1)));
       }
       if (!is_v) {
         const int r = __shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + key / 16);
         on = r >= 0 && u.lo + NK * i + key < hi;
-        d = __ldg(reinterpret_cast<const float *>(dp + (size_t)max(r, 0) * (16 * SW * 4)));
+        d = __ldg(d_of + ((size_t)max(r, 0) * (16 * SW) + (key & 15) * SW));
       }
     };
     auto put = [&](uint32_t dst) {
@@ -339,13 +388,9 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
         const uint4 x = raw[w];
         const uint32_t at = dst + (w * RP + key0) * 16;
         if (TYPE == PK_KV_Q8) {
-          // two chunks of 8 dimensions; half the lanes of a row begin with the
-          // second, so that eight lanes' stores touch every bank once
-          const bool swap = sub >= RL / 2;
-          const uint32_t a0 = swap ? x.z : x.x, a1 = swap ? x.w : x.y, b0 = swap ? x.x : x.z, b1 = swap ? x.y : x.w;
-          const uint32_t ca = at + (2 * sub + swap) * L::CH, cb = at + (2 * sub + !swap) * L::CH;
-          sts128(ca, codes_of(a0, 0x4140), codes_of(a0, 0x4342), codes_of(a1, 0x4140), codes_of(a1, 0x4342));
-          sts128(cb, codes_of(b0, 0x4140), codes_of(b0, 0x4342), codes_of(b1, 0x4140), codes_of(b1, 0x4342));
+          // two chunks of 8 dimensions
+          sts128(at + 2 * sub * L::CH, codes_of(x.x, 0x4140), codes_of(x.x, 0x4342), codes_of(x.y, 0x4140), codes_of(x.y, 0x4342));
+          sts128(at + (2 * sub + 1) * L::CH, codes_of(x.z, 0x4140), codes_of(x.z, 0x4342), codes_of(x.w, 0x4140), codes_of(x.w, 0x4342));
         } else {  // four chunks, one sub-scale
           const int s = (int)((subs[w] >> (4 * sub)) & 15u);
           const uint32_t s2 = dup_h(s), m2 = dup_h(-1032 * s), y[4] = {x.x, x.y, x.z, x.w};
@@ -360,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     // tile i - 2's scores are full, so tile i - 4's weights have been used
     auto put_scales = [&](int i) {
       uint8_t *sc = smem + L::SC + (i & 3) * L::SCB;
-      reinterpret_cast<float *>(sc)[half * NK + key] = on ? d : 0.0f;
+      reinterpret_cast<float *>(sc)[half * NK + key] = on ? half ? d : fminf(fmaxf(d * (a.q.scale * kLog2e), -3e38f), 3e38f) : 0.0f;  // (finite: a query may be 0)
       if (half == 0) {
         const unsigned m = __ballot_sync(0xffffffffu, on);
         if (lane == 0) reinterpret_cast<uint32_t *>(sc + 2 * NK * 4)[key >> 5] = m;
@@ -373,40 +418,76 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
     for (int i = 0; i < nt; i++) {
       // K's buffer is free once tile i - 2's scores are there, V's once its
       // products with V are
-      if (i >= 2) wait((is_v ? pvdone : sfull) + 8 * (i & 1), ((i - 2) >> 1) & 1, abort);
+      if (i >= 2)
+        for (int m = 0; m < nblk; m++) wait(is_v ? pvdone_of(m, i) : sfull_of(m, i), ((i - 2) >> 1) & 1, abort);
       put(sb + (is_v ? L::V : L::K) + (i & 1) * L::TILE);
       if (!is_v) put_scales(i);
       fence_async_smem();
       mbar_arrive(is_v ? vready + 8 * (i & 1) : kready + 8 * (i & 3));
       if (i + 1 < nt) ask(i + 1);
     }
-    set_regs<true, REGS>();
+    };
+    if (warp < WS + 4) role(std::false_type());
+    else role(std::true_type());
   } else {  // ------------------------------------------------------------ softmax
-    set_regs<true, REGS_SOFT>();
-    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    set_regs<true, L::REGS_SOFT>();
+    const int blk = BLK == 1 ? 0 : warp >> 2;
+    const uint32_t lanes = ((uint32_t)((warp & 3) * 32) << 16) + blk * L::COLS;
     const bool work = tile0 + warp * 32 < u.rows;  // (the whole warp)
     const int tok = min(row, u.rows - 1) / a.group;
     float m = -CUDART_INF_F, l = 0.0f;
     const float2 rs2 = make_float2(rs, rs);
-    auto pv_wait = [&](int i) { wait(pvdone + 8 * (i & 1), (i >> 1) & 1, abort); };
+    auto pv_wait = [&](int i) { wait(pvdone_of(blk, i), (i >> 1) & 1, abort); };
+    // f32: a tile's products with V are added to the row's sums here, as the
+    // tensor core's own additions cut off what they shift out; `added` tiles are
+    float o[NT == 2 ? DH : 1];
+    int added = 0;
+    if (NT == 2) {
+#pragma unroll
+      for (int j = 0; j < DH; j++) o[NT == 2 ? j : 0] = 0.0f;
+    }
+    auto add_o = [&](int i) {  // tile i's
+      pv_wait(i);
+      tc_fence_after();
+      __syncwarp();
+      float v[2][16];
+      const uint32_t at = tmem + lanes + L::O_COL + (i & 1) * DH;
+      ask16(at, v[0]);
+#pragma unroll
+      for (int c = 0; c < DH / 16; c++) {
+        wait16(v[c & 1]);
+        if (c + 1 < DH / 16) ask16(at + 16 * (c + 1), v[(c + 1) & 1]);
+#pragma unroll
+        for (int j = 0; j < 16; j++) o[NT == 2 ? 16 * c + j : 0] += v[c & 1][j];
+      }
+      added = i + 1;
+    };
     // O's row times f, once the products before are done (i > 0)
     auto scale_o = [&](int i, float f) {
       if (i == 0) return;
-      pv_wait(i - 1);
-      tc_fence_after();
-#pragma unroll 1
-      for (int c = 0; c < DH / 16; c++) {
-        float v[16];
-        __syncwarp();
-        ld16(tmem + lanes + L::O_COL + 16 * c, v);
+      if constexpr (NT == 2) {
+        if (added < i) add_o(i - 1);
 #pragma unroll
-        for (int j = 0; j < 16; j++) v[j] *= f;
-        st16(tmem + lanes + L::O_COL + 16 * c, reinterpret_cast<const uint32_t(&)[16]>(v));
+        for (int j = 0; j < DH; j++) o[j] *= f;
+      } else {
+        pv_wait(i - 1);
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < DH / 16; c++) {
+          float v[16];
+          uint32_t x[16];
+          __syncwarp();
+          ld16(tmem + lanes + L::O_COL + 16 * c, v);
+#pragma unroll
+          for (int j = 0; j < 16; j++) x[j] = __float_as_uint(v[j] * f);
+          st16(tmem + lanes + L::O_COL + 16 * c, x);
+        }
       }
     };
+    if (blk < nblk)
     for (int i = 0; i < nt; i++) {
       const int b = i & 1, p0 = u.lo + NK * i;
-      wait(sfull + 8 * b, (i >> 1) & 1, abort);
+      wait(sfull_of(blk, i), (i >> 1) & 1, abort);
       tc_fence_after();
       if (work) {
         const uint8_t *sc = smem + L::SC + (i & 3) * L::SCB;
@@ -416,51 +497,56 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
         const float vmax = fmaxf(__uint_as_float(r4.z), __uint_as_float(r4.w));
         const bool masked = p0 + NK > min(u.sv.ctx, hi) || held != ~0ull;
         const uint32_t cols = tmem + lanes + L::S_COL + NK * b;
-        float t[32];
-        float2 *t2 = reinterpret_cast<float2 *>(t);
-        auto scores = [&](int c) {  // D^K q'.c of positions 32 c ..
-          __syncwarp();
-          ld32(cols + 32 * c, t);
+        // quarter k of the tile's positions: D^K q'.c of the products in t
+        auto scores = [&](int k, float (&t)[16]) {
 #pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const float4 d = dk4[8 * c + j];
-            t2[2 * j] = mul2(t2[2 * j], make_float2(d.x, d.y));
-            t2[2 * j + 1] = mul2(t2[2 * j + 1], make_float2(d.z, d.w));
+          for (int j = 0; j < 4; j++) {
+            const float4 d = dk4[4 * k + j];
+            const float2 x = mul2(make_float2(t[4 * j], t[4 * j + 1]), make_float2(d.x, d.y));
+            const float2 y = mul2(make_float2(t[4 * j + 2], t[4 * j + 3]), make_float2(d.z, d.w));
+            t[4 * j] = x.x, t[4 * j + 1] = x.y, t[4 * j + 2] = y.x, t[4 * j + 3] = y.y;
           }
         };
-        uint32_t w[2][16];
+        uint32_t w[32 * NT];
         float2 sum[2];
-        auto weights = [&](int c, uint32_t seen) {  // of the scores in t
+        auto weights = [&](int k, const float (&t)[16], float m, uint32_t seen) {  // of the products in t
           const float2 mu2 = make_float2(-m, -m);
 #pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const float4 d = dv4[8 * c + j];
+          for (int j = 0; j < 4; j++) {
+            const float4 dk = dk4[4 * k + j], d = dv4[4 * k + j];
 #pragma unroll
             for (int e = 0; e < 2; e++) {
-              float2 x = fma2(t2[2 * j + e], rs2, mu2);
+              float2 x = make_float2(t[4 * j + 2 * e], t[4 * j + 2 * e + 1]);
+              const float2 dke = e ? make_float2(dk.z, dk.w) : make_float2(dk.x, dk.y);
+              x = F16 ? fma2(x, dke, mu2) : fma2(mul2(x, dke), rs2, mu2);
               x.x = ex2(x.x);
               x.y = ex2(x.y);
-              if (seen != 0xffffffffu) {
+              if (seen != 0xffffu) {
                 if (!((seen >> (4 * j + 2 * e)) & 1)) x.x = 0.0f;
                 if (!((seen >> (4 * j + 2 * e + 1)) & 1)) x.y = 0.0f;
               }
               sum[e] = add2(sum[e], x);
               x = mul2(x, e ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
-              if (seen != 0xffffffffu) {  // (a scale that is not seen may be anything)
+              if (seen != 0xffffu) {  // (a scale that is not seen may be anything)
                 if (!((seen >> (4 * j + 2 * e)) & 1)) x.x = 0.0f;
                 if (!((seen >> (4 * j + 2 * e + 1)) & 1)) x.y = 0.0f;
               }
-              w[c][2 * j + e] = pack2(x.x, x.y);
+              w[8 * k + 2 * j + e] = pack2(x.x, x.y);
+              if (NT == 2) w[32 * (NT - 1) + 8 * k + 2 * j + e] = rest2(x.x, x.y, w[8 * k + 2 * j + e]);
             }
           }
         };
         bool longer = masked;
-        if (!masked) {
+        if (!masked) {  // a quarter is on its way while the one before is worked on
+          float t[2][16];
           sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+          __syncwarp();
+          ask16(cols, t[0]);
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
-            scores(c);
-            weights(c, 0xffffffffu);
+          for (int k = 0; k < 4; k++) {
+            wait16(t[k & 1]);
+            if (k < 3) ask16(cols + 16 * (k + 1), t[(k + 1) & 1]);
+            weights(k, t[k & 1], m, 0xffffu);
           }
           const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
           longer = __any_sync(0xffffffffu, !(all * vmax <= TOP && all <= 0x1p100f));  // (m is -inf at first: infinite)
@@ -468,23 +554,27 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
         }
         if (longer) {
           const uint64_t vis = !masked ? ~0ull : row < u.rows ? held & seen_by(a, u, tok, p0, hi) : 0;
-          float mx = -CUDART_INF_F, top = 0.0f;
+          float mx = -CUDART_INF_F, top = 0.0f, t[16];
 #pragma unroll 1
-          for (int c = 0; c < 2; c++) {
-            scores(c);
+          for (int k = 0; k < 4; k++) {
+            __syncwarp();
+            ld16(cols + 16 * k, t);
+            scores(k, t);
 #pragma unroll
-            for (int j = 0; j < 32; j++)
-              if ((vis >> (32 * c + j)) & 1) mx = fmaxf(mx, t[j]);
+            for (int j = 0; j < 16; j++)
+              if ((vis >> (16 * k + j)) & 1) mx = fmaxf(mx, t[j]);
           }
           mx *= rs;
           // (every lane goes through the loads from TMEM, rows that see nothing too)
           const float *dv = reinterpret_cast<const float *>(dv4);
 #pragma unroll 1
-          for (int c = 0; c < 2; c++) {
-            scores(c);
+          for (int k = 0; k < 4; k++) {
+            __syncwarp();
+            ld16(cols + 16 * k, t);
+            scores(k, t);
 #pragma unroll
-            for (int j = 0; j < 32; j++)
-              if ((vis >> (32 * c + j)) & 1) top = fmaxf(top, ex2(fmaf(t[j], rs, -mx)) * dv[32 * c + j]);
+            for (int j = 0; j < 16; j++)
+              if ((vis >> (16 * k + j)) & 1) top = fmaxf(top, ex2(fmaf(t[j], rs, -mx)) * dv[16 * k + j]);
           }
           float f = 1.0f;
           const float most = mx + log2f(fmaxf(top, 0x1p-100f));  // the largest product's exponent
@@ -496,27 +586,31 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
           }
           if (__any_sync(0xffffffffu, f != 1.0f)) scale_o(i, f);
           sum[0] = sum[1] = make_float2(0.0f, 0.0f);
-          const float keep = m;
-          if (m == -CUDART_INF_F) m = 0.0f;  // (nothing seen yet: every weight is masked)
 #pragma unroll
-          for (int c = 0; c < 2; c++) {
-            scores(c);
-            weights(c, (uint32_t)(vis >> (32 * c)));
+          for (int k = 0; k < 4; k++) {
+            __syncwarp();
+            ld16(cols + 16 * k, t);
+            weights(k, t, m == -CUDART_INF_F ? 0.0f : m, (uint32_t)(vis >> (16 * k)) & 0xffffu);  // (nothing seen yet: all are masked)
           }
-          m = keep;
           l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
         }
         __syncwarp();
-        st16(cols, w[0]);  // the weights take their scores' columns, two a column
-        st16(cols + 16, w[1]);
+#pragma unroll
+        for (int n = 0; n < 2 * NT; n++) st16(cols + 16 * n, w + 16 * n);  // the weights take their scores' columns, two a column
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       }
       tc_fence_before();
-      mbar_arrive(pready + 8 * b);
+      mbar_arrive(pready_of(blk, i));
+      if (NT == 2 && work && added < i) add_o(i - 1);
     }
     // ---- the rows
-    if (nt > 0) pv_wait(nt - 1);
+    if (nt > 0 && blk < nblk) {
+      pv_wait(nt - 1);
+      if (NT == 2 && work) add_o(nt - 1);
+    }
     tc_fence_after();
+    // (a cluster's sums take the operands' place: all blocks' products are done)
+    if (BLK > 1 && cluster) asm volatile("bar.sync 1, %0;" ::"r"(SOFT) : "memory");
     if (work) {
       const int i = tok, h = u.h * a.group + (min(row, u.rows - 1) - i * a.group);
       const long long at = u.sv.first + i;
@@ -534,56 +628,78 @@ __global__ void __launch_bounds__(THREADS, 2) k_kv_attn_tc(const AttnKArgs a) {
       float *po = !part ? nullptr : cluster ? reinterpret_cast<float *>(smem) + tid * (DH + 4) : a.part_o + ((at * a.q.n_head + h) * a.n_chunk + u.ch) * DH;
       const long long off = at * a.q.out_tok_stride + (long long)h * a.q.out_head_stride;
 #pragma unroll
-      for (int c = 0; c < DH / 32; c++) {
-        float v[32];
+      for (int c = 0; c < DH / 16; c++) {
+        float v[16];
         __syncwarp();
-        if (nt > 0) {
-          ld32(tmem + lanes + L::O_COL + 32 * c, v);
+        if (NT == 2) {
+#pragma unroll
+          for (int j = 0; j < 16; j++) v[j] = o[NT == 2 ? 16 * c + j : 0];
+        } else if (nt > 0) {
+          ld16(tmem + lanes + L::O_COL + 16 * c, v);
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; j++) v[j] = 0.0f;
+          for (int j = 0; j < 16; j++) v[j] = 0.0f;
         }
 #pragma unroll
-        for (int k = 0; k < 4 && on; k++) {
+        for (int k = 0; k < 2 && on; k++) {
           float x[8];
 #pragma unroll
           for (int j = 0; j < 8; j++) x[dim8<TYPE>(j)] = f == 0.0f ? 0.0f : v[8 * k + j] * f;
-          const int d0 = 32 * c + 8 * k;
+          const int d0 = 16 * c + 8 * k;
           if (part) store_n<float, 8>(po + d0, true, x);
-          else if (a.q.type == T_F16) store_n<__half, 8>(reinterpret_cast<__half *>(a.q.out) + off + d0, a.vec_o, x);
-          else store_n<__nv_bfloat16, 8>(reinterpret_cast<__nv_bfloat16 *>(a.q.out) + off + d0, a.vec_o, x);
+          else store_n<E, 8>(reinterpret_cast<E *>(a.q.out) + off + d0, a.vec_o, x);
         }
       }
     }
     __syncwarp();
-    set_regs<false, REGS>();
+    set_regs<false, L::REGS>();
   }
   tc_fence_before();
   __syncthreads();
+  // Only here, after the softmax warps have had their registers and given them
+  // back: taken earlier (by warps without a tile) they would be missing there.
+  if (warp >= WS && (BLK > 1 || warp < WS + 8)) set_regs<true, L::REGS>();
   if (cluster) join_cluster<DH>(a, u, tile0, ROWS, sb, sb + L::ML, THREADS);
-  if (warp == 12) {
+  if (warp == WS + 8) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(L::COLS) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(BLK * L::COLS) : "memory");
   }
+}
+
+struct Kernel {
+  void (*k)(AttnKArgs);
+  int threads, smem, regs;
+};
+template <int TYPE, int DH, class E, int BLK>
+Kernel kernel_as() {
+  using L = Lay<DH, terms_of<E>, BLK>;
+  return {k_kv_attn_tc<TYPE, DH, E, BLK>, L::THREADS, L::BYTES, L::REGS};
+}
+template <class E, int BLK>
+Kernel kernel_of(const pk_kv_cache &c) {
+  if constexpr (terms_of<E> == 2) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 64, E, BLK>() : kernel_as<PK_KV_Q4, 64, E, BLK>();
+  else
+    return c.type == PK_KV_Q8 ? (c.head_dim == 64 ? kernel_as<PK_KV_Q8, 64, E, BLK>() : kernel_as<PK_KV_Q8, 128, E, BLK>())
+                              : (c.head_dim == 64 ? kernel_as<PK_KV_Q4, 64, E, BLK>() : kernel_as<PK_KV_Q4, 128, E, BLK>());
 }
 
 }  // namespace
 
 cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int cluster, unsigned blocks, cudaStream_t st) {
-  void (*k)(AttnKArgs) = a.c.type == PK_KV_Q8 ? (a.c.head_dim == 64 ? k_kv_attn_tc<PK_KV_Q8, 64> : k_kv_attn_tc<PK_KV_Q8, 128>)
-                                              : (a.c.head_dim == 64 ? k_kv_attn_tc<PK_KV_Q4, 64> : k_kv_attn_tc<PK_KV_Q4, 128>);
-  const int smem = a.c.head_dim == 64 ? Lay<64>::BYTES : Lay<128>::BYTES;
+  const int e = a.q.type == T_F32 ? 0 : a.q.type == T_F16 ? 1 : 2;
+  const Kernel k = e == 0             ? kernel_of<float, 2>(a.c)
+                   : e == 1           ? kernel_of<__half, 1>(a.c) : kernel_of<__nv_bfloat16, 1>(a.c);
   // the split of the registers would wait forever for what a launch does not have
   static std::atomic<unsigned> checked{0};
-  const unsigned bit = 1u << (2 * (a.c.type == PK_KV_Q4) + (a.c.head_dim == 128));
+  const unsigned bit = 1u << (e * 4 + 2 * (a.c.type == PK_KV_Q4) + (a.c.head_dim == 128));
   if (!(checked.load(std::memory_order_relaxed) & bit)) {
     cudaFuncAttributes f;
-    const cudaError_t e = cudaFuncGetAttributes(&f, reinterpret_cast<const void *>(k));
-    if (e != cudaSuccess) return e;
-    if (f.numRegs != REGS) return cudaErrorInvalidConfiguration;
+    const cudaError_t err = cudaFuncGetAttributes(&f, reinterpret_cast<const void *>(k.k));
+    if (err != cudaSuccess) return err;
+    if (f.numRegs != k.regs) return cudaErrorInvalidConfiguration;
     checked.fetch_or(bit, std::memory_order_relaxed);
   }
-  return launch_cluster(k, cluster, dim3(blocks), dim3(THREADS), smem, st, a);
+  return launch_cluster(k.k, cluster, dim3(blocks), dim3(k.threads), k.smem, st, a);
 }
 
 }  // namespace pk
