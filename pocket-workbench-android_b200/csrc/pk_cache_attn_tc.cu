@@ -66,9 +66,10 @@ struct Lay {
   static constexpr int SC = OPS > SUMS ? OPS : SUMS;  // (a cluster's sums take the operands' place)
   // of four tiles: D^K [NK], D^V [NK]; positions that hold something (2 words), largest D^V of 32 (2)
   static constexpr int SCB = 2 * NK * 4 + 16, BAR = SC + 4 * SCB, ML = BAR + 64 + 48 * BLK, BYTES = ML + ROWS * 8;
-  // TMEM columns of a block of 128 rows: two buffers of scores, the output (f32: two buffers)
-  static constexpr int S_COL = 0, O_COL = 2 * NK, COLS = 256;
-  static_assert(NT * DH <= 128 && CTAS * BLK * COLS <= 512, "the columns there are");
+  // TMEM columns of a block of 128 rows: two buffers of scores, the output;
+  // f32 weights' two terms have their own, f16 ones take their scores'
+  static constexpr int S_COL = 0, O_COL = 2 * NK, P_COL = O_COL + DH, COLS = 256;
+  static_assert(O_COL + DH + (NT == 2 ? NK : 0) <= COLS && CTAS * BLK * COLS <= 512, "the columns there are");
 };
 
 // mbar_test that may sleep for up to 20 us: 13 warps that ask again and again
@@ -139,8 +140,30 @@ __device__ __forceinline__ void ld16(uint32_t t, float (&v)[16]) {
   ask16(t, v);
   wait16(v);
 }
-__device__ __forceinline__ void st16(uint32_t t, const uint32_t *v) {
-  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+// The same 16 columns with four lanes a row: thread (lane) holds rows lane / 4
+// + 8 j of the warp's 32 (j < 4), columns 8 g + 2 (lane % 4) and the next
+// (g < 2), as pairs p = 4 (j / 2) + 2 g + j % 2 of v: what the tensor core's
+// own operand fragments look like.
+__device__ __forceinline__ void ask_quads(uint32_t t, float (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(t));
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
+               : "r"(t + (16u << 16)));
+}
+__device__ __forceinline__ void st_quads(uint32_t t, const float (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+  asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t + (16u << 16)), "f"(v[8]), "f"(v[9]), "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15])
+               : "memory");
+}
+// 16 columns of f16 pairs: a thread's pairs of columns above, in order of
+// groups of 8, rows lane / 4 + 8 j and the next: v of rows j < 2, u of j >= 2.
+__device__ __forceinline__ void st_pairs(uint32_t t, const uint32_t *v, const uint32_t *u) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t + (16u << 16)), "r"(u[0]), "r"(u[1]), "r"(u[2]), "r"(u[3]), "r"(u[4]), "r"(u[5]), "r"(u[6]), "r"(u[7])
                : "memory");
 }
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
@@ -324,8 +347,8 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
       for (int m = 0; m < nblk; m++) {
         wait(pready_of(m, i), (i >> 1) & 1, abort);
         tc_fence_after();
-        uint32_t w = tmem + m * L::COLS + L::S_COL + (i & 1) * NK, v = sb + L::V + (i & 1) * L::TILE;
-        uint32_t o = tmem + m * L::COLS + L::O_COL + (NT == 2 ? (i & 1) * DH : 0);
+        uint32_t w = tmem + m * L::COLS + (NT == 2 ? L::P_COL : L::S_COL + (i & 1) * NK), v = sb + L::V + (i & 1) * L::TILE;
+        uint32_t o = tmem + m * L::COLS + L::O_COL;
         asm volatile("" : "+r"(w), "+r"(v), "+r"(o));
 #pragma unroll
         for (int n = NT - 1; n >= 0; n--)
@@ -435,52 +458,57 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
     const uint32_t lanes = ((uint32_t)((warp & 3) * 32) << 16) + blk * L::COLS;
     const bool work = tile0 + warp * 32 < u.rows;  // (the whole warp)
     const int tok = min(row, u.rows - 1) / a.group;
-    float m = -CUDART_INF_F, l = 0.0f;
-    const float2 rs2 = make_float2(rs, rs);
+    const int quad = lane & 3;
+    // of rows lane / 4 + 8 j: the scale, the reference, this thread's part of the sum
+    float rs4[4], m4[4], l4[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      rs4[j] = __shfl_sync(0xffffffffu, rs, (lane >> 2) + 8 * j);
+      m4[j] = -CUDART_INF_F;
+      l4[j] = 0.0f;
+    }
     auto pv_wait = [&](int i) { wait(pvdone_of(blk, i), (i >> 1) & 1, abort); };
-    // f32: a tile's products with V are added to the row's sums here, as the
+    // f32: a tile's products with V are added to the rows' sums here, as the
     // tensor core's own additions cut off what they shift out; `added` tiles are
-    float o[NT == 2 ? DH : 1];
+    float o[NT == 2 ? DH : 16];
     int added = 0;
     if (NT == 2) {
 #pragma unroll
       for (int j = 0; j < DH; j++) o[NT == 2 ? j : 0] = 0.0f;
     }
-    auto add_o = [&](int i) {  // tile i's
-      pv_wait(i);
+    auto add_o = [&](int n) {  // so that n tiles are
+      if (added >= n) return;  // (the same for the whole warp)
+      added = n;
+      pv_wait(n - 1);
       tc_fence_after();
       __syncwarp();
-      float v[2][16];
-      const uint32_t at = tmem + lanes + L::O_COL + (i & 1) * DH;
-      ask16(at, v[0]);
 #pragma unroll
       for (int c = 0; c < DH / 16; c++) {
-        wait16(v[c & 1]);
-        if (c + 1 < DH / 16) ask16(at + 16 * (c + 1), v[(c + 1) & 1]);
+        float v[16];
+        ask_quads(tmem + lanes + L::O_COL + 16 * c, v);
+        wait16(v);
 #pragma unroll
-        for (int j = 0; j < 16; j++) o[NT == 2 ? 16 * c + j : 0] += v[c & 1][j];
+        for (int j = 0; j < 16; j++) o[NT == 2 ? 16 * c + j : 0] += v[j];
       }
-      added = i + 1;
     };
-    // O's row times f, once the products before are done (i > 0)
-    auto scale_o = [&](int i, float f) {
+    // O's rows times f, once the products before are done (i > 0)
+    auto scale_o = [&](int i, const float (&f)[4]) {
       if (i == 0) return;
       if constexpr (NT == 2) {
-        if (added < i) add_o(i - 1);
 #pragma unroll
-        for (int j = 0; j < DH; j++) o[j] *= f;
+        for (int j = 0; j < DH; j++) o[j] *= f[2 * ((j >> 3) & 1) + ((j >> 1) & 1)];
       } else {
         pv_wait(i - 1);
         tc_fence_after();
 #pragma unroll 1
         for (int c = 0; c < DH / 16; c++) {
           float v[16];
-          uint32_t x[16];
           __syncwarp();
-          ld16(tmem + lanes + L::O_COL + 16 * c, v);
+          ask_quads(tmem + lanes + L::O_COL + 16 * c, v);
+          wait16(v);
 #pragma unroll
-          for (int j = 0; j < 16; j++) x[j] = __float_as_uint(v[j] * f);
-          st16(tmem + lanes + L::O_COL + 16 * c, x);
+          for (int j = 0; j < 16; j++) v[j] *= f[2 * (j >> 3) + ((j >> 1) & 1)];
+          st_quads(tmem + lanes + L::O_COL + 16 * c, v);
         }
       }
     };
@@ -491,124 +519,200 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
       tc_fence_after();
       if (work) {
         const uint8_t *sc = smem + L::SC + (i & 3) * L::SCB;
-        const float4 *dk4 = reinterpret_cast<const float4 *>(sc), *dv4 = reinterpret_cast<const float4 *>(sc + NK * 4);
+        const float2 *dk2 = reinterpret_cast<const float2 *>(sc) + quad, *dv2 = dk2 + NK / 2;
         const uint4 r4 = *reinterpret_cast<const uint4 *>(sc + 2 * NK * 4);
         const uint64_t held = (uint64_t)r4.y << 32 | r4.x;
         const float vmax = fmaxf(__uint_as_float(r4.z), __uint_as_float(r4.w));
         const bool masked = p0 + NK > min(u.sv.ctx, hi) || held != ~0ull;
         const uint32_t cols = tmem + lanes + L::S_COL + NK * b;
-        // quarter k of the tile's positions: D^K q'.c of the products in t
-        auto scores = [&](int k, float (&t)[16]) {
+        // columns 8 (2 k + g) + 2 quad and the next of a row's 64
+        auto bits = [&](uint64_t vis, int k, int g) { return (uint32_t)(vis >> (16 * k + 8 * g + 2 * quad)); };
+        // weights of the products in t, 16 columns; f16: all 64 columns' are
+        // kept (their scores may be needed again), f32: those of two steps
+        constexpr int WK = NT == 1 ? 4 : 2;
+        uint32_t w[NT][2][4 * WK];
+        float2 sum[4];
+        auto weights = [&](int k0, int k1, const float (&t)[16], const float (&m)[4], const uint64_t *vis) {  // step k0 + k1
+          const int k = k0 + k1;
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float4 d = dk4[4 * k + j];
-            const float2 x = mul2(make_float2(t[4 * j], t[4 * j + 1]), make_float2(d.x, d.y));
-            const float2 y = mul2(make_float2(t[4 * j + 2], t[4 * j + 3]), make_float2(d.z, d.w));
-            t[4 * j] = x.x, t[4 * j + 1] = x.y, t[4 * j + 2] = y.x, t[4 * j + 3] = y.y;
-          }
-        };
-        uint32_t w[32 * NT];
-        float2 sum[2];
-        auto weights = [&](int k, const float (&t)[16], float m, uint32_t seen) {  // of the products in t
-          const float2 mu2 = make_float2(-m, -m);
+          for (int g = 0; g < 2; g++) {
+            const float2 dk = dk2[4 * (2 * k + g)], dv = dv2[4 * (2 * k + g)];
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float4 dk = dk4[4 * k + j], d = dv4[4 * k + j];
-#pragma unroll
-            for (int e = 0; e < 2; e++) {
-              float2 x = make_float2(t[4 * j + 2 * e], t[4 * j + 2 * e + 1]);
-              const float2 dke = e ? make_float2(dk.z, dk.w) : make_float2(dk.x, dk.y);
-              x = F16 ? fma2(x, dke, mu2) : fma2(mul2(x, dke), rs2, mu2);
+            for (int j = 0; j < 4; j++) {
+              const int p = 4 * (j >> 1) + 2 * g + (j & 1), at = 2 * (2 * k1 + g) + (j & 1);
+              float2 x = make_float2(t[2 * p], t[2 * p + 1]);
+              x = F16 ? fma2(x, dk, make_float2(-m[j], -m[j])) : fma2(mul2(x, dk), make_float2(rs4[j], rs4[j]), make_float2(-m[j], -m[j]));
               x.x = ex2(x.x);
               x.y = ex2(x.y);
-              if (seen != 0xffffu) {
-                if (!((seen >> (4 * j + 2 * e)) & 1)) x.x = 0.0f;
-                if (!((seen >> (4 * j + 2 * e + 1)) & 1)) x.y = 0.0f;
-              }
-              sum[e] = add2(sum[e], x);
-              x = mul2(x, e ? make_float2(d.z, d.w) : make_float2(d.x, d.y));
-              if (seen != 0xffffu) {  // (a scale that is not seen may be anything)
-                if (!((seen >> (4 * j + 2 * e)) & 1)) x.x = 0.0f;
-                if (!((seen >> (4 * j + 2 * e + 1)) & 1)) x.y = 0.0f;
-              }
-              w[8 * k + 2 * j + e] = pack2(x.x, x.y);
-              if (NT == 2) w[32 * (NT - 1) + 8 * k + 2 * j + e] = rest2(x.x, x.y, w[8 * k + 2 * j + e]);
+              const uint32_t seen = vis ? bits(vis[j], k, g) : 3u;
+              if (vis) x.x = seen & 1 ? x.x : 0.0f, x.y = seen & 2 ? x.y : 0.0f;
+              sum[j] = add2(sum[j], x);
+              x = mul2(x, dv);
+              if (vis) x.x = seen & 1 ? x.x : 0.0f, x.y = seen & 2 ? x.y : 0.0f;  // (a scale that is not seen may be anything)
+              w[0][j >> 1][at] = pack2(x.x, x.y);
+              if (NT == 2) w[NT - 1][j >> 1][at] = rest2(x.x, x.y, w[0][j >> 1][at]);
             }
           }
         };
-        bool longer = masked;
-        if (!masked) {  // a quarter is on its way while the one before is worked on
-          float t[2][16];
-          sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+        // f32: half h of the tile's are stored, the products with those of the
+        // tile before being done
+        auto put_two = [&](int h) {
+          add_o(i);
           __syncwarp();
-          ask16(cols, t[0]);
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            wait16(t[k & 1]);
-            if (k < 3) ask16(cols + 16 * (k + 1), t[(k + 1) & 1]);
-            weights(k, t[k & 1], m, 0xffffu);
+          for (int n = 0; n < NT; n++) st_pairs(tmem + lanes + L::P_COL + n * (NK / 2) + 16 * h, w[n][0], w[n][1]);
+        };
+        bool longer = masked;
+        if (!masked) {
+          sum[0] = sum[1] = sum[2] = sum[3] = make_float2(0.0f, 0.0f);
+          __syncwarp();
+          if constexpr (NT == 1) {  // 16 columns are on their way while those before are worked on
+            float t[2][16];
+            ask_quads(cols, t[0]);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+              wait16(t[k & 1]);
+              if (k < 3) ask_quads(cols + 16 * (k + 1), t[(k + 1) & 1]);
+              weights(0, k, t[k & 1], m4, nullptr);
+            }
+          } else {
+#pragma unroll 1
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+              for (int k = 0; k < 2; k++) {
+                float t[16];
+                ask_quads(cols + 32 * h + 16 * k, t);
+                wait16(t);
+                weights(2 * h, k, t, m4, nullptr);
+              }
+              put_two(h);
+            }
           }
-          const float all = (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-          longer = __any_sync(0xffffffffu, !(all * vmax <= TOP && all <= 0x1p100f));  // (m is -inf at first: infinite)
-          if (!longer) l += all;
+          // (a thread's part of a row's sum is at least the largest of its
+          // weights; m is -inf at first: infinite)
+          bool over = false;
+          float all[4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            all[j] = sum[j].x + sum[j].y;
+            over |= !(all[j] * vmax <= TOP && all[j] <= 0x1p100f);
+          }
+          longer = __any_sync(0xffffffffu, over);
+          if (!longer) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) l4[j] += all[j];
+          }
         }
         if (longer) {
-          const uint64_t vis = !masked ? ~0ull : row < u.rows ? held & seen_by(a, u, tok, p0, hi) : 0;
-          float mx = -CUDART_INF_F, top = 0.0f, t[16];
-#pragma unroll 1
-          for (int k = 0; k < 4; k++) {
-            __syncwarp();
-            ld16(cols + 16 * k, t);
-            scores(k, t);
+          if (NT == 2) add_o(i);
+          const uint64_t mine = !masked ? ~0ull : row < u.rows ? held & seen_by(a, u, tok, p0, hi) : 0;
+          uint64_t vis[4];
+          float mx[4], top[4], f[4], m[4];
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-              if ((vis >> (16 * k + j)) & 1) mx = fmaxf(mx, t[j]);
+          for (int j = 0; j < 4; j++) {
+            vis[j] = __shfl_sync(0xffffffffu, mine, (lane >> 2) + 8 * j);
+            mx[j] = -CUDART_INF_F;
+            top[j] = 0.0f;
           }
-          mx *= rs;
           // (every lane goes through the loads from TMEM, rows that see nothing too)
-          const float *dv = reinterpret_cast<const float *>(dv4);
+          auto over_seen = [&](auto step) {
 #pragma unroll 1
-          for (int k = 0; k < 4; k++) {
-            __syncwarp();
-            ld16(cols + 16 * k, t);
-            scores(k, t);
+            for (int k = 0; k < 4; k++) {
+              float t[16];
+              __syncwarp();
+              ask_quads(cols + 16 * k, t);
+              wait16(t);
 #pragma unroll
-            for (int j = 0; j < 16; j++)
-              if ((vis >> (16 * k + j)) & 1) top = fmaxf(top, ex2(fmaf(t[j], rs, -mx)) * dv[16 * k + j]);
-          }
-          float f = 1.0f;
-          const float most = mx + log2f(fmaxf(top, 0x1p-100f));  // the largest product's exponent
-          if (mx != -CUDART_INF_F && (m == -CUDART_INF_F || most > m + 8.0f || mx > m + 90.0f)) {
-            const float now = fmaxf(most - 6.0f, mx - 90.0f);
-            f = ex2(m - now);
-            l *= f;
-            m = now;
-          }
-          if (__any_sync(0xffffffffu, f != 1.0f)) scale_o(i, f);
-          sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+              for (int g = 0; g < 2; g++) {
+                const float2 dk = dk2[4 * (2 * k + g)], dv = dv2[4 * (2 * k + g)];
 #pragma unroll
-          for (int k = 0; k < 4; k++) {
-            __syncwarp();
-            ld16(cols + 16 * k, t);
-            weights(k, t, m == -CUDART_INF_F ? 0.0f : m, (uint32_t)(vis >> (16 * k)) & 0xffffu);  // (nothing seen yet: all are masked)
+                for (int j = 0; j < 4; j++) {
+                  const int p = 4 * (j >> 1) + 2 * g + (j & 1);
+                  const uint32_t seen = bits(vis[j], k, g);
+                  if (seen & 1) step(j, t[2 * p] * dk.x, dv.x);
+                  if (seen & 2) step(j, t[2 * p + 1] * dk.y, dv.y);
+                }
+              }
+            }
+          };
+          auto quad_max = [](float x) {
+            x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+            return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+          };
+          over_seen([&](int j, float x, float) { mx[j] = fmaxf(mx[j], x * rs4[j]); });
+#pragma unroll
+          for (int j = 0; j < 4; j++) mx[j] = quad_max(mx[j]);
+          over_seen([&](int j, float x, float dv) { top[j] = fmaxf(top[j], ex2(fmaf(x, rs4[j], -mx[j])) * dv); });
+          bool moved = false;
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            f[j] = 1.0f;
+            const float most = mx[j] + log2f(fmaxf(quad_max(top[j]), 0x1p-100f));  // the largest product's exponent
+            if (mx[j] != -CUDART_INF_F && (m4[j] == -CUDART_INF_F || most > m4[j] + 8.0f || mx[j] > m4[j] + 90.0f)) {
+              const float now = fmaxf(most - 6.0f, mx[j] - 90.0f);
+              f[j] = ex2(m4[j] - now);
+              l4[j] *= f[j];
+              m4[j] = now;
+              moved |= f[j] != 1.0f;
+            }
+            m[j] = m4[j] == -CUDART_INF_F ? 0.0f : m4[j];  // (nothing seen yet: all are masked)
           }
-          l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+          if (__any_sync(0xffffffffu, moved)) scale_o(i, f);
+          sum[0] = sum[1] = sum[2] = sum[3] = make_float2(0.0f, 0.0f);
+#pragma unroll(NT == 1 ? 4 : 1)
+          for (int h = 0; h < 4 / WK; h++) {
+#pragma unroll
+            for (int k = 0; k < WK; k++) {
+              float t[16];
+              __syncwarp();
+              ask_quads(cols + 16 * (WK * h + k), t);
+              wait16(t);
+              weights(WK * h, k, t, m, vis);
+            }
+            if (NT == 2) put_two(h);
+          }
+#pragma unroll
+          for (int j = 0; j < 4; j++) l4[j] += sum[j].x + sum[j].y;
         }
         __syncwarp();
-#pragma unroll
-        for (int n = 0; n < 2 * NT; n++) st16(cols + 16 * n, w + 16 * n);  // the weights take their scores' columns, two a column
+        if (NT == 1) {  // the weights take their scores' columns, two a column
+          st_pairs(cols, w[0][0], w[0][1]);
+          st_pairs(cols + 16, w[0][0] + (NT == 1 ? 8 : 0), w[0][1] + (NT == 1 ? 8 : 0));
+        }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
       }
       tc_fence_before();
       mbar_arrive(pready_of(blk, i));
-      if (NT == 2 && work && added < i) add_o(i - 1);
     }
     // ---- the rows
     if (nt > 0 && blk < nblk) {
       pv_wait(nt - 1);
-      if (NT == 2 && work) add_o(nt - 1);
+      if (NT == 2 && work) add_o(nt);
     }
     tc_fence_after();
+    // one row a lane again
+    float m = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      float x = l4[j];
+      x += __shfl_xor_sync(0xffffffffu, x, 1);
+      x += __shfl_xor_sync(0xffffffffu, x, 2);
+      x = __shfl_sync(0xffffffffu, x, 4 * (lane & 7));
+      const float y = __shfl_sync(0xffffffffu, m4[j], 4 * (lane & 7));
+      if ((lane >> 3) == j) l = x, m = y;
+    }
+    if constexpr (NT == 2) {
+      const float ok = *abort ? CUDART_NAN_F : 1.0f;
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < DH / 16; c++) {
+        float v[16];
+#pragma unroll
+        for (int j = 0; j < 16; j++) v[j] = o[16 * c + j] * ok;
+        st_quads(tmem + lanes + L::O_COL + 16 * c, v);
+      }
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    }
     // (a cluster's sums take the operands' place: all blocks' products are done)
     if (BLK > 1 && cluster) asm volatile("bar.sync 1, %0;" ::"r"(SOFT) : "memory");
     if (work) {
@@ -631,10 +735,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
       for (int c = 0; c < DH / 16; c++) {
         float v[16];
         __syncwarp();
-        if (NT == 2) {
-#pragma unroll
-          for (int j = 0; j < 16; j++) v[j] = o[NT == 2 ? 16 * c + j : 0];
-        } else if (nt > 0) {
+        if (NT == 2 || nt > 0) {
           ld16(tmem + lanes + L::O_COL + 16 * c, v);
         } else {
 #pragma unroll
