@@ -83,15 +83,27 @@ __device__ __forceinline__ bool mbar_sleep(uint32_t b, uint32_t parity) {
       : "memory");
   return ok != 0;
 }
-// Waits for phase `parity` of mbarrier bar; called by whole warps, whose lanes
-// leave it together (tcgen05 loads and stores are the whole warp's).
-__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int *abort) {
+// Waits for phase `parity` of mbarrier bar: one thread, or a whole warp, whose
+// lanes leave it together (tcgen05 loads and stores are the whole warp's).
+__device__ __forceinline__ void wait_one(uint32_t bar, uint32_t parity, volatile int *abort) {
   if (!mbar_sleep(bar, parity)) {
     const unsigned long long t0 = gtime_ns();
     while (!mbar_sleep(bar, parity) && !*abort)
       if (gtime_ns() - t0 > WAIT_NS) *abort = 1;
   }
+}
+__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, volatile int *abort) {
+  wait_one(bar, parity, abort);
   __syncwarp();
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n selp.u32 %0, 1, 0, e;\n}" : "=r"(one));
+  return one != 0;
+}
+// Signals mbarrier bar once this thread's products so far are done.
+__device__ __forceinline__ void commit_one(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // This warpgroup's registers a thread from here on.
@@ -109,8 +121,8 @@ __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, bool
   // f32 sums, f16 operands, B N-major when BMN, M 128
   constexpr uint32_t idesc = (1u << 4) | ((BMN ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   asm volatile(
-      "{\n .reg .pred p, e;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(d),
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(d),
       "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0), "r"(0), "r"(0), "r"(0)
       : "memory");
 }
@@ -119,8 +131,8 @@ template <int N, bool BMN>
 __device__ __forceinline__ void mma_f16_ts(uint32_t d, uint32_t a, uint64_t b, bool acc) {
   constexpr uint32_t idesc = (1u << 4) | ((BMN ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
   asm volatile(
-      "{\n .reg .pred p, e;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
-      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(d),
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n}" ::"r"(d),
       "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)acc), "r"(0), "r"(0), "r"(0), "r"(0)
       : "memory");
 }
@@ -320,44 +332,43 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
 
   if (warp >= WS + 8) {  // ------------------------------------------- products
     if (BLK > 1) set_regs<false, L::REGS_MMA>();
-    // (addresses made anew each time: kept across the loop, the descriptors
-    // alone would take most of the registers)
-    auto scores = [&](int i) {
-      wait(kready + 8 * (i & 3), (i >> 2) & 1, abort);
-      tc_fence_after();
-      for (int m = 0; m < nblk; m++) {
-        uint32_t q = sb + L::Q + m * (128 * 16), k = sb + L::K + (i & 1) * L::TILE, dt = tmem + m * L::COLS + L::S_COL + (i & 1) * NK;
-        asm volatile("" : "+r"(q), "+r"(k), "+r"(dt));
-#pragma unroll
-        for (int n = NT - 1; n >= 0; n--)  // (the smaller term first)
-#pragma unroll
-          for (int s = 0; s < DH / 16; s++)
-            mma_f16<NK, false>(dt, tc_desc(q + n * L::QT + s * 2 * (ROWS * 16), ROWS * 16, 128), tc_desc(k + s * 2 * L::CH, L::CH, 128),
-                               s > 0 || n < NT - 1);
-        if (lane == 0) mbar_arrive(sfull_of(m, i));
-        __syncwarp();
-        tc_commit(sfull_of(m, i));
-      }
-    };
-    const int tiles = warp == WS + 8 ? nt : 0;
-    if (tiles > 0) scores(0);
-    for (int i = 0; i < tiles; i++) {
-      if (i + 1 < nt) scores(i + 1);  // (into the columns of tile i - 1's weights: products are done in order)
-      wait(vready + 8 * (i & 1), (i >> 1) & 1, abort);
-      for (int m = 0; m < nblk; m++) {
-        wait(pready_of(m, i), (i >> 1) & 1, abort);
+    // one thread issues them all (elected anew for each, they take twice as long)
+    if (warp == WS + 8 && elect_one()) {
+      const uint64_t qd = tc_desc(sb + L::Q, ROWS * 16, 128), kd = tc_desc(sb + L::K, L::CH, 128), vd = tc_desc(sb + L::V, 128, L::CH);
+      auto scores = [&](int i) {
+        wait_one(kready + 8 * (i & 3), (i >> 2) & 1, abort);
         tc_fence_after();
-        uint32_t w = tmem + m * L::COLS + (NT == 2 ? L::P_COL : L::S_COL + (i & 1) * NK), v = sb + L::V + (i & 1) * L::TILE;
-        uint32_t o = tmem + m * L::COLS + L::O_COL;
-        asm volatile("" : "+r"(w), "+r"(v), "+r"(o));
+        for (int m = 0; m < nblk; m++) {
+          const uint64_t q = qd + m * 128, k = kd + (i & 1) * (L::TILE / 16);
+          const uint32_t dt = tmem + m * L::COLS + L::S_COL + (i & 1) * NK;
 #pragma unroll
-        for (int n = NT - 1; n >= 0; n--)
+          for (int n = NT - 1; n >= 0; n--)  // (the smaller term first)
 #pragma unroll
-          for (int s = 0; s < NK / 16; s++)
-            mma_f16_ts<DH, true>(o, w + n * (NK / 2) + s * 8, tc_desc(v + s * 16 * 16, 128, L::CH), (NT == 1 && i > 0) || s > 0 || n < NT - 1);
-        tc_commit(pvdone_of(m, i));
+            for (int s = 0; s < DH / 16; s++)
+              mma_f16<NK, false>(dt, q + (n * L::QT / 16 + s * 2 * ROWS), k + s * 2 * (L::CH / 16), s > 0 || n < NT - 1);
+          mbar_arrive(sfull_of(m, i));
+          commit_one(sfull_of(m, i));
+        }
+      };
+      if (nt > 0) scores(0);
+      for (int i = 0; i < nt; i++) {
+        if (i + 1 < nt) scores(i + 1);  // (into the columns of tile i - 1's weights: products are done in order)
+        wait_one(vready + 8 * (i & 1), (i >> 1) & 1, abort);
+        for (int m = 0; m < nblk; m++) {
+          wait_one(pready_of(m, i), (i >> 1) & 1, abort);
+          tc_fence_after();
+          const uint32_t w = tmem + m * L::COLS + (NT == 2 ? L::P_COL : L::S_COL + (i & 1) * NK), o = tmem + m * L::COLS + L::O_COL;
+          const uint64_t v = vd + (i & 1) * (L::TILE / 16);
+#pragma unroll
+          for (int n = NT - 1; n >= 0; n--)
+#pragma unroll
+            for (int s = 0; s < NK / 16; s++)
+              mma_f16_ts<DH, true>(o, w + n * (NK / 2) + s * 8, v + s * 16, (NT == 1 && i > 0) || s > 0 || n < NT - 1);
+          commit_one(pvdone_of(m, i));
+        }
       }
     }
+    __syncwarp();
   } else if (tid >= SOFT) {  // ---------------------------------------- codes
     // 16 bytes of a row a lane (RL lanes a row), NP passes of RP rows; a
     // thread's row of pass w is w * RP + key0.  Eight lanes that store together
