@@ -678,10 +678,11 @@ Variant variant_as() {
   using G = Geo<TYPE, DH, NT, NB, RG>;
   return {k_kv_attn<TYPE, DH, NT, NB, RG>, G::SMEM, G::ROWS};
 }
-// From TC_FROM rows on half-precision queries take the tcgen05 kernel.
-// (16 rows: 281 us here and 513 there for 40 sequences of 15000 positions; 24: 513 and 517.)
-constexpr long long TC_FROM = 17;
-constexpr long long TC32_FROM = 33;
+// From TC_FROM rows on half-precision queries take the tcgen05 kernel (16 rows:
+// 281 us here and 513 there for 40 sequences of 15000 positions; 24: 513 and
+// 517), f32 ones of head_dim 64 from TC32_FROM (8 sequences of 2000 positions,
+// 36 heads: 32 rows 91 us here; 33 rows 138 and 111; 128 rows 253 and 130).
+constexpr long long TC_FROM = 17, TC32_FROM = 33;
 template <int TYPE, int DH, int NT>
 Variant variant_rows(long long rows) {
   if (rows <= 8) return variant_as<TYPE, DH, NT, 1, 1>();
@@ -689,12 +690,11 @@ Variant variant_rows(long long rows) {
   if constexpr (NT == 1) {
     static_assert(TC_FROM == 17, "half-precision rows past 16");
     return {nullptr, 0, 128};
+  } else if constexpr (DH == 64) {
+    static_assert(TC32_FROM == 33, "f32 rows past 32");
+    return rows <= 32 ? variant_as<TYPE, DH, NT, 4, 1>() : Variant{nullptr, 0, 256};
   } else {
-    if (DH == 64 && rows >= TC32_FROM) return {nullptr, 0, 256};
-    constexpr int NBM = DH == 128 ? 2 : 4;
-    if (rows <= 8 * NBM) return variant_as<TYPE, DH, NT, NBM, 1>();
-    if (rows <= 16 * NBM) return variant_as<TYPE, DH, NT, NBM, 2>();
-    return variant_as<TYPE, DH, NT, NBM, 4>();
+    return rows <= 32 ? variant_as<TYPE, DH, NT, 2, 2>() : variant_as<TYPE, DH, NT, 2, 4>();
   }
 }
 template <int TYPE, int DH>
@@ -713,7 +713,10 @@ Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int ty
 // shared memory (up to 16 are made 8): that saves the scratch and a second
 // launch, 13 us to 11 for one token at 1500 positions.  Elsewhere a cluster's
 // CTAs would hold their SMs until its longest is done (eight 16K streams 171 us
-// against 150), so their parts go through the scratch.
+// against 150), so their parts go through the scratch.  The kernel with one CTA
+// an SM takes the number of chunks with the least rounds, each as long as its
+// tiles and 8 more for its beginning and end (two prompt chunks, 144 CTAs: one
+// chunk 148 us, two 164, eight 210).
 struct Split {
   int chunk, n_chunk, row_tiles;
   bool cluster;
@@ -725,7 +728,7 @@ Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, const Vari
   const long long units = (long long)s.n_seq * c.n_kv * p.row_tiles, want = 148 * 8;
   const long long most = (s.max_len + MIN_CHUNK - 1) / MIN_CHUNK;
   long long n = std::max<long long>(1, std::min(most, want / units));
-  if (!v.k && v.rows == 256) {  // one CTA an SM: the number of chunks that takes the least rounds of tiles and beginnings
+  if (v.rows == 256) {
     const long long top = std::min(most, std::max<long long>(1, want / units));
     long long best = 0;
     for (long long c = 1; c <= top; c++) {
@@ -733,7 +736,7 @@ Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, const Vari
       if (c == 1 || t < best) best = t, n = c;
     }
   }
-  const long long slots = v.k || v.rows == 128 ? 296 : 128;  // CTAs that are sure to run at once, in clusters too
+  const long long slots = v.rows == 256 ? 128 : 296;  // CTAs that run at once, in clusters too
   if (n > 8 && n <= 16 && units * 8 <= slots) n = 8;
   p.chunk = (int)(((s.max_len + n - 1) / n + 63) / 64 * 64);
   p.n_chunk = (int)((s.max_len + (long long)p.chunk - 1) / p.chunk);

@@ -1,22 +1,37 @@
 // pk_cache_attn_tc.cu -- attention over the quantised cache for many query
-// rows of a kv head (drafted trees, prompt chunks; half-precision queries) on
-// the fifth-generation tensor cores.  The formulas are pk_cache_attn.cu's.
+// rows of a kv head (drafted trees, prompt chunks) on the fifth-generation
+// tensor cores.  The formulas are pk_cache_attn.cu's.
 //
-// A CTA takes 128 rows (token, query head) of one kv head over one chunk of
-// positions, 64 at a time: S = Q K^T (M 128 x N 64 x K head_dim) into one of
-// two TMEM buffers, weights P in their place, O += P V (M 128 x N head_dim x
-// K 64) in TMEM.  416 threads:
-//   warps 0-3   softmax: thread = row = TMEM lane.  Scores from TMEM, the
-//               scales D^K and D^V applied in f32 (two at a time), weights as
-//               f16 into the scores' columns.
-//   warps 4-7   K's codes, and the scales of both: a tile's are asked for a
-//               tile ahead, made f16 (exact) and put into the operand's layout.
-//   warps 8-11  V's codes.
-//   warp 12     issues the products.
-// Two CTAs share an SM (100 KB and 256 TMEM columns each), so that one's
-// products run beside the other's softmax.  Operands are in the canonical
-// layout without swizzle, core matrices of 8 rows x 16 bytes.  V's rows are
-// stored as K's, which makes it an N-major operand.
+// A CTA takes one or two blocks of 128 rows (token, query head) of one kv head
+// over one chunk of positions, 64 at a time: S = Q K^T (M 128 x N 64 x K
+// head_dim) into one of two TMEM buffers, weights P, O += P V (M 128 x N
+// head_dim x K 64) in TMEM.  Warps, of a block each where it says so:
+//   4 a block  softmax.  Four lanes share a row (the layout of the tensor
+//              core's own fragments): a thread has 4 rows and a quarter of the
+//              columns, and so reads a quarter of the tile's scales D^K and
+//              D^V (with a row a thread, those reads, 512 bytes to the warp
+//              however few they are, were a third of shared memory's time).
+//   4          K's codes, and the scales of both: a tile's are asked for a
+//              tile ahead, made f16 (exact) and put into the operand's layout.
+//   4          V's codes.
+//   1          issues the products.
+// Half precision: one block, P as f16 in S's columns, O summed in TMEM, and two
+// CTAs an SM (100 KB and 256 TMEM columns each), so that one's products run
+// beside the other's softmax.  f32 (head_dim 64): queries and weights are two
+// f16 terms each (2^-22), and a tile's O is added to the row's sums in
+// registers, because the tensor core's sums drop what they shift out; two
+// blocks share a CTA's codes, one CTA an SM.  Operands are in the canonical
+// layout without swizzle, core matrices of 8 rows x 16 bytes (a product takes
+// 61 cycles so, 66 with 128-byte swizzle).  V's rows are stored as K's, which
+// makes it an N-major operand.
+//
+// Measured: 8 sequences of 32000 positions with trees of 64, 64 heads over 8,
+// f16, Q8: 749 us, 715 TFLOP/s; 40 sequences of up to 15000 positions, 5 drafts
+// each, bf16, Q4: 236 us; two prompt chunks of 509 tokens behind up to 2900
+// positions, 36 heads, f32, Q8: 148 us.  What bounds it: a product of N 64
+// takes as long as one of N 128, so the tensor core is busy for 830 cycles of
+// the 1,400 or so that a tile of 64 positions takes an SM; 128 positions a step
+// would need 384 TMEM columns a CTA.
 //
 // A row keeps one reference m for its weights 2^(s - m): they are summed as
 // they are and multiplied by D^V into f16.  It is set so that the row's
@@ -47,14 +62,16 @@ constexpr unsigned long long WAIT_NS = 2000000000ull;
 template <class E>
 constexpr int terms_of = std::is_same_v<E, float> ? 2 : 1;
 
-template <int DH, int NT, int BLK>
+// Geometry, by the terms.
+template <int DH, int NT>
 struct Lay {
+  static constexpr int BLK = NT;  // blocks of 128 rows
   // (two blocks: whole warpgroups, as the last one gives registers away too)
   static constexpr int ROWS = 128 * BLK, SOFT = 128 * BLK, CONV = 128, MMA = BLK == 1 ? 32 : 128, THREADS = SOFT + 2 * CONV + MMA;
   // Registers a thread: at launch, and after the others have given the softmax
   // warps theirs.
-  static constexpr int CTAS = BLK == 1 ? 2 : 1, REGS = BLK == 1 ? 72 : 96, REGS_SOFT = BLK == 1 ? 104 : NT == 2 ? 168 : 152;
-  static constexpr int REGS_CONV = BLK == 1 ? 56 : NT == 2 ? 48 : 64, REGS_MMA = BLK == 1 ? REGS : 48;
+  static constexpr int CTAS = BLK == 1 ? 2 : 1, REGS = BLK == 1 ? 72 : 96, REGS_SOFT = BLK == 1 ? 104 : 168;
+  static constexpr int REGS_CONV = BLK == 1 ? 56 : 48, REGS_MMA = BLK == 1 ? REGS : 48;
   static_assert(SOFT * REGS_SOFT + 2 * CONV * REGS_CONV + MMA * REGS_MMA <= THREADS * REGS, "no more than the launch's");
   static_assert(CTAS * THREADS * REGS <= 65536, "all of an SM's CTAs");
   // chunks of 16 bytes (8 dimensions) of consecutive positions; one chunk's
@@ -208,9 +225,10 @@ __host__ __device__ constexpr int dim8(int i) {
   return TYPE == PK_KV_Q8 ? i : (i / 2) + 4 * (i % 2);
 }
 
-// This thread's query row into the operand, f16 as it is, bf16 scaled to
-// |q'| < 2 and rounded to f16 (exact down to 2^-24 of the row's largest); its
-// scale (the D^K that the row meets have log2(e) * scale in them).
+// This thread's query row into the operand, f16 as it is, others scaled to
+// |q'| < 2 and rounded to f16 (bf16: exact down to 2^-24 of the row's largest;
+// f32: a second term holds the rest); its scale (the D^K that the row meets
+// have log2(e) * scale in them).
 template <int TYPE, int DH, class E>
 __device__ __forceinline__ float put_q(const AttnKArgs &a, const Unit &u, int row, uint32_t dst, int stride, int term) {
   constexpr bool F16 = std::is_same_v<E, __half>;
@@ -271,10 +289,10 @@ __device__ __forceinline__ uint64_t seen_by(const AttnKArgs &a, const Unit &u, i
   return v & ones(hi - p0) & ones(u.sv.ctx + u.sv.n - p0);
 }
 
-template <int TYPE, int DH, class E, int BLK>
-__global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, terms_of<E>, BLK>::CTAS) k_kv_attn_tc(const AttnKArgs a) {
-  constexpr int NT = terms_of<E>;
-  using L = Lay<DH, NT, BLK>;
+template <int TYPE, int DH, class E>
+__global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_of<E>>::CTAS) k_kv_attn_tc(const AttnKArgs a) {
+  constexpr int NT = terms_of<E>, BLK = NT;
+  using L = Lay<DH, NT>;
   constexpr int ROWS = L::ROWS, SOFT = L::SOFT, CONV = L::CONV, THREADS = L::THREADS, WS = SOFT / 32;
   constexpr bool F16 = std::is_same_v<E, __half>;
   constexpr int RB = TYPE == PK_KV_Q8 ? DH : DH / 2, SW = TYPE == PK_KV_Q8 ? 1 : 2;
@@ -375,8 +393,9 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
     // have RS parts of a row and 8 / RS rows, so that they touch every bank
     // once (a part's chunks are 2 or 4 strides from the next part's).
     set_regs<false, L::REGS_CONV>();
-    auto role = [&](auto v_role) {
-    constexpr bool is_v = decltype(v_role)::value;
+    // (one body for both: two cost 15% by their size alone, the SM's warps being
+    // in all parts of the loops at once)
+    const bool is_v = warp >= WS + 4;
     constexpr int RL = RB / 16, RP = CONV / RL, NP = NK / RP;
     constexpr int RS = TYPE == PK_KV_Q8 ? 4 : 2;
     const int ct = (tid - SOFT) & (CONV - 1);
@@ -460,9 +479,6 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
       mbar_arrive(is_v ? vready + 8 * (i & 1) : kready + 8 * (i & 3));
       if (i + 1 < nt) ask(i + 1);
     }
-    };
-    if (warp < WS + 4) role(std::false_type());
-    else role(std::true_type());
   } else {  // ------------------------------------------------------------ softmax
     set_regs<true, L::REGS_SOFT>();
     const int blk = BLK == 1 ? 0 : warp >> 2;
@@ -782,25 +798,24 @@ struct Kernel {
   void (*k)(AttnKArgs);
   int threads, smem, regs;
 };
-template <int TYPE, int DH, class E, int BLK>
+template <int TYPE, int DH, class E>
 Kernel kernel_as() {
-  using L = Lay<DH, terms_of<E>, BLK>;
-  return {k_kv_attn_tc<TYPE, DH, E, BLK>, L::THREADS, L::BYTES, L::REGS};
+  using L = Lay<DH, terms_of<E>>;
+  return {k_kv_attn_tc<TYPE, DH, E>, L::THREADS, L::BYTES, L::REGS};
 }
-template <class E, int BLK>
+template <class E>
 Kernel kernel_of(const pk_kv_cache &c) {
-  if constexpr (terms_of<E> == 2) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 64, E, BLK>() : kernel_as<PK_KV_Q4, 64, E, BLK>();
-  else
-    return c.type == PK_KV_Q8 ? (c.head_dim == 64 ? kernel_as<PK_KV_Q8, 64, E, BLK>() : kernel_as<PK_KV_Q8, 128, E, BLK>())
-                              : (c.head_dim == 64 ? kernel_as<PK_KV_Q4, 64, E, BLK>() : kernel_as<PK_KV_Q4, 128, E, BLK>());
+  if (c.head_dim == 64) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 64, E>() : kernel_as<PK_KV_Q4, 64, E>();
+  if constexpr (terms_of<E> == 1) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 128, E>() : kernel_as<PK_KV_Q4, 128, E>();
+  return {};
 }
 
 }  // namespace
 
 cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int cluster, unsigned blocks, cudaStream_t st) {
   const int e = a.q.type == T_F32 ? 0 : a.q.type == T_F16 ? 1 : 2;
-  const Kernel k = e == 0             ? kernel_of<float, 2>(a.c)
-                   : e == 1           ? kernel_of<__half, 1>(a.c) : kernel_of<__nv_bfloat16, 1>(a.c);
+  const Kernel k = e == 0 ? kernel_of<float>(a.c) : e == 1 ? kernel_of<__half>(a.c) : kernel_of<__nv_bfloat16>(a.c);
+  if (!k.k) return cudaErrorInvalidValue;
   // the split of the registers would wait forever for what a launch does not have
   static std::atomic<unsigned> checked{0};
   const unsigned bit = 1u << (e * 4 + 2 * (a.c.type == PK_KV_Q4) + (a.c.head_dim == 128));

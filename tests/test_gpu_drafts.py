@@ -316,6 +316,73 @@ def test_attention_causal(pk, kind, dh, ty, shape):
     check_attention(su, q, su.cache.attend(su.seqs, q))
 
 
+WIDE = [
+    # row counts around a block of 128 and two, of one tile of positions and of many (two f32 prompts are split over a
+    # cluster, the last one's over the scratch), with sequences that have nothing
+    ([0], [33], 1, 1, 16),
+    ([0, 90, 0], [129, 0, 1], 1, 1, 16),
+    ([63, 64, 1], [64, 1, 40], 8, 2, 16),
+    ([0, 700], [257, 31], 3, 3, 32),
+    ([2500, 40], [200, 130], 2, 2, 64),
+    ([1700], [64], 40, 20, 64),
+]
+
+
+@pytest.mark.parametrize("kind", ["q8", "q4"])
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("ty", list(DT))
+@pytest.mark.parametrize("shape", WIDE)
+def test_attention_wide(pk, kind, dh, ty, shape):
+    lens, new, n_head, n_kv, page = shape
+    su = Setup(pk, lens, new, kind, n_kv, dh, page, seed=dh + n_head, extra_rows=1)
+    su.fill(pk)
+    q = randn((su.n_tok, n_head, dh), 8, DT[ty], std=1.5)
+    check_attention(su, q, su.cache.attend(su.seqs, q))
+    see = {s: torch.rand((n, n), generator=gen(50 + s), device="cuda") < 0.3 for s, n in enumerate(new)}
+    words = max(1, -(-max(new) // 64))
+    mask = torch.zeros((su.n_tok, words), dtype=torch.int64)
+    for s, n in enumerate(new):
+        for i in range(n):
+            bits = sum(1 << int(j) for j in see[s][i].nonzero()[:, 0].tolist())
+            for w in range(words):
+                x = (bits >> (64 * w)) & (2 ** 64 - 1)
+                mask[int(su.start[s]) + i, w] = x - 2 ** 64 if x >= 2 ** 63 else x
+    check_attention(su, q, su.cache.attend(su.seqs, q, mask=mask.cuda()), see=lambda s, n: see[s])
+
+
+@pytest.mark.parametrize("ty", list(DT))
+@pytest.mark.parametrize("dh", [64, 128])
+def test_attention_query_range(pk, dh, ty):
+    """Rows of very different sizes side by side, rows of zeros, and rows of infinities and NaN, which spoil no other."""
+    su = Setup(pk, [333], [140], "q8", 1, dh, 16, seed=4)
+    su.fill(pk)
+    q = randn((140, 2, dh), 8, torch.float32)
+    q[0::7] *= 100.0
+    q[1::7] *= 6e-8 if ty == "f16" else 1e-30
+    q[2::7] = 0
+    q = q.to(DT[ty])
+    bad = torch.zeros(140, dtype=torch.bool, device="cuda")
+    bad[[5, 12, 61, 139]] = True
+    q[5], q[12, :, 3], q[61, 1] = math.inf, math.nan, -math.inf
+    q[139, 0, 0] = math.nan
+    clean = torch.where(bad[:, None, None], torch.zeros_like(q), q)
+    # Rows of large scores may have one weight that counts, and a V code of 0 there: then what is left are products
+    # w D^V below f16's normal values, off by 2^-25 each, where the row's largest is 2^6 or more.  With D <= max |v| / 97
+    # (Q4's codes go to 97 at least, Q8's to 127) and |c| <= 127, n positions are off by n 2^-31 127 / 97 of the largest
+    # p max |v|; n 2^-30 of it is allowed.
+    k64, v64 = decoded(su.cache)
+    pg, sl = su.rows(0)
+    for scale, x in ((dh ** -0.5, q), (dh ** -0.5, clean), (0.3, clean), (1e-3, clean)):
+        got = su.cache.attend(su.seqs, x, scale=scale)
+        want, absv, dots = attention(su, clean, scale=scale)
+        p = (clean.double() @ k64[pg, 0, sl].T * scale).masked_fill(torch.ones((140, 473), device="cuda").triu(334).bool()[:, None], -math.inf)
+        most = (torch.softmax(p, -1) * v64[pg, 0, sl].abs().amax(-1)).amax(-1, keepdim=True)
+        ok = ~bad if x is q else torch.ones_like(bad)
+        assert torch.isfinite(got[ok].double()).all()
+        lim = attn_bound(clean, want, absv, dots, dh) + 473 * 2.0 ** -30 * most
+        assert ((got.double() - want).abs() <= lim)[ok].all(), scale
+
+
 def tree(n, seed, empty=()):
     """Ancestor bits of a random tree, parents first; rows of `empty` see nothing new."""
     rng = np.random.default_rng(seed)
