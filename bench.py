@@ -59,7 +59,7 @@ def parse_args():
     p.add_argument("--stream-ctx", type=int, default=512, help="KV positions of each stream")
     p.add_argument("--stream-prompt", type=int, default=None,
                    help="prompt tokens prefilled into each stream's cache (default 323)")
-    p.add_argument("--kv", choices=("f32", "f16"), default="f32",
+    p.add_argument("--kv", choices=("f32", "f16", "q8", "q4"), default="f32",
                    help="K/V cache entry type of the streams case (pk_set_kv_type)")
     p.add_argument("--stream-pos", type=int, default=None,
                    help="decode the streams at this position (past the prompt: zero-filled cache entries; "
@@ -837,7 +837,8 @@ def run_streams(args):
     if rank == 0:
         hbm, peak_kind = peaks()
         mean_pos = p0 + 1 + min(args.steps, CYCLE) / 2
-        kv_pos_bytes = spec.kv_bytes_per_position() // (2 if args.kv == "f16" else 1)
+        row = {"f32": 4 * spec.head_dim, "f16": 2 * spec.head_dim, "q8": spec.head_dim + 4, "q4": spec.head_dim // 2 + 8}[args.kv]
+        kv_pos_bytes = spec.kv_bytes_per_position() // (4 * spec.head_dim) * row
         step_bytes = info["stream_bytes"] + len(mine) * kv_pos_bytes * mean_pos
         gbs = step_bytes / (ms_step / 1000.0) / 1e9
         line = {

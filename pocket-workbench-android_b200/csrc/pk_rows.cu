@@ -22,6 +22,7 @@ namespace {
 // its place in the head and goes from head to head, so its cosines and sines
 // stay in registers and its addresses are additions (with an item's place
 // divided out anew, index arithmetic was half the kernel's instructions).
+// 8191 tokens of 72 heads of 64, 48 rotated, f16: 34 us, 69% of a copy's rate.
 constexpr int RT = 256;
 // AL: whole runs, aligned to their size; otherwise moved by elements, the last
 // run of an odd head_dim one short (n < V).
