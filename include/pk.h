@@ -387,6 +387,9 @@ int pk_kv_keep(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const int *keep
  *   mask    device, [n_tok][mask_words], or null
  * Scores and sums are f32; a softmax weight times its V scale is rounded to
  * f16 as a fraction of the row's largest (to two f16 terms for f32 queries).
+ * A query row with infinities or NaN gives NaN, and leaves other rows as they
+ * are up to rounding.  The kernels' own waits are bounded: one that runs out
+ * after 2 s, which a working device never sees, leaves NaN in its rows.
  * scratch: pk_kv_attn_scratch_bytes bytes of device memory, 16-byte aligned
  * (may be null when that is 0), which calls that overlap in time, replays of
  * captured graphs among them, must not share. */

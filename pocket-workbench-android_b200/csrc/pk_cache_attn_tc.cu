@@ -89,8 +89,8 @@ struct Lay {
   static_assert(O_COL + DH + (NT == 2 ? NK : 0) <= COLS && CTAS * BLK * COLS <= 512, "the columns there are");
 };
 
-// mbar_test that may sleep for up to 20 us: 13 warps that ask again and again
-// take a third of an SM's issue slots.
+// mbar_test that may sleep for up to 20 us: warps that ask again and again take
+// issue slots from the others (prompt chunks 154 us so, 148 asleep).
 __device__ __forceinline__ bool mbar_sleep(uint32_t b, uint32_t parity) {
   uint32_t ok;
   asm volatile(
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
 
   if (warp >= WS + 8) {  // ------------------------------------------- products
     if (BLK > 1) set_regs<false, L::REGS_MMA>();
-    // one thread issues them all (elected anew for each, they take twice as long)
+    // one thread issues them all
     if (warp == WS + 8 && elect_one()) {
       const uint64_t qd = tc_desc(sb + L::Q, ROWS * 16, 128), kd = tc_desc(sb + L::K, L::CH, 128), vd = tc_desc(sb + L::V, 128, L::CH);
       auto scores = [&](int i) {

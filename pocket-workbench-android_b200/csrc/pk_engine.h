@@ -165,7 +165,7 @@ class Engine {
   const int *d_qiota_ = nullptr, *d_qstart_ = nullptr;
   const double *d_qturns_ = nullptr;
   float qgain_ = 1.0f;
-  uint8_t *q_scratch_[6] = {};
+  uint8_t *q_scratch_[NLANES] = {};
   size_t q_scratch_bytes_ = 0;
   size_t qpool_half(int n_pages) const;
   int setup_qcache();
