@@ -350,6 +350,49 @@ def test_attention_wide(pk, kind, dh, ty, shape):
     check_attention(su, q, su.cache.attend(su.seqs, q, mask=mask.cuda()), see=lambda s, n: see[s])
 
 
+def test_attention_wide_side_by_side(pk):
+    """Kernels that take a half or all of an SM's tensor memory, on two streams at once and replayed from graphs: the
+    results of each alone."""
+    runs = []
+    for i, (ty, dh, lens, new, heads) in enumerate((("f32", 64, [900, 3], [300, 140], 12), ("f16", 128, [2000], [90], 24), ("bf16", 64, [50, 800], [33, 64], 16))):
+        su = Setup(pk, lens, new, "q8", heads // 2, dh, 64, seed=i)
+        su.fill(pk)
+        q = randn((su.n_tok, heads, dh), 8 + i, DT[ty])
+        want = su.cache.attend(su.seqs, q)
+        out = [torch.empty_like(q) for _ in range(2)]
+        scratch = [torch.empty(max(16, su.cache.attend_scratch_bytes(su.seqs, heads, q.dtype)), dtype=torch.uint8, device="cuda") for _ in range(2)]
+        runs.append((su, q, want, out, scratch))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+
+    def go(w, order):
+        for j in order:
+            su, q, _, out, scratch = runs[j]
+            su.cache.attend(su.seqs, q, out=out[w], scratch=scratch[w])
+
+    graphs = []
+    for w, order in enumerate(([0, 1, 2], [2, 0, 1])):
+        with torch.cuda.stream(streams[w]):
+            go(w, order)
+        streams[w].synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=streams[w]):
+            go(w, order)
+        graphs.append(g)
+    for _, _, _, out, _ in runs:
+        for o in out:
+            o.zero_()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for w in range(2):
+            with torch.cuda.stream(streams[w]):
+                go(w, [w, 2, 1 - w])
+                graphs[w].replay()
+    torch.cuda.synchronize()
+    for _, _, want, out, _ in runs:
+        assert torch.equal(out[0], want) and torch.equal(out[1], want)
+
+
 @pytest.mark.parametrize("ty", list(DT))
 @pytest.mark.parametrize("dh", [64, 128])
 def test_attention_query_range(pk, dh, ty):

@@ -105,6 +105,21 @@ def test_prompts_in_lanes(pk, paths, name, kind):
     assert a.generate(np.concatenate([ids, ids[:9]]), 2, stop_at_eog=False)["prefill_cached_tokens"] > 0
 
 
+def test_lanes_with_the_tensor_memory_matvecs(pk, paths):
+    """Six lanes of chunks whose matvecs and attention both use tensor memory: the default matvecs' tokens (the two
+    paths give the same bits)."""
+    ids = synth.prompt_ids(31, 250, synth.SMALL_Q40.n_vocab)
+    want = pk.Engine(paths["q40"], n_ctx=320, kv="q8").generate(ids, 12, stop_at_eog=False)["gen_ids"]
+    pk.set_matmul_path("tcgen05")
+    try:
+        e = pk.Engine(paths["q40"], n_ctx=320, kv="q8")
+        for _ in range(3):
+            assert e.generate(ids, 12, stop_at_eog=False)["gen_ids"] == want
+            e.forward(ids[:1], [0])  # (drops the prefix)
+    finally:
+        pk.set_matmul_path("mma.sync")
+
+
 @pytest.mark.parametrize("kind", ["q8", "q4"])
 @pytest.mark.parametrize("name", ["tiny", "q8down", "dh128"])
 def test_streams(pk, paths, name, kind):
