@@ -175,6 +175,23 @@ def test_long_history(pk, paths):
     assert np.linalg.norm(x - y) <= 0.02 * np.linalg.norm(x)
 
 
+@pytest.mark.parametrize("kind", ["q8", "q4"])
+def test_device_steps(pk, paths, kind):
+    """Steps kept on the device (one graph a step), a rewound position, the fast order, and the per-kernel profile."""
+    ids = synth.prompt_ids(37, 70, synth.TINY.n_vocab)
+    want = pk.Engine(paths["tiny"], n_ctx=256, kv=kind).generate(ids, 20, stop_at_eog=False)["gen_ids"]
+    e = pk.Engine(paths["tiny"], n_ctx=256, kv=kind, order="fast")
+    e.generate(ids, 1, stop_at_eog=False)
+    assert list(e.decode_steps_device(20)) == want
+    e.set_position(70)
+    e.generate(ids, 1, stop_at_eog=False)
+    assert list(e.decode_steps_device(5)) == want[:5]
+    names = {r["name"] for r in e.decode_profile()}
+    assert {"k_rope", "k_kv_store", "k_kv_attn"} <= names
+    e.generate(ids, 1, stop_at_eog=False)
+    assert list(e.decode_steps_device(5)) == want[:5]
+
+
 def test_refusals(pk, paths):
     e = pk.Engine(paths["tiny"], n_ctx=128, kv="q8")
     ids = synth.prompt_ids(3, 4, synth.TINY.n_vocab)
