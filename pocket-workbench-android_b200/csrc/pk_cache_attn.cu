@@ -719,10 +719,13 @@ Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int ty
 // shared memory (up to 16 are made 8): that saves the scratch and a second
 // launch, 13 us to 11 for one token at 1500 positions.  Elsewhere a cluster's
 // CTAs would hold their SMs until its longest is done (eight 16K streams 171 us
-// against 150), so their parts go through the scratch.  The kernel with one CTA
-// an SM takes the number of chunks with the least rounds, each as long as its
-// tiles and 8 more for its beginning and end (two prompt chunks, 144 CTAs: one
-// chunk 148 us, two 164, eight 210).
+// against 150), so their parts go through the scratch.  The tcgen05 kernel's chunks
+// are as many as take the least time by its rounds of CTAs: a CTA costs its
+// tiles of 64 positions and 16 more (one CTA an SM: 8) for its beginning and
+// its part of the sums, and where two share an SM a tile takes 8 fifths of what
+// it takes alone (64 tokens at 8000 positions, 64 heads over 8: 4 chunks, one
+// CTA an SM, 53 us, 8 chunks 66, one 127, 37 100; 32 sequences of 2000: one
+// chunk 61, two 79, four 100; the wide trees 770, 799 and 750).
 struct Split {
   int chunk, n_chunk, row_tiles;
   bool cluster;
@@ -734,16 +737,18 @@ Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, const Vari
   const long long units = (long long)s.n_seq * c.n_kv * p.row_tiles, want = 148 * 8;
   const long long most = (s.max_len + MIN_CHUNK - 1) / MIN_CHUNK;
   long long n = std::max<long long>(1, std::min(most, want / units));
-  if (v.rows == 256) {
-    const long long top = std::min(most, std::max<long long>(1, want / units));
+  if (!v.k) {
     long long best = 0;
+    const long long top = n;
     for (long long c = 1; c <= top; c++) {
-      const long long t = (units * c + 147) / 148 * ((s.max_len / c + 63) / 64 + 8);
+      const long long ctas = units * c, left = ctas % 296, tiles = ((s.max_len + 63) / 64 + c - 1) / c;
+      const long long t = v.rows == 256 ? (ctas + 147) / 148 * (tiles + 8)
+                                        : (ctas / 296 * 8 + (left == 0 ? 0 : left <= 148 ? 5 : 8)) * (tiles + 16);
       if (c == 1 || t < best) best = t, n = c;
     }
   }
   const long long slots = v.rows == 256 ? 128 : 296;  // CTAs that run at once, in clusters too
-  if (n > 8 && n <= 16 && units * 8 <= slots) n = 8;
+  if (v.k && n > 8 && n <= 16 && units * 8 <= slots) n = 8;
   p.chunk = (int)(((s.max_len + n - 1) / n + 63) / 64 * 64);
   p.n_chunk = (int)((s.max_len + (long long)p.chunk - 1) / p.chunk);
   p.cluster = p.n_chunk > 1 && p.n_chunk <= 8 && units * p.n_chunk <= slots;
