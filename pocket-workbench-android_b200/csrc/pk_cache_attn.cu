@@ -684,10 +684,12 @@ Variant variant_as() {
   using G = Geo<TYPE, DH, NT, NB, RG>;
   return {k_kv_attn<TYPE, DH, NT, NB, RG>, G::SMEM, G::ROWS};
 }
-// From TC_FROM rows on half-precision queries take the tcgen05 kernel (16 rows:
-// 281 us here and 513 there for 40 sequences of 15000 positions; 24: 513 and
-// 517), f32 ones of head_dim 64 from TC32_FROM (8 sequences of 2000 positions,
-// 36 heads: 32 rows 91 us here; 33 rows 138 and 111; 128 rows 253 and 130).
+// From TC_FROM rows on half-precision queries take the tcgen05 kernel, whose
+// time hardly depends on the rows up to 128 (40 sequences of 7500 and 15000
+// positions, Q4: 16 rows 252 us here and 340 there, 8 rows 188 and 337; past 16
+// a row tile here takes twice as long), f32 ones of head_dim 64 from TC32_FROM
+// (8 sequences of 2000 positions, 36 heads: 32 rows 91 us here; 33 rows 138 and
+// 111; 128 rows 253 and 130).
 constexpr long long TC_FROM = 17, TC32_FROM = 33;
 template <int TYPE, int DH, int NT>
 Variant variant_rows(long long rows) {
