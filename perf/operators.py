@@ -22,18 +22,12 @@ SIZE = {"f32": 4, "f16": 2, "bf16": 2}
 BIG = 2.0 ** 127  # larger magnitudes are stored as this
 
 
-_module = []
-
-
 def _pk():
-    if _module:
-        return _module[0]
     path = os.path.join(os.getcwd(), "pocket-workbench-android_b200")
     if path not in sys.path:
         sys.path.insert(0, path)
     import pocketinfer
 
-    _module.append(pocketinfer)
     return pocketinfer
 
 
