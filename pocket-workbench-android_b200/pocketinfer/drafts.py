@@ -6,7 +6,8 @@
 
 Nothing here waits for the device, and every call can be captured into a CUDA graph once its outputs and scratch are
 passed in (or come from the graph's own pool).  Calls run on the tensors' device, on its current stream or on the
-`stream` given (a raw cudaStream_t).
+`stream` given (a raw cudaStream_t).  With `stream`, what a call makes (outputs, scratch) comes from that stream's
+memory; the caller orders its own tensors, and its later use of the outputs, against that stream.
 """
 from __future__ import annotations
 
@@ -99,20 +100,30 @@ def _dtype(t, who):
     return code
 
 
-def _call(fn, device, stream, used, *args):
-    """fn(*args, stream) on device number `device`; `used`: tensors made by this call, which a stream that is not the
-    current one must be known to use."""
+def _call(fn, device, stream, *args):
+    """fn(*args, stream) on device number `device`."""
     if stream is None and current_device() == device:
         rc = fn(*args, raw_stream(device))
     else:
         with torch.cuda.device(device):
             rc = fn(*args, raw_stream(device) if stream is None else stream)
-            if stream is not None and used:
-                ext = torch.cuda.ExternalStream(stream)
-                for t in used:
-                    t.record_stream(ext)
     if rc:
         raise PkError(rc, last_error())
+
+
+def _new(make, device, stream, kept=True):
+    """make(), a tensor or some, on device number `device` for a call on `stream`: from that stream's pool, because a
+    block freed on the current stream may still be in use there.  kept: the caller gets them and may use them on the
+    current stream too, which the allocator then has to know."""
+    if stream == raw_stream(device):
+        return make()
+    here = torch.cuda.current_stream(device)
+    with torch.cuda.device(device), torch.cuda.stream(torch.cuda.ExternalStream(stream, device=device)):
+        made = make()
+    if kept:
+        for t in made if isinstance(made, tuple) else (made,):
+            t.record_stream(here)
+    return made
 
 
 def _i32(t, device, name, dims):
@@ -187,17 +198,17 @@ class KvCache:
 
     def store(self, seqs: KvSeqs, k, v, stream=None):
         """Quantises rows k, v [n_tok, n_kv, head_dim] of the new tokens into the cache."""
-        _call(_L.pk_kv_store, self.device, stream, (), self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "store"))
+        _call(_L.pk_kv_store, self.device, stream, self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "store"))
 
     def load(self, seqs: KvSeqs, dtype=None, out=None, stream=None):
         """(k, v) [n_tok, n_kv, head_dim] of positions ctx .. read back; rows that no sequence has keep what they held."""
-        made = ()
         if out is None:
             dh, dt, dev = self.head_dim, dtype or torch.float32, self.k.device
             shape, st = (seqs.n_tok, self.n_kv, dh), (self.n_kv * dh, dh, 1)
-            made = out = torch.empty_strided(shape, st, dtype=dt, device=dev), torch.empty_strided(shape, st, dtype=dt, device=dev)
+            make = lambda: torch.empty_strided(shape, st, dtype=dt, device=dev)  # noqa: E731
+            out = (make(), make()) if stream is None else _new(lambda: (make(), make()), self.device, stream)
         k, v = out
-        _call(_L.pk_kv_load, self.device, stream, made, self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "load"))
+        _call(_L.pk_kv_load, self.device, stream, self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "load"))
         return k, v
 
     def keep(self, seqs: KvSeqs, keep, n_keep, stream=None):
@@ -206,7 +217,7 @@ class KvCache:
         _i32(n_keep, self.device, "n_keep", 1)
         if keep.shape[0] != seqs.n_seq or n_keep.shape[0] != seqs.n_seq or seqs.device != self.device:
             _bad("keep: one row and one count a sequence, on the cache's device")
-        _call(_L.pk_kv_keep, self.device, stream, (), self.ref, seqs.ref, keep.data_ptr(), keep.shape[1], n_keep.data_ptr())
+        _call(_L.pk_kv_keep, self.device, stream, self.ref, seqs.ref, keep.data_ptr(), keep.shape[1], n_keep.data_ptr())
 
     def attend(self, seqs: KvSeqs, q, mask=None, scale: float | None = None, out=None, scratch=None, stream=None):
         """Attention of the new tokens q [n_tok, n_head, head_dim] over the cache; mask: int64 [n_tok, words], bit j of
@@ -221,10 +232,8 @@ class KvCache:
             if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != shape[0] or not mask.is_contiguous() or mask.get_device() != dev:
                 _bad("attend: mask must be a contiguous int64 tensor [n_tok, words] on the cache's device")
             words, bits = mask.shape[1], mask.data_ptr()
-        made = ()
         if out is None:
-            out = _like(q)
-            made = (out,)
+            out = _like(q) if stream is None else _new(lambda: _like(q), dev, stream)
         elif out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or out.stride(2) != 1:
             _bad("attend: out must be as q")
         ptr, size = None, seqs.scratch.get((shape[1], code, self.kind, self.n_kv, self.head_dim))
@@ -235,13 +244,13 @@ class KvCache:
                 _bad("attend: scratch must be contiguous and on the cache's device")
             ptr, size = scratch.data_ptr(), scratch.numel() * scratch.element_size()
         elif size:
-            scratch = self.ks.new_empty((size + 3) // 4)
-            made += (scratch,)
+            make = lambda: self.ks.new_empty((size + 3) // 4)  # noqa: E731
+            scratch = make() if stream is None else _new(make, dev, stream, kept=False)
             ptr = scratch.data_ptr()
         o = out.stride()
         args = PACK_QUERY(q.data_ptr(), out.data_ptr(), bits, s[0], s[1], o[0], o[1], code, shape[1], words,
                           self.head_dim ** -0.5 if scale is None else scale)
-        _call(_L.pk_kv_attn, dev, stream, made, self.ref, seqs.ref, args, ptr, size)
+        _call(_L.pk_kv_attn, dev, stream, self.ref, seqs.ref, args, ptr, size)
         return out
 
     def attend_scratch_bytes(self, seqs: KvSeqs, n_head: int, dtype) -> int:
@@ -291,14 +300,13 @@ def rope(table: RopeTable, pos, q, k=None, layout: str = "interleaved", out_q=No
     if dev < 0:
         _bad("rope: the table is not on a CUDA device")
     _i32(pos, dev, "pos", 1)
-    code, shape, made = _dtype(q, "rope"), q.shape, []
+    code, shape = _dtype(q, "rope"), q.shape
     n, dh = pos.shape[0], shape[-1]
     qs = q.stride()
     if len(shape) != 3 or shape[0] != n or qs[2] != 1 or q.get_device() != dev:
         _bad("rope: q must be [n_tok, heads, head_dim] on the table's device, with contiguous heads")
     if out_q is None:
-        out_q = _like(q)
-        made.append(out_q)
+        out_q = _like(q) if stream is None else _new(lambda: _like(q), dev, stream)
     elif out_q.shape != shape or out_q.dtype != q.dtype or out_q.get_device() != dev or out_q.stride(2) != 1:
         _bad("rope: an output is not as its input")
     qt, ks, kt, kp, kq, nk = out_q.stride(), _NO_ROWS, _NO_ROWS, 0, 0, 0
@@ -307,14 +315,13 @@ def rope(table: RopeTable, pos, q, k=None, layout: str = "interleaved", out_q=No
         if len(kshape) != 3 or kshape[0] != n or kshape[2] != dh or ks[2] != 1 or k.dtype != q.dtype or k.get_device() != dev:
             _bad("rope: k must be [n_tok, heads, head_dim] of q's type on the table's device, with contiguous heads")
         if out_k is None:
-            out_k = _like(k)
-            made.append(out_k)
+            out_k = _like(k) if stream is None else _new(lambda: _like(k), dev, stream)
         elif out_k.shape != kshape or out_k.dtype != q.dtype or out_k.get_device() != dev or out_k.stride(2) != 1:
             _bad("rope: an output is not as its input")
         kt, kp, kq, nk = out_k.stride(), k.data_ptr(), out_k.data_ptr(), kshape[1]
     args = PACK_ROPE(q.data_ptr(), kp, out_q.data_ptr(), kq, pos.data_ptr(), table.turns.data_ptr(), qs[0], qs[1], ks[0], ks[1], qt[0],
                      qt[1], kt[0], kt[1], code, pairs, n, shape[1], nk, dh, table.n_rot, table.gain)
-    _call(_L.pk_rope, dev, stream, made, args)
+    _call(_L.pk_rope, dev, stream, args)
     return out_q, out_k
 
 
@@ -346,10 +353,8 @@ def logit_rules(logits, repeat=None, freq=None, presence=None, hist=None, n_hist
     if dev < 0 or len(shape) not in (1, 2) or st[-1] != 1:
         _bad("logit_rules: logits must be [rows, n] on a CUDA device, with contiguous rows")
     rows, n = shape if len(shape) == 2 else (1, shape[0])
-    made = ()
     if out is None:
-        out = _like(logits)
-        made = (out,)
+        out = _like(logits) if stream is None else _new(lambda: _like(logits), dev, stream)
     elif out.shape != shape or out.dtype != logits.dtype or out.get_device() != dev or out.stride(-1) != 1:
         _bad("logit_rules: out must be as the logits")
     f, i = torch.float32, torch.int32
@@ -364,6 +369,6 @@ def logit_rules(logits, repeat=None, freq=None, presence=None, hist=None, n_hist
     args = PACK_RULES(_row_value(repeat, "repeat", f, rows, dev), _row_value(freq, "freq", f, rows, dev),
                       _row_value(presence, "presence", f, rows, dev), hp, _row_value(n_hist, "n_hist", i, rows, dev), ip, bp, ap,
                       hs, bs, as_, hn, bn)
-    _call(_L.pk_apply_logit_rules, dev, stream, made, logits.data_ptr(), out.data_ptr(), code, rows, n, st[0] if len(st) == 2 else n,
+    _call(_L.pk_apply_logit_rules, dev, stream, logits.data_ptr(), out.data_ptr(), code, rows, n, st[0] if len(st) == 2 else n,
           out.stride(0) if len(st) == 2 else n, args)
     return out

@@ -827,6 +827,52 @@ def test_raw_stream_argument(pk):
     assert all(torch.equal(g, want) for g in got)
 
 
+def test_memory_of_a_call_on_another_stream(pk):
+    """What a call on `stream` makes is never a block that was freed on the current stream, where work that still reads
+    it may be queued; and once the caller lets go of it, it is not reused before the current stream is done with it."""
+    su = Setup(pk, [6000], [2], "q8", 2, 64, 16, seed=1)
+    su.fill(pk)
+    q, x, pos = randn((2, 4, 64), 3), randn((2, 1000), 4), i32([3, 4])
+    table = pk.RopeTable(64)
+    size = su.cache.attend_scratch_bytes(su.seqs, 4, q.dtype)
+    assert size > 0
+    calls = {"attend": lambda st: su.cache.attend(su.seqs, q, stream=st), "load": lambda st: su.cache.load(su.seqs, stream=st),
+             "rope": lambda st: pk.rope(table, pos, q, q[:, :2], stream=st), "rules": lambda st: pk.logit_rules(x, stream=st)}
+    want = {n: f(None) for n, f in calls.items()}
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    flat = lambda r: r if isinstance(r, tuple) else (r,)  # noqa: E731
+    for n, f in calls.items():
+        f(side.cuda_stream)  # (the side stream's own pool has what the call needs)
+        torch.cuda.synchronize()
+        # blocks of the sizes that the call makes, whose copies wait behind a long kernel when they are freed
+        sizes = [t.numel() * t.element_size() for t in flat(want[n])] + ([size] if n == "attend" else [])
+        blocks = [torch.full((s,), 7, dtype=torch.uint8, device="cuda") for s in sizes]
+        at = {b.data_ptr() for b in blocks}
+        torch.cuda._sleep(200_000_000)
+        copies = [b.clone() for b in blocks]
+        del blocks
+        got = f(side.cuda_stream)
+        assert not at & {t.data_ptr() for t in flat(got)}, n
+        side.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(flat(got), flat(want[n]))), n
+        assert all((c == 7).all() for c in copies), n
+    for n, f in calls.items():
+        got = f(side.cuda_stream)
+        torch.cuda.current_stream().wait_stream(side)
+        torch.cuda._sleep(200_000_000)
+        copies = [t.clone() for t in flat(got)]
+        del got
+        with torch.cuda.stream(side):
+            for t in flat(want[n]):
+                torch.full_like(t, 9.0)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(copies, flat(want[n]))), n
+    with torch.cuda.stream(side):  # the current stream by its number
+        assert torch.equal(su.cache.attend(su.seqs, q, stream=side.cuda_stream), want["attend"])
+    torch.cuda.synchronize()
+
+
 def test_refusals_on_the_device(pk):
     su = Setup(pk, [5], [2], "q8", 2, 64, 16)
     k = randn((2, 2, 64), 1)
