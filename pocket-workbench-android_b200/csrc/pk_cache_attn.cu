@@ -80,7 +80,7 @@ __device__ __forceinline__ void load_q(const AttnKArgs &a, const Unit &u, int ro
   float m = 0.0f;
 #pragma unroll
   for (int j = 0; j < DH / 4; j++) {
-    if (!on) x[j] = 0.0f;
+    x[j] = on ? inf_nan(x[j]) : 0.0f;
     m = fmaxf(m, fabsf(x[j]));
   }
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));

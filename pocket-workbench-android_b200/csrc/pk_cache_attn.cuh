@@ -26,6 +26,10 @@ __device__ __forceinline__ uint32_t rest2(float a, float b, uint32_t hi) {
   return pack2(a - f.x, b - f.y);
 }
 
+// x, and NaN for infinities: a query's infinity would give scores of -inf where
+// all codes that it meets have the other sign, as if nothing were seen.
+__device__ __forceinline__ float inf_nan(float x) { return x + (x - x); }
+
 __device__ __forceinline__ void cp16(uint32_t dst, const void *src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }

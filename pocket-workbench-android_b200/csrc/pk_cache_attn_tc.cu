@@ -256,7 +256,7 @@ __device__ __forceinline__ float put_q(const AttnKArgs &a, const Unit &u, int ro
       load_n<E, 8>(p + 8 * c, a.vec_q, x);
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const float x0 = x[dim8<TYPE>(2 * j)] * down, x1 = x[dim8<TYPE>(2 * j + 1)] * down;
+        const float x0 = inf_nan(x[dim8<TYPE>(2 * j)]) * down, x1 = inf_nan(x[dim8<TYPE>(2 * j + 1)]) * down;
         w[j] = pack2(x0, x1);
         if (terms_of<E> == 2) rest[j] = rest2(x0, x1, w[j]);
       }

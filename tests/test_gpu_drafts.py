@@ -426,6 +426,31 @@ def test_attention_query_range(pk, dh, ty):
         assert ((got.double() - want).abs() <= lim)[ok].all(), scale
 
 
+@pytest.mark.parametrize("ty", list(DT))
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("heads", [4, 64])
+def test_attention_bad_query_rows(pk, dh, ty, heads):
+    """Query rows with an infinity or NaN give NaN wherever they see something, also where all their scores are -inf
+    (codes of one sign, one position); they give 0 where they see nothing, and leave the other rows as they were."""
+    for lens, new in (([0], [2]), ([70], [3])):
+        su = Setup(pk, lens, new, "q8", 1, dh, 16)
+        t = lens[0] + new[0]
+        k = randn((t, 1, dh), 1).abs() + 0.1
+        su.cache.store(pk.KvSeqs(i32([0, t]), i32([0]), su.seqs.pages, t, t, t), k, k)
+        q = randn((new[0], heads, dh), 2).to(DT[ty])
+        clean = su.cache.attend(su.seqs, q)
+        last = new[0] - 1
+        for h, (d, x) in enumerate(((0, -math.inf), (5, math.inf), (dh - 1, math.nan))):
+            q[last, h, d] = x
+        got = su.cache.attend(su.seqs, q)
+        assert torch.isnan(got[last, :3]).all()
+        got[last, :3] = clean[last, :3]
+        assert torch.equal(got, clean)
+        none = su.cache.attend(pk.KvSeqs(su.seqs.start, i32([0]), su.seqs.pages, new[0], new[0], t), q,
+                               mask=torch.zeros((new[0], 1), dtype=torch.int64, device="cuda"))
+        assert (none == 0).all()
+
+
 def tree(n, seed, empty=()):
     """Ancestor bits of a random tree, parents first; rows of `empty` see nothing new."""
     rng = np.random.default_rng(seed)
