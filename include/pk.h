@@ -355,8 +355,8 @@ typedef struct {
  * masked (attention) or zero (pk_kv_load).  start ascends within 0 .. n_tok,
  * the token arrays' rows; rows that no sequence has are neither read nor
  * written.  max_new and max_len are bounds the host knows: of the new tokens
- * of one sequence, and of its committed positions and new tokens together;
- * what is beyond them is left out.  A page that a call writes belongs to one
+ * of one sequence (any number from n_tok on means n_tok), and of its committed
+ * positions and new tokens together; what is beyond them is left out.  A page that a call writes belongs to one
  * sequence of it. */
 typedef struct {
   const int *start, *ctx, *pages;
@@ -385,6 +385,7 @@ int pk_kv_keep(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const int *keep
  * are seen by none.  A row that sees nothing gets 0.
  *   q, out  [n_tok][n_head][head_dim] of one type, strides in elements
  *   mask    device, [n_tok][mask_words], or null
+ * n_tok * n_head and n_seq * n_kv are at most 2^31 - 1.
  * Scores and sums are f32; a softmax weight times its V scale is rounded to
  * f16 as a fraction of the row's largest (to two f16 terms for f32 queries).
  * A query row with infinities or NaN gives NaN, and leaves other rows as they

@@ -759,14 +759,23 @@ Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, const Vari
 
 }  // namespace
 
-size_t kv_attn_scratch_bytes(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type) {
+// max_new is the caller's bound and may be any number; no sequence has more new
+// tokens than there are, which the kernel, the grid and the scratch go by.
+static pk_kv_seqs bounded(pk_kv_seqs s) {
+  s.max_new = std::min(s.max_new, s.n_tok);
+  return s;
+}
+
+size_t kv_attn_scratch_bytes(const pk_kv_cache &c, const pk_kv_seqs &seqs, int n_head, int type) {
+  const pk_kv_seqs s = bounded(seqs);
   const Split p = split_of(c, s, n_head, variant_of(c, s, n_head, type));
   if (p.n_chunk <= 1 || p.cluster) return 0;
   return (size_t)s.n_tok * n_head * p.n_chunk * (c.head_dim + 2) * sizeof(float);
 }
 
-cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_query &q, void *scratch,
+cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &seqs, const pk_kv_query &q, void *scratch,
                            cudaStream_t st) {
+  const pk_kv_seqs s = bounded(seqs);
   const Variant v = variant_of(c, s, q.n_head, q.type);
   const Split p = split_of(c, s, q.n_head, v);
   AttnKArgs a{};

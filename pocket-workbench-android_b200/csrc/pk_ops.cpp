@@ -53,6 +53,10 @@ int check_seqs(const char *who, const pk_kv_seqs *s) {
   if (((uintptr_t)s->start | (uintptr_t)s->ctx | (uintptr_t)s->pages) & 3) return bad(w + ": misaligned sequence array");
   return PK_OK;
 }
+// Query rows, and (sequence, kv head) pairs, that a grid can number.
+bool fits_grid(const pk_kv_cache *c, const pk_kv_seqs *s, int n_head) {
+  return (int64_t)s->n_tok * n_head <= 0x7fffffff && (int64_t)s->n_seq * c->n_kv <= 0x7fffffff;
+}
 bool nothing(const pk_kv_seqs *s) { return s->n_seq == 0 || s->n_tok == 0 || s->max_new == 0 || s->max_len == 0; }
 
 int check_rows(const char *who, const pk_kv_cache *c, const void *k, const void *v, int type, int64_t ts, int64_t hs) {
@@ -105,7 +109,7 @@ int pk_kv_keep(const pk_kv_cache *c, const pk_kv_seqs *s, const int *keep, int k
 
 size_t pk_kv_attn_scratch_bytes(const pk_kv_cache *c, const pk_kv_seqs *s, int n_head, int type) {
   if (check_cache("pk_kv_attn_scratch_bytes", c) || check_seqs("pk_kv_attn_scratch_bytes", s)) return 0;
-  if (nothing(s) || n_head < 1 || n_head % c->n_kv || !is_float_type(type)) return 0;
+  if (nothing(s) || n_head < 1 || n_head % c->n_kv || !is_float_type(type) || !fits_grid(c, s, n_head)) return 0;
   return kv_attn_scratch_bytes(*c, *s, n_head, type);
 }
 
@@ -119,6 +123,7 @@ int pk_kv_attn(const pk_kv_cache *c, const pk_kv_seqs *s, const pk_kv_query *q, 
   if (!(q->scale > 0.0f) || !std::isfinite(q->scale)) return bad("pk_kv_attn: scale must be positive and finite");
   if (q->mask && (q->mask_words < 1 || q->mask_words > 4096)) return bad("pk_kv_attn: mask_words must be 1 to 4096 with a mask");
   if (nothing(s)) return PK_OK;
+  if (!fits_grid(c, s, q->n_head)) return bad("pk_kv_attn: n_tok * n_head and n_seq * n_kv are at most 2^31 - 1");
   if (!q->q || !q->out) return bad("pk_kv_attn: null q or out");
   if (((uintptr_t)q->q | (uintptr_t)q->out) & elem_mask(q->type) || ((uintptr_t)q->mask & 7)) return bad("pk_kv_attn: misaligned q, out or mask");
   const int64_t st[4] = {q->q_tok_stride, q->q_head_stride, q->out_tok_stride, q->out_head_stride};

@@ -89,6 +89,25 @@ def test_attention(pk):
     assert str(need) in pk.last_error()
 
 
+def test_attention_bound_of_new_tokens(pk):
+    """Any max_new past the tokens that there are means the same: the same scratch, and more rows than a grid has are
+    refused."""
+    lib = pk.lib()
+
+    def need(n_head, type_=0, **kw):
+        return lib.pk_kv_attn_scratch_bytes(C.byref(cache(n_kv=1)), C.byref(seqs(max_len=100000, max_pages=4096, **kw)), n_head, type_)
+
+    for type_ in (0, 1, 30):
+        for n_head in (1, 8, 512, 1 << 20):
+            want = need(n_head, type_, max_new=8)
+            for most in (9, 1 << 20, 1 << 30, (1 << 31) - 1):
+                assert need(n_head, type_, max_new=most) == want, (type_, n_head, most)
+    assert need(1 << 20, n_tok=1 << 20, max_new=(1 << 31) - 1) == 0
+    for kw, n_head in (({"n_tok": 1 << 20}, 1 << 20), ({"n_seq": (1 << 31) - 1}, 4)):
+        s, q = seqs(max_new=(1 << 31) - 1, **kw), query(n_head=n_head)
+        assert lib.pk_kv_attn(C.byref(cache()), C.byref(s), C.byref(q), A, 1 << 60, None) == INVALID, kw
+
+
 def test_rope(pk):
     lib = pk.lib()
     out, g = (C.c_double * 64)(), C.c_float()

@@ -574,6 +574,21 @@ def test_attention_bounds_are_kept(pk):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("ty", list(DT))
+def test_attention_wide_bound_of_new_tokens(pk, ty):
+    """A max_new far past the tokens that there are changes nothing."""
+    su = Setup(pk, [900, 3], [2, 1], "q8", 2, 64, 16)
+    su.fill(pk)
+    q = randn((3, 128, 64), 8, DT[ty])
+    for most in (3, 1000, 2 ** 31 - 1):
+        seqs = pk.KvSeqs(su.seqs.start, su.seqs.ctx, su.seqs.pages, 3, most, su.max_len)
+        got = su.cache.attend(seqs, q)
+        check_attention(su, q, got)
+        if most > 3:
+            assert torch.equal(got, last)
+        last = got
+
+
 def test_attention_repeats_bit_for_bit(pk):
     su = Setup(pk, [3000, 1200, 5], [7, 1, 3], "q4", 2, 128, 16)
     su.fill(pk)
