@@ -43,7 +43,9 @@
 // 2^(old - new).
 //
 // Every wait is bounded: one that runs out sets the CTA's abort flag, after
-// which no wait waits, and its rows are written as NaN.
+// which no wait for a buffer waits, and its rows are written as NaN.  The warp
+// that issues the products waits for all of them before it lets go of the
+// tensor memory, flag or not.
 #include <algorithm>
 #include <atomic>
 #include <type_traits>
@@ -308,8 +310,8 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sb = shaddr(smem);
   // barriers: K and scales ready x 4, V ready x 2; the TMEM address, the abort
-  // flag; for each block of 128 rows: S full x 2, P ready x 2, PV done x 2
-  const uint32_t bar = sb + L::BAR, kready = bar, vready = bar + 32, blocks = bar + 64;
+  // flag; all products done; for each block of 128 rows: S full x 2, P ready x 2, PV done x 2
+  const uint32_t bar = sb + L::BAR, kready = bar, vready = bar + 32, done = bar + 56, blocks = bar + 64;
   volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 52);
   const int nblk = BLK == 1 ? 1 : min(BLK, (u.rows - tile0 + 127) / 128);  // that have rows
   auto sfull_of = [&](int blk, int i) { return blocks + 48 * blk + 8 * (i & 1); };
@@ -325,6 +327,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
         mbar_init(pvdone_of(m, i), 1);
       }
     }
+    mbar_init(done, 1);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -385,6 +388,15 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
           commit_one(pvdone_of(m, i));
         }
       }
+      // the operands and the tensor memory are theirs until they are done, also
+      // where a wait ran out and nobody waited for them
+      commit_one(done);
+      const unsigned long long t0 = gtime_ns();
+      while (!mbar_sleep(done, 0))
+        if (gtime_ns() - t0 > WAIT_NS) {
+          *abort = 1;
+          break;
+        }
     }
     __syncwarp();
   } else if (tid >= SOFT) {  // ---------------------------------------- codes
