@@ -303,7 +303,8 @@ int pk_decode_profile(pk_engine *eng, pk_kernel_stat *out, int cap, int *n_out);
  * the readers of one phase wait for a tag nothing writes, so every bounded
  * wait in the kernel runs out.  *status receives the launch's status
  * (PK_ERR_TIMEOUT expected); the engine stays usable and the sequence is
- * unchanged.  PK_ERR_UNSUPPORTED when the persistent kernel is not in use. */
+ * unchanged.  With a quantised K/V cache, one attention launch whose waits run
+ * out.  PK_ERR_UNSUPPORTED when neither kernel is in use. */
 int pk_selftest_bounded_wait(pk_engine *eng, int *status);
 
 /* Records layer-0 intermediates for parity bisection (Engine.dbg). */
@@ -390,7 +391,8 @@ int pk_kv_keep(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const int *keep
  * f16 as a fraction of the row's largest (to two f16 terms for f32 queries).
  * A query row with infinities or NaN gives NaN, and leaves other rows as they
  * are up to rounding.  The kernels' own waits are bounded: one that runs out
- * after 2 s, which a working device never sees, leaves NaN in its rows.
+ * after 2 s, which a working device never sees, leaves NaN in its rows (engine
+ * calls return PK_ERR_TIMEOUT then).
  * scratch: pk_kv_attn_scratch_bytes bytes of device memory, 16-byte aligned
  * (may be null when that is 0), which calls that overlap in time, replays of
  * captured graphs among them, must not share. */

@@ -24,8 +24,12 @@ cudaError_t launch_kv_keep(const pk_kv_cache &c, const pk_kv_seqs &s, const int 
 
 // (0: no partial results)
 size_t kv_attn_scratch_bytes(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type);
+// err: a device word (or null) that PK_ERR_TIMEOUT is put into when a bounded
+// wait runs out; poison: a self-test in which they do.
 cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_query &q, void *scratch,
-                           cudaStream_t st);
+                           cudaStream_t st, int *err = nullptr, bool poison = false);
+// Whether this call's kernel has bounded waits (the tcgen05 one).
+bool kv_attn_waits(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type);
 
 cudaError_t launch_rope(const pk_rope_args &a, cudaStream_t st);
 cudaError_t launch_logit_rules(const void *logits, void *out, int type, int rows, int n, long in_stride,

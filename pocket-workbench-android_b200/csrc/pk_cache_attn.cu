@@ -773,8 +773,12 @@ size_t kv_attn_scratch_bytes(const pk_kv_cache &c, const pk_kv_seqs &seqs, int n
   return (size_t)s.n_tok * n_head * p.n_chunk * (c.head_dim + 2) * sizeof(float);
 }
 
+bool kv_attn_waits(const pk_kv_cache &c, const pk_kv_seqs &seqs, int n_head, int type) {
+  return !variant_of(c, bounded(seqs), n_head, type).k;
+}
+
 cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &seqs, const pk_kv_query &q, void *scratch,
-                           cudaStream_t st) {
+                           cudaStream_t st, int *err, bool poison) {
   const pk_kv_seqs s = bounded(seqs);
   const Variant v = variant_of(c, s, q.n_head, q.type);
   const Split p = split_of(c, s, q.n_head, v);
@@ -789,6 +793,8 @@ cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &seqs, const p
   const size_t rows = (size_t)s.n_tok * q.n_head;
   a.part_o = reinterpret_cast<float *>(scratch);
   a.cluster = p.cluster;
+  a.err = err;
+  a.poison = poison;
   a.part_ml = p.n_chunk > 1 && !a.cluster ? reinterpret_cast<float2 *>(a.part_o + rows * p.n_chunk * c.head_dim) : nullptr;
   const long long blocks = (long long)s.n_seq * c.n_kv * p.row_tiles * p.n_chunk, jb = ((long long)rows + 3) / 4;
   if (blocks > 0x7fffffffLL || (long long)rows > 0x7fffffffLL) return cudaErrorInvalidValue;

@@ -45,6 +45,8 @@ struct AttnKArgs {
   float2 *part_ml; // [n_tok][n_head][n_chunk]
   int chunk, n_chunk, row_tiles, group, page_shift, vec_q, vec_o;
   int cluster;  // 1: a sequence's chunks are a cluster's CTAs, which add up among themselves
+  int *err;     // null, or a device word that PK_ERR_TIMEOUT goes to when a bounded wait ran out
+  int poison;   // 1 (self-test): the codes never arrive, so that the waits run out
 };
 
 // A CTA's work: one chunk of positions [lo, hi) for one tile of the rows (token

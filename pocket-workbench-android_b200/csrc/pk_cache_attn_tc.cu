@@ -479,8 +479,9 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
         if (lane == 0) reinterpret_cast<uint32_t *>(sc + 2 * NK * 4 + 8)[key >> 5] = x;
       }
     };
-    if (nt > 0) ask(0);
-    for (int i = 0; i < nt; i++) {
+    const int n = a.poison ? 0 : nt;
+    if (n > 0) ask(0);
+    for (int i = 0; i < n; i++) {
       // K's buffer is free once tile i - 2's scores are there, V's once its
       // products with V are
       if (i >= 2)
@@ -489,7 +490,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
       if (!is_v) put_scales(i);
       fence_async_smem();
       mbar_arrive(is_v ? vready + 8 * (i & 1) : kready + 8 * (i & 3));
-      if (i + 1 < nt) ask(i + 1);
+      if (i + 1 < n) ask(i + 1);
     }
   } else {  // ------------------------------------------------------------ softmax
     set_regs<true, L::REGS_SOFT>();
@@ -800,6 +801,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
   // back: taken earlier (by warps without a tile) they would be missing there.
   if (warp >= WS && (BLK > 1 || warp < WS + 8)) set_regs<true, L::REGS>();
   if (cluster) join_cluster<DH>(a, u, tile0, ROWS, sb, sb + L::ML, THREADS);
+  if (tid == 0 && a.err && *abort) atomicCAS(a.err, 0, PK_ERR_TIMEOUT);
   if (warp == WS + 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(BLK * L::COLS) : "memory");

@@ -418,6 +418,10 @@ int Engine::setup_qcache() {
     s.n_seq = b; s.max_new = 1;
     q_scratch_bytes_ = std::max(q_scratch_bytes_, kv_attn_scratch_bytes(kc, s, c.n_head, PK_TYPE_F32));
   }
+  if (!(q_err_ = mv_tc_error_word())) return set_error(PK_ERR_CUDA, "no error word of the tensor-core kernels");
+  pk_kv_seqs one{};
+  one.n_seq = one.n_tok = one.max_new = 1;
+  q_waits1_ = kv_attn_waits(kc, one, c.n_head, PK_TYPE_F32);
   std::vector<int> ids((size_t)std::max(np * max_batch_, 65)), start;
   for (size_t i = 0; i < ids.size(); i++) ids[i] = (int)i;
   for (int b = 0; b <= max_batch_; b++) {
@@ -476,7 +480,7 @@ int Engine::q_attend(const QPool &p, const pk_kv_seqs &s, int l, float *q, float
   pk_kv_query qa{};
   qa.q = q; qa.out = out; qa.q_tok_stride = qa.out_tok_stride = qdim; qa.q_head_stride = qa.out_head_stride = dh;
   qa.type = PK_TYPE_F32; qa.n_head = c.n_head; qa.scale = 1.0f / sqrtf((float)dh);
-  PROF("k_kv_attn", 2.0 * c.n_head_kv * kv_pos * row + 8.0 * n * qdim, launch_kv_attn(cache, s, qa, q_scratch_[li], st));
+  PROF("k_kv_attn", 2.0 * c.n_head_kv * kv_pos * row + 8.0 * n * qdim, launch_kv_attn(cache, s, qa, q_scratch_[li], st, q_err_));
   return PK_OK;
 }
 
@@ -603,12 +607,13 @@ int Engine::setup_decode() {
 // error code.  The finish counter is reset and the tag epoch advanced (the
 // stopped launch did not advance it), so words that launch left behind can
 // never match the next launch's tags.
-// After b > 1 work: the tensor-core matvec's error word (a bounded wait in
-// one of its CTAs ran out), read and cleared.
+// After b > 1 work, streams and quantised caches: the error word of the
+// tensor-core matvecs and attention (a bounded wait in one of their CTAs ran
+// out), read and cleared.
 int Engine::check_tc_error() {
   const int t = mv_tc_error(true);
-  if (t == PK_ERR_TIMEOUT) return set_error(PK_ERR_TIMEOUT, "a tensor-core matvec's bounded wait ran out");
-  if (t) return set_error(t, "reading the tensor-core matvec's error word");
+  if (t == PK_ERR_TIMEOUT) return set_error(PK_ERR_TIMEOUT, "a bounded wait of a tensor-core matvec or attention ran out");
+  if (t) return set_error(t, "reading the tensor-core kernels' error word");
   return PK_OK;
 }
 
@@ -857,7 +862,7 @@ int Engine::forward_inner(const uint32_t *ids, const int *pos, int b, bool want_
     const int rc = check_decode_error();
     if (rc) return rc;
   }
-  if (b > 1) {
+  if (b > 1 || q_waits1_) {
     const int rc = check_tc_error();
     if (rc) return rc;
   }
@@ -1097,6 +1102,7 @@ int Engine::decode_steps_device(int n_steps, uint32_t *out_ids, float *device_ms
   cudaEventDestroy(e1);
   if (e != cudaSuccess) return cuda_error(e, "decode_steps_device");
   rc = check_decode_error();
+  if (!rc && q_waits1_) rc = check_tc_error();
   if (rc) return rc;
   if (device_ms) *device_ms = ms;
   if (out_ids) std::memcpy(out_ids, hist.data(), (size_t)n_steps * 4);
@@ -1215,6 +1221,7 @@ int Engine::stream_prefill(int s, const uint32_t *prompt, int n) {
     rc = e != cudaSuccess ? cuda_error(e, "stream prefill ids") : enqueue_forward(n, true, false);
     const cudaError_t es = cudaStreamSynchronize(st_);
     if (!rc && es != cudaSuccess) rc = cuda_error(es, "stream prefill");
+    if (!rc) rc = check_tc_error();
   }
   uint32_t tok = 0;
   if (!rc) rc = argmax(&tok);
@@ -1334,6 +1341,7 @@ int Engine::streams_decode(int n_steps, uint32_t *out_ids, float *device_ms) {
   cudaEventDestroy(e1);
   if (e != cudaSuccess) return cuda_error(e, "streams decode");
   if (es != cudaSuccess) return cuda_error(es, "streams decode");
+  if (const int rc = check_tc_error()) return rc;
   for (int s = 0; s < S; s++) {
     const uint32_t *hs = hist.data() + (size_t)s * n_ctx_;
     if (out_ids) {
@@ -1365,9 +1373,27 @@ int Engine::streams_set_position(int pos) {
 // that no phase writes: every CTA's bounded wait runs out, the launch stops
 // with PK_ERR_TIMEOUT in the error word and returns, and the engine recovers
 // (the error path resets the counters and advances the tag epoch).  The
-// launch does not feed a token back, so the sequence is unchanged.
+// launch does not feed a token back, so the sequence is unchanged.  With a
+// quantised cache: one launch of a largest batch's attention, whose codes
+// never arrive, if that is the kernel with bounded waits.
 int Engine::selftest_bounded_wait(int *status) {
   if (!loaded_) return set_error(PK_ERR_INVALID, "no model loaded");
+  if (kv_q_) {
+    const int dh = cfg_.head_dim, qdim = cfg_.n_head * dh;
+    pk_kv_seqs s{};
+    s.start = d_qstart_ + 2 * max_batch_; s.ctx = d_qstart_; s.pages = qcur_.pages;  // ctx 0
+    s.n_seq = 1; s.max_pages = (n_ctx_ + QPAGE - 1) / QPAGE; s.n_tok = s.max_new = max_batch_; s.max_len = n_ctx_;
+    pk_kv_query q{};
+    q.q = q_; q.out = attn_; q.q_tok_stride = q.out_tok_stride = qdim; q.q_head_stride = q.out_head_stride = dh;
+    q.type = PK_TYPE_F32; q.n_head = cfg_.n_head; q.scale = 1.0f;
+    if (!kv_attn_waits(qlayer(qcur_, 0), s, cfg_.n_head, PK_TYPE_F32))
+      return set_error(PK_ERR_UNSUPPORTED, "no bounded waits in the attention over this cache");
+    PK_CK(cudaSetDevice(device_));
+    PK_CK(launch_kv_attn(qlayer(qcur_, 0), s, q, q_scratch_[0], st_, q_err_, true));
+    PK_CK(cudaStreamSynchronize(st_));
+    *status = check_tc_error();
+    return PK_OK;
+  }
   if (!use_decode_) return set_error(PK_ERR_UNSUPPORTED, "the persistent decode kernel is not in use");
   if (next_pos_ + 1 > n_ctx_) return set_error(PK_ERR_CONTEXT_FULL, "context full");
   h_pos_[0] = next_pos_;

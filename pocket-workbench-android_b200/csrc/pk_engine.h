@@ -167,6 +167,8 @@ class Engine {
   float qgain_ = 1.0f;
   uint8_t *q_scratch_[NLANES] = {};
   size_t q_scratch_bytes_ = 0;
+  int *q_err_ = nullptr;     // device: the tensor-core kernels' error word
+  bool q_waits1_ = false;    // one token's attention has bounded waits
   size_t qpool_half(int n_pages) const;
   int setup_qcache();
   QPool qstream(int s) const;

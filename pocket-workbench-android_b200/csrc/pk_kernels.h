@@ -74,6 +74,9 @@ cudaError_t launch_mv_multi(int n, const MvOut *outs, const Q8Dev &act, cudaStre
 bool mv_tc_supports(const DevTensor &w, const Q8Dev &act);
 cudaError_t launch_mv_tc(int n, const MvOut *outs, const Q8Dev &act, cudaStream_t st);
 int mv_tc_error(bool clear);
+// The word itself on the current device (null: an error), for other kernels
+// with bounded waits.
+int *mv_tc_error_word();
 // Selects the b > 8 matvec kernel: 0 mma.sync tiles, 1 tcgen05.
 void set_mv_path(int path);
 

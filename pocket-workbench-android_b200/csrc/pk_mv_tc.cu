@@ -694,6 +694,11 @@ cudaError_t launch_mv_tc(int n, const MvOut *outs, const Q8Dev &act, cudaStream_
   return cudaLaunchKernelEx(&cfg, k_mv_tc, ss, act);
 }
 
+int *mv_tc_error_word() {
+  void *p = nullptr;
+  return cudaGetSymbolAddress(&p, g_tc_err) == cudaSuccess ? static_cast<int *>(p) : nullptr;
+}
+
 int mv_tc_error(bool clear) {
   int v = 0;
   if (cudaMemcpyFromSymbol(&v, g_tc_err, sizeof(int)) != cudaSuccess) return PK_ERR_CUDA;

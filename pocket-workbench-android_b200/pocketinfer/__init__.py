@@ -444,8 +444,8 @@ class Engine:
                 for s in stats[: n.value]]
 
     def selftest_bounded_wait(self) -> int:
-        """One persistent-kernel launch whose bounded waits are made to run out;
-        returns the status that launch produced (PK_ERR_TIMEOUT = 8 expected)."""
+        """One launch of the persistent kernel (of the attention over a quantised
+        cache) whose bounded waits are made to run out; returns the status that launch produced (PK_ERR_TIMEOUT = 8 expected)."""
         st = C.c_int()
         _check(lib().pk_selftest_bounded_wait(self.h, C.byref(st)))
         return st.value

@@ -204,3 +204,20 @@ def test_refusals(pk, paths):
     assert pk.lib().pk_set_kv_type(e.h, pk.KV_Q8) != 0
     with pytest.raises(KeyError):
         pk.Engine(paths["tiny"], n_ctx=128, kv="q5")
+
+
+def test_a_wait_that_runs_out_is_an_error(pk, paths):
+    """An attention launch whose codes never arrive ends after its bounded waits, the engine reports it, and goes on as
+    one that has not seen it."""
+    spec = synth.SMALL_Q40
+    ids = synth.prompt_ids(31, 40, spec.n_vocab)
+    ref, e = (pk.Engine(paths["q40"], n_ctx=128, kv="q8") for _ in range(2))
+    want = ref.generate(ids, 8, stop_at_eog=False)["gen_ids"]
+    assert e.generate(ids, 8, stop_at_eog=False)["gen_ids"] == want
+    assert e.selftest_bounded_wait() == 8  # PK_ERR_TIMEOUT
+    e.forward(ids[:32], list(range(32)))
+    ref.forward(ids[:32], list(range(32)))
+    assert np.array_equal(e.logits().view(np.uint32), ref.logits().view(np.uint32))
+    assert e.generate(ids, 8, stop_at_eog=False)["gen_ids"] == want
+    with pytest.raises(pk.PkError):  # (no attention with waits at head_dim 128 in f32)
+        pk.Engine(paths["dh128"], n_ctx=128, kv="q8").selftest_bounded_wait()
