@@ -131,6 +131,15 @@ def _i32(t, device, name, dims):
         _bad(f"{name} must be a contiguous int32 tensor of {dims} dimension(s) on device {device}")
 
 
+def _mask(t, rows, device):
+    """(words a row, address).  No words at all have no address, which would mean causal."""
+    if t.dtype != torch.int64 or t.dim() != 2 or t.shape[0] != rows or not t.is_contiguous() or t.get_device() != device:
+        _bad("attend: mask must be a contiguous int64 tensor [n_tok, words] on the cache's device")
+    if t.shape[1] < 1:
+        _bad("attend: a mask has one word a token or more")
+    return t.shape[1], t.data_ptr()
+
+
 def _like(x):
     return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
@@ -227,11 +236,7 @@ class KvCache:
             _bad("attend: q must be [n_tok, n_head, head_dim] with contiguous heads")
         if q.get_device() != dev or seqs.device != dev:
             _bad("attend: q and the sequences must be on the cache's device")
-        words = bits = 0
-        if mask is not None:
-            if mask.dtype != torch.int64 or mask.dim() != 2 or mask.shape[0] != shape[0] or not mask.is_contiguous() or mask.get_device() != dev:
-                _bad("attend: mask must be a contiguous int64 tensor [n_tok, words] on the cache's device")
-            words, bits = mask.shape[1], mask.data_ptr()
+        words, bits = (0, 0) if mask is None else _mask(mask, shape[0], dev)
         if out is None:
             out = _like(q) if stream is None else _new(lambda: _like(q), dev, stream)
         elif out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or out.stride(2) != 1:

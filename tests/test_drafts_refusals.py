@@ -169,6 +169,18 @@ def test_binding_refuses_host_tensors(pk):
             bad()
 
 
+def test_mask_without_words(pk):
+    """A mask of no words is refused: its tensor has no address, and no address means causal."""
+    torch = pytest.importorskip("torch")
+    with pytest.raises(pk.PkError):  # (sets the binding up)
+        pk.logit_rules(torch.zeros(2, 8))
+    m = lambda *s: torch.zeros(s, dtype=torch.int64)  # noqa: E731
+    assert D._mask(m(3, 1), 3, -1)[0] == 1 and D._mask(m(3, 70), 3, -1)[0] == 70
+    for bad in (m(3, 0), m(2, 1), m(3), m(3, 2)[:, :1], m(3, 1).int(), m(0, 0)):
+        with pytest.raises(pk.PkError):
+            D._mask(bad, 3, -1)
+
+
 def test_packed_structures_match_the_header():
     """The packed bytes have the fields where the ctypes structures (the C layouts) have them."""
     q = D.PACK_QUERY(1, 2, 3, 4, 5, 6, 7, 8, 9, 10, 0.5)
