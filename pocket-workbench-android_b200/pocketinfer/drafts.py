@@ -150,6 +150,9 @@ class KvSeqs:
 
     def __init__(self, start, ctx, pages, n_tok: int, max_new: int, max_len: int):
         _init()
+        for x, name in ((n_tok, "n_tok"), (max_new, "max_new"), (max_len, "max_len")):
+            if not 0 <= x <= 0x7FFFFFFF:  # (the structure's field would hold another number, 0 for 2^32)
+                _bad(f"{name} {x} is not within 0 .. 2^31 - 1")
         device, n = start.get_device(), ctx.numel()
         for t, name, dims in ((start, "start", 1), (ctx, "ctx", 1), (pages, "pages", 2)):
             _i32(t, device, name, dims)

@@ -169,6 +169,14 @@ def test_binding_refuses_host_tensors(pk):
             bad()
 
 
+@pytest.mark.parametrize("bounds", [(2 ** 32, 4, 100), (8, 2 ** 32, 100), (8, 4, 2 ** 32), (8, 4, 2 ** 31), (-1, 4, 100), (8, -4, 100), (8, 4, -2 ** 32)])
+def test_bounds_that_the_structure_cannot_hold(pk, bounds):
+    torch = pytest.importorskip("torch")
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    with pytest.raises(pk.PkError, match="not within"):
+        pk.KvSeqs(i(3), i(2), i(2, 4), *bounds)
+
+
 def test_mask_without_words(pk):
     """A mask of no words is refused: its tensor has no address, and no address means causal."""
     torch = pytest.importorskip("torch")
