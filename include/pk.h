@@ -357,7 +357,8 @@ typedef struct {
  * the token arrays' rows; rows that no sequence has are neither read nor
  * written.  max_new and max_len are bounds the host knows: of the new tokens
  * of one sequence (any number from n_tok on means n_tok), and of its committed
- * positions and new tokens together; what is beyond them is left out.  A page that a call writes belongs to one
+ * positions and new tokens together; what is beyond them is left out (all of
+ * a sequence with a negative ctx).  A page that a call writes belongs to one
  * sequence of it. */
 typedef struct {
   const int *start, *ctx, *pages;

@@ -72,9 +72,10 @@ __device__ __forceinline__ uint32_t nibbles_of(uint32_t w, uint32_t s, uint32_t 
 __device__ __forceinline__ uint32_t dup_h(int s) { return h2u(__half2half2(__int2half_rn(s))); }
 
 // One sequence's bounds, made safe whatever the device arrays hold: rows
-// [first, first + n) of the token arrays, n <= max_new, and committed
-// positions ctx >= 0; total = positions in reach, at most max_len and what
-// the page table addresses.
+// [first, first + n) of the token arrays, n <= max_new; total = positions in
+// reach, at most max_len and what the page table addresses (none for a
+// negative ctx); committed positions ctx, at most as many (what is past them
+// is out of reach anyway, and sums with a larger one could wrap).
 struct SeqView {
   int first, n, ctx, total;
 };
@@ -83,8 +84,8 @@ __device__ __forceinline__ SeqView seq_view(const pk_kv_seqs &q, int page_size, 
   const int a = __ldg(q.start + s), b = __ldg(q.start + s + 1), c = __ldg(q.ctx + s);
   v.first = min(max(a, 0), q.n_tok);
   v.n = min(max(min(b, q.n_tok) - v.first, 0), q.max_new);
-  v.ctx = c;
   const long long cap = min((long long)q.max_pages * page_size, (long long)q.max_len);
+  v.ctx = (int)min((long long)c, cap);
   v.total = c < 0 ? 0 : (int)min((long long)c + v.n, cap);
   return v;
 }

@@ -574,6 +574,66 @@ def test_attention_bounds_are_kept(pk):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("ty,heads", [("f32", 2), ("f32", 64), ("f16", 2), ("bf16", 64)])
+@pytest.mark.parametrize("start,ctx", [([-3, 6], 100), ([0, 900], 100), ([5, 2], 100), ([2, 4], 100), ([7, 9], 100), ([0, 6], -7), ([0, 6], 103),
+                                       ([0, 6], 106), ([0, 6], 110), ([0, 6], 2 ** 31 - 1), ([0, 6], -2 ** 31)])
+def test_arrays_that_contradict_the_bounds(pk, start, ctx, ty, heads):
+    """start and ctx outside the host's bounds mean what is left of them within: every row, slot and page of the calls'
+    outputs against that, and everything around them (more pages, rows and elements) as it was."""
+    dh, n_tok, max_len, page = 64, 6, 106, 16
+    a, b = (min(max(x, 0), n_tok) for x in start)
+    n, total = max(b - a, 0), 0 if ctx < 0 else min(ctx + max(b - a, 0), max_len)
+    pool = [torch.full((11, 2, page, w), 77, dtype=t, device="cuda") for w, t in ((dh, torch.uint8), (dh, torch.uint8), (1, torch.float32), (1, torch.float32))]
+    cache = pk.KvCache(*(t[2:9] for t in pool), "q8", dh)
+    table = i32([[4, 0, 6, 1, 3, 2, 5]])
+    cache.store(pk.KvSeqs(i32([0, max_len]), i32([0]), table, max_len, max_len, max_len), randn((max_len, 2, dh), 1), randn((max_len, 2, dh), 2))
+    seqs = pk.KvSeqs(i32(start), i32([ctx]), table, n_tok, n_tok, max_len)
+    k, v = randn((n_tok, 2, dh), 3, DT[ty]), randn((n_tok, 2, dh), 4, DT[ty])
+    want = [t.clone() for t in pool]
+    codes = pk.KvCache.empty(1, page, 2, dh)
+    codes.store(pk.KvSeqs(i32([0, n_tok]), i32([0]), i32([[0]]), n_tok, n_tok, n_tok), k, v)
+    for i in range(n):
+        p = ctx + i
+        if 0 <= ctx and p < total:
+            for w, c in zip(want, (codes.k, codes.v, codes.ks, codes.vs)):
+                w[2 + int(table[0, p // page]), :, p % page] = c[0, :, a + i]
+    cache.store(seqs, k, v)
+    same = lambda x, y: torch.equal(x.view(torch.uint8), y.view(torch.uint8))  # noqa: E731
+    assert all(same(x, w) for x, w in zip(pool, want))
+
+    k64, v64 = decoded(cache)
+    at = torch.arange(total, device="cuda")
+    k64, v64 = (x[table[0, at // page].long(), :, at % page] for x in (k64, v64))  # [total, 2, dh]
+    big = torch.full((2, n_tok + 4, 2, dh), 5.0, dtype=DT[ty], device="cuda")
+    cache.load(seqs, out=(big[0, 2:-2], big[1, 2:-2]))
+    for x, y in ((big[0], k64), (big[1], v64)):
+        for i in range(n):
+            got = x[2 + a + i].double()
+            assert torch.equal(got, y[ctx + i].float().to(DT[ty]).double()) if 0 <= ctx and ctx + i < total else (got == 0).all()
+        assert (x[:2 + a] == 5).all() and (x[2 + a + n:] == 5).all()
+
+    q = randn((n_tok, heads, dh), 5, DT[ty])
+    out = torch.full((n_tok + 4, heads, dh), 5.0, dtype=DT[ty], device="cuda")
+    cache.attend(seqs, q, out=out[2:-2])
+    assert (out[:2 + a] == 5).all() and (out[2 + a + n:] == 5).all()
+    for i in range(n):
+        see = (at < ctx) | (at - ctx <= i)
+        for h in range(heads):
+            x, kk, vv = q[a + i, h].double(), k64[:, h * 2 // heads], v64[:, h * 2 // heads]
+            p = torch.softmax((kk @ x * dh ** -0.5).masked_fill(~see, -math.inf), 0)
+            y, absv = (p @ vv, p @ vv.abs()) if total else (torch.zeros(dh, dtype=torch.float64, device="cuda"),) * 2
+            dots = (kk.abs() @ x.abs() * dh ** -0.5).amax() if total else torch.tensor(0.0, device="cuda")
+            assert ((out[2 + a + i, h].double() - y).abs() <= attn_bound(q, y, absv, dots.double()[None], dh)).all()
+    keep = i32([[3, 2, 5]])
+    moved = [t.clone() for t in pool]
+    for j, x in enumerate((3, 2, 5)):
+        if 0 <= ctx and x < n and ctx + x < total:
+            for w, t in zip(moved, pool):
+                w[2 + int(table[0, (ctx + j) // page]), :, (ctx + j) % page] = t[2 + int(table[0, (ctx + x) // page]), :, (ctx + x) % page]
+    cache.keep(seqs, keep, i32([3]))
+    assert all(same(x, w) for x, w in zip(pool, moved))
+
+
 @pytest.mark.parametrize("ty", list(DT))
 def test_attention_wide_bound_of_new_tokens(pk, ty):
     """A max_new far past the tokens that there are changes nothing."""
