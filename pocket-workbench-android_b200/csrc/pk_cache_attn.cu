@@ -90,7 +90,7 @@ __device__ __forceinline__ void load_q(const AttnKArgs &a, const Unit &u, int ro
   const float up = __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
 #pragma unroll
   for (int j = 0; j < DH / 4; j++) x[j] *= down;
-  rs = a.q.scale * kLog2e * up;
+  rs = fmaxf(a.q.scale * kLog2e * up, 0x1p-149f);  // (not 0, times which a masked -inf would be NaN)
 }
 template <int DH>
 __device__ __forceinline__ void load_q_any(const AttnKArgs &a, const Unit &u, int row, int t, float (&x)[DH / 4], float &rs) {

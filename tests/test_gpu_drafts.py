@@ -451,6 +451,16 @@ def test_attention_bad_query_rows(pk, dh, ty, heads):
         assert (none == 0).all()
 
 
+@pytest.mark.parametrize("ty,heads", [("f32", 2), ("f32", 64), ("bf16", 2), ("bf16", 64), ("f16", 2)])
+def test_attention_scores_below_f32(pk, ty, heads):
+    """Scale and query so small that their product has no f32 value: all that is seen counts alike, the rest not at all."""
+    su = Setup(pk, [20], [3], "q8", 1, 64, 16)
+    su.fill(pk)
+    q = (randn((3, heads, 64), 1) * (1e-7 if ty == "f16" else 1e-32)).to(DT[ty])
+    for scale in (1e-20, 1e-38):
+        check_attention(su, q, su.cache.attend(su.seqs, q, scale=scale), scale=scale)
+
+
 def tree(n, seed, empty=()):
     """Ancestor bits of a random tree, parents first; rows of `empty` see nothing new."""
     rng = np.random.default_rng(seed)
