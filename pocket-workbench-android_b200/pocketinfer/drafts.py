@@ -140,6 +140,11 @@ def _mask(t, rows, device):
     return t.shape[1], t.data_ptr()
 
 
+def _same_strides(k, v):
+    """Of tensors of one shape; what steps a dimension of size 1 has means nothing."""
+    return k.stride() == v.stride() or all(a == b or n == 1 for a, b, n in zip(k.stride(), v.stride(), k.shape))
+
+
 def _like(x):
     return torch.empty_like(x) if x.is_contiguous() else torch.empty(x.shape, dtype=x.dtype, device=x.device)
 
@@ -204,12 +209,13 @@ class KvCache:
             _bad(f"{who}: the sequences are on another device")
         if k.shape != shape or v.shape != shape:
             _bad(f"{who}: k and v must be {shape}")
-        if k.dtype != v.dtype or k.get_device() != self.device or v.get_device() != self.device or v.stride() != st or st[2] != 1:
+        if k.dtype != v.dtype or k.get_device() != self.device or v.get_device() != self.device or not _same_strides(k, v) or st[2] != 1:
             _bad(f"{who}: k and v must be on the cache's device and share type and strides, with contiguous heads")
         return _dtype(k, who), st[0], st[1]
 
     def store(self, seqs: KvSeqs, k, v, stream=None):
-        """Quantises rows k, v [n_tok, n_kv, head_dim] of the new tokens into the cache."""
+        """Quantises rows k, v [n_tok, n_kv, head_dim] of the new tokens into the cache.  k and v have the same strides:
+        those of one fused projection do, also after rope() in place (out_q, out_k)."""
         _call(_L.pk_kv_store, self.device, stream, self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "store"))
 
     def load(self, seqs: KvSeqs, dtype=None, out=None, stream=None):

@@ -177,6 +177,16 @@ def test_bounds_that_the_structure_cannot_hold(pk, bounds):
         pk.KvSeqs(i(3), i(2), i(2, 4), *bounds)
 
 
+def test_strides_of_single_rows(pk):
+    """K and V of one token or one head are alike whatever the strides of those dimensions."""
+    torch = pytest.importorskip("torch")
+    f = torch.zeros((4, 6, 64))
+    for k, v, ok in ((f[:1, :2], torch.zeros(1, 2, 64), True), (f[:, :1], f[:, 5:], True), (f[:1, :1], torch.zeros(1, 1, 64), True),
+                     (f[:, :2], f[:, 4:], True), (f[:, :2], torch.zeros(4, 2, 64), False), (f[:, :1], torch.zeros(4, 1, 64), False),
+                     (f[:1, :2], torch.zeros(1, 64, 2).transpose(1, 2), False)):
+        assert D._same_strides(k, v) == ok, (k.stride(), v.stride())
+
+
 def test_mask_without_words(pk):
     """A mask of no words is refused: its tensor has no address, and no address means causal."""
     torch = pytest.importorskip("torch")

@@ -241,6 +241,18 @@ def test_store_leaves_the_rest(pk, kind):
     assert torch.equal(ko[:4], k64[table[0, 0], :, 10:14].float().transpose(0, 1))
 
 
+def test_store_and_load_single_rows(pk):
+    """One token or one head: K and V of different strides in that dimension."""
+    for n_tok, n_kv in ((1, 3), (5, 1), (1, 1)):
+        su = Setup(pk, [7], [n_tok], "q8", n_kv, 64, 16)
+        k = randn((n_tok, n_kv, 64), 1)
+        v = randn((n_tok, n_kv + 2, 64), 2)[:, 1:1 + n_kv] if n_tok == 1 else randn((n_tok, n_kv, 64), 2)[:, ::2]
+        su.cache.store(su.seqs, k, v)
+        out = torch.zeros_like(k), torch.zeros((n_tok, n_kv + 3, 64), device="cuda")[:, :n_kv] if n_tok == 1 else torch.zeros_like(v)
+        su.cache.load(su.seqs, out=out)
+        assert torch.equal(out[0], stored(k, "q8")) and torch.equal(out[1], stored(v, "q8"))
+
+
 @pytest.mark.parametrize("kind", ["q8", "q4"])
 @pytest.mark.parametrize("dh", [64, 128])
 def test_keep_moves_the_accepted_path(pk, kind, dh):
