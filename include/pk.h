@@ -390,6 +390,9 @@ int pk_kv_keep(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const int *keep
  * n_tok * n_head and n_seq * n_kv are at most 2^31 - 1.
  * Scores and sums are f32; a softmax weight times its V scale is rounded to
  * f16 as a fraction of the row's largest (to two f16 terms for f32 queries).
+ * Half-precision queries' outputs are summed in the tensor core, which does
+ * not round but cuts off, over so few positions at a time that it stays under
+ * an eighth of the output's rounding.
  * A query row with infinities or NaN gives NaN, and leaves other rows as they
  * are up to rounding.  The kernels' own waits are bounded: one that runs out
  * after 2 s, which a working device never sees, leaves NaN in its rows (engine

@@ -728,25 +728,35 @@ Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int ty
 // it takes alone (64 tokens at 8000 positions, 64 heads over 8: 4 chunks, one
 // CTA an SM, 53 us, 8 chunks 66, one 127, 37 100; 32 sequences of 2000: one
 // chunk 61, two 79, four 100; the wide trees 770, 799 and 750).
+//
+// Half-precision queries' outputs are summed by the tensor core, which cuts off
+// what it shifts out: less than 2^-23 of the sum each step of 16 positions, all
+// to one side where V's values have one sign (measured: 2^-27.1 of it a position
+// on tcgen05, a quarter on mma.sync, whose four groups of warps have sums of
+// their own).  A chunk's length keeps that under an eighth of the output's
+// rounding, 2^-14 for f16 and 2^-11 for bf16; chunks are added in f32.
+constexpr long long SUM_F16 = 8192, SUM_BF16 = 65536;  // positions of one such sum
 struct Split {
   int chunk, n_chunk, row_tiles;
   bool cluster;
 };
-Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, const Variant &v) {
+Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type, const Variant &v) {
   Split p;
   const long long rows = (long long)s.max_new * (n_head / c.n_kv);
   p.row_tiles = (int)((rows + v.rows - 1) / v.rows);
   const long long units = (long long)s.n_seq * c.n_kv * p.row_tiles, want = 148 * 8;
   const long long most = (s.max_len + MIN_CHUNK - 1) / MIN_CHUNK;
-  long long n = std::max<long long>(1, std::min(most, want / units));
+  const long long sum = (type == T_F16 ? SUM_F16 : SUM_BF16) * (v.k ? 4 : 1);
+  const long long least = type == T_F32 ? 1 : (s.max_len + sum - 1) / sum;
+  long long n = std::max(least, std::min(most, want / units));
   if (!v.k) {
     long long best = 0;
     const long long top = n;
-    for (long long c = 1; c <= top; c++) {
+    for (long long c = least; c <= top; c++) {
       const long long ctas = units * c, left = ctas % 296, tiles = ((s.max_len + 63) / 64 + c - 1) / c;
       const long long t = v.rows == 256 ? (ctas + 147) / 148 * (tiles + 8)
                                         : (ctas / 296 * 8 + (left == 0 ? 0 : left <= 148 ? 5 : 8)) * (tiles + 16);
-      if (c == 1 || t < best) best = t, n = c;
+      if (c == least || t < best) best = t, n = c;
     }
   }
   const long long slots = v.rows == 256 ? 128 : 296;  // CTAs that run at once, in clusters too
@@ -759,29 +769,31 @@ Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, const Vari
 
 }  // namespace
 
-// max_new is the caller's bound and may be any number; no sequence has more new
-// tokens than there are, which the kernel, the grid and the scratch go by.
-static pk_kv_seqs bounded(pk_kv_seqs s) {
+// max_new and max_len are the caller's bounds and may be any numbers; no
+// sequence has more new tokens than there are, or more positions than its pages
+// hold, which the kernel, the grid and the scratch go by.
+static pk_kv_seqs bounded(const pk_kv_cache &c, pk_kv_seqs s) {
   s.max_new = std::min(s.max_new, s.n_tok);
+  s.max_len = (int)std::min<long long>(s.max_len, (long long)s.max_pages * c.page_size);
   return s;
 }
 
 size_t kv_attn_scratch_bytes(const pk_kv_cache &c, const pk_kv_seqs &seqs, int n_head, int type) {
-  const pk_kv_seqs s = bounded(seqs);
-  const Split p = split_of(c, s, n_head, variant_of(c, s, n_head, type));
+  const pk_kv_seqs s = bounded(c, seqs);
+  const Split p = split_of(c, s, n_head, type, variant_of(c, s, n_head, type));
   if (p.n_chunk <= 1 || p.cluster) return 0;
   return (size_t)s.n_tok * n_head * p.n_chunk * (c.head_dim + 2) * sizeof(float);
 }
 
 bool kv_attn_waits(const pk_kv_cache &c, const pk_kv_seqs &seqs, int n_head, int type) {
-  return !variant_of(c, bounded(seqs), n_head, type).k;
+  return !variant_of(c, bounded(c, seqs), n_head, type).k;
 }
 
 cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &seqs, const pk_kv_query &q, void *scratch,
                            cudaStream_t st, int *err, bool poison) {
-  const pk_kv_seqs s = bounded(seqs);
+  const pk_kv_seqs s = bounded(c, seqs);
   const Variant v = variant_of(c, s, q.n_head, q.type);
-  const Split p = split_of(c, s, q.n_head, v);
+  const Split p = split_of(c, s, q.n_head, q.type, v);
   AttnKArgs a{};
   a.c = c; a.s = s; a.q = q;
   a.chunk = p.chunk; a.n_chunk = p.n_chunk; a.row_tiles = p.row_tiles;

@@ -671,6 +671,29 @@ def test_attention_wide_bound_of_new_tokens(pk, ty):
         last = got
 
 
+@pytest.mark.parametrize("ty,total", [("f16", 131072), ("bf16", 262144), ("f32", 131072)])
+@pytest.mark.parametrize("heads", [1, 40])
+def test_attention_sums_of_long_histories(pk, ty, total, heads):
+    """V of one sign over long histories, so many sequences that each would be one sum: what the sums drop must not show.
+    Single errors are as large as the weights' and outputs' roundings, their mean over 16 rows of 64 is not: a rounding
+    within half a step u has a standard deviation of u / sqrt(3), the mean of 1024 a 32nd of it, and 5 of those pass by
+    chance once in a million runs; an eighth of u is what the sums may drop.  f32: total / 16 additions, each within half a
+    step of the sum, 5 standard deviations likewise."""
+    dh, page, n = 64, 4096, 640
+    cache = pk.KvCache.empty(total // page, page, 1, dh)
+    pages = torch.arange(total // page, dtype=torch.int32, device="cuda")[None]
+    v = randn((total, 1, dh), 2).abs() + 0.25
+    cache.store(pk.KvSeqs(i32([0, total]), i32([0]), pages, total, total, total), randn((total, 1, dh), 1), v)
+    q = randn((16, heads, dh), 3, DT[ty]).repeat(n // 16, 1, 1)
+    seqs = pk.KvSeqs(i32(range(n + 1)), i32([total - 1] * n), pages.expand(n, -1).contiguous(), n, 1, total)
+    got = cache.attend(seqs, q)[:16, heads - 1].double()
+    k64, v64 = (x[:, 0].reshape(total, dh) for x in decoded(cache))
+    want = torch.softmax(q[:16, heads - 1].double() @ k64.T * dh ** -0.5, -1) @ v64
+    off = ((got - want) / want).mean().abs().item()
+    u = torch.finfo(DT[ty]).eps / 2
+    assert off <= (5 * u * math.sqrt(total / 16) if ty == "f32" else u / 8 + 5 * u / math.sqrt(3) / 32), off
+
+
 def test_attention_repeats_bit_for_bit(pk):
     su = Setup(pk, [3000, 1200, 5], [7, 1, 3], "q4", 2, 128, 16)
     su.fill(pk)
