@@ -559,6 +559,79 @@ def test_attention_extremes(pk):
     assert torch.equal(got, good)
 
 
+@pytest.mark.parametrize("kind", ["q8", "q4"])
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("ty", list(DT))
+@pytest.mark.parametrize("new,heads", [(4, 8), (40, 8)])
+def test_attention_scales_apart(pk, kind, dh, ty, new, heads):
+    """V rows 10^10 apart in size under weights of every size, for few rows and for many (another kernel), in a chunk of
+    its own and split.  The products w D^V lie on a grid of 2^-24 where the row's largest is 2^6 or more, so each is off by
+    2^-25 2^-6 of that largest, p max |v| 127 / 97 at the most: n positions by n 2^-30 of the largest p max |v|."""
+    for lens in ([600], [5000]):
+        su = Setup(pk, lens, [new], kind, 2, dh, 16, seed=6)
+        su.fill(pk)
+        pg, sl = su.rows(0)
+        su.cache.vs[pg[::7], :, sl[::7], 0] *= 1e4
+        su.cache.vs[pg[::5], :, sl[::5], 0] *= 1e-6
+        k64, v64 = decoded(su.cache)
+        total = lens[0] + new
+        vis = (torch.arange(total, device="cuda")[None] <= lens[0] + torch.arange(new, device="cuda")[:, None])[:, None]
+        for std in (1e-4, 1.0, 12.0):
+            q = randn((new, heads, dh), 8, DT[ty], std=std)
+            got = su.cache.attend(su.seqs, q)
+            want, absv, dots = attention(su, q)
+            most = torch.empty((new, heads, 1), dtype=torch.float64, device="cuda")
+            for h in range(2):
+                k, v = k64[pg, h, sl], v64[pg, h, sl]
+                mine = slice(h * heads // 2, (h + 1) * heads // 2)
+                p = torch.softmax((q[:, mine].double() @ k.T * dh ** -0.5).masked_fill(~vis, -math.inf), -1)
+                most[:, mine] = (p * v.abs().amax(-1)).amax(-1, keepdim=True)
+            lim = attn_bound(q, want, absv, dots, dh) + total * 2.0 ** -30 * most
+            assert torch.isfinite(got).all()
+            assert ((got.double() - want).abs() <= lim).all(), (std, ((got.double() - want).abs() / lim).max().item())
+
+
+@pytest.mark.parametrize("kind", ["q8", "q4"])
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("ty", list(DT))
+def test_attention_wide_masked_garbage(pk, kind, dh, ty):
+    """Many rows: NaN and infinite scales behind the sequences' ends, under masked drafts and in pages that are none, also
+    whole tiles of those, never reach a result."""
+    lens, new = [37, 290, 0], [40, 70, 33]
+    su = Setup(pk, lens, new, kind, 2, dh, 16, slack=1)
+    su.fill(pk)
+    hidden = {0: (1, 17), 1: (0, 33, 69), 2: (32,)}  # drafts that no row sees
+    gone = {0: (), 1: (2, 8, 9, 10, 11, 12), 2: (1,)}  # pages that are none
+    used = torch.zeros(su.cache.ks.shape[:3], dtype=torch.bool, device="cuda")
+    table = su.table.copy()
+    for s in range(3):
+        pg, sl = su.rows(s)
+        used[pg, :, sl] = True
+        for j in hidden[s]:
+            used[pg[lens[s] + j], :, sl[lens[s] + j]] = False
+        for i, j in enumerate(gone[s]):
+            used[pg[j * 16]] = False
+            table[s, j] = (-1, su.cache.n_pages, -2 ** 31, 2 ** 31 - 1)[i % 4]
+    see = {}
+    for s, n in enumerate(new):
+        see[s] = torch.rand((n, n), generator=gen(70 + s), device="cuda") < 0.4
+        see[s][:, list(hidden[s])] = False
+        see[s][3] = False
+    rows = [[sum(1 << int(j) for j in r.nonzero()[:, 0].tolist()) for r in see[s]] for s in range(3)]
+    mask = words_of(sum(rows, []), 2)
+    q = randn((sum(new), 8, dh), 8, DT[ty])
+    seqs = pk.KvSeqs(su.seqs.start, su.seqs.ctx, i32(table), su.n_tok, su.max_new, su.max_len)
+    holes = lambda s: torch.isin(torch.arange(lens[s] + new[s], device="cuda") // 16, torch.tensor(gone[s], device="cuda"))  # noqa: E731
+    for bad in (math.nan, math.inf):
+        for t in (su.cache.ks, su.cache.vs):
+            t[..., 0][~used] = bad
+        got = su.cache.attend(seqs, q, mask=mask)
+        for t in (su.cache.ks, su.cache.vs):
+            t[..., 0][~used] = 0.0
+        check_attention(su, q, got, see=lambda s, n: see[s], holes=holes)
+        assert (got[su.start[2] + 3] == 0).all()
+
+
 @pytest.mark.parametrize("ty", list(DT))
 def test_attention_strides(pk, ty):
     """Queries and outputs inside larger tensors, unaligned; rows behind the last sequence and everything between keep
