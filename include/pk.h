@@ -421,9 +421,13 @@ int pk_kv_attn(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const pk_kv_que
  *                   divided by factor, the fastest not at all
  *   PK_ROPE_YARN    pairs that turn at most `low` times in n_ctx_train
  *                   positions divided by factor, those that turn at least
- *                   `high` times kept, linear in between; gain
- *                   0.1 ln(factor) + 1 (or the one given)
- * factors (host, n_rot / 2 values or null) divides each pair's turns first. */
+ *                   `high` times kept, linear in a pair's number of turns in
+ *                   between; gain 0.1 ln(factor) + 1 (or the one given)
+ * factors (host, n_rot / 2 values or null) divides each pair's turns first.
+ * Checkpoints made for a ramp that is linear in the pair's index i instead (from
+ * the pair that turns `high` times to the one that turns `low` times) take
+ * other turns: PK_ROPE_NONE with factors[i] = 1 / (keep_i + (1 - keep_i) /
+ * factor), keep_i the ramp's share of unscaled turns, and the gain given. */
 #define PK_ROPE_NONE 0
 #define PK_ROPE_LINEAR 1
 #define PK_ROPE_NTK 2

@@ -277,7 +277,9 @@ class KvCache:
 
 class RopeTable:
     """The turns a position of n_rot / 2 pairs, on the device, and the gain (pk_rope_turns).  yarn: pairs that turn at
-    most `low` times in n_ctx_train positions are slowed by `factor`, those that turn `high` times or more are kept."""
+    most `low` times in n_ctx_train positions are slowed by `factor`, those that turn `high` times or more are kept, linear
+    in the turns between them.  A ramp that is linear in the pair's index, which some checkpoints were made for, is given
+    as factors, 1 / (keep + (1 - keep) / factor) a pair, with the gain."""
 
     def __init__(self, n_rot: int, theta: float = 10000.0, scaling: str = "none", factor: float = 1.0, n_ctx_train: int = 0,
                  low: float = 1.0, high: float = 32.0, gain: float | None = None, factors=None, device="cuda"):

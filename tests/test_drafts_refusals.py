@@ -187,6 +187,26 @@ def test_strides_of_single_rows(pk):
         assert D._same_strides(k, v) == ok, (k.stride(), v.stride())
 
 
+@pytest.mark.parametrize("n_rot,theta,ctx,factor", [(128, 10000.0, 4096, 8.0), (64, 500000.0, 8192, 32.0), (48, 10000.0, 2048, 4.0)])
+def test_ramp_by_index_as_factors(pk, n_rot, theta, ctx, factor):
+    """The long-context ramp that is linear in the pair's index, through factors: every turn within the factor's rounding
+    to f32.  It is not the one that is linear in the turns."""
+    at = lambda turns: n_rot / 2 * math.log(ctx / (turns * 2 * math.pi)) / math.log(theta)  # noqa: E731  (pair that turns so often)
+    lo, hi = max(math.floor(at(32.0)), 0), min(math.ceil(at(1.0)), n_rot - 1)
+    want, factors = [], []
+    for i in range(n_rot // 2):
+        keep = 1.0 - min(max((i - lo) / max(hi - lo, 0.001), 0.0), 1.0)
+        f = theta ** (-2.0 * i / n_rot) / (2 * math.pi)
+        want.append(f / factor * (1 - keep) + f * keep)
+        factors.append(1.0 / (keep + (1 - keep) / factor))
+    gain = 0.1 * math.log(factor) + 1
+    table = pk.RopeTable(n_rot, theta, factors=factors, gain=gain, device="cpu")
+    assert abs(table.gain - gain) < 1e-7 * gain
+    assert all(abs(a - b) <= b * (2.0 ** -24 + 1e-14) for a, b in zip(table.turns.tolist(), want))
+    other = pk.RopeTable(n_rot, theta, "yarn", factor, ctx, device="cpu")
+    assert max(a / b for a, b in zip(other.turns.tolist(), want)) > 1.3 or min(a / b for a, b in zip(other.turns.tolist(), want)) < 0.8
+
+
 def test_mask_without_words(pk):
     """A mask of no words is refused: its tensor has no address, and no address means causal."""
     torch = pytest.importorskip("torch")
