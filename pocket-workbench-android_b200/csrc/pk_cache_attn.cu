@@ -728,17 +728,10 @@ Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int ty
 // it takes alone (64 tokens at 8000 positions, 64 heads over 8: 4 chunks, one
 // CTA an SM, 53 us, 8 chunks 66, one 127, 37 100; 32 sequences of 2000: one
 // chunk 61, two 79, four 100; the wide trees 770, 799 and 750).
-//
-// Half-precision queries' outputs are summed by the tensor core, which cuts off
-// what it shifts out: less than 2^-23 of the sum each step of 16 positions, all
-// to one side where V's values have one sign (measured: 2^-27.1 of it a position
-// on tcgen05, a quarter on mma.sync, whose four groups of warps have sums of
-// their own).  A chunk's length keeps that under an eighth of the output's
-// rounding, 2^-14 for f16 and 2^-11 for bf16; chunks are added in f32.
-constexpr long long SUM_F16 = 8192, SUM_BF16 = 65536;  // positions of one such sum
 struct Split {
   int chunk, n_chunk, row_tiles;
   bool cluster;
+  bool parts;  // partial results go through the scratch
 };
 Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type, const Variant &v) {
   Split p;
@@ -746,24 +739,24 @@ Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type, 
   p.row_tiles = (int)((rows + v.rows - 1) / v.rows);
   const long long units = (long long)s.n_seq * c.n_kv * p.row_tiles, want = 148 * 8;
   const long long most = (s.max_len + MIN_CHUNK - 1) / MIN_CHUNK;
-  const long long sum = (type == T_F16 ? SUM_F16 : SUM_BF16) * (v.k ? 4 : 1);
-  const long long least = type == T_F32 ? 1 : (s.max_len + sum - 1) / sum;
+  const long long sum = sum_most(type), least = v.k && type != T_F32 ? (s.max_len + 4 * sum - 1) / (4 * sum) : 1;
   long long n = std::max(least, std::min(most, want / units));
   if (!v.k) {
     long long best = 0;
     const long long top = n;
-    for (long long c = least; c <= top; c++) {
+    for (long long c = 1; c <= top; c++) {
       const long long ctas = units * c, left = ctas % 296, tiles = ((s.max_len + 63) / 64 + c - 1) / c;
       const long long t = v.rows == 256 ? (ctas + 147) / 148 * (tiles + 8)
                                         : (ctas / 296 * 8 + (left == 0 ? 0 : left <= 148 ? 5 : 8)) * (tiles + 16);
-      if (c == least || t < best) best = t, n = c;
+      if (c == 1 || t < best) best = t, n = c;
     }
   }
   const long long slots = v.rows == 256 ? 128 : 296;  // CTAs that run at once, in clusters too
-  if (v.k && n > 8 && n <= 16 && units * 8 <= slots) n = 8;
+  if (v.k && n > 8 && n <= 16 && least <= 8 && units * 8 <= slots) n = 8;
   p.chunk = (int)(((s.max_len + n - 1) / n + 63) / 64 * 64);
   p.n_chunk = (int)((s.max_len + (long long)p.chunk - 1) / p.chunk);
   p.cluster = p.n_chunk > 1 && p.n_chunk <= 8 && units * p.n_chunk <= slots;
+  p.parts = (p.n_chunk > 1 && !p.cluster) || (!v.k && type != T_F32 && p.chunk > sum);
   return p;
 }
 
@@ -781,7 +774,7 @@ static pk_kv_seqs bounded(const pk_kv_cache &c, pk_kv_seqs s) {
 size_t kv_attn_scratch_bytes(const pk_kv_cache &c, const pk_kv_seqs &seqs, int n_head, int type) {
   const pk_kv_seqs s = bounded(c, seqs);
   const Split p = split_of(c, s, n_head, type, variant_of(c, s, n_head, type));
-  if (p.n_chunk <= 1 || p.cluster) return 0;
+  if (!p.parts) return 0;
   return (size_t)s.n_tok * n_head * p.n_chunk * (c.head_dim + 2) * sizeof(float);
 }
 
@@ -807,7 +800,7 @@ cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &seqs, const p
   a.cluster = p.cluster;
   a.err = err;
   a.poison = poison;
-  a.part_ml = p.n_chunk > 1 && !a.cluster ? reinterpret_cast<float2 *>(a.part_o + rows * p.n_chunk * c.head_dim) : nullptr;
+  a.part_ml = p.parts ? reinterpret_cast<float2 *>(a.part_o + rows * p.n_chunk * c.head_dim) : nullptr;
   const long long blocks = (long long)s.n_seq * c.n_kv * p.row_tiles * p.n_chunk, jb = ((long long)rows + 3) / 4;
   if (blocks > 0x7fffffffLL || (long long)rows > 0x7fffffffLL) return cudaErrorInvalidValue;
   const int cluster = a.cluster ? p.n_chunk : 1;

@@ -37,11 +37,20 @@ __device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_grou
 template <int N>
 __device__ __forceinline__ void cp_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
+// Half-precision queries' outputs are summed by the tensor core, which cuts off
+// what it shifts out: less than 2^-23 of the sum each step of 16 positions, all
+// to one side where V's values have one sign (measured: 2^-27.1 of it a position
+// on tcgen05, a quarter on mma.sync, whose four groups of warps have sums of
+// their own).  A sum goes over so many positions that this stays under an eighth
+// of the output's rounding, 2^-14 for f16 and 2^-11 for bf16; then on mma.sync
+// the chunk ends, and on tcgen05 the sum is added to the scratch in f32.
+__host__ __device__ constexpr int sum_most(int type) { return type == T_F16 ? 8192 : 65536; }
+
 struct AttnKArgs {
   pk_kv_cache c;
   pk_kv_seqs s;
   pk_kv_query q;
-  float *part_o;   // [n_tok][n_head][n_chunk][DH]
+  float *part_o;   // [n_tok][n_head][n_chunk][DH]: chunks' parts, or what long sums gave up so far
   float2 *part_ml; // [n_tok][n_head][n_chunk]
   int chunk, n_chunk, row_tiles, group, page_shift, vec_q, vec_o;
   int cluster;  // 1: a sequence's chunks are a cluster's CTAs, which add up among themselves

@@ -15,8 +15,8 @@
 //              tile ahead, made f16 (exact) and put into the operand's layout.
 //   4          V's codes.
 //   1          issues the products.
-// Half precision: one block, P as f16 in S's columns, O summed in TMEM, and two
-// CTAs an SM (100 KB and 256 TMEM columns each), so that one's products run
+// Half precision: one block, P as f16 in S's columns, O summed in TMEM (long
+// sums in parts, added up in the scratch), and two CTAs an SM (100 KB and 256 TMEM columns each), so that one's products run
 // beside the other's softmax.  f32 (head_dim 64): queries and weights are two
 // f16 terms each (2^-22), and a tile's O is added to the row's sums in
 // registers, because the tensor core's sums drop what they shift out; two
@@ -59,6 +59,10 @@ namespace {
 
 constexpr int NK = 64;                      // positions a tile
 constexpr unsigned long long WAIT_NS = 2000000000ull;
+// Tiles of one sum in TMEM (half precision).  Chunks of more take the kernel's
+// LONG form: its additions to the scratch cost the others 2% by their size.
+template <class E>
+constexpr int SUM_TILES = sum_most(std::is_same_v<E, __half> ? T_F16 : T_BF16) / NK;
 
 // Terms of a query or weight: one f16 for half precision, two for f32.
 template <class E>
@@ -183,6 +187,13 @@ __device__ __forceinline__ void ask_quads(uint32_t t, float (&v)[16]) {
                : "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
                : "r"(t + (16u << 16)));
 }
+// The first 16 of the warp's 32 rows only (j < 2), and their arrival.
+__device__ __forceinline__ void ask_half(uint32_t t, float (&v)[8]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n tcgen05.wait::ld.sync.aligned;"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "r"(t)
+               : "memory");
+}
 __device__ __forceinline__ void st_quads(uint32_t t, const float (&v)[16]) {
   asm volatile("tcgen05.st.sync.aligned.16x256b.x2.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(t), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
                : "memory");
@@ -291,7 +302,7 @@ __device__ __forceinline__ uint64_t seen_by(const AttnKArgs &a, const Unit &u, i
   return v & ones(hi - p0) & ones(u.sv.ctx + u.sv.n - p0);
 }
 
-template <int TYPE, int DH, class E>
+template <int TYPE, int DH, class E, bool LONG>
 __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_of<E>>::CTAS) k_kv_attn_tc(const AttnKArgs a) {
   constexpr int NT = terms_of<E>, BLK = NT;
   using L = Lay<DH, NT>;
@@ -384,7 +395,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
           for (int n = NT - 1; n >= 0; n--)
 #pragma unroll
             for (int s = 0; s < NK / 16; s++)
-              mma_f16_ts<DH, true>(o, w + n * (NK / 2) + s * 8, v + s * 16, (NT == 1 && i > 0) || s > 0 || n < NT - 1);
+              mma_f16_ts<DH, true>(o, w + n * (NK / 2) + s * 8, v + s * 16, (NT == 1 && (LONG ? i % SUM_TILES<E> != 0 : i > 0)) || s > 0 || n < NT - 1);
           commit_one(pvdone_of(m, i));
         }
       }
@@ -531,6 +542,42 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
         for (int j = 0; j < 16; j++) o[NT == 2 ? 16 * c + j : 0] += v[j];
       }
     };
+    // half precision: the sum of tiles .. i - 1 is added to what the scratch has
+    // of the row, beside the reference that it was made with (16 rows at a time:
+    // registers of the whole loop are few)
+    auto keep_o = [&](int i) {
+      pv_wait(i - 1);
+      tc_fence_after();
+#pragma unroll 1
+      for (int half = 0; half < 2; half++) {
+        const float m[2] = {half ? m4[2] : m4[0], half ? m4[3] : m4[1]};
+        float *to[2];
+        float g[2];
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const int row = tile0 + warp * 32 + (lane >> 2) + 16 * half + 8 * j, r = min(row, u.rows - 1), t = r / a.group;
+          const long long at = ((long long)(u.sv.first + t) * a.q.n_head + u.h * a.group + r - t * a.group) * a.n_chunk + u.ch;
+          to[j] = a.part_o + at * DH + 2 * quad;
+          const float before = i > SUM_TILES<E> ? a.part_ml[at].x : -CUDART_INF_F;
+          g[j] = before == -CUDART_INF_F ? 0.0f : ex2(before - m[j]);
+          __syncwarp();
+          if (quad == 0 && row < u.rows) a.part_ml[at].x = m[j];
+        }
+#pragma unroll 1
+        for (int c = 0; c < DH / 16; c++) {
+          float v[8];
+          __syncwarp();
+          ask_half(tmem + lanes + ((uint32_t)(16 * half) << 16) + L::O_COL + 16 * c, v);
+#pragma unroll
+          for (int p = 0; p < 4; p++) {  // row 8 (p % 2), columns 8 (p / 2) and the next
+            if (tile0 + warp * 32 + (lane >> 2) + 16 * half + 8 * (p & 1) >= u.rows) continue;
+            float2 *x = reinterpret_cast<float2 *>(to[p & 1] + 16 * c + 8 * (p >> 1));
+            const float2 o = make_float2(v[2 * p], v[2 * p + 1]);
+            *x = i > SUM_TILES<E> ? fma2(*x, make_float2(g[p & 1], g[p & 1]), o) : o;
+          }
+        }
+      }
+    };
     // O's rows times f, once the products before are done (i > 0)
     auto scale_o = [&](int i, const float (&f)[4]) {
       if (i == 0) return;
@@ -558,6 +605,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
       wait(sfull_of(blk, i), (i >> 1) & 1, abort);
       tc_fence_after();
       if (work) {
+        if (LONG && i > 0 && i % SUM_TILES<E> == 0) keep_o(i);
         const uint8_t *sc = smem + L::SC + (i & 3) * L::SCB;
         const float2 *dk2 = reinterpret_cast<const float2 *>(sc) + quad, *dv2 = dk2 + NK / 2;
         const uint4 r4 = *reinterpret_cast<const uint4 *>(sc + 2 * NK * 4);
@@ -759,7 +807,11 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
       const int i = tok, h = u.h * a.group + (min(row, u.rows - 1) - i * a.group);
       const long long at = u.sv.first + i;
       const bool on = row < u.rows, part = u.nch > 1;
-      float f = 1.0f;
+      float f = 1.0f, g = 0.0f;  // g: of what a long sum has in the scratch
+      if (LONG && nt > SUM_TILES<E> && on) {
+        const float before = a.part_ml[(at * a.q.n_head + h) * a.n_chunk + u.ch].x;
+        g = before == -CUDART_INF_F ? 0.0f : ex2(before - m);
+      }
       if (*abort) f = l = CUDART_NAN_F;
       if (part) {
         if (on && cluster) *reinterpret_cast<float2 *>(smem + L::ML + tid * 8) = make_float2(m, l);
@@ -780,6 +832,11 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
         } else {
 #pragma unroll
           for (int j = 0; j < 16; j++) v[j] = 0.0f;
+        }
+        if (LONG && nt > SUM_TILES<E> && on) {
+          const float *p = a.part_o + ((at * a.q.n_head + h) * a.n_chunk + u.ch) * DH + 16 * c;
+#pragma unroll
+          for (int j = 0; j < 16; j++) v[j] = fmaf(g, p[j], v[j]);
         }
 #pragma unroll
         for (int k = 0; k < 2 && on; k++) {
@@ -813,14 +870,16 @@ struct Kernel {
   int threads, smem, regs;
 };
 template <int TYPE, int DH, class E>
-Kernel kernel_as() {
+Kernel kernel_as(bool many) {
   using L = Lay<DH, terms_of<E>>;
-  return {k_kv_attn_tc<TYPE, DH, E>, L::THREADS, L::BYTES, L::REGS};
+  if constexpr (terms_of<E> == 1)
+    if (many) return {k_kv_attn_tc<TYPE, DH, E, true>, L::THREADS, L::BYTES, L::REGS};
+  return {k_kv_attn_tc<TYPE, DH, E, false>, L::THREADS, L::BYTES, L::REGS};
 }
 template <class E>
-Kernel kernel_of(const pk_kv_cache &c) {
-  if (c.head_dim == 64) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 64, E>() : kernel_as<PK_KV_Q4, 64, E>();
-  if constexpr (terms_of<E> == 1) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 128, E>() : kernel_as<PK_KV_Q4, 128, E>();
+Kernel kernel_of(const pk_kv_cache &c, bool many) {
+  if (c.head_dim == 64) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 64, E>(many) : kernel_as<PK_KV_Q4, 64, E>(many);
+  if constexpr (terms_of<E> == 1) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 128, E>(many) : kernel_as<PK_KV_Q4, 128, E>(many);
   return {};
 }
 
@@ -828,11 +887,12 @@ Kernel kernel_of(const pk_kv_cache &c) {
 
 cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int cluster, unsigned blocks, cudaStream_t st) {
   const int e = a.q.type == T_F32 ? 0 : a.q.type == T_F16 ? 1 : 2;
-  const Kernel k = e == 0 ? kernel_of<float>(a.c) : e == 1 ? kernel_of<__half>(a.c) : kernel_of<__nv_bfloat16>(a.c);
+  const bool many = e && a.chunk > sum_most(a.q.type);  // (positions; only half precision sums in TMEM)
+  const Kernel k = e == 0 ? kernel_of<float>(a.c, many) : e == 1 ? kernel_of<__half>(a.c, many) : kernel_of<__nv_bfloat16>(a.c, many);
   if (!k.k) return cudaErrorInvalidValue;
   // the split of the registers would wait forever for what a launch does not have
   static std::atomic<unsigned> checked{0};
-  const unsigned bit = 1u << (e * 4 + 2 * (a.c.type == PK_KV_Q4) + (a.c.head_dim == 128));
+  const unsigned bit = 1u << (16 * many + e * 4 + 2 * (a.c.type == PK_KV_Q4) + (a.c.head_dim == 128));
   if (!(checked.load(std::memory_order_relaxed) & bit)) {
     cudaFuncAttributes f;
     const cudaError_t err = cudaFuncGetAttributes(&f, reinterpret_cast<const void *>(k.k));

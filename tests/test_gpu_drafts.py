@@ -767,6 +767,36 @@ def test_attention_sums_of_long_histories(pk, ty, total, heads):
     assert off <= (5 * u * math.sqrt(total / 16) if ty == "f32" else u / 8 + 5 * u / math.sqrt(3) / 32), off
 
 
+@pytest.mark.parametrize("kind,dh,ty,total", [("q8", 64, "f16", 100003), ("q4", 128, "f16", 70001), ("q8", 128, "bf16", 140009), ("q4", 64, "bf16", 140009)])
+@pytest.mark.parametrize("n", [37, 100, 592])
+def test_attention_long_sums_in_parts(pk, kind, dh, ty, total, n):
+    """Sums longer than one that the tensor core keeps, for as many sequences as make a cluster's chunks, chunks in the
+    scratch, and one chunk each: scores that grow along the history, so that rows' references move late, and two new
+    tokens with a mask."""
+    page, heads = 1024, 20
+    np_ = -(-total // page)
+    cache = pk.KvCache.empty(np_, page, 1, dh, kind)
+    pages = torch.arange(np_, dtype=torch.int32, device="cuda").flip(0)[None].contiguous()
+    up = torch.linspace(-0.5, 2.5, total, device="cuda")[:, None, None]
+    k, v = randn((total, 1, dh), 1, std=0.3) + up, randn((total, 1, dh), 2)
+    cache.store(pk.KvSeqs(i32([0, total]), i32([0]), pages, total, total, total), k, v)
+    q = (randn((2 * n, heads, dh), 3, std=0.5) + 0.8).to(DT[ty])
+    seqs = pk.KvSeqs(i32(range(0, 2 * n + 1, 2)), i32([total - 2] * n), pages.expand(n, -1).contiguous(), 2 * n, 2, total)
+    mask = torch.tensor([[1], [2]], device="cuda").repeat(n, 1)
+    got = cache.attend(seqs, q, mask=mask)
+    k64, v64 = (x.flip(0)[:, 0].reshape(-1, dh)[:total] for x in decoded(cache))
+    for t in (0, 1, 5, 2 * n - 2, 2 * n - 1):
+        x = q[t].double()
+        w = x @ k64.T * dh ** -0.5
+        w[:, total - 1 if t % 2 == 0 else total - 2] = -math.inf
+        p = torch.softmax(w, -1)
+        want, absv, dots = p @ v64, p @ v64.abs(), (x.abs() @ k64.abs().T * dh ** -0.5).amax(-1)
+        most = (p * v64.abs().amax(-1)).amax(-1, keepdim=True)
+        # (the sums may drop an eighth of the output's rounding, eps / 16, of what they add up)
+        lim = attn_bound(q, want, absv, dots, dh) + absv * torch.finfo(DT[ty]).eps / 16 + total * 2.0 ** -30 * most
+        assert ((got[t].double() - want).abs() <= lim).all(), (t, ((got[t].double() - want).abs() / lim).max().item())
+
+
 def test_attention_repeats_bit_for_bit(pk):
     su = Setup(pk, [3000, 1200, 5], [7, 1, 3], "q4", 2, 128, 16)
     su.fill(pk)
