@@ -187,6 +187,7 @@ class KvCache:
                 _bad(f"a cache array is not a contiguous {dt} tensor {tuple(shape)} on {k.device}")
         self.k, self.v, self.ks, self.vs, self.kind, self.head_dim = k, v, ks, vs, kind, head_dim
         self.n_pages, self.n_kv, self.page_size = k.shape[:3]
+        self.shape = (kind, self.n_kv, head_dim, self.page_size)  # what the scratch of attend() depends on
         self.device = k.get_device()
         self.c = KvCacheC(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), KINDS[kind], self.n_pages,
                           self.page_size, self.n_kv, head_dim)
@@ -250,7 +251,7 @@ class KvCache:
             out = _like(q) if stream is None else _new(lambda: _like(q), dev, stream)
         elif out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or out.stride(2) != 1:
             _bad("attend: out must be as q")
-        ptr, size = None, seqs.scratch.get((shape[1], code, self.kind, self.n_kv, self.head_dim))
+        ptr, size = None, seqs.scratch.get((shape[1], code) + self.shape)
         if size is None:
             size = self.attend_scratch_bytes(seqs, shape[1], q.dtype)
         if scratch is not None:
@@ -271,7 +272,7 @@ class KvCache:
         """Bytes of scratch that attend() needs (0: none); kept with the sequences, whose bounds do not change."""
         code = _type_of[dtype]
         n = _L.pk_kv_attn_scratch_bytes(self.ref, seqs.ref, n_head, code)
-        seqs.scratch[n_head, code, self.kind, self.n_kv, self.head_dim] = n
+        seqs.scratch[(n_head, code) + self.shape] = n
         return n
 
 

@@ -1121,6 +1121,23 @@ def test_memory_of_a_call_on_another_stream(pk):
     torch.cuda.synchronize()
 
 
+def test_scratch_of_two_page_sizes(pk):
+    """The same sequences over caches of other page sizes: a page table reaches further there, and the scratch is sized
+    for each."""
+    pages = i32(range(40)).reshape(1, 40)
+    seqs = pk.KvSeqs(i32([0, 1]), i32([600]), pages, 1, 1, 1 << 20)
+    q = randn((1, 2, 64), 1)
+    sizes, outs = [], []
+    for page in (16, 256, 16):
+        cache = pk.KvCache.empty(40, page, 2, 64)
+        cache.store(pk.KvSeqs(i32([0, 601]), i32([0]), pages, 601, 601, 601), randn((601, 2, 64), 2), randn((601, 2, 64), 3))
+        outs.append(cache.attend(seqs, q))
+        sizes.append(cache.attend_scratch_bytes(seqs, 2, q.dtype))
+        assert torch.equal(cache.attend(seqs, q), outs[-1])
+    assert sizes[0] == sizes[2] < sizes[1] and torch.equal(outs[0], outs[2])
+    assert (outs[0] - outs[1]).abs().max() <= 2.0 ** -18 * outs[0].abs().max()
+
+
 def test_refusals_on_the_device(pk):
     su = Setup(pk, [5], [2], "q8", 2, 64, 16)
     k = randn((2, 2, 64), 1)
