@@ -7,7 +7,8 @@
 Nothing here waits for the device, and every call can be captured into a CUDA graph once its outputs and scratch are
 passed in (or come from the graph's own pool).  Calls run on the tensors' device, on its current stream or on the
 `stream` given (a raw cudaStream_t).  With `stream`, what a call makes (outputs, scratch) comes from that stream's
-memory; the caller orders its own tensors, and its later use of the outputs, against that stream.
+memory, and the tensors that it uses are not given to others before that stream is done with them; the caller orders
+what they hold, and its later use of the outputs, against that stream.
 """
 from __future__ import annotations
 
@@ -100,13 +101,20 @@ def _dtype(t, who):
     return code
 
 
-def _call(fn, device, stream, *args):
-    """fn(*args, stream) on device number `device`."""
+def _call(fn, device, stream, used, *args):
+    """fn(*args, stream) on device number `device`; used: the call's tensors and lists of them, which may be freed before
+    a stream that is not the current one has come to the call."""
     if stream is None and current_device() == device:
         rc = fn(*args, raw_stream(device))
     else:
         with torch.cuda.device(device):
             rc = fn(*args, raw_stream(device) if stream is None else stream)
+        if stream is not None and stream != raw_stream(device):
+            other = torch.cuda.ExternalStream(stream, device=device)
+            for x in used:
+                for t in x if isinstance(x, tuple) else (x,):
+                    if t is not None:
+                        t.record_stream(other)
     if rc:
         raise PkError(rc, last_error())
 
@@ -167,6 +175,7 @@ class KvSeqs:
         self.device, self.n_seq, self.n_tok, self.max_new, self.max_len = device, n, n_tok, max_new, max_len
         self.c = KvSeqsC(start.data_ptr(), ctx.data_ptr(), pages.data_ptr(), n, pages.shape[1], n_tok, max_new, max_len)
         self.ref = C.byref(self.c)
+        self.tensors = (start, ctx, pages)
         self.scratch = {}  # bytes that attend() needs, by what they depend on besides
 
 
@@ -192,6 +201,7 @@ class KvCache:
         self.c = KvCacheC(k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr(), KINDS[kind], self.n_pages,
                           self.page_size, self.n_kv, head_dim)
         self.ref = C.byref(self.c)
+        self.tensors = (k, v, ks, vs)
 
     @classmethod
     def empty(cls, n_pages: int, page_size: int, n_kv: int, head_dim: int, kind: str = "q8", device="cuda"):
@@ -217,7 +227,7 @@ class KvCache:
     def store(self, seqs: KvSeqs, k, v, stream=None):
         """Quantises rows k, v [n_tok, n_kv, head_dim] of the new tokens into the cache.  k and v have the same strides:
         those of one fused projection do, also after rope() in place (out_q, out_k)."""
-        _call(_L.pk_kv_store, self.device, stream, self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "store"))
+        _call(_L.pk_kv_store, self.device, stream, (self.tensors, seqs.tensors, k, v), self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "store"))
 
     def load(self, seqs: KvSeqs, dtype=None, out=None, stream=None):
         """(k, v) [n_tok, n_kv, head_dim] of positions ctx .. read back; rows that no sequence has keep what they held."""
@@ -227,7 +237,7 @@ class KvCache:
             make = lambda: torch.empty_strided(shape, st, dtype=dt, device=dev)  # noqa: E731
             out = (make(), make()) if stream is None else _new(lambda: (make(), make()), self.device, stream)
         k, v = out
-        _call(_L.pk_kv_load, self.device, stream, self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "load"))
+        _call(_L.pk_kv_load, self.device, stream, (self.tensors, seqs.tensors, k, v), self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "load"))
         return k, v
 
     def keep(self, seqs: KvSeqs, keep, n_keep, stream=None):
@@ -236,7 +246,7 @@ class KvCache:
         _i32(n_keep, self.device, "n_keep", 1)
         if keep.shape[0] != seqs.n_seq or n_keep.shape[0] != seqs.n_seq or seqs.device != self.device:
             _bad("keep: one row and one count a sequence, on the cache's device")
-        _call(_L.pk_kv_keep, self.device, stream, self.ref, seqs.ref, keep.data_ptr(), keep.shape[1], n_keep.data_ptr())
+        _call(_L.pk_kv_keep, self.device, stream, (self.tensors, seqs.tensors, keep, n_keep), self.ref, seqs.ref, keep.data_ptr(), keep.shape[1], n_keep.data_ptr())
 
     def attend(self, seqs: KvSeqs, q, mask=None, scale: float | None = None, out=None, scratch=None, stream=None):
         """Attention of the new tokens q [n_tok, n_head, head_dim] over the cache; mask: int64 [n_tok, words], bit j of
@@ -265,7 +275,7 @@ class KvCache:
         o = out.stride()
         args = PACK_QUERY(q.data_ptr(), out.data_ptr(), bits, s[0], s[1], o[0], o[1], code, shape[1], words,
                           self.head_dim ** -0.5 if scale is None else scale)
-        _call(_L.pk_kv_attn, dev, stream, self.ref, seqs.ref, args, ptr, size)
+        _call(_L.pk_kv_attn, dev, stream, (self.tensors, seqs.tensors, q, mask, out, scratch), self.ref, seqs.ref, args, ptr, size)
         return out
 
     def attend_scratch_bytes(self, seqs: KvSeqs, n_head: int, dtype) -> int:
@@ -338,7 +348,7 @@ def rope(table: RopeTable, pos, q, k=None, layout: str = "interleaved", out_q=No
         kt, kp, kq, nk = out_k.stride(), k.data_ptr(), out_k.data_ptr(), kshape[1]
     args = PACK_ROPE(q.data_ptr(), kp, out_q.data_ptr(), kq, pos.data_ptr(), table.turns.data_ptr(), qs[0], qs[1], ks[0], ks[1], qt[0],
                      qt[1], kt[0], kt[1], code, pairs, n, shape[1], nk, dh, table.n_rot, table.gain)
-    _call(_L.pk_rope, dev, stream, args)
+    _call(_L.pk_rope, dev, stream, (table.turns, pos, q, k, out_q, out_k), args)
     return out_q, out_k
 
 
@@ -386,6 +396,6 @@ def logit_rules(logits, repeat=None, freq=None, presence=None, hist=None, n_hist
     args = PACK_RULES(_row_value(repeat, "repeat", f, rows, dev), _row_value(freq, "freq", f, rows, dev),
                       _row_value(presence, "presence", f, rows, dev), hp, _row_value(n_hist, "n_hist", i, rows, dev), ip, bp, ap,
                       hs, bs, as_, hn, bn)
-    _call(_L.pk_apply_logit_rules, dev, stream, logits.data_ptr(), out.data_ptr(), code, rows, n, st[0] if len(st) == 2 else n,
+    _call(_L.pk_apply_logit_rules, dev, stream, (logits, out, repeat, freq, presence, hist, n_hist, bias_id, bias, allow), logits.data_ptr(), out.data_ptr(), code, rows, n, st[0] if len(st) == 2 else n,
           out.stride(0) if len(st) == 2 else n, args)
     return out

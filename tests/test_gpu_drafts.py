@@ -1121,6 +1121,42 @@ def test_memory_of_a_call_on_another_stream(pk):
     torch.cuda.synchronize()
 
 
+def test_tensors_of_a_call_on_another_stream(pk):
+    """Tensors that the caller lets go of right after a call on `stream` are not reused before that stream has come to it."""
+    su = Setup(pk, [6000], [2], "q8", 2, 64, 16, seed=1)
+    su.fill(pk)
+    q, kv, x = randn((2, 4, 64), 3), randn((2, 2, 64), 5), randn((2, 1000), 4)
+    table = lambda: pk.RopeTable(64)  # noqa: E731
+    one = torch.ones(2, device="cuda")
+
+    def seqs():
+        return pk.KvSeqs(su.seqs.start.clone(), su.seqs.ctx.clone(), su.seqs.pages.clone(), 2, 2, 6002)
+
+    def store(st):
+        cache = pk.KvCache(*(t.clone() for t in (su.cache.k, su.cache.v, su.cache.ks, su.cache.vs)), "q8", 64)
+        if st is not None:
+            side.wait_stream(torch.cuda.current_stream())
+        cache.store(seqs(), kv.clone(), (kv * 2).clone(), stream=st)
+        return cache.load(su.seqs, stream=st)
+
+    calls = {"attend": lambda st: su.cache.attend(seqs(), q.clone(), stream=st), "rope": lambda st: pk.rope(table(), i32([3, 4]), q.clone(), kv.clone(), stream=st),
+             "rules": lambda st: pk.logit_rules(x.clone(), hist=i32([[1, 2, 3]]), presence=one.clone(), bias_id=i32([[5]]), bias=one[:1].clone()[None], stream=st),
+             "store": store}
+    flat = lambda r: r if isinstance(r, tuple) else (r,)  # noqa: E731
+    side = torch.cuda.Stream()
+    for n, f in calls.items():
+        want = f(None)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            torch.cuda._sleep(400_000_000)
+        got = f(side.cuda_stream)  # (its inputs are ready long before the sleep is over)
+        junk = [torch.full((m,), 255, dtype=torch.uint8, device="cuda") for m in (8, 512, 1024, 2048, 4096, 8192, 32768) for _ in range(40)]
+        junk += [torch.full_like(su.cache.k, 255) for _ in range(2)] + [torch.full_like(su.cache.ks, 9.0) for _ in range(2)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(flat(got), flat(want))), n
+        del junk
+
+
 def test_scratch_of_two_page_sizes(pk):
     """The same sequences over caches of other page sizes: a page table reaches further there, and the scratch is sized
     for each."""
