@@ -360,18 +360,18 @@ typedef struct {
  * is no page: what would be written there is dropped, what would be read is
  * masked (attention) or zero (pk_kv_load).  start ascends within 0 .. n_tok,
  * the token arrays' rows; rows that no sequence has are not written, and what
- * they hold does not matter (it may be read).  max_new and max_len are bounds the host knows: of the new tokens
- * of one sequence (any number from n_tok on means n_tok), and of its committed
- * positions and new tokens together; what is beyond them is left out (all of
- * a sequence with a negative ctx).  A page that a call writes belongs to one
- * sequence of it. */
+ * they hold does not matter (it may be read).  max_new and max_len are bounds
+ * the host knows: of the new tokens of one sequence (any number from n_tok on
+ * means n_tok), and of its committed positions and new tokens together; what
+ * is beyond them is left out (all of a sequence with a negative ctx).  A page
+ * that a call writes belongs to one sequence of it. */
 typedef struct {
   const int *start, *ctx, *pages;
   int n_seq, max_pages, n_tok, max_new, max_len;
 } pk_kv_seqs;
 
 /* K and V rows of the new tokens, [n_tok][n_kv][head_dim] with strides in
- * elements (head_dim contiguous), quantised into the cache; and positions
+ * elements (the same for both, head_dim contiguous), quantised into the cache; and positions
  * ctx[s] .. read back from it into rows start[s] .. of k and v. */
 int pk_kv_store(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const void *k, const void *v, int type,
                 int64_t tok_stride, int64_t head_stride, void *stream);

@@ -28,8 +28,10 @@
 // the V rows as its output dimensions.
 //
 // Measured: one token at 1500 positions, 64 heads over 8 of 128, Q8: 10 us a
-// call; 8 sequences at 16256, 36 heads of 64, f32, Q8: 133 to 146 us, 67 to 74%
-// of a copy's rate.  What bounds it: memory for few rows, the matrix
+// call; 8 sequences at 16256, 36 heads of 64, f32, Q8: 139 to 149 us by the box,
+// 71 to 66% of a copy's rate; f32 of head_dim 128 with many rows, which have no
+// tcgen05 kernel: 8 sequences of 8000 with trees of 64, 64 heads over 8, Q8:
+// 1,136 us (f16 there: 199).  What bounds it: memory for few rows, the matrix
 // instructions' 550 TFLOP/s and the codes' conversion for many, which is why
 // those go to pk_cache_attn_tc.cu.
 #include <math_constants.h>
@@ -727,7 +729,8 @@ Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int ty
 // its part of the sums, and where two share an SM a tile takes 8 fifths of what
 // it takes alone (64 tokens at 8000 positions, 64 heads over 8: 4 chunks, one
 // CTA an SM, 53 us, 8 chunks 66, one 127, 37 100; 32 sequences of 2000: one
-// chunk 61, two 79, four 100; the wide trees 770, 799 and 750).
+// chunk 61, two 79, four 100; the wide trees 770, 799 and 750, one and four of
+// which this estimates within 1% of each other).
 struct Split {
   int chunk, n_chunk, row_tiles;
   bool cluster;

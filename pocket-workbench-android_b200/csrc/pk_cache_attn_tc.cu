@@ -26,9 +26,9 @@
 // makes it an N-major operand.
 //
 // Measured: 8 sequences of 32000 positions with trees of 64, 64 heads over 8,
-// f16, Q8: 749 us, 715 TFLOP/s; 40 sequences of up to 15000 positions, 5 drafts
-// each, bf16, Q4: 236 us; two prompt chunks of 509 tokens behind up to 2900
-// positions, 36 heads, f32, Q8: 148 us.  What bounds it: a product of N 64
+// f16, Q8: 800 to 847 us by the box, 672 to 635 TFLOP/s; 40 sequences of up to
+// 15000 positions, 5 drafts each, bf16, Q4: 238 us; two prompt chunks of 509
+// tokens behind up to 2900 positions, 36 heads, f32, Q8: 146 to 151 us.  What bounds it: a product of N 64
 // takes as long as one of N 128, so the tensor core is busy for 830 cycles of
 // the 1,400 or so that a tile of 64 positions takes an SM; 128 positions a step
 // would need 384 TMEM columns a CTA.
