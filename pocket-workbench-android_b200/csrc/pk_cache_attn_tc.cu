@@ -857,12 +857,16 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
   // Only here, after the softmax warps have had their registers and given them
   // back: taken earlier (by warps without a tile) they would be missing there.
   if (warp >= WS && (BLK > 1 || warp < WS + 8)) set_regs<true, L::REGS>();
-  if (cluster) join_cluster<DH>(a, u, tile0, ROWS, sb, sb + L::ML, THREADS);
-  if (tid == 0 && a.err && *abort) atomicCAS(a.err, 0, PK_ERR_TIMEOUT);
+  // Before the cluster's sums: a CTA that waited for its cluster with tensor
+  // memory in hand could wait for one that waits for tensor memory, which a CTA
+  // of another kernel's cluster in the same state holds.
   if (warp == WS + 8) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(BLK * L::COLS) : "memory");
   }
+  __syncwarp();
+  if (cluster) join_cluster<DH>(a, u, tile0, ROWS, sb, sb + L::ML, THREADS);
+  if (tid == 0 && a.err && *abort) atomicCAS(a.err, 0, PK_ERR_TIMEOUT);
 }
 
 struct Kernel {

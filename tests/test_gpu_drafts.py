@@ -405,6 +405,25 @@ def test_attention_wide_side_by_side(pk):
         assert torch.equal(out[0], want) and torch.equal(out[1], want)
 
 
+def test_attention_clusters_side_by_side(pk):
+    """Kernels whose CTAs wait for their cluster's and share an SM's tensor memory, on four streams at once."""
+    runs = []
+    for i, (ty, dh) in enumerate((("f16", 64), ("bf16", 64), ("f16", 128), ("f32", 64))):
+        su = Setup(pk, [6000], [40 if ty == "f32" else 20], "q8", 32, dh, 64, seed=i)
+        su.fill(pk)
+        q = randn((su.n_tok, 32, dh), 8 + i, DT[ty])
+        assert su.cache.attend_scratch_bytes(su.seqs, 32, q.dtype) == 0  # (a cluster's sums, or one chunk)
+        runs.append((su, q, su.cache.attend(su.seqs, q), torch.empty_like(q), torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(60):
+        for su, q, _, out, st in runs:
+            with torch.cuda.stream(st):
+                su.cache.attend(su.seqs, q, out=out)
+    torch.cuda.synchronize()
+    for _, _, want, out, _ in runs:
+        assert torch.equal(out, want)
+
+
 @pytest.mark.parametrize("ty", list(DT))
 @pytest.mark.parametrize("dh", [64, 128])
 def test_attention_query_range(pk, dh, ty):
@@ -795,6 +814,25 @@ def test_attention_long_sums_in_parts(pk, kind, dh, ty, total, n):
         # (the sums may drop an eighth of the output's rounding, eps / 16, of what they add up)
         lim = attn_bound(q, want, absv, dots, dh) + absv * torch.finfo(DT[ty]).eps / 16 + total * 2.0 ** -30 * most
         assert ((got[t].double() - want).abs() <= lim).all(), (t, ((got[t].double() - want).abs() / lim).max().item())
+
+
+@pytest.mark.parametrize("ty,heads", [("f32", 2), ("f32", 32), ("f16", 2), ("bf16", 32)])
+def test_attention_mask_of_few_words(pk, ty, heads):
+    """New tokens past the mask's words are seen by none; sequences share the pages of a prefix; the output may be the
+    query itself."""
+    lens, n = [64, 64, 64], 100
+    su = Setup(pk, lens, [n] * 3, "q4", 2, 64, 16, seed=9)
+    su.fill(pk)
+    su.table[:, :4] = su.table[0, :4]
+    su.seqs = pk.KvSeqs(su.seqs.start, su.seqs.ctx, i32(su.table), su.n_tok, n, su.max_len)
+    q = randn((3 * n, heads, 64), 8, DT[ty])
+    see = torch.rand((3, n, n), generator=gen(3), device="cuda") < 0.5
+    mask = words_of([sum(1 << int(j) for j in r.nonzero()[:, 0].tolist() if j < 64) for s in range(3) for r in see[s]], 1)
+    see[:, :, 64:] = False
+    want = su.cache.attend(su.seqs, q, mask=mask)
+    check_attention(su, q, want, see=lambda s, n: see[s])
+    again = q.clone()
+    assert su.cache.attend(su.seqs, again, mask=mask, out=again) is again and torch.equal(again, want)
 
 
 def test_attention_repeats_bit_for_bit(pk):
