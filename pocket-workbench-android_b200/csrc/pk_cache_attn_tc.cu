@@ -434,6 +434,9 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
     // positions 16 (x & 3) .. of tile x >> 2, in units of 16 rows (a page is 16
     // positions or more): -1 where there is no page.  Such rows are read from
     // the cache's first, whose codes are as good as any (their scales are 0).
+    // All are read past L1: a prompt's chunks run in streams of their own, and
+    // while one stores rows, which this launch waits for, another's attention may
+    // have brought their lines, with the rows as they were, into this SM's L1.
     int rows16 = -1;
     const uint8_t *codes = reinterpret_cast<const uint8_t *>(is_v ? a.c.v : a.c.k);
     const uint32_t *subs_of = reinterpret_cast<const uint32_t *>(is_v ? a.c.vs : a.c.ks);
@@ -449,13 +452,13 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
 #pragma unroll
       for (int w = 0; w < NP; w++) {
         const uint32_t r = max(__shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + w * (RP / 16) + key0 / 16), 0);
-        raw[w] = __ldg(reinterpret_cast<const uint4 *>(codes + ((size_t)r * (16 * RB) + ((key0 & 15) * RB + 16 * sub))));
-        if (TYPE == PK_KV_Q4) subs[w] = __ldg(subs_of + ((size_t)r * (16 * SW) + ((key0 & 15) * SW + 1)));
+        raw[w] = __ldcg(reinterpret_cast<const uint4 *>(codes + ((size_t)r * (16 * RB) + ((key0 & 15) * RB + 16 * sub))));
+        if (TYPE == PK_KV_Q4) subs[w] = __ldcg(subs_of + ((size_t)r * (16 * SW) + ((key0 & 15) * SW + 1)));
       }
       if (!is_v) {
         const int r = __shfl_sync(0xffffffffu, rows16, 4 * (i & 7) + key / 16);
         on = r >= 0 && u.lo + NK * i + key < hi;
-        d = __ldg(d_of + ((size_t)max(r, 0) * (16 * SW) + (key & 15) * SW));
+        d = __ldcg(d_of + ((size_t)max(r, 0) * (16 * SW) + (key & 15) * SW));
       }
     };
     auto put = [&](uint32_t dst) {
