@@ -102,8 +102,8 @@ def _dtype(t, who):
 
 
 def _call(fn, device, stream, used, *args):
-    """fn(*args, stream) on device number `device`; used: the call's tensors and lists of them, which may be freed before
-    a stream that is not the current one has come to the call."""
+    """fn(*args, stream) on device number `device`; used: with a stream given, the call's tensors and lists of them,
+    which may be freed before that stream has come to the call."""
     if stream is None and current_device() == device:
         rc = fn(*args, raw_stream(device))
     else:
@@ -150,7 +150,7 @@ def _mask(t, rows, device):
 
 def _same_strides(k, v):
     """Of tensors of one shape; what steps a dimension of size 1 has means nothing."""
-    return k.stride() == v.stride() or all(a == b or n == 1 for a, b, n in zip(k.stride(), v.stride(), k.shape))
+    return all(a == b or n == 1 for a, b, n in zip(k.stride(), v.stride(), k.shape))
 
 
 def _like(x):
@@ -220,14 +220,14 @@ class KvCache:
             _bad(f"{who}: the sequences are on another device")
         if k.shape != shape or v.shape != shape:
             _bad(f"{who}: k and v must be {shape}")
-        if k.dtype != v.dtype or k.get_device() != self.device or v.get_device() != self.device or not _same_strides(k, v) or st[2] != 1:
+        if k.dtype != v.dtype or k.get_device() != self.device or v.get_device() != self.device or (v.stride() != st and not _same_strides(k, v)) or st[2] != 1:
             _bad(f"{who}: k and v must be on the cache's device and share type and strides, with contiguous heads")
         return _dtype(k, who), st[0], st[1]
 
     def store(self, seqs: KvSeqs, k, v, stream=None):
         """Quantises rows k, v [n_tok, n_kv, head_dim] of the new tokens into the cache.  k and v have the same strides:
         those of one fused projection do, also after rope() in place (out_q, out_k)."""
-        _call(_L.pk_kv_store, self.device, stream, (self.tensors, seqs.tensors, k, v), self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "store"))
+        _call(_L.pk_kv_store, self.device, stream, stream is not None and (self.tensors, seqs.tensors, k, v), self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "store"))
 
     def load(self, seqs: KvSeqs, dtype=None, out=None, stream=None):
         """(k, v) [n_tok, n_kv, head_dim] of positions ctx .. read back; rows that no sequence has keep what they held."""
@@ -237,7 +237,7 @@ class KvCache:
             make = lambda: torch.empty_strided(shape, st, dtype=dt, device=dev)  # noqa: E731
             out = (make(), make()) if stream is None else _new(lambda: (make(), make()), self.device, stream)
         k, v = out
-        _call(_L.pk_kv_load, self.device, stream, (self.tensors, seqs.tensors, k, v), self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "load"))
+        _call(_L.pk_kv_load, self.device, stream, stream is not None and (self.tensors, seqs.tensors, k, v), self.ref, seqs.ref, k.data_ptr(), v.data_ptr(), *self._rows(seqs, k, v, "load"))
         return k, v
 
     def keep(self, seqs: KvSeqs, keep, n_keep, stream=None):
@@ -246,7 +246,7 @@ class KvCache:
         _i32(n_keep, self.device, "n_keep", 1)
         if keep.shape[0] != seqs.n_seq or n_keep.shape[0] != seqs.n_seq or seqs.device != self.device:
             _bad("keep: one row and one count a sequence, on the cache's device")
-        _call(_L.pk_kv_keep, self.device, stream, (self.tensors, seqs.tensors, keep, n_keep), self.ref, seqs.ref, keep.data_ptr(), keep.shape[1], n_keep.data_ptr())
+        _call(_L.pk_kv_keep, self.device, stream, stream is not None and (self.tensors, seqs.tensors, keep, n_keep), self.ref, seqs.ref, keep.data_ptr(), keep.shape[1], n_keep.data_ptr())
 
     def attend(self, seqs: KvSeqs, q, mask=None, scale: float | None = None, out=None, scratch=None, stream=None):
         """Attention of the new tokens q [n_tok, n_head, head_dim] over the cache; mask: int64 [n_tok, words], bit j of
@@ -261,7 +261,7 @@ class KvCache:
             out = _like(q) if stream is None else _new(lambda: _like(q), dev, stream)
         elif out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or out.stride(2) != 1:
             _bad("attend: out must be as q")
-        ptr, size = None, seqs.scratch.get((shape[1], code) + self.shape)
+        ptr, size = None, seqs.scratch.get((shape[1], code, self.shape))
         if size is None:
             size = self.attend_scratch_bytes(seqs, shape[1], q.dtype)
         if scratch is not None:
@@ -275,14 +275,14 @@ class KvCache:
         o = out.stride()
         args = PACK_QUERY(q.data_ptr(), out.data_ptr(), bits, s[0], s[1], o[0], o[1], code, shape[1], words,
                           self.head_dim ** -0.5 if scale is None else scale)
-        _call(_L.pk_kv_attn, dev, stream, (self.tensors, seqs.tensors, q, mask, out, scratch), self.ref, seqs.ref, args, ptr, size)
+        _call(_L.pk_kv_attn, dev, stream, stream is not None and (self.tensors, seqs.tensors, q, mask, out, scratch), self.ref, seqs.ref, args, ptr, size)
         return out
 
     def attend_scratch_bytes(self, seqs: KvSeqs, n_head: int, dtype) -> int:
         """Bytes of scratch that attend() needs (0: none); kept with the sequences, whose bounds do not change."""
         code = _type_of[dtype]
         n = _L.pk_kv_attn_scratch_bytes(self.ref, seqs.ref, n_head, code)
-        seqs.scratch[(n_head, code) + self.shape] = n
+        seqs.scratch[n_head, code, self.shape] = n
         return n
 
 
@@ -348,7 +348,7 @@ def rope(table: RopeTable, pos, q, k=None, layout: str = "interleaved", out_q=No
         kt, kp, kq, nk = out_k.stride(), k.data_ptr(), out_k.data_ptr(), kshape[1]
     args = PACK_ROPE(q.data_ptr(), kp, out_q.data_ptr(), kq, pos.data_ptr(), table.turns.data_ptr(), qs[0], qs[1], ks[0], ks[1], qt[0],
                      qt[1], kt[0], kt[1], code, pairs, n, shape[1], nk, dh, table.n_rot, table.gain)
-    _call(_L.pk_rope, dev, stream, (table.turns, pos, q, k, out_q, out_k), args)
+    _call(_L.pk_rope, dev, stream, stream is not None and (table.turns, pos, q, k, out_q, out_k), args)
     return out_q, out_k
 
 
@@ -396,6 +396,6 @@ def logit_rules(logits, repeat=None, freq=None, presence=None, hist=None, n_hist
     args = PACK_RULES(_row_value(repeat, "repeat", f, rows, dev), _row_value(freq, "freq", f, rows, dev),
                       _row_value(presence, "presence", f, rows, dev), hp, _row_value(n_hist, "n_hist", i, rows, dev), ip, bp, ap,
                       hs, bs, as_, hn, bn)
-    _call(_L.pk_apply_logit_rules, dev, stream, (logits, out, repeat, freq, presence, hist, n_hist, bias_id, bias, allow), logits.data_ptr(), out.data_ptr(), code, rows, n, st[0] if len(st) == 2 else n,
+    _call(_L.pk_apply_logit_rules, dev, stream, stream is not None and (logits, out, repeat, freq, presence, hist, n_hist, bias_id, bias, allow), logits.data_ptr(), out.data_ptr(), code, rows, n, st[0] if len(st) == 2 else n,
           out.stride(0) if len(st) == 2 else n, args)
     return out
