@@ -611,6 +611,7 @@ int Engine::setup_decode() {
 // tensor-core matvecs and attention (a bounded wait in one of their CTAs ran
 // out), read and cleared.
 int Engine::check_tc_error() {
+  PK_CK(cudaSetDevice(device_));  // (the word is a symbol, one a device)
   const int t = mv_tc_error(true);
   if (t == PK_ERR_TIMEOUT) return set_error(PK_ERR_TIMEOUT, "a bounded wait of a tensor-core matvec or attention ran out");
   if (t) return set_error(t, "reading the tensor-core kernels' error word");
