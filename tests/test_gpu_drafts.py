@@ -302,6 +302,22 @@ def test_cache_beyond_4_gib(pk):
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("kind,n_pages", [("q8", 80000), ("q4", 160000)])
+def test_attention_of_many_rows_beyond_4_gib(pk, kind, n_pages):
+    """The same for many query rows a kv head, whose codes and scales are read by another kernel."""
+    at = [n_pages - 1, n_pages - 2, 1, n_pages - 3]
+    cache, small = (pk.KvCache.empty(n, 64, 8, 128, kind) for n in (n_pages, 4))
+    k, v = randn((243, 8, 128), 1), randn((243, 8, 128), 2)
+    for c, pages in ((cache, at), (small, [0, 1, 2, 3])):
+        c.store(pk.KvSeqs(i32([0, 243]), i32([0]), i32([pages]), 243, 243, 243), k, v)
+    for ty in ("f16", "f32"):
+        q = randn((43, 8, 128), 6, DT[ty])
+        got, want = (c.attend(pk.KvSeqs(i32([0, 43]), i32([200]), i32([p]), 43, 43, 243), q) for c, p in ((cache, at), (small, [0, 1, 2, 3])))
+        assert torch.equal(got, want)
+        got = cache.load(pk.KvSeqs(i32([0, 43]), i32([200]), i32([at]), 43, 43, 243))
+        assert torch.equal(got[0], stored(k, kind)[200:]) and torch.equal(got[1], stored(v, kind)[200:])
+
+
 # ---------------------------------------------------------------- attention
 
 SHAPES = [
