@@ -417,6 +417,63 @@ size_t pk_kv_attn_scratch_bytes(const pk_kv_cache *cache, const pk_kv_seqs *seqs
 int pk_kv_attn(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const pk_kv_query *query, void *scratch,
                size_t scratch_bytes, void *stream);
 
+/* The same attention where sequences share a prefix, which is read and
+ * multiplied once for all of them.  Group g is the sequences first[g] ..
+ * first[g + 1] - 1, whose first len[g] positions hold the same K and V; they
+ * are read from the pages of sequence first[g], and whatever pages the others
+ * have there is not looked at (of the last len[g] % 16 of them each reads its
+ * own).  first ascends within 0 .. n_seq; a sequence of no group, or with fewer
+ * committed positions than its group shares, is computed by itself, and so are
+ * all of a group that has more new tokens than max_tok.  len is cut to max_len.
+ * max_own bounds a sequence's positions besides the shared ones (all of one
+ * that is computed by itself), new ones included; what is beyond is left out.
+ * The result is pk_kv_attn's up to rounding: the order of sums differs. */
+typedef struct {
+  const int *first;  /* device, [n_group + 1] */
+  const int *len;    /* device, [n_group] */
+  int n_group, max_tok, max_len, max_own;
+} pk_kv_shared;
+size_t pk_kv_attn_shared_scratch_bytes(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const pk_kv_shared *shared,
+                                       int n_head, int type);
+int pk_kv_attn_shared(const pk_kv_cache *cache, const pk_kv_seqs *seqs, const pk_kv_shared *shared,
+                      const pk_kv_query *query, void *scratch, size_t scratch_bytes, void *stream);
+
+/* Page tables and slot maps of a step, from the requests' lengths (device
+ * arrays; no host copy, one launch).  Slot s of n_seq has ctx[s] committed
+ * positions and gets n_new[s] tokens; it holds held[s] pages, pages[s][0 ..
+ * held[s]), of which the first shared[s] are others' too.  `free` lists the
+ * pages that nobody holds, n_free of them.
+ *   A slot with done[s] != 0 gives its pages back: those from shared[s] on
+ *   follow the list in the slots' and their own order, its held pages' entries
+ *   become -1.  It gets no tokens.  Nor does one with a negative ctx, which
+ *   keeps its pages.
+ *   start: the new tokens before each slot's, at most n_tok.
+ *   A slot with new tokens takes the pages that ctx + its tokens need besides
+ *   those that it holds (max_pages at most), in the slots' order, each the
+ *   list's last.  Where the list has no more, held grows by fewer, the entries
+ *   become -1 and lacking counts them: what is stored there is dropped.
+ *   pos, seq, slot of token t: its position, its slot s, and page * page_size +
+ *   position % page_size (-1: no page).  Rows behind the last token: 0, -1, -1.
+ * Of the list, entries taken become -1 (those of pages given back and not
+ * taken again follow what is left).  Negative counts mean 0, held more than
+ * max_pages that, shared more than held that.  The lists and tables that are
+ * not written stay as they are.
+ * Outputs may be the inputs they follow, all of pages, held, free and n_free or
+ * none; else they do not overlap.  A list longer than free_cap is cut.
+ * n_seq is at most 16384. */
+typedef struct {
+  const int *ctx, *n_new;             /* [n_seq] */
+  const int *pages, *held;            /* [n_seq][max_pages], [n_seq] */
+  const int *free, *n_free;           /* [free_cap], [1] */
+  const int *done, *shared;           /* [n_seq], or null: none */
+  int *pages_out, *held_out, *free_out, *n_free_out;
+  int *start, *lacking;               /* [n_seq + 1], [1] */
+  int *pos, *seq;                     /* [n_tok], or null */
+  int64_t *slot;                      /* [n_tok], or null */
+  int n_seq, max_pages, free_cap, n_tok, page_size;
+} pk_kv_plan_args;
+int pk_kv_plan(const pk_kv_plan_args *args, void *stream);
+
 /* Rotary positions.  pk_rope_turns (host code) writes the n_rot / 2 pairs'
  * turns a position, theta^(-2 i / n_rot) / (2 pi) in double, and the gain of
  * the rotated values; the caller keeps the table in device memory.  Scaling
@@ -480,6 +537,35 @@ typedef struct {
 } pk_logit_rules;
 int pk_apply_logit_rules(const void *logits, void *out, int type, int rows, int n, int64_t in_stride,
                          int64_t out_stride, const pk_logit_rules *rules, void *stream);
+
+/* A token for every row of logits [rows][n], from given random numbers u.  With
+ * w_t = exp((x_t - max x) / temp):
+ *   order   larger logits first, of equal ones the lower index
+ *   kept    the tokens with w_t >= min_p (at least the first); of these the first
+ *           top_k; of these the shortest run from the first on that has top_p of
+ *           the weight of all of them (at least the first)
+ *   tok     the first kept token, by index, up to which the kept weights come
+ *           to more than u times their sum
+ *   prob    its share of the kept weights
+ *   kept    how many tokens were kept
+ * Weights and sums are 64-bit (fixed-point sums, so that no order of additions
+ * changes a token): weights below 2^-44 of the largest (2^-32 at 2^30 tokens)
+ * may count as nothing.  temp <= 0 keeps the first token alone.  -inf and NaN are
+ * never kept; a row of nothing else gives tok -1, prob 0, kept 0.  Where +inf
+ * stands, +inf alone has weight.  NaN settings mean: temp 0, top_p 1, min_p 0.
+ * No scratch, no rng: u in [0, 1) is the caller's (below 0 and NaN count as 0,
+ * 1 and above as the largest number below 1). */
+typedef struct {
+  const float *u;     /* [rows] */
+  const float *temp;  /* [rows], or null: 1 */
+  const int *top_k;   /* [rows], or null; <= 0: all */
+  const float *top_p; /* [rows], or null; >= 1: all */
+  const float *min_p; /* [rows], or null; <= 0: all */
+  int *tok;           /* [rows] */
+  float *prob;        /* [rows], or null */
+  int *kept;          /* [rows], or null */
+} pk_sample_args;
+int pk_sample_rows(const void *logits, int type, int rows, int n, int64_t stride, const pk_sample_args *args, void *stream);
 
 /* ------------------------------------------------- tensor-parallel decode
  * No reference counterpart: the reference runs one engine per process on the

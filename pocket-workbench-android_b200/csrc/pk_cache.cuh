@@ -89,21 +89,23 @@ __device__ __forceinline__ SeqView seq_view(const pk_kv_seqs &q, int page_size, 
   v.total = c < 0 ? 0 : (int)min((long long)c + v.n, cap);
   return v;
 }
-// The sequence that token row t belongs to (the last s with start[s] <= t), by
-// a whole warp: 32 probes a level.  -1 when t lies before the first.
-__device__ __forceinline__ int seq_of(const pk_kv_seqs &q, int t, int lane) {
-  int lo = 0, len = q.n_seq;  // start[lo .. lo + len) holds the answer
+// The last i < n with at[i] <= t, by a whole warp: 32 probes a level.  -1 when
+// t lies before the first.
+__device__ __forceinline__ int last_at(const int *at, int n, int t, int lane) {
+  int lo = 0, len = n;  // at[lo .. lo + len) holds the answer
   while (len > 1) {
     const int step = (len + 31) / 32, i = lo + lane * step;
-    const bool le = lane * step < len && __ldg(q.start + i) <= t;
+    const bool le = lane * step < len && __ldg(at + i) <= t;
     const int n = __popc(__ballot_sync(0xffffffffu, le));
     if (n == 0) return -1;
     const int adv = (n - 1) * step;
     lo += adv;
     len = min(step, len - adv);
   }
-  return __ldg(q.start + lo) <= t ? lo : -1;
+  return __ldg(at + lo) <= t ? lo : -1;
 }
+// The sequence that token row t belongs to (the last s with start[s] <= t).
+__device__ __forceinline__ int seq_of(const pk_kv_seqs &q, int t, int lane) { return last_at(q.start, q.n_seq, t, lane); }
 // Index of the cache row of (position p, kv head h), or -1 where there is no page.
 __device__ __forceinline__ long long row_at(const pk_kv_cache &c, const pk_kv_seqs &q, int s, int p, int h) {
   const int j = p / c.page_size;

@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
   pdl_wait();
   const Unit u = unit_of(a);
   const int tile0 = u.rt * G::ROWS;
-  if (tile0 >= u.rows || (u.ch >= max(u.nch, 1) && !(a.cluster && u.nch > 1))) return;
+  if (idle(a, u, tile0)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int rg = warp % RG, kg = warp / RG, row0 = tile0 + rg * 8 * NB;
   // without a mask nobody sees past the tile's last token
@@ -579,17 +579,17 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
       if (d0 == 0) sfin[r] = make_float2(M, L);
       continue;
     }
-    if (u.nch > 1) {
+    if (u.part) {
       if (d0 == 0) {
         const int i = (tile0 + r) / a.group, h = u.h * a.group + (tile0 + r) - i * a.group;
-        a.part_ml[((long long)(u.sv.first + i) * a.q.n_head + h) * a.n_chunk + u.ch] = make_float2(M, L);
+        a.part_ml[((long long)(u.sv.first + i) * a.q.n_head + h) * a.n_part + u.slot] = make_float2(M, L);
       }
     } else {
       const float inv = L > 0.0f || isnan(L) ? 1.0f / L : 0.0f;
 #pragma unroll
       for (int j = 0; j < DH / 8; j++) acc[j] *= inv;
     }
-    write_row<DH>(a, u, tile0 + r, d0, acc, u.nch > 1);
+    write_row<DH>(a, u, tile0 + r, d0, acc, u.part);
   }
   if (cluster) join_cluster<DH>(a, u, tile0, G::ROWS, shaddr(so), shaddr(sfin), 32 * AW);
 }
@@ -613,12 +613,21 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) k_kv_attn_join(const At
   const int s = seq_of(a.s, (int)tok, lane);
   if (s < 0) return;
   const SeqView sv = seq_view(a.s, a.c.page_size, s);
-  const int nch = (sv.total + a.chunk - 1) / a.chunk;
-  if (tok - sv.first >= sv.n || nch <= 1) return;
-  const float2 *ml = a.part_ml + row * a.n_chunk;
-  const float *po = a.part_o + row * a.n_chunk * DH + V * lane;
+  int nch = (sv.total + a.chunk - 1) / a.chunk, npre = 0;
+  if (tok - sv.first >= sv.n) return;
+  if (a.mode == ATTN_OWN) {
+    const OwnView v = own_view(a, s, sv);
+    npre = (v.base + a.pre_chunk - 1) / a.pre_chunk;
+    nch = npre + (v.total - v.base + a.chunk - 1) / a.chunk;
+  } else if (nch <= 1) {
+    return;
+  }
+  // (parts npre .. are the row's own, which lie from n_pre on)
+  const float2 *ml = a.part_ml + row * a.n_part;
+  const float *po = a.part_o + row * a.n_part * DH + V * lane;
+  auto at = [&](int c) { return c < npre ? c : c - npre + a.n_pre; };
   float M = -CUDART_INF_F;
-  for (int c = w + W * lane; c < nch; c += 32 * W) M = fmaxf(M, ml[c].x);
+  for (int c = w + W * lane; c < nch; c += 32 * W) M = fmaxf(M, ml[at(c)].x);
 #pragma unroll
   for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
   float L = 0.0f, acc[V];
@@ -629,7 +638,7 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) k_kv_attn_join(const At
     float v[4][V];
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      const int c = min(c0 + k * W, nch - 1);
+      const int c = at(min(c0 + k * W, nch - 1));
       x[k] = ml[c];
       if (V == 4) *reinterpret_cast<float4 *>(v[k]) = *reinterpret_cast<const float4 *>(po + (size_t)c * DH);
       else *reinterpret_cast<float2 *>(v[k]) = *reinterpret_cast<const float2 *>(po + (size_t)c * DH);
@@ -736,7 +745,8 @@ struct Split {
   bool cluster;
   bool parts;  // partial results go through the scratch
 };
-Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type, const Variant &v) {
+// parts: through the scratch in any case.
+Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type, const Variant &v, bool parts = false) {
   Split p;
   const long long rows = (long long)s.max_new * (n_head / c.n_kv);
   p.row_tiles = (int)((rows + v.rows - 1) / v.rows);
@@ -755,11 +765,11 @@ Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type, 
     }
   }
   const long long slots = v.rows == 256 ? 128 : 296;  // CTAs that run at once, in clusters too
-  if (v.k && n > 8 && n <= 16 && least <= 8 && units * 8 <= slots) n = 8;
+  if (!parts && v.k && n > 8 && n <= 16 && least <= 8 && units * 8 <= slots) n = 8;
   p.chunk = (int)(((s.max_len + n - 1) / n + 63) / 64 * 64);
   p.n_chunk = (int)((s.max_len + (long long)p.chunk - 1) / p.chunk);
-  p.cluster = p.n_chunk > 1 && p.n_chunk <= 8 && units * p.n_chunk <= slots;
-  p.parts = (p.n_chunk > 1 && !p.cluster) || (!v.k && type != T_F32 && p.chunk > sum);
+  p.cluster = !parts && p.n_chunk > 1 && p.n_chunk <= 8 && units * p.n_chunk <= slots;
+  p.parts = parts || (p.n_chunk > 1 && !p.cluster) || (!v.k && type != T_F32 && p.chunk > sum);
   return p;
 }
 
@@ -785,34 +795,114 @@ bool kv_attn_waits(const pk_kv_cache &c, const pk_kv_seqs &seqs, int n_head, int
   return !variant_of(c, bounded(c, seqs), n_head, type).k;
 }
 
-cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &seqs, const pk_kv_query &q, void *scratch,
-                           cudaStream_t st, int *err, bool poison) {
-  const pk_kv_seqs s = bounded(c, seqs);
-  const Variant v = variant_of(c, s, q.n_head, q.type);
-  const Split p = split_of(c, s, q.n_head, q.type, v);
+// What the launches of a call share.
+static AttnKArgs args_of(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_query &q) {
   AttnKArgs a{};
   a.c = c; a.s = s; a.q = q;
-  a.chunk = p.chunk; a.n_chunk = p.n_chunk; a.row_tiles = p.row_tiles;
   a.group = q.n_head / c.n_kv;
   while ((1 << a.page_shift) < c.page_size) a.page_shift++;
   const uintptr_t es = q.type == T_F32 ? 4 : 2;
   a.vec_q = (((uintptr_t)q.q | (uintptr_t)q.q_tok_stride * es | (uintptr_t)q.q_head_stride * es) & 15) == 0;
   a.vec_o = (((uintptr_t)q.out | (uintptr_t)q.out_tok_stride * es | (uintptr_t)q.out_head_stride * es) & 15) == 0;
-  const size_t rows = (size_t)s.n_tok * q.n_head;
-  a.part_o = reinterpret_cast<float *>(scratch);
+  return a;
+}
+// units: sequences, or groups of them.
+static cudaError_t launch_parts(AttnKArgs &a, const Variant &v, const Split &p, int units, cudaStream_t st) {
+  a.chunk = p.chunk; a.n_chunk = p.n_chunk; a.row_tiles = p.row_tiles;
   a.cluster = p.cluster;
+  const long long blocks = (long long)units * a.c.n_kv * p.row_tiles * p.n_chunk;
+  if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+  const int cluster = a.cluster ? p.n_chunk : 1;
+  if (!v.k) return launch_kv_attn_tc(a, cluster, (unsigned)blocks, st);
+  return launch_cluster(v.k, cluster, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
+}
+static cudaError_t launch_join(const AttnKArgs &a, cudaStream_t st) {
+  const size_t rows = (size_t)a.s.n_tok * a.q.n_head;
+  if (a.n_part <= 8)
+    return launch(a.c.head_dim == 64 ? k_kv_attn_join<64, 1> : k_kv_attn_join<128, 1>, dim3((unsigned)((rows + 3) / 4)), dim3(128), 0, st, a);
+  return launch(a.c.head_dim == 64 ? k_kv_attn_join<64, 8> : k_kv_attn_join<128, 8>, dim3((unsigned)rows), dim3(256), 0, st, a);
+}
+
+cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &seqs, const pk_kv_query &q, void *scratch,
+                           cudaStream_t st, int *err, bool poison) {
+  const pk_kv_seqs s = bounded(c, seqs);
+  const Variant v = variant_of(c, s, q.n_head, q.type);
+  const Split p = split_of(c, s, q.n_head, q.type, v);
+  AttnKArgs a = args_of(c, s, q);
+  const size_t rows = (size_t)s.n_tok * q.n_head;
+  if (rows > 0x7fffffff) return cudaErrorInvalidValue;
+  a.n_part = p.n_chunk;
+  a.part_o = reinterpret_cast<float *>(scratch);
+  a.part_ml = p.parts ? reinterpret_cast<float2 *>(a.part_o + rows * p.n_chunk * c.head_dim) : nullptr;
   a.err = err;
   a.poison = poison;
-  a.part_ml = p.parts ? reinterpret_cast<float2 *>(a.part_o + rows * p.n_chunk * c.head_dim) : nullptr;
-  const long long blocks = (long long)s.n_seq * c.n_kv * p.row_tiles * p.n_chunk, jb = ((long long)rows + 3) / 4;
-  if (blocks > 0x7fffffffLL || (long long)rows > 0x7fffffffLL) return cudaErrorInvalidValue;
-  const int cluster = a.cluster ? p.n_chunk : 1;
-  cudaError_t e;
-  if (!v.k) e = launch_kv_attn_tc(a, cluster, (unsigned)blocks, st);
-  else e = launch_cluster(v.k, cluster, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
-  if (e != cudaSuccess || p.n_chunk <= 1 || a.cluster) return e;
-  if (p.n_chunk <= 8) return launch(c.head_dim == 64 ? k_kv_attn_join<64, 1> : k_kv_attn_join<128, 1>, dim3((unsigned)jb), dim3(128), 0, st, a);
-  return launch(c.head_dim == 64 ? k_kv_attn_join<64, 8> : k_kv_attn_join<128, 8>, dim3((unsigned)rows), dim3(256), 0, st, a);
+  const cudaError_t e = launch_parts(a, v, p, s.n_seq, st);
+  return e != cudaSuccess || p.n_chunk <= 1 || a.cluster ? e : launch_join(a, st);
+}
+
+// Shared prefixes: the groups as sequences of their tokens over the positions
+// that they share, then each sequence over the rest of its own, and a launch
+// that joins the parts.
+namespace {
+struct Shared {
+  pk_kv_seqs pre, own;  // bounds of the two
+  Variant pre_v, own_v;
+  Split pre_p, own_p;
+};
+Shared shared_plan(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_shared &sh, int n_head, int type) {
+  Shared x;
+  x.pre = x.own = s;
+  x.pre.n_seq = sh.n_group;
+  x.pre.max_new = std::min(sh.max_tok, s.n_tok);
+  x.pre.max_len = std::min(sh.max_len, s.max_len) & ~15;
+  // (and up to 15 of a shared length that is no multiple of 16)
+  x.own.max_len = (int)std::min((long long)sh.max_own + 15, (long long)s.max_len);
+  x.pre_p = x.own_p = Split{};
+  if (x.pre.n_seq > 0 && x.pre.max_new > 0 && x.pre.max_len > 0) {
+    x.pre_v = variant_of(c, x.pre, n_head, type);
+    x.pre_p = split_of(c, x.pre, n_head, type, x.pre_v, true);
+  }
+  if (x.own.max_len > 0) {
+    x.own_v = variant_of(c, x.own, n_head, type);
+    x.own_p = split_of(c, x.own, n_head, type, x.own_v, true);
+  }
+  return x;
+}
+}  // namespace
+
+size_t kv_attn_shared_scratch_bytes(const pk_kv_cache &c, const pk_kv_seqs &seqs, const pk_kv_shared &sh, int n_head, int type) {
+  const pk_kv_seqs s = bounded(c, seqs);
+  const Shared x = shared_plan(c, s, sh, n_head, type);
+  return (size_t)s.n_tok * n_head * (x.pre_p.n_chunk + x.own_p.n_chunk) * (c.head_dim + 2) * sizeof(float);
+}
+
+cudaError_t launch_kv_attn_shared(const pk_kv_cache &c, const pk_kv_seqs &seqs, const pk_kv_shared &sh, const pk_kv_query &q,
+                                  void *scratch, cudaStream_t st) {
+  const pk_kv_seqs s = bounded(c, seqs);
+  const Shared x = shared_plan(c, s, sh, q.n_head, q.type);
+  const size_t rows = (size_t)s.n_tok * q.n_head;
+  if (rows > 0x7fffffff) return cudaErrorInvalidValue;
+  AttnKArgs a = args_of(c, s, q);
+  a.sh = sh;
+  if (x.pre_p.n_chunk == 0) a.sh.n_group = 0;
+  a.n_pre = x.pre_p.n_chunk;
+  a.pre_chunk = std::max(x.pre_p.chunk, 1);
+  a.n_part = a.n_pre + x.own_p.n_chunk;
+  a.part_o = reinterpret_cast<float *>(scratch);
+  a.part_ml = reinterpret_cast<float2 *>(a.part_o + rows * a.n_part * c.head_dim);
+  cudaError_t e = cudaSuccess;
+  if (a.n_pre > 0) {
+    AttnKArgs b = a;
+    b.mode = ATTN_PREFIX;
+    b.q.mask = nullptr;
+    e = launch_parts(b, x.pre_v, x.pre_p, sh.n_group, st);
+    if (e != cudaSuccess) return e;
+  }
+  a.mode = ATTN_OWN;
+  a.part0 = a.n_pre;
+  a.chunk = 64;
+  if (x.own_p.n_chunk > 0) e = launch_parts(a, x.own_v, x.own_p, s.n_seq, st);
+  return e != cudaSuccess ? e : launch_join(a, st);
 }
 
 }  // namespace pk

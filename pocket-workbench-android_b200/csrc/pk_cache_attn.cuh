@@ -50,20 +50,61 @@ struct AttnKArgs {
   pk_kv_cache c;
   pk_kv_seqs s;
   pk_kv_query q;
-  float *part_o;   // [n_tok][n_head][n_chunk][DH]: chunks' parts, or what long sums gave up so far
-  float2 *part_ml; // [n_tok][n_head][n_chunk]
+  float *part_o;   // [n_tok][n_head][n_part][DH]: chunks' parts, or what long sums gave up so far
+  float2 *part_ml; // [n_tok][n_head][n_part]
   int chunk, n_chunk, row_tiles, group, page_shift, vec_q, vec_o;
   int cluster;  // 1: a sequence's chunks are a cluster's CTAs, which add up among themselves
   int *err;     // null, or a device word that PK_ERR_TIMEOUT goes to when a bounded wait ran out
   int poison;   // 1 (self-test): the codes never arrive, so that the waits run out
+  // What a launch goes over: all of each sequence, each group's shared prefix,
+  // or what each sequence has besides it.  The last two leave their chunks'
+  // parts in the scratch, a row's n_part of them: the prefix's from 0 on, its
+  // own from n_pre on.
+  int mode, part0, n_part, n_pre, pre_chunk;
+  pk_kv_shared sh;
 };
+enum : int { ATTN_ALL = 0, ATTN_PREFIX = 1, ATTN_OWN = 2 };
+
+// Group g's sequences [s0, s1), their tokens [t0, t0 + n), and the positions
+// that they share, of which `base`, a multiple of 16 as tiles are, are computed
+// for all; none (0) where the group has no tokens, or more than max_tok.
+struct GroupView {
+  int s0, s1, t0, n, len, base;
+};
+__device__ __forceinline__ GroupView group_view(const AttnKArgs &a, int g) {
+  GroupView v;
+  v.s0 = min(max(__ldg(a.sh.first + g), 0), a.s.n_seq);
+  v.s1 = min(max(__ldg(a.sh.first + g + 1), v.s0), a.s.n_seq);
+  v.t0 = min(max(__ldg(a.s.start + v.s0), 0), a.s.n_tok);
+  v.n = min(max(__ldg(a.s.start + v.s1), v.t0), a.s.n_tok) - v.t0;
+  const long long cap = min(min((long long)a.s.max_pages * a.c.page_size, (long long)a.s.max_len), (long long)a.sh.max_len);
+  v.len = (int)min((long long)max(__ldg(a.sh.len + g), 0), cap);
+  if (v.n < 1 || v.n > a.sh.max_tok) v.n = v.len = 0;
+  v.base = v.len & ~15;
+  return v;
+}
+// The positions of sequence s (a whole warp asks) that are left to itself: from
+// base, which its group's prefix reaches to, up to total.
+struct OwnView {
+  int base, total;
+};
+__device__ __forceinline__ OwnView own_view(const AttnKArgs &a, int s, const SeqView &sv) {
+  int base = 0, len = 0;
+  const int g = a.sh.n_group > 0 ? last_at(a.sh.first, a.sh.n_group, s, threadIdx.x & 31) : -1;
+  if (g >= 0) {
+    const GroupView v = group_view(a, g);
+    if (s >= v.s0 && s < v.s1 && sv.ctx >= v.len) base = v.base, len = v.len;
+  }
+  return {base, max(base, (int)min((long long)sv.total, (long long)len + a.sh.max_own))};
+}
 
 // A CTA's work: one chunk of positions [lo, hi) for one tile of the rows (token
 // i, query head of kv head h) of one sequence.  Sequences of more than one
 // chunk (nch) leave theirs in the scratch, or to the cluster.
 struct Unit {
   SeqView sv;
-  int s, h, rt, ch, lo, hi, nch, rows;
+  int s, h, rt, ch, lo, hi, nch, rows, slot;  // (slot: of its part among a row's)
+  bool part;
 };
 __device__ __forceinline__ Unit unit_of(const AttnKArgs &a) {
   Unit u;
@@ -75,12 +116,31 @@ __device__ __forceinline__ Unit unit_of(const AttnKArgs &a) {
   id /= (unsigned)a.row_tiles;
   u.h = (int)(id % (unsigned)a.c.n_kv);
   u.s = (int)(id / (unsigned)a.c.n_kv);
-  u.sv = seq_view(a.s, a.c.page_size, u.s);
+  int base = 0;
+  if (a.mode == ATTN_PREFIX) {
+    const GroupView g = group_view(a, u.s);
+    u.s = g.s0;  // (whose pages are read)
+    u.sv = SeqView{g.t0, g.n, g.base, g.base};
+  } else {
+    u.sv = seq_view(a.s, a.c.page_size, u.s);
+    if (a.mode == ATTN_OWN && u.sv.n > 0) {
+      const OwnView v = own_view(a, u.s, u.sv);
+      base = v.base;
+      u.sv.total = v.total;
+    }
+  }
   u.rows = u.sv.n * a.group;
-  u.nch = (u.sv.total + a.chunk - 1) / a.chunk;
-  u.lo = u.ch * a.chunk;
+  u.nch = (u.sv.total - base + a.chunk - 1) / a.chunk;
+  u.lo = base + u.ch * a.chunk;
   u.hi = min(u.sv.total, u.lo + a.chunk);
+  u.slot = a.part0 + u.ch;
+  u.part = a.mode != ATTN_ALL || u.nch > 1;
   return u;
+}
+// Has this CTA nothing to do?  (Rows that see nothing are written by their first chunk, or by the joining launch.)
+__device__ __forceinline__ bool idle(const AttnKArgs &a, const Unit &u, int tile0) {
+  if (tile0 >= u.rows) return true;
+  return u.ch >= (a.mode == ATTN_ALL ? max(u.nch, 1) : u.nch) && !(a.cluster && u.nch > 1);
 }
 
 // Does row (token i) see draft j?
@@ -118,7 +178,7 @@ __device__ __forceinline__ void write_row(const AttnKArgs &a, const Unit &u, int
   const int i = row / a.group, h = u.h * a.group + row - i * a.group;
   const long long tok = u.sv.first + i;
   if (part) {
-    float *p = a.part_o + ((tok * a.q.n_head + h) * a.n_chunk + u.ch) * DH + d0;
+    float *p = a.part_o + ((tok * a.q.n_head + h) * a.n_part + u.slot) * DH + d0;
 #pragma unroll
     for (int j = 0; j < DH / 8; j += 4) *reinterpret_cast<float4 *>(p + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
     return;

@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
   const Unit u = unit_of(a);
   const int tile0 = u.rt * ROWS;
   const bool cluster = a.cluster && u.nch > 1;
-  if (tile0 >= u.rows || (u.ch >= max(u.nch, 1) && !cluster)) {
+  if (idle(a, u, tile0)) {
     pdl_trigger();
     return;
   }
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
 #pragma unroll
         for (int j = 0; j < 2; j++) {
           const int row = tile0 + warp * 32 + (lane >> 2) + 16 * half + 8 * j, r = min(row, u.rows - 1), t = r / a.group;
-          const long long at = ((long long)(u.sv.first + t) * a.q.n_head + u.h * a.group + r - t * a.group) * a.n_chunk + u.ch;
+          const long long at = ((long long)(u.sv.first + t) * a.q.n_head + u.h * a.group + r - t * a.group) * a.n_part + u.slot;
           to[j] = a.part_o + at * DH + 2 * quad;
           const float before = i > SUM_TILES<E> ? a.part_ml[at].x : -CUDART_INF_F;
           g[j] = before == -CUDART_INF_F ? 0.0f : ex2(before - m[j]);
@@ -809,22 +809,22 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
     if (work) {
       const int i = tok, h = u.h * a.group + (min(row, u.rows - 1) - i * a.group);
       const long long at = u.sv.first + i;
-      const bool on = row < u.rows, part = u.nch > 1;
+      const bool on = row < u.rows, part = u.part;
       float f = 1.0f, g = 0.0f;  // g: of what a long sum has in the scratch
       if (LONG && nt > SUM_TILES<E> && on) {
-        const float before = a.part_ml[(at * a.q.n_head + h) * a.n_chunk + u.ch].x;
+        const float before = a.part_ml[(at * a.q.n_head + h) * a.n_part + u.slot].x;
         g = before == -CUDART_INF_F ? 0.0f : ex2(before - m);
       }
       if (*abort) f = l = CUDART_NAN_F;
       if (part) {
         if (on && cluster) *reinterpret_cast<float2 *>(smem + L::ML + tid * 8) = make_float2(m, l);
-        else if (on) a.part_ml[((at * a.q.n_head + h) * a.n_chunk) + u.ch] = make_float2(m, l);
+        else if (on) a.part_ml[((at * a.q.n_head + h) * a.n_part) + u.slot] = make_float2(m, l);
       } else {
         f *= l > 0.0f || isnan(l) ? 1.0f / l : 0.0f;
       }
       if (l == 0.0f) f = 0.0f;
       // (in a cluster: into shared memory, where the operands were)
-      float *po = !part ? nullptr : cluster ? reinterpret_cast<float *>(smem) + tid * (DH + 4) : a.part_o + ((at * a.q.n_head + h) * a.n_chunk + u.ch) * DH;
+      float *po = !part ? nullptr : cluster ? reinterpret_cast<float *>(smem) + tid * (DH + 4) : a.part_o + ((at * a.q.n_head + h) * a.n_part + u.slot) * DH;
       const long long off = at * a.q.out_tok_stride + (long long)h * a.q.out_head_stride;
 #pragma unroll
       for (int c = 0; c < DH / 16; c++) {
@@ -837,7 +837,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
           for (int j = 0; j < 16; j++) v[j] = 0.0f;
         }
         if (LONG && nt > SUM_TILES<E> && on) {
-          const float *p = a.part_o + ((at * a.q.n_head + h) * a.n_chunk + u.ch) * DH + 16 * c;
+          const float *p = a.part_o + ((at * a.q.n_head + h) * a.n_part + u.slot) * DH + 16 * c;
 #pragma unroll
           for (int j = 0; j < 16; j++) v[j] = fmaf(g, p[j], v[j]);
         }

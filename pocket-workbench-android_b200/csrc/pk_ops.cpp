@@ -1,5 +1,5 @@
-// pk_ops.cpp -- extern "C" entry points of the drafted-decoding operators
-// (include/pk.h): arguments are checked here, before anything is launched.
+// pk_ops.cpp -- extern "C" entry points of the drafted-decoding and serving
+// operators (include/pk.h): arguments are checked here, before anything is launched.
 #include <cuda_runtime.h>
 
 #include <cmath>
@@ -69,6 +69,39 @@ int check_rows(const char *who, const pk_kv_cache *c, const void *k, const void 
   return PK_OK;
 }
 
+int check_query(const char *who, const pk_kv_cache *c, const pk_kv_seqs *s, const pk_kv_query *q) {
+  const std::string w(who);
+  if (!q) return bad(w + ": null query");
+  if (!is_float_type(q->type)) return set_error(PK_ERR_UNSUPPORTED, w + ": element type " + std::to_string(q->type) + " is not f32, f16 or bf16");
+  if (q->n_head < 1 || q->n_head % c->n_kv) return bad(w + ": n_head must be a positive multiple of n_kv");
+  if (!(q->scale > 0.0f) || !std::isfinite(q->scale)) return bad(w + ": scale must be positive and finite");
+  if (q->mask && (q->mask_words < 1 || q->mask_words > 4096)) return bad(w + ": mask_words must be 1 to 4096 with a mask");
+  if (nothing(s)) return PK_OK;
+  if (!fits_grid(c, s, q->n_head)) return bad(w + ": n_tok * n_head and n_seq * n_kv are at most 2^31 - 1");
+  if (!q->q || !q->out) return bad(w + ": null q or out");
+  if (((uintptr_t)q->q | (uintptr_t)q->out) & elem_mask(q->type) || ((uintptr_t)q->mask & 7)) return bad(w + ": misaligned q, out or mask");
+  const int64_t st[4] = {q->q_tok_stride, q->q_head_stride, q->out_tok_stride, q->out_head_stride};
+  for (int64_t x : st)
+    if (x < 0 || x > (1LL << 40)) return bad(w + ": stride out of range");
+  if ((q->out_head_stride < c->head_dim && q->n_head > 1) || (q->out_tok_stride < c->head_dim && s->n_tok > 1))
+    return bad(w + ": out strides are less than head_dim");
+  return PK_OK;
+}
+int check_shared(const char *who, const pk_kv_seqs *s, const pk_kv_shared *sh) {
+  const std::string w(who);
+  if (!sh) return bad(w + ": null groups");
+  if (sh->n_group < 0 || sh->n_group > s->n_seq || sh->max_tok < 0 || sh->max_len < 0 || sh->max_own < 0)
+    return bad(w + ": negative count, or more groups than sequences");
+  if (sh->n_group > 0 && (!sh->first || !sh->len || (((uintptr_t)sh->first | (uintptr_t)sh->len) & 3)))
+    return bad(w + ": null or misaligned group array");
+  return PK_OK;
+}
+int check_scratch(const char *who, size_t need, const void *scratch, size_t bytes) {
+  if (need && (!scratch || bytes < need || ((uintptr_t)scratch & 15)))
+    return bad(std::string(who) + ": scratch must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
+  return PK_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -117,24 +150,72 @@ int pk_kv_attn(const pk_kv_cache *c, const pk_kv_seqs *s, const pk_kv_query *q, 
                void *stream) {
   if (int rc = check_cache("pk_kv_attn", c)) return rc;
   if (int rc = check_seqs("pk_kv_attn", s)) return rc;
-  if (!q) return bad("pk_kv_attn: null query");
-  if (!is_float_type(q->type)) return set_error(PK_ERR_UNSUPPORTED, "pk_kv_attn: element type " + std::to_string(q->type) + " is not f32, f16 or bf16");
-  if (q->n_head < 1 || q->n_head % c->n_kv) return bad("pk_kv_attn: n_head must be a positive multiple of n_kv");
-  if (!(q->scale > 0.0f) || !std::isfinite(q->scale)) return bad("pk_kv_attn: scale must be positive and finite");
-  if (q->mask && (q->mask_words < 1 || q->mask_words > 4096)) return bad("pk_kv_attn: mask_words must be 1 to 4096 with a mask");
+  if (int rc = check_query("pk_kv_attn", c, s, q)) return rc;
   if (nothing(s)) return PK_OK;
-  if (!fits_grid(c, s, q->n_head)) return bad("pk_kv_attn: n_tok * n_head and n_seq * n_kv are at most 2^31 - 1");
-  if (!q->q || !q->out) return bad("pk_kv_attn: null q or out");
-  if (((uintptr_t)q->q | (uintptr_t)q->out) & elem_mask(q->type) || ((uintptr_t)q->mask & 7)) return bad("pk_kv_attn: misaligned q, out or mask");
-  const int64_t st[4] = {q->q_tok_stride, q->q_head_stride, q->out_tok_stride, q->out_head_stride};
-  for (int64_t x : st)
-    if (x < 0 || x > (1LL << 40)) return bad("pk_kv_attn: stride out of range");
-  if ((q->out_head_stride < c->head_dim && q->n_head > 1) || (q->out_tok_stride < c->head_dim && s->n_tok > 1))
-    return bad("pk_kv_attn: out strides are less than head_dim");
   const size_t need = kv_attn_scratch_bytes(*c, *s, q->n_head, q->type);
-  if (need && (!scratch || scratch_bytes < need || ((uintptr_t)scratch & 15)))
-    return bad("pk_kv_attn: scratch must be 16-byte aligned and hold " + std::to_string(need) + " bytes");
+  if (int rc = check_scratch("pk_kv_attn", need, scratch, scratch_bytes)) return rc;
   CK(launch_kv_attn(*c, *s, *q, scratch, (cudaStream_t)stream));
+  return PK_OK;
+}
+
+size_t pk_kv_attn_shared_scratch_bytes(const pk_kv_cache *c, const pk_kv_seqs *s, const pk_kv_shared *sh, int n_head, int type) {
+  const char *who = "pk_kv_attn_shared_scratch_bytes";
+  if (check_cache(who, c) || check_seqs(who, s) || check_shared(who, s, sh)) return 0;
+  if (nothing(s) || n_head < 1 || n_head % c->n_kv || !is_float_type(type) || !fits_grid(c, s, n_head)) return 0;
+  return kv_attn_shared_scratch_bytes(*c, *s, *sh, n_head, type);
+}
+
+int pk_kv_attn_shared(const pk_kv_cache *c, const pk_kv_seqs *s, const pk_kv_shared *sh, const pk_kv_query *q, void *scratch,
+                      size_t scratch_bytes, void *stream) {
+  const char *who = "pk_kv_attn_shared";
+  if (int rc = check_cache(who, c)) return rc;
+  if (int rc = check_seqs(who, s)) return rc;
+  if (int rc = check_shared(who, s, sh)) return rc;
+  if (int rc = check_query(who, c, s, q)) return rc;
+  if (nothing(s)) return PK_OK;
+  const size_t need = kv_attn_shared_scratch_bytes(*c, *s, *sh, q->n_head, q->type);
+  if (int rc = check_scratch(who, need, scratch, scratch_bytes)) return rc;
+  CK(launch_kv_attn_shared(*c, *s, *sh, *q, scratch, (cudaStream_t)stream));
+  return PK_OK;
+}
+
+int pk_kv_plan(const pk_kv_plan_args *a, void *stream) {
+  if (!a) return bad("pk_kv_plan: null argument");
+  if (a->n_seq < 0 || a->n_seq > 16384 || a->n_tok < 0 || a->n_tok > (1 << 30) || a->max_pages < 0 || a->free_cap < 0)
+    return bad("pk_kv_plan: count out of range (n_seq at most 16384, n_tok 2^30)");
+  if ((int64_t)a->n_seq * a->max_pages > 0x7fffffff) return bad("pk_kv_plan: n_seq * max_pages is at most 2^31 - 1");
+  if (a->page_size < 16 || a->page_size > 65536 || (a->page_size & (a->page_size - 1)))
+    return bad("pk_kv_plan: page_size must be a power of two from 16 to 65536");
+  const bool seqs = a->n_seq > 0, tables = seqs && a->max_pages > 0;
+  if ((seqs && (!a->ctx || !a->n_new || !a->held || !a->held_out)) || (tables && (!a->pages || !a->pages_out)) ||
+      (a->free_cap > 0 && (!a->free || !a->free_out)) || !a->n_free || !a->n_free_out || !a->start || !a->lacking)
+    return bad("pk_kv_plan: null array");
+  const uintptr_t all = (uintptr_t)a->ctx | (uintptr_t)a->n_new | (uintptr_t)a->pages | (uintptr_t)a->held | (uintptr_t)a->free |
+                        (uintptr_t)a->n_free | (uintptr_t)a->done | (uintptr_t)a->shared | (uintptr_t)a->pages_out |
+                        (uintptr_t)a->held_out | (uintptr_t)a->free_out | (uintptr_t)a->n_free_out | (uintptr_t)a->start |
+                        (uintptr_t)a->lacking | (uintptr_t)a->pos | (uintptr_t)a->seq;
+  if ((all & 3) || ((uintptr_t)a->slot & 7)) return bad("pk_kv_plan: misaligned array");
+  // in place: all of what is there
+  const bool in_place = a->n_free_out == a->n_free;
+  if ((seqs && (a->held_out == a->held) != in_place) || (tables && (a->pages_out == a->pages) != in_place) ||
+      (a->free_cap > 0 && (a->free_out == a->free) != in_place))
+    return bad("pk_kv_plan: pages, held, free and n_free are all updated in place or none is");
+  CK(launch_kv_plan(*a, in_place, (cudaStream_t)stream));
+  return PK_OK;
+}
+
+int pk_sample_rows(const void *logits, int type, int rows, int n, int64_t stride, const pk_sample_args *a, void *stream) {
+  if (!is_float_type(type)) return set_error(PK_ERR_UNSUPPORTED, "pk_sample_rows: element type " + std::to_string(type) + " is not f32, f16 or bf16");
+  if (!a) return bad("pk_sample_rows: null arguments");
+  if (rows < 0 || rows > (1 << 24) || n < 1 || n > (1 << 30)) return bad("pk_sample_rows: rows must be 0 to 2^24 and n 1 to 2^30");
+  if (rows == 0) return PK_OK;
+  if (!logits || !a->u || !a->tok) return bad("pk_sample_rows: null logits, u or tok");
+  if ((uintptr_t)logits & elem_mask(type)) return bad("pk_sample_rows: misaligned logits");
+  if (((uintptr_t)a->u | (uintptr_t)a->temp | (uintptr_t)a->top_k | (uintptr_t)a->top_p | (uintptr_t)a->min_p | (uintptr_t)a->tok |
+       (uintptr_t)a->prob | (uintptr_t)a->kept) & 3)
+    return bad("pk_sample_rows: misaligned array");
+  if (stride < 0 || stride > (1LL << 40)) return bad("pk_sample_rows: row stride out of range");
+  CK(launch_sample(logits, type, rows, n, (long)stride, *a, (cudaStream_t)stream));
   return PK_OK;
 }
 

@@ -18,8 +18,9 @@ import ctypes as C
 import os
 import subprocess
 
-from . import drafts
+from . import drafts, serving
 from .drafts import KvCache, KvSeqs, RopeTable, logit_rules, rope
+from .serving import KvPlan, KvShared, kv_plan, sample_rows
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG_DIR = os.path.dirname(HERE)
@@ -50,6 +51,7 @@ SYMBOLS = [
     "pk_tokenizer_load", "pk_tokenizer_free", "pk_tokenizer_info_get", "pk_tokenize", "pk_token_bytes",
     "pk_token_is_eog", "pk_utf8_flush", "pk_text_find", "pk_chat_apply", "pk_chat_prompt", "pk_chat_is_minicpm5", "pk_chat_direct_suffix", "pk_chat_thinking_suffix",
     "pk_kv_store", "pk_kv_load", "pk_kv_keep", "pk_kv_attn_scratch_bytes", "pk_kv_attn", "pk_rope_turns", "pk_rope", "pk_apply_logit_rules",
+    "pk_kv_attn_shared_scratch_bytes", "pk_kv_attn_shared", "pk_kv_plan", "pk_sample_rows",
 ]
 
 

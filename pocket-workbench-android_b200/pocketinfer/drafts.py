@@ -67,6 +67,9 @@ SIGNATURES = {
     "pk_kv_keep": ([P, P, P, I, P, P], I), "pk_kv_attn_scratch_bytes": ([P, P, I, I], SZ),
     "pk_kv_attn": ([P, P, P, P, SZ, P], I), "pk_rope_turns": ([P, P, P], I), "pk_rope": ([P, P], I),
     "pk_apply_logit_rules": ([P, P, I, I, I, I64, I64, P, P], I),
+    # (serving.py)
+    "pk_kv_attn_shared_scratch_bytes": ([P, P, P, I, I], SZ), "pk_kv_attn_shared": ([P, P, P, P, P, SZ, P], I),
+    "pk_kv_plan": ([P, P], I), "pk_sample_rows": ([P, I, I, I, I64, P, P], I),
 }
 
 torch = None  # set by _init, with the library and the error type
@@ -248,9 +251,10 @@ class KvCache:
             _bad("keep: one row and one count a sequence, on the cache's device")
         _call(_L.pk_kv_keep, self.device, stream, stream is not None and (self.tensors, seqs.tensors, keep, n_keep), self.ref, seqs.ref, keep.data_ptr(), keep.shape[1], n_keep.data_ptr())
 
-    def attend(self, seqs: KvSeqs, q, mask=None, scale: float | None = None, out=None, scratch=None, stream=None):
+    def attend(self, seqs: KvSeqs, q, mask=None, scale: float | None = None, out=None, scratch=None, stream=None, shared=None):
         """Attention of the new tokens q [n_tok, n_head, head_dim] over the cache; mask: int64 [n_tok, words], bit j of
-        token i set where it sees new token j (None: causal).  scratch: a uint8 tensor of attend_scratch_bytes()."""
+        token i set where it sees new token j (None: causal).  scratch: a uint8 tensor of attend_scratch_bytes().  shared:
+        a KvShared, the prefixes that sequences share, each computed once for all of them."""
         code, shape, s, dev = _dtype(q, "attend"), q.shape, q.stride(), self.device
         if len(shape) != 3 or shape[0] != seqs.n_tok or shape[2] != self.head_dim or s[2] != 1:
             _bad("attend: q must be [n_tok, n_head, head_dim] with contiguous heads")
@@ -261,9 +265,11 @@ class KvCache:
             out = _like(q) if stream is None else _new(lambda: _like(q), dev, stream)
         elif out.shape != shape or out.dtype != q.dtype or out.get_device() != dev or out.stride(2) != 1:
             _bad("attend: out must be as q")
-        ptr, size = None, seqs.scratch.get((shape[1], code, self.shape))
+        if shared is not None and shared.device != dev:
+            _bad("attend: the shared prefixes are on another device")
+        ptr, size = None, seqs.scratch.get((shape[1], code, self.shape, shared and shared.key))
         if size is None:
-            size = self.attend_scratch_bytes(seqs, shape[1], q.dtype)
+            size = self.attend_scratch_bytes(seqs, shape[1], q.dtype, shared)
         if scratch is not None:
             if scratch.get_device() != dev or not scratch.is_contiguous():
                 _bad("attend: scratch must be contiguous and on the cache's device")
@@ -275,14 +281,20 @@ class KvCache:
         o = out.stride()
         args = PACK_QUERY(q.data_ptr(), out.data_ptr(), bits, s[0], s[1], o[0], o[1], code, shape[1], words,
                           self.head_dim ** -0.5 if scale is None else scale)
-        _call(_L.pk_kv_attn, dev, stream, stream is not None and (self.tensors, seqs.tensors, q, mask, out, scratch), self.ref, seqs.ref, args, ptr, size)
+        if shared is None:
+            _call(_L.pk_kv_attn, dev, stream, stream is not None and (self.tensors, seqs.tensors, q, mask, out, scratch), self.ref, seqs.ref, args, ptr, size)
+        else:
+            _call(_L.pk_kv_attn_shared, dev, stream, stream is not None and (self.tensors, seqs.tensors, shared.tensors, q, mask, out, scratch), self.ref, seqs.ref, shared.ref, args, ptr, size)
         return out
 
-    def attend_scratch_bytes(self, seqs: KvSeqs, n_head: int, dtype) -> int:
+    def attend_scratch_bytes(self, seqs: KvSeqs, n_head: int, dtype, shared=None) -> int:
         """Bytes of scratch that attend() needs (0: none); kept with the sequences, whose bounds do not change."""
         code = _type_of[dtype]
-        n = _L.pk_kv_attn_scratch_bytes(self.ref, seqs.ref, n_head, code)
-        seqs.scratch[n_head, code, self.shape] = n
+        if shared is None:
+            n = _L.pk_kv_attn_scratch_bytes(self.ref, seqs.ref, n_head, code)
+        else:
+            n = _L.pk_kv_attn_shared_scratch_bytes(self.ref, seqs.ref, shared.ref, n_head, code)
+        seqs.scratch[n_head, code, self.shape, shared and shared.key] = n
         return n
 
 
