@@ -101,19 +101,14 @@ def kv_plan(ctx, n_new, pages, held, free, n_free, page_size: int, n_tok: int, d
     wide, cap = pages.shape[1], free.shape[0]
     i32, where = _d.torch.int32, ctx.device
 
-    def make():
-        # one block for all the int32 results (a tensor of its own each costs as much as the launch), each at 16 bytes
-        sizes = [n + 1, n_tok, n_tok, 1] + ([] if in_place else [n * wide, n, cap, 1])
-        at = [0]
-        for x in sizes:
-            at.append(at[-1] + (x + 3) // 4 * 4)
-        block = _d.torch.empty(at[-1], dtype=i32, device=where)
-        parts = [block[a:a + x] for a, x in zip(at, sizes)]
-        return (_d.torch.empty(n_tok, dtype=_d.torch.int64, device=where), *parts)
-
+    # one block for all results (a tensor of its own each costs more than the launch, and so does a slice each), each at
+    # 16 bytes: they and the gaps behind them by turns
+    sizes = (2 * n_tok, n + 1, n_tok, n_tok, 1) if in_place else (2 * n_tok, n + 1, n_tok, n_tok, 1, n * wide, n, cap, 1)
+    cuts = [x for size in sizes for x in (size, -size % 4)]
+    make = lambda: _d.torch.empty(sum(cuts), dtype=i32, device=where).split_with_sizes(cuts)  # noqa: E731
     made = make() if stream is None else _new(make, dev, stream)
-    slot, start, pos, seq, lacking = made[:5]
-    out = (pages, held, free, n_free) if in_place else (made[5].view(n, wide), made[6], made[7], made[8])
+    slot, start, pos, seq, lacking = made[0].view(_d.torch.int64), made[2], made[4], made[6], made[8]
+    out = (pages, held, free, n_free) if in_place else (made[10].view(n, wide), made[12], made[14], made[16])
     ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     args = PACK_PLAN(ctx.data_ptr(), n_new.data_ptr(), pages.data_ptr(), held.data_ptr(), free.data_ptr(), n_free.data_ptr(), ptr(done), ptr(shared),
                      *[t.data_ptr() for t in out], start.data_ptr(), lacking.data_ptr(), pos.data_ptr(), seq.data_ptr(), slot.data_ptr(), n, wide, cap,
