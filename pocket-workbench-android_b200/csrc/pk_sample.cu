@@ -6,26 +6,28 @@
 // All three rules keep a beginning of that order, so what is kept is everything
 // down to one (logit, index), the cut.  Without a sort of the row:
 //   1  the largest logit: y <= 0.  min_p is a least logit.
-//   2  a histogram of y in steps of a 16th of a nat: of tokens for top-k, for
-//      top-p of their weights as multiples of the bin's lowest, in 2^-15 (a 6e-5th
-//      is allowed for that and f32's logarithms).  Its sums from the top say
-//      which bins hold the cut.
+//   2  a histogram: for top-k of y, for top-p of the weights by their exponents
+//      and first three bits, in 2^-15 of the exponent's power (a 6e-5th is
+//      allowed for that).  Its sums from the top say which bins hold the cut, and
+//      a search among floats, by the same function, which logits begin and end
+//      them.
 //   3  the tokens of those bins (or of all bins down to there, if they are few,
-//      for top-k and top-p at once) are sorted and added up exactly, beginning
-//      with the exact weight above them.  If they are too many, as in rows of
-//      equal logits, halving steps on (logit, index) come before.
+//      for top-k and top-p at once) are sorted by one CTA and added up exactly,
+//      beginning with the exact weight above them.  If they are too many, as in rows of equal logits,
+//      halving steps on (logit, index) come before.
 //   4  sums of the kept weights by index, the token in whose part u falls.
 // A token depends on sums of a whole vocabulary next to whose borders u may lie:
 // at 128256 borders an error of 2^-24 would change one token in a hundred.  So
-// weights are made in double, 2^y from a table of 256 and three terms of the
-// series (1.4e-13), and added as 64-bit integers, in which no order matters:
-// 2^-q steps of the largest, n 2^q <= 2^62.
+// weights are made in double, 2^y from a table and a few terms of the series
+// (1.4e-13), and added as 64-bit integers, in which no order matters: 2^-q steps
+// of the largest, n 2^q <= 2^62.
 //
 // A row is read once, into the shared memory of a cluster of up to 8 CTAs, and
 // gone over there; rows that do not fit are read again each time.
 #include <math_constants.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "pk_cache.cuh"
 #include "pk_cache.h"
@@ -37,9 +39,10 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int ST = 512, SW = ST / 32;  // threads, warps
-constexpr int BINS = 512, CAP = 512;   // of the histogram; tokens that are sorted
+constexpr int BINS = 512, CAP = 512;   // of the histogram; tokens that one CTA sorts
 static_assert(BINS == ST && CAP == ST, "a bin and a sorted token a thread");
-constexpr float MARGIN = 6e-5f;
+constexpr int TB = 4, TABLE = 1 << TB;  // table of 2^(i / TABLE): 16 entries of 8 bytes are in different banks
+constexpr float MARGIN = 6e-5f;        // of sums of the histogram's weights, with 16 bits of each
 constexpr int LAST = 0x7fffffff;
 constexpr float MAXF = 3.402823466e38f;
 
@@ -48,18 +51,18 @@ struct SampleK {
   long long stride;
   int n, cluster, seg;   // seg: positions a CTA, whole 16-byte vectors
   int q;                 // fixed-point bits of a weight
-  float unit, margin;    // a bin's lowest weight in the histogram; what its sums may be off by
+  int drop;              // bits of a weight's 21 that the histogram leaves out
   pk_sample_args p;
 };
 
 struct Smem {  // behind the row's values
   uint32_t hist[2][BINS];  // of even and of odd lanes, which then collide less
   u64 cand[CAP];
-  double table[256];
+  double table[TABLE];
   u64 warp[SW], x[6];   // of the CTA's warps; what the cluster's CTAs tell each other
   double off_min, off_low;
   uint32_t warp2[SW], n_cand, lo, hi, at, above, first;
-  float warpf[SW], cut_x;
+  float warpf[SW], cut_x, edge[2];
   int cut_i;
 };
 
@@ -98,8 +101,8 @@ struct Row {
   int tid, lane, warp;
   int shift, end;     // position p is token p - shift; positions of this row: shift .. end - 1
   int p0, vecs, per;  // this CTA's first position, its vectors, those of a warp (its own run of them)
-  float top = 0.0f, low = 0.0f;  // the largest logit; what is below `low` has no weight
-  double step = 0.0, zero = 0.0;  // 256 log2(e) / temp; 1.5 * 2^52 less the largest logit's steps
+  float top = 0.0f, low = 0.0f, none = 0.0f;  // the largest logit; what is below `low` has no weight, nor has `none`
+  double step = 0.0, zero = 0.0;  // TABLE log2(e) / temp; 1.5 * 2^52 less the largest logit's steps
   double scale = 0.0;  // log2(e) / temp
   bool exact = false;  // steps of logits themselves would lose bits: those of their differences
   float cx = 0.0f;     // the cut: kept is what is larger, or equal with an index up to ci
@@ -140,14 +143,23 @@ struct Row {
     });
   }
   __device__ __forceinline__ bool kept(float x, int i) const { return x >= cx && (x > cx || i <= ci); }
+  __device__ __forceinline__ void kept4(const float *x, int i, bool (&on)[4]) const {
+#pragma unroll
+    for (int e = 0; e < 4; e++) on[e] = x[e] >= cx;
+    if (ci != LAST) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) on[e] = on[e] && (x[e] > cx || i + e <= ci);
+    }
+  }
 
-  // The weight times 2^q (and a factor within 2^(1/512) of 1, the same for the
-  // whole row), for low <= x <= top.  Where +inf is the largest, everything
-  // below has none (low).
-  __device__ __forceinline__ double weight(float x) const {
+  // The weight times 2^q (and a factor within 2^(1/2/TABLE) of 1, the same for
+  // the whole row), for x <= top; EX: as `exact` says.  What is below `low`, and
+  // `none`, have one that rounds to 0: without EX x has to be `none` or more.
+  template <bool EX>
+  __device__ __forceinline__ double weight_as(float x) const {
     double v;
-    if (exact) {
-      v = x == top ? 0.0 : ((double)x - (double)top) * scale;
+    if (EX) {
+      v = x == top ? 0.0 : x >= low ? ((double)x - (double)top) * scale : -100.0;
     } else {  // x in double without the conversion, of which an SM makes 16 a cycle; 0 and subnormals become up to 2^-126
       const int u = __float_as_int(x);
       v = __hiloint2double(((u >> 3) & 0x8fffffff) + (896 << 20), u << 29);
@@ -155,33 +167,35 @@ struct Row {
     const double t = fma(v, step, zero);  // its low bits are the number of steps, rounded
     const double r = fma(v, step, zero - t);  // what is left of them, -0.5 .. 0.5
     const int k = __double2loint(t);
-    double f = 3.308302680541371e-09;  // (ln(2) / 256)^i / i!
-    f = fma(f, r, 3.665565596910106e-06);
-    f = fma(f, r, 0.0027076061740622863);
-    f = fma(f, r, 1.0) * sm.table[k & 255];
-    return __hiloint2double(__double2hiint(f) + ((k & ~255) << 12), __double2loint(f));
+    // 2^(r / TABLE): terms (ln(2) / TABLE)^i / i!
+    constexpr double L = 0.6931471805599453 / TABLE;
+    double f = fma(L * L * L * L * L / 120, r, L * L * L * L / 24);
+    f = fma(f, r, L * L * L / 6);
+    f = fma(f, r, L * L / 2);
+    f = fma(f, r, L);
+    f = fma(f, r, 1.0) * sm.table[k & (TABLE - 1)];
+    return __hiloint2double(__double2hiint(f) + ((k & ~(TABLE - 1)) << (20 - TB)), __double2loint(f));
   }
-  // the same, rounded to an integer
+  __device__ __forceinline__ double weight(float x) const {
+    x = fmaxf(x, none);
+    return exact ? weight_as<true>(x) : weight_as<false>(x);
+  }
+  // the same, rounded to an integer, plus ONE
   static constexpr u64 ONE = 0x4330000000000000ull;  // 2^52's bits
-  __device__ __forceinline__ u64 made(float x) const { return (u64)__double_as_longlong(weight(x) + 4503599627370496.0) - ONE; }
-  __device__ __forceinline__ u64 fixed(float x) const { return x >= low ? made(x) : 0; }
+  __device__ __forceinline__ u64 raw(double w) const { return (u64)__double_as_longlong(w + 4503599627370496.0); }
+  __device__ __forceinline__ u64 fixed(float x) const { return raw(weight(x)) - ONE; }
+  // f(std::true_type or std::false_type), as `exact` is: passes that make weights, twice in the code
+  template <class F>
+  __device__ __forceinline__ void as_exact(F f) const {
+    if (exact) f(std::true_type{});
+    else f(std::false_type{});
+  }
   // of four those that are `on`
+  template <bool EX>
   __device__ __forceinline__ void add4(const float *x, const bool (&on)[4], u64 &sum) const {
     if (!(on[0] || on[1] || on[2] || on[3])) return;
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const u64 w = made(on[e] ? x[e] : top);
-      if (on[e]) sum += w;
-    }
-  }
-  __device__ __forceinline__ u64 sum_kept(const float *x, int i) const {
-    const float least = fmaxf(cx, low);
-    bool on[4];
-#pragma unroll
-    for (int e = 0; e < 4; e++) on[e] = x[e] >= least && (x[e] > cx || i + e <= ci);
-    u64 sum = 0;
-    add4(x, on, sum);
-    return sum;
+    for (int e = 0; e < 4; e++) sum += raw(weight_as<EX>(on[e] ? fmaxf(x[e], none) : none)) - ONE;
   }
 
   __device__ __forceinline__ u64 sum_warp(u64 v) const {
@@ -251,7 +265,7 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
   const float top_p = a.p.top_p ? __ldg(a.p.top_p + row) : 1.0f, min_p = a.p.min_p ? __ldg(a.p.min_p + row) : 0.0f;
   const int top_k = a.p.top_k ? __ldg(a.p.top_k + row) : 0;
   r.scale = 1.4426950408889634074 / (double)temp;
-  if (tid < 256) sm.table[tid] = exp2((double)tid / 256.0 + (double)a.q);
+  if (tid < TABLE) sm.table[tid] = exp2((double)tid / TABLE + (double)a.q);
   if (tid == ST - 1) {
     sm.n_cand = 0;
     sm.first = LAST;
@@ -301,21 +315,31 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
   r.cx = -MAXF;
   if (min_p > 0.0f) r.cx = inf ? r.top : fminf(fmaxf(__double2float_ru((double)r.top + sm.off_min), -MAXF), r.top);
   r.low = inf ? r.top : fmaxf(__double2float_rd((double)r.top - sm.off_low), -MAXF);
-  // steps of 2^(1/256): of the logits themselves where they keep 2^-40 of one
+  // steps of 2^(1/TABLE): of the logits themselves where they keep 2^-40 of one
   // (the last bits of what is below 2^-126 count at temperatures like 2^-80 only)
-  r.step = 256.0 * r.scale;
+  r.step = TABLE * r.scale;
   r.zero = 6755399441055744.0;
-  r.exact = inf || temp < 0x1p-80f || !(fabs((double)r.top * r.step) < 0x1p50);
-  if (r.exact) r.step = 256.0;
+  r.none = r.low;
+  r.exact = inf || temp < 0x1p-80f || !(fabs((double)r.top * r.step) < 0x1p50) || !(r.low > -MAXF);
+  if (r.exact) r.step = TABLE, r.none = -CUDART_INF_F;
   else r.zero -= rint((double)r.top * r.step);
 
   // ---- 2, 3: the cut of top-k, then of top-p
   bool do_k = top_k > 0 && top_k < a.n, do_p = top_p < 1.0f;
-  const float per_unit = fmaxf(fminf(16.0f / temp, 1e30f), 1e-38f);  // (not 0, which times infinity is NaN)
-  // y in bins
-  auto place = [&](float x) { return x == r.top ? 0.0f : (r.top - x) * per_unit; };
-  bool added = false;   // sum and n have what is before the tokens in question
-  float from_bin = 0.0f;  // where those begin
+  // bins of 1/16 nat for top-k: to the nearest, by an addition in which the
+  // sum's last bits are the number (what the constant loses shifts all alike)
+  const float per_unit = fmaxf(fminf(16.0f / temp, 1e30f), 1e-38f);
+  const float bias = fminf(fmaxf(rintf(r.top * per_unit), -4e6f), 4e6f);
+  const bool near = fabsf(r.top * per_unit) < 4e6f;
+  auto bin_k = [&](float x) {
+    const float d = near ? fmaf(x, -per_unit, bias) : x == r.top ? 0.0f : (r.top - x) * per_unit;
+    return __float_as_uint(fminf(fmaxf(d, 0.0f), (float)(BINS - 1)) + 8388608.0f) & 1023u;  // (NaN, of infinities: 0)
+  };
+  // for top-p by the weight's exponent and three bits: bin 0 has the largest
+  const int hi_top = __double2hiint(r.weight(r.top)) >> 17;
+  auto bin_p = [&](double w) { return (uint32_t)min(hi_top - (__double2hiint(w) >> 17), BINS - 1); };
+  float before_x = CUDART_NAN_F;  // logits from here on are before those in question
+  bool added = false;             // sum and n have them
   u64 sum = 0;
   uint32_t n = 0;
   for (bool again = false; do_k || do_p; again = true) {
@@ -329,28 +353,35 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
     uint32_t *hist = sm.hist[lane & 1];
     u64 weight = 0;
     if (weigh) {
-      r.each4([&](const float *x, int i) {
-        weight += r.sum_kept(x, i);
+      r.as_exact([&](auto ex) {
+        r.each4([&](const float *x, int i) {
+          bool on[4];
+          r.kept4(x, i, on);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          if (!r.kept(x[e], i + e)) continue;
-          const float d = place(x[e]);
-          if (d < (float)(BINS - 1)) {  // 2^((b + 1 - d) / 16 nat) of the bin's lowest weight
-            const int b = (int)d;
-            float over;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(over) : "f"(((float)(b + 1) - d) * (1.4426950408889634f / 16.0f)));
-            atomicAdd(hist + b, (uint32_t)__float2int_rn(over * a.unit));
+          for (int e = 0; e < 4; e++) {
+            const double w = r.template weight_as<decltype(ex)::value>(on[e] ? fmaxf(x[e], r.none) : r.none);
+            weight += r.raw(w) - r.ONE;
+            if (on[e] && x[e] >= r.low) atomicAdd(hist + bin_p(w), ((__double2hiint(w) & 0xfffffu) | 0x100000u) >> a.drop);
           }
-        }
+        });
       });
-      r.sum_to(weight, 1);
+      weight = r.sum_warp(weight);
+      if (lane == 0) sm.warp[warp] = weight;
     } else {
-      r.each([&](float x, int i) {
-        if (r.kept(x, i)) atomicAdd(hist + (int)fminf(place(x), (float)(BINS - 1)), 1u);  // (NaN, of infinities: the last)
+      r.each4([&](const float *x, int i) {
+        bool on[4];
+        r.kept4(x, i, on);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (on[e]) atomicAdd(hist + bin_k(x[e]), 1u);
       });
     }
     __syncthreads();
     sm.hist[0][tid] += sm.hist[1][tid];
+    if (weigh && warp == 0) {
+      weight = r.sum_warp(lane < SW ? sm.warp[lane] : 0);
+      if (lane == 0) sm.x[1] = weight;
+    }
     if (tid == 0) sm.lo = sm.hi = BINS - 1;
     r.sync();
     if (weigh) weight = r.all_sum(1);
@@ -365,10 +396,9 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
 #pragma unroll
       for (int k = 0; k < 8; k++) {
         m += (float)v[k];
-        c += !weigh ? v[k] : v[k] ? (uint32_t)((float)v[k] * (1.0f / a.unit)) + 1 : 0;
+        c += weigh ? v[k] >> (20 - a.drop) : v[k];
       }
-      m *= exp2f((float)(tid + 1) * (-1.4426950408889634f / 16.0f));
-      if (weigh && tid == BINS - 1) c = (uint32_t)a.n;  // (not counted)
+      m *= exp2f((float)(((hi_top - tid) >> 3) - (hi_top >> 3)));
     }
     uint32_t cs = c;
     float ms = m;
@@ -392,8 +422,8 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
     const uint32_t k = min((uint32_t)top_k, total);
     // (sums of weights need not ascend by the last bit: the first bin that passes)
     uint32_t l = BINS - 1, h = BINS - 1;
-    if (do_k ? cs >= k : ms >= mass * top_p * (1.0f - a.margin)) l = tid;
-    if (do_k ? cs >= k : ms >= mass * top_p * (1.0f + a.margin)) h = tid;
+    if (do_k ? cs >= k : ms >= mass * top_p * (1.0f - MARGIN)) l = tid;
+    if (do_k ? cs >= k : ms >= mass * top_p * (1.0f + MARGIN)) h = tid;
     l = __reduce_min_sync(0xffffffffu, l);
     h = __reduce_min_sync(0xffffffffu, h);
     if (lane == 0 && l < BINS - 1) atomicMin(&sm.lo, l);
@@ -414,17 +444,50 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
     if (whole) lo = 0, above = 0;
     const bool both = do_k && do_p && whole;
     uint32_t inside = down - above;
-    // (by bins, or after halving by order) is it in question? is it before?
+    // The least floats of bins below lo (that are before those in question) and
+    // of bins up to hi, a warp each: 33 floats around where the bin should end,
+    // or, if it does not there, 33 that divide all, and so on.
+    if (warp < 2) {
+      const int b = warp == 0 ? lo - 1 : hi;
+      auto in = [&](uint32_t key) {
+        const float x = of_key(key);
+        return (int)(do_k ? bin_k(x) : x >= r.low ? bin_p(r.weight(x)) : (uint32_t)(BINS - 1)) <= b;
+      };
+      const uint32_t least = key_of(-CUDART_INF_F);
+      uint32_t from = least, to = key_of(r.top);  // (of which one is not looked at, the other is in bin 0)
+      if (b < 0 || b == BINS - 1) {
+        from = to = b < 0 ? 0 : key_of(-MAXF);
+      } else {
+        double g;
+        if (do_k) g = ((double)bias - b - 0.5) / (double)per_unit;
+        else g = (log2(__hiloint2double((hi_top - b) << 17, 0)) - a.q) * TABLE;
+        if (!do_k) g = r.exact ? (double)r.top + g / TABLE / r.scale : (g - (r.zero - 6755399441055744.0)) / r.step;
+        const uint32_t at = min(max(key_of((float)g), least + 17), to - min(to - least - 17, 16u));
+        const bool here = lane == 0 ? !in(at - 16) : lane == 1 ? in(at + 16) : true;
+        if (to - least > 64 && __all_sync(0xffffffffu, here)) from = at - 16, to = at + 16;
+      }
+      while (to - from > 1) {
+        const uint32_t step = (to - from + 31) / 32, at = from + min((uint32_t)(lane + 1) * step, to - from);
+        const uint32_t lanes = __ballot_sync(0xffffffffu, in(at));  // (`to` is among them)
+        const int f = __ffs(lanes) - 1;
+        const uint32_t next = __shfl_sync(0xffffffffu, at, f);
+        from = f > 0 ? __shfl_sync(0xffffffffu, at, max(f - 1, 0)) : from;
+        to = next;
+      }
+      if (lane == 0) sm.edge[warp] = b < 0 ? CUDART_NAN_F : of_key(to);
+    }
+    __syncthreads();
+    before_x = sm.edge[0];
+    const float last_x = weigh ? fmaxf(sm.edge[1], r.low) : sm.edge[1];  // (what has no weight is not in the histogram)
+    // (by logits, or after halving by order) is it in question? is it before?
     u64 o_lo = 0, o_hi = ~0ull, base_w = 0;
     bool by_order = false;
-    const float d_lo = (float)lo, d_hi = hi == BINS - 1 ? CUDART_INF_F : (float)(hi + 1);
     auto side = [&](float x, int i) {  // 0: in question, 1: before, -1: behind
       if (by_order) {
         const u64 o = order_of(x, i);
         return o > o_hi ? 1 : o < o_lo ? -1 : 0;
       }
-      const float d = place(x);
-      return d < d_lo ? 1 : d >= d_hi && hi < BINS - 1 ? -1 : 0;
+      return x >= before_x ? 1 : x >= last_x ? 0 : -1;
     };
     const double target = (double)top_p * (double)weight;
     if (inside > CAP) {
@@ -490,51 +553,71 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
     }
     // the tokens in question to the first CTA, and the exact weight before them
     added = weigh && !by_order;
-    from_bin = d_lo;
     sum = 0;
     n = 0;
     const uint32_t to = map_rank(shaddr(&sm.cand[0]), 0), counter = map_rank(shaddr(&sm.n_cand), 0);
-    r.each4([&](const float *x, int i) {
-      bool before[4];
+    auto take = [&](float x, int i) {
+      uint32_t at;
+      asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(counter) : "memory");
+      if (at < CAP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + at * 8), "l"(order_of(x, i)) : "memory");
+    };
+    if (by_order) {
+      r.each([&](float x, int i) {
+        if (r.kept(x, i) && side(x, i) == 0) take(x, i);
+      });
+    } else {
+      r.as_exact([&](auto ex) {
+        r.each4([&](const float *x, int i) {
+          if (!(x[0] >= last_x || x[1] >= last_x || x[2] >= last_x || x[3] >= last_x)) return;
+          bool on[4], before[4];
+          r.kept4(x, i, on);
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const bool on = r.kept(x[e], i + e);
-        const int s = on ? side(x[e], i + e) : -1;
-        before[e] = s > 0 && x[e] >= r.low;
-        n += s > 0;
-        if (s == 0) {
-          uint32_t at;
-          asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(counter) : "memory");
-          if (at < CAP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + at * 8), "l"(order_of(x[e], i + e)) : "memory");
-        }
-      }
-      if (added) r.add4(x, before, sum);
-    });
-    if (added) r.sum_to(sum, 5);
+          for (int e = 0; e < 4; e++) {
+            before[e] = on[e] && x[e] >= before_x;
+            n += before[e];
+            if (on[e] && !before[e] && x[e] >= last_x) take(x[e], i + e);
+          }
+          if (added) r.template add4<decltype(ex)::value>(x, before, sum);
+        });
+      });
+      if (added) r.sum_to(sum, 5);
+    }
     r.sync();
+    u64 *sorted = reinterpret_cast<u64 *>(sm.hist[0]);  // (which has been read)
+    static_assert(sizeof(sm.hist) >= CAP * sizeof(u64), "room");
     if (rank == 0) {
       if (added) base_w = r.all_sum(5);
-      const int nc = min((int)sm.n_cand, CAP);
+      const int nc = min((int)sm.n_cand, CAP), lists = (nc + 31) / 32;
       u64 v = tid < nc ? sm.cand[tid] : 0;
-      int n2 = 32;
-      while (n2 < nc) n2 *= 2;
       __syncthreads();
-      if (warp * 32 < n2) {  // (whole warps; the barrier below is theirs)
-        for (int size = 2; size <= n2; size *= 2)
+      if (warp < lists) {  // each warp sorts its 32
+#pragma unroll
+        for (int size = 2; size <= 32; size *= 2)
+#pragma unroll
           for (int j = size / 2; j > 0; j /= 2) {
-            u64 o;
-            if (j >= 32) {
-              sm.cand[tid] = v;
-              asm volatile("bar.sync 1, %0;" ::"r"(n2) : "memory");
-              o = sm.cand[tid ^ j];
-              asm volatile("bar.sync 1, %0;" ::"r"(n2) : "memory");
-            } else {
-              o = __shfl_xor_sync(0xffffffffu, v, j);
-            }
-            const bool down_here = (tid & size) == 0, low_half = (tid & j) == 0;
+            const u64 o = __shfl_xor_sync(0xffffffffu, v, j);
+            const bool down_here = (lane & size) == 0, low_half = (lane & j) == 0;
             v = down_here == low_half ? max(v, o) : min(v, o);
           }
+        sm.cand[tid] = v;
       }
+      __syncthreads();
+      if (warp < lists) {  // and finds how many of the other lists' are before each
+        int place = lane;
+#pragma unroll 4
+        for (int w = 0; w < lists; w++) {
+          const u64 *o = sm.cand + 32 * w;
+          int b = 0;
+#pragma unroll
+          for (int j = 16; j > 0; j /= 2) b += o[b + j - 1] > v ? j : 0;
+          b += o[b] > v;
+          place += w == warp ? 0 : b;
+        }
+        __syncwarp();
+        if (v) sorted[place] = v;
+      }
+      __syncthreads();
+      v = tid < nc ? sorted[tid] : 0;
       const float x = of_key((uint32_t)(v >> 32));
       // the last one that top-k leaves
       const int most = do_k ? min(nc, (int)(k - above)) : nc;
@@ -563,17 +646,32 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
   }
 
   // ---- 4: the kept weights by index (of what came before the tokens in question they are there)
-  if (!added) sum = 0, n = 0;
-  r.each4([&](const float *x, int i) {
-    const float least = fmaxf(r.cx, r.low);
-    bool on[4];
+  if (!added) sum = 0, n = 0, before_x = CUDART_NAN_F;
+  r.as_exact([&](auto ex) {
+    if (r.ci == LAST && r.cx <= r.none) {  // nothing is cut off that has a weight
+      uint32_t made = 0;
+      r.each4([&](const float *x, int) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      on[e] = r.kept(x[e], i + e) && !(added && place(x[e]) < from_bin);
-      n += on[e];
-      on[e] = on[e] && x[e] >= least;
+        for (int e = 0; e < 4; e++) {
+          n += x[e] >= r.cx;
+          sum += r.raw(r.template weight_as<decltype(ex)::value>(fmaxf(x[e], r.none)));
+        }
+        made += 4;
+      });
+      sum -= made * r.ONE;
+    } else {
+      r.each4([&](const float *x, int i) {
+        if (!(x[0] >= r.cx || x[1] >= r.cx || x[2] >= r.cx || x[3] >= r.cx)) return;
+        bool on[4];
+        r.kept4(x, i, on);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          on[e] = on[e] && !(x[e] >= before_x);
+          n += on[e];
+        }
+        r.template add4<decltype(ex)::value>(x, on, sum);
+      });
     }
-    r.add4(x, on, sum);
   });
   sum = r.sum_warp(sum);
   n = __reduce_add_sync(0xffffffffu, n);
@@ -618,7 +716,7 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
       if (i < w1) {
         r.vec(i, x);
 #pragma unroll
-        for (int e = 0; e < V; e += 4) mine += r.sum_kept(x + e, token + e);
+        for (int e = 0; e < V; e++) mine += r.kept(x[e], token + e) ? r.fixed(x[e]) : 0;
       }
       const u64 b0 = from + r.scan(mine);
       if (mine && pass >= b0 && pass < b0 + mine) {
@@ -660,16 +758,15 @@ cudaError_t launch_sample(const void *logits, int type, int rows, int n, long st
   // CTAs a row: by what they hold, two an SM, one where rows are longer; more where the rows leave SMs without any
   const long long vecs = ((long long)n + 2 * v - 2) / v, most = 96 * 1024 / 16, wide = 208 * 1024 / 16;
   long long c = std::min(8LL, (vecs + most - 1) / most);
-  while (c < 8 && rows * c * 2 <= 148 && vecs >= 512 * c) c *= 2;
+  while (c < 8 && rows * c * 2 <= 296 && vecs >= 512 * c) c *= 2;
   c = std::min(c, 8LL);
   const long long seg = (vecs + c - 1) / c;
   const bool big = seg > wide;
   a.cluster = (int)c;
   a.seg = (int)(seg * v);
-  // a weight is at most 1.0645 of its bin's lowest: in 2^-15 steps 65536 of a bin and CTA fit 32 bits
-  a.unit = 32768.0f;
-  for (long long x = 65536; x < a.seg; x *= 2) a.unit *= 0.5f;
-  a.margin = MARGIN + 1.0f / a.unit;
+  // 21 bits of a weight, of which 16 are kept: 65536 of a bin and CTA fit 32 bits
+  a.drop = 5;
+  for (long long x = 65536; x < a.seg; x *= 2) a.drop++;
   const int smem = (int)sizeof(Smem) + (big ? 0 : (int)(seg * 16));
   const dim3 grid((unsigned)(rows * c)), block(ST);
 #define GO(E) launch_cluster(big ? k_sample<E, true> : k_sample<E, false>, (int)c, grid, block, smem, st, a)
