@@ -6,16 +6,19 @@
 // All three rules keep a beginning of that order, so what is kept is everything
 // down to one (logit, index), the cut.  Without a sort of the row:
 //   1  the largest logit: y <= 0.  min_p is a least logit.
-//   2  a histogram: for top-k of y, for top-p of the weights by their exponents
-//      and first three bits, in 2^-15 of the exponent's power (a 6e-5th is
-//      allowed for that).  Its sums from the top say which bins hold the cut, and
-//      a search among floats, by the same function, which logits begin and end
-//      them.
-//   3  the tokens of those bins (or of all bins down to there, if they are few,
-//      for top-k and top-p at once) are sorted by one CTA and added up exactly,
-//      beginning with the exact weight above them.  If they are too many, as in rows of equal logits,
-//      halving steps on (logit, index) come before.
-//   4  sums of the kept weights by index, the token in whose part u falls.
+//   2  a histogram.  For top-k of the threads' largest logits by y: the k-th of
+//      them is a lower bound of the k-th of all that few more logits pass.  Where
+//      k is too large for that, of all logits.  For top-p of all weights, made in
+//      f32, by their exponents and first five bits, in 2^-15 of the exponent's
+//      power (a 6e-5th is allowed for all that).  Its sums from the top say which
+//      bins hold the cut, and a search among floats, by the same function, which
+//      logits begin and end them.
+//   3  one pass makes the exact sums of all weights and of those before the bins
+//      in question, and collects these bins' tokens in one CTA, which sorts them
+//      and adds them up.  If they are too many, as in rows of equal logits, halving
+//      steps on (logit, index) come before.  Where nothing is before them, as for
+//      top-k, that CTA has all it needs for top-p and the token, too.
+//   4  else sums of the kept weights by index, the token in whose part u falls.
 // A token depends on sums of a whole vocabulary next to whose borders u may lie:
 // at 128256 borders an error of 2^-24 would change one token in a hundred.  So
 // weights are made in double, 2^y from a table and a few terms of the series
@@ -39,8 +42,9 @@ namespace {
 typedef unsigned long long u64;
 
 constexpr int ST = 512, SW = ST / 32;  // threads, warps
-constexpr int BINS = 512, CAP = 512;   // of the histogram; tokens that one CTA sorts
-static_assert(BINS == ST && CAP == ST, "a bin and a sorted token a thread");
+constexpr int BINS = 1024, CAP = 512;  // of the histogram; tokens that one CTA sorts
+constexpr int FEW = 128;               // that one warp sorts
+static_assert(BINS == 2 * ST && CAP == ST, "two bins and a sorted token a thread");
 constexpr int TB = 4, TABLE = 1 << TB;  // table of 2^(i / TABLE): 16 entries of 8 bytes are in different banks
 constexpr float MARGIN = 6e-5f;        // of sums of the histogram's weights, with 16 bits of each
 constexpr int LAST = 0x7fffffff;
@@ -51,7 +55,8 @@ struct SampleK {
   long long stride;
   int n, cluster, seg;   // seg: positions a CTA, whole 16-byte vectors
   int q;                 // fixed-point bits of a weight
-  int drop;              // bits of a weight's 21 that the histogram leaves out
+  int drop;              // bits of a weight's 24 that the histogram leaves out
+  float margin;          // what its sums may be off by
   pk_sample_args p;
 };
 
@@ -59,10 +64,11 @@ struct Smem {  // behind the row's values
   uint32_t hist[2][BINS];  // of even and of odd lanes, which then collide less
   u64 cand[CAP];
   double table[TABLE];
-  u64 warp[SW], x[6];   // of the CTA's warps; what the cluster's CTAs tell each other
+  u64 warp[SW], warpb[SW], told[2], x[6];   // of the CTA's warps; what the cluster's CTAs tell each other
   double off_min, off_low;
   uint32_t warp2[SW], n_cand, lo, hi, at, above, first;
   float warpf[SW], cut_x, edge[2];
+  uint32_t n_all;
   int cut_i;
 };
 
@@ -87,6 +93,46 @@ __device__ __forceinline__ uint32_t peer32(const void *p, int rank) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(map_rank(shaddr(p), rank)) : "memory");
   return v;
+}
+
+// Lane l holds elements l, 32 + l ..: sorted, the largest first.
+template <int J>
+__device__ __forceinline__ void sort_warp(u64 (&v)[J], int lane) {
+#pragma unroll
+  for (int size = 2; size <= 32 * J; size *= 2)
+#pragma unroll
+    for (int j = size / 2; j > 0; j /= 2)
+#pragma unroll
+      for (int i = 0; i < J; i++) {
+        const bool down = ((i * 32 + (size < 32 ? lane : 0)) & size) == 0;
+        const bool falls = size < 32 ? (lane & size) == 0 : down;
+        if (j >= 32) {
+          const int o = i ^ (j / 32);
+          if (o > i) {
+            const u64 a = v[i], b = v[o];
+            v[i] = falls ? max(a, b) : min(a, b);
+            v[o] = falls ? min(a, b) : max(a, b);
+          }
+        } else {
+          const u64 o = __shfl_xor_sync(0xffffffffu, v[i], j);
+          v[i] = falls == ((lane & j) == 0) ? max(v[i], o) : min(v[i], o);
+        }
+      }
+}
+// Inclusive sums in that order.
+template <int J>
+__device__ __forceinline__ void scan_warp(u64 (&v)[J], int lane) {
+  u64 before = 0;
+#pragma unroll
+  for (int i = 0; i < J; i++) {
+#pragma unroll
+    for (int j = 1; j < 32; j *= 2) {
+      const u64 y = __shfl_up_sync(0xffffffffu, v[i], j);
+      if (lane >= j) v[i] += y;
+    }
+    v[i] += before;
+    before = __shfl_sync(0xffffffffu, v[i], 31);
+  }
 }
 
 template <class E> constexpr int VE = 16 / (int)sizeof(E);
@@ -214,6 +260,35 @@ struct Row {
     }
   }
   __device__ __forceinline__ u64 all_sum(int i) const { return sum_warp(lane < a.cluster ? peer64(&sm.x[i], lane) : 0); }
+  // The CTA's n values (0 behind them), the largest first.  Each warp sorts its 32
+  // and finds how many of the other lists' are before each of them.
+  __device__ __forceinline__ u64 sorted(u64 v, int n) const {
+    const int lists = (n + 31) / 32;
+    u64 *out = reinterpret_cast<u64 *>(sm.hist[0]);  // (which has been read)
+    static_assert(sizeof(sm.hist[0]) >= CAP * sizeof(u64), "room");
+    __syncthreads();
+    if (warp < lists) {
+      u64 one[1] = {v};
+      sort_warp(one, lane);
+      sm.cand[tid] = v = one[0];
+    }
+    __syncthreads();
+    if (warp < lists) {
+      int place = lane;
+#pragma unroll 4
+      for (int w = 0; w < lists; w++) {
+        const u64 *o = sm.cand + 32 * w;
+        int b = 0;
+#pragma unroll
+        for (int j = 16; j > 0; j /= 2) b += o[b + j - 1] > v ? j : 0;
+        b += o[b] > v;
+        place += w == warp ? 0 : b;
+      }
+      if (v) out[place] = v;
+    }
+    __syncthreads();
+    return tid < n ? out[tid] : 0;
+  }
   // exclusive sums over the CTA's threads
   __device__ __forceinline__ u64 scan(u64 v) const {
     u64 x = v;
@@ -230,6 +305,12 @@ struct Row {
     return before + x - v;
   }
 };
+
+// The first token whose sum passes floor(u W) passes u W (u below 0 and NaN: the first).
+__device__ __forceinline__ u64 pass_of(float u, u64 all) {
+  const double goal = (double)u * (double)all;
+  return min(goal > 0.0 ? (goal < 9.2e18 ? (u64)goal : all) : 0, all - 1);
+}
 
 template <class E, bool BIG>
 __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
@@ -267,7 +348,8 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
   r.scale = 1.4426950408889634074 / (double)temp;
   if (tid < TABLE) sm.table[tid] = exp2((double)tid / TABLE + (double)a.q);
   if (tid == ST - 1) {
-    sm.n_cand = 0;
+    sm.n_cand = sm.n_all = 0;
+    sm.told[0] = sm.told[1] = 0;
     sm.first = LAST;
     sm.off_min = log2((double)min_p) / r.scale;  // w >= min_p where x >= top + this
     sm.off_low = (a.q + 2.0) / r.scale;          // what is further below rounds to nothing
@@ -277,8 +359,8 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
   __syncthreads();
 
   // ---- 1: the largest
+  float best = -CUDART_INF_F;  // of this thread's
   {
-    float best = -CUDART_INF_F;
     r.each4([&](const float *x, int) { best = fmaxf(fmaxf(best, fmaxf(x[0], x[1])), fmaxf(x[2], x[3])); });
     const uint32_t k = __reduce_max_sync(0xffffffffu, key_of(best));
     if (lane == 0) sm.warp2[warp] = k;
@@ -326,47 +408,51 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
 
   // ---- 2, 3: the cut of top-k, then of top-p
   bool do_k = top_k > 0 && top_k < a.n, do_p = top_p < 1.0f;
-  // bins of 1/16 nat for top-k: to the nearest, by an addition in which the
+  // bins of 1/32 nat for top-k: to the nearest, by an addition in which the
   // sum's last bits are the number (what the constant loses shifts all alike)
-  const float per_unit = fmaxf(fminf(16.0f / temp, 1e30f), 1e-38f);
+  const float per_unit = fmaxf(fminf(32.0f / temp, 1e30f), 1e-38f);
   const float bias = fminf(fmaxf(rintf(r.top * per_unit), -4e6f), 4e6f);
   const bool near = fabsf(r.top * per_unit) < 4e6f;
   auto bin_k = [&](float x) {
     const float d = near ? fmaf(x, -per_unit, bias) : x == r.top ? 0.0f : (r.top - x) * per_unit;
-    return __float_as_uint(fminf(fmaxf(d, 0.0f), (float)(BINS - 1)) + 8388608.0f) & 1023u;  // (NaN, of infinities: 0)
+    return (int)(__float_as_uint(fminf(fmaxf(d, 0.0f), (float)(BINS - 1)) + 8388608.0f) & 2047u);  // (NaN, of infinities: 0)
   };
-  // for top-p by the weight's exponent and three bits: bin 0 has the largest
-  const int hi_top = __double2hiint(r.weight(r.top)) >> 17;
-  auto bin_p = [&](double w) { return (uint32_t)min(hi_top - (__double2hiint(w) >> 17), BINS - 1); };
+  // for top-p by the f32 weight's exponent and five bits: bin 0 is 1; the last
+  // one's, below 2^-31, are not counted
+  const float slope = (float)r.scale;
+  auto weight_p = [&](float x) {
+    float y = (x - r.top) * slope, w;
+    if (inf) y = x == r.top ? 0.0f : -200.0f;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(y));
+    return __float_as_uint(w);
+  };
+  auto bin_p = [&](uint32_t w) { return min((127 << 5) - (int)(w >> 18), BINS - 1); };
   float before_x = CUDART_NAN_F;  // logits from here on are before those in question
-  bool added = false;             // sum and n have them
-  u64 sum = 0;
+  u64 sum = 0;                    // their weights and number
   uint32_t n = 0;
+  bool maxima = do_k && top_k <= ST * a.cluster / 4;  // of the threads' first
   for (bool again = false; do_k || do_p; again = true) {
-    const bool weigh = !do_k;  // top-p of all that is kept: their exact weight
+    const bool weigh = !do_k;  // top-p of all that is kept
     if (again) {
       r.sync();  // (the histogram has been read)
       for (int i = tid; i < 2 * BINS; i += ST) sm.hist[0][i] = 0;
-      if (tid == 0) sm.n_cand = 0;
+      if (tid == 0) sm.n_cand = sm.n_all = 0, sm.told[0] = sm.told[1] = 0;
       __syncthreads();
     }
     uint32_t *hist = sm.hist[lane & 1];
-    u64 weight = 0;
     if (weigh) {
-      r.as_exact([&](auto ex) {
-        r.each4([&](const float *x, int i) {
-          bool on[4];
-          r.kept4(x, i, on);
+      r.each4([&](const float *x, int i) {
+        bool on[4];
+        r.kept4(x, i, on);
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const double w = r.template weight_as<decltype(ex)::value>(on[e] ? fmaxf(x[e], r.none) : r.none);
-            weight += r.raw(w) - r.ONE;
-            if (on[e] && x[e] >= r.low) atomicAdd(hist + bin_p(w), ((__double2hiint(w) & 0xfffffu) | 0x100000u) >> a.drop);
-          }
-        });
+        for (int e = 0; e < 4; e++) {
+          const uint32_t w = weight_p(x[e]);
+          const int b = bin_p(w);
+          if (on[e] && b < BINS - 1) atomicAdd(hist + b, ((w & 0x7fffffu) | 0x800000u) >> a.drop);
+        }
       });
-      weight = r.sum_warp(weight);
-      if (lane == 0) sm.warp[warp] = weight;
+    } else if (maxima) {
+      if (best >= r.cx) atomicAdd(hist + bin_k(best), 1u);
     } else {
       r.each4([&](const float *x, int i) {
         bool on[4];
@@ -378,30 +464,30 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
     }
     __syncthreads();
     sm.hist[0][tid] += sm.hist[1][tid];
-    if (weigh && warp == 0) {
-      weight = r.sum_warp(lane < SW ? sm.warp[lane] : 0);
-      if (lane == 0) sm.x[1] = weight;
-    }
+    sm.hist[0][tid + ST] += sm.hist[1][tid + ST];
     if (tid == 0) sm.lo = sm.hi = BINS - 1;
     r.sync();
-    if (weigh) weight = r.all_sum(1);
-    // bin tid of the whole row, and the sums down to it: tokens (for top-p, what
-    // they are at the most), weights
-    uint32_t c = 0;
-    float m = 0.0f;
+    // bins 2 tid and 2 tid + 1 of the whole row, and the sums down to them: tokens
+    // (for top-p, what they are at the most), weights
+    uint32_t c[2] = {0, 0};
+    float m[2] = {0.0f, 0.0f};
     {
-      uint32_t v[8];
+      u64 v[8];
 #pragma unroll
-      for (int k = 0; k < 8; k++) v[k] = k < a.cluster ? peer32(&sm.hist[0][tid], k) : 0;
+      for (int k = 0; k < 8; k++) v[k] = k < a.cluster ? peer64(&sm.hist[0][2 * tid], k) : 0;
 #pragma unroll
-      for (int k = 0; k < 8; k++) {
-        m += (float)v[k];
-        c += weigh ? v[k] >> (20 - a.drop) : v[k];
-      }
-      m *= exp2f((float)(((hi_top - tid) >> 3) - (hi_top >> 3)));
+      for (int k = 0; k < 8; k++)
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const uint32_t x = (uint32_t)(v[k] >> (32 * j));
+          m[j] += (float)x;
+          c[j] += weigh ? x >> (23 - a.drop) : x;
+        }
+#pragma unroll
+      for (int j = 0; j < 2; j++) m[j] *= exp2f((float)(-((2 * tid + j + 31) >> 5)));
     }
-    uint32_t cs = c;
-    float ms = m;
+    uint32_t cs = c[0] + c[1];
+    float ms = m[0] + m[1];
 #pragma unroll
     for (int i = 1; i < 32; i *= 2) {
       const uint32_t y = __shfl_up_sync(0xffffffffu, cs, i);
@@ -419,11 +505,16 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
       mass += sm.warpf[w];
     }
     cs += cb, ms += mb;
-    const uint32_t k = min((uint32_t)top_k, total);
     // (sums of weights need not ascend by the last bit: the first bin that passes)
+    const uint32_t k = (uint32_t)top_k;
     uint32_t l = BINS - 1, h = BINS - 1;
-    if (do_k ? cs >= k : ms >= mass * top_p * (1.0f - MARGIN)) l = tid;
-    if (do_k ? cs >= k : ms >= mass * top_p * (1.0f + MARGIN)) h = tid;
+#pragma unroll
+    for (int j = 1; j >= 0; j--) {
+      const uint32_t cj = j ? cs : cs - c[1];
+      const float mj = j ? ms : ms - m[1];
+      if (do_k ? cj >= k : mj >= mass * top_p * (1.0f - a.margin)) l = 2 * tid + j;
+      if (do_k ? cj >= k : mj >= mass * top_p * (1.0f + a.margin)) h = 2 * tid + j;
+    }
     l = __reduce_min_sync(0xffffffffu, l);
     h = __reduce_min_sync(0xffffffffu, h);
     if (lane == 0 && l < BINS - 1) atomicMin(&sm.lo, l);
@@ -431,19 +522,16 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
     __syncthreads();
     const int hi = (int)sm.hi;
     int lo = (int)sm.lo;
-    if (tid == hi) sm.at = cs;
-    if (tid == lo) sm.above = cs - c;
+    if (tid == hi / 2) sm.at = hi & 1 ? cs : cs - c[1];
+    if (tid == lo / 2) sm.above = cs - c[1] - (lo & 1 ? 0 : c[0]);
     __syncthreads();
-    const uint32_t down = sm.at;  // tokens down to bin hi
-    uint32_t above = sm.above;    // before bin lo
-    if (do_k && (uint32_t)top_k >= total && down > CAP) {  // top-k keeps them all
+    if (do_k && !maxima && k >= total && total > CAP) {  // top-k keeps them all
       do_k = false;
       continue;
     }
-    const bool whole = down <= CAP;
+    uint32_t above = sm.above;  // tokens before bin lo (top-k of all)
+    const bool whole = maxima || (sm.at <= CAP && (do_k || hi < BINS - 1));  // all down to there, if they are few
     if (whole) lo = 0, above = 0;
-    const bool both = do_k && do_p && whole;
-    uint32_t inside = down - above;
     // The least floats of bins below lo (that are before those in question) and
     // of bins up to hi, a warp each: 33 floats around where the bin should end,
     // or, if it does not there, 33 that divide all, and so on.
@@ -451,17 +539,15 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
       const int b = warp == 0 ? lo - 1 : hi;
       auto in = [&](uint32_t key) {
         const float x = of_key(key);
-        return (int)(do_k ? bin_k(x) : x >= r.low ? bin_p(r.weight(x)) : (uint32_t)(BINS - 1)) <= b;
+        return (do_k ? bin_k(x) : bin_p(weight_p(x))) <= b;
       };
       const uint32_t least = key_of(-CUDART_INF_F);
       uint32_t from = least, to = key_of(r.top);  // (of which one is not looked at, the other is in bin 0)
       if (b < 0 || b == BINS - 1) {
         from = to = b < 0 ? 0 : key_of(-MAXF);
       } else {
-        double g;
-        if (do_k) g = ((double)bias - b - 0.5) / (double)per_unit;
-        else g = (log2(__hiloint2double((hi_top - b) << 17, 0)) - a.q) * TABLE;
-        if (!do_k) g = r.exact ? (double)r.top + g / TABLE / r.scale : (g - (r.zero - 6755399441055744.0)) / r.step;
+        const double g = do_k ? ((double)bias - b - 0.5) / (double)per_unit
+                              : (double)r.top + (double)log2f(__uint_as_float((uint32_t)((127 << 5) - b) << 18)) / (double)slope;
         const uint32_t at = min(max(key_of((float)g), least + 17), to - min(to - least - 17, 16u));
         const bool here = lane == 0 ? !in(at - 16) : lane == 1 ? in(at + 16) : true;
         if (to - least > 64 && __all_sync(0xffffffffu, here)) from = at - 16, to = at + 16;
@@ -479,51 +565,100 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
     __syncthreads();
     before_x = sm.edge[0];
     const float last_x = weigh ? fmaxf(sm.edge[1], r.low) : sm.edge[1];  // (what has no weight is not in the histogram)
-    // (by logits, or after halving by order) is it in question? is it before?
-    u64 o_lo = 0, o_hi = ~0ull, base_w = 0;
-    bool by_order = false;
-    auto side = [&](float x, int i) {  // 0: in question, 1: before, -1: behind
-      if (by_order) {
-        const u64 o = order_of(x, i);
-        return o > o_hi ? 1 : o < o_lo ? -1 : 0;
-      }
-      return x >= before_x ? 1 : x >= last_x ? 0 : -1;
+
+    // ---- 3
+    const uint32_t to = map_rank(shaddr(&sm.cand[0]), 0), counter = map_rank(shaddr(&sm.n_cand), 0);
+    uint32_t taken = 0;
+    auto take = [&](float x, int i) {
+      uint32_t at;
+      asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(counter) : "memory");
+      if (at < CAP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + at * 8), "l"(order_of(x, i)) : "memory");
+      taken++;
     };
+    // so that every CTA has the number of all that were taken
+    auto tell_taken = [&]() {
+      taken = __reduce_add_sync(0xffffffffu, taken);
+      if (taken && lane < a.cluster) asm volatile("red.relaxed.cluster.shared::cluster.add.u32 [%0], %1;" ::"r"(map_rank(shaddr(&sm.n_all), lane)), "r"(taken) : "memory");
+    };
+    u64 weight = 0;
+    sum = 0;
+    n = 0;
+    if (weigh) {
+      r.as_exact([&](auto ex) {
+        uint32_t made = 0, made_before = 0;
+        r.each4([&](const float *x, int i) {
+          bool on[4];
+          r.kept4(x, i, on);
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const u64 w = r.raw(r.template weight_as<decltype(ex)::value>(on[e] ? fmaxf(x[e], r.none) : r.none));
+            weight += w;
+            if (on[e] && x[e] >= before_x) sum += w, made_before++;
+          }
+          made += 4;
+          if (x[0] >= last_x || x[1] >= last_x || x[2] >= last_x || x[3] >= last_x) {
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+              if (on[e] && x[e] >= last_x && !(x[e] >= before_x)) take(x[e], i + e);
+          }
+        });
+        weight -= made * r.ONE;
+        sum -= made_before * r.ONE;
+        n = made_before;
+      });
+      tell_taken();
+      const u64 w0 = r.sum_warp(weight), w1 = r.sum_warp(sum);
+      if (lane == 0) sm.warp[warp] = w0, sm.warpb[warp] = w1;
+      __syncthreads();
+      if (warp < 2) {
+        const u64 v = r.sum_warp(lane < SW ? (warp ? sm.warpb : sm.warp)[lane] : 0);
+        if (lane < a.cluster) asm volatile("red.relaxed.cluster.shared::cluster.add.u64 [%0], %1;" ::"r"(map_rank(shaddr(&sm.told[warp]), lane)), "l"(v) : "memory");
+      }
+    } else {
+      r.each4([&](const float *x, int i) {
+        if (!(x[0] >= last_x || x[1] >= last_x || x[2] >= last_x || x[3] >= last_x)) return;
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (x[e] >= last_x && !(x[e] >= before_x) && r.kept(x[e], i + e)) take(x[e], i + e);
+      });
+      tell_taken();
+    }
+    r.sync();
+    uint32_t inside = sm.n_all;
+    if (maxima && inside > CAP) {  // (equal logits, or thousands near the threads' k-th)
+      maxima = false;
+      continue;
+    }
+    if (whole && inside <= CAP && rank > 0) return;  // (the first CTA has all that it needs)
+    weight = sm.told[0];
+    u64 base_w = sm.told[1];
     const double target = (double)top_p * (double)weight;
-    if (inside > CAP) {
-      // Halving.  The order's bounds first, and the exact weight before them.
-      u64 least = ~0ull, most = 0, before = 0, n_in = 0;
+    u64 o_lo = 0, o_hi = ~0ull;
+    const bool halve = inside > CAP;
+    if (halve) {
+      // The order's bounds of those in question first.
+      u64 least = ~0ull, most = 0;
+      auto asked = [&](float x, int i) { return x >= last_x && !(x >= before_x) && r.kept(x, i); };
       r.each([&](float x, int i) {
-        if (!r.kept(x, i)) return;
-        const int s = side(x, i);
-        if (s == 0) n_in++, least = min(least, order_of(x, i)), most = max(most, order_of(x, i));
-        if (s > 0 && weigh) before += r.fixed(x);
+        if (asked(x, i)) least = min(least, order_of(x, i)), most = max(most, order_of(x, i));
       });
 #pragma unroll
       for (int j = 16; j > 0; j >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, j)), most = max(most, __shfl_xor_sync(0xffffffffu, most, j));
-      __syncthreads();
-      r.sum_to(before, 2);
-      __syncthreads();
-      r.sum_to(n_in, 5);
-      __syncthreads();
       if (tid == 0) sm.x[3] = ~0ull, sm.x[4] = 0;
       __syncthreads();
       if (lane == 0) atomicMin(&sm.x[3], least), atomicMax(&sm.x[4], most);
       r.sync();
-      base_w = r.all_sum(2);
-      inside = (uint32_t)r.all_sum(5);
       for (int j = 0; j < a.cluster; j++) {
         const u64 x = peer64(&sm.x[3], j), y = peer64(&sm.x[4], j);
         if (j == 0 || x < o_lo) o_lo = x;
         if (j == 0 || y > o_hi) o_hi = y;
       }
-      by_order = true;
       r.sync();  // (the slots are written again)
       for (int turn = 0; inside > CAP && turn < 64; turn++) {  // (orders differ: 63 at most)
         const u64 mid = o_lo + (o_hi - o_lo) / 2;
         u64 n_up = 0, w_up = 0;
         r.each([&](float x, int i) {
-          if (!r.kept(x, i)) return;
+          if (!asked(x, i)) return;
           const u64 o = order_of(x, i);
           if (o > mid && o <= o_hi) {
             n_up++;
@@ -549,104 +684,121 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
           base_w += w_up;
         }
       }
+      if (tid == 0) sm.n_cand = 0;
+      r.sync();
+      r.each([&](float x, int i) {
+        if (asked(x, i) && order_of(x, i) >= o_lo && order_of(x, i) <= o_hi) take(x, i);
+      });
       r.sync();
     }
-    // the tokens in question to the first CTA, and the exact weight before them
-    added = weigh && !by_order;
-    sum = 0;
-    n = 0;
-    const uint32_t to = map_rank(shaddr(&sm.cand[0]), 0), counter = map_rank(shaddr(&sm.n_cand), 0);
-    auto take = [&](float x, int i) {
-      uint32_t at;
-      asm volatile("atom.relaxed.cluster.shared::cluster.add.u32 %0, [%1], 1;" : "=r"(at) : "r"(counter) : "memory");
-      if (at < CAP) asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(to + at * 8), "l"(order_of(x, i)) : "memory");
-    };
-    if (by_order) {
-      r.each([&](float x, int i) {
-        if (r.kept(x, i) && side(x, i) == 0) take(x, i);
-      });
-    } else {
-      r.as_exact([&](auto ex) {
-        r.each4([&](const float *x, int i) {
-          if (!(x[0] >= last_x || x[1] >= last_x || x[2] >= last_x || x[3] >= last_x)) return;
-          bool on[4], before[4];
-          r.kept4(x, i, on);
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            before[e] = on[e] && x[e] >= before_x;
-            n += before[e];
-            if (on[e] && !before[e] && x[e] >= last_x) take(x[e], i + e);
-          }
-          if (added) r.template add4<decltype(ex)::value>(x, before, sum);
-        });
-      });
-      if (added) r.sum_to(sum, 5);
-    }
-    r.sync();
-    u64 *sorted = reinterpret_cast<u64 *>(sm.hist[0]);  // (which has been read)
-    static_assert(sizeof(sm.hist) >= CAP * sizeof(u64), "room");
+    const bool last = whole && !halve;  // the first CTA goes on to the token
     if (rank == 0) {
-      if (added) base_w = r.all_sum(5);
-      const int nc = min((int)sm.n_cand, CAP), lists = (nc + 31) / 32;
-      u64 v = tid < nc ? sm.cand[tid] : 0;
-      __syncthreads();
-      if (warp < lists) {  // each warp sorts its 32
+      const int nc = min((int)sm.n_cand, CAP);
+      if (nc <= FEW) {
+        if (warp == 0) {
+          auto few = [&](auto j) {
+            constexpr int J = decltype(j)::value;
+            u64 v[J], w[J], s[J];
 #pragma unroll
-        for (int size = 2; size <= 32; size *= 2)
+            for (int i = 0; i < J; i++) v[i] = 32 * i + lane < nc ? sm.cand[32 * i + lane] : 0;
+            sort_warp(v, lane);
+            int cut = do_k ? min(nc, (int)(k - above)) : nc;  // how many are kept
+            if (!do_k || last) {
 #pragma unroll
-          for (int j = size / 2; j > 0; j /= 2) {
-            const u64 o = __shfl_xor_sync(0xffffffffu, v, j);
-            const bool down_here = (lane & size) == 0, low_half = (lane & j) == 0;
-            v = down_here == low_half ? max(v, o) : min(v, o);
-          }
-        sm.cand[tid] = v;
-      }
-      __syncthreads();
-      if (warp < lists) {  // and finds how many of the other lists' are before each
-        int place = lane;
-#pragma unroll 4
-        for (int w = 0; w < lists; w++) {
-          const u64 *o = sm.cand + 32 * w;
-          int b = 0;
+              for (int i = 0; i < J; i++) s[i] = w[i] = 32 * i + lane < cut ? r.fixed(of_key((uint32_t)(v[i] >> 32))) : 0;
+              scan_warp(s, lane);
+              if (do_p) {  // up to the first with which they have top_p of the weight
+                const double goal = do_k ? (double)top_p * (double)__shfl_sync(0xffffffffu, s[J - 1], 31) : target;
+                int first = cut - 1;
 #pragma unroll
-          for (int j = 16; j > 0; j /= 2) b += o[b + j - 1] > v ? j : 0;
-          b += o[b] > v;
-          place += w == warp ? 0 : b;
+                for (int i = J - 1; i >= 0; i--) {
+                  const uint32_t lanes = __ballot_sync(0xffffffffu, 32 * i + lane < cut && (double)(base_w + s[i]) >= goal);
+                  if (lanes) first = 32 * i + __ffs(lanes) - 1;
+                }
+                cut = first + 1;
+              }
+            }
+            if (!last) {
+#pragma unroll
+              for (int i = 0; i < J; i++)
+                if (32 * i + lane == cut - 1) sm.cut_x = of_key((uint32_t)(v[i] >> 32)), sm.cut_i = (int)~(uint32_t)v[i];
+              return;
+            }
+            // the kept ones by index (the largest first: from the least ~index on), and the one where u falls
+            u64 *few_w = reinterpret_cast<u64 *>(sm.hist[1]), all_w = 0;
+#pragma unroll
+            for (int i = 0; i < J; i++) {
+              const int at = 32 * i + lane;
+              if (at < cut) all_w += w[i];
+              few_w[at] = w[i];
+              v[i] = at < cut ? (u64)(uint32_t)v[i] << 10 | (uint32_t)at : 0;
+            }
+            __syncwarp();
+            all_w = r.sum_warp(all_w);
+            sort_warp(v, lane);
+#pragma unroll
+            for (int i = 0; i < J; i++) s[i] = w[i] = v[i] ? few_w[v[i] & 1023] : 0;
+            scan_warp(s, lane);
+            const u64 pass = pass_of(u, all_w);
+#pragma unroll
+            for (int i = 0; i < J; i++)
+              if (w[i] && pass < s[i] && pass >= s[i] - w[i]) {
+                a.p.tok[row] = (int)~(uint32_t)(v[i] >> 10);
+                if (a.p.prob) a.p.prob[row] = (float)((double)w[i] / (double)all_w);
+                if (a.p.kept) a.p.kept[row] = cut;
+              }
+          };
+          if (nc <= 32) few(std::integral_constant<int, 1>{});
+          else if (nc <= 64) few(std::integral_constant<int, 2>{});
+          else few(std::integral_constant<int, 4>{});
         }
-        __syncwarp();
-        if (v) sorted[place] = v;
-      }
-      __syncthreads();
-      v = tid < nc ? sorted[tid] : 0;
-      const float x = of_key((uint32_t)(v >> 32));
-      // the last one that top-k leaves
-      const int most = do_k ? min(nc, (int)(k - above)) : nc;
-      int cut = most - 1;
-      if (!do_k || both) {
-        const u64 w = tid < most ? r.fixed(x) : 0, b = r.scan(w);
-        double goal = target;
-        if (both) {
+      } else {
+        // the same with a thread for each
+        u64 v = r.sorted(tid < nc ? sm.cand[tid] : 0, nc);
+        int cut = do_k ? min(nc, (int)(k - above)) : nc;
+        u64 w = 0, all_w = 0;
+        if (!do_k || last) {
+          w = tid < cut ? r.fixed(of_key((uint32_t)(v >> 32))) : 0;
+          const u64 b = r.scan(w);
           if (tid == ST - 1) sm.x[4] = b + w;
+          if (tid == 0) sm.at = (uint32_t)cut - 1;
           __syncthreads();
-          goal = (double)top_p * (double)sm.x[4];
+          all_w = sm.x[4];
+          __syncthreads();
+          if (do_p) {
+            const double goal = do_k ? (double)top_p * (double)all_w : target;
+            if (tid < cut && (double)(base_w + b + w) >= goal && (tid == 0 || (double)(base_w + b) < goal)) sm.at = (uint32_t)tid, sm.x[4] = b + w;
+            __syncthreads();
+            cut = (int)sm.at + 1;
+            all_w = sm.x[4];
+          }
         }
-        if (tid == 0) sm.at = (uint32_t)cut;
-        __syncthreads();
-        if (tid < most && (double)(base_w + b + w) >= goal && (tid == 0 || (double)(base_w + b) < goal)) sm.at = (uint32_t)tid;
-        __syncthreads();
-        cut = (int)sm.at;
+        if (!last) {
+          if (tid == cut - 1) sm.cut_x = of_key((uint32_t)(v >> 32)), sm.cut_i = (int)~(uint32_t)v;
+        } else {
+          u64 *few_w = reinterpret_cast<u64 *>(sm.hist[1]);
+          few_w[tid] = w;
+          v = r.sorted(tid < cut ? (u64)(uint32_t)v << 10 | (uint32_t)tid : 0, cut);
+          w = v ? few_w[v & 1023] : 0;
+          const u64 b = r.scan(w), pass = pass_of(u, all_w);
+          if (w && pass >= b && pass < b + w) {
+            a.p.tok[row] = (int)~(uint32_t)(v >> 10);
+            if (a.p.prob) a.p.prob[row] = (float)((double)w / (double)all_w);
+            if (a.p.kept) a.p.kept[row] = cut;
+          }
+        }
       }
-      if (tid == cut) sm.cut_x = x, sm.cut_i = (int)~(uint32_t)v;
+      if (last) return;
     }
     r.sync();
     r.cx = __uint_as_float(peer32(&sm.cut_x, 0));
     r.ci = (int)peer32(&sm.cut_i, 0);
-    if (do_k && !both) do_k = false;
-    else do_k = do_p = false;
+    if (do_k) do_k = maxima = false;
+    else do_p = false;
   }
 
-  // ---- 4: the kept weights by index (of what came before the tokens in question they are there)
-  if (!added) sum = 0, n = 0, before_x = CUDART_NAN_F;
+  // ---- 4: the kept weights by index (of what came before top-p's tokens in question they are there)
+  if (!(top_p < 1.0f)) sum = 0, n = 0, before_x = CUDART_NAN_F;
   r.as_exact([&](auto ex) {
     if (r.ci == LAST && r.cx <= r.none) {  // nothing is cut off that has a weight
       uint32_t made = 0;
@@ -699,10 +851,7 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
       all_n += c[j];
     }
   }
-  // the first token whose sum passes floor(u W) passes u W (u below 0 and NaN: the first)
-  const double goal = (double)u * (double)all_w;
-  u64 pass = goal > 0.0 ? (goal < 9.2e18 ? (u64)goal : all_w) : 0;
-  pass = min(pass, all_w - 1);
+  const u64 pass = pass_of(u, all_w);
   if (pass >= before && pass - before < sm.x[2]) {  // one CTA: of the warp in whose run it falls all threads take a vector
     u64 from = before;
     int w = 0;
@@ -764,9 +913,10 @@ cudaError_t launch_sample(const void *logits, int type, int rows, int n, long st
   const bool big = seg > wide;
   a.cluster = (int)c;
   a.seg = (int)(seg * v);
-  // 21 bits of a weight, of which 16 are kept: 65536 of a bin and CTA fit 32 bits
-  a.drop = 5;
+  // 24 bits of a weight, of which 16 are kept: 65536 of a bin and CTA fit 32 bits
+  a.drop = 8;
   for (long long x = 65536; x < a.seg; x *= 2) a.drop++;
+  a.margin = MARGIN + (float)n * 0x1p-31f;
   const int smem = (int)sizeof(Smem) + (big ? 0 : (int)(seg * 16));
   const dim3 grid((unsigned)(rows * c)), block(ST);
 #define GO(E) launch_cluster(big ? k_sample<E, true> : k_sample<E, false>, (int)c, grid, block, smem, st, a)
