@@ -15,8 +15,8 @@
 //      logits begin and end them.
 //   3  one pass makes the exact sums of all weights and of those before the bins
 //      in question, and collects these bins' tokens in one CTA, which sorts them
-//      and adds them up.  If they are too many, as in rows of equal logits, halving
-//      steps on (logit, index) come before.  Where nothing is before them, as for
+//      and adds them up.  If they are too many, as in rows of equal logits, exact
+//      histograms of 512 parts of the order come before.  Where nothing is before them, as for
 //      top-k, that CTA has all it needs for top-p and the token, too.
 //   4  else sums of the kept weights by index, the token in whose part u falls.
 // A token depends on sums of a whole vocabulary next to whose borders u may lie:
@@ -66,7 +66,8 @@ struct Smem {  // behind the row's values
   double table[TABLE];
   u64 warp[SW], warpb[SW], told[2], x[6];   // of the CTA's warps; what the cluster's CTAs tell each other
   double off_min, off_low;
-  uint32_t warp2[SW], n_cand, lo, hi, at, above, first;
+  u64 base_w;
+  uint32_t warp2[SW], n_cand, lo, hi, at, above, inside, first;
   float warpf[SW], cut_x, edge[2];
   uint32_t n_all;
   int cut_i;
@@ -159,24 +160,63 @@ struct Row {
     else asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   __device__ __forceinline__ E load(long long p) const { return p >= shift && p < end ? base[p - shift] : from_f<E>(-CUDART_INF_F); }
-  __device__ __forceinline__ void vec(int i, float (&x)[V]) const {  // vector i of this CTA
-    if (BIG) {
+  __device__ __forceinline__ uint4 words(int i) const {  // vector i of this CTA
+    if (!BIG) return data[i];
+    const long long p = (long long)p0 + (long long)i * V;
+    if (p >= shift && p + V <= end) return __ldcg(reinterpret_cast<const uint4 *>(base + (p - shift)));
+    uint4 w;
+    E *v = reinterpret_cast<E *>(&w);
 #pragma unroll
-      for (int e = 0; e < V; e++) x[e] = to_f(load((long long)p0 + (long long)i * V + e));
-    } else {
-      const uint4 w = data[i];
-      const E *v = reinterpret_cast<const E *>(&w);
-#pragma unroll
-      for (int e = 0; e < V; e++) x[e] = to_f(v[e]);
-    }
+    for (int e = 0; e < V; e++) v[e] = load(p + e);
+    return w;
   }
+  __device__ __forceinline__ void floats(const uint4 &w, float (&x)[V]) const {
+    const E *v = reinterpret_cast<const E *>(&w);
+#pragma unroll
+    for (int e = 0; e < V; e++) x[e] = to_f(v[e]);
+  }
+  __device__ __forceinline__ void vec(int i, float (&x)[V]) const { floats(words(i), x); }
   // f(four values, the first's token) for this thread's, in order.  NaN compares as false everywhere.
   template <class F>
   __device__ __forceinline__ void each4(F f) const {
     const int w1 = min(vecs, (warp + 1) * per);
-    for (int i = warp * per + lane; i < w1; i += 32) {
+    auto one = [&](int i, const uint4 &w) {
       float x[V];
-      vec(i, x);
+      floats(w, x);
+#pragma unroll
+      for (int e = 0; e < V; e += 4) f(x + e, p0 + i * V + e - shift);
+    };
+    int i = warp * per + lane;
+    if (BIG) {  // two vectors ahead
+      uint4 w[2];
+#pragma unroll
+      for (int j = 0; j < 2; j++) w[j] = i + 32 * j < w1 ? words(i + 32 * j) : uint4{};
+      for (; i < w1; i += 64) {
+#pragma unroll
+        for (int j = 0; j < 2; j++) {
+          const uint4 now = w[j];
+          const int next = i + 32 * j + 64;
+          if (next < w1) w[j] = words(next);
+          if (i + 32 * j < w1) one(i + 32 * j, now);
+        }
+      }
+    } else {
+      for (; i < w1; i += 32) one(i, words(i));
+    }
+  }
+  // the same for whole warps, with -inf past the end
+  template <class F>
+  __device__ __forceinline__ void each_warp(F f) const {
+    const int w1 = min(vecs, (warp + 1) * per);
+    for (int i0 = warp * per; i0 < w1; i0 += 32) {
+      const int i = i0 + lane;
+      float x[V];
+      if (i < w1) {
+        vec(i, x);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; e++) x[e] = -CUDART_INF_F;
+      }
 #pragma unroll
       for (int e = 0; e < V; e += 4) f(x + e, p0 + i * V + e - shift);
     }
@@ -312,7 +352,8 @@ __device__ __forceinline__ u64 pass_of(float u, u64 all) {
   return min(goal > 0.0 ? (goal < 9.2e18 ? (u64)goal : all) : 0, all - 1);
 }
 
-template <class E, bool BIG>
+// RULES: min_p, top_k or top_p are given.
+template <class E, bool BIG, bool RULES>
 __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
   constexpr int V = VE<E>;
   extern __shared__ __align__(16) uint8_t smem[];
@@ -343,8 +384,8 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
   const float u = __ldg(a.p.u + row), temp = a.p.temp ? __ldg(a.p.temp + row) : 1.0f;
-  const float top_p = a.p.top_p ? __ldg(a.p.top_p + row) : 1.0f, min_p = a.p.min_p ? __ldg(a.p.min_p + row) : 0.0f;
-  const int top_k = a.p.top_k ? __ldg(a.p.top_k + row) : 0;
+  const float top_p = RULES && a.p.top_p ? __ldg(a.p.top_p + row) : 1.0f, min_p = RULES && a.p.min_p ? __ldg(a.p.min_p + row) : 0.0f;
+  const int top_k = RULES && a.p.top_k ? __ldg(a.p.top_k + row) : 0;
   r.scale = 1.4426950408889634074 / (double)temp;
   if (tid < TABLE) sm.table[tid] = exp2((double)tid / TABLE + (double)a.q);
   if (tid == ST - 1) {
@@ -407,7 +448,7 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
   else r.zero -= rint((double)r.top * r.step);
 
   // ---- 2, 3: the cut of top-k, then of top-p
-  bool do_k = top_k > 0 && top_k < a.n, do_p = top_p < 1.0f;
+  bool do_k = RULES && top_k > 0 && top_k < a.n, do_p = RULES && top_p < 1.0f;
   // bins of 1/32 nat for top-k: to the nearest, by an addition in which the
   // sum's last bits are the number (what the constant loses shifts all alike)
   const float per_unit = fmaxf(fminf(32.0f / temp, 1e30f), 1e-38f);
@@ -430,7 +471,7 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
   float before_x = CUDART_NAN_F;  // logits from here on are before those in question
   u64 sum = 0;                    // their weights and number
   uint32_t n = 0;
-  bool maxima = do_k && top_k <= ST * a.cluster / 4;  // of the threads' first
+  bool maxima = do_k && top_k <= min(ST * a.cluster / 2, 352);  // of the threads' first (which 431 of all pass, on average, at the most)
   for (bool again = false; do_k || do_p; again = true) {
     const bool weigh = !do_k;  // top-p of all that is kept
     if (again) {
@@ -506,7 +547,7 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
     }
     cs += cb, ms += mb;
     // (sums of weights need not ascend by the last bit: the first bin that passes)
-    const uint32_t k = (uint32_t)top_k;
+    const uint32_t k = (uint32_t)max(top_k, 1);
     uint32_t l = BINS - 1, h = BINS - 1;
 #pragma unroll
     for (int j = 1; j >= 0; j--) {
@@ -584,28 +625,36 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
     sum = 0;
     n = 0;
     if (weigh) {
-      r.as_exact([&](auto ex) {
+      const bool plain = r.ci == LAST && r.cx <= r.none;  // nothing is cut off that has a weight
+      auto pass = [&](auto ex, auto pl) {
+        constexpr bool EX = decltype(ex)::value, PL = decltype(pl)::value;
         uint32_t made = 0, made_before = 0;
         r.each4([&](const float *x, int i) {
           bool on[4];
-          r.kept4(x, i, on);
+          float y[4];
+          if (!PL) r.kept4(x, i, on);
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const u64 w = r.raw(r.template weight_as<decltype(ex)::value>(on[e] ? fmaxf(x[e], r.none) : r.none));
+            y[e] = fmaxf(x[e], r.none);
+            if (!PL && !on[e]) y[e] = r.none;
+            const u64 w = r.raw(r.template weight_as<EX>(y[e]));
             weight += w;
-            if (on[e] && x[e] >= before_x) sum += w, made_before++;
+            if (y[e] >= before_x) sum += w, made_before++;
           }
           made += 4;
-          if (x[0] >= last_x || x[1] >= last_x || x[2] >= last_x || x[3] >= last_x) {
+          if (fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= last_x) {
 #pragma unroll
             for (int e = 0; e < 4; e++)
-              if (on[e] && x[e] >= last_x && !(x[e] >= before_x)) take(x[e], i + e);
+              if (y[e] >= last_x && !(y[e] >= before_x) && (PL || on[e])) take(x[e], i + e);
           }
         });
         weight -= made * r.ONE;
         sum -= made_before * r.ONE;
         n = made_before;
-      });
+      };
+      if (r.exact) pass(std::true_type{}, std::false_type{});
+      else if (plain) pass(std::false_type{}, std::true_type{});
+      else pass(std::false_type{}, std::false_type{});
       tell_taken();
       const u64 w0 = r.sum_warp(weight), w1 = r.sum_warp(sum);
       if (lane == 0) sm.warp[warp] = w0, sm.warpb[warp] = w1;
@@ -633,65 +682,87 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
     weight = sm.told[0];
     u64 base_w = sm.told[1];
     const double target = (double)top_p * (double)weight;
-    u64 o_lo = 0, o_hi = ~0ull;
-    const bool halve = inside > CAP;
-    if (halve) {
-      // The order's bounds of those in question first.
-      u64 least = ~0ull, most = 0;
-      auto asked = [&](float x, int i) { return x >= last_x && !(x >= before_x) && r.kept(x, i); };
-      r.each([&](float x, int i) {
-        if (asked(x, i)) least = min(least, order_of(x, i)), most = max(most, order_of(x, i));
-      });
+    const bool many = inside > CAP;
+    if (many) {
+      // The order's range is narrowed to one of 512 parts of it at a time, by their
+      // numbers of tokens and exact weights (seven times at the most).
+      u64 o_lo = order_of(last_x, LAST), o_hi = order_of(before_x == before_x ? before_x : r.top, 0);
+      uint32_t *part_n = sm.hist[0];
+      u64 *part_w = reinterpret_cast<u64 *>(sm.hist[1]);
+      static_assert(sizeof(sm.hist[1]) >= ST * sizeof(u64), "room");
+      auto asked = [&](float x, int i) {
+        if (!(x >= last_x) || x >= before_x || !r.kept(x, i)) return false;
+        const u64 o = order_of(x, i);
+        return o >= o_lo && o <= o_hi;
+      };
+      for (int turn = 0; inside > CAP && turn < 8; turn++) {
+        const int shift = max(0, 64 - 9 - __clzll((long long)(o_hi - o_lo)));
+        part_n[tid] = 0;
+        part_w[tid] = 0;
+        __syncthreads();
+        r.each_warp([&](const float *x, int i) {
 #pragma unroll
-      for (int j = 16; j > 0; j >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, j)), most = max(most, __shfl_xor_sync(0xffffffffu, most, j));
-      if (tid == 0) sm.x[3] = ~0ull, sm.x[4] = 0;
-      __syncthreads();
-      if (lane == 0) atomicMin(&sm.x[3], least), atomicMax(&sm.x[4], most);
-      r.sync();
-      for (int j = 0; j < a.cluster; j++) {
-        const u64 x = peer64(&sm.x[3], j), y = peer64(&sm.x[4], j);
-        if (j == 0 || x < o_lo) o_lo = x;
-        if (j == 0 || y > o_hi) o_hi = y;
-      }
-      r.sync();  // (the slots are written again)
-      for (int turn = 0; inside > CAP && turn < 64; turn++) {  // (orders differ: 63 at most)
-        const u64 mid = o_lo + (o_hi - o_lo) / 2;
-        u64 n_up = 0, w_up = 0;
-        r.each([&](float x, int i) {
-          if (!asked(x, i)) return;
-          const u64 o = order_of(x, i);
-          if (o > mid && o <= o_hi) {
-            n_up++;
-            if (weigh) w_up += r.fixed(x);
+          for (int e = 0; e < 4; e++) {
+            const bool on = asked(x[e], i + e);
+            const uint32_t lanes = __ballot_sync(0xffffffffu, on);
+            if (!lanes) continue;
+            const int part = (int)((o_hi - order_of(x[e], i + e)) >> shift);
+            const u64 w = on && weigh ? r.fixed(x[e]) : 0;
+            // (equal logits by thousands are in one part: one addition a warp)
+            const int first = __shfl_sync(0xffffffffu, part, __ffs(lanes) - 1);
+            if (__all_sync(0xffffffffu, !on || part == first)) {
+              const u64 all_w = r.sum_warp(w);
+              if (lane == 0) {
+                atomicAdd(part_n + first, (uint32_t)__popc(lanes));
+                if (weigh) atomicAdd(part_w + first, all_w);
+              }
+            } else if (on) {
+              atomicAdd(part_n + part, 1u);
+              if (weigh) atomicAdd(part_w + part, w);
+            }
           }
         });
-        // (slots in turn: a CTA may be a step ahead of one that still reads)
-        const int at = 2 + (turn & 1);
-        r.sum_to(n_up, at);
-        __syncthreads();
-        r.sum_to(w_up, at + 2);
         r.sync();
-        n_up = r.all_sum(at);
-        w_up = r.all_sum(at + 2);
-        const bool up = do_k ? above + n_up >= k : (double)(base_w + w_up) >= target;
-        if (up) {
-          o_lo = mid + 1;
-          inside = (uint32_t)n_up;
-        } else {
-          o_hi = mid;
-          inside -= (uint32_t)n_up;
-          above += (uint32_t)n_up;
-          base_w += w_up;
+        uint32_t c = 0;
+        u64 w = 0;
+        for (int j = 0; j < a.cluster; j++) c += peer32(part_n + tid, j), w += peer64(part_w + tid, j);
+        uint32_t cs = c;
+#pragma unroll
+        for (int i = 1; i < 32; i *= 2) {
+          const uint32_t y = __shfl_up_sync(0xffffffffu, cs, i);
+          if (lane >= i) cs += y;
         }
+        if (lane == 31) sm.warp2[warp] = cs;
+        if (tid == 0) sm.at = ~0u;
+        const u64 wb = base_w + r.scan(w);  // (its barriers order warp2 and at, too)
+        uint32_t cb = above + cs - c, all_c = above;
+        for (int i = 0; i < SW; i++) {
+          if (i < warp) cb += sm.warp2[i];
+          all_c += sm.warp2[i];
+        }
+        // the part with which the goal is reached; if none does, the last one
+        if (c && (do_k ? cb < k && cb + c >= k : (double)wb < target && (double)(wb + w) >= target)) sm.at = (uint32_t)tid, sm.above = cb, sm.inside = c, sm.base_w = wb;
+        __syncthreads();
+        const bool none = sm.at == ~0u;
+        __syncthreads();
+        if (none && c && cb + c == all_c) sm.at = (uint32_t)tid, sm.above = cb, sm.inside = c, sm.base_w = wb;
+        __syncthreads();
+        const u64 to = o_hi - ((u64)sm.at << shift), span = (1ull << shift) - 1;
+        o_lo = to - o_lo > span ? to - span : o_lo;
+        o_hi = to;
+        above = sm.above;
+        inside = sm.inside;
+        base_w = sm.base_w;
+        r.sync();  // (the parts have been read)
       }
       if (tid == 0) sm.n_cand = 0;
       r.sync();
       r.each([&](float x, int i) {
-        if (asked(x, i) && order_of(x, i) >= o_lo && order_of(x, i) <= o_hi) take(x, i);
+        if (asked(x, i)) take(x, i);
       });
       r.sync();
     }
-    const bool last = whole && !halve;  // the first CTA goes on to the token
+    const bool last = whole && !many;  // the first CTA goes on to the token
     if (rank == 0) {
       const int nc = min((int)sm.n_cand, CAP);
       if (nc <= FEW) {
@@ -813,13 +884,16 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
       sum -= made * r.ONE;
     } else {
       r.each4([&](const float *x, int i) {
-        if (!(x[0] >= r.cx || x[1] >= r.cx || x[2] >= r.cx || x[3] >= r.cx)) return;
-        bool on[4];
+        // (most are neither: that first)
+        bool on[4], any = false;
+#pragma unroll
+        for (int e = 0; e < 4; e++) any |= x[e] >= r.cx && !(RULES && x[e] >= before_x);
+        if (!any) return;
         r.kept4(x, i, on);
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          on[e] = on[e] && !(x[e] >= before_x);
-          n += on[e];
+          if (RULES) on[e] = on[e] && !(x[e] >= before_x);
+          n += on[e] ? 1 : 0;
         }
         r.template add4<decltype(ex)::value>(x, on, sum);
       });
@@ -904,7 +978,11 @@ cudaError_t launch_sample(const void *logits, int type, int rows, int n, long st
   int bits = 0;
   while ((1LL << bits) < n) bits++;
   a.q = std::min(50, 62 - bits);
-  // CTAs a row: by what they hold, two an SM, one where rows are longer; more where the rows leave SMs without any
+  // CTAs a row: by what they hold, two an SM, one where rows are longer; more
+  // where the rows leave SMs without any.  (250 f32 rows of 128256, each with its
+  // own rules: 6 CTAs 170 us, 4 193, and read again from L2 for every pass, 2 213
+  // and one 312, which waits for the longest row; 64 bf16 rows of 73448: 4 CTAs
+  // 56, 2 60, 6 77.)
   const long long vecs = ((long long)n + 2 * v - 2) / v, most = 96 * 1024 / 16, wide = 208 * 1024 / 16;
   long long c = std::min(8LL, (vecs + most - 1) / most);
   while (c < 8 && rows * c * 2 <= 296 && vecs >= 512 * c) c *= 2;
@@ -919,7 +997,8 @@ cudaError_t launch_sample(const void *logits, int type, int rows, int n, long st
   a.margin = MARGIN + (float)n * 0x1p-31f;
   const int smem = (int)sizeof(Smem) + (big ? 0 : (int)(seg * 16));
   const dim3 grid((unsigned)(rows * c)), block(ST);
-#define GO(E) launch_cluster(big ? k_sample<E, true> : k_sample<E, false>, (int)c, grid, block, smem, st, a)
+  const bool rules = p.top_k || p.top_p || p.min_p;
+#define GO(E) launch_cluster(rules ? big ? k_sample<E, true, true> : k_sample<E, false, true> : big ? k_sample<E, true, false> : k_sample<E, false, false>, (int)c, grid, block, smem, st, a)
   return type == T_F32 ? GO(float) : type == T_F16 ? GO(__half) : GO(__nv_bfloat16);
 #undef GO
 }
