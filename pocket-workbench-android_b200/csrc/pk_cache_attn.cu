@@ -477,11 +477,17 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
   using G = Geo<TYPE, DH, NT, NB, RG>;
   using T = typename G::T;
   extern __shared__ __align__(128) uint8_t smem[];
+  // (the launch after the prefixes' does not wait before it reads what they read,
+  // so theirs lets it begin only when all before them is done)
+  if (a.mode == ATTN_PREFIX) pdl_wait();
   pdl_trigger();
-  pdl_wait();
+  if (a.mode != ATTN_PREFIX && !a.early) pdl_wait();
   const Unit u = unit_of(a);
   const int tile0 = u.rt * G::ROWS;
-  if (idle(a, u, tile0)) return;
+  if (idle(a, u, tile0)) {
+    end_early(a);
+    return;
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int rg = warp % RG, kg = warp / RG, row0 = tile0 + rg * 8 * NB;
   // without a mask nobody sees past the tile's last token
@@ -557,6 +563,7 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
     }
   __syncthreads();
   const bool cluster = a.cluster && u.nch > 1;
+  if (a.merge && a.early) pdl_wait();
   for (int x = threadIdx.x; x < G::ROWS * 8; x += 32 * AW) {
     const int r = x >> 3, d0 = (x & 7) * (DH / 8);
     if (tile0 + r >= u.rows) continue;
@@ -584,6 +591,8 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
         const int i = (tile0 + r) / a.group, h = u.h * a.group + (tile0 + r) - i * a.group;
         a.part_ml[((long long)(u.sv.first + i) * a.q.n_head + h) * a.n_part + u.slot] = make_float2(M, L);
       }
+    } else if (a.merge) {
+      merge_in<DH / 8>(merge_of<DH>(a, u, tile0 + r, M, L), DH, d0, acc);
     } else {
       const float inv = L > 0.0f || isnan(L) ? 1.0f / L : 0.0f;
 #pragma unroll
@@ -591,6 +600,7 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
     }
     write_row<DH>(a, u, tile0 + r, d0, acc, u.part);
   }
+  if (!a.merge) end_early(a);
   if (cluster) join_cluster<DH>(a, u, tile0, G::ROWS, shaddr(so), shaddr(sfin), 32 * AW);
 }
 
@@ -720,8 +730,17 @@ template <int TYPE, int DH>
 Variant variant_type(int type, long long rows) {
   return type == T_F32 ? variant_rows<TYPE, DH, 2>(rows) : variant_rows<TYPE, DH, 1>(rows);
 }
-Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type) {
-  const long long rows = (long long)s.max_new * (n_head / c.n_kv);
+// short: half-precision rows past 16 may take the kernel for few rows, a tile of
+// 16 at a time, where that is less work: a CTA of the tcgen05 kernel costs its
+// tiles of 64 positions and 16 more for its beginning and end, one here 4 more,
+// and its tiles take three quarters of the time (a 96 sequence batch of 24 rows
+// and 300 positions each: SHORT_NOTE).
+Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type, bool short_too = false) {
+  long long rows = (long long)s.max_new * (n_head / c.n_kv);
+  if (short_too && type != T_F32 && rows > 16) {
+    const long long tiles = (s.max_len + 63) / 64;
+    if ((rows + 15) / 16 * (tiles + 4) * 3 < (rows + 127) / 128 * (tiles + 16) * 4) rows = 16;
+  }
   if (c.type == PK_KV_Q8) return c.head_dim == 64 ? variant_type<PK_KV_Q8, 64>(type, rows) : variant_type<PK_KV_Q8, 128>(type, rows);
   return c.head_dim == 64 ? variant_type<PK_KV_Q4, 64>(type, rows) : variant_type<PK_KV_Q4, 128>(type, rows);
 }
@@ -848,6 +867,7 @@ struct Shared {
   pk_kv_seqs pre, own;  // bounds of the two
   Variant pre_v, own_v;
   Split pre_p, own_p;
+  bool merge;  // the second launch joins
 };
 Shared shared_plan(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_shared &sh, int n_head, int type) {
   Shared x;
@@ -858,13 +878,22 @@ Shared shared_plan(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_shared
   // (and up to 15 of a shared length that is no multiple of 16)
   x.own.max_len = (int)std::min((long long)sh.max_own + 15, (long long)s.max_len);
   x.pre_p = x.own_p = Split{};
+  x.merge = false;
   if (x.pre.n_seq > 0 && x.pre.max_new > 0 && x.pre.max_len > 0) {
-    x.pre_v = variant_of(c, x.pre, n_head, type);
+    x.pre_v = variant_of(c, x.pre, n_head, type, true);
     x.pre_p = split_of(c, x.pre, n_head, type, x.pre_v, true);
   }
   if (x.own.max_len > 0) {
-    x.own_v = variant_of(c, x.own, n_head, type);
+    x.own_v = variant_of(c, x.own, n_head, type, true);
     x.own_p = split_of(c, x.own, n_head, type, x.own_v, true);
+    // One chunk a sequence, which joins the prefix's parts itself, where its time
+    // is less than a joining launch's or there are CTAs enough.
+    const long long units = (long long)s.n_seq * c.n_kv * x.own_p.row_tiles;
+    if (x.pre_p.n_chunk <= MERGE && (x.own.max_len <= 1536 || units >= 296) && (type == T_F32 || x.own.max_len <= sum_most(type))) {
+      x.own_p.n_chunk = 1;
+      x.own_p.chunk = (x.own.max_len + 63) / 64 * 64;
+      x.merge = true;
+    }
   }
   return x;
 }
@@ -873,7 +902,7 @@ Shared shared_plan(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_shared
 size_t kv_attn_shared_scratch_bytes(const pk_kv_cache &c, const pk_kv_seqs &seqs, const pk_kv_shared &sh, int n_head, int type) {
   const pk_kv_seqs s = bounded(c, seqs);
   const Shared x = shared_plan(c, s, sh, n_head, type);
-  return (size_t)s.n_tok * n_head * (x.pre_p.n_chunk + x.own_p.n_chunk) * (c.head_dim + 2) * sizeof(float);
+  return (size_t)s.n_tok * n_head * (x.pre_p.n_chunk + (x.merge ? 0 : x.own_p.n_chunk)) * (c.head_dim + 2) * sizeof(float);
 }
 
 cudaError_t launch_kv_attn_shared(const pk_kv_cache &c, const pk_kv_seqs &seqs, const pk_kv_shared &sh, const pk_kv_query &q,
@@ -887,7 +916,7 @@ cudaError_t launch_kv_attn_shared(const pk_kv_cache &c, const pk_kv_seqs &seqs, 
   if (x.pre_p.n_chunk == 0) a.sh.n_group = 0;
   a.n_pre = x.pre_p.n_chunk;
   a.pre_chunk = std::max(x.pre_p.chunk, 1);
-  a.n_part = a.n_pre + x.own_p.n_chunk;
+  a.n_part = a.n_pre + (x.merge ? 0 : x.own_p.n_chunk);
   a.part_o = reinterpret_cast<float *>(scratch);
   a.part_ml = reinterpret_cast<float2 *>(a.part_o + rows * a.n_part * c.head_dim);
   cudaError_t e = cudaSuccess;
@@ -901,8 +930,10 @@ cudaError_t launch_kv_attn_shared(const pk_kv_cache &c, const pk_kv_seqs &seqs, 
   a.mode = ATTN_OWN;
   a.part0 = a.n_pre;
   a.chunk = 64;
+  a.merge = x.merge;
+  a.early = a.n_pre > 0;
   if (x.own_p.n_chunk > 0) e = launch_parts(a, x.own_v, x.own_p, s.n_seq, st);
-  return e != cudaSuccess ? e : launch_join(a, st);
+  return e != cudaSuccess || a.merge ? e : launch_join(a, st);
 }
 
 }  // namespace pk

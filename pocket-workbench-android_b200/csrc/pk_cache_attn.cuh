@@ -59,10 +59,15 @@ struct AttnKArgs {
   // What a launch goes over: all of each sequence, each group's shared prefix,
   // or what each sequence has besides it.  The last two leave their chunks'
   // parts in the scratch, a row's n_part of them: the prefix's from 0 on, its
-  // own from n_pre on.
-  int mode, part0, n_part, n_pre, pre_chunk;
+  // own from n_pre on.  merge: what a sequence has besides is one chunk, whose CTA
+  // adds the prefix's parts (up to MERGE of them) to its rows and writes them out.
+  int mode, part0, n_part, n_pre, pre_chunk, merge;
+  // 1: the launch before this one is the prefixes', which began when all earlier
+  // work was done, and is waited for only where its parts are needed.
+  int early;
   pk_kv_shared sh;
 };
+constexpr int MERGE = 8;
 enum : int { ATTN_ALL = 0, ATTN_PREFIX = 1, ATTN_OWN = 2 };
 
 // Group g's sequences [s0, s1), their tokens [t0, t0 + n), and the positions
@@ -134,13 +139,75 @@ __device__ __forceinline__ Unit unit_of(const AttnKArgs &a) {
   u.lo = base + u.ch * a.chunk;
   u.hi = min(u.sv.total, u.lo + a.chunk);
   u.slot = a.part0 + u.ch;
-  u.part = a.mode != ATTN_ALL || u.nch > 1;
+  u.part = (a.mode != ATTN_ALL && !a.merge) || u.nch > 1;
   return u;
 }
 // Has this CTA nothing to do?  (Rows that see nothing are written by their first chunk, or by the joining launch.)
 __device__ __forceinline__ bool idle(const AttnKArgs &a, const Unit &u, int tile0) {
   if (tile0 >= u.rows) return true;
-  return u.ch >= (a.mode == ATTN_ALL ? max(u.nch, 1) : u.nch) && !(a.cluster && u.nch > 1);
+  return u.ch >= (a.mode == ATTN_ALL || a.merge ? max(u.nch, 1) : u.nch) && !(a.cluster && u.nch > 1);
+}
+// Beside the prefixes' launch: it is not over before one CTA (the last) has seen
+// that end, as what follows waits for this launch alone.
+__device__ __forceinline__ void end_early(const AttnKArgs &a) {
+  if (a.early && blockIdx.x == gridDim.x - 1) pdl_wait();
+}
+
+// A row's sum L of weights 2^(s - M) and the parts of its prefix: the factors by
+// which both are added up, f[c] of the parts and `own`, over their common sum.
+// (Read past L1, written by a launch that may have run beside this one.)
+struct Merge {
+  float f[MERGE], own;
+  const float *part;
+  int n;
+};
+template <int DH>
+__device__ __forceinline__ Merge merge_of(const AttnKArgs &a, const Unit &u, int row, float M, float L) {
+  Merge g;
+  const int i = row / a.group, h = u.h * a.group + row - i * a.group;
+  const long long at = ((long long)(u.sv.first + i) * a.q.n_head + h) * a.n_part;
+  g.n = (u.lo + a.pre_chunk - 1) / a.pre_chunk;  // (one chunk: it begins where the prefix ends)
+  g.part = a.part_o + at * DH;
+  float2 ml[MERGE];
+  float top = L == 0.0f ? -CUDART_INF_F : M;
+#pragma unroll
+  for (int c = 0; c < MERGE; c++) {
+    ml[c] = c < g.n ? __ldcg(a.part_ml + at + c) : make_float2(-CUDART_INF_F, 0.0f);
+    top = fmaxf(top, ml[c].x);
+  }
+  g.own = L == 0.0f ? 0.0f : ex2(M - top);  // a NaN sum stays one
+  float all = g.own * L;
+#pragma unroll
+  for (int c = 0; c < MERGE; c++) {
+    g.f[c] = ml[c].y == 0.0f ? 0.0f : ex2(ml[c].x - top);
+    all = fmaf(g.f[c], ml[c].y, all);
+  }
+  const float inv = all > 0.0f || isnan(all) ? 1.0f / all : 0.0f;
+  g.own *= inv;
+#pragma unroll
+  for (int c = 0; c < MERGE; c++) g.f[c] *= inv;
+  return g;
+}
+// N elements from d0 on.
+template <int N>
+__device__ __forceinline__ void merge_in(const Merge &g, int dh, int d0, float (&x)[N]) {
+#pragma unroll
+  for (int j = 0; j < N; j++) x[j] = g.own == 0.0f ? 0.0f : x[j] * g.own;
+#pragma unroll
+  for (int c = 0; c < MERGE; c++) {
+    if (c >= g.n) break;
+    const float4 *p = reinterpret_cast<const float4 *>(g.part + (size_t)c * dh + d0);
+#pragma unroll
+    for (int j = 0; j < N / 4; j++) {
+      const float4 v = __ldcg(p + j);
+      if (g.f[c] != 0.0f) {
+        x[4 * j] = fmaf(g.f[c], v.x, x[4 * j]);
+        x[4 * j + 1] = fmaf(g.f[c], v.y, x[4 * j + 1]);
+        x[4 * j + 2] = fmaf(g.f[c], v.z, x[4 * j + 2]);
+        x[4 * j + 3] = fmaf(g.f[c], v.w, x[4 * j + 3]);
+      }
+    }
+  }
 }
 
 // Does row (token i) see draft j?

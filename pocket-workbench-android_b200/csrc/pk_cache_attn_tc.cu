@@ -310,11 +310,12 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
   constexpr bool F16 = std::is_same_v<E, __half>;
   constexpr int RB = TYPE == PK_KV_Q8 ? DH : DH / 2, SW = TYPE == PK_KV_Q8 ? 1 : 2;
   extern __shared__ __align__(1024) uint8_t smem[];
-  pdl_wait();
+  if (!a.early) pdl_wait();
   const Unit u = unit_of(a);
   const int tile0 = u.rt * ROWS;
   const bool cluster = a.cluster && u.nch > 1;
   if (idle(a, u, tile0)) {
+    end_early(a);
     pdl_trigger();
     return;
   }
@@ -816,7 +817,12 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
         g = before == -CUDART_INF_F ? 0.0f : ex2(before - m);
       }
       if (*abort) f = l = CUDART_NAN_F;
-      if (part) {
+      Merge mg{};
+      if (a.merge) {
+        if (a.early) pdl_wait();
+        mg = merge_of<DH>(a, u, min(row, u.rows - 1), m, l);
+        if (*abort) mg.own = CUDART_NAN_F;
+      } else if (part) {
         if (on && cluster) *reinterpret_cast<float2 *>(smem + L::ML + tid * 8) = make_float2(m, l);
         else if (on) a.part_ml[((at * a.q.n_head + h) * a.n_part) + u.slot] = make_float2(m, l);
       } else {
@@ -847,6 +853,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
 #pragma unroll
           for (int j = 0; j < 8; j++) x[dim8<TYPE>(j)] = f == 0.0f ? 0.0f : v[8 * k + j] * f;
           const int d0 = 16 * c + 8 * k;
+          if (a.merge) merge_in<8>(mg, DH, d0, x);
           if (part) store_n<float, 8>(po + d0, true, x);
           else store_n<E, 8>(reinterpret_cast<E *>(a.q.out) + off + d0, a.vec_o, x);
         }
@@ -869,6 +876,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
   }
   __syncwarp();
   if (cluster) join_cluster<DH>(a, u, tile0, ROWS, sb, sb + L::ML, THREADS);
+  if (!a.merge) end_early(a);
   if (tid == 0 && a.err && *abort) atomicCAS(a.err, 0, PK_ERR_TIMEOUT);
 }
 
