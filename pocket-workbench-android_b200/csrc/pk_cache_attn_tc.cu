@@ -280,6 +280,44 @@ __device__ __forceinline__ float put_q(const AttnKArgs &a, const Unit &u, int ro
   return up;
 }
 
+// The same by two threads a row, half of it each (half precision).
+template <int TYPE, int DH, class E>
+__device__ __forceinline__ float put_q_half(const AttnKArgs &a, const Unit &u, int row, int part, uint32_t dst, int stride) {
+  constexpr bool F16 = std::is_same_v<E, __half>;
+  constexpr int N = DH / 16;  // vectors of 8
+  const bool on = row < u.rows;
+  const int i = row / a.group, h = u.h * a.group + row - i * a.group;
+  const E *p = reinterpret_cast<const E *>(a.q.q) + (on ? (long long)(u.sv.first + i) * a.q.q_tok_stride + (long long)h * a.q.q_head_stride : 0) + part * (DH / 2);
+  uint4 raw[N];
+  const E *x = reinterpret_cast<const E *>(raw);
+  if (on && a.vec_q) {
+#pragma unroll
+    for (int c = 0; c < N; c++) raw[c] = __ldg(reinterpret_cast<const uint4 *>(p) + c);
+  } else {
+    E *y = reinterpret_cast<E *>(raw);
+#pragma unroll
+    for (int j = 0; j < 8 * N; j++) y[j] = on ? p[j] : from_f<E>(0.0f);
+  }
+  float m = 0.0f;
+  if (!F16) {
+#pragma unroll
+    for (int j = 0; j < 8 * N; j++) m = fmaxf(m, fabsf(to_f(x[j])));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  }
+  int e = (int)(__float_as_uint(m) >> 23) - 127;
+  e = m > 0.0f ? min(max(e, -100), 126) : 0;
+  const float up = __int_as_float((e + 127) << 23), down = __int_as_float((127 - e) << 23);
+#pragma unroll
+  for (int c = 0; c < N; c++) {
+    uint32_t w[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      w[j] = pack2(inf_nan(to_f(x[8 * c + dim8<TYPE>(2 * j)])) * down, inf_nan(to_f(x[8 * c + dim8<TYPE>(2 * j + 1)])) * down);
+    sts128(dst + (part * N + c) * stride, w[0], w[1], w[2], w[3]);
+  }
+  return up;
+}
+
 // Which of positions p0 .. p0 + 63 token i sees (bit by position).
 __device__ __forceinline__ uint64_t seen_by(const AttnKArgs &a, const Unit &u, int i, int p0, int hi) {
   auto ones = [](int n) { return n >= 64 ? ~0ull : n <= 0 ? 0ull : (1ull << n) - 1; };
@@ -349,7 +387,14 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
   }
   const int row = tile0 + tid;
   float rs = 0.0f;
-  if (tid < SOFT) {
+  if (BLK == 1) {  // (the code warps, which are twice as many; the scales go by way of the sums' place)
+    if (tid >= SOFT && tid < SOFT + 2 * CONV) {
+      const int r = (tid - SOFT) >> 1, part = tid & 1;
+      const float up = put_q_half<TYPE, DH, std::conditional_t<BLK == 1, E, __half>>(a, u, tile0 + r, part, sb + L::Q + r * 16, ROWS * 16);
+      if (part == 0) *reinterpret_cast<float *>(smem + L::ML + r * 8) = up;
+      fence_async_smem();
+    }
+  } else if (tid < SOFT) {
     rs = put_q<TYPE, DH, E>(a, u, row, sb + L::Q + tid * 16, ROWS * 16, L::QT);
     fence_async_smem();
   }
@@ -509,6 +554,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
     }
   } else {  // ------------------------------------------------------------ softmax
     set_regs<true, L::REGS_SOFT>();
+    if (BLK == 1) rs = *reinterpret_cast<volatile float *>(smem + L::ML + tid * 8);
     const int blk = BLK == 1 ? 0 : warp >> 2;
     const uint32_t lanes = ((uint32_t)((warp & 3) * 32) << 16) + blk * L::COLS;
     const bool work = tile0 + warp * 32 < u.rows;  // (the whole warp)
@@ -654,8 +700,8 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
 #pragma unroll
           for (int n = 0; n < NT; n++) st_pairs(tmem + lanes + L::P_COL + n * (NK / 2) + 16 * h, w[n][0], w[n][1]);
         };
-        bool longer = masked;
-        if (!masked) {
+        bool longer = masked || i == 0;  // (the first tile has no reference yet)
+        if (!longer) {
           sum[0] = sum[1] = sum[2] = sum[3] = make_float2(0.0f, 0.0f);
           __syncwarp();
           if constexpr (NT == 1) {  // 16 columns are on their way while those before are worked on
@@ -680,8 +726,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
               put_two(h);
             }
           }
-          // (a thread's part of a row's sum is at least the largest of its
-          // weights; m is -inf at first: infinite)
+          // (a thread's part of a row's sum is at least the largest of its weights)
           bool over = false;
           float all[4];
 #pragma unroll
@@ -805,34 +850,29 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
       }
       asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
     }
-    // (a cluster's sums take the operands' place: all blocks' products are done)
-    if (BLK > 1 && cluster) asm volatile("bar.sync 1, %0;" ::"r"(SOFT) : "memory");
+    // The rows go by way of the operands' place (all blocks' products are done): a
+    // cluster's are added up there, others leave it a whole row at a time (a row
+    // a lane, 32 rows' lines a store, took 8,000 cycles).
+    if (BLK > 1) asm volatile("bar.sync 1, %0;" ::"r"(SOFT) : "memory");
     if (work) {
       const int i = tok, h = u.h * a.group + (min(row, u.rows - 1) - i * a.group);
-      const long long at = u.sv.first + i;
+      const long long at = u.sv.first + i, slot = (at * a.q.n_head + h) * a.n_part + u.slot;
       const bool on = row < u.rows, part = u.part;
       float f = 1.0f, g = 0.0f;  // g: of what a long sum has in the scratch
       if (LONG && nt > SUM_TILES<E> && on) {
-        const float before = a.part_ml[(at * a.q.n_head + h) * a.n_part + u.slot].x;
+        const float before = a.part_ml[slot].x;
         g = before == -CUDART_INF_F ? 0.0f : ex2(before - m);
       }
       if (*abort) f = l = CUDART_NAN_F;
-      Merge mg{};
-      if (a.merge) {
-        if (a.early) pdl_wait();
-        mg = merge_of<DH>(a, u, min(row, u.rows - 1), m, l);
-        if (*abort) mg.own = CUDART_NAN_F;
-      } else if (part) {
+      if (part) {
         if (on && cluster) *reinterpret_cast<float2 *>(smem + L::ML + tid * 8) = make_float2(m, l);
-        else if (on) a.part_ml[((at * a.q.n_head + h) * a.n_part) + u.slot] = make_float2(m, l);
-      } else {
+        else if (on) a.part_ml[slot] = make_float2(m, l);
+      } else if (!a.merge) {
         f *= l > 0.0f || isnan(l) ? 1.0f / l : 0.0f;
       }
       if (l == 0.0f) f = 0.0f;
-      // (in a cluster: into shared memory, where the operands were)
-      float *po = !part ? nullptr : cluster ? reinterpret_cast<float *>(smem) + tid * (DH + 4) : a.part_o + ((at * a.q.n_head + h) * a.n_part + u.slot) * DH;
-      const long long off = at * a.q.out_tok_stride + (long long)h * a.q.out_head_stride;
-#pragma unroll
+      float *so = reinterpret_cast<float *>(smem) + tid * (DH + 4);
+#pragma unroll 1
       for (int c = 0; c < DH / 16; c++) {
         float v[16];
         __syncwarp();
@@ -843,19 +883,56 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
           for (int j = 0; j < 16; j++) v[j] = 0.0f;
         }
         if (LONG && nt > SUM_TILES<E> && on) {
-          const float *p = a.part_o + ((at * a.q.n_head + h) * a.n_part + u.slot) * DH + 16 * c;
+          const float *p = a.part_o + slot * DH + 16 * c;
 #pragma unroll
           for (int j = 0; j < 16; j++) v[j] = fmaf(g, p[j], v[j]);
         }
 #pragma unroll
-        for (int k = 0; k < 2 && on; k++) {
+        for (int k = 0; k < 2; k++) {
           float x[8];
 #pragma unroll
           for (int j = 0; j < 8; j++) x[dim8<TYPE>(j)] = f == 0.0f ? 0.0f : v[8 * k + j] * f;
-          const int d0 = 16 * c + 8 * k;
-          if (a.merge) merge_in<8>(mg, DH, d0, x);
-          if (part) store_n<float, 8>(po + d0, true, x);
-          else store_n<E, 8>(reinterpret_cast<E *>(a.q.out) + off + d0, a.vec_o, x);
+          store_n<float, 8>(so + 16 * c + 8 * k, true, x);
+        }
+      }
+      __syncwarp();
+      if (!cluster) {
+        Merge mg{};
+        if (a.merge) {
+          if (a.early) pdl_wait();
+          mg = merge_of<DH>(a, u, min(row, u.rows - 1), m, l);
+        }
+        constexpr int LR = DH / 4, RP = 32 / LR;  // lanes a row, rows at a time
+        const int sub = lane / LR, d0 = (lane % LR) * 4, rows = min(32, u.rows - tile0 - warp * 32);
+        const long long off = part ? slot * DH : at * a.q.out_tok_stride + (long long)h * a.q.out_head_stride;
+#pragma unroll 1
+        for (int r0 = 0; r0 < rows; r0 += RP) {
+          const int r = min(r0 + sub, 31);
+          const long long to = __shfl_sync(0xffffffffu, off, r) + d0;
+          const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem) + (warp * 32 + r) * (DH + 4) + d0);
+          float x[4] = {v.x, v.y, v.z, v.w};
+          if (a.merge) {
+            Merge one;
+            one.n = mg.n;  // (of one sequence)
+            one.own = __shfl_sync(0xffffffffu, mg.own, r);
+            one.part = reinterpret_cast<const float *>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(mg.part), r));
+#pragma unroll
+            for (int c = 0; c < MERGE; c++)
+              if (c < mg.n) one.f[c] = __shfl_sync(0xffffffffu, mg.f[c], r);
+            if (r0 + sub < rows) merge_in<4>(one, DH, d0, x);
+          }
+          if (r0 + sub >= rows) continue;
+          if (part) {
+            *reinterpret_cast<float4 *>(a.part_o + to) = make_float4(x[0], x[1], x[2], x[3]);
+          } else if (NT == 2) {
+            store_n<float, 4>(reinterpret_cast<float *>(a.q.out) + to, a.vec_o, x);
+          } else if (a.vec_o) {
+            E y[4] = {from_f<E>(x[0]), from_f<E>(x[1]), from_f<E>(x[2]), from_f<E>(x[3])};
+            *reinterpret_cast<uint2 *>(reinterpret_cast<E *>(a.q.out) + to) = *reinterpret_cast<const uint2 *>(y);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) reinterpret_cast<E *>(a.q.out)[to + j] = from_f<E>(x[j]);
+          }
         }
       }
     }

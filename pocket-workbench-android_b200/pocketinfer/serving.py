@@ -85,34 +85,37 @@ def kv_plan(ctx, n_new, pages, held, free, n_free, page_size: int, n_tok: int, d
     of the token arrays (at least the new tokens; rows behind them get position 0, sequence -1, slot -1).  in_place: pages,
     held, free and n_free are updated themselves; otherwise the results are new tensors."""
     _init()
-    dev, n = ctx.get_device(), ctx.shape[0] if ctx.dim() == 1 else -1
+    torch = _d.torch
+    i32, dev, n = torch.int32, ctx.get_device(), ctx.shape[0] if ctx.dim() == 1 else -1
     if dev < 0 or n < 0:
         _bad("kv_plan: ctx must be [n_seq] on a CUDA device")
-    for t, name, dims in ((ctx, "ctx", 1), (n_new, "n_new", 1), (pages, "pages", 2), (held, "held", 1), (free, "free", 1), (n_free, "n_free", 1),
-                          (done, "done", 1), (shared, "shared", 1)):
-        if t is not None:
-            _i32(t, dev, name, dims)
-            if name not in ("free", "n_free") and t.shape[0] != n:
-                _bad(f"kv_plan: {name} has {t.shape[0]} entries for {n} slots")
-    if n_free.shape[0] != 1:
-        _bad("kv_plan: n_free is one number")
+    ptrs = []
+    for t, name, shape in ((ctx, "ctx", (n,)), (n_new, "n_new", (n,)), (pages, "pages", None), (held, "held", (n,)), (free, "free", None),
+                           (n_free, "n_free", (1,)), (done, "done", (n,)), (shared, "shared", (n,))):
+        if t is None:
+            ptrs.append(0)
+            continue
+        if t.dtype is not i32 or t.get_device() != dev or not t.is_contiguous() or (shape is not None and t.shape != shape):
+            _bad(f"kv_plan: {name} must be a contiguous int32 tensor{'' if shape is None else f' of {shape[0]}'} on device {dev}")
+        ptrs.append(t.data_ptr())
+    if pages.dim() != 2 or pages.shape[0] != n or free.dim() != 1:
+        _bad("kv_plan: pages must be [n_seq, max_pages] and free a list")
     if not 0 <= n_tok <= 1 << 30:
         _bad("kv_plan: n_tok must be 0 to 2^30")
     wide, cap = pages.shape[1], free.shape[0]
-    i32, where = _d.torch.int32, ctx.device
-
-    # one block for all results (a tensor of its own each costs more than the launch, and so does a slice each), each at
-    # 16 bytes: they and the gaps behind them by turns
-    sizes = (2 * n_tok, n + 1, n_tok, n_tok, 1) if in_place else (2 * n_tok, n + 1, n_tok, n_tok, 1, n * wide, n, cap, 1)
-    cuts = [x for size in sizes for x in (size, -size % 4)]
-    make = lambda: _d.torch.empty(sum(cuts), dtype=i32, device=where).split_with_sizes(cuts)  # noqa: E731
+    # one block for all results (a tensor of its own each costs more than the launch): first what has to be aligned
+    table = 0 if in_place else n * wide + (n * wide & 1)
+    sizes = (table, 2 * n_tok, n + 1, n_tok, n_tok, 1) if in_place else (table, 2 * n_tok, n + 1, n_tok, n_tok, 1, n, cap, 1)
+    make = lambda: torch.empty(sum(sizes), dtype=i32, device=ctx.device).split_with_sizes(sizes)  # noqa: E731
     made = make() if stream is None else _new(make, dev, stream)
-    slot, start, pos, seq, lacking = made[0].view(_d.torch.int64), made[2], made[4], made[6], made[8]
-    out = (pages, held, free, n_free) if in_place else (made[10].view(n, wide), made[12], made[14], made[16])
-    ptr = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
-    args = PACK_PLAN(ctx.data_ptr(), n_new.data_ptr(), pages.data_ptr(), held.data_ptr(), free.data_ptr(), n_free.data_ptr(), ptr(done), ptr(shared),
-                     *[t.data_ptr() for t in out], start.data_ptr(), lacking.data_ptr(), pos.data_ptr(), seq.data_ptr(), slot.data_ptr(), n, wide, cap,
-                     n_tok, page_size)
+    slot, start, pos, seq, lacking = made[1].view(torch.int64), made[2], made[3], made[4], made[5]
+    if in_place:
+        out, to = (pages, held, free, n_free), (ptrs[2], ptrs[3], ptrs[4], ptrs[5])
+    else:
+        block = made[0] if table == n * wide else made[0][:-1]
+        out = (block.view(n, wide), made[6], made[7], made[8])
+        to = (block.data_ptr(), made[6].data_ptr(), made[7].data_ptr(), made[8].data_ptr())
+    args = PACK_PLAN(*ptrs, *to, start.data_ptr(), lacking.data_ptr(), pos.data_ptr(), seq.data_ptr(), slot.data_ptr(), n, wide, cap, n_tok, page_size)
     _call(_d._L.pk_kv_plan, dev, stream, stream is not None and (ctx, n_new, pages, held, free, n_free, done, shared, made), args)
     return KvPlan(start, pos, seq, slot, *out, lacking)
 
