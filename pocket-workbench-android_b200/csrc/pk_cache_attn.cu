@@ -867,6 +867,7 @@ struct Shared {
   pk_kv_seqs pre, own;  // bounds of the two
   Variant pre_v, own_v;
   Split pre_p, own_p;
+  bool wide;   // the first is pk_cache_prefix.cu's
   bool merge;  // the second launch joins
 };
 Shared shared_plan(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_shared &sh, int n_head, int type) {
@@ -878,10 +879,26 @@ Shared shared_plan(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_shared
   // (and up to 15 of a shared length that is no multiple of 16)
   x.own.max_len = (int)std::min((long long)sh.max_own + 15, (long long)s.max_len);
   x.pre_p = x.own_p = Split{};
-  x.merge = false;
+  x.wide = x.merge = false;
   if (x.pre.n_seq > 0 && x.pre.max_new > 0 && x.pre.max_len > 0) {
     x.pre_v = variant_of(c, x.pre, n_head, type, true);
     x.pre_p = split_of(c, x.pre, n_head, type, x.pre_v, true);
+    // Half precision with more than a block of 128 rows: chunks by the rounds of
+    // CTAs that they take, one an SM, at a CTA's tiles of 128 positions and 10 more.
+    const long long rows = (long long)x.pre.max_new * (n_head / c.n_kv);
+    x.wide = type != T_F32 && rows > 128;
+    if (x.wide) {
+      x.pre_p.row_tiles = (int)((rows + PREFIX_ROWS - 1) / PREFIX_ROWS);
+      const long long units = (long long)sh.n_group * c.n_kv * x.pre_p.row_tiles, all = (x.pre.max_len + 127) / 128;
+      const long long least = (x.pre.max_len + sum_most(type) - 1) / sum_most(type), most = std::max<long long>(least, MERGE);
+      long long n = least, best = 0;
+      for (long long k = least; k <= std::min(all, most); k++) {
+        const long long t = (units * k + 147) / 148 * ((all + k - 1) / k + 10);
+        if (k == least || t < best) best = t, n = k;
+      }
+      x.pre_p.chunk = (int)((all + n - 1) / n * 128);
+      x.pre_p.n_chunk = (int)((x.pre.max_len + (long long)x.pre_p.chunk - 1) / x.pre_p.chunk);
+    }
   }
   if (x.own.max_len > 0) {
     x.own_v = variant_of(c, x.own, n_head, type, true);
@@ -924,7 +941,14 @@ cudaError_t launch_kv_attn_shared(const pk_kv_cache &c, const pk_kv_seqs &seqs, 
     AttnKArgs b = a;
     b.mode = ATTN_PREFIX;
     b.q.mask = nullptr;
-    e = launch_parts(b, x.pre_v, x.pre_p, sh.n_group, st);
+    if (x.wide) {
+      b.chunk = x.pre_p.chunk; b.n_chunk = x.pre_p.n_chunk; b.row_tiles = x.pre_p.row_tiles;
+      const long long blocks = (long long)sh.n_group * c.n_kv * b.row_tiles * b.n_chunk;
+      if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
+      e = launch_kv_prefix(b, (unsigned)blocks, st);
+    } else {
+      e = launch_parts(b, x.pre_v, x.pre_p, sh.n_group, st);
+    }
     if (e != cudaSuccess) return e;
   }
   a.mode = ATTN_OWN;
