@@ -29,7 +29,7 @@ namespace {
 constexpr int PK_N = 128, PROWS = 256;  // positions a tile, rows a CTA
 constexpr int PSOFT = 256, PCONV = 128, PMMA = 128, PTHREADS = PSOFT + 2 * PCONV + PMMA, PWS = PSOFT / 32;
 // registers a thread: at launch, then by warps
-constexpr int PREGS = 96, PREGS_SOFT = 160, PREGS_CONV = 64, PREGS_MMA = 32;
+constexpr int PREGS = 96, PREGS_SOFT = 168, PREGS_CONV = 56, PREGS_MMA = 32;
 static_assert(PSOFT * PREGS_SOFT + 2 * PCONV * PREGS_CONV + PMMA * PREGS_MMA <= PTHREADS * PREGS, "no more than the launch's");
 
 template <int DH>
@@ -238,10 +238,14 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
     const uint32_t cols = tmem + lanes + L::S_COL;
     // of rows lane / 4 + 8 j: the scale, the reference, this thread's part of the sum
     const float rs = *reinterpret_cast<volatile float *>(smem + L::RS + tid * 4);
+    // (the scale and less the reference as pairs, too)
     float rs4[4], m4[4], l4[4];
+    uint64_t scale2[4], less4[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
       rs4[j] = __shfl_sync(0xffffffffu, rs, (lane >> 2) + 8 * j);
+      scale2[j] = pair_of(rs4[j], rs4[j]);
+      less4[j] = 0;
       m4[j] = -CUDART_INF_F;
       l4[j] = 0.0f;
     }
@@ -252,34 +256,35 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
         tc_fence_after();
         if (work) {
           const uint8_t *sc = smem + L::SC + (i & 3) * L::SCB;
-          const float2 *dk2 = reinterpret_cast<const float2 *>(sc) + quad, *dv2 = dk2 + PK_N / 2, *off2 = dk2 + PK_N;
+          const uint64_t *dk2 = reinterpret_cast<const uint64_t *>(sc) + quad, *dv2 = dk2 + PK_N / 2, *off2 = dk2 + PK_N;
           const uint4 held = *reinterpret_cast<const uint4 *>(sc + 3 * PK_N * 4), r4 = *reinterpret_cast<const uint4 *>(sc + 3 * PK_N * 4 + 16);
           const float vmax = fmaxf(fmaxf(__uint_as_float(r4.x), __uint_as_float(r4.y)), fmaxf(__uint_as_float(r4.z), __uint_as_float(r4.w)));
           const bool masked = (held.x & held.y & held.z & held.w) != 0xffffffffu;
           uint32_t w[2][32];
-          float2 sum[4];
-          // the weights of the products in t, columns 16 k .. of 128
-          auto weights = [&](int k, const float (&t)[16], const float (&m)[4], bool add) {
+          uint64_t sum[4];
+          // the weights of the products in t, columns 16 k .. of 128, less the references
+          auto weights = [&](int k, const float (&t)[16], const uint64_t (&less)[4], bool add) {
 #pragma unroll
             for (int g = 0; g < 2; g++) {
-              const float2 dk = dk2[4 * (2 * k + g)], dv = dv2[4 * (2 * k + g)];
-              const float2 off = add ? off2[4 * (2 * k + g)] : make_float2(0.0f, 0.0f);
+              const uint64_t dk = dk2[4 * (2 * k + g)], dv = dv2[4 * (2 * k + g)], off = add ? off2[4 * (2 * k + g)] : 0;
 #pragma unroll
               for (int j = 0; j < 4; j++) {
                 const int p = 4 * (j >> 1) + 2 * g + (j & 1), at = 2 * (2 * k + g) + (j & 1);
-                float2 x = make_float2(t[2 * p], t[2 * p + 1]);
-                x = F16 ? fma2(x, dk, make_float2(-m[j], -m[j])) : fma2(mul2(x, dk), make_float2(rs4[j], rs4[j]), make_float2(-m[j], -m[j]));
+                uint64_t x = pair_of(t[2 * p], t[2 * p + 1]);
+                x = F16 ? fma2(x, dk, less[j]) : fma2(mul2(x, dk), scale2[j], less[j]);
                 if (add) x = add2(x, off);
-                x.x = ex2(x.x);
-                x.y = ex2(x.y);
+                float2 y = unpair(x);
+                y.x = ex2(y.x);
+                y.y = ex2(y.y);
+                x = pair_of(y.x, y.y);
                 sum[j] = add2(sum[j], x);
-                x = mul2(x, dv);
-                w[j >> 1][at] = pack2(x.x, x.y);
+                y = unpair(mul2(x, dv));
+                w[j >> 1][at] = pack2(y.x, y.y);
               }
             }
           };
-          auto all_weights = [&](const float (&m)[4], bool add) {
-            sum[0] = sum[1] = sum[2] = sum[3] = make_float2(0.0f, 0.0f);
+          auto all_weights = [&](const uint64_t (&less)[4], bool add) {
+            sum[0] = sum[1] = sum[2] = sum[3] = 0;
             __syncwarp();
             float t[2][16];  // 16 columns are on their way while those before are worked on
             ask_quads(cols, t[0]);
@@ -287,23 +292,24 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
             for (int k = 0; k < 8; k++) {
               wait16(t[k & 1]);
               if (k < 7) ask_quads(cols + 16 * (k + 1), t[(k + 1) & 1]);
-              weights(k, t[k & 1], m, add);
+              weights(k, t[k & 1], less, add);
             }
           };
           bool longer = masked || i == 0;  // (the first tile has no reference yet)
           if (!longer) {
-            all_weights(m4, false);
+            all_weights(less4, false);
             // (a thread's part of a row's sum is at least the largest of its weights)
             bool over = false;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-              const float all = sum[j].x + sum[j].y;
+              const float2 y = unpair(sum[j]);
+              const float all = y.x + y.y;
               over |= !(all * vmax <= TOP && all <= 0x1p100f);
             }
             longer = __any_sync(0xffffffffu, over);
           }
           if (longer) {
-            float mx[4], top[4], f[4], m[4];
+            float mx[4], top[4], f[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) mx[j] = -CUDART_INF_F, top[j] = 0.0f;
             auto quad_max = [](float x) {
@@ -319,7 +325,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
                 wait16(t);
 #pragma unroll
                 for (int g = 0; g < 2; g++) {
-                  const float2 dk = dk2[4 * (2 * k + g)], dv = dv2[4 * (2 * k + g)], off = off2[4 * (2 * k + g)];
+                  const float2 dk = unpair(dk2[4 * (2 * k + g)]), dv = unpair(dv2[4 * (2 * k + g)]), off = unpair(off2[4 * (2 * k + g)]);
 #pragma unroll
                   for (int j = 0; j < 4; j++) {
                     const int p = 4 * (j >> 1) + 2 * g + (j & 1);
@@ -346,7 +352,8 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
                 m4[j] = now;
                 moved |= f[j] != 1.0f;
               }
-              m[j] = m4[j] == -CUDART_INF_F ? 0.0f : m4[j];  // (nothing seen yet: all are masked)
+              const float less = m4[j] == -CUDART_INF_F ? 0.0f : -m4[j];  // (nothing seen yet: all are masked)
+              less4[j] = pair_of(less, less);
             }
             if (i > 0 && __any_sync(0xffffffffu, moved)) {  // O's rows, once the products before are done
               pv_wait(i - 1);
@@ -362,10 +369,13 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
                 st_quads(tmem + lanes + L::O_COL + 16 * c, v);
               }
             }
-            all_weights(m, true);
+            all_weights(less4, true);
           }
 #pragma unroll
-          for (int j = 0; j < 4; j++) l4[j] += sum[j].x + sum[j].y;
+          for (int j = 0; j < 4; j++) {
+            const float2 y = unpair(sum[j]);
+            l4[j] += y.x + y.y;
+          }
           __syncwarp();
           // the weights take their scores' columns, two a column
 #pragma unroll
