@@ -730,17 +730,16 @@ template <int TYPE, int DH>
 Variant variant_type(int type, long long rows) {
   return type == T_F32 ? variant_rows<TYPE, DH, 2>(rows) : variant_rows<TYPE, DH, 1>(rows);
 }
-// short: half-precision rows past 16 may take the kernel for few rows, a tile of
-// 16 at a time, where that is less work: a CTA of the tcgen05 kernel costs its
-// tiles of 64 positions and 16 more for its beginning and end, one here 4 more,
-// and its tiles take three quarters of the time (a 96 sequence batch of 24 rows
-// and 300 positions each: SHORT_NOTE).
+// short_too: half-precision rows past 16 may take the kernel here, a tile of 16 at
+// a time, where that is less work: a CTA of the tcgen05 kernel costs its tiles of
+// 64 positions and 16 more for its beginning and end, one here 4 more, and its
+// tiles three quarters of the time (96 sequences of 24 rows and up to 318
+// positions behind 12 prefixes: the call 91 us so, 108 with the tcgen05 kernel,
+// 93 with tiles of 32 rows; 4 answers to a prompt of 700: 17, 31 and 18).
 Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type, bool short_too = false) {
   long long rows = (long long)s.max_new * (n_head / c.n_kv);
-  if (short_too && type != T_F32 && rows > 16) {
-    const long long tiles = (s.max_len + 63) / 64;
-    if ((rows + 15) / 16 * (tiles + 4) * 3 < (rows + 127) / 128 * (tiles + 16) * 4) rows = 16;
-  }
+  const long long tiles = (s.max_len + 63) / 64;
+  if (short_too && type != T_F32 && rows >= TC_FROM && (rows + 15) / 16 * (tiles + 4) * 3 < (rows + 127) / 128 * (tiles + 16) * 4) rows = TC_FROM - 1;
   if (c.type == PK_KV_Q8) return c.head_dim == 64 ? variant_type<PK_KV_Q8, 64>(type, rows) : variant_type<PK_KV_Q8, 128>(type, rows);
   return c.head_dim == 64 ? variant_type<PK_KV_Q4, 64>(type, rows) : variant_type<PK_KV_Q4, 128>(type, rows);
 }

@@ -95,7 +95,7 @@ struct OwnView {
 };
 __device__ __forceinline__ OwnView own_view(const AttnKArgs &a, int s, const SeqView &sv) {
   int base = 0, len = 0;
-  const int g = a.sh.n_group > 0 ? last_at(a.sh.first, a.sh.n_group, s, threadIdx.x & 31) : -1;
+  const int g = a.sh.n_group > 1 ? last_at(a.sh.first, a.sh.n_group, s, threadIdx.x & 31) : a.sh.n_group - 1;
   if (g >= 0) {
     const GroupView v = group_view(a, g);
     if (s >= v.s0 && s < v.s1 && sv.ctx >= v.len) base = v.base, len = v.len;
@@ -188,23 +188,27 @@ __device__ __forceinline__ Merge merge_of(const AttnKArgs &a, const Unit &u, int
   for (int c = 0; c < MERGE; c++) g.f[c] *= inv;
   return g;
 }
-// N elements from d0 on.
+// N elements from d0 on.  (All parts' loads of four elements are asked for together.)
 template <int N>
 __device__ __forceinline__ void merge_in(const Merge &g, int dh, int d0, float (&x)[N]) {
 #pragma unroll
   for (int j = 0; j < N; j++) x[j] = g.own == 0.0f ? 0.0f : x[j] * g.own;
+  const float4 *p = reinterpret_cast<const float4 *>(g.part + d0);
 #pragma unroll
-  for (int c = 0; c < MERGE; c++) {
-    if (c >= g.n) break;
-    const float4 *p = reinterpret_cast<const float4 *>(g.part + (size_t)c * dh + d0);
+  for (int j = 0; j < N / 4; j++) {
+    float4 v[MERGE];
 #pragma unroll
-    for (int j = 0; j < N / 4; j++) {
-      const float4 v = __ldcg(p + j);
-      if (g.f[c] != 0.0f) {
-        x[4 * j] = fmaf(g.f[c], v.x, x[4 * j]);
-        x[4 * j + 1] = fmaf(g.f[c], v.y, x[4 * j + 1]);
-        x[4 * j + 2] = fmaf(g.f[c], v.z, x[4 * j + 2]);
-        x[4 * j + 3] = fmaf(g.f[c], v.w, x[4 * j + 3]);
+    for (int c = 0; c < MERGE; c++) {
+      v[c] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (c < g.n) v[c] = __ldcg(p + j + (size_t)c * (dh / 4));
+    }
+#pragma unroll
+    for (int c = 0; c < MERGE; c++) {
+      if (c < g.n && g.f[c] != 0.0f) {
+        x[4 * j] = fmaf(g.f[c], v[c].x, x[4 * j]);
+        x[4 * j + 1] = fmaf(g.f[c], v[c].y, x[4 * j + 1]);
+        x[4 * j + 2] = fmaf(g.f[c], v[c].z, x[4 * j + 2]);
+        x[4 * j + 3] = fmaf(g.f[c], v[c].w, x[4 * j + 3]);
       }
     }
   }
