@@ -721,7 +721,7 @@ Variant variant_rows(long long rows) {
     return {nullptr, 0, 128};
   } else if constexpr (DH == 64) {
     static_assert(TC32_FROM == 33, "f32 rows past 32");
-    return rows <= 32 ? variant_as<TYPE, DH, NT, 4, 1>() : Variant{nullptr, 0, 256};
+    return rows <= 32 ? variant_as<TYPE, DH, NT, 4, 1>() : Variant{nullptr, 0, rows <= 128 ? 128 : 256};
   } else {
     return rows <= 32 ? variant_as<TYPE, DH, NT, 2, 2>() : variant_as<TYPE, DH, NT, 2, 4>();
   }
@@ -831,7 +831,7 @@ static cudaError_t launch_parts(AttnKArgs &a, const Variant &v, const Split &p, 
   const long long blocks = (long long)units * a.c.n_kv * p.row_tiles * p.n_chunk;
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   const int cluster = a.cluster ? p.n_chunk : 1;
-  if (!v.k) return launch_kv_attn_tc(a, cluster, (unsigned)blocks, st);
+  if (!v.k) return launch_kv_attn_tc(a, v.rows, cluster, (unsigned)blocks, st);
   return launch_cluster(v.k, cluster, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
 }
 static cudaError_t launch_join(const AttnKArgs &a, cudaStream_t st) {

@@ -306,8 +306,8 @@ __device__ __forceinline__ void join_cluster(const AttnKArgs &a, const Unit &u, 
 }
 
 // The tcgen05 kernel's launch (pk_cache_attn_tc.cu): one or two blocks of 128
-// rows of a kv head a CTA (two CTAs an SM, or one).
-cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int cluster, unsigned blocks, cudaStream_t st);
+// rows of a kv head a CTA (two CTAs an SM, or one; two for f32 alone).
+cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int rows, int cluster, unsigned blocks, cudaStream_t st);
 // The shared prefixes' of many half-precision rows, 256 a CTA (pk_cache_prefix.cu).
 constexpr int PREFIX_ROWS = 256;
 cudaError_t launch_kv_prefix(const AttnKArgs &a, unsigned blocks, cudaStream_t st);

@@ -67,15 +67,14 @@ template <class E>
 constexpr int terms_of = std::is_same_v<E, float> ? 2 : 1;
 
 // Geometry, by the terms.
-template <int DH, int NT>
+template <int DH, int NT, int BLK>  // BLK blocks of 128 rows
 struct Lay {
-  static constexpr int BLK = NT;  // blocks of 128 rows
   // (two blocks: whole warpgroups, as the last one gives registers away too)
   static constexpr int ROWS = 128 * BLK, SOFT = 128 * BLK, CONV = 128, MMA = BLK == 1 ? 32 : 128, THREADS = SOFT + 2 * CONV + MMA;
   // Registers a thread: at launch, and after the others have given the softmax
   // warps theirs.
-  static constexpr int CTAS = BLK == 1 ? 2 : 1, REGS = BLK == 1 ? 72 : 96, REGS_SOFT = BLK == 1 ? 104 : 168;
-  static constexpr int REGS_CONV = BLK == 1 ? 56 : 48, REGS_MMA = BLK == 1 ? REGS : 48;
+  static constexpr int CTAS = BLK == 1 ? 2 : 1, REGS = BLK == 1 ? 72 : 96, REGS_SOFT = BLK > 1 ? 168 : NT == 1 ? 104 : 136;
+  static constexpr int REGS_CONV = BLK > 1 ? 48 : NT == 1 ? 56 : 40, REGS_MMA = BLK == 1 ? REGS : 48;
   static_assert(SOFT * REGS_SOFT + 2 * CONV * REGS_CONV + MMA * REGS_MMA <= THREADS * REGS, "no more than the launch's");
   static_assert(CTAS * THREADS * REGS <= 65536, "all of an SM's CTAs");
   // chunks of 16 bytes (8 dimensions) of consecutive positions; one chunk's
@@ -157,10 +156,10 @@ __device__ __forceinline__ uint64_t seen_by(const AttnKArgs &a, const Unit &u, i
   return v & ones(hi - p0) & ones(u.sv.ctx + u.sv.n - p0);
 }
 
-template <int TYPE, int DH, class E, bool LONG>
-__global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_of<E>>::CTAS) k_kv_attn_tc(const AttnKArgs a) {
-  constexpr int NT = terms_of<E>, BLK = NT;
-  using L = Lay<DH, NT>;
+template <int TYPE, int DH, class E, bool LONG, int BLK>
+__global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, terms_of<E>, BLK>::CTAS) k_kv_attn_tc(const AttnKArgs a) {
+  constexpr int NT = terms_of<E>;
+  using L = Lay<DH, NT, BLK>;
   constexpr int ROWS = L::ROWS, SOFT = L::SOFT, CONV = L::CONV, THREADS = L::THREADS, WS = SOFT / 32;
   constexpr bool F16 = std::is_same_v<E, __half>;
   constexpr int RB = TYPE == PK_KV_Q8 ? DH : DH / 2, SW = TYPE == PK_KV_Q8 ? 1 : 2;
@@ -204,10 +203,10 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
   }
   const int row = tile0 + tid;
   float rs = 0.0f;
-  if (BLK == 1) {  // (the code warps, which are twice as many; the scales go by way of the sums' place)
+  if (NT == 1) {  // (the code warps, which are twice as many; the scales go by way of the sums' place)
     if (tid >= SOFT && tid < SOFT + 2 * CONV) {
       const int r = (tid - SOFT) >> 1, part = tid & 1;
-      const float up = put_q_half<TYPE, DH, std::conditional_t<BLK == 1, E, __half>>(a, u, tile0 + r, part, sb + L::Q + r * 16, ROWS * 16);
+      const float up = put_q_half<TYPE, DH, std::conditional_t<NT == 1, E, __half>>(a, u, tile0 + r, part, sb + L::Q + r * 16, ROWS * 16);
       if (part == 0) *reinterpret_cast<float *>(smem + L::ML + r * 8) = up;
       fence_async_smem();
     }
@@ -371,7 +370,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>>::THREADS, Lay<DH, terms_o
     }
   } else {  // ------------------------------------------------------------ softmax
     set_regs<true, L::REGS_SOFT>();
-    if (BLK == 1) rs = *reinterpret_cast<volatile float *>(smem + L::ML + tid * 8);
+    if (NT == 1) rs = *reinterpret_cast<volatile float *>(smem + L::ML + tid * 8);
     const int blk = BLK == 1 ? 0 : warp >> 2;
     const uint32_t lanes = ((uint32_t)((warp & 3) * 32) << 16) + blk * L::COLS;
     const bool work = tile0 + warp * 32 < u.rows;  // (the whole warp)
@@ -778,30 +777,31 @@ struct Kernel {
   void (*k)(AttnKArgs);
   int threads, smem, regs;
 };
-template <int TYPE, int DH, class E>
+template <int TYPE, int DH, class E, int BLK>
 Kernel kernel_as(bool many) {
-  using L = Lay<DH, terms_of<E>>;
+  using L = Lay<DH, terms_of<E>, BLK>;
   if constexpr (terms_of<E> == 1)
-    if (many) return {k_kv_attn_tc<TYPE, DH, E, true>, L::THREADS, L::BYTES, L::REGS};
-  return {k_kv_attn_tc<TYPE, DH, E, false>, L::THREADS, L::BYTES, L::REGS};
+    if (many) return {k_kv_attn_tc<TYPE, DH, E, true, BLK>, L::THREADS, L::BYTES, L::REGS};
+  return {k_kv_attn_tc<TYPE, DH, E, false, BLK>, L::THREADS, L::BYTES, L::REGS};
 }
-template <class E>
+template <class E, int BLK>
 Kernel kernel_of(const pk_kv_cache &c, bool many) {
-  if (c.head_dim == 64) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 64, E>(many) : kernel_as<PK_KV_Q4, 64, E>(many);
-  if constexpr (terms_of<E> == 1) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 128, E>(many) : kernel_as<PK_KV_Q4, 128, E>(many);
+  if (c.head_dim == 64) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 64, E, BLK>(many) : kernel_as<PK_KV_Q4, 64, E, BLK>(many);
+  if constexpr (terms_of<E> == 1) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 128, E, BLK>(many) : kernel_as<PK_KV_Q4, 128, E, BLK>(many);
   return {};
 }
 
 }  // namespace
 
-cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int cluster, unsigned blocks, cudaStream_t st) {
+cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int rows, int cluster, unsigned blocks, cudaStream_t st) {
   const int e = a.q.type == T_F32 ? 0 : a.q.type == T_F16 ? 1 : 2;
   const bool many = e && a.chunk > sum_most(a.q.type);  // (positions; only half precision sums in TMEM)
-  const Kernel k = e == 0 ? kernel_of<float>(a.c, many) : e == 1 ? kernel_of<__half>(a.c, many) : kernel_of<__nv_bfloat16>(a.c, many);
+  const Kernel k = e == 0 ? rows == 256 ? kernel_of<float, 2>(a.c, many) : kernel_of<float, 1>(a.c, many)
+                   : e == 1 ? kernel_of<__half, 1>(a.c, many) : kernel_of<__nv_bfloat16, 1>(a.c, many);
   if (!k.k) return cudaErrorInvalidValue;
   // the split of the registers would wait forever for what a launch does not have
   static std::atomic<unsigned> checked{0};
-  const unsigned bit = 1u << (16 * many + e * 4 + 2 * (a.c.type == PK_KV_Q4) + (a.c.head_dim == 128));
+  const unsigned bit = 1u << (16 * many + (e == 0 && rows == 256 ? 3 : e) * 4 + 2 * (a.c.type == PK_KV_Q4) + (a.c.head_dim == 128));
   if (!(checked.load(std::memory_order_relaxed) & bit)) {
     cudaFuncAttributes f;
     const cudaError_t err = cudaFuncGetAttributes(&f, reinterpret_cast<const void *>(k.k));
