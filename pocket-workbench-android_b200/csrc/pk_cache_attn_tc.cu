@@ -156,7 +156,8 @@ __device__ __forceinline__ uint64_t seen_by(const AttnKArgs &a, const Unit &u, i
   return v & ones(hi - p0) & ones(u.sv.ctx + u.sv.n - p0);
 }
 
-template <int TYPE, int DH, class E, bool LONG, int BLK>
+// JOINS: rows are joined with their prefixes' parts (a.merge).
+template <int TYPE, int DH, class E, bool LONG, int BLK, bool JOINS>
 __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, terms_of<E>, BLK>::CTAS) k_kv_attn_tc(const AttnKArgs a) {
   constexpr int NT = terms_of<E>;
   using L = Lay<DH, NT, BLK>;
@@ -516,8 +517,8 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
 #pragma unroll
           for (int n = 0; n < NT; n++) st_pairs(tmem + lanes + L::P_COL + n * (NK / 2) + 16 * h, w[n][0], w[n][1]);
         };
-        bool longer = masked || i == 0;  // (the first tile has no reference yet)
-        if (!longer) {
+        bool longer = masked;
+        if (!masked) {
           sum[0] = sum[1] = sum[2] = sum[3] = make_float2(0.0f, 0.0f);
           __syncwarp();
           if constexpr (NT == 1) {  // 16 columns are on their way while those before are worked on
@@ -542,7 +543,8 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
               put_two(h);
             }
           }
-          // (a thread's part of a row's sum is at least the largest of its weights)
+          // (a thread's part of a row's sum is at least the largest of its
+          // weights; m is -inf at first: infinite)
           bool over = false;
           float all[4];
 #pragma unroll
@@ -683,7 +685,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
       if (part) {
         if (on && cluster) *reinterpret_cast<float2 *>(smem + L::ML + tid * 8) = make_float2(m, l);
         else if (on) a.part_ml[slot] = make_float2(m, l);
-      } else if (!a.merge) {
+      } else if (!JOINS) {
         f *= l > 0.0f || isnan(l) ? 1.0f / l : 0.0f;
       }
       if (l == 0.0f) f = 0.0f;
@@ -714,7 +716,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
       __syncwarp();
       if (!cluster) {
         Merge mg{};
-        if (a.merge) {
+        if (JOINS) {
           if (a.early) pdl_wait();
           mg = merge_of<DH>(a, u, min(row, u.rows - 1), m, l);
         }
@@ -727,7 +729,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
           const long long to = __shfl_sync(0xffffffffu, off, r) + d0;
           const float4 v = *reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(smem) + (warp * 32 + r) * (DH + 4) + d0);
           float x[4] = {v.x, v.y, v.z, v.w};
-          if (a.merge) {
+          if (JOINS) {
             Merge one;
             one.n = mg.n;  // (of one sequence)
             one.own = __shfl_sync(0xffffffffu, mg.own, r);
@@ -769,7 +771,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
   }
   __syncwarp();
   if (cluster) join_cluster<DH>(a, u, tile0, ROWS, sb, sb + L::ML, THREADS);
-  if (!a.merge) end_early(a);
+  if (!JOINS) end_early(a);
   if (tid == 0 && a.err && *abort) atomicCAS(a.err, 0, PK_ERR_TIMEOUT);
 }
 
@@ -778,16 +780,17 @@ struct Kernel {
   int threads, smem, regs;
 };
 template <int TYPE, int DH, class E, int BLK>
-Kernel kernel_as(bool many) {
+Kernel kernel_as(bool many, bool joins) {
   using L = Lay<DH, terms_of<E>, BLK>;
+  if (joins) return {k_kv_attn_tc<TYPE, DH, E, false, BLK, true>, L::THREADS, L::BYTES, L::REGS};
   if constexpr (terms_of<E> == 1)
-    if (many) return {k_kv_attn_tc<TYPE, DH, E, true, BLK>, L::THREADS, L::BYTES, L::REGS};
-  return {k_kv_attn_tc<TYPE, DH, E, false, BLK>, L::THREADS, L::BYTES, L::REGS};
+    if (many) return {k_kv_attn_tc<TYPE, DH, E, true, BLK, false>, L::THREADS, L::BYTES, L::REGS};
+  return {k_kv_attn_tc<TYPE, DH, E, false, BLK, false>, L::THREADS, L::BYTES, L::REGS};
 }
 template <class E, int BLK>
-Kernel kernel_of(const pk_kv_cache &c, bool many) {
-  if (c.head_dim == 64) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 64, E, BLK>(many) : kernel_as<PK_KV_Q4, 64, E, BLK>(many);
-  if constexpr (terms_of<E> == 1) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 128, E, BLK>(many) : kernel_as<PK_KV_Q4, 128, E, BLK>(many);
+Kernel kernel_of(const pk_kv_cache &c, bool many, bool joins) {
+  if (c.head_dim == 64) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 64, E, BLK>(many, joins) : kernel_as<PK_KV_Q4, 64, E, BLK>(many, joins);
+  if constexpr (terms_of<E> == 1) return c.type == PK_KV_Q8 ? kernel_as<PK_KV_Q8, 128, E, BLK>(many, joins) : kernel_as<PK_KV_Q4, 128, E, BLK>(many, joins);
   return {};
 }
 
@@ -795,13 +798,13 @@ Kernel kernel_of(const pk_kv_cache &c, bool many) {
 
 cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int rows, int cluster, unsigned blocks, cudaStream_t st) {
   const int e = a.q.type == T_F32 ? 0 : a.q.type == T_F16 ? 1 : 2;
-  const bool many = e && a.chunk > sum_most(a.q.type);  // (positions; only half precision sums in TMEM)
-  const Kernel k = e == 0 ? rows == 256 ? kernel_of<float, 2>(a.c, many) : kernel_of<float, 1>(a.c, many)
-                   : e == 1 ? kernel_of<__half, 1>(a.c, many) : kernel_of<__nv_bfloat16, 1>(a.c, many);
+  const bool joins = a.merge, many = e && !joins && a.chunk > sum_most(a.q.type);  // (positions; only half precision sums in TMEM)
+  const Kernel k = e == 0 ? rows == 256 ? kernel_of<float, 2>(a.c, many, joins) : kernel_of<float, 1>(a.c, many, joins)
+                   : e == 1 ? kernel_of<__half, 1>(a.c, many, joins) : kernel_of<__nv_bfloat16, 1>(a.c, many, joins);
   if (!k.k) return cudaErrorInvalidValue;
   // the split of the registers would wait forever for what a launch does not have
-  static std::atomic<unsigned> checked{0};
-  const unsigned bit = 1u << (16 * many + (e == 0 && rows == 256 ? 3 : e) * 4 + 2 * (a.c.type == PK_KV_Q4) + (a.c.head_dim == 128));
+  static std::atomic<uint64_t> checked{0};
+  const uint64_t bit = 1ull << (32 * joins + 16 * many + (e == 0 && rows == 256 ? 3 : e) * 4 + 2 * (a.c.type == PK_KV_Q4) + (a.c.head_dim == 128));
   if (!(checked.load(std::memory_order_relaxed) & bit)) {
     cudaFuncAttributes f;
     const cudaError_t err = cudaFuncGetAttributes(&f, reinterpret_cast<const void *>(k.k));
