@@ -46,7 +46,7 @@ constexpr int BINS = 1024, CAP = 512;  // of the histogram; tokens that one CTA 
 constexpr int FEW = 128;               // that one warp sorts
 static_assert(BINS == 2 * ST && CAP == ST, "two bins and a sorted token a thread");
 constexpr int TB = 4, TABLE = 1 << TB;  // table of 2^(i / TABLE): 16 entries of 8 bytes are in different banks
-constexpr float MARGIN = 6e-5f;        // of sums of the histogram's weights, with 16 bits of each
+constexpr float MARGIN = 3e-5f;        // of the histogram's weights in f32, besides the bits that they lose
 constexpr int LAST = 0x7fffffff;
 constexpr float MAXF = 3.402823466e38f;
 
@@ -994,7 +994,7 @@ cudaError_t launch_sample(const void *logits, int type, int rows, int n, long st
   // 24 bits of a weight, of which 16 are kept: 65536 of a bin and CTA fit 32 bits
   a.drop = 8;
   for (long long x = 65536; x < a.seg; x *= 2) a.drop++;
-  a.margin = MARGIN + (float)n * 0x1p-31f;
+  a.margin = MARGIN + (float)(1 << a.drop) * 0x1p-23f + (float)n * 0x1p-31f;  // (the last bin's weights are left out)
   const int smem = (int)sizeof(Smem) + (big ? 0 : (int)(seg * 16));
   const dim3 grid((unsigned)(rows * c)), block(ST);
   const bool rules = p.top_k || p.top_p || p.min_p;

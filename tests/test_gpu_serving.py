@@ -267,6 +267,95 @@ def test_shared_bounds(pk, ty):
     assert (got[a].double() - cut[a].double()).abs().max() <= lim * cut[a].double().abs().max()
 
 
+@pytest.mark.parametrize("kind", ["q8", "q4"])
+@pytest.mark.parametrize("dh", [64, 128])
+@pytest.mark.parametrize("ty", list(DT))
+def test_shared_many_rows(pk, kind, dh, ty):
+    """Hundreds of rows a group: several tiles, a prefix of several chunks that ends inside a tile, pages of it missing,
+    garbage where nothing is read, V rows far apart in size, and rows of NaN and infinities that stay their own."""
+    groups, new = [(9300, 45), (260, 30), (2000, 3)], [2] * 45 + [1] * 30 + [7, 1, 60]
+    own = [(7 * i) % 40 for i in range(78)]
+    su = SharedSetup(pk, groups, own, new, kind, 2, dh, 32, seed=3)
+    c = su.cache
+    table = su.shared_seqs.pages
+    holes = {}
+    for g, gone in ((0, (0, 5, 100, 200)), (1, (3,)), (2, (0, 1, 2))):  # pages of the prefix that are none
+        table[int(su.first[g]), list(gone)] = -1
+        for s in range(int(su.first[g]), int(su.first[g + 1])):
+            holes[s] = gone
+    free = sorted(set(range(c.n_pages)) - set(su.table.ravel().tolist()))
+    for t in (c.ks, c.vs):
+        t[free, ..., 0] = math.nan
+    for s in range(45):  # a few large rows, in every copy of the prefix
+        c.vs[torch.as_tensor(su.table[s, :9].astype(np.int64)).cuda(), :, ::3, 0] *= 300.0
+    q = randn((su.n_tok, 8, dh), 8, DT[ty], std=1.5)
+
+    def gone(s):
+        p = torch.arange(su.lens[s] + su.new[s], device="cuda")
+        return ((p[:, None] // 32) == torch.tensor(holes[s], device="cuda")[None]).any(1) & (p < groups[su.lead[s]][0] // 16 * 16)
+
+    got = su.attend(q)
+    check_attention(su, q, got, holes=gone)
+    bad = q.clone()
+    bad[5, 3] = math.nan
+    bad[91, 0, 7] = math.inf
+    other = su.attend(bad)
+    assert torch.isnan(other[5, 3]).all() and torch.isnan(other[91, 0]).all()
+    same = torch.ones(q.shape[:2], dtype=torch.bool, device="cuda")
+    same[5, 3] = same[91, 0] = False
+    assert (other[same].double() - got[same].double()).abs().max() <= 4 * torch.finfo(DT[ty]).eps * got.double().abs().max()
+
+
+@pytest.mark.parametrize("ty", list(DT))
+def test_shared_nothing_of_ones_own(pk, ty):
+    """max_own 0: every row sees its group's prefix alone, and of a sequence in no group nothing."""
+    groups = [(208, 20), (96, 2)]
+    su = SharedSetup(pk, groups, [0] * 22, [1] * 22, "q8", 2, 64, 16, seed=6)
+    q = randn((su.n_tok, 16, 64), 3, DT[ty])
+    sh = pk.KvShared(i32([0, 20]), i32([208]), 20, 208, 0)
+    got = su.cache.attend(su.shared_seqs, q, shared=sh)
+    cut = Setup.__new__(Setup)
+    cut.__dict__.update(su.__dict__)
+    cut.lens, cut.new = [207] * 20, [1] * 20  # (its last position as if it were the token's own)
+    cut.start = su.start[:21]
+    want, absv, dots = attention(cut, q[:20])
+    from test_gpu_drafts import attn_bound
+
+    assert ((got[:20].double() - want).abs() <= attn_bound(q[:20], want, absv, dots, 64)).all()
+    assert (got[20:] == 0).all()
+
+
+def test_shared_side_by_side(pk):
+    """Calls of different shapes at once on two streams and in captured graphs, each with its own scratch."""
+    runs = []
+    for i, (ty, dh, case) in enumerate((("f16", 128, 5), ("f32", 64, 4), ("bf16", 64, 7), ("f16", 64, 2), ("bf16", 128, 6))):
+        groups, own, new, n_head, n_kv, page = GROUPS[case]
+        su = SharedSetup(pk, groups, own, new, "q4" if i % 2 else "q8", n_kv, dh, page, seed=i)
+        q = randn((su.n_tok, n_head, dh), i, DT[ty])
+        runs.append((su, q, su.attend(q)))
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    graphs = []
+    for j, (su, q, want) in enumerate(runs):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = su.attend(q)
+        graphs.append((g, out))
+    torch.cuda.synchronize()
+    for turn in range(10):
+        got = []
+        for w, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                for j in range(len(runs)):
+                    k = (j + w + turn) % len(runs)
+                    if w == 2:
+                        graphs[k][0].replay()
+                    else:
+                        got.append((k, runs[k][0].attend(runs[k][1])))
+        torch.cuda.synchronize()
+        for k, o in got + [(k, o) for k, (_, o) in enumerate(graphs)]:
+            assert torch.equal(o, runs[k][2]), k
+
+
 def test_shared_strides_scratch_and_order(pk):
     """Strided and unaligned rows, a given scratch, a second call that gives the same bits, and rows in any place."""
     su = SharedSetup(pk, *GROUPS[5][:3], "q8", 2, 128, 64, seed=9)
