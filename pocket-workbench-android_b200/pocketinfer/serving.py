@@ -89,24 +89,30 @@ def kv_plan(ctx, n_new, pages, held, free, n_free, page_size: int, n_tok: int, d
     i32, dev, n = torch.int32, ctx.get_device(), ctx.shape[0] if ctx.dim() == 1 else -1
     if dev < 0 or n < 0:
         _bad("kv_plan: ctx must be [n_seq] on a CUDA device")
-    ptrs = []
-    for t, name, shape in ((ctx, "ctx", (n,)), (n_new, "n_new", (n,)), (pages, "pages", None), (held, "held", (n,)), (free, "free", None),
-                           (n_free, "n_free", (1,)), (done, "done", (n,)), (shared, "shared", (n,))):
-        if t is None:
-            ptrs.append(0)
-            continue
-        if t.dtype is not i32 or t.get_device() != dev or not t.is_contiguous() or (shape is not None and t.shape != shape):
-            _bad(f"kv_plan: {name} must be a contiguous int32 tensor{'' if shape is None else f' of {shape[0]}'} on device {dev}")
-        ptrs.append(t.data_ptr())
-    if pages.dim() != 2 or pages.shape[0] != n or free.dim() != 1:
-        _bad("kv_plan: pages must be [n_seq, max_pages] and free a list")
+    whole = (n,)
+    if done is None or shared is None:
+        for t, name in ((done, "done"), (shared, "shared")):
+            if t is not None and (t.dtype is not i32 or t.get_device() != dev or t.shape != whole or not t.is_contiguous()):
+                _bad(f"kv_plan: {name} must be a contiguous int32 tensor of {n} on device {dev}")
+        per_slot, ends = (ctx, n_new, held), (0 if done is None else done.data_ptr(), 0 if shared is None else shared.data_ptr())
+    else:
+        per_slot, ends = (ctx, n_new, held, done, shared), (done.data_ptr(), shared.data_ptr())
+    for t in per_slot:
+        if t.dtype is not i32 or t.shape != whole or t.get_device() != dev or not t.is_contiguous():
+            _bad(f"kv_plan: ctx, n_new, held, done and shared must be contiguous int32 tensors of {n} on device {dev}")
+    for t in (pages, free, n_free):
+        if t.dtype is not i32 or t.get_device() != dev or not t.is_contiguous():
+            _bad(f"kv_plan: pages, free and n_free must be contiguous int32 tensors on device {dev}")
+    ptrs = (ctx.data_ptr(), n_new.data_ptr(), pages.data_ptr(), held.data_ptr(), free.data_ptr(), n_free.data_ptr())
+    if pages.dim() != 2 or pages.shape[0] != n or free.dim() != 1 or n_free.shape != (1,):
+        _bad("kv_plan: pages must be [n_seq, max_pages], free a list and n_free one number")
     if not 0 <= n_tok <= 1 << 30:
         _bad("kv_plan: n_tok must be 0 to 2^30")
     wide, cap = pages.shape[1], free.shape[0]
     # one block for all results (a tensor of its own each costs more than the launch): first what has to be aligned
     table = 0 if in_place else n * wide + (n * wide & 1)
     sizes = (table, 2 * n_tok, n + 1, n_tok, n_tok, 1) if in_place else (table, 2 * n_tok, n + 1, n_tok, n_tok, 1, n, cap, 1)
-    make = lambda: torch.empty(sum(sizes), dtype=i32, device=ctx.device).split_with_sizes(sizes)  # noqa: E731
+    make = lambda: ctx.new_empty(sum(sizes)).split_with_sizes(sizes)  # noqa: E731
     made = make() if stream is None else _new(make, dev, stream)
     slot, start, pos, seq, lacking = made[1].view(torch.int64), made[2], made[3], made[4], made[5]
     if in_place:
@@ -115,7 +121,7 @@ def kv_plan(ctx, n_new, pages, held, free, n_free, page_size: int, n_tok: int, d
         block = made[0] if table == n * wide else made[0][:-1]
         out = (block.view(n, wide), made[6], made[7], made[8])
         to = (block.data_ptr(), made[6].data_ptr(), made[7].data_ptr(), made[8].data_ptr())
-    args = PACK_PLAN(*ptrs, *to, start.data_ptr(), lacking.data_ptr(), pos.data_ptr(), seq.data_ptr(), slot.data_ptr(), n, wide, cap, n_tok, page_size)
+    args = PACK_PLAN(*ptrs, *ends, *to, start.data_ptr(), lacking.data_ptr(), pos.data_ptr(), seq.data_ptr(), slot.data_ptr(), n, wide, cap, n_tok, page_size)
     _call(_d._L.pk_kv_plan, dev, stream, stream is not None and (ctx, n_new, pages, held, free, n_free, done, shared, made), args)
     return KvPlan(start, pos, seq, slot, *out, lacking)
 
@@ -135,12 +141,11 @@ def sample_rows(logits, u, temp=None, top_k=None, top_p=None, min_p=None, stream
     if u is None:
         _bad("sample_rows: u is missing")
 
-    def make():
-        block = _d.torch.empty((3, rows), dtype=i, device=logits.device)
-        return block[0], block[1].view(f), block[2]
-
+    at_u = _row_value(u, "u", f, rows, dev)
+    make = lambda: u.new_empty((3, rows)).unbind()  # noqa: E731
     tok, prob, kept = made = make() if stream is None else _new(make, dev, stream)
-    args = PACK_SAMPLE(_row_value(u, "u", f, rows, dev), _row_value(temp, "temp", f, rows, dev), _row_value(top_k, "top_k", i, rows, dev),
+    tok, kept = tok.view(i), kept.view(i)
+    args = PACK_SAMPLE(at_u, _row_value(temp, "temp", f, rows, dev), _row_value(top_k, "top_k", i, rows, dev),
                        _row_value(top_p, "top_p", f, rows, dev), _row_value(min_p, "min_p", f, rows, dev), tok.data_ptr(), prob.data_ptr(), kept.data_ptr())
     _call(_d._L.pk_sample_rows, dev, stream, stream is not None and (logits, u, temp, top_k, top_p, min_p, made), logits.data_ptr(), code, rows, n,
           st[0] if len(st) == 2 else n, args)
