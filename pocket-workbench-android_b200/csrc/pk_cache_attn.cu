@@ -730,16 +730,23 @@ template <int TYPE, int DH>
 Variant variant_type(int type, long long rows) {
   return type == T_F32 ? variant_rows<TYPE, DH, 2>(rows) : variant_rows<TYPE, DH, 1>(rows);
 }
-// short_too: half-precision rows past 16 may take the kernel here, a tile of 16 at
-// a time, where that is less work: a CTA of the tcgen05 kernel costs its tiles of
-// 64 positions and 16 more for its beginning and end, one here 4 more, and its
-// tiles three quarters of the time (96 sequences of 24 rows and up to 318
-// positions behind 12 prefixes: the call 91 us so, 108 with the tcgen05 kernel,
-// 93 with tiles of 32 rows; 4 answers to a prompt of 700: 17, 31 and 18).
-Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type, bool short_too = false) {
+// tiles_too: more than 8 rows may go a tile of 8 at a time, each reading the cache
+// again (from L2), where that is less work.  Against the tcgen05 kernel, a CTA of
+// which costs its tiles of 64 positions and 16 more for its beginning and end, one
+// here costs 4 more; its tile takes 10 eighteenths of the time there, and 10
+// thirty-sixths where CTAs are so few that only their latency counts.  Against
+// wider tiles here it is better in the second case, where there is little to do:
+// code for 16 rows a warp is twice as long, and a CTA of few tiles waits for
+// instructions most of its time.  (96 sequences of 24 rows and up to 318 positions behind 12
+// prefixes: the call 69 us so, 91 with tiles of 16, 108 with the tcgen05 kernel; 4
+// answers to a prompt of 700: 12, 17 and 31.)
+Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type, bool tiles_too = false) {
   long long rows = (long long)s.max_new * (n_head / c.n_kv);
-  const long long tiles = (s.max_len + 63) / 64;
-  if (short_too && type != T_F32 && rows >= TC_FROM && (rows + 15) / 16 * (tiles + 4) * 3 < (rows + 127) / 128 * (tiles + 16) * 4) rows = TC_FROM - 1;
+  if (tiles_too && rows > 8) {
+    const long long tiles = (s.max_len + 63) / 64, each = (rows + 7) / 8;
+    const bool few = (long long)s.n_seq * c.n_kv * each <= 148, tc = rows >= (type != T_F32 ? TC_FROM : c.head_dim == 64 ? TC32_FROM : 1LL << 40);
+    if (tc ? each * (tiles + 4) * 10 < (rows + 127) / 128 * (tiles + 16) * (few ? 36 : 18) : few && each * tiles <= 256) rows = 8;
+  }
   if (c.type == PK_KV_Q8) return c.head_dim == 64 ? variant_type<PK_KV_Q8, 64>(type, rows) : variant_type<PK_KV_Q8, 128>(type, rows);
   return c.head_dim == 64 ? variant_type<PK_KV_Q4, 64>(type, rows) : variant_type<PK_KV_Q4, 128>(type, rows);
 }
@@ -859,8 +866,12 @@ cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &seqs, const p
 }
 
 // Shared prefixes: the groups as sequences of their tokens over the positions
-// that they share, then each sequence over the rest of its own, and a launch
-// that joins the parts.
+// that they share, then each sequence over the rest of its own.  The second launch
+// begins beside the first one's last CTAs (it reads nothing that the first one
+// writes until it joins) and adds the prefix's parts to its rows itself where a
+// sequence's rest is one chunk; otherwise a third one joins all parts.  64 streams
+// behind 4001 positions: 70 us with three launches one after another, 53 so; every
+// stream by itself over all its positions 350.
 namespace {
 struct Shared {
   pk_kv_seqs pre, own;  // bounds of the two

@@ -17,6 +17,14 @@
 // Warps: 8 softmax (4 a block, four lanes a row as there), 4 that make K's codes
 // f16 and pass on both scales, 4 for V's, 4 of which one thread issues the
 // products.  Waits are bounded as there.
+//
+// Measured: two prefixes of 24000 positions under 800 tokens each, 64 heads over 8
+// of 128, bf16, Q8: 1.55 ms, 812 TFLOP/s (the kernel of 128 rows: 1.72 ms).  What
+// bounds it: a block's tile takes its softmax warps 3,300 cycles and its products
+// 1,040, the two blocks' products 2,080 of every 4,600; shared memory is three
+// quarters busy between the products' operands, the codes made f16 and the
+// scales.  Twice the softmax warps, two for the same rows, took 1.80 ms (their
+// registers did not hold a tile's weights).
 #include <algorithm>
 #include <atomic>
 

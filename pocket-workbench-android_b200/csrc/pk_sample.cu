@@ -27,6 +27,14 @@
 //
 // A row is read once, into the shared memory of a cluster of up to 8 CTAs, and
 // gone over there; rows that do not fit are read again each time.
+//
+// Measured: 250 f32 rows of 128256: the largest alone 51 us, temperature alone
+// 97, top-k 40 93, top-p 0.6 at temperature 1.5 230, rows with rules of their own
+// 160 (the rows' bytes take 20); 64 bf16 rows of 73448, top-p 0.9: 40; one f32
+// row of 73448, all rules: 10.  What bounds it: instructions (64 M for the 250
+// rows with rules, 1.8 a cycle and SM; 33 an element for an exact weight) and the
+// steps that a cluster takes one after another, during which two CTAs an SM leave
+// it half idle.
 #include <math_constants.h>
 
 #include <algorithm>
