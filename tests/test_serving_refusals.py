@@ -73,7 +73,7 @@ def test_plan(pk):
     # in place: all of them or none
     same = {"pages": A, "pages_out": A, "held": A + 512, "held_out": A + 512, "free": A + 1024, "free_out": A + 1024, "n_free": A + 2048, "n_free_out": A + 2048}
     for name in ("pages_out", "held_out", "free_out", "n_free_out"):
-        assert call(**{**same, name: A + 3072}) == INVALID, name
+        assert call(**{**same, name: A + 4096}) == INVALID, name
         assert "in place" in pk.last_error()
     assert lib.pk_kv_plan(None, None) == INVALID
 
