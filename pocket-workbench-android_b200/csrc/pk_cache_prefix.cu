@@ -37,7 +37,7 @@ namespace {
 constexpr int PK_N = 128, PROWS = 256;  // positions a tile, rows a CTA
 constexpr int PSOFT = 256, PCONV = 128, PMMA = 128, PTHREADS = PSOFT + 2 * PCONV + PMMA, PWS = PSOFT / 32;
 // registers a thread: at launch, then by warps
-constexpr int PREGS = 96, PREGS_SOFT = 168, PREGS_CONV = 56, PREGS_MMA = 32;
+constexpr int PREGS = 96, PREGS_SOFT = 160, PREGS_CONV = 64, PREGS_MMA = 32;
 static_assert(PSOFT * PREGS_SOFT + 2 * PCONV * PREGS_CONV + PMMA * PREGS_MMA <= PTHREADS * PREGS, "no more than the launch's");
 
 template <int DH>
@@ -45,11 +45,61 @@ struct PLay {
   static constexpr int CH = PK_N * 16 + 16, TILE = DH / 8 * CH;  // chunks of 16 bytes (8 dimensions) of a tile's positions, padded
   static constexpr int Q = 0, K = PROWS * DH * 2, V = K + 2 * TILE, OPS = V + 2 * TILE, SUMS = PROWS * (DH + 4) * 4;
   static constexpr int SC = OPS > SUMS ? OPS : SUMS;
-  // of four tiles: D^K, D^V, what is added to the scores (0 or -inf); positions that hold something (4 words), largest D^V of 32 (4)
-  static constexpr int SCB = 3 * PK_N * 4 + 32, BAR = SC + 4 * SCB, RS = BAR + 64 + 48 * 2, BYTES = RS + PROWS * 4;
+  // of four tiles: D^K, D^V, what is added to the scores (0 or -inf), log2 D^V; positions that hold something (4 words), largest D^V of 32 (4)
+  static constexpr int SCB = 4 * PK_N * 4 + 32, BAR = SC + 4 * SCB, BYTES = BAR + 64 + 48 * 2 + 8;
   static constexpr int S_COL = 0, O_COL = PK_N, COLS = 256;  // of a block's
   static_assert(BYTES <= 227 * 1024, "an SM's");
 };
+
+// A warp's 32 query rows into the operand, as put_q_half does: eight rows at a
+// time, four lanes a row (eight lanes that store together have a vector of each
+// row: no bank twice); up[j]: the scale of row lane % 8 + 8 j.
+template <int TYPE, int DH, class E>
+__device__ __forceinline__ void put_q_rows(const AttnKArgs &a, const Unit &u, int row0, uint32_t dst, float (&up)[4]) {
+  constexpr bool F16 = std::is_same_v<E, __half>;
+  constexpr int N = DH / 32;  // vectors of 8 a lane
+  const int lane = threadIdx.x & 31, part = lane >> 3;
+  uint4 raw[4][N];
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const int row = row0 + 8 * k + (lane & 7), i = row / a.group, h = u.h * a.group + row - i * a.group;
+    const bool on = row < u.rows;
+    const E *p = reinterpret_cast<const E *>(a.q.q) + (on ? (long long)(u.sv.first + i) * a.q.q_tok_stride + (long long)h * a.q.q_head_stride : 0) + part * 8;
+    if (on && a.vec_q) {
+#pragma unroll
+      for (int c = 0; c < N; c++) raw[k][c] = __ldg(reinterpret_cast<const uint4 *>(p + 32 * c));
+    } else {
+      E *y = reinterpret_cast<E *>(raw[k]);
+#pragma unroll
+      for (int j = 0; j < 8 * N; j++) y[j] = on ? p[j / 8 * 32 + j % 8] : from_f<E>(0.0f);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const E *x = reinterpret_cast<const E *>(raw[k]);
+    float m = 0.0f;
+    if (!F16) {
+#pragma unroll
+      for (int j = 0; j < 8 * N; j++) m = fmaxf(m, fabsf(to_f(x[j])));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+    }
+    int e = (int)(__float_as_uint(m) >> 23) - 127;
+    e = m > 0.0f ? min(max(e, -100), 126) : 0;
+    const float down = __int_as_float((127 - e) << 23);
+    up[k] = __int_as_float((e + 127) << 23);
+#pragma unroll
+    for (int c = 0; c < N; c++) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const float x0 = to_f(x[8 * c + dim8<TYPE>(2 * j)]), x1 = to_f(x[8 * c + dim8<TYPE>(2 * j + 1)]);
+        w[j] = pack2(fmaf(x0, down, x0 - x0), fmaf(x1, down, x1 - x1));  // (infinities as NaN)
+      }
+      sts128(dst + (8 * k + (lane & 7)) * 16 + (part + 4 * c) * (PROWS * 16), w[0], w[1], w[2], w[3]);
+    }
+  }
+}
 
 template <int TYPE, int DH, class E>
 __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
@@ -67,8 +117,8 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const uint32_t sb = shaddr(smem);
   // barriers: K and scales ready x 4, V ready x 2; the TMEM address, the abort
-  // flag; all products done; for each block of 128 rows: S full x 2, P ready x 2, PV done x 2
-  const uint32_t bar = sb + L::BAR, kready = bar, vready = bar + 32, done = bar + 56, blocks = bar + 64;
+  // flag; all products done; for each block of 128 rows: S full x 2, P ready x 2, PV done x 2; Q ready
+  const uint32_t bar = sb + L::BAR, kready = bar, vready = bar + 32, done = bar + 56, blocks = bar + 64, qready = bar + 160;
   volatile int *abort = reinterpret_cast<volatile int *>(smem + L::BAR + 52);
   const int nblk = min(2, (u.rows - tile0 + 127) / 128);  // that have rows
   auto sfull_of = [&](int blk, int i) { return blocks + 48 * blk + 8 * (i & 1); };
@@ -85,18 +135,13 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
       }
     }
     mbar_init(done, 1);
+    mbar_init(qready, PSOFT);
     *abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == PWS + 8) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(bar + 48), "r"(2 * L::COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
-  if (tid < 2 * PROWS) {
-    const int r = tid >> 1, part = tid & 1;
-    const float up = put_q_half<TYPE, DH, E>(a, u, tile0 + r, part, sb + L::Q + r * 16, PROWS * 16);
-    if (part == 0) *reinterpret_cast<float *>(smem + L::RS + r * 4) = up;
-    fence_async_smem();
   }
   tc_fence_before();
   __syncthreads();
@@ -111,12 +156,13 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
       const uint64_t qd = tc_desc(sb + L::Q, PROWS * 16, 128), kd = tc_desc(sb + L::K, L::CH, 128), vd = tc_desc(sb + L::V, 128, L::CH);
       auto scores = [&](int i, int m) {
         const uint64_t q = qd + m * 128, k = kd + (i & 1) * (L::TILE / 16);
-#pragma unroll
+#pragma unroll 1
         for (int s = 0; s < DH / 16; s++)
           mma_f16<PK_N, false>(tmem + m * L::COLS + L::S_COL, q + s * 2 * PROWS, k + s * 2 * (L::CH / 16), s > 0);
         mbar_arrive(sfull_of(m, i));
         commit_one(sfull_of(m, i));
       };
+      wait_one(qready, 0, abort);
       wait_one(kready, 0, abort);
       tc_fence_after();
       for (int m = 0; m < nblk; m++) scores(0, m);
@@ -128,7 +174,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
           tc_fence_after();
           const uint32_t w = tmem + m * L::COLS + L::S_COL, o = tmem + m * L::COLS + L::O_COL;
           const uint64_t v = vd + (i & 1) * (L::TILE / 16);
-#pragma unroll
+#pragma unroll 1
           for (int s = 0; s < PK_N / 16; s++) mma_f16_ts<DH, true>(o, w + s * 8, v + s * 16, i > 0 || s > 0);
           commit_one(pvdone_of(m, i));
           if (i + 1 < nt) scores(i + 1, m);  // (over the weights just used: products are done in order)
@@ -216,11 +262,12 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
       f[ct] = on ? fminf(fmaxf(dk * (a.q.scale * kLog2e), -3e38f), 3e38f) : 0.0f;  // (finite: a query may be 0)
       f[PK_N + ct] = on ? dv : 0.0f;
       f[2 * PK_N + ct] = on ? 0.0f : -CUDART_INF_F;
+      f[3 * PK_N + ct] = on ? log2f(fabsf(dv)) : -CUDART_INF_F;
       const unsigned m = __ballot_sync(0xffffffffu, on);
       const uint32_t x = __reduce_max_sync(0xffffffffu, on ? __float_as_uint(dv) & 0x7fffffffu : 0);
       if (lane == 0) {
-        reinterpret_cast<uint32_t *>(sc + 3 * PK_N * 4)[ct >> 5] = m;
-        reinterpret_cast<uint32_t *>(sc + 3 * PK_N * 4 + 16)[ct >> 5] = x;
+        reinterpret_cast<uint32_t *>(sc + 4 * PK_N * 4)[ct >> 5] = m;
+        reinterpret_cast<uint32_t *>(sc + 4 * PK_N * 4 + 16)[ct >> 5] = x;
       }
     };
     const int n = a.poison ? 0 : 2 * nt;
@@ -244,14 +291,17 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
     const bool work = tile0 + warp * 32 < u.rows;  // (the whole warp)
     const int row = tile0 + tid, quad = lane & 3;
     const uint32_t cols = tmem + lanes + L::S_COL;
+    float up[4];
+    put_q_rows<TYPE, DH, E>(a, u, tile0 + warp * 32, sb + L::Q + warp * 32 * 16, up);
+    fence_async_smem();
+    mbar_arrive(qready);
     // of rows lane / 4 + 8 j: the scale, the reference, this thread's part of the sum
-    const float rs = *reinterpret_cast<volatile float *>(smem + L::RS + tid * 4);
     // (the scale and less the reference as pairs, too)
     float rs4[4], m4[4], l4[4];
     uint64_t scale2[4], less4[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      rs4[j] = __shfl_sync(0xffffffffu, rs, (lane >> 2) + 8 * j);
+      rs4[j] = __shfl_sync(0xffffffffu, up[j], lane >> 2);
       scale2[j] = pair_of(rs4[j], rs4[j]);
       less4[j] = 0;
       m4[j] = -CUDART_INF_F;
@@ -264,8 +314,8 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
         tc_fence_after();
         if (work) {
           const uint8_t *sc = smem + L::SC + (i & 3) * L::SCB;
-          const uint64_t *dk2 = reinterpret_cast<const uint64_t *>(sc) + quad, *dv2 = dk2 + PK_N / 2, *off2 = dk2 + PK_N;
-          const uint4 held = *reinterpret_cast<const uint4 *>(sc + 3 * PK_N * 4), r4 = *reinterpret_cast<const uint4 *>(sc + 3 * PK_N * 4 + 16);
+          const uint64_t *dk2 = reinterpret_cast<const uint64_t *>(sc) + quad, *dv2 = dk2 + PK_N / 2, *off2 = dk2 + PK_N, *log2v = dk2 + 3 * (PK_N / 2);
+          const uint4 held = *reinterpret_cast<const uint4 *>(sc + 4 * PK_N * 4), r4 = *reinterpret_cast<const uint4 *>(sc + 4 * PK_N * 4 + 16);
           const float vmax = fmaxf(fmaxf(__uint_as_float(r4.x), __uint_as_float(r4.y)), fmaxf(__uint_as_float(r4.z), __uint_as_float(r4.w)));
           const bool masked = (held.x & held.y & held.z & held.w) != 0xffffffffu;
           uint32_t w[2][32];
@@ -319,40 +369,36 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
           if (longer) {
             float mx[4], top[4], f[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) mx[j] = -CUDART_INF_F, top[j] = 0.0f;
+            for (int j = 0; j < 4; j++) mx[j] = top[j] = -CUDART_INF_F;
             auto quad_max = [](float x) {
               x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
               return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
             };
-            auto over_all = [&](auto step) {
+            // (of a tile with nothing in it mx is -inf, and its products NaN, which count for nothing)
 #pragma unroll 1
-              for (int k = 0; k < 8; k++) {
-                float t[16];
-                __syncwarp();
-                ask_quads(cols + 16 * k, t);
-                wait16(t);
+            for (int k = 0; k < 8; k++) {
+              float t[16];
+              __syncwarp();
+              ask_quads(cols + 16 * k, t);
+              wait16(t);
 #pragma unroll
-                for (int g = 0; g < 2; g++) {
-                  const float2 dk = unpair(dk2[4 * (2 * k + g)]), dv = unpair(dv2[4 * (2 * k + g)]), off = unpair(off2[4 * (2 * k + g)]);
+              for (int g = 0; g < 2; g++) {
+                const float2 dk = unpair(dk2[4 * (2 * k + g)]), lv = unpair(log2v[4 * (2 * k + g)]), off = unpair(off2[4 * (2 * k + g)]);
 #pragma unroll
-                  for (int j = 0; j < 4; j++) {
-                    const int p = 4 * (j >> 1) + 2 * g + (j & 1);
-                    step(j, fmaf(t[2 * p] * dk.x, rs4[j], off.x), dv.x);
-                    step(j, fmaf(t[2 * p + 1] * dk.y, rs4[j], off.y), dv.y);
-                  }
+                for (int j = 0; j < 4; j++) {
+                  const int p = 4 * (j >> 1) + 2 * g + (j & 1);
+                  const float x = fmaf(t[2 * p] * dk.x, rs4[j], off.x), y = fmaf(t[2 * p + 1] * dk.y, rs4[j], off.y);
+                  mx[j] = fmaxf(mx[j], fmaxf(x, y));
+                  top[j] = fmaxf(top[j], fmaxf(x + lv.x, y + lv.y));
                 }
               }
-            };
-            over_all([&](int j, float x, float) { mx[j] = fmaxf(mx[j], x); });
-#pragma unroll
-            for (int j = 0; j < 4; j++) mx[j] = quad_max(mx[j]);
-            // (of a tile with nothing in it mx is -inf, and its products NaN, which count for nothing)
-            over_all([&](int j, float x, float dv) { top[j] = fmaxf(top[j], ex2(x - mx[j]) * dv); });
+            }
             bool moved = false;
 #pragma unroll
             for (int j = 0; j < 4; j++) {
               f[j] = 1.0f;
-              const float most = mx[j] + log2f(fmaxf(quad_max(top[j]), 0x1p-100f));  // the largest product's exponent
+              mx[j] = quad_max(mx[j]);
+              const float most = fmaxf(quad_max(top[j]), mx[j] - 100.0f);  // the largest product's exponent
               if (mx[j] != -CUDART_INF_F && (m4[j] == -CUDART_INF_F || most > m4[j] + 8.0f || mx[j] > m4[j] + 90.0f)) {
                 const float now = fmaxf(most - 6.0f, mx[j] - 90.0f);
                 f[j] = ex2(m4[j] - now);
