@@ -53,30 +53,34 @@ struct PLay {
 
 // A warp's 32 query rows into the operand, as put_q_half does: eight rows at a
 // time, four lanes a row (eight lanes that store together have a vector of each
-// row: no bank twice); up[j]: the scale of row lane % 8 + 8 j.
+// row: no bank twice); rs[j]: the scale of row lane / 4 + 8 j.
 template <int TYPE, int DH, class E>
-__device__ __forceinline__ void put_q_rows(const AttnKArgs &a, const Unit &u, int row0, uint32_t dst, float (&up)[4]) {
+__device__ __forceinline__ void put_q_rows(const AttnKArgs &a, const Unit &u, int row0, uint32_t dst, float (&rs)[4]) {
   constexpr bool F16 = std::is_same_v<E, __half>;
   constexpr int N = DH / 32;  // vectors of 8 a lane
   const int lane = threadIdx.x & 31, part = lane >> 3;
-  uint4 raw[4][N];
-#pragma unroll
-  for (int k = 0; k < 4; k++) {
+  uint4 next[N];
+  auto ask = [&](int k) {
     const int row = row0 + 8 * k + (lane & 7), i = row / a.group, h = u.h * a.group + row - i * a.group;
     const bool on = row < u.rows;
     const E *p = reinterpret_cast<const E *>(a.q.q) + (on ? (long long)(u.sv.first + i) * a.q.q_tok_stride + (long long)h * a.q.q_head_stride : 0) + part * 8;
     if (on && a.vec_q) {
 #pragma unroll
-      for (int c = 0; c < N; c++) raw[k][c] = __ldg(reinterpret_cast<const uint4 *>(p + 32 * c));
+      for (int c = 0; c < N; c++) next[c] = __ldg(reinterpret_cast<const uint4 *>(p + 32 * c));
     } else {
-      E *y = reinterpret_cast<E *>(raw[k]);
+      E *y = reinterpret_cast<E *>(next);
 #pragma unroll
       for (int j = 0; j < 8 * N; j++) y[j] = on ? p[j / 8 * 32 + j % 8] : from_f<E>(0.0f);
     }
-  }
-#pragma unroll
+  };
+  ask(0);
+#pragma unroll 1
   for (int k = 0; k < 4; k++) {
-    const E *x = reinterpret_cast<const E *>(raw[k]);
+    uint4 raw[N];
+#pragma unroll
+    for (int c = 0; c < N; c++) raw[c] = next[c];
+    if (k < 3) ask(k + 1);
+    const E *x = reinterpret_cast<const E *>(raw);
     float m = 0.0f;
     if (!F16) {
 #pragma unroll
@@ -86,8 +90,9 @@ __device__ __forceinline__ void put_q_rows(const AttnKArgs &a, const Unit &u, in
     }
     int e = (int)(__float_as_uint(m) >> 23) - 127;
     e = m > 0.0f ? min(max(e, -100), 126) : 0;
-    const float down = __int_as_float((127 - e) << 23);
-    up[k] = __int_as_float((e + 127) << 23);
+    const float down = __int_as_float((127 - e) << 23), up = __shfl_sync(0xffffffffu, __int_as_float((e + 127) << 23), lane >> 2);
+#pragma unroll
+    for (int j = 0; j < 4; j++) rs[j] = j == k ? up : rs[j];
 #pragma unroll
     for (int c = 0; c < N; c++) {
       uint32_t w[4];
@@ -291,17 +296,15 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
     const bool work = tile0 + warp * 32 < u.rows;  // (the whole warp)
     const int row = tile0 + tid, quad = lane & 3;
     const uint32_t cols = tmem + lanes + L::S_COL;
-    float up[4];
-    put_q_rows<TYPE, DH, E>(a, u, tile0 + warp * 32, sb + L::Q + warp * 32 * 16, up);
-    fence_async_smem();
-    mbar_arrive(qready);
     // of rows lane / 4 + 8 j: the scale, the reference, this thread's part of the sum
     // (the scale and less the reference as pairs, too)
-    float rs4[4], m4[4], l4[4];
+    float rs4[4] = {1.0f, 1.0f, 1.0f, 1.0f}, m4[4], l4[4];
+    put_q_rows<TYPE, DH, E>(a, u, tile0 + warp * 32, sb + L::Q + warp * 32 * 16, rs4);
+    fence_async_smem();
+    mbar_arrive(qready);
     uint64_t scale2[4], less4[4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      rs4[j] = __shfl_sync(0xffffffffu, up[j], lane >> 2);
       scale2[j] = pair_of(rs4[j], rs4[j]);
       less4[j] = 0;
       m4[j] = -CUDART_INF_F;
