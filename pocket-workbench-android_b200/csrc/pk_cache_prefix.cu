@@ -397,6 +397,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
               }
             }
             bool moved = false;
+            uint64_t now4[4];
 #pragma unroll
             for (int j = 0; j < 4; j++) {
               f[j] = 1.0f;
@@ -409,8 +410,9 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
                 m4[j] = now;
                 moved |= f[j] != 1.0f;
               }
-              const float less = m4[j] == -CUDART_INF_F ? 0.0f : -m4[j];  // (nothing seen yet: all are masked)
-              less4[j] = pair_of(less, less);
+              // (nothing seen yet: all are masked; the next tile's weights will be infinite)
+              less4[j] = pair_of(-m4[j], -m4[j]);
+              now4[j] = m4[j] == -CUDART_INF_F ? 0 : less4[j];
             }
             if (i > 0 && __any_sync(0xffffffffu, moved)) {  // O's rows, once the products before are done
               pv_wait(i - 1);
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
                 st_quads(tmem + lanes + L::O_COL + 16 * c, v);
               }
             }
-            all_weights(less4, true);
+            all_weights(now4, true);
           }
 #pragma unroll
           for (int j = 0; j < 4; j++) {

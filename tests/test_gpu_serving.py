@@ -306,6 +306,24 @@ def test_shared_many_rows(pk, kind, dh, ty):
     assert (other[same].double() - got[same].double()).abs().max() <= 4 * torch.finfo(DT[ty]).eps * got.double().abs().max()
 
 
+@pytest.mark.parametrize("kind,dh,ty", [("q8", 128, "bf16"), ("q8", 64, "f16"), ("q4", 128, "f16"), ("q4", 64, "bf16")])
+def test_shared_whole_tiles_missing(pk, kind, dh, ty):
+    """Pages that are none over whole runs of 128 positions, a chunk's first among them: what follows still counts."""
+    gone = tuple(range(4)) + tuple(range(16, 20)) + tuple(range(36, 48))
+    su = SharedSetup(pk, [(2000, 40), (300, 25)], [(5 * i) % 30 for i in range(65)], [2] * 40 + [4] * 25, kind, 2, dh, 32, seed=12)
+    table = su.shared_seqs.pages
+    holes = {s: gone if s < 40 else (0, 1, 2, 3) for s in range(65)}
+    for g in range(2):
+        table[int(su.first[g]), list(holes[int(su.first[g])])] = -1
+    q = randn((su.n_tok, 8, dh), 4, DT[ty], std=1.5)
+
+    def missing(s):
+        p = torch.arange(su.lens[s] + su.new[s], device="cuda")
+        return ((p[:, None] // 32) == torch.tensor(holes[s], device="cuda")[None]).any(1) & (p < (2000 if s < 40 else 288))
+
+    check_attention(su, q, su.attend(q), holes=missing)
+
+
 @pytest.mark.parametrize("ty", list(DT))
 def test_shared_nothing_of_ones_own(pk, ty):
     """max_own 0: every row sees its group's prefix alone, and of a sequence in no group nothing."""
