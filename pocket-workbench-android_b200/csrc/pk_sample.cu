@@ -30,7 +30,7 @@
 //
 // Measured: 250 f32 rows of 128256: the largest alone 51 us, temperature alone
 // 97, top-k 40 93, top-p 0.6 at temperature 1.5 230, rows with rules of their own
-// 160 (the rows' bytes take 20); 64 bf16 rows of 73448, top-p 0.9: 40; one f32
+// 149 (the rows' bytes take 20); 64 bf16 rows of 73448, top-p 0.9: 41; one f32
 // row of 73448, all rules: 10.  What bounds it: instructions (64 M for the 250
 // rows with rules, 1.8 a cycle and SM; 33 an element for an exact weight) and the
 // steps that a cluster takes one after another, during which two CTAs an SM leave
@@ -988,10 +988,10 @@ cudaError_t launch_sample(const void *logits, int type, int rows, int n, long st
   a.q = std::min(50, 62 - bits);
   // CTAs a row: by what they hold, two an SM, one where rows are longer; more
   // where the rows leave SMs without any.  (250 f32 rows of 128256, each with its
-  // own rules: 6 CTAs 170 us, 4 193, and read again from L2 for every pass, 2 213
-  // and one 312, which waits for the longest row; 64 bf16 rows of 73448: 4 CTAs
-  // 56, 2 60, 6 77.)
-  const long long vecs = ((long long)n + 2 * v - 2) / v, most = 96 * 1024 / 16, wide = 208 * 1024 / 16;
+  // own rules: 5 CTAs 149 us, 6 156, 4 (one an SM) 189, and read again from L2 for
+  // every pass, 2 195 and one 288, which waits for the longest row; 64 bf16 rows of
+  // 73448: 4 CTAs 41, 2 55, 6 60.)
+  const long long vecs = ((long long)n + 2 * v - 2) / v, most = (113 * 1024 - (int)sizeof(Smem)) / 16, wide = 208 * 1024 / 16;
   long long c = std::min(8LL, (vecs + most - 1) / most);
   while (c < 8 && rows * c * 2 <= 296 && vecs >= 512 * c) c *= 2;
   c = std::min(c, 8LL);
