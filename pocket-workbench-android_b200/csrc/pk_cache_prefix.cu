@@ -19,12 +19,17 @@
 // products.  Waits are bounded as there.
 //
 // Measured: two prefixes of 24000 positions under 800 tokens each, 64 heads over 8
-// of 128, bf16, Q8: 1.55 ms, 812 TFLOP/s (the kernel of 128 rows: 1.72 ms).  What
-// bounds it: a block's tile takes its softmax warps 3,300 cycles and its products
-// 1,040, the two blocks' products 2,080 of every 4,600; shared memory is three
-// quarters busy between the products' operands, the codes made f16 and the
-// scales.  Twice the softmax warps, two for the same rows, took 1.80 ms (their
-// registers did not hold a tile's weights).
+// of 128, bf16, Q8: 1.39 ms, 905 TFLOP/s (the kernel of 128 rows: 1.72 ms).  What
+// bounds it: a block's tile takes its softmax warps 2,600 cycles beside the other
+// block's (exponentials of both alone are 2,050) and then 1,040 of products and 700
+// on the way there and back, 4,300 in all, of which the two blocks' products fill
+// 2,080.  Twice the softmax warps, two for the same rows: 2.01 ms for the call, then
+// 1.76 (their registers did not hold a tile's weights).  The thread that issues the
+// products has few registers: with its loops unrolled they were spilled, 1.55 ms.
+// One chunk of four tiles takes 43,000 cycles: 13,000 until the queries are there,
+// 8,000 for the first tile, 13,000 the others, 8,000 to write the rows.  Slower: one
+// arrival a warp for one a thread, a first reference from 32 positions, rows by
+// bulk copies (each 3% and more of the call).
 #include <algorithm>
 #include <atomic>
 
