@@ -28,8 +28,8 @@
 // A row is read once, into the shared memory of a cluster of up to 8 CTAs, and
 // gone over there; rows that do not fit are read again each time.
 //
-// Measured: 250 f32 rows of 128256: the largest alone 51 us, temperature alone
-// 97, top-k 40 93, top-p 0.6 at temperature 1.5 230, rows with rules of their own
+// Measured: 250 f32 rows of 128256: the largest alone 45 us, temperature alone
+// 90, top-k 40 86, top-p 0.6 at temperature 1.5 208, rows with rules of their own
 // 149 (the rows' bytes take 20); 64 bf16 rows of 73448, top-p 0.9: 41; one f32
 // row of 73448, all rules: 10.  What bounds it: instructions (64 M for the 250
 // rows with rules, 1.8 a cycle and SM; 33 an element for an exact weight) and the
