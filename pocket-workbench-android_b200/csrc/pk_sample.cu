@@ -458,9 +458,11 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
   // ---- 2, 3: the cut of top-k, then of top-p
   bool do_k = RULES && top_k > 0 && top_k < a.n, do_p = RULES && top_p < 1.0f;
   // bins of 1/32 nat for top-k: to the nearest, by an addition in which the
-  // sum's last bits are the number (what the constant loses shifts all alike)
+  // sum's last bits are the number (what the constant loses shifts all alike).
+  // The largest is in bin 0: below 4e6 a product is rounded by 1/8 at the most, so
+  // that its floor is no more than 1/8 above the product itself, and bin 0 ends at 1/2.
   const float per_unit = fmaxf(fminf(32.0f / temp, 1e30f), 1e-38f);
-  const float bias = fminf(fmaxf(rintf(r.top * per_unit), -4e6f), 4e6f);
+  const float bias = fminf(fmaxf(floorf(r.top * per_unit), -4e6f), 4e6f);
   const bool near = fabsf(r.top * per_unit) < 4e6f;
   auto bin_k = [&](float x) {
     const float d = near ? fmaf(x, -per_unit, bias) : x == r.top ? 0.0f : (r.top - x) * per_unit;
@@ -603,7 +605,8 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
       }
       while (to - from > 1) {
         const uint32_t step = (to - from + 31) / 32, at = from + min((uint32_t)(lane + 1) * step, to - from);
-        const uint32_t lanes = __ballot_sync(0xffffffffu, in(at));  // (`to` is among them)
+        const uint32_t lanes = __ballot_sync(0xffffffffu, in(at));  // (`to` is among them: the largest is in bin 0)
+        if (!lanes) break;
         const int f = __ffs(lanes) - 1;
         const uint32_t next = __shfl_sync(0xffffffffu, at, f);
         from = f > 0 ? __shfl_sync(0xffffffffu, at, max(f - 1, 0)) : from;
