@@ -470,14 +470,20 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
   };
   // for top-p by the f32 weight's exponent and five bits: bin 0 is 1; the last
   // one's, below 2^-31, are not counted
-  const float slope = (float)r.scale;
+  // y = (x - top) scale, with both times `pre`: 1 but where differences may overflow
+  // (temperatures past 2^60) or count as subnormals (below 4e-39, of logits below
+  // 2^-40; larger ones are 2^-64 apart, which any such slope makes nothing of).  So
+  // the slope is finite, and the largest has y = 0 (of infinities NaN, counted as 0).
+  const float pre = r.scale < 0x1p-60 ? 0.5f : r.scale > (double)MAXF && fabsf(r.top) < 0x1p-40f ? 0x1p100f : 1.0f;
+  const float less = -r.top * pre, slope = inf ? 1.0f : (float)fmin(r.scale / (double)pre, (double)MAXF);
   auto weight_p = [&](float x) {
-    float y = (x - r.top) * slope, w;
-    if (inf) y = x == r.top ? 0.0f : -200.0f;
+    const float y = fminf(fmaf(x, pre, less) * slope, 0.0f);
+    float w;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(w) : "f"(y));
     return __float_as_uint(w);
   };
-  auto bin_p = [&](uint32_t w) { return min((127 << 5) - (int)(w >> 18), BINS - 1); };
+  // (unsigned: what would be before bin 0 goes to the last one, so that no bin is out of range)
+  auto bin_p = [&](uint32_t w) { return (int)min((127u << 5) - (w >> 18), (uint32_t)(BINS - 1)); };
   float before_x = CUDART_NAN_F;  // logits from here on are before those in question
   u64 sum = 0;                    // their weights and number
   uint32_t n = 0;
@@ -598,7 +604,7 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
         from = to = b < 0 ? 0 : key_of(-MAXF);
       } else {
         const double g = do_k ? ((double)bias - b - 0.5) / (double)per_unit
-                              : (double)r.top + (double)log2f(__uint_as_float((uint32_t)((127 << 5) - b) << 18)) / (double)slope;
+                              : (double)r.top + (double)log2f(__uint_as_float((uint32_t)((127 << 5) - b) << 18)) / r.scale;
         const uint32_t at = min(max(key_of((float)g), least + 17), to - min(to - least - 17, 16u));
         const bool here = lane == 0 ? !in(at - 16) : lane == 1 ? in(at + 16) : true;
         if (to - least > 64 && __all_sync(0xffffffffu, here)) from = at - 16, to = at + 16;

@@ -1,4 +1,5 @@
-"""The serving operators where settings and sizes are at their ends: equal logits at temperatures that are no power of two."""
+"""The serving operators where settings and sizes are at their ends: equal logits at temperatures that are no power of two,
+temperatures of every size."""
 import math
 
 import numpy as np
@@ -8,7 +9,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from test_gpu_drafts import DT, gen, i32  # noqa: E402
-from test_gpu_serving import check_draw  # noqa: E402
+from test_gpu_serving import check_draw, likely  # noqa: E402
 
 
 def halves():
@@ -42,3 +43,33 @@ def test_draw_equal_logits_at_temperatures(pk, ty):
             for k in (17, 250, n // 2, n - 3):
                 for p in (1.0, 0.6):
                     check_draw(pk, x, u, temp=temp, top_k=i32([k] * rows), top_p=torch.full((rows,), p, device="cuda"))
+
+
+@pytest.mark.parametrize("ty", list(DT))
+@pytest.mark.parametrize("n", [3, 50, 3001, 40000])
+def test_draw_top_p_at_all_temperatures(pk, ty, n):
+    """Temperatures that are subnormal, infinite, or so large that differences of logits overflow, beside top_p."""
+    top = float(torch.finfo(DT[ty]).max)
+    x = torch.empty((7, n), device="cuda")
+    x[:4] = likely(4, n, 5, "f32") if n > 20 else torch.tensor([1.0, 0.5, 2.0], device="cuda")
+    x[1, ::2] = -math.inf
+    x[2, n // 2] = math.inf
+    x[4] = torch.where(torch.arange(n, device="cuda") % 3 == 1, top, -top)
+    x[5] = top * torch.linspace(-1, 1, n, device="cuda")
+    x[6] = -1e-40 * (torch.arange(n, device="cuda") % 50)  # (0 in half precision)
+    x = x.to(DT[ty])
+    u = torch.rand(7, generator=gen(n), device="cuda")
+    full = lambda v: torch.full((7,), v, device="cuda")  # noqa: E731
+    for t in (1e-45, 1e-40, 4e-39, 4.3e-39, 1e-30, 1e-20, 1e20, 1e38, 3e38, math.inf):
+        for p in (0.0, 1e-6, 0.37, 0.9, 0.9999999):
+            check_draw(pk, x, u, temp=full(t), top_p=full(p))
+        check_draw(pk, x, u, temp=full(t), top_p=full(0.6), top_k=i32([0, 5, 600, n - 1, 2, 0, 7]), min_p=full(1e-3))
+
+
+def test_draw_top_p_at_all_temperatures_of_long_rows(pk):
+    """The same where a row does not fit its CTAs' shared memory."""
+    x = likely(3, 700001, 5, "f32")
+    x[1] = 3e38 * torch.linspace(-1, 1, 700001, device="cuda")
+    u = torch.rand(3, generator=gen(2), device="cuda")
+    for t in (1e-45, 4e-39, 1.0, 3e38, math.inf):
+        check_draw(pk, x, u, temp=torch.full((3,), t, device="cuda"), top_p=torch.full((3,), 0.37, device="cuda"))
