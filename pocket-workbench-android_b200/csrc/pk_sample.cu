@@ -253,7 +253,7 @@ struct Row {
   __device__ __forceinline__ double weight_as(float x) const {
     double v;
     if (EX) {
-      v = x == top ? 0.0 : x >= low ? ((double)x - (double)top) * scale : -100.0;
+      v = x == top ? 0.0 : x >= low ? fmax(((double)x - (double)top) * scale, -100.0) : -100.0;
     } else {  // x in double without the conversion, of which an SM makes 16 a cycle; 0 and subnormals become up to 2^-126
       const int u = __float_as_int(x);
       v = __hiloint2double(((u >> 3) & 0x8fffffff) + (896 << 20), u << 29);
@@ -451,7 +451,9 @@ __global__ void __launch_bounds__(ST, 2) k_sample(const SampleK a) {
   r.step = TABLE * r.scale;
   r.zero = 6755399441055744.0;
   r.none = r.low;
-  r.exact = inf || temp < 0x1p-80f || !(fabs((double)r.top * r.step) < 0x1p50) || !(r.low > -MAXF);
+  // (and where `low`, the float below what has a weight, is so far below it that its
+  // steps leave the exponents there are: 2^-100 rounds to 0, 2^-900 is still a number)
+  r.exact = inf || temp < 0x1p-80f || !(fabs((double)r.top * r.step) < 0x1p50) || !(r.low > -MAXF) || !(((double)r.top - (double)r.low) * r.scale < 900.0);
   if (r.exact) r.step = TABLE, r.none = -CUDART_INF_F;
   else r.zero -= rint((double)r.top * r.step);
 

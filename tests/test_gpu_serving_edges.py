@@ -73,3 +73,23 @@ def test_draw_top_p_at_all_temperatures_of_long_rows(pk):
     u = torch.rand(3, generator=gen(2), device="cuda")
     for t in (1e-45, 4e-39, 1.0, 3e38, math.inf):
         check_draw(pk, x, u, temp=torch.full((3,), t, device="cuda"), top_p=torch.full((3,), 0.37, device="cuda"))
+
+
+@pytest.mark.parametrize("ty", list(DT))
+@pytest.mark.parametrize("n", [20, 3001, 40000])
+def test_draw_small_temperatures(pk, ty, n):
+    """Temperatures at which the next float below the largest logit has a weight of 2^-100 to 2^-(10^9): the largest alone
+    counts, or all that are equal to it, and the others have none."""
+    x = torch.empty((5, n), device="cuda")
+    x[:4] = likely(4, n, 5, "f32")
+    x[1] = 12.0 + x[1].abs().clamp(max=3.0)
+    x[2, n // 3] = 60.0
+    x[3, ::4] = 21.5
+    x[4] = 9.75
+    x = x.to(DT[ty])
+    x[4, ::2] = torch.nextafter(x[4, :1].float(), torch.zeros((), device="cuda")).to(DT[ty]) if ty == "f32" else x[4, 0] - x[4, 0] * torch.finfo(DT[ty]).eps
+    u = torch.rand(5, generator=gen(n), device="cuda")
+    full = lambda v: torch.full((5,), v, device="cuda")  # noqa: E731
+    for t in (1e-6, 1e-7, 3e-8, 1e-8, 3e-9, 2.5e-9, 2e-9, 1.5e-9, 1e-9, 7e-10, 5e-10, 3e-10, 1e-10, 1e-11, 1e-12, 1e-14, 2.4e-17, 1e-18):
+        for kw in ({}, {"top_p": full(0.9)}, {"top_k": i32([15] * 5)}, {"min_p": full(1e-3), "top_p": full(0.4)}):
+            check_draw(pk, x, u, temp=full(t), **kw)
