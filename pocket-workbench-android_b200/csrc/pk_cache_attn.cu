@@ -940,7 +940,8 @@ cudaError_t launch_kv_attn_shared(const pk_kv_cache &c, const pk_kv_seqs &seqs, 
   if (rows > 0x7fffffff) return cudaErrorInvalidValue;
   AttnKArgs a = args_of(c, s, q);
   a.sh = sh;
-  if (x.pre_p.n_chunk == 0) a.sh.n_group = 0;
+  // (The groups stay also where nothing is computed for all of one: what a sequence
+  // has besides is counted from its group's shared length, 15 at the most then.)
   a.n_pre = x.pre_p.n_chunk;
   a.pre_chunk = std::max(x.pre_p.chunk, 1);
   a.n_part = a.n_pre + (x.merge ? 0 : x.own_p.n_chunk);

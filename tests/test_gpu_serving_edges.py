@@ -1,5 +1,5 @@
 """The serving operators where settings and sizes are at their ends: equal logits at temperatures that are no power of two,
-temperatures of every size."""
+temperatures of every size, shared prefixes shorter than a tile."""
 import math
 
 import numpy as np
@@ -8,8 +8,8 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_drafts import DT, gen, i32  # noqa: E402
-from test_gpu_serving import check_draw, likely  # noqa: E402
+from test_gpu_drafts import DT, check_attention, gen, i32, randn  # noqa: E402
+from test_gpu_serving import SharedSetup, check_draw, likely  # noqa: E402
 
 
 def halves():
@@ -93,3 +93,40 @@ def test_draw_small_temperatures(pk, ty, n):
     for t in (1e-6, 1e-7, 3e-8, 1e-8, 3e-9, 2.5e-9, 2e-9, 1.5e-9, 1e-9, 7e-10, 5e-10, 3e-10, 1e-10, 1e-11, 1e-12, 1e-14, 2.4e-17, 1e-18):
         for kw in ({}, {"top_p": full(0.9)}, {"top_k": i32([15] * 5)}, {"min_p": full(1e-3), "top_p": full(0.4)}):
             check_draw(pk, x, u, temp=full(t), **kw)
+
+
+SHORT = [
+    # (groups of (positions shared, sequences), own positions, new tokens): the longest prefix is under a tile
+    ([(1, 3)], [0, 40, 7], [1, 1, 1]),
+    ([(8, 2), (0, 1)], [60, 0, 20], [1, 3, 1]),
+    ([(15, 4), (3, 2)], [3, 0, 90, 700, 5, 0], [2, 1, 1, 1, 4, 2]),
+    ([(15, 30)], [(11 * i) % 70 for i in range(30)], [3] * 30),
+]
+
+
+@pytest.mark.parametrize("kind, dh", [("q8", 64), ("q8", 128), ("q4", 64), ("q4", 128)])
+@pytest.mark.parametrize("ty", list(DT))
+@pytest.mark.parametrize("case", range(len(SHORT)))
+def test_shared_short_prefixes(pk, kind, dh, ty, case):
+    """max_own is of the positions besides the shared ones also where those are too few to be computed for all."""
+    su = SharedSetup(pk, *SHORT[case], kind, 2, dh, 16, seed=case)
+    assert su.shared.max_len == max(n for n, _ in SHORT[case][0]) < 16
+    for heads in (2, 16):
+        q = randn((su.n_tok, heads, dh), 8, DT[ty], std=1.5)
+        check_attention(su, q, su.attend(q))
+
+
+@pytest.mark.parametrize("ty", list(DT))
+def test_shared_bounds_under_a_tile(pk, ty):
+    """The same where the sequences' own bound, or max_len alone, is under a tile; and no tokens of a group at all."""
+    su = SharedSetup(pk, [(8, 3)], [2, 0, 4], [1, 3, 2], "q8", 2, 64, 16, seed=1)
+    assert su.max_len < 16
+    q = randn((su.n_tok, 4, 64), 8, DT[ty])
+    check_attention(su, q, su.attend(q))
+    su = SharedSetup(pk, [(15, 3), (12, 2)], [20, 0, 37, 50, 1], [1, 3, 2, 1, 1], "q8", 2, 64, 16, seed=2)
+    q = randn((su.n_tok, 4, 64), 8, DT[ty])
+    for max_len in (15, 17):
+        check_attention(su, q, su.cache.attend(su.seqs, q, shared=pk.KvShared(su.shared.first, su.shared.len, su.shared.max_tok, max_len, 51)))
+    # (cut to 9, six positions more of a sequence are besides them; max_tok 0: all of a sequence are)
+    check_attention(su, q, su.cache.attend(su.seqs, q, shared=pk.KvShared(su.shared.first, su.shared.len, su.shared.max_tok, 9, 51 + 6)))
+    check_attention(su, q, su.cache.attend(su.seqs, q, shared=pk.KvShared(su.shared.first, su.shared.len, 0, 9, 15 + 51 + 6)))
