@@ -472,20 +472,23 @@ struct Geo {
   static constexpr int SMEM = RING + RG * W::QBYTES > END ? RING + RG * W::QBYTES : END;
 };
 
-template <int TYPE, int DH, int NT, int NB, int RG>
+// SHARED: calls over shared prefixes, a form of its own, as the registers that
+// joining takes cost others CTAs (104 and 176 a thread for 96 and 140 with 8 f32 rows
+// of 64 and of 128 dimensions).
+template <int TYPE, int DH, int NT, int NB, int RG, bool SHARED>
 __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
   using G = Geo<TYPE, DH, NT, NB, RG>;
   using T = typename G::T;
   extern __shared__ __align__(128) uint8_t smem[];
   // (the launch after the prefixes' does not wait before it reads what they read,
   // so theirs lets it begin only when all before them is done)
-  if (a.mode == ATTN_PREFIX) pdl_wait();
+  if (SHARED && a.mode == ATTN_PREFIX) pdl_wait();
   pdl_trigger();
-  if (a.mode != ATTN_PREFIX && !a.early) pdl_wait();
-  const Unit u = unit_of(a);
+  if (!SHARED || (a.mode != ATTN_PREFIX && !a.early)) pdl_wait();
+  const Unit u = unit_of<SHARED>(a);
   const int tile0 = u.rt * G::ROWS;
-  if (idle(a, u, tile0)) {
-    end_early(a);
+  if (idle<SHARED>(a, u, tile0)) {
+    if (SHARED) end_early(a);
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -563,7 +566,7 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
     }
   __syncthreads();
   const bool cluster = a.cluster && u.nch > 1;
-  if (a.merge && a.early) pdl_wait();
+  if (SHARED && a.merge && a.early) pdl_wait();
   for (int x = threadIdx.x; x < G::ROWS * 8; x += 32 * AW) {
     const int r = x >> 3, d0 = (x & 7) * (DH / 8);
     if (tile0 + r >= u.rows) continue;
@@ -591,7 +594,7 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
         const int i = (tile0 + r) / a.group, h = u.h * a.group + (tile0 + r) - i * a.group;
         a.part_ml[((long long)(u.sv.first + i) * a.q.n_head + h) * a.n_part + u.slot] = make_float2(M, L);
       }
-    } else if (a.merge) {
+    } else if (SHARED && a.merge) {
       merge_in<DH / 8>(merge_of<DH>(a, u, tile0 + r, M, L), DH, d0, acc);
     } else {
       const float inv = L > 0.0f || isnan(L) ? 1.0f / L : 0.0f;
@@ -600,7 +603,7 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
     }
     write_row<DH>(a, u, tile0 + r, d0, acc, u.part);
   }
-  if (!a.merge) end_early(a);
+  if (SHARED && !a.merge) end_early(a);
   if (cluster) join_cluster<DH>(a, u, tile0, G::ROWS, shaddr(so), shaddr(sfin), 32 * AW);
 }
 
@@ -697,13 +700,13 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) k_kv_attn_join(const At
 // steps of 8 up to 32 a warp (16 where f32's two terms double the query
 // fragments of 128 dimensions), then two or four warps side by side.
 struct Variant {
-  void (*k)(AttnKArgs) = nullptr;
+  void (*k)(AttnKArgs) = nullptr, (*shared)(AttnKArgs) = nullptr;
   int smem = 0, rows = 0;
 };
 template <int TYPE, int DH, int NT, int NB, int RG>
 Variant variant_as() {
   using G = Geo<TYPE, DH, NT, NB, RG>;
-  return {k_kv_attn<TYPE, DH, NT, NB, RG>, G::SMEM, G::ROWS};
+  return {k_kv_attn<TYPE, DH, NT, NB, RG, false>, k_kv_attn<TYPE, DH, NT, NB, RG, true>, G::SMEM, G::ROWS};
 }
 // From TC_FROM rows on half-precision queries take the tcgen05 kernel, whose
 // time hardly depends on the rows up to 128 (40 sequences of 7500 and 15000
@@ -718,10 +721,10 @@ Variant variant_rows(long long rows) {
   if (rows <= 16) return variant_as<TYPE, DH, NT, 2, 1>();
   if constexpr (NT == 1) {
     static_assert(TC_FROM == 17, "half-precision rows past 16");
-    return {nullptr, 0, 128};
+    return {nullptr, nullptr, 0, 128};
   } else if constexpr (DH == 64) {
     static_assert(TC32_FROM == 33, "f32 rows past 32");
-    return rows <= 32 ? variant_as<TYPE, DH, NT, 4, 1>() : Variant{nullptr, 0, rows <= 128 ? 128 : 256};
+    return rows <= 32 ? variant_as<TYPE, DH, NT, 4, 1>() : Variant{nullptr, nullptr, 0, rows <= 128 ? 128 : 256};
   } else {
     return rows <= 32 ? variant_as<TYPE, DH, NT, 2, 2>() : variant_as<TYPE, DH, NT, 2, 4>();
   }
@@ -839,7 +842,7 @@ static cudaError_t launch_parts(AttnKArgs &a, const Variant &v, const Split &p, 
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   const int cluster = a.cluster ? p.n_chunk : 1;
   if (!v.k) return launch_kv_attn_tc(a, v.rows, cluster, (unsigned)blocks, st);
-  return launch_cluster(v.k, cluster, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
+  return launch_cluster(a.mode == ATTN_ALL ? v.k : v.shared, cluster, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
 }
 static cudaError_t launch_join(const AttnKArgs &a, cudaStream_t st) {
   const size_t rows = (size_t)a.s.n_tok * a.q.n_head;

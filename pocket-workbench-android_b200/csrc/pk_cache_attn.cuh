@@ -111,6 +111,8 @@ struct Unit {
   int s, h, rt, ch, lo, hi, nch, rows, slot;  // (slot: of its part among a row's)
   bool part;
 };
+// SHARED: a launch may be a prefix's or what is besides one (a.mode).
+template <bool SHARED = true>
 __device__ __forceinline__ Unit unit_of(const AttnKArgs &a) {
   Unit u;
   unsigned id = blockIdx.x;
@@ -122,13 +124,13 @@ __device__ __forceinline__ Unit unit_of(const AttnKArgs &a) {
   u.h = (int)(id % (unsigned)a.c.n_kv);
   u.s = (int)(id / (unsigned)a.c.n_kv);
   int base = 0;
-  if (a.mode == ATTN_PREFIX) {
+  if (SHARED && a.mode == ATTN_PREFIX) {
     const GroupView g = group_view(a, u.s);
     u.s = g.s0;  // (whose pages are read)
     u.sv = SeqView{g.t0, g.n, g.base, g.base};
   } else {
     u.sv = seq_view(a.s, a.c.page_size, u.s);
-    if (a.mode == ATTN_OWN && u.sv.n > 0) {
+    if (SHARED && a.mode == ATTN_OWN && u.sv.n > 0) {
       const OwnView v = own_view(a, u.s, u.sv);
       base = v.base;
       u.sv.total = v.total;
@@ -138,14 +140,15 @@ __device__ __forceinline__ Unit unit_of(const AttnKArgs &a) {
   u.nch = (u.sv.total - base + a.chunk - 1) / a.chunk;
   u.lo = base + u.ch * a.chunk;
   u.hi = min(u.sv.total, u.lo + a.chunk);
-  u.slot = a.part0 + u.ch;
-  u.part = (a.mode != ATTN_ALL && !a.merge) || u.nch > 1;
+  u.slot = (SHARED ? a.part0 : 0) + u.ch;
+  u.part = (SHARED && a.mode != ATTN_ALL && !a.merge) || u.nch > 1;
   return u;
 }
 // Has this CTA nothing to do?  (Rows that see nothing are written by their first chunk, or by the joining launch.)
+template <bool SHARED = true>
 __device__ __forceinline__ bool idle(const AttnKArgs &a, const Unit &u, int tile0) {
   if (tile0 >= u.rows) return true;
-  return u.ch >= (a.mode == ATTN_ALL || a.merge ? max(u.nch, 1) : u.nch) && !(a.cluster && u.nch > 1);
+  return u.ch >= (!SHARED || a.mode == ATTN_ALL || a.merge ? max(u.nch, 1) : u.nch) && !(a.cluster && u.nch > 1);
 }
 // Beside the prefixes' launch: it is not over before one CTA (the last) has seen
 // that end, as what follows waits for this launch alone.
