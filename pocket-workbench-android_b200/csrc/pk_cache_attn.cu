@@ -480,8 +480,9 @@ __global__ void __launch_bounds__(32 * AW) k_kv_attn(const AttnKArgs a) {
   using G = Geo<TYPE, DH, NT, NB, RG>;
   using T = typename G::T;
   extern __shared__ __align__(128) uint8_t smem[];
-  // (the launch after the prefixes' does not wait before it reads what they read,
-  // so theirs lets it begin only when all before them is done)
+  // (a prefixes' launch has all work before it behind it as it begins, and so has the
+  // launch that it lets begin; its wait, for nothing, in one place with the others'
+  // takes a register more: 12 groups 74 us for 68)
   if (SHARED && a.mode == ATTN_PREFIX) pdl_wait();
   pdl_trigger();
   if (!SHARED || (a.mode != ATTN_PREFIX && !a.early)) pdl_wait();
@@ -842,7 +843,7 @@ static cudaError_t launch_parts(AttnKArgs &a, const Variant &v, const Split &p, 
   if (blocks > 0x7fffffffLL) return cudaErrorInvalidValue;
   const int cluster = a.cluster ? p.n_chunk : 1;
   if (!v.k) return launch_kv_attn_tc(a, v.rows, cluster, (unsigned)blocks, st);
-  return launch_cluster(a.mode == ATTN_ALL ? v.k : v.shared, cluster, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
+  return launch_as(a.mode != ATTN_PREFIX, a.mode == ATTN_ALL ? v.k : v.shared, cluster, dim3((unsigned)blocks), dim3(32 * AW), v.smem, st, a);
 }
 static cudaError_t launch_join(const AttnKArgs &a, cudaStream_t st) {
   const size_t rows = (size_t)a.s.n_tok * a.q.n_head;
@@ -871,7 +872,12 @@ cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &seqs, const p
 // Shared prefixes: the groups as sequences of their tokens over the positions
 // that they share, then each sequence over the rest of its own.  The second launch
 // begins beside the first one's last CTAs (it reads nothing that the first one
-// writes until it joins) and adds the prefix's parts to its rows itself where a
+// writes until it joins).  What it reads before it waits (lengths, tables, queries,
+// the cache) earlier work may have written: the first launch is therefore not
+// programmatic, so that in the stream's order all of that work is done and its
+// writes are in memory before the first launch begins, and the second begins after
+// it.  (Both programmatic takes as long: four answers to a prompt 10.9 us and 11.0,
+// 64 streams 47.4 and 46.7; a second launch that waits first: 15.6 and 50.4.)  It adds the prefix's parts to its rows itself where a
 // sequence's rest is one chunk; otherwise a third one joins all parts.  64 streams
 // behind 4001 positions: 48 us, 17 less than with three launches one after another;
 // every stream by itself over all its positions 101.

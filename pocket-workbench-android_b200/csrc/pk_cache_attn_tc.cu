@@ -812,7 +812,7 @@ cudaError_t launch_kv_attn_tc(const AttnKArgs &a, int rows, int cluster, unsigne
     if (f.numRegs != k.regs) return cudaErrorInvalidConfiguration;
     checked.fetch_or(bit, std::memory_order_relaxed);
   }
-  return launch_cluster(k.k, cluster, dim3(blocks), dim3(k.threads), k.smem, st, a);
+  return launch_as(a.mode != ATTN_PREFIX, k.k, cluster, dim3(blocks), dim3(k.threads), k.smem, st, a);
 }
 
 }  // namespace pk

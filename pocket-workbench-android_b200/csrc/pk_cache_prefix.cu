@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(PTHREADS, 1) k_kv_prefix(const AttnKArgs a) {
   constexpr bool F16 = std::is_same_v<E, __half>;
   constexpr int RB = TYPE == PK_KV_Q8 ? DH : DH / 2, SW = TYPE == PK_KV_Q8 ? 1 : 2;
   extern __shared__ __align__(1024) uint8_t smem[];
-  pdl_wait();
+  // (launched when all before it is done: nothing to wait for)
   const Unit u = unit_of(a);
   const int tile0 = u.rt * PROWS;
   if (idle(a, u, tile0)) {
@@ -532,7 +532,7 @@ cudaError_t launch_kv_prefix(const AttnKArgs &a, unsigned blocks, cudaStream_t s
     if (f.numRegs != PREGS) return cudaErrorInvalidConfiguration;
     checked.fetch_or(bit, std::memory_order_relaxed);
   }
-  return launch(k, dim3(blocks), dim3(PTHREADS), smem, st, a);
+  return launch_as(false, k, 1, dim3(blocks), dim3(PTHREADS), smem, st, a);
 }
 
 }  // namespace pk

@@ -1,4 +1,4 @@
-// pk_launch.h -- launches of the drafted-decoding kernels: programmatic (the
+// pk_launch.h -- launches of the drafted-decoding and serving kernels: programmatic (the
 // next kernel in the stream may be scheduled before this one ends; every one
 // waits for the one before it first), optionally in clusters.
 #pragma once
@@ -43,8 +43,11 @@ inline cudaError_t allow_smem(const void *f, int smem) {
   return cudaSuccess;
 }
 
+// programmatic false: this kernel begins when all work before it in the stream is
+// done and its writes are in memory (which those that follow programmatically then
+// rely on before they wait, too).
 template <class... KArgs, class... Args>
-cudaError_t launch_cluster(void (*kernel)(KArgs...), int cluster, dim3 grid, dim3 block, int smem, cudaStream_t st, Args... args) {
+cudaError_t launch_as(bool programmatic, void (*kernel)(KArgs...), int cluster, dim3 grid, dim3 block, int smem, cudaStream_t st, Args... args) {
   const cudaError_t e = allow_smem(reinterpret_cast<const void *>(kernel), smem);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg{};
@@ -53,14 +56,22 @@ cudaError_t launch_cluster(void (*kernel)(KArgs...), int cluster, dim3 grid, dim
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = st;
   cudaLaunchAttribute at[2] = {};
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = (unsigned)cluster;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  if (programmatic) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 1) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+    at[cfg.numAttrs].val.clusterDim.y = at[cfg.numAttrs].val.clusterDim.z = 1;
+    cfg.numAttrs++;
+  }
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+template <class... KArgs, class... Args>
+cudaError_t launch_cluster(void (*kernel)(KArgs...), int cluster, dim3 grid, dim3 block, int smem, cudaStream_t st, Args... args) {
+  return launch_as(true, kernel, cluster, grid, block, smem, st, args...);
 }
 template <class... KArgs, class... Args>
 cudaError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, int smem, cudaStream_t st, Args... args) {

@@ -130,3 +130,54 @@ def test_shared_bounds_under_a_tile(pk, ty):
     # (cut to 9, six positions more of a sequence are besides them; max_tok 0: all of a sequence are)
     check_attention(su, q, su.cache.attend(su.seqs, q, shared=pk.KvShared(su.shared.first, su.shared.len, su.shared.max_tok, 9, 51 + 6)))
     check_attention(su, q, su.cache.attend(su.seqs, q, shared=pk.KvShared(su.shared.first, su.shared.len, 0, 9, 15 + 51 + 6)))
+
+
+@pytest.mark.parametrize("ty, dh, heads", [("f16", 128, 16), ("bf16", 64, 40), ("f32", 64, 4), ("f32", 64, 40), ("f32", 128, 16)])
+def test_shared_reads_what_was_just_written(pk, ty, dh, heads):
+    """Queries, lengths, tables and the cache are written by the calls right before, which nobody waits for: the results are
+    those of calls that were waited for, bit by bit, also from a captured graph."""
+    su = SharedSetup(pk, [(700, 6), (90, 3)], [(37 * i) % 120 for i in range(9)], [2] * 9, "q8", 2, dh, 32, seed=4)
+    sq, c, n = su.shared_seqs, su.cache, su.n_tok
+    k, v = (randn((n, 2, dh), 40 + i, DT[ty]) for i in range(2))
+    qs = [randn((n, heads, dh), i, DT[ty]) for i in range(6)]
+    ctx = [sq.ctx - i for i in range(6)]  # (the first of a group keeps its prefix: own positions 0 .. only shrink)
+    for x in ctx:
+        x[[0, 6]] = sq.ctx[[0, 6]]
+    q = torch.empty_like(qs[0])
+    cells = [t.clone() for t in (c.k, c.v, c.ks, c.vs)]
+
+    def step(i):
+        for t, was in zip((c.k, c.v, c.ks, c.vs), cells):
+            t.copy_(was)
+        sq.ctx.copy_(ctx[i])
+        sq.pages.copy_(table)
+        c.store(sq, k * (1 + i), v * (1 + i))
+        q.copy_(qs[i])
+
+    table = sq.pages.clone()
+    want = []
+    for i in range(6):
+        step(i)
+        torch.cuda.synchronize()
+        want.append(su.attend(q))
+        torch.cuda.synchronize()
+    got = []
+    for i in range(30):
+        sq.pages.fill_(-1)
+        step(i % 6)
+        got.append(su.attend(q))
+        q.fill_(math.nan)
+    torch.cuda.synchronize()
+    assert all(torch.equal(got[i], want[i % 6]) for i in range(30))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = []
+        for i in range(6):
+            sq.pages.fill_(-1)
+            step(i)
+            out.append(su.attend(q))
+            q.fill_(math.nan)
+    for _ in range(5):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
