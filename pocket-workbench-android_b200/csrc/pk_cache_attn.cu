@@ -697,6 +697,39 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) k_kv_attn_join(const At
   }
 }
 
+// The tcgen05 kernel's time for so many CTAs of so many tiles of 64 positions, by
+// rounds.  A CTA costs 16 tiles more for its beginning and its part of the sums (one
+// CTA an SM, two blocks of 128 rows: 8).  Half precision, in proportions: where two
+// share an SM a tile takes 8 fifths of what it takes alone (64 tokens at 8000
+// positions, 64 heads over 8: 4 chunks, one CTA an SM, 53 us, 8 chunks 66, one 127,
+// 37 100; 32 sequences of 2000: one chunk 61, two 79, four 100; wide trees 770, 799
+// and 750, one and four of which this estimates within 1% of each other).  f32
+// (head_dim 64), in 100 ns: 1.4 us a tile in CTAs of two blocks, 1.5 in one of one
+// block that has an SM to itself, 1.8 in two.
+long long tc_time(int type, int rows, long long ctas, long long tiles) {
+  if (rows == 256) return (ctas + 147) / 148 * 14 * (tiles + 8);
+  const long long left = ctas % 296, one = type == T_F32 ? 15 : 5, two = type == T_F32 ? 18 : 8;
+  return (ctas / 296 * two + (left == 0 ? 0 : left <= 148 ? one : two)) * (tiles + 16);
+}
+// The chunks of the least time, up to `top` and from one on.  f32 CTAs of one block
+// in clusters of three to eight do not all run at once past 216 (a cluster is one
+// part of the chip's): a sequence of 8000, 36 heads: 6 chunks 61 us, 8 88; a cluster
+// as large where the parts go through the scratch is none.
+long long tc_chunks(int type, int rows, long long units, int max_len, long long top, bool parts, long long *time = nullptr) {
+  long long n = 1, best = 0;
+  for (long long c = 1; c <= top; c++) {
+    const long long ctas = units * c;
+    if (type == T_F32 && rows == 128 && !parts && c > 2 && c <= 8 && ctas > 216 && ctas <= 296) continue;
+    const long long t = tc_time(type, rows, ctas, ((max_len + 63LL) / 64 + c - 1) / c);
+    if (c == 1 || t < best) best = t, n = c;
+  }
+  if (time) *time = best;
+  return n;
+}
+constexpr long long WANT = 148 * 8;  // CTAs
+// Chunks there may be: WANT CTAs, none under MIN_CHUNK positions.
+long long most_chunks(long long units, int max_len) { return std::max(1LL, std::min((max_len + MIN_CHUNK - 1LL) / MIN_CHUNK, WANT / units)); }
+
 // The kernel's variant by the rows that a kv head's tile may have: columns in
 // steps of 8 up to 32 a warp (16 where f32's two terms double the query
 // fragments of 128 dimensions), then two or four warps side by side.
@@ -751,8 +784,21 @@ Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int ty
     const bool few = (long long)s.n_seq * c.n_kv * each <= 148, tc = rows >= (type != T_F32 ? TC_FROM : c.head_dim == 64 ? TC32_FROM : 1LL << 40);
     if (tc ? each * (tiles + 4) * 10 < (rows + 127) / 128 * (tiles + 16) * (few ? 36 : 18) : few && each * tiles <= 256) rows = 8;
   }
-  if (c.type == PK_KV_Q8) return c.head_dim == 64 ? variant_type<PK_KV_Q8, 64>(type, rows) : variant_type<PK_KV_Q8, 128>(type, rows);
-  return c.head_dim == 64 ? variant_type<PK_KV_Q4, 64>(type, rows) : variant_type<PK_KV_Q4, 128>(type, rows);
+  Variant v = c.type == PK_KV_Q8 ? c.head_dim == 64 ? variant_type<PK_KV_Q8, 64>(type, rows) : variant_type<PK_KV_Q8, 128>(type, rows)
+                                 : c.head_dim == 64 ? variant_type<PK_KV_Q4, 64>(type, rows) : variant_type<PK_KV_Q4, 128>(type, rows);
+  // f32 rows that one block holds: in CTAs of one block, two an SM, or in CTAs of two,
+  // one of them without rows, one an SM, which are done sooner where CTAs are few
+  // (36 heads; one block and two: 64 tokens of a sequence at 8000 61 and 60 us, 128
+  // at 4000 47 and 43, 3 sequences of 2000 with 33 49 and 57; 8 of them with 64 each
+  // 87 and 119, 4 of 16000 with 128 284 and 359).
+  if (!v.k && type == T_F32 && v.rows == 128 && !tiles_too) {
+    const long long units = (long long)s.n_seq * c.n_kv, top = most_chunks(units, s.max_len);
+    long long one = 0, two = 0;
+    tc_chunks(type, 128, units, s.max_len, top, false, &one);
+    tc_chunks(type, 256, units, s.max_len, top, false, &two);
+    if (two <= one) v.rows = 256;
+  }
+  return v;
 }
 
 // Chunks of a sequence's positions: so many that 148 SMs have about eight CTAs
@@ -762,13 +808,7 @@ Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int ty
 // launch, 13 us to 11 for one token at 1500 positions.  Elsewhere a cluster's
 // CTAs would hold their SMs until its longest is done (eight 16K streams 171 us
 // against 150), so their parts go through the scratch.  The tcgen05 kernel's chunks
-// are as many as take the least time by its rounds of CTAs: a CTA costs its
-// tiles of 64 positions and 16 more (one CTA an SM: 8) for its beginning and
-// its part of the sums, and where two share an SM a tile takes 8 fifths of what
-// it takes alone (64 tokens at 8000 positions, 64 heads over 8: 4 chunks, one
-// CTA an SM, 53 us, 8 chunks 66, one 127, 37 100; 32 sequences of 2000: one
-// chunk 61, two 79, four 100; the wide trees 770, 799 and 750, one and four of
-// which this estimates within 1% of each other).
+// are as many as take the least time by tc_time.
 struct Split {
   int chunk, n_chunk, row_tiles;
   bool cluster;
@@ -779,20 +819,10 @@ Split split_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int type, 
   Split p;
   const long long rows = (long long)s.max_new * (n_head / c.n_kv);
   p.row_tiles = (int)((rows + v.rows - 1) / v.rows);
-  const long long units = (long long)s.n_seq * c.n_kv * p.row_tiles, want = 148 * 8;
-  const long long most = (s.max_len + MIN_CHUNK - 1) / MIN_CHUNK;
+  const long long units = (long long)s.n_seq * c.n_kv * p.row_tiles;
   const long long sum = sum_most(type), least = v.k && type != T_F32 ? (s.max_len + 4 * sum - 1) / (4 * sum) : 1;
-  long long n = std::max(least, std::min(most, want / units));
-  if (!v.k) {
-    long long best = 0;
-    const long long top = n;
-    for (long long c = 1; c <= top; c++) {
-      const long long ctas = units * c, left = ctas % 296, tiles = ((s.max_len + 63) / 64 + c - 1) / c;
-      const long long t = v.rows == 256 ? (ctas + 147) / 148 * (tiles + 8)
-                                        : (ctas / 296 * 8 + (left == 0 ? 0 : left <= 148 ? 5 : 8)) * (tiles + 16);
-      if (c == 1 || t < best) best = t, n = c;
-    }
-  }
+  long long n = std::max(least, most_chunks(units, s.max_len));
+  if (!v.k) n = tc_chunks(type, v.rows, units, s.max_len, n, parts);
   const long long slots = v.rows == 256 ? 128 : 296;  // CTAs that run at once, in clusters too
   if (!parts && v.k && n > 8 && n <= 16 && least <= 8 && units * 8 <= slots) n = 8;
   p.chunk = (int)(((s.max_len + n - 1) / n + 63) / 64 * 64);

@@ -1,5 +1,6 @@
 """The serving operators where settings and sizes are at their ends: equal logits at temperatures that are no power of two,
-temperatures of every size, shared prefixes shorter than a tile."""
+temperatures of every size, shared prefixes shorter than a tile, calls right behind what they read; and the forms of the
+attention that f32 rows take by their number."""
 import math
 
 import numpy as np
@@ -8,7 +9,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_drafts import DT, check_attention, gen, i32, randn  # noqa: E402
+from test_gpu_drafts import DT, Setup, check_attention, gen, i32, randn  # noqa: E402
 from test_gpu_serving import SharedSetup, check_draw, likely  # noqa: E402
 
 
@@ -181,3 +182,23 @@ def test_shared_reads_what_was_just_written(pk, ty, dh, heads):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("kind", ["q8", "q4"])
+@pytest.mark.parametrize("lens, new, n_kv, heads", [
+    ([700, 0, 33], [64, 40, 1], 3, 3),            # few CTAs: of two blocks, one without rows, several chunks
+    ([900, 30, 0, 871, 512, 64], [33, 1, 40, 7, 33, 2], 36, 36),  # many: of one block, two an SM
+    ([6400, 5000, 10, 6000], [3, 1, 40, 16], 36, 36),             # of one block, chunks in clusters
+    ([3000] * 30, [5] * 30, 8, 64),               # eight query heads a kv head
+    ([20000], [100], 36, 36),                     # chunks through the scratch
+])
+def test_attention_of_33_to_128_f32_rows(pk, kind, lens, new, n_kv, heads):
+    """Every form that f32 rows of head_dim 64 take on the tensor cores, causal and with a mask of one's own token alone."""
+    su = Setup(pk, lens, new, kind, n_kv, 64, 64, seed=3)
+    su.fill(pk)
+    q = randn((su.n_tok, heads, 64), 8)
+    check_attention(su, q, su.cache.attend(su.seqs, q))
+    alone = torch.zeros((su.n_tok, 1), dtype=torch.int64, device="cuda")
+    for s, n in enumerate(new):
+        alone[int(su.start[s]):int(su.start[s]) + n, 0] = torch.ones((), dtype=torch.int64, device="cuda") << torch.arange(n, device="cuda")
+    check_attention(su, q, su.cache.attend(su.seqs, q, mask=alone), see=lambda s, n: torch.eye(n, dtype=torch.bool, device="cuda"))
