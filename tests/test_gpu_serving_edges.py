@@ -9,7 +9,7 @@ import pytest
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_drafts import DT, Setup, check_attention, gen, i32, randn  # noqa: E402
+from test_gpu_drafts import DT, Setup, check_attention, gen, i32, randn, words_of  # noqa: E402
 from test_gpu_serving import SharedSetup, check_draw, likely  # noqa: E402
 
 
@@ -198,7 +198,5 @@ def test_attention_of_33_to_128_f32_rows(pk, kind, lens, new, n_kv, heads):
     su.fill(pk)
     q = randn((su.n_tok, heads, 64), 8)
     check_attention(su, q, su.cache.attend(su.seqs, q))
-    alone = torch.zeros((su.n_tok, 1), dtype=torch.int64, device="cuda")
-    for s, n in enumerate(new):
-        alone[int(su.start[s]):int(su.start[s]) + n, 0] = torch.ones((), dtype=torch.int64, device="cuda") << torch.arange(n, device="cuda")
+    alone = words_of([1 << j for n in new for j in range(n)], 2)  # (token 64 of a sequence is in the second word)
     check_attention(su, q, su.cache.attend(su.seqs, q, mask=alone), see=lambda s, n: torch.eye(n, dtype=torch.bool, device="cuda"))
