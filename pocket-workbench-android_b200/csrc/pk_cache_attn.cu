@@ -740,7 +740,14 @@ struct Variant {
 template <int TYPE, int DH, int NT, int NB, int RG>
 Variant variant_as() {
   using G = Geo<TYPE, DH, NT, NB, RG>;
-  return {k_kv_attn<TYPE, DH, NT, NB, RG, false>, k_kv_attn<TYPE, DH, NT, NB, RG, true>, G::SMEM, G::ROWS};
+  // Eight half-precision rows of 64 Q8 codes: four CTAs an SM by their shared memory,
+  // where registers allow five and 148 SMs then have the eight that each gets in one
+  // round and part of another (36 heads: 8 streams of 16256 121 us with five, 109 with
+  // four, 16 of 16000 224 and 199, one of 4000 12.7 and 11.7; 4 kv heads: 8 of 4000
+  // 13.5 and 12.3, 16 of 16000 37.3 and 38.9).  In 4 bits five are no slower.
+  constexpr bool FOUR = TYPE == PK_KV_Q8 && DH == 64 && NT == 1 && NB == 1;
+  constexpr int SMEM = FOUR && G::SMEM < 48 * 1024 ? 48 * 1024 : G::SMEM;
+  return {k_kv_attn<TYPE, DH, NT, NB, RG, false>, k_kv_attn<TYPE, DH, NT, NB, RG, true>, SMEM, G::ROWS};
 }
 // From TC_FROM rows on half-precision queries take the tcgen05 kernel, whose
 // time hardly depends on the rows up to 128 (40 sequences of 7500 and 15000
