@@ -959,10 +959,15 @@ Shared shared_plan(const pk_kv_cache &c, const pk_kv_seqs &s, const pk_kv_shared
   if (x.own.max_len > 0) {
     x.own_v = variant_of(c, x.own, n_head, type, true);
     x.own_p = split_of(c, x.own, n_head, type, x.own_v, true);
-    // One chunk a sequence, which joins the prefix's parts itself, where its time
-    // is less than a joining launch's or there are CTAs enough.
+    // One chunk a sequence, which joins the prefix's parts itself, where there are CTAs
+    // enough for the length: 16 positions a CTA (behind 1000 positions, f16, 64 heads
+    // over 8 of 128, so and in three launches: 4 streams, 32 CTAs, 300 of their own 12.8
+    // and 13.6 us, 700 15.8 and 14.6, 1500 21.9 and 14.6; 16 streams, 128 CTAs, 1500
+    // 28.5 and 32.4, 2500 38.9 and 42.7, 4000 57.4 and 51.1; 30, 240 CTAs, 2500 51.3
+    // and 57.6, 4000 70.9 and 70.3; 4 of f32, 36 heads of 64, 144 CTAs, 1000 15.5 and
+    // 19.5, 2500 27.6 and 27.3, 4000 39.6 and 32.0).
     const long long units = (long long)s.n_seq * c.n_kv * x.own_p.row_tiles;
-    if (x.pre_p.n_chunk <= MERGE && (x.own.max_len <= 1536 || units >= 296) && (type == T_F32 || x.own.max_len <= sum_most(type))) {
+    if (x.pre_p.n_chunk <= MERGE && (x.own.max_len <= 16 * units || units >= 296) && (type == T_F32 || x.own.max_len <= sum_most(type))) {
       x.own_p.n_chunk = 1;
       x.own_p.chunk = (x.own.max_len + 63) / 64 * 64;
       x.merge = true;
