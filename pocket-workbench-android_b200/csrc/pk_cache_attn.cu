@@ -753,8 +753,8 @@ Variant variant_as() {
 // time hardly depends on the rows up to 128 (40 sequences of 7500 and 15000
 // positions, Q4: 16 rows 252 us here and 340 there, 8 rows 188 and 337; past 16
 // a row tile here takes twice as long), f32 ones of head_dim 64 from TC32_FROM
-// (8 sequences of 2000 positions, 36 heads: 32 rows 91 us here; 33 rows 138 and
-// 111; 128 rows 253 and 130).
+// (8 sequences of 2000 positions, 36 heads: 32 rows 91 us here, 33 rows 138 here and
+// 84 there, 128 rows 253 and 95; of 16000 positions 32 rows 367 here, 33 529 there).
 constexpr long long TC_FROM = 17, TC32_FROM = 33;
 template <int TYPE, int DH, int NT>
 Variant variant_rows(long long rows) {
@@ -913,8 +913,9 @@ cudaError_t launch_kv_attn(const pk_kv_cache &c, const pk_kv_seqs &seqs, const p
 // the cache) earlier work may have written: the first launch is therefore not
 // programmatic, so that in the stream's order all of that work is done and its
 // writes are in memory before the first launch begins, and the second begins after
-// it.  (Both programmatic takes as long: four answers to a prompt 10.9 us and 11.0,
-// 64 streams 47.4 and 46.7; a second launch that waits first: 15.6 and 50.4.)  It adds the prefix's parts to its rows itself where a
+// it.  (Both programmatic: as long in a graph, four answers to a prompt 10.9 us and
+// 11.0, 64 streams 47.4 and 46.7, and 1 to 2 us less called from a stream, 48.9 and
+// 49.7; a second launch that waits first: 15.6 and 50.4.)  It adds the prefix's parts to its rows itself where a
 // sequence's rest is one chunk; otherwise a third one joins all parts.  64 streams
 // behind 4001 positions: 48 us, 17 less than with three launches one after another;
 // every stream by itself over all its positions 101.

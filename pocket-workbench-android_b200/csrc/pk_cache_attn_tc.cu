@@ -20,7 +20,8 @@
 // beside the other's softmax.  f32 (head_dim 64): queries and weights are two
 // f16 terms each (2^-22), and a tile's O is added to the row's sums in
 // registers, because the tensor core's sums drop what they shift out; two
-// blocks share a CTA's codes, one CTA an SM.  Operands are in the canonical
+// blocks share a CTA's codes, one CTA an SM, or, up to 128 rows and where CTAs fill
+// the chip, one block a CTA, two an SM (pk_cache_attn.cu has the rule).  Operands are in the canonical
 // layout without swizzle, core matrices of 8 rows x 16 bytes (a product takes
 // 61 cycles so, 66 with 128-byte swizzle).  V's rows are stored as K's, which
 // makes it an N-major operand.
