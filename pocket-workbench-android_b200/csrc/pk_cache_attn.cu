@@ -698,29 +698,36 @@ __global__ void __launch_bounds__(W == 1 ? 128 : 32 * W) k_kv_attn_join(const At
 }
 
 // The tcgen05 kernel's time for so many CTAs of so many tiles of 64 positions, by
-// rounds.  A CTA costs 16 tiles more for its beginning and its part of the sums (one
-// CTA an SM, two blocks of 128 rows: 8).  Half precision, in proportions: where two
-// share an SM a tile takes 8 fifths of what it takes alone (64 tokens at 8000
-// positions, 64 heads over 8: 4 chunks, one CTA an SM, 53 us, 8 chunks 66, one 127,
-// 37 100; 32 sequences of 2000: one chunk 61, two 79, four 100; wide trees 770, 799
-// and 750, one and four of which this estimates within 1% of each other).  f32
-// (head_dim 64), in 100 ns: 1.4 us a tile in CTAs of two blocks, 1.5 in one of one
-// block that has an SM to itself, 1.8 in two.
+// rounds: a tile's time, and as many tiles more for a CTA's beginning and its part of
+// the sums.  Half precision, in proportions: 16 tiles more, and where two CTAs share
+// an SM a tile takes 8 fifths of what it takes alone (64 tokens at 8000 positions, 64
+// heads over 8: 4 chunks, one CTA an SM, 53 us, 8 chunks 66, one 127, 37 100; 32
+// sequences of 2000: one chunk 61, two 79, four 100; wide trees 770, 799 and 750, one
+// and four of which this estimates within 1% of each other).  f32 (head_dim 64), in
+// 100 ns: CTAs of two blocks, one an SM, 1.3 us and 11 tiles (36 heads, 64 tokens of a
+// sequence at 8000: one chunk 182 us, two 98, four 60); of one block, 1.5 and 14 where
+// it has the SM to itself (one chunk 216, two 119), 2.0 and 9 where two share it (8
+// sequences with 33 tokens, at 2000 82, at 16000 529; 40 of 200, 16 heads, 67).
 long long tc_time(int type, int rows, long long ctas, long long tiles) {
-  if (rows == 256) return (ctas + 147) / 148 * 14 * (tiles + 8);
-  const long long left = ctas % 296, one = type == T_F32 ? 15 : 5, two = type == T_F32 ? 18 : 8;
-  return (ctas / 296 * two + (left == 0 ? 0 : left <= 148 ? one : two)) * (tiles + 16);
+  if (rows == 256) return (ctas + 147) / 148 * 13 * (tiles + 11);
+  const long long rounds = ctas / 296, left = ctas % 296;
+  const bool one = left > 0 && left <= 148, two = left > 148;
+  if (type == T_F32) return (rounds + two) * 20 * (tiles + 9) + one * 15 * (tiles + 14);
+  return (rounds * 8 + (one ? 5 : two ? 8 : 0)) * (tiles + 16);
 }
-// The chunks of the least time, up to `top` and from one on.  f32 CTAs of one block
-// in clusters of three to eight do not all run at once past 216 (a cluster is one
-// part of the chip's): a sequence of 8000, 36 heads: 6 chunks 61 us, 8 88; a cluster
-// as large where the parts go through the scratch is none.
+// The chunks of the least time, up to `top` and from one on.  Not those of f32 in
+// clusters that do not all run at once: of CTAs of one block 148 SMs have room for 296
+// alone or in pairs, for 259 in clusters of seven; of two blocks for 130 and more, but
+// 105 in clusters of seven and 120 of eight (a sequence of 8000, 36 heads, 64 tokens:
+// 6 chunks 61 us, 8 88; of 3712, 16 heads, 43 tokens, two blocks: 8 48, 9 25).
 long long tc_chunks(int type, int rows, long long units, int max_len, long long top, bool parts, long long *time = nullptr) {
   long long n = 1, best = 0;
   for (long long c = 1; c <= top; c++) {
     const long long ctas = units * c;
-    if (type == T_F32 && rows == 128 && !parts && c > 2 && c <= 8 && ctas > 216 && ctas <= 296) continue;
-    const long long t = tc_time(type, rows, ctas, ((max_len + 63LL) / 64 + c - 1) / c);
+    const bool cluster = !parts && c > 1 && c <= 8 && ctas <= (rows == 256 ? 128 : 296);
+    if (type == T_F32 && cluster && c > 2 && ctas > (rows == 128 ? 256 : c < 7 ? 128 : 105)) continue;
+    long long t = tc_time(type, rows, ctas, ((max_len + 63LL) / 64 + c - 1) / c);
+    if (type == T_F32 && !parts && c > 1 && !cluster) t += 25;  // (a launch that joins)
     if (c == 1 || t < best) best = t, n = c;
   }
   if (time) *time = best;
@@ -796,14 +803,15 @@ Variant variant_of(const pk_kv_cache &c, const pk_kv_seqs &s, int n_head, int ty
   // f32 rows that one block holds: in CTAs of one block, two an SM, or in CTAs of two,
   // one of them without rows, one an SM, which are done sooner where CTAs are few
   // (36 heads; one block and two: 64 tokens of a sequence at 8000 61 and 60 us, 128
-  // at 4000 47 and 43, 3 sequences of 2000 with 33 49 and 57; 8 of them with 64 each
-  // 87 and 119, 4 of 16000 with 128 284 and 359).
+  // at 4000 47 and 43, 4 sequences of 1000 with 128 45 and 43; 3 of 2000 with 33 49 and
+  // 57, 8 of them with 64 87 and 119, 4 of 16000 with 128 284 and 359; 40 of 183 with
+  // 35, 16 heads, 67 and 96).  Estimates within a twentieth count as equal.
   if (!v.k && type == T_F32 && v.rows == 128 && !tiles_too) {
     const long long units = (long long)s.n_seq * c.n_kv, top = most_chunks(units, s.max_len);
     long long one = 0, two = 0;
     tc_chunks(type, 128, units, s.max_len, top, false, &one);
     tc_chunks(type, 256, units, s.max_len, top, false, &two);
-    if (two <= one) v.rows = 256;
+    if (two * 20 <= one * 21) v.rows = 256;
   }
   return v;
 }

@@ -671,8 +671,11 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
     }
     // The rows go by way of the operands' place (all blocks' products are done): a
     // cluster's are added up there, others leave it a whole row at a time (a row
-    // a lane, 32 rows' lines a store, took 8,000 cycles).
-    if (BLK > 1) asm volatile("bar.sync 1, %0;" ::"r"(SOFT) : "memory");
+    // a lane, 32 rows' lines a store, took 8,000 cycles).  Rows of which the first of
+    // two blocks has all leave the registers as they are: the calls that take that
+    // form are short (two sequences of 115 with 40 rows 15.2 us by shared memory, 14.3 so).
+    const bool direct = BLK == 2 && !JOINS && !cluster && u.rows <= 128;
+    if (BLK > 1 && !direct) asm volatile("bar.sync 1, %0;" ::"r"(SOFT) : "memory");
     if (work) {
       const int i = tok, h = u.h * a.group + (min(row, u.rows - 1) - i * a.group);
       const long long at = u.sv.first + i, slot = (at * a.q.n_head + h) * a.n_part + u.slot;
@@ -711,11 +714,12 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
           float x[8];
 #pragma unroll
           for (int j = 0; j < 8; j++) x[dim8<TYPE>(j)] = f == 0.0f ? 0.0f : v[8 * k + j] * f;
-          store_n<float, 8>(so + 16 * c + 8 * k, true, x);
+          if (!direct) store_n<float, 8>(so + 16 * c + 8 * k, true, x);
+          else if (on) store_n<float, 8>((part ? a.part_o + slot * DH : reinterpret_cast<float *>(a.q.out) + at * a.q.out_tok_stride + (long long)h * a.q.out_head_stride) + 16 * c + 8 * k, part || a.vec_o, x);
         }
       }
       __syncwarp();
-      if (!cluster) {
+      if (!direct && !cluster) {
         Merge mg{};
         if (JOINS) {
           if (a.early) pdl_wait();
@@ -724,7 +728,7 @@ __global__ void __launch_bounds__(Lay<DH, terms_of<E>, BLK>::THREADS, Lay<DH, te
         constexpr int LR = DH / 4, RP = 32 / LR;  // lanes a row, rows at a time
         const int sub = lane / LR, d0 = (lane % LR) * 4, rows = min(32, u.rows - tile0 - warp * 32);
         const long long off = part ? slot * DH : at * a.q.out_tok_stride + (long long)h * a.q.out_head_stride;
-#pragma unroll 1
+#pragma unroll (JOINS ? 1 : 4)
         for (int r0 = 0; r0 < rows; r0 += RP) {
           const int r = min(r0 + sub, 31);
           const long long to = __shfl_sync(0xffffffffu, off, r) + d0;

@@ -191,6 +191,8 @@ def test_shared_reads_what_was_just_written(pk, ty, dh, heads):
     ([6400, 5000, 10, 6000], [3, 1, 40, 16], 36, 36),             # of one block, chunks in clusters
     ([3000] * 30, [5] * 30, 8, 64),               # eight query heads a kv head
     ([20000], [100], 36, 36),                     # chunks through the scratch
+    ([8000], [64], 36, 36),                       # of two blocks, chunks through the scratch
+    ([150] * 20, [128] * 20, 8, 8),               # of one block without a row to spare, many of few tiles
 ])
 def test_attention_of_33_to_128_f32_rows(pk, kind, lens, new, n_kv, heads):
     """Every form that f32 rows of head_dim 64 take on the tensor cores, causal and with a mask of one's own token alone."""
