@@ -30,7 +30,7 @@
 //
 // Measured: 250 f32 rows of 128256: the largest alone 45 us, temperature alone
 // 90, top-k 40 88, top-p 0.6 at temperature 1.5 209, rows with rules of their own
-// 141 to 150 by the box (the rows' bytes take 20); 64 bf16 rows of 73448, top-p 0.9:
+// 141 to 156 by the rows (their bytes take 20); 64 bf16 rows of 73448, top-p 0.9:
 // 41; one f32 row of 73448, all rules: 10.  What bounds it: instructions (60 M for
 // the 250 rows with rules, 1.8 a cycle and SM; 33 an element for an exact weight)
 // and the steps that a cluster takes one after another, during which two CTAs an SM
