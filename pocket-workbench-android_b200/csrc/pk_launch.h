@@ -1,6 +1,7 @@
 // pk_launch.h -- launches of the drafted-decoding and serving kernels: programmatic (the
 // next kernel in the stream may be scheduled before this one ends; every one
-// waits for the one before it first), optionally in clusters.
+// waits for the one before it first, but the second over shared prefixes, see
+// pk_cache_attn.cu), optionally in clusters.
 #pragma once
 #include <cuda_runtime.h>
 
